@@ -273,6 +273,95 @@ int wkv_ddlerp_backward(int B, int T, int C, int nmix, const void *x, const void
                         void *gx, void *gm, void *gshift_out, float *gmaa, void *workspace,
                         size_t workspace_bytes, void *stream);
 
+/* ------------------------------------------------ beside the time-mix recurrences --
+ * A second kind of recurrence with a carried state -- the selective state space scan, with
+ * its short causal convolution and the norm in front of such a layer.  (No counterpart in
+ * RWKV-infctx-trainer; the contract is that of wkv5/wkv6: state in, state out, the gradient
+ * of both, segments chained.)  Tensors are contiguous unless a stride is given; any size and
+ * alignment is taken, 16-byte aligned rows run faster.  A NULL gradient output is not
+ * computed, a NULL incoming gradient is zero.  Backward calls give the same bits every time.
+ *
+ * wkv_rms_norm_*: h = x + residual (residual NULL: h = x), y = weight h / sqrt(mean(h^2) + eps)
+ *   over the C channels of each row, 1 <= C <= 16384.  x, y in `dtype`; residual, h in
+ *   `res_dtype` (dtype or WKV_F32; without a residual: dtype); weight [C] in `w_dtype`.
+ *   y is formed from h before its rounding.  With `scale` y is e4m3 bytes that stand for
+ *   y * scale: one scale a row (group = 0), or one per `group` channels (32, 64, 128, 256; the
+ *   last may be shorter), scale [rows, ceil(C/group)] = max|y| / 448, 1 where the maximum is
+ *   below 2^-100.
+ *   Backward (of the form without `scale`): h (x where there was no residual), gy, gh (NULL: 0) -> gx in dtype,
+ *   gresidual in res_dtype, gweight in w_dtype. */
+typedef struct wkv_rms_norm_args {
+    long long rows;
+    int C, group;
+    int dtype, res_dtype, w_dtype;
+    float eps;
+    const void *x, *residual, *weight;
+    void *y, *h;
+    float *scale;
+    const void *gy, *gh;
+    void *gx, *gresidual, *gweight;
+    void *workspace;
+    size_t workspace_bytes;
+} wkv_rms_norm_args_t;
+int wkv_rms_norm_forward(const wkv_rms_norm_args_t *a, void *stream);
+size_t wkv_rms_norm_backward_workspace(const wkv_rms_norm_args_t *a);
+int wkv_rms_norm_backward(const wkv_rms_norm_args_t *a, void *stream);
+
+/* wkv_causal_conv_*: s_t = bias + sum_j weight[d,j] x_{t-W+1+j}, y = silu(s) (silu != 0) or s, 2 <= W <= 4.
+ *   x [B,T,D] with strides x_batch, x_token (elements, channels adjacent); weight [D,W], bias
+ *   [D] (or NULL) in w_dtype; state_in [B,W-1,D] (or NULL: zeros) the inputs before the first
+ *   token, state_out the last W-1 inputs.  state_out may be state_in's memory for calls of at
+ *   most 16 tokens.  Gradients: gx [B,T,D], gweight, gbias in w_dtype, gstate_in. */
+typedef struct wkv_causal_conv_args {
+    int B, T, D, W;
+    int dtype, w_dtype, silu;
+    long long x_batch, x_token;
+    const void *x, *weight, *bias, *state_in;
+    void *y, *state_out;
+    const void *gy, *gstate_out;
+    void *gx, *gweight, *gbias, *gstate_in;
+    void *workspace;
+    size_t workspace_bytes;
+} wkv_causal_conv_args_t;
+int wkv_causal_conv_forward(const wkv_causal_conv_args_t *a, void *stream);
+size_t wkv_causal_conv_backward_workspace(const wkv_causal_conv_args_t *a);
+int wkv_causal_conv_backward(const wkv_causal_conv_args_t *a, void *stream);
+
+/* wkv_selective_scan_*: per channel d and state n (1 <= N <= 64),
+ *     dt = softplus(delta + delta_bias)  (softplus = 0: delta + delta_bias),
+ *     h_t = exp(dt A[d,n]) h_{t-1} + dt u B_t[n],   y_t = (sum_n C_t[n] h_t + D[d] u) * silu(z)
+ *   u, delta, z (or NULL: no gate) [B,T,D] and Bm, Cm [B,T,G,N] in `dtype`, each with its own
+ *   batch and token stride (elements); channel d uses row d / (D/G) of Bm and Cm.  A [D,N],
+ *   Dskip [D] (or NULL), delta_bias [D] (or NULL), the states [B,D,N]: fp32.  state_out may be
+ *   state_in's memory when T is 0 or 1.
+ *   time_groups: 0 = the library decides, n = every row is cut into n spans of tokens that run
+ *   in parallel; the workspace sizes depend on it.  ckpt (wkv_selective_scan_ckpt_bytes()):
+ *   the state at every 16th token, left by the forward call for the backward call, which
+ *   needs it.  Gradients: gu, gdelta, gz [B,T,D], gB, gC [B,T,G,N] in dtype; gA, gD, gbias,
+ *   gstate_in fp32. */
+typedef struct wkv_selective_scan_args {
+    int B, T, D, N, G;
+    int dtype, softplus, time_groups;
+    const void *u, *delta, *Bm, *Cm, *z;
+    long long u_batch, u_token, delta_batch, delta_token, B_batch, B_token, C_batch, C_token, z_batch, z_token;
+    const float *A, *Dskip, *delta_bias, *state_in;
+    void *y;
+    float *state_out;
+    const void *gy;
+    const float *gstate_out;
+    void *gu, *gdelta, *gz, *gB, *gC;
+    float *gA, *gD, *gbias, *gstate_in;
+    void *ckpt;
+    size_t ckpt_bytes;
+    void *workspace;
+    size_t workspace_bytes;
+} wkv_selective_scan_args_t;
+size_t wkv_selective_scan_ckpt_bytes(const wkv_selective_scan_args_t *a);
+size_t wkv_selective_scan_forward_workspace(const wkv_selective_scan_args_t *a);
+int wkv_selective_scan_forward(const wkv_selective_scan_args_t *a, void *stream);
+size_t wkv_selective_scan_backward_workspace(const wkv_selective_scan_args_t *a);
+int wkv_selective_scan_backward(const wkv_selective_scan_args_t *a, void *stream);
+
 /* Library build identification: "wkv_b200 <n> sm_100a". */
 const char *wkv_version(void);
 

@@ -4,6 +4,8 @@ libwkv_b200.so; there is no fallback if that fails."""
 from . import _lib
 from ._lib import (WKV_PATH_AUTO, WKV_PATH_CHUNKED, WKV_PATH_SCALAR, WKV_STATE_KV, WKV_STATE_VK,
                    WKV_W_NEGEXP, WKV_W_RAW)
+from .norm import rms_norm, rms_norm_q8
+from .ssm import causal_conv, causal_conv_step, selective_scan, selective_scan_step
 from .timemix import ddlerp, lnx_gate
 from .timemix_block import RWKV_TimeMix, RWKV_TimeMix6_0, RWKV_TimeMix_v4, TimeMixState
 from .wkv4 import WKVFunction, register_torch_op, wkv, wkv_op
@@ -19,5 +21,6 @@ __all__ = [
     "WKV5", "wkv5", "WKV5_CUDA", "RUN_WKV5_CUDA", "wkv5_cuda_kernel",
     "WKV6", "wkv6", "WKV6STATE_CUDA", "RUN_WKV6STATE_CUDA", "wkv6state_cuda_kernel",
     "wkv6_cuda_kernel", "lnx_gate", "ddlerp", "RWKV_TimeMix", "RWKV_TimeMix6_0",
-    "RWKV_TimeMix_v4", "TimeMixState",
+    "RWKV_TimeMix_v4", "TimeMixState", "rms_norm", "rms_norm_q8", "causal_conv", "causal_conv_step",
+    "selective_scan", "selective_scan_step",
 ]

@@ -40,6 +40,41 @@ class WkvArgs(ctypes.Structure):
     ]
 
 
+class RmsNormArgs(ctypes.Structure):
+    _fields_ = [
+        ("rows", ctypes.c_longlong), ("C", ctypes.c_int), ("group", ctypes.c_int),
+        ("dtype", ctypes.c_int), ("res_dtype", ctypes.c_int), ("w_dtype", ctypes.c_int), ("eps", ctypes.c_float),
+        ("x", _vp), ("residual", _vp), ("weight", _vp), ("y", _vp), ("h", _vp), ("scale", _vp),
+        ("gy", _vp), ("gh", _vp), ("gx", _vp), ("gresidual", _vp), ("gweight", _vp),
+        ("workspace", _vp), ("workspace_bytes", ctypes.c_size_t),
+    ]
+
+
+class CausalConvArgs(ctypes.Structure):
+    _fields_ = [
+        ("B", ctypes.c_int), ("T", ctypes.c_int), ("D", ctypes.c_int), ("W", ctypes.c_int),
+        ("dtype", ctypes.c_int), ("w_dtype", ctypes.c_int), ("silu", ctypes.c_int),
+        ("x_batch", ctypes.c_longlong), ("x_token", ctypes.c_longlong),
+        ("x", _vp), ("weight", _vp), ("bias", _vp), ("state_in", _vp), ("y", _vp), ("state_out", _vp),
+        ("gy", _vp), ("gstate_out", _vp), ("gx", _vp), ("gweight", _vp), ("gbias", _vp), ("gstate_in", _vp),
+        ("workspace", _vp), ("workspace_bytes", ctypes.c_size_t),
+    ]
+
+
+class SelectiveScanArgs(ctypes.Structure):
+    _fields_ = [
+        ("B", ctypes.c_int), ("T", ctypes.c_int), ("D", ctypes.c_int), ("N", ctypes.c_int), ("G", ctypes.c_int),
+        ("dtype", ctypes.c_int), ("softplus", ctypes.c_int), ("time_groups", ctypes.c_int),
+        ("u", _vp), ("delta", _vp), ("Bm", _vp), ("Cm", _vp), ("z", _vp),
+        *((f"{n}_{s}", ctypes.c_longlong) for n in ("u", "delta", "B", "C", "z") for s in ("batch", "token")),
+        ("A", _vp), ("Dskip", _vp), ("delta_bias", _vp), ("state_in", _vp), ("y", _vp), ("state_out", _vp),
+        ("gy", _vp), ("gstate_out", _vp),
+        ("gu", _vp), ("gdelta", _vp), ("gz", _vp), ("gB", _vp), ("gC", _vp),
+        ("gA", _vp), ("gD", _vp), ("gbias", _vp), ("gstate_in", _vp),
+        ("ckpt", _vp), ("ckpt_bytes", ctypes.c_size_t), ("workspace", _vp), ("workspace_bytes", ctypes.c_size_t),
+    ]
+
+
 EXPORTS = [
     "wkv_error_string", "wkv_version", "wkv56_uses_chunked", "wkv56_state_ckpt_bytes",
     "wkv4_forward_workspace", "wkv4_forward", "wkv4_backward_workspace", "wkv4_backward",
@@ -50,6 +85,10 @@ EXPORTS = [
     "wkv_selftest_wait_timeout", "wkv56_selftest_abort", "wkv56_group_states_bytes",
     "wkv_lnx_gate_forward", "wkv_lnx_gate_backward_workspace", "wkv_lnx_gate_backward",
     "wkv_ddlerp_forward", "wkv_ddlerp_backward_workspace", "wkv_ddlerp_backward",
+    "wkv_rms_norm_forward", "wkv_rms_norm_backward_workspace", "wkv_rms_norm_backward",
+    "wkv_causal_conv_forward", "wkv_causal_conv_backward_workspace", "wkv_causal_conv_backward",
+    "wkv_selective_scan_ckpt_bytes", "wkv_selective_scan_forward_workspace", "wkv_selective_scan_forward",
+    "wkv_selective_scan_backward_workspace", "wkv_selective_scan_backward",
 ]
 
 _lib = None
@@ -142,6 +181,17 @@ def load() -> ctypes.CDLL:
     lib.wkv_ddlerp_backward_workspace.argtypes = [i, i, i, i]
     lib.wkv_ddlerp_backward.restype = i
     lib.wkv_ddlerp_backward.argtypes = [i, i, i, i] + [f] * 10 + [_vp, sz, _vp]
+    for name, args in (("rms_norm", RmsNormArgs), ("causal_conv", CausalConvArgs), ("selective_scan", SelectiveScanArgs)):
+        for d in ("forward", "backward"):
+            fn = getattr(lib, f"wkv_{name}_{d}")
+            fn.restype = i
+            fn.argtypes = [ctypes.POINTER(args), _vp]
+            if d == "backward" or name == "selective_scan":
+                ws = getattr(lib, f"wkv_{name}_{d}_workspace")
+                ws.restype = sz
+                ws.argtypes = [ctypes.POINTER(args)]
+    lib.wkv_selective_scan_ckpt_bytes.restype = sz
+    lib.wkv_selective_scan_ckpt_bytes.argtypes = [ctypes.POINTER(SelectiveScanArgs)]
     for v in ("wkv5", "wkv6"):
         for d in ("forward", "backward"):
             fn = getattr(lib, f"{v}_{d}")

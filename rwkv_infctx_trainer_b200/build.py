@@ -17,10 +17,10 @@ CSRC = os.path.join(PKG, "csrc")
 LIB = os.path.join(PKG, "libwkv_b200.so")
 STAMP = LIB + ".digest"
 SOURCES = ["wkv_api.cu", "wkv4.cu", "wkv4_par.cu", "wkv56_scalar.cu", "wkv56_chunked.cu", "wkv56_chunked_bwd.cu",
-           "timemix_fused.cu", "decode.cu"]
+           "timemix_fused.cu", "decode.cu", "rms_norm.cu", "causal_conv.cu", "selective_scan.cu", "param_fold.cu"]
 NATIVE_NAME = "_wkv_native"
 NATIVE = os.path.join(PKG, NATIVE_NAME + ".so")
-NATIVE_SOURCES = ["native_ops.cpp", "native_timemix.cpp", "native_blocks.cpp"]
+NATIVE_SOURCES = ["native_ops.cpp", "native_timemix.cpp", "native_blocks.cpp", "native_ssm.cpp"]
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
               "--use_fast_math", "-Xcompiler", "-fPIC"]
 

@@ -415,6 +415,7 @@ py::object none_or(const Tensor &t) { return t.defined() ? py::cast(t) : py::non
 
 void bind_timemix(py::module_ &m);
 void bind_blocks(py::module_ &m);
+void bind_ssm(py::module_ &m);
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("wkv56_apply", &wkv56_apply);
@@ -442,4 +443,5 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
           });
     bind_timemix(m);
     bind_blocks(m);
+    bind_ssm(m);
 }

@@ -1,0 +1,364 @@
+// Root-mean-square norm with the residual's addition, its gradient, and the same with an output in 8 bits.
+//
+//   h = x + residual        (stored in the residual's type; without a residual h = x and is not stored)
+//   y = weight * h * r,     r = 1 / sqrt(mean(h^2) + eps)
+//   8 bits: scale = max|y| / 448 over the row, or over each group of channels; q = e4m3(y / scale)
+//
+//   backward, with gh the gradient that reaches h from elsewhere:
+//   xh = h r,  gx = gh + r (gy weight - xh mean(gy weight xh)),  gweight = sum over the rows of gy xh
+//
+// All are bound by HBM: a row crosses once per pass, a thread owns runs of 8 channels and keeps them in registers from
+// the sum to the output; the next row's values are on their way meanwhile.  A CTA takes every gridDim-th row, so that the
+// weights (and the sums of their gradient) stay in registers.  Sums are fp32 and in a fixed order.
+#include <cuda_fp8.h>
+
+#include "elem_io.cuh"
+#include "wkv_internal.h"
+
+namespace wkv {
+namespace {
+
+constexpr int RUN = 8;            // channels a thread takes at once
+
+// sums (or maxima of non-negative values, given as bits) over the CTA; `red` has a place for each warp and is reused by
+// alternating halves
+__device__ __forceinline__ float cta_sum(float v, float *red, int nwarp) {
+    v = warp_sum(v);
+    if (nwarp == 1) return v;
+    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
+    __syncthreads();
+    v = (threadIdx.x & 31) < nwarp ? red[threadIdx.x & 31] : 0.f;
+    return warp_sum(v);
+}
+__device__ __forceinline__ float2 cta_sum2(float2 v, float2 *red, int nwarp) {
+    v.x = warp_sum(v.x); v.y = warp_sum(v.y);
+    if (nwarp == 1) return v;
+    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
+    __syncthreads();
+    v = (threadIdx.x & 31) < nwarp ? red[threadIdx.x & 31] : make_float2(0.f, 0.f);
+    v.x = warp_sum(v.x); v.y = warp_sum(v.y);
+    return v;
+}
+__device__ __forceinline__ uint32_t warp_max_bits(uint32_t v, int lanes) {
+    for (int o = lanes >> 1; o > 0; o >>= 1) v = max(v, __shfl_xor_sync(0xffffffffu, v, o));
+    return v;
+}
+
+struct NormArgs {
+    const void *x, *res, *w;
+    void *y, *h;
+    float *scale;
+    long long rows;
+    int C, w_dtype, group, ngroup, vec;
+    float eps;
+};
+
+// scale and 1 / scale for a largest value given as bits: as an unsigned number a NaN is above every other value, so one in
+// the row makes the scale, and with it every value of the row, NaN.  Below 2^-100 (a row of zeros) the scale is 1.
+__device__ __forceinline__ float q8_scale(uint32_t top) {
+    const float m = __uint_as_float(top);
+    return m <= 7.8886e-31f ? 1.f : m * (1.f / 448.f);
+}
+
+template <typename X, typename R, int NV, bool Q8>
+__global__ void __launch_bounds__(512) k_rms_norm_fwd(NormArgs a) {
+    pdl_wait();
+    pdl_trigger();
+    __shared__ float red[2][16];
+    __shared__ uint32_t redm[2][16];
+    const int tid = threadIdx.x, nt = blockDim.x, nwarp = nt >> 5, C = a.C;
+    const X *x = (const X *)a.x;
+    const R *res = (const R *)a.res;
+    const bool vec = a.vec;
+    float w[NV][RUN];
+    int left[NV];                       // channels of the run that exist
+#pragma unroll
+    for (int i = 0; i < NV; i++) {
+        const int c = (tid + i * nt) * RUN;
+        left[i] = min(RUN, C - c);
+#pragma unroll
+        for (int q = 0; q < RUN; q++) w[i][q] = q < left[i] ? param_at(a.w, a.w_dtype, c + q) : 0.f;
+    }
+    Raw<X, RUN> rx[NV];
+    Raw<R, RUN> rr[NV];
+    auto fetch = [&](long long row) {
+#pragma unroll
+        for (int i = 0; i < NV; i++) {
+            const size_t at = (size_t)row * C + (size_t)(tid + i * nt) * RUN;
+            rx[i].zero(); rr[i].zero();
+            if (left[i] > 0 && row < a.rows) {
+                rx[i].load(x + at, vec, left[i]);
+                if (res) rr[i].load(res + at, vec, left[i]);
+            }
+        }
+    };
+    fetch(blockIdx.x);
+    int par = 0;
+    for (long long row = blockIdx.x; row < a.rows; row += gridDim.x, par ^= 1) {
+        float h[NV][RUN], ss = 0.f;
+#pragma unroll
+        for (int i = 0; i < NV; i++) {
+            float t[RUN];
+            rx[i].get(h[i]);
+            rr[i].get(t);
+#pragma unroll
+            for (int q = 0; q < RUN; q++) { h[i][q] += t[q]; ss += h[i][q] * h[i][q]; }
+        }
+        fetch(row + gridDim.x);
+        if (a.h) {
+#pragma unroll
+            for (int i = 0; i < NV; i++) {
+                Raw<R, RUN> o;
+                o.put(h[i]);
+                if (left[i] > 0) o.store((R *)a.h + (size_t)row * C + (size_t)(tid + i * nt) * RUN, vec, left[i]);
+            }
+        }
+        const float r = rsqrtf(cta_sum(ss, red[par], nwarp) / (float)C + a.eps);
+#pragma unroll
+        for (int i = 0; i < NV; i++)
+#pragma unroll
+            for (int q = 0; q < RUN; q++) h[i][q] = h[i][q] * r * w[i][q];
+        if (!Q8) {
+#pragma unroll
+            for (int i = 0; i < NV; i++) {
+                Raw<X, RUN> o;
+                o.put(h[i]);
+                if (left[i] > 0) o.store((X *)a.y + (size_t)row * C + (size_t)(tid + i * nt) * RUN, vec, left[i]);
+            }
+            continue;
+        }
+        uint32_t top[NV];
+#pragma unroll
+        for (int i = 0; i < NV; i++) {
+            top[i] = 0u;
+#pragma unroll
+            for (int q = 0; q < RUN; q++)
+                if (q < left[i]) top[i] = max(top[i], __float_as_uint(h[i][q]) & 0x7FFFFFFFu);
+        }
+        if (a.group) {
+            // a group is group / 8 neighbouring lanes of one warp
+            const int lanes = a.group / RUN;
+#pragma unroll
+            for (int i = 0; i < NV; i++) {
+                top[i] = warp_max_bits(top[i], lanes);
+                if (left[i] > 0 && (tid & (lanes - 1)) == 0) a.scale[(size_t)row * a.ngroup + (tid + i * nt) / lanes] = q8_scale(top[i]);
+            }
+        } else {
+#pragma unroll
+            for (int i = 1; i < NV; i++) top[0] = max(top[0], top[i]);
+            uint32_t m = warp_max_bits(top[0], 32);
+            if (nwarp > 1) {
+                if ((tid & 31) == 0) redm[par][tid >> 5] = m;
+                __syncthreads();
+                m = warp_max_bits((tid & 31) < nwarp ? redm[par][tid & 31] : 0u, 32);
+            }
+#pragma unroll
+            for (int i = 0; i < NV; i++) top[i] = m;
+            if (tid == 0) a.scale[row] = q8_scale(m);
+        }
+#pragma unroll
+        for (int i = 0; i < NV; i++) {
+            const float inv = 1.f / q8_scale(top[i]);
+            uint32_t o[2] = {0u, 0u};
+#pragma unroll
+            for (int q = 0; q < RUN; q += 2) {
+                // to nearest, at most 448; a NaN stays one
+                const uint32_t two = __nv_cvt_float2_to_fp8x2(make_float2(h[i][q] * inv, h[i][q + 1] * inv), __NV_SATFINITE, __NV_E4M3);
+                o[q / 4] |= two << (8 * (q & 3));
+            }
+            if (left[i] > 0) {
+                unsigned char *p = (unsigned char *)a.y + (size_t)row * C + (size_t)(tid + i * nt) * RUN;
+                if (vec) *reinterpret_cast<uint2 *>(p) = make_uint2(o[0], o[1]);
+                else {
+#pragma unroll
+                    for (int q = 0; q < RUN; q++)
+                        if (q < left[i]) p[q] = (unsigned char)(o[q / 4] >> (8 * (q & 3)));
+                }
+            }
+        }
+    }
+}
+
+struct NormBwdArgs {
+    const void *h, *w, *gy, *gh;
+    void *gx, *gres;
+    float *part;                        // [gridDim.x, C], NULL when the weight needs no gradient
+    long long rows;
+    int C, w_dtype, vec;
+    float eps;
+};
+
+template <typename X, typename R, int NV>
+__global__ void __launch_bounds__(512) k_rms_norm_bwd(NormBwdArgs a) {
+    pdl_wait();
+    pdl_trigger();
+    __shared__ float2 red[2][16];
+    const int tid = threadIdx.x, nt = blockDim.x, nwarp = nt >> 5, C = a.C;
+    const R *h = (const R *)a.h, *gh = (const R *)a.gh;
+    const X *gy = (const X *)a.gy;
+    const bool vec = a.vec;
+    float w[NV][RUN], gw[NV][RUN];
+    int left[NV];
+#pragma unroll
+    for (int i = 0; i < NV; i++) {
+        const int c = (tid + i * nt) * RUN;
+        left[i] = min(RUN, C - c);
+#pragma unroll
+        for (int q = 0; q < RUN; q++) { w[i][q] = q < left[i] ? param_at(a.w, a.w_dtype, c + q) : 0.f; gw[i][q] = 0.f; }
+    }
+    Raw<R, RUN> rh[NV], rg[NV];
+    Raw<X, RUN> ry[NV];
+    auto fetch = [&](long long row) {
+#pragma unroll
+        for (int i = 0; i < NV; i++) {
+            const size_t at = (size_t)row * C + (size_t)(tid + i * nt) * RUN;
+            rh[i].zero(); rg[i].zero(); ry[i].zero();
+            if (left[i] > 0 && row < a.rows) {
+                rh[i].load(h + at, vec, left[i]);
+                if (gy) ry[i].load(gy + at, vec, left[i]);
+                if (gh) rg[i].load(gh + at, vec, left[i]);
+            }
+        }
+    };
+    fetch(blockIdx.x);
+    int par = 0;
+    for (long long row = blockIdx.x; row < a.rows; row += gridDim.x, par ^= 1) {
+        float hv[NV][RUN], g[NV][RUN];
+        float2 s = make_float2(0.f, 0.f);       // sum h^2, sum gy w h
+        Raw<R, RUN> keep[NV];
+#pragma unroll
+        for (int i = 0; i < NV; i++) {
+            rh[i].get(hv[i]);
+            ry[i].get(g[i]);
+            keep[i] = rg[i];
+#pragma unroll
+            for (int q = 0; q < RUN; q++) { s.x += hv[i][q] * hv[i][q]; s.y += g[i][q] * w[i][q] * hv[i][q]; }
+        }
+        fetch(row + gridDim.x);
+        s = cta_sum2(s, red[par], nwarp);
+        const float r = rsqrtf(s.x / (float)C + a.eps), m = s.y * r / (float)C;      // m = mean(gy w xh)
+#pragma unroll
+        for (int i = 0; i < NV; i++) {
+            float o[RUN];
+            keep[i].get(o);
+#pragma unroll
+            for (int q = 0; q < RUN; q++) {
+                const float xh = hv[i][q] * r;
+                gw[i][q] += g[i][q] * xh;
+                o[q] += r * (g[i][q] * w[i][q] - xh * m);
+            }
+            if (left[i] > 0) {
+                const size_t at = (size_t)row * C + (size_t)(tid + i * nt) * RUN;
+                if (a.gx) { Raw<X, RUN> t; t.put(o); t.store((X *)a.gx + at, vec, left[i]); }
+                if (a.gres) { Raw<R, RUN> t; t.put(o); t.store((R *)a.gres + at, vec, left[i]); }
+            }
+        }
+    }
+    if (a.part) {
+#pragma unroll
+        for (int i = 0; i < NV; i++)
+#pragma unroll
+            for (int q = 0; q < RUN; q++)
+                if (q < left[i]) a.part[(size_t)blockIdx.x * C + (tid + i * nt) * RUN + q] = gw[i][q];
+    }
+}
+
+constexpr int MAX_C = 16384;
+// runs per thread: two up to 8192 channels, four above (512 threads)
+inline int runs_per_thread(int C) { return C <= 8192 ? 2 : 4; }
+inline int threads_for(int C) {
+    const int nv = runs_per_thread(C), t = ((C + RUN - 1) / RUN + nv - 1) / nv;
+    return (t + 31) / 32 * 32;
+}
+// CTAs: every SM full (2048 threads forward, by registers 1024 backward), and no more than rows
+inline int ctas_for(long long rows, int C, int per_sm_threads) {
+    int per_sm = per_sm_threads / threads_for(C);
+    per_sm = per_sm < 1 ? 1 : per_sm > 16 ? 16 : per_sm;
+    const long long n = (long long)device_sm_count() * per_sm;
+    return (int)(rows < n ? rows : n);
+}
+
+int check_norm(const wkv_rms_norm_args_t *a) {
+    if (!a) return WKV_ERR_NULL;
+    if (a->rows < 0 || a->C < 1 || a->C > MAX_C) return WKV_ERR_SHAPE;
+    if (!known_dtype(a->dtype) || !known_dtype(a->w_dtype)) return WKV_ERR_DTYPE;
+    if (a->res_dtype != a->dtype && a->res_dtype != WKV_F32) return WKV_ERR_DTYPE;
+    if (!a->weight) return WKV_ERR_NULL;
+    return WKV_OK;
+}
+
+// f is called with one value of x's type and one of the residual's
+template <class Fn>
+int by_types(int dtype, int res_dtype, Fn f) {
+    return by_dtype(dtype, [&](auto x) {
+        using X = decltype(x);
+        return res_dtype == dtype ? f(X{}, X{}) : f(X{}, float{});
+    });
+}
+
+}  // namespace
+}  // namespace wkv
+
+using namespace wkv;
+
+extern "C" int wkv_rms_norm_forward(const wkv_rms_norm_args_t *a, void *stream) {
+    int e = check_norm(a);
+    if (e != WKV_OK) return e;
+    if (a->scale) {
+        if (a->group != 0 && a->group != 32 && a->group != 64 && a->group != 128 && a->group != 256) return WKV_ERR_SHAPE;
+    }
+    if (a->rows == 0) return WKV_OK;
+    if (!a->x || !a->y || (a->residual && !a->h)) return WKV_ERR_NULL;
+    if (!a->residual && a->res_dtype != a->dtype) return WKV_ERR_DTYPE;
+    NormArgs k = {};
+    k.x = a->x; k.res = a->residual; k.w = a->weight; k.y = a->y; k.h = a->residual ? a->h : nullptr;
+    k.scale = a->scale;
+    k.rows = a->rows; k.C = a->C; k.w_dtype = a->w_dtype; k.eps = a->eps;
+    k.group = a->scale ? a->group : 0;
+    k.ngroup = k.group ? (a->C + k.group - 1) / k.group : 1;
+    k.vec = a->C % RUN == 0 && all_aligned({a->x, a->residual, a->y, k.h});
+    const int nt = threads_for(a->C), nb = ctas_for(a->rows, a->C, 2048), nv = runs_per_thread(a->C);
+    cudaStream_t s = (cudaStream_t)stream;
+    return by_types(a->dtype, a->res_dtype, [&](auto x, auto r) {
+        using X = decltype(x);
+        using R = decltype(r);
+        if (k.scale) return launch_chained(nv == 2 ? k_rms_norm_fwd<X, R, 2, true> : k_rms_norm_fwd<X, R, 4, true>, dim3(nb), dim3(nt), 0, s, k);
+        return launch_chained(nv == 2 ? k_rms_norm_fwd<X, R, 2, false> : k_rms_norm_fwd<X, R, 4, false>, dim3(nb), dim3(nt), 0, s, k);
+    });
+}
+
+extern "C" size_t wkv_rms_norm_backward_workspace(const wkv_rms_norm_args_t *a) {
+    if (check_norm(a) != WKV_OK) return 0;
+    return align256((size_t)ctas_for(a->rows, a->C, 1024) * a->C * 4);
+}
+
+extern "C" int wkv_rms_norm_backward(const wkv_rms_norm_args_t *a, void *stream) {
+    int e = check_norm(a);
+    if (e != WKV_OK) return e;
+    cudaStream_t s = (cudaStream_t)stream;
+    const int nt = threads_for(a->C), nb = ctas_for(a->rows, a->C, 1024), nv = runs_per_thread(a->C);
+    if (a->rows > 0 && !a->h) return WKV_ERR_NULL;
+    if (a->gweight && a->rows > 0) {
+        if (!a->workspace || a->workspace_bytes < wkv_rms_norm_backward_workspace(a)) return WKV_ERR_WORKSPACE;
+        if (!aligned16(a->workspace)) return WKV_ERR_ALIGN;
+    }
+    NormBwdArgs k = {};
+    k.h = a->h; k.w = a->weight; k.gy = a->gy; k.gh = a->gh; k.gx = a->gx; k.gres = a->gresidual;
+    k.part = a->gweight ? (float *)a->workspace : nullptr;
+    k.rows = a->rows; k.C = a->C; k.w_dtype = a->w_dtype; k.eps = a->eps;
+    k.vec = a->C % RUN == 0 && all_aligned({a->h, a->gy, a->gh, a->gx, a->gresidual});
+    if (a->rows > 0) {
+        e = by_types(a->dtype, a->res_dtype, [&](auto x, auto r) {
+            using X = decltype(x);
+            using R = decltype(r);
+            return launch_chained(nv == 2 ? k_rms_norm_bwd<X, R, 2> : k_rms_norm_bwd<X, R, 4>, dim3(nb), dim3(nt), 0, s, k);
+        });
+        if (e != WKV_OK) return e;
+    }
+    if (!a->gweight) return WKV_OK;
+    FoldOut f = {};
+    f.p[0] = a->gweight; f.dtype[0] = a->w_dtype;
+    f.start[0] = 0;
+    for (int i = 1; i < 5; i++) f.start[i] = a->C;
+    return fold_params((const float *)a->workspace, nb, a->C, f, s);
+}

@@ -1,0 +1,272 @@
+"""The selective scan against its formulas in 64 bits: forward, backward, single tokens, segments."""
+import pytest
+import torch
+
+import ssm_testlib as S
+
+pytestmark = pytest.mark.gpu
+BF, HF, F32 = torch.bfloat16, torch.float16, torch.float32
+
+
+def call(c, softplus=True, **kw):
+    import rwkv_infctx_trainer_b200 as W
+    a = {n: c[n] for n in ("u", "delta", "A", "B", "C", "D", "z", "delta_bias", "state")}
+    a.update(kw)
+    return W.selective_scan(a["u"], a["delta"], a["A"], a["B"], a["C"], a["D"], a["z"], a["delta_bias"], softplus, a["state"])
+
+
+def reference(c, softplus, grads, mag):
+    return S.scan_ref(c["u"], c["delta"], c["A"], c["B"], c["C"], c["D"], c["z"], c["delta_bias"], softplus, c["state"],
+                      c["gy"] if grads else None, c["gs"] if grads else None, mag)
+
+
+def check(c, got, softplus=True, grads=True):
+    want, mag = reference(c, softplus, grads, False), reference(c, softplus, grads, True)
+    B, T, D = c["u"].shape
+    N = c["A"].shape[1]
+    for n, t in got.items():
+        S.close(n, t, want[n], mag[n], S.scan_K(n, B, T, D, N))
+
+
+def train(c, softplus=True):
+    leaves = {n: c[n].detach().requires_grad_(True) for n in S.SCAN_LEAVES if c[n] is not None}
+    y, s = call(c, softplus, **leaves)
+    grads = torch.autograd.grad((y, s), list(leaves.values()), (c["gy"], c["gs"]))
+    names = dict(zip(S.SCAN_LEAVES, S.SCAN_GRADS))
+    return {"y": y, "state": s, **{names[n]: g for n, g in zip(leaves, grads)}}
+
+
+# lengths around a block of 16 tokens and its half, and where a row is cut into spans (128 and up)
+@pytest.mark.parametrize("T", [1, 2, 7, 8, 9, 15, 16, 17, 31, 33, 130, 300])
+@pytest.mark.parametrize("dtype", [BF, HF, F32])
+def test_lengths(T, dtype):
+    c = S.scan_case(T, 2, T, 37, 16, 1, dtype)
+    check(c, train(c))
+
+
+# states that fill no lane, one lane to sixteen a channel; channels that fill no warp, in one group and in several
+@pytest.mark.parametrize("N", [1, 3, 4, 5, 8, 11, 16, 20, 32, 33, 64])
+@pytest.mark.parametrize("D,G", [(1, 1), (40, 1), (69, 3), (130, 2)])
+def test_states_and_channels(N, D, G):
+    c = S.scan_case(N * 100 + D, 2, 21, D, N, G, F32)
+    check(c, train(c))
+
+
+@pytest.mark.parametrize("gate,skip,bias,state,softplus", [(False, True, True, True, True), (True, False, True, True, True),
+                                                           (True, True, False, True, True), (True, True, True, False, True),
+                                                           (False, False, False, False, True), (True, True, True, True, False)])
+@pytest.mark.parametrize("T", [1, 40, 200])
+def test_optional_inputs(gate, skip, bias, state, softplus, T):
+    c = S.scan_case(T, 3, T, 24, 16, 1, BF, gate, skip, bias, state)
+    if not softplus:
+        c["delta"] = c["delta"].abs() * 0.2
+        if bias:
+            c["delta_bias"] = c["delta_bias"].abs() * 0.01
+    check(c, train(c, softplus), softplus)
+
+
+@pytest.mark.parametrize("T", [5, 150])
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_views_of_wider_tensors(T, dtype):
+    c = S.scan_case(T, 2, T, 48, 16, 2, dtype, strided=True)
+    assert not c["u"].is_contiguous() and not c["B"].is_contiguous()
+    got = train(c)
+    check(c, got)
+    # the bits of contiguous copies (odd starts included), channels that are not adjacent are copied
+    d = {n: (t.contiguous() if t is not None else None) for n, t in c.items()}
+    for n, t in train(d).items():
+        assert torch.equal(t, got[n]), n
+    turned = dict(d, u=d["u"].transpose(1, 2).contiguous().transpose(1, 2))
+    for n, t in train(turned).items():
+        assert torch.equal(t, got[n]), n
+
+
+@pytest.mark.parametrize("offset", [1, 3])
+def test_tensors_that_start_anywhere(offset):
+    c = S.scan_case(3, 2, 20, 40, 16, 1, BF)
+    want = train(c)
+
+    def moved(t):
+        buf = torch.empty(t.numel() + 8, dtype=t.dtype, device=t.device)
+        v = buf[offset:offset + t.numel()].view(t.shape)
+        v.copy_(t)
+        return v
+
+    for n, t in train({n: (moved(t) if t is not None else None) for n, t in c.items()}).items():
+        assert torch.equal(t, want[n]), n
+
+
+def test_empty_calls():
+    import rwkv_infctx_trainer_b200 as W
+    c = S.scan_case(1, 2, 0, 24, 16, 1, BF)
+    got = train(c)
+    assert got["y"].shape == (2, 0, 24) and torch.equal(got["state"], c["state"]) and torch.equal(got["gstate"], c["gs"])
+    for n in ("gA", "gD", "gbias"):
+        assert float(got[n].abs().max()) == 0.0
+    y, s = call(dict(c, state=None))
+    assert float(s.abs().max()) == 0.0
+    for B, D in ((0, 24), (2, 0)):
+        c = S.scan_case(1, B, 3, D, 16, 1, BF)
+        got = train(c)
+        assert got["y"].shape == (B, 3, D) and got["state"].shape == (B, D, 16)
+        assert float(got["gA"].abs().sum()) == 0.0
+        assert W.selective_scan_step(c["u"][:, 0], c["delta"][:, 0], c["A"], c["B"][:, 0], c["C"][:, 0], c["state"]).shape == (B, D)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_segments_are_the_unsplit_row(dtype):
+    """three segments with the state and its gradient carried: the gradients of one call"""
+    T, cuts = 100, [(0, 33), (33, 34), (34, 100)]
+    c = S.scan_case(8, 2, T, 20, 16, 1, dtype)
+    leaves = {n: c[n].detach().requires_grad_(True) for n in S.SCAN_LEAVES}
+    s, ys = leaves["state"], []
+    for a, b in cuts:
+        seg = {n: leaves[n][:, a:b] for n in ("u", "delta", "B", "C", "z")}
+        y, s = call(c, **{**leaves, **seg, "state": s})
+        ys.append(y)
+    y = torch.cat(ys, 1)
+    grads = torch.autograd.grad((y, s), list(leaves.values()), (c["gy"], c["gs"]))
+    names = dict(zip(S.SCAN_LEAVES, S.SCAN_GRADS))
+    check(c, {"y": y, "state": s, **{names[n]: g for n, g in zip(leaves, grads)}})
+
+
+@pytest.mark.parametrize("N,G", [(16, 1), (16, 4), (5, 1), (64, 2), (8, 1)])
+@pytest.mark.parametrize("dtype", [BF, HF, F32])
+def test_single_tokens_continue_a_prompt(N, G, dtype):
+    import rwkv_infctx_trainer_b200 as W
+    T, P = 40, 33
+    c = S.scan_case(N, 3, T, 36, N, G, dtype)
+    cut = lambda a, b: {n: (c[n][:, a:b]) for n in ("u", "delta", "B", "C", "z")}
+    y, s = call(dict(c, **cut(0, P)))
+    ys, address = [y], s.data_ptr()
+    for t in range(P, T):
+        v = s._version
+        ys.append(W.selective_scan_step(c["u"][:, t], c["delta"][:, t], c["A"], c["B"][:, t], c["C"][:, t], s, c["D"], c["z"][:, t],
+                                        c["delta_bias"]).unsqueeze(1))
+        assert s._version > v and s.data_ptr() == address
+    check(c, {"y": torch.cat(ys, 1), "state": s}, grads=False)
+    if G == 1:      # B and C without the dimension of the groups
+        s2 = s.clone()
+        a = W.selective_scan_step(c["u"][:, 0], c["delta"][:, 0], c["A"], c["B"][:, 0, 0], c["C"][:, 0, 0], s)
+        b = W.selective_scan_step(c["u"][:, 0], c["delta"][:, 0], c["A"], c["B"][:, 0], c["C"][:, 0], s2)
+        assert torch.equal(a, b) and torch.equal(s, s2)
+
+
+def test_gradients_against_differences():
+    """<grad, v> of the fp32 call against central differences of the formulas in 64 bits.  Step 1e-4: the differences are
+    off by about 1e-8 of the third derivative, the gradient by K 2^-24 of its terms' magnitude."""
+    c = S.scan_case(5, 2, 19, 10, 6, 2, F32)
+    got = train(c)
+    mag = reference(c, True, True, True)
+    for n, gname in zip(S.SCAN_LEAVES, S.SCAN_GRADS):
+        v = torch.randn_like(c[n]).double()
+
+        def loss(e):
+            o = reference(dict(c, **{n: c[n].double() + e * v}), True, False, False)
+            return float((o["y"] * c["gy"].double()).sum() + (o["state"] * c["gs"].double()).sum())
+
+        want = (loss(1e-4) - loss(-1e-4)) / 2e-4
+        m = float((mag[gname] * v.abs()).sum())
+        assert abs(float((got[gname].double() * v).sum()) - want) <= (S.scan_K(gname, 2, 19, 10, 6) * S.U + 1e-6) * m, n
+
+
+def test_incoming_gradients_that_are_missing():
+    """y alone, and the state alone, have the gradients that zeros in the other's place give"""
+    for T in (5, 160):
+        c = S.scan_case(2, 2, T, 24, 16, 1, BF)
+        for use in ("gy", "gs"):
+            leaves = {n: c[n].detach().requires_grad_(True) for n in S.SCAN_LEAVES}
+            y, s = call(c, **leaves)
+            out = (y, c["gy"]) if use == "gy" else (s, c["gs"])
+            got = torch.autograd.grad(out[0], list(leaves.values()), out[1], allow_unused=True)
+            z = dict(c, **{("gs" if use == "gy" else "gy"): torch.zeros_like(c["gs" if use == "gy" else "gy"])})
+            want = train(z)
+            for n, g in zip(S.SCAN_GRADS, got):
+                assert torch.equal(g, want[n]), (use, n)
+
+
+@pytest.mark.parametrize("n", S.SCAN_LEAVES)
+def test_one_gradient_alone(n):
+    """what is asked for alone has the bits that it has among all"""
+    c = S.scan_case(4, 2, 140, 24, 16, 1, BF)
+    want = train(c)[dict(zip(S.SCAN_LEAVES, S.SCAN_GRADS))[n]]
+    leaf = c[n].detach().requires_grad_(True)
+    y, s = call(c, **{n: leaf})
+    assert torch.equal(torch.autograd.grad((y, s), leaf, (c["gy"], c["gs"]))[0], want)
+
+
+def test_repeatable_and_types_of_parameters():
+    c = S.scan_case(6, 3, 170, 72, 16, 1, BF)
+    a, b = train(c), train(c)
+    for n in a:
+        assert torch.equal(a[n], b[n]), n
+    half = dict(c, **{n: c[n].to(BF) for n in ("A", "D", "delta_bias", "state")})
+    got = train(half)
+    for n, g in (("A", "gA"), ("D", "gD"), ("delta_bias", "gbias"), ("state", "gstate")):
+        assert got[g].dtype == BF, n
+    check(half, got)
+
+
+def test_strong_and_weak_decays():
+    """decays that underflow at once and decays of one, steps of up to 30 and as small as 1e-9"""
+    c = S.scan_case(7, 1, 64, 32, 8, 1, F32)
+    c["A"][:8] *= 200.0
+    c["A"][8:16] = 0.0
+    c["delta"][:, ::5] += 30.0
+    c["delta"][:, 1::5] -= 20.0
+    # (an argument of up to 30 in the exponential of softplus and 30 x 1600 in a decay: errors of 30 2^-24 and, in terms that
+    # do not underflow, of the exponent they are left with)
+    got = train(c)
+    want, mag = reference(c, True, True, False), reference(c, True, True, True)
+    for n, t in got.items():
+        S.close(n, t, want[n], mag[n], S.scan_K(n, 1, 64, 32, 8) + 128)
+
+
+def test_nan_and_infinity_stay_with_their_channel():
+    c = S.scan_case(9, 2, 40, 24, 16, 1, F32)
+    want, _ = call(c)
+    for bad in (float("nan"), float("inf")):
+        d = dict(c, u=c["u"].clone())
+        d["u"][0, 10, 5] = bad
+        y, s = call(d)
+        keep = torch.ones_like(y, dtype=torch.bool)
+        keep[0, 10:, 5] = False
+        assert torch.equal(y[keep], want[keep])
+        assert not torch.isfinite(y[0, 10:, 5]).any()
+        assert not torch.isfinite(s[0, 5]).any() and torch.isfinite(s[1]).all()
+
+
+def test_every_cut_of_a_row_into_spans():
+    """the C ABI with each number of spans: the same results up to the re-association of the fold (a fold multiplies a
+    span's contribution by one exp of the sum of dt instead of by each token's), and the fixed bits of one span where the
+    library would take one"""
+    import ctypes
+    from rwkv_infctx_trainer_b200 import _lib as L
+    lib = L.load()
+    B, T, D, N, G = 2, 167, 40, 16, 2
+    c = S.scan_case(10, B, T, D, N, G, BF)
+    st = torch.cuda.current_stream().cuda_stream
+    for groups in (1, 2, 3, 5, 11, 1000):
+        a = L.SelectiveScanArgs(B=B, T=T, D=D, N=N, G=G, dtype=L.WKV_BF16, softplus=1, time_groups=groups)
+        for n, f in (("u", "u"), ("delta", "delta"), ("B", "Bm"), ("C", "Cm"), ("z", "z")):
+            setattr(a, f, c[n].data_ptr())
+            setattr(a, n + "_batch", c[n].stride(0))
+            setattr(a, n + "_token", c[n].stride(1))
+        out = {"y": torch.empty_like(c["u"]), "state": torch.empty_like(c["state"]), "gu": torch.empty_like(c["u"]),
+               "gdelta": torch.empty_like(c["u"]), "gz": torch.empty_like(c["u"]), "gB": torch.empty_like(c["B"]),
+               "gC": torch.empty_like(c["B"]), "gA": torch.empty_like(c["A"]), "gD": torch.empty_like(c["D"]),
+               "gbias": torch.empty_like(c["D"]), "gstate": torch.empty_like(c["state"])}
+        for f, t in (("A", c["A"]), ("Dskip", c["D"]), ("delta_bias", c["delta_bias"]), ("state_in", c["state"]), ("gy", c["gy"]),
+                     ("gstate_out", c["gs"]), ("y", out["y"]), ("state_out", out["state"]), ("gstate_in", out["gstate"]),
+                     *((n, out[n]) for n in ("gu", "gdelta", "gz", "gB", "gC", "gA", "gD", "gbias"))):
+            setattr(a, f, t.data_ptr())
+        n = lib.wkv_selective_scan_ckpt_bytes(ctypes.byref(a))
+        ck = torch.empty(n, dtype=torch.uint8, device="cuda")
+        a.ckpt, a.ckpt_bytes = ck.data_ptr(), n
+        for fn in ("forward", "backward"):
+            n = getattr(lib, f"wkv_selective_scan_{fn}_workspace")(ctypes.byref(a))
+            ws = torch.empty(n, dtype=torch.uint8, device="cuda")
+            a.workspace, a.workspace_bytes = ws.data_ptr() if n else None, n
+            L.check(getattr(lib, f"wkv_selective_scan_{fn}")(ctypes.byref(a), st), fn)
+        torch.cuda.synchronize()
+        check(c, out)
