@@ -288,8 +288,8 @@ int wkv_ddlerp_backward(int B, int T, int C, int nmix, const void *x, const void
  *   y * scale: one scale a row (group = 0), or one per `group` channels (32, 64, 128, 256; the
  *   last may be shorter), scale [rows, ceil(C/group)] = max|y| / 448, 1 where the maximum is
  *   below 2^-100.
- *   Backward (of the form without `scale`): h (x where there was no residual), gy, gh (NULL: 0) -> gx in dtype,
- *   gresidual in res_dtype, gweight in w_dtype. */
+ *   Backward (of the form without `scale`): from h where it is given, else from x + residual (an h in 16 bits has lost
+ *   digits); gy, gh (NULL: 0) -> gx in dtype, gresidual in res_dtype, gweight in w_dtype. */
 typedef struct wkv_rms_norm_args {
     long long rows;
     int C, group;

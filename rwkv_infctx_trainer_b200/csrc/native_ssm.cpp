@@ -34,20 +34,23 @@ struct Rows {
     Tensor t;
     int64_t batch = 0, token = 0;
 };
-// t: [B, T, ...] with everything behind T one run of `n` elements
-Rows rows_of(const Tensor &t, int64_t n) {
+// t: [B, T, ...], or [B, ...] for one token, with everything behind one run of `n` elements
+Rows rows_of(const Tensor &t, int64_t n, bool one_token) {
     if (!t.defined()) return {};
+    const int64_t lead = one_token ? 1 : 2;
+    const auto sizes = t.sizes(), strides = t.strides();
     int64_t run = 1;
     bool packed = true;
-    for (int64_t i = t.dim() - 1; i >= 2; i--) {
-        if (t.size(i) != 1 && t.stride(i) != run) packed = false;
-        run *= t.size(i);
+    for (int64_t i = t.dim() - 1; i >= lead; i--) {
+        if (sizes[i] != 1 && strides[i] != run) packed = false;
+        run *= sizes[i];
     }
+    // (offsets inside a block of tokens are 32-bit, and a dimension of one element may have any stride)
+    if (!one_token && sizes[1] > 1 && strides[1] > (1 << 26)) packed = false;
     const Tensor c = packed ? t : t.contiguous();
-    // (a dimension of one element may have any stride)
-    return {c, c.size(0) > 1 ? c.stride(0) : n * c.size(1), c.size(1) > 1 ? c.stride(1) : n};
+    const int64_t token = one_token || c.size(1) <= 1 ? n : c.stride(1);
+    return {c, c.size(0) > 1 ? c.stride(0) : token, token};
 }
-Tensor with_token(const Tensor &t) { return t.defined() ? t.unsqueeze(1) : t; }
 
 // ------------------------------------------------------------------------------ norm
 struct NormCall {
@@ -86,7 +89,8 @@ struct RmsNormBackward : OpNode {
     variable_list apply(variable_list &&grads) override {
         at::AutoDispatchBelowADInplaceOrView below;
         const variable_list st = unpack();
-        const Tensor &h = st[0], &weight = st[1];
+        const Tensor &weight = st[0], &x = st[1], &residual = st[2], &kept = st[3];
+        const Tensor &h = kept.defined() ? kept : residual.defined() ? residual : x;      // (of h's size and type)
         c10::cuda::OptionalCUDAGuard guard(h.device());
         const Tensor gy = grads[0].defined() ? as_contig(grads[0], x_type) : Tensor();
         const Tensor gh = has_residual && grads[1].defined() ? as_contig(grads[1], h.scalar_type()) : Tensor();
@@ -101,7 +105,7 @@ struct RmsNormBackward : OpNode {
         a.rows = h.numel() / h.size(-1);
         a.dtype = dtype_code(x_type); a.res_dtype = dtype_code(h.scalar_type()); a.w_dtype = dtype_code(weight.scalar_type());
         a.eps = (float)eps;
-        a.weight = ptr(weight); a.h = ptr(h); a.gy = ptr(gy); a.gh = ptr(gh);
+        a.weight = ptr(weight); a.x = ptr(x); a.residual = ptr(residual); a.h = ptr(kept); a.gy = ptr(gy); a.gh = ptr(gh);
         a.gx = ptr(gx); a.gresidual = ptr(gres); a.gweight = ptr(gw);
         if (want_w) {
             a.workspace_bytes = wkv_rms_norm_backward_workspace(&a);
@@ -128,20 +132,21 @@ variable_list rms_norm(const Tensor &x, const Tensor &weight, const OptTensor &r
         node->x_type = x.scalar_type();
         node->w_type = weight.scalar_type();
     }
-    Tensor y, h, saved_x, saved_w;
+    Tensor y, h;
+    NormCall c;
     {
         at::AutoDispatchBelowADInplaceOrView below;
-        NormCall c = norm_call(x, weight, residual, eps);
+        c = norm_call(x, weight, residual, eps);
         y = fresh_like(c.x);
         if (residual.defined()) h = fresh_like(c.residual);
         c.a.y = ptr(y); c.a.h = ptr(h);
         check(wkv_rms_norm_forward(&c.a, stream_of(x)), "wkv_rms_norm_forward");
-        saved_x = c.x;
-        saved_w = c.weight;
     }
     if (save) {
-        // h is an output of the node: kept as an alias that has no history (and whose in-place changes are noticed)
-        node->keep({h.defined() ? h.detach() : saved_x, saved_w});
+        // An fp32 h serves the backward pass as well as its terms; it is an output of the node: kept as an alias that has no
+        // history (and whose in-place changes are noticed).
+        if (h.defined() && h.scalar_type() == at::kFloat) node->keep({c.weight, Tensor(), Tensor(), h.detach()});
+        else node->keep({c.weight, c.x, c.residual, Tensor()});
         torch::autograd::set_history(y, node);
         if (h.defined()) torch::autograd::set_history(h, node);
     }
@@ -186,14 +191,15 @@ void check_conv(const Tensor &x, const Tensor &weight, const Tensor &bias, const
     check_sizes(bias, {D}, "bias");
     check_sizes(state, {B, weight.size(-1) - 1, D}, "state");
 }
-ConvCall conv_call(const Rows &x, const Tensor &weight, const Tensor &bias, const Tensor &state, bool silu) {
+// sizes: [B,T,D], or [B,D] for one token
+ConvCall conv_call(const Rows &x, at::IntArrayRef sizes, const Tensor &weight, const Tensor &bias, const Tensor &state, bool silu) {
     ConvCall c;
     c.x = x;
     const auto pt = bias.defined() && bias.scalar_type() != weight.scalar_type() ? at::kFloat : param_type(weight);
     c.weight = as_contig(weight, pt);
     if (bias.defined()) c.bias = as_contig(bias, pt);
     if (state.defined()) c.state = as_contig(state, x.t.scalar_type());
-    c.a.B = small(x.t.size(0), "B"); c.a.T = small(x.t.size(1), "T"); c.a.D = small(x.t.size(2), "D");
+    c.a.B = small(sizes[0], "B"); c.a.T = sizes.size() == 2 ? 1 : small(sizes[1], "T"); c.a.D = small(sizes.back(), "D");
     c.a.W = (int)weight.size(-1);
     c.a.dtype = dtype_code(x.t.scalar_type()); c.a.w_dtype = dtype_code(pt);
     c.a.silu = silu;
@@ -212,7 +218,7 @@ struct CausalConvBackward : OpNode {
         const variable_list st = unpack();
         const Tensor &x = st[0];
         c10::cuda::OptionalCUDAGuard guard(x.device());
-        ConvCall c = conv_call(rows_of(x, x.size(2)), st[1], st[2], st[3], silu);
+        ConvCall c = conv_call(rows_of(x, x.size(2), false), x.sizes(), st[1], st[2], st[3], silu);
         const auto dt = x.scalar_type(), pt = c.weight.scalar_type();
         const int64_t B = x.size(0), D = x.size(2), W = c.a.W;
         const Tensor gy = grads[0].defined() ? as_contig(grads[0], dt) : Tensor(), gs = grads[1].defined() ? as_contig(grads[1], dt) : Tensor();
@@ -253,7 +259,7 @@ std::tuple<Tensor, Tensor> causal_conv(const Tensor &x, const Tensor &weight, co
     Tensor y, s;
     {
         at::AutoDispatchBelowADInplaceOrView below;
-        ConvCall c = conv_call(rows_of(x, x.size(2)), weight, bias, state, silu);
+        ConvCall c = conv_call(rows_of(x, x.size(2), false), x.sizes(), weight, bias, state, silu);
         y = fresh(x.sizes(), x.scalar_type(), x);
         s = fresh({x.size(0), c.a.W - 1, x.size(2)}, x.scalar_type(), x);
         c.a.y = ptr(y); c.a.state_out = ptr(s);
@@ -276,7 +282,7 @@ Tensor causal_conv_step(const Tensor &x, const Tensor &state, const Tensor &weig
     refuse_grad({&x, &state, &weight, &bias}, "causal_conv_step", "causal_conv");
     require_cuda({&x, &state, &weight, &bias});
     c10::cuda::OptionalCUDAGuard guard(x.device());
-    ConvCall c = conv_call(rows_of(x.unsqueeze(1), x.size(1)), weight, bias, state, silu);
+    ConvCall c = conv_call(rows_of(x, x.size(1), true), x.sizes(), weight, bias, state, silu);
     Tensor y = fresh(x.sizes(), x.scalar_type(), x);
     c.a.y = ptr(y); c.a.state_out = ptr(state);
     check(wkv_causal_conv_forward(&c.a, stream_of(x)), "wkv_causal_conv_forward");
@@ -290,14 +296,15 @@ struct ScanCall {
     Tensor A, D, bias, state;
     wkv_selective_scan_args_t a = {};
 };
-// u, delta, z [B,T,D]; A [D,N]; B, C [B,T,N] or [B,T,G,N]; D, delta_bias [D]; state [B,D,N]
+// u, delta, z [B,T,D]; A [D,N]; B, C [B,T,N] or [B,T,G,N]; D, delta_bias [D]; state [B,D,N]; for one token without T
 void check_scan(const Tensor &u, const Tensor &delta, const Tensor &A, const Tensor &Bm, const Tensor &Cm, const Tensor &D, const Tensor &z,
                 const Tensor &bias, const Tensor &state) {
     const auto dt = u.scalar_type();
     dtype_code(dt);
     for (auto [t, name] : {std::pair<const Tensor *, const char *>{&delta, "delta"}, {&Bm, "B"}, {&Cm, "C"}, {&z, "z"}}) check_type(*t, dt, name);
     for (auto [t, name] : {std::pair<const Tensor *, const char *>{&A, "A"}, {&D, "D"}, {&bias, "delta_bias"}, {&state, "state"}}) check_param(*t, name);
-    const int64_t B = u.size(0), T = u.size(1), d = u.size(2);
+    const bool one = u.dim() == 2;
+    const int64_t B = u.size(0), T = one ? 1 : u.size(1), d = u.size(-1);
     TORCH_CHECK_VALUE(A.dim() == 2 && A.size(0) == d && A.size(1) >= 1 && A.size(1) <= 64, "A must be [D,N] with D = ", d, " and 1 <= N <= 64, got ", A.sizes());
     const int64_t N = A.size(1);
     check_sizes(delta, u.sizes(), "delta");
@@ -305,25 +312,26 @@ void check_scan(const Tensor &u, const Tensor &delta, const Tensor &A, const Ten
     check_sizes(D, {d}, "D");
     check_sizes(bias, {d}, "delta_bias");
     check_sizes(state, {B, d, N}, "state");
-    const int64_t G = Bm.dim() == 4 ? Bm.size(2) : 1;
+    const int64_t lead = one ? 1 : 2, G = Bm.dim() == lead + 2 ? Bm.size(lead) : 1;
     TORCH_CHECK_VALUE(G >= 1 && d % G == 0, "the groups of B must divide the channels: ", G, " of ", d);
-    TORCH_CHECK_VALUE(Bm.dim() == 4 ? Bm.sizes() == at::IntArrayRef({B, T, G, N}) : Bm.sizes() == at::IntArrayRef({B, T, N}),
-                      "B must be [B,T,N] or [B,T,G,N], got ", Bm.sizes());
+    TORCH_CHECK_VALUE((Bm.dim() == lead + 1 || Bm.dim() == lead + 2) && Bm.size(0) == B && (one || Bm.size(1) == T) && Bm.size(-1) == N,
+                      one ? "B must be [B,N] or [B,G,N], got " : "B must be [B,T,N] or [B,T,G,N], got ", Bm.sizes());
     check_sizes(Cm, Bm.sizes(), "C");
     require_cuda({&u, &delta, &A, &Bm, &Cm, &D, &z, &bias, &state});
 }
 ScanCall scan_call(const Tensor &u, const Tensor &delta, const Tensor &A, const Tensor &Bm, const Tensor &Cm, const Tensor &D, const Tensor &z,
                    const Tensor &bias, const Tensor &state, bool softplus) {
     ScanCall c;
-    const int64_t d = u.size(2), N = A.size(1), G = Bm.dim() == 4 ? Bm.size(2) : 1;
-    c.u = rows_of(u, d); c.delta = rows_of(delta, d); c.z = rows_of(z, d);
-    c.B = rows_of(Bm, G * N); c.C = rows_of(Cm, G * N);
+    const bool one = u.dim() == 2;
+    const int64_t lead = one ? 1 : 2, d = u.size(-1), N = A.size(1), G = Bm.dim() == lead + 2 ? Bm.size(lead) : 1;
+    c.u = rows_of(u, d, one); c.delta = rows_of(delta, d, one); c.z = rows_of(z, d, one);
+    c.B = rows_of(Bm, G * N, one); c.C = rows_of(Cm, G * N, one);
     c.A = as_contig(A, at::kFloat);
     if (D.defined()) c.D = as_contig(D, at::kFloat);
     if (bias.defined()) c.bias = as_contig(bias, at::kFloat);
     if (state.defined()) c.state = as_contig(state, at::kFloat);
     wkv_selective_scan_args_t &a = c.a;
-    a.B = small(u.size(0), "B"); a.T = small(u.size(1), "T"); a.D = small(d, "D"); a.N = (int)N; a.G = (int)G;
+    a.B = small(u.size(0), "B"); a.T = one ? 1 : small(u.size(1), "T"); a.D = small(d, "D"); a.N = (int)N; a.G = (int)G;
     a.dtype = dtype_code(u.scalar_type()); a.softplus = softplus;
     a.u = ptr(c.u.t); a.delta = ptr(c.delta.t); a.Bm = ptr(c.B.t); a.Cm = ptr(c.C.t); a.z = ptr(c.z.t);
     a.u_batch = c.u.batch; a.u_token = c.u.token; a.delta_batch = c.delta.batch; a.delta_token = c.delta.token;
@@ -410,15 +418,13 @@ std::tuple<Tensor, Tensor> selective_scan(const Tensor &u, const Tensor &delta, 
 Tensor selective_scan_step(const Tensor &u, const Tensor &delta, const Tensor &A, const Tensor &Bm, const Tensor &Cm, const Tensor &state,
                            const OptTensor &D_, const OptTensor &z_, const OptTensor &bias_, bool softplus) {
     const Tensor D = opt(D_), z = opt(z_), bias = opt(bias_);
-    TORCH_CHECK_VALUE(u.dim() == 2 && delta.dim() == 2 && (Bm.dim() == 2 || Bm.dim() == 3) && Cm.dim() == Bm.dim() && (!z.defined() || z.dim() == 2),
-                      "u, delta, z must be [B,D]; B, C [B,N] or [B,G,N]");
+    TORCH_CHECK_VALUE(u.dim() == 2, "u must be [B,D], got ", u.sizes());
     refuse_grad({&u, &delta, &A, &Bm, &Cm, &D, &z, &bias, &state}, "selective_scan_step", "selective_scan");
-    const Tensor u1 = with_token(u), d1 = with_token(delta), B1 = with_token(Bm), C1 = with_token(Cm), z1 = with_token(z);
     check_type(state, at::kFloat, "state");
     check_in_place(state, "selective_scan_step");
-    check_scan(u1, d1, A, B1, C1, D, z1, bias, state);
+    check_scan(u, delta, A, Bm, Cm, D, z, bias, state);
     c10::cuda::OptionalCUDAGuard guard(u.device());
-    ScanCall c = scan_call(u1, d1, A, B1, C1, D, z1, bias, state, softplus);
+    ScanCall c = scan_call(u, delta, A, Bm, Cm, D, z, bias, state, softplus);
     Tensor y = fresh(u.sizes(), u.scalar_type(), u);
     c.a.y = ptr(y); c.a.state_out = (float *)ptr(state);
     check(wkv_selective_scan_forward(&c.a, stream_of(u)), "wkv_selective_scan_forward");

@@ -7,6 +7,9 @@
 //   backward, with gh the gradient that reaches h from elsewhere:
 //   xh = h r,  gx = gh + r (gy weight - xh mean(gy weight xh)),  gweight = sum over the rows of gy xh
 //
+// Both passes start from the sum before it is rounded: a backward pass from an h in bf16 was 2^-9 off in gweight, which is
+// a sum in fp32.
+//
 // All are bound by HBM: a row crosses once per pass, a thread owns runs of 8 channels and keeps them in registers from
 // the sum to the output; the next row's values are on their way meanwhile.  A CTA takes every gridDim-th row, so that the
 // weights (and the sums of their gradient) stay in registers.  Sums are fp32 and in a fixed order.
@@ -180,7 +183,7 @@ __global__ void __launch_bounds__(512) k_rms_norm_fwd(NormArgs a) {
 }
 
 struct NormBwdArgs {
-    const void *h, *w, *gy, *gh;
+    const void *h, *x, *res, *w, *gy, *gh;         // h, or x and the residual
     void *gx, *gres;
     float *part;                        // [gridDim.x, C], NULL when the weight needs no gradient
     long long rows;
@@ -188,14 +191,15 @@ struct NormBwdArgs {
     float eps;
 };
 
-template <typename X, typename R, int NV>
+// SUM: h = x + residual (or x alone), else h is read
+template <typename X, typename R, int NV, bool SUM>
 __global__ void __launch_bounds__(512) k_rms_norm_bwd(NormBwdArgs a) {
     pdl_wait();
     pdl_trigger();
     __shared__ float2 red[2][16];
     const int tid = threadIdx.x, nt = blockDim.x, nwarp = nt >> 5, C = a.C;
-    const R *h = (const R *)a.h, *gh = (const R *)a.gh;
-    const X *gy = (const X *)a.gy;
+    const R *h = SUM ? (const R *)a.res : (const R *)a.h, *gh = (const R *)a.gh;
+    const X *x = (const X *)a.x, *gy = (const X *)a.gy;
     const bool vec = a.vec;
     float w[NV][RUN], gw[NV][RUN];
     int left[NV];
@@ -207,14 +211,16 @@ __global__ void __launch_bounds__(512) k_rms_norm_bwd(NormBwdArgs a) {
         for (int q = 0; q < RUN; q++) { w[i][q] = q < left[i] ? param_at(a.w, a.w_dtype, c + q) : 0.f; gw[i][q] = 0.f; }
     }
     Raw<R, RUN> rh[NV], rg[NV];
-    Raw<X, RUN> ry[NV];
+    Raw<X, RUN> ry[NV], rx[SUM ? NV : 1];
     auto fetch = [&](long long row) {
 #pragma unroll
         for (int i = 0; i < NV; i++) {
             const size_t at = (size_t)row * C + (size_t)(tid + i * nt) * RUN;
             rh[i].zero(); rg[i].zero(); ry[i].zero();
+            if (SUM) rx[i].zero();
             if (left[i] > 0 && row < a.rows) {
-                rh[i].load(h + at, vec, left[i]);
+                if (h) rh[i].load(h + at, vec, left[i]);
+                if (SUM) rx[i].load(x + at, vec, left[i]);
                 if (gy) ry[i].load(gy + at, vec, left[i]);
                 if (gh) rg[i].load(gh + at, vec, left[i]);
             }
@@ -230,6 +236,12 @@ __global__ void __launch_bounds__(512) k_rms_norm_bwd(NormBwdArgs a) {
         for (int i = 0; i < NV; i++) {
             rh[i].get(hv[i]);
             ry[i].get(g[i]);
+            if (SUM) {
+                float t[RUN];
+                rx[i].get(t);
+#pragma unroll
+                for (int q = 0; q < RUN; q++) hv[i][q] += t[q];
+            }
             keep[i] = rg[i];
 #pragma unroll
             for (int q = 0; q < RUN; q++) { s.x += hv[i][q] * hv[i][q]; s.y += g[i][q] * w[i][q] * hv[i][q]; }
@@ -337,21 +349,23 @@ extern "C" int wkv_rms_norm_backward(const wkv_rms_norm_args_t *a, void *stream)
     if (e != WKV_OK) return e;
     cudaStream_t s = (cudaStream_t)stream;
     const int nt = threads_for(a->C), nb = ctas_for(a->rows, a->C, 1024), nv = runs_per_thread(a->C);
-    if (a->rows > 0 && !a->h) return WKV_ERR_NULL;
+    if (a->rows > 0 && !a->h && !a->x) return WKV_ERR_NULL;
+    if (!a->h && !a->residual && a->res_dtype != a->dtype) return WKV_ERR_DTYPE;
     if (a->gweight && a->rows > 0) {
         if (!a->workspace || a->workspace_bytes < wkv_rms_norm_backward_workspace(a)) return WKV_ERR_WORKSPACE;
         if (!aligned16(a->workspace)) return WKV_ERR_ALIGN;
     }
     NormBwdArgs k = {};
-    k.h = a->h; k.w = a->weight; k.gy = a->gy; k.gh = a->gh; k.gx = a->gx; k.gres = a->gresidual;
+    k.h = a->h; k.x = a->x; k.res = a->residual; k.w = a->weight; k.gy = a->gy; k.gh = a->gh; k.gx = a->gx; k.gres = a->gresidual;
     k.part = a->gweight ? (float *)a->workspace : nullptr;
     k.rows = a->rows; k.C = a->C; k.w_dtype = a->w_dtype; k.eps = a->eps;
-    k.vec = a->C % RUN == 0 && all_aligned({a->h, a->gy, a->gh, a->gx, a->gresidual});
+    k.vec = a->C % RUN == 0 && all_aligned({a->h, a->x, a->residual, a->gy, a->gh, a->gx, a->gresidual});
     if (a->rows > 0) {
         e = by_types(a->dtype, a->res_dtype, [&](auto x, auto r) {
             using X = decltype(x);
             using R = decltype(r);
-            return launch_chained(nv == 2 ? k_rms_norm_bwd<X, R, 2> : k_rms_norm_bwd<X, R, 4>, dim3(nb), dim3(nt), 0, s, k);
+            if (k.h) return launch_chained(nv == 2 ? k_rms_norm_bwd<X, R, 2, false> : k_rms_norm_bwd<X, R, 4, false>, dim3(nb), dim3(nt), 0, s, k);
+            return launch_chained(nv == 2 ? k_rms_norm_bwd<X, R, 2, true> : k_rms_norm_bwd<X, R, 4, true>, dim3(nb), dim3(nt), 0, s, k);
         });
         if (e != WKV_OK) return e;
     }

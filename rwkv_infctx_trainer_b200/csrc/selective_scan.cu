@@ -10,11 +10,13 @@
 //   gdt_t = u_t (G_t . B_t) + sum_n G_t A a_t h_{t-1},  gA = sum_t G_t dt_t a_t h_{t-1}
 //   gz_t = gy_t y_t silu'(z_t)  (y before the gate),  gD = sum dy u,  gdelta = gdt sigmoid(delta + bias)
 //
-// A thread owns four states of a channel and keeps them in fp32 registers; LPC lanes share a channel (N <= 4 LPC, padded
-// states have A = B = C = 0 and stay zero), a warp 32/LPC channels.  Tokens come in blocks of 16: what is per token and
-// channel (softplus, gates, loads, stores) is divided among the channel's lanes, lane q taking the tokens that are q mod LPC;
-// sums over n are exchanged so that each lane ends with those of its own tokens.  Warps do not wait for one another in the
-// forward pass.
+// A thread owns four states of each of two neighbouring channels and keeps them in fp32 registers (pairs of states, on packed
+// instructions); LPC lanes share the two channels (N <= 4 LPC, padded states have A = B = C = 0 and stay zero), a warp has
+// 64 / LPC channels.  Two channels, because what bounded a thread with one was the shared memory's path to the registers:
+// B and C of a token are 32 bytes a lane, 8 of the 12 cycles that a warp's loads took per token.  Tokens come in blocks of 16:
+// what is per token and channel (softplus, gates, loads, stores) is divided among the channels' lanes, lane q taking the
+// tokens that are q mod LPC; sums over n are exchanged so that each lane ends with those of its own tokens.
+// Warps do not wait for one another in the forward pass.
 //
 // Few chains (B x D): the tokens of a row are cut into spans that run in parallel.  The decay over a span is exp(A sum dt),
 // so a first pass leaves each span's contribution from zero and sum dt, and the full pass starts from their fold.
@@ -40,7 +42,7 @@ __device__ __forceinline__ float ex2(float x) {
 struct ScanArgs {
     int B, T, D, N, G, Dg, softplus;
     int ncb, nspan, span_blocks, nblk;           // channel blocks per group, spans of a row, their length, blocks of a row
-    int vec_b, vec_c;
+    int vec_b, vec_c, vec_a, vec_s;
     const void *u, *delta, *Bm, *Cm, *z;
     long long u_batch, u_token, delta_batch, delta_token, B_batch, B_token, C_batch, C_token, z_batch, z_token;
     const float *A, *Dskip, *bias, *state_in;
@@ -54,51 +56,132 @@ struct ScanArgs {
     float *part_bc, *part;                       // [ncb, B, T, G, 8 LPC]; [B * nspan, D (N + 2)]
 };
 
-// softplus(x) and its derivative sigmoid(x), for any x: with t = e^-|x| no term overflows and log1p keeps small steps exact
+__device__ __forceinline__ float rcp(float x) {
+    float y;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ float sigm(float x) { return rcp(1.f + ex2(-LOG2E * x)); }
+
+// softplus(x) = max(x, 0) + log(1 + t), t = e^-|x|, and with SIG its derivative sigmoid(x), for any x: no term overflows.
+// log(1 + t) = 2 artanh(s), s = t / (2 + t) <= 1/3: its power series up to s^13 is off by less than 2 s^15 / 15, a
+// relative 1.4e-8, and keeps the digits of small steps (log of a rounded 1 + t does not).
+template <bool SIG>
 __device__ __forceinline__ float softplus(float x, float &sig) {
-    const float t = __expf(-fabsf(x)), r = __fdividef(1.f, 1.f + t);
-    sig = x >= 0.f ? r : t * r;
-    // (fmaxf drops a NaN, log1pf brings it back)
-    return fmaxf(x, 0.f) + log1pf(t);
+    const float t = ex2(-LOG2E * fabsf(x));
+    float s;
+    if (SIG) {
+        const float w = rcp((1.f + t) * (2.f + t)), r = (2.f + t) * w;       // r = 1 / (1 + t)
+        s = t * (1.f + t) * w;
+        sig = x >= 0.f ? r : t * r;
+    } else {
+        s = t * rcp(2.f + t);
+    }
+    const float s2 = s * s;
+    float p = 1.f / 13.f;
+    p = p * s2 + 1.f / 11.f;
+    p = p * s2 + 1.f / 9.f;
+    p = p * s2 + 1.f / 7.f;
+    p = p * s2 + 1.f / 5.f;
+    p = p * s2 + 1.f / 3.f;
+    p = p * s2 + 1.f;
+    // (fmaxf drops a NaN, s brings it back)
+    return fmaxf(x, 0.f) + 2.f * s * p;
 }
 
-// What a warp works on: LPC lanes a channel, lane = c * LPC + q.
+template <bool SIG, int PT>
+__device__ __forceinline__ void softplus_all(f2 (&x)[PT], f2 (&sig)[PT]) {
+#pragma unroll
+    for (int i = 0; i < PT; i++) {
+        f2 g;
+        x[i] = make_float2(softplus<SIG>(x[i].x, g.x), softplus<SIG>(x[i].y, g.y));
+        if (SIG) sig[i] = g;
+    }
+}
+
+// What a warp works on: LPC lanes for two channels, lane = c * LPC + q.
 template <int LPC>
 struct Geo {
-    static constexpr int CPW = 32 / LPC;         // channels of a warp
+    static constexpr int CL = 32 / LPC;          // pairs of channels of a warp
+    static constexpr int CPW = 2 * CL;           // channels of a warp
     static constexpr int PT = TB / LPC;          // tokens of a block that are a lane's own
     static constexpr int NP = 4 * LPC;           // states with padding
     static constexpr int NI = (TB * LPC + 31) / 32;      // runs of four of a B or C block that a lane loads
+    // rows of what a warp keeps per token and pair of channels, padded so that lanes that write neighbouring tokens use
+    // different banks (16 and 8 bytes an element)
+    static constexpr int ROW16 = CL + (LPC == 2 ? 4 : LPC == 4 ? 2 : 1);
+    static constexpr int ROW8 = CL + (LPC == 2 ? 8 : LPC == 4 ? 4 : LPC == 8 ? 2 : 1);
 };
 
-// the values of a block that a lane brings in, on their way while the block before is worked on
-template <typename F, int LPC>
-struct BlockBC {
-    Raw<F, 4> b[Geo<LPC>::NI], c[Geo<LPC>::NI];
-    __device__ __forceinline__ void load(const ScanArgs &a, int batch, int grp, int t0, int t_end, int lane) {
+// A lane's own tokens of a block in one tensor: token q + LPC i of the block, 64-bit block address, 32-bit offsets inside
+// (the host checks the strides).  Tokens behind the row's last are read as the last one, without a branch around the loads,
+// and made zero later; rows of B and C behind it are zeros at once.
+//
+// FAST: the two channels are one aligned access in every tensor, and so are runs of four of B and C; else the second channel
+// is `second` elements on (0 where there is none).  Compiled apart: a branch at each access keeps the compiler from moving
+// work across it, and with one or two warps on a scheduler that is what a token's time was (forward 94 us of 4 x 512 tokens of
+// 4096 channels with the branches).
+template <typename F, int LPC, bool FAST>
+struct Own {
+    Raw<F, 2> v[Geo<LPC>::PT];
+    __device__ __forceinline__ void load(const F *block, int token_stride, int q, int last, int second) {
 #pragma unroll
-        for (int k = 0; k < Geo<LPC>::NI; k++) {
-            const int i = lane + 32 * k, t = t0 + i / LPC, n0 = 4 * (i % LPC), n = min(4, a.N - n0);
-            b[k].zero();
-            c[k].zero();
-            if (i < TB * LPC && t < t_end && n > 0) {
-                b[k].load((const F *)a.Bm + (size_t)batch * a.B_batch + (size_t)t * a.B_token + (size_t)grp * a.N + n0, a.vec_b, n);
-                c[k].load((const F *)a.Cm + (size_t)batch * a.C_batch + (size_t)t * a.C_token + (size_t)grp * a.N + n0, a.vec_c, n);
+        for (int i = 0; i < Geo<LPC>::PT; i++) {
+            const F *p = block + (long long)min(q + LPC * i, last) * token_stride;
+            if (FAST) {
+                v[i].load(p, true, 2);
+            } else {
+                alignas(8) const F two[2] = {p[0], p[second]};
+                v[i] = *reinterpret_cast<const Raw<F, 2> *>(two);
             }
         }
     }
-    // sB, sC: [TB][NP]
-    __device__ __forceinline__ void put(float *sB, float *sC, int lane) const {
+    __device__ __forceinline__ f2 get(int i) const {
+        float f[2];
+        v[i].get(f);
+        return make_float2(f[0], f[1]);
+    }
+};
+template <typename F>
+__device__ __forceinline__ f2 pair_of(const Raw<F, 2> &r) {
+    float f[2];
+    r.get(f);
+    return make_float2(f[0], f[1]);
+}
+template <bool FAST, typename F>
+__device__ __forceinline__ void store_pair(F *p, bool second, f2 v) {
+    const float f[2] = {v.x, v.y};
+    if (FAST) {
+        Raw<F, 2> r;
+        r.put(f);
+        r.store(p, true, 2);
+    } else {
+        Elem<F>::st(p, v.x);
+        if (second) Elem<F>::st(p + 1, v.y);
+    }
+}
+
+// the rows of B or C of a block, on their way while the block before is worked on
+template <typename F, int LPC, bool FAST>
+struct BlockRows {
+    Raw<F, 4> r[Geo<LPC>::NI];
+    // p: row of the block's first token, state 0
+    __device__ __forceinline__ void load(const F *p, int token_stride, bool vec, int N, int last, int lane) {
+#pragma unroll
+        for (int k = 0; k < Geo<LPC>::NI; k++) {
+            const int i = lane + 32 * k, n0 = 4 * (i % LPC), n = min(4, N - n0);
+            r[k].zero();
+            if (n > 0 && i / LPC <= min(last, TB - 1)) r[k].load(p + (long long)(i / LPC) * token_stride + n0, FAST || vec, n);
+        }
+    }
+    // to: [TB][NP]
+    __device__ __forceinline__ void put(float *to, int lane) const {
 #pragma unroll
         for (int k = 0; k < Geo<LPC>::NI; k++) {
             const int i = lane + 32 * k;
-            if (i < TB * LPC) {
-                float f[4];
-                b[k].get(f);
-                *reinterpret_cast<float4 *>(sB + 4 * i) = make_float4(f[0], f[1], f[2], f[3]);
-                c[k].get(f);
-                *reinterpret_cast<float4 *>(sC + 4 * i) = make_float4(f[0], f[1], f[2], f[3]);
-            }
+            float f[4];
+            r[k].get(f);
+            if (TB * LPC >= 32 || i < TB * LPC) *reinterpret_cast<float4 *>(to + 4 * i) = make_float4(f[0], f[1], f[2], f[3]);
         }
     }
 };
@@ -121,492 +204,780 @@ __device__ __forceinline__ float sum_tokens(float (&v)[NB], int q) {
     return s;
 }
 
-__device__ __forceinline__ void load_states(const float *p, size_t at, int n0, int N, float *h) {
+// four neighbouring states as two pairs; `swap`: the second pair first
+__device__ __forceinline__ void load_states(const float *p, size_t at, int n0, int N, f2 (&h)[2], bool swap = false) {
+    float f[4];
+    if (p != nullptr && N % 4 == 0 && (reinterpret_cast<uintptr_t>(p) & 15u) == 0) {
+        const float4 v = n0 < N ? *reinterpret_cast<const float4 *>(p + at + n0) : make_float4(0.f, 0.f, 0.f, 0.f);
+        f[0] = v.x; f[1] = v.y; f[2] = v.z; f[3] = v.w;
+    } else {
 #pragma unroll
-    for (int i = 0; i < 4; i++) h[i] = p != nullptr && n0 + i < N ? p[at + n0 + i] : 0.f;
+        for (int i = 0; i < 4; i++) f[i] = p != nullptr && n0 + i < N ? p[at + n0 + i] : 0.f;
+    }
+    const f2 a = make_float2(f[0], f[1]), b = make_float2(f[2], f[3]);
+    h[0] = swap ? b : a;
+    h[1] = swap ? a : b;
 }
-__device__ __forceinline__ void store_states(float *p, size_t at, int n0, int N, const float *h) {
+__device__ __forceinline__ void store_states(float *p, size_t at, int n0, int N, const f2 (&h)[2], bool swap = false) {
+    const f2 a = swap ? h[1] : h[0], b = swap ? h[0] : h[1];
+    const float f[4] = {a.x, a.y, b.x, b.y};
     if (N % 4 == 0 && (reinterpret_cast<uintptr_t>(p) & 15u) == 0) {
-        if (n0 < N) *reinterpret_cast<float4 *>(p + at + n0) = make_float4(h[0], h[1], h[2], h[3]);
+        if (n0 < N) *reinterpret_cast<float4 *>(p + at + n0) = make_float4(f[0], f[1], f[2], f[3]);
     } else {
 #pragma unroll
         for (int i = 0; i < 4; i++)
-            if (n0 + i < N) p[at + n0 + i] = h[i];
+            if (n0 + i < N) p[at + n0 + i] = f[i];
     }
 }
+// A log2(e) of four states.  An infinite A (the exponential of a large parameter) becomes the largest number: its decay is
+// zero all the same, and tokens behind a row's end, with a step of zero, keep the state.
+__device__ __forceinline__ void load_decays(const float *A, size_t at, int n0, int N, f2 (&A2)[2], bool swap = false) {
+    constexpr float MOST = 3.4e38f;
+    auto clamp = [](float x) { return x < -MOST ? -MOST : x > MOST ? MOST : x; };      // (a NaN stays)
+    load_states(A, at, n0, N, A2, swap);
+#pragma unroll
+    for (int i = 0; i < 2; i++) A2[i] = make_float2(clamp(A2[i].x * LOG2E), clamp(A2[i].y * LOG2E));
+}
+__device__ __forceinline__ f2 ex2(f2 x) { return make_float2(ex2(x.x), ex2(x.y)); }
+// two pairs of floats in shared memory
+__device__ __forceinline__ void pairs_at(const float *p, f2 &a, f2 &b) {
+    const float4 v = *reinterpret_cast<const float4 *>(p);
+    a = make_float2(v.x, v.y);
+    b = make_float2(v.z, v.w);
+}
+
+// The unit of a warp of the forward and the summary kernels: ((batch * spans + span) * G + group) * ncb + channel block.
+struct Unit {
+    int cb, grp, span, b;
+    __device__ __forceinline__ Unit(const ScanArgs &a, long long i, int nspan) {
+        cb = (int)(i % a.ncb);
+        i /= a.ncb;
+        grp = (int)(i % a.G);
+        i /= a.G;
+        span = (int)(i % nspan);
+        b = (int)(i / nspan);
+    }
+};
 
 // Forward.  SUMMARY: only the span's contribution from zero and its sum of dt.
-template <typename F, int LPC, bool SUMMARY>
-__global__ void __launch_bounds__(128) k_scan_fwd(ScanArgs a) {
+template <typename F, int LPC, bool SUMMARY, bool FAST>
+__global__ void __launch_bounds__(128, SUMMARY ? 4 : 3) k_scan_fwd(ScanArgs a) {
     pdl_wait();
     pdl_trigger();
     using P = Geo<LPC>;
-    __shared__ __align__(16) float2 s_dt[4][TB][P::CPW];
-    __shared__ __align__(16) float s_b[4][TB * P::NP], s_c[4][TB * P::NP];
+    __shared__ __align__(16) float4 s_dt[4][TB][P::ROW16];              // dt, dt u of the first channel, of the second
+    __shared__ __align__(16) float s_b[4][TB * P::NP], s_c[SUMMARY ? 1 : 4][TB * P::NP];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, c = lane / LPC, q = lane % LPC;
-    // unit = ((batch * spans + span) * G + group) * ncb + channel block
-    long long unit = (long long)blockIdx.x * 4 + warp;
-    const int cb = (int)(unit % a.ncb);
-    unit /= a.ncb;
-    const int grp = (int)(unit % a.G);
-    unit /= a.G;
-    const int nspan = SUMMARY ? a.nspan - 1 : a.nspan;       // (nobody asks for the last span's contribution)
-    const int span = (int)(unit % nspan), b = (int)(unit / nspan);
-    if (b >= a.B) return;
-    const int cg = cb * P::CPW + c, ch = grp * a.Dg + cg, n0 = 4 * q;
-    const bool live = cg < a.Dg;
+    const Unit un(a, (long long)blockIdx.x * 4 + warp, SUMMARY ? a.nspan - 1 : a.nspan);     // (nobody asks for the last span's contribution)
+    if (un.b >= a.B) return;
+    const int b = un.b, grp = un.grp, cg = un.cb * P::CPW + 2 * c, n0 = 4 * q;
+    const bool live = cg < a.Dg, live2 = cg + 1 < a.Dg;
+    const int ch = grp * a.Dg + (live ? cg : 0), second = live2 ? 1 : 0;    // (lanes without a channel read another's, and write nothing)
     const size_t row = ((size_t)b * a.D + ch) * a.N;         // of [B, D, N]
-    float A2[4], h[4];
-    load_states(live ? a.A : nullptr, (size_t)ch * a.N, n0, a.N, A2);
-#pragma unroll
-    for (int i = 0; i < 4; i++) A2[i] *= LOG2E;
+    const int up = second * a.N;                              // to the second channel's states
+    f2 A2[2][2], h[2][2];
+    load_decays(a.A, (size_t)ch * a.N, n0, a.N, A2[0]);
+    load_decays(a.A, (size_t)ch * a.N + up, n0, a.N, A2[1]);
     if (SUMMARY) {
-#pragma unroll
-        for (int i = 0; i < 4; i++) h[i] = 0.f;
+        h[0][0] = h[0][1] = h[1][0] = h[1][1] = both(0.f);
     } else {
-        load_states(live ? a.state_in : nullptr, row, n0, a.N, h);
-        for (int j = 0; j < span; j++) {
+        load_states(a.state_in, row, n0, a.N, h[0]);
+        load_states(a.state_in, row + up, n0, a.N, h[1]);
+        for (int j = 0; j < un.span; j++) {
             const size_t at = ((size_t)b * a.nspan + j) * a.D + ch;
-            float U[4];
-            load_states(live ? a.span_state : nullptr, at * a.N, n0, a.N, U);
-            const float s = live ? a.span_dt[at] : 0.f;
 #pragma unroll
-            for (int i = 0; i < 4; i++) h[i] = ex2(A2[i] * s) * h[i] + U[i];
-        }
-    }
-    const float bias = live && a.bias ? a.bias[ch] : 0.f, dskip = live && a.Dskip ? a.Dskip[ch] : 0.f;
-    const int blk1 = min((span + 1) * a.span_blocks, a.nblk);
-    const F *pu = (const F *)a.u + (size_t)b * a.u_batch + ch, *pd = (const F *)a.delta + (size_t)b * a.delta_batch + ch;
-    const F *pz = a.z ? (const F *)a.z + (size_t)b * a.z_batch + ch : nullptr;
-
-    F ru[P::PT], rd[P::PT], rz[P::PT];
-    BlockBC<F, LPC> bc;
-    auto fetch = [&](int blk) {
-        if (blk >= blk1) return;
+            for (int k = 0; k < 2; k++) {
+                f2 U[2];
+                load_states(a.span_state, at * a.N + k * up, n0, a.N, U);
+                const f2 s = both(a.span_dt[at + k * second]);
 #pragma unroll
-        for (int i = 0; i < P::PT; i++) {
-            const int t = blk * TB + q + LPC * i;
-            if (live && t < a.T) {
-                ru[i] = pu[(size_t)t * a.u_token];
-                rd[i] = pd[(size_t)t * a.delta_token];
-                if (!SUMMARY && pz) rz[i] = pz[(size_t)t * a.z_token];
+                for (int i = 0; i < 2; i++) h[k][i] = fma2(ex2(mul2(A2[k][i], s)), h[k][i], U[i]);
             }
         }
-        bc.load(a, b, grp, blk * TB, a.T, lane);
+    }
+    const f2 bias = a.bias ? make_float2(a.bias[ch], a.bias[ch + second]) : both(0.f);
+    const f2 dskip = a.Dskip ? make_float2(a.Dskip[ch], a.Dskip[ch + second]) : both(0.f);
+    const int blk0 = un.span * a.span_blocks, blk1 = min(blk0 + a.span_blocks, a.nblk), t0 = blk0 * TB;
+    const int su = (int)a.u_token, sd = (int)a.delta_token, sz = (int)a.z_token, sB = (int)a.B_token, sC = (int)a.C_token;
+    const F *pu = (const F *)a.u + (size_t)b * a.u_batch + (size_t)t0 * a.u_token + ch;
+    const F *pd = (const F *)a.delta + (size_t)b * a.delta_batch + (size_t)t0 * a.delta_token + ch;
+    const F *pz = (const F *)a.z + (size_t)b * a.z_batch + (size_t)t0 * a.z_token + ch;
+    const F *pB = (const F *)a.Bm + (size_t)b * a.B_batch + (size_t)t0 * a.B_token + (size_t)grp * a.N;
+    const F *pC = (const F *)a.Cm + (size_t)b * a.C_batch + (size_t)t0 * a.C_token + (size_t)grp * a.N;
+    F *py = SUMMARY ? nullptr : (F *)a.y + ((size_t)b * a.T + t0 + q) * a.D + ch;
+    float *ck = !SUMMARY && a.ckpt && live ? a.ckpt + (((size_t)b * a.nblk + blk0) * a.D + ch) * a.N : nullptr;
+    const bool gated = !SUMMARY && a.z != nullptr;
+
+    Own<F, LPC, FAST> ru, rd, rz;
+    BlockRows<F, LPC, FAST> rB, rC;
+    int last = a.T - 1 - t0;             // the row's last token, counted from the block to be fetched
+    auto fetch = [&]() {
+        ru.load(pu, su, q, last, second);
+        rd.load(pd, sd, q, last, second);
+        if (gated) rz.load(pz, sz, q, last, second);
+        rB.load(pB, sB, a.vec_b, a.N, last, lane);
+        if (!SUMMARY) rC.load(pC, sC, a.vec_c, a.N, last, lane);
+        pu += (long long)su * TB; pd += (long long)sd * TB; pz += (long long)sz * TB;
+        pB += (long long)sB * TB; pC += (long long)sC * TB;
     };
-    fetch(span * a.span_blocks);
-    float total = 0.f;                   // SUMMARY: the lane's part of sum dt
-    for (int blk = span * a.span_blocks; blk < blk1; blk++) {
-        if (!SUMMARY && a.ckpt && live) store_states(a.ckpt, (((size_t)b * a.nblk + blk) * a.D + ch) * a.N, n0, a.N, h);
-        float u[P::PT], z[P::PT];
+    fetch();
+    f2 total = both(0.f);                // SUMMARY: the lane's part of sum dt
+    for (int blk = blk0; blk < blk1; blk++) {
+        if (ck) {
+            store_states(ck, 0, n0, a.N, h[0]);
+            if (live2) store_states(ck, a.N, n0, a.N, h[1]);
+            ck += (size_t)a.D * a.N;
+        }
+        f2 u[P::PT], z[P::PT], y[P::PT], step[P::PT];
         __syncwarp();                    // (the block before has been read)
 #pragma unroll
         for (int i = 0; i < P::PT; i++) {
-            const int t = q + LPC * i;
-            float dt = 0.f;
-            u[i] = 0.f;
-            z[i] = 0.f;
-            if (live && blk * TB + t < a.T) {
-                u[i] = Elem<F>::ld(&ru[i]);
-                dt = Elem<F>::ld(&rd[i]) + bias;
-                float sig;
-                if (a.softplus) dt = softplus(dt, sig);
-                if (!SUMMARY && pz) z[i] = Elem<F>::ld(&rz[i]);
-            }
-            s_dt[warp][t][c] = make_float2(dt, dt * u[i]);
-            total += dt;
+            u[i] = ru.get(i);
+            step[i] = add2(rd.get(i), bias);
+            z[i] = rz.get(i);            // (not used without a gate)
         }
-        bc.put(s_b[warp], s_c[warp], lane);
-        __syncwarp();
-        fetch(blk + 1);
+        if (a.softplus) softplus_all<false>(step, step);
 #pragma unroll
         for (int i = 0; i < P::PT; i++) {
-            float yv[LPC];
+            f2 dt = step[i];
+            if (q + LPC * i > last) dt = u[i] = both(0.f);    // behind the row: a = 1, nothing is added
+            s_dt[warp][q + LPC * i][c] = make_float4(dt.x, dt.x * u[i].x, dt.y, dt.y * u[i].y);
+            if (SUMMARY) total = add2(total, dt);
+        }
+        rB.put(s_b[warp], lane);
+        if (!SUMMARY) rC.put(s_c[warp], lane);
+        __syncwarp();
+        const int end = last;
+        last -= TB;
+        if (blk + 1 < blk1) fetch();
 #pragma unroll
-            for (int j = 0; j < LPC; j++) {
-                const int t = i * LPC + j;
-                const float2 d = s_dt[warp][t][c];
-                const float4 Bv = *reinterpret_cast<const float4 *>(&s_b[warp][t * P::NP + n0]);
-                h[0] = ex2(d.x * A2[0]) * h[0] + d.y * Bv.x;
-                h[1] = ex2(d.x * A2[1]) * h[1] + d.y * Bv.y;
-                h[2] = ex2(d.x * A2[2]) * h[2] + d.y * Bv.z;
-                h[3] = ex2(d.x * A2[3]) * h[3] + d.y * Bv.w;
-                if (!SUMMARY) {
-                    const float4 Cv = *reinterpret_cast<const float4 *>(&s_c[warp][t * P::NP + n0]);
-                    yv[j] = (Cv.x * h[0] + Cv.y * h[1]) + (Cv.z * h[2] + Cv.w * h[3]);
+        for (int i = 0; i < P::PT; i++) {
+            float y0[LPC], y1[LPC];
+            constexpr int GT = LPC < 4 ? LPC : 4;
+#pragma unroll
+            for (int j0 = 0; j0 < LPC; j0 += GT) {
+                f2 dec[GT][2][2], in[GT][2][2];
+#pragma unroll
+                for (int j = 0; j < GT; j++) {
+                    const int t = i * LPC + j0 + j;
+                    const float4 d = s_dt[warp][t][c];
+                    f2 B[2];
+                    pairs_at(&s_b[warp][t * P::NP + n0], B[0], B[1]);
+#pragma unroll
+                    for (int m = 0; m < 2; m++) {
+                        dec[j][0][m] = mul2(both(d.x), A2[0][m]);
+                        dec[j][1][m] = mul2(both(d.z), A2[1][m]);
+                        in[j][0][m] = mul2(both(d.y), B[m]);
+                        in[j][1][m] = mul2(both(d.w), B[m]);
+                    }
+                }
+#pragma unroll
+                for (int j = 0; j < GT; j++)
+#pragma unroll
+                    for (int m = 0; m < 2; m++) { dec[j][0][m] = ex2(dec[j][0][m]); dec[j][1][m] = ex2(dec[j][1][m]); }
+#pragma unroll
+                for (int j = 0; j < GT; j++) {
+                    const int t = i * LPC + j0 + j;
+#pragma unroll
+                    for (int m = 0; m < 2; m++) {
+                        h[0][m] = fma2(dec[j][0][m], h[0][m], in[j][0][m]);
+                        h[1][m] = fma2(dec[j][1][m], h[1][m], in[j][1][m]);
+                    }
+                    if (!SUMMARY) {
+                        f2 C[2];
+                        pairs_at(&s_c[warp][t * P::NP + n0], C[0], C[1]);
+                        const f2 s0 = fma2(C[1], h[0][1], mul2(C[0], h[0][0])), s1 = fma2(C[1], h[1][1], mul2(C[0], h[1][0]));
+                        y0[j0 + j] = s0.x + s0.y;
+                        y1[j0 + j] = s1.x + s1.y;
+                    }
                 }
             }
-            if (!SUMMARY) {
-                float y = sum_tokens<LPC, LPC>(yv, q) + dskip * u[i];
-                if (pz) y *= z[i] * sigmoidf(z[i]);
-                const int t = blk * TB + i * LPC + q;
-                if (live && t < a.T) Elem<F>::st((F *)a.y + ((size_t)b * a.T + t) * a.D + ch, y);
+            if (!SUMMARY) y[i] = make_float2(sum_tokens<LPC, LPC>(y0, q), sum_tokens<LPC, LPC>(y1, q));
+        }
+        if (!SUMMARY) {
+#pragma unroll
+            for (int i = 0; i < P::PT; i++) y[i] = fma2(dskip, u[i], y[i]);
+            if (gated) {
+#pragma unroll
+                for (int i = 0; i < P::PT; i++) y[i] = mul2(y[i], make_float2(z[i].x * sigm(z[i].x), z[i].y * sigm(z[i].y)));
             }
+            if (live) {
+#pragma unroll
+                for (int i = 0; i < P::PT; i++)
+                    if (q + LPC * i <= end) store_pair<FAST>(py + (long long)(LPC * i) * a.D, live2, y[i]);
+            }
+            py += (long long)TB * a.D;
         }
     }
     if (SUMMARY) {
 #pragma unroll
-        for (int m = 1; m < LPC; m <<= 1) total += __shfl_xor_sync(FULL_MASK, total, m);
-        const size_t at = ((size_t)b * a.nspan + span) * a.D + ch;
-        if (live) store_states(a.span_state, at * a.N, n0, a.N, h);
-        if (live && q == 0) a.span_dt[at] = total;
-    } else if (span == a.nspan - 1 && a.state_out && live) {
-        store_states(a.state_out, row, n0, a.N, h);
+        for (int m = 1; m < LPC; m <<= 1)
+            total = add2(total, make_float2(__shfl_xor_sync(FULL_MASK, total.x, m), __shfl_xor_sync(FULL_MASK, total.y, m)));
+        const size_t at = ((size_t)b * a.nspan + un.span) * a.D + ch;
+        if (live) {
+            store_states(a.span_state, at * a.N, n0, a.N, h[0]);
+            if (q == 0) a.span_dt[at] = total.x;
+        }
+        if (live2) {
+            store_states(a.span_state, (at + 1) * a.N, n0, a.N, h[1]);
+            if (q == 0) a.span_dt[at + 1] = total.y;
+        }
+    } else if (un.span == a.nspan - 1 && a.state_out) {
+        if (live) store_states(a.state_out, row, n0, a.N, h[0]);
+        if (live2) store_states(a.state_out, row + a.N, n0, a.N, h[1]);
     }
 }
 
-// One token: a thread for four states; state_out may be state_in (each thread reads its own before it writes).
-template <typename F, int LPC>
+// One token: a thread for four states of a channel, 16 bytes of each tensor, in R rows; state_out may be state_in (each
+// thread reads its own before it writes).  LANES a channel, N <= 4 LANES.  Bound by HBM where rows are many: with four rows a
+// thread A and the parameters are read once for four, and four states are on their way at once.
+template <typename F, int LANES, int R>
 __global__ void __launch_bounds__(256) k_scan_step(ScanArgs a) {
     pdl_wait();
     pdl_trigger();
-    const long long i = ((long long)blockIdx.x * 256 + threadIdx.x) / LPC;
-    const int q = threadIdx.x % LPC, n0 = 4 * q;
-    const bool live = i < (long long)a.B * a.D;
-    const int b = live ? (int)(i / a.D) : 0, ch = live ? (int)(i - (long long)b * a.D) : 0, grp = ch / a.Dg;
-    const size_t row = ((size_t)b * a.D + ch) * a.N;
-    float h[4], A2[4], Bv[4], Cv[4];
-    load_states(live ? a.state_in : nullptr, row, n0, a.N, h);
-    load_states(a.A, (size_t)ch * a.N, n0, a.N, A2);
-    const F *pB = (const F *)a.Bm + (size_t)b * a.B_batch + (size_t)grp * a.N, *pC = (const F *)a.Cm + (size_t)b * a.C_batch + (size_t)grp * a.N;
+    const int i = (blockIdx.x * 256 + threadIdx.x) / LANES, n0 = 4 * (threadIdx.x % LANES), n = a.N - n0;
+    const bool live = i < a.D;
+    const int ch = live ? i : 0, grp = ch / a.Dg, b0 = blockIdx.y * R;
+    Raw<float, 4> rA, rh[R];
+    Raw<F, 4> rB[R], rC[R];
+    float u[R], dt[R], z[R];
 #pragma unroll
-    for (int k = 0; k < 4; k++) {
-        Bv[k] = n0 + k < a.N ? Elem<F>::ld(pB + n0 + k) : 0.f;
-        Cv[k] = n0 + k < a.N ? Elem<F>::ld(pC + n0 + k) : 0.f;
-    }
-    const float u = Elem<F>::ld((const F *)a.u + (size_t)b * a.u_batch + ch);
-    float dt = Elem<F>::ld((const F *)a.delta + (size_t)b * a.delta_batch + ch) + (a.bias ? a.bias[ch] : 0.f), sig;
-    if (a.softplus) dt = softplus(dt, sig);
-    float y = 0.f;
-#pragma unroll
-    for (int k = 0; k < 4; k++) {
-        h[k] = ex2(dt * (A2[k] * LOG2E)) * h[k] + dt * u * Bv[k];
-        y += Cv[k] * h[k];
-    }
-#pragma unroll
-    for (int m = 1; m < LPC; m <<= 1) y += __shfl_xor_sync(FULL_MASK, y, m);
-    if (!live) return;
-    if (a.state_out) store_states(a.state_out, row, n0, a.N, h);
-    if (q == 0) {
-        if (a.Dskip) y += a.Dskip[ch] * u;
-        if (a.z) {
-            const float z = Elem<F>::ld((const F *)a.z + (size_t)b * a.z_batch + ch);
-            y *= z * sigmoidf(z);
+    for (int r = 0; r < R; r++) {
+        const int b = min(b0 + r, a.B - 1);              // (rows behind the last: read as the last, not written)
+        rh[r].zero();
+        rB[r].zero();
+        rC[r].zero();
+        if (n > 0) {
+            if (a.state_in) rh[r].load(a.state_in + ((size_t)b * a.D + ch) * a.N + n0, a.vec_s, n);
+            rB[r].load((const F *)a.Bm + (size_t)b * a.B_batch + (size_t)grp * a.N + n0, a.vec_b, n);
+            rC[r].load((const F *)a.Cm + (size_t)b * a.C_batch + (size_t)grp * a.N + n0, a.vec_c, n);
         }
-        Elem<F>::st((F *)a.y + (size_t)b * a.D + ch, y);
+        u[r] = Elem<F>::ld((const F *)a.u + (size_t)b * a.u_batch + ch);
+        dt[r] = Elem<F>::ld((const F *)a.delta + (size_t)b * a.delta_batch + ch);
+        z[r] = a.z ? Elem<F>::ld((const F *)a.z + (size_t)b * a.z_batch + ch) : 0.f;
+    }
+    rA.zero();
+    if (n > 0) rA.load(a.A + (size_t)ch * a.N + n0, a.vec_a, n);
+    const float bias = a.bias ? a.bias[ch] : 0.f, dskip = a.Dskip ? a.Dskip[ch] : 0.f;
+    float A[4];
+    rA.get(A);
+#pragma unroll
+    for (int r = 0; r < R; r++) {
+        float h[4], B[4], C[4], y = 0.f, sig, d = dt[r] + bias;
+        if (a.softplus) d = softplus<false>(d, sig);
+        rh[r].get(h);
+        rB[r].get(B);
+        rC[r].get(C);
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            h[k] = ex2(d * (A[k] * LOG2E)) * h[k] + d * u[r] * B[k];
+            y += C[k] * h[k];
+        }
+#pragma unroll
+        for (int m = 1; m < LANES; m <<= 1) y += __shfl_xor_sync(FULL_MASK, y, m);
+        if (live && b0 + r < a.B) {
+            if (a.state_out && n > 0) {
+                rh[r].put(h);
+                rh[r].store(a.state_out + ((size_t)(b0 + r) * a.D + ch) * a.N + n0, a.vec_s, n);
+            }
+            if (n0 == 0) {
+                y += dskip * u[r];
+                if (a.z) y *= z[r] * sigm(z[r]);
+                Elem<F>::st((F *)a.y + (size_t)(b0 + r) * a.D + ch, y);
+            }
+        }
     }
 }
 
 // Backward, summary: what a span sends to the state before it, from zero behind it, and its sum of dt.
-template <typename F, int LPC>
+template <typename F, int LPC, bool FAST>
 __global__ void __launch_bounds__(128) k_scan_bwd_summary(ScanArgs a) {
     pdl_wait();
     pdl_trigger();
     using P = Geo<LPC>;
-    __shared__ __align__(16) float2 s_dt[4][TB][P::CPW];
-    __shared__ __align__(16) float s_b[4][TB * P::NP], s_c[4][TB * P::NP];
+    __shared__ __align__(16) float4 s_dt[4][TB][P::ROW16];              // dt, dy of the first channel, of the second
+    __shared__ __align__(16) float s_c[4][TB * P::NP];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, c = lane / LPC, q = lane % LPC;
-    long long unit = (long long)blockIdx.x * 4 + warp;
-    const int cb = (int)(unit % a.ncb);
-    unit /= a.ncb;
-    const int grp = (int)(unit % a.G);
-    unit /= a.G;
-    const int span = 1 + (int)(unit % (a.nspan - 1)), b = (int)(unit / (a.nspan - 1));       // (nobody asks for the first's)
-    if (b >= a.B) return;
-    const int cg = cb * P::CPW + c, ch = grp * a.Dg + cg, n0 = 4 * q;
-    const bool live = cg < a.Dg;
-    float A2[4], E[4];
-    load_states(live ? a.A : nullptr, (size_t)ch * a.N, n0, a.N, A2);
-#pragma unroll
-    for (int i = 0; i < 4; i++) { A2[i] *= LOG2E; E[i] = 0.f; }
-    const float bias = live && a.bias ? a.bias[ch] : 0.f;
-    const F *pd = (const F *)a.delta + (size_t)b * a.delta_batch + ch;
-    const F *pg = a.gy ? (const F *)a.gy + (size_t)b * a.T * a.D + ch : nullptr;
-    const F *pz = a.z ? (const F *)a.z + (size_t)b * a.z_batch + ch : nullptr;
-    const int blk0 = span * a.span_blocks, blk1 = min(blk0 + a.span_blocks, a.nblk);
-    F rg[P::PT], rd[P::PT], rz[P::PT];
-    BlockBC<F, LPC> bc;
-    auto fetch = [&](int blk) {
-        if (blk < blk0) return;
-#pragma unroll
-        for (int i = 0; i < P::PT; i++) {
-            const int t = blk * TB + q + LPC * i;
-            if (live && t < a.T) {
-                if (pg) rg[i] = pg[(size_t)t * a.D];
-                rd[i] = pd[(size_t)t * a.delta_token];
-                if (pz) rz[i] = pz[(size_t)t * a.z_token];
-            }
-        }
-        bc.load(a, b, grp, blk * TB, a.T, lane);
+    const Unit un(a, (long long)blockIdx.x * 4 + warp, a.nspan - 1);
+    if (un.b >= a.B) return;
+    const int b = un.b, grp = un.grp, span = un.span + 1, cg = un.cb * P::CPW + 2 * c, n0 = 4 * q;      // (nobody asks for the first span's)
+    const bool live = cg < a.Dg, live2 = cg + 1 < a.Dg;
+    const int ch = grp * a.Dg + (live ? cg : 0), second = live2 ? 1 : 0;
+    f2 A2[2][2], E[2][2];
+    load_decays(a.A, (size_t)ch * a.N, n0, a.N, A2[0]);
+    load_decays(a.A, (size_t)(ch + second) * a.N, n0, a.N, A2[1]);
+    E[0][0] = E[0][1] = E[1][0] = E[1][1] = both(0.f);
+    const f2 bias = a.bias ? make_float2(a.bias[ch], a.bias[ch + second]) : both(0.f);
+    const int blk0 = span * a.span_blocks, blk1 = min(blk0 + a.span_blocks, a.nblk), t0 = (blk1 - 1) * TB;
+    const int sd = (int)a.delta_token, sz = (int)a.z_token, sC = (int)a.C_token;
+    const F *pd = (const F *)a.delta + (size_t)b * a.delta_batch + (size_t)t0 * a.delta_token + ch;
+    const F *pz = (const F *)a.z + (size_t)b * a.z_batch + (size_t)t0 * a.z_token + ch;
+    const F *pg = (const F *)a.gy + ((size_t)b * a.T + t0) * a.D + ch;
+    const F *pC = (const F *)a.Cm + (size_t)b * a.C_batch + (size_t)t0 * a.C_token + (size_t)grp * a.N;
+    Own<F, LPC, FAST> rd, rz, rg;
+    BlockRows<F, LPC, FAST> rC;
+    int last = a.T - 1 - t0;
+    auto fetch = [&]() {
+        rd.load(pd, sd, q, last, second);
+        if (a.gy) rg.load(pg, a.D, q, last, second);
+        if (a.z) rz.load(pz, sz, q, last, second);
+        rC.load(pC, sC, a.vec_c, a.N, last, lane);
+        pd -= (long long)sd * TB; pz -= (long long)sz * TB; pg -= (long long)a.D * TB; pC -= (long long)sC * TB;
     };
-    fetch(blk1 - 1);
-    float total = 0.f;
+    fetch();
+    f2 total = both(0.f);
     for (int blk = blk1 - 1; blk >= blk0; blk--) {
         __syncwarp();
+        f2 step[P::PT], g[P::PT];
 #pragma unroll
         for (int i = 0; i < P::PT; i++) {
-            const int t = q + LPC * i;
-            float dt = 0.f, dy = 0.f;
-            if (live && blk * TB + t < a.T) {
-                if (pg) dy = Elem<F>::ld(&rg[i]);
-                dt = Elem<F>::ld(&rd[i]) + bias;
-                float sig;
-                if (a.softplus) dt = softplus(dt, sig);
-                if (pz) {
-                    const float z = Elem<F>::ld(&rz[i]);
-                    dy *= z * sigmoidf(z);
-                }
-            }
-            s_dt[warp][t][c] = make_float2(dt, dy);
-            total += dt;
+            step[i] = add2(rd.get(i), bias);
+            g[i] = a.gy ? rg.get(i) : both(0.f);
         }
-        bc.put(s_b[warp], s_c[warp], lane);
+        if (a.softplus) softplus_all<false>(step, step);
+        if (a.z) {
+#pragma unroll
+            for (int i = 0; i < P::PT; i++) {
+                const f2 z = rz.get(i);
+                g[i] = mul2(g[i], make_float2(z.x * sigm(z.x), z.y * sigm(z.y)));
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < P::PT; i++) {
+            f2 dt = step[i], dy = g[i];
+            if (q + LPC * i > last) dt = dy = both(0.f);
+            s_dt[warp][q + LPC * i][c] = make_float4(dt.x, dy.x, dt.y, dy.y);
+            total = add2(total, dt);
+        }
+        rC.put(s_c[warp], lane);
         __syncwarp();
-        fetch(blk - 1);
+        last += TB;
+        if (blk > blk0) fetch();
 #pragma unroll
         for (int t = TB - 1; t >= 0; t--) {
-            const float2 d = s_dt[warp][t][c];
-            const float4 Cv = *reinterpret_cast<const float4 *>(&s_c[warp][t * P::NP + n0]);
-            E[0] = ex2(d.x * A2[0]) * (Cv.x * d.y + E[0]);
-            E[1] = ex2(d.x * A2[1]) * (Cv.y * d.y + E[1]);
-            E[2] = ex2(d.x * A2[2]) * (Cv.z * d.y + E[2]);
-            E[3] = ex2(d.x * A2[3]) * (Cv.w * d.y + E[3]);
+            const float4 d = s_dt[warp][t][c];
+            f2 C[2];
+            pairs_at(&s_c[warp][t * P::NP + n0], C[0], C[1]);
+#pragma unroll
+            for (int m = 0; m < 2; m++) {
+                E[0][m] = mul2(ex2(mul2(both(d.x), A2[0][m])), fma2(C[m], both(d.y), E[0][m]));
+                E[1][m] = mul2(ex2(mul2(both(d.z), A2[1][m])), fma2(C[m], both(d.w), E[1][m]));
+            }
         }
     }
 #pragma unroll
-    for (int m = 1; m < LPC; m <<= 1) total += __shfl_xor_sync(FULL_MASK, total, m);
+    for (int m = 1; m < LPC; m <<= 1)
+        total = add2(total, make_float2(__shfl_xor_sync(FULL_MASK, total.x, m), __shfl_xor_sync(FULL_MASK, total.y, m)));
     const size_t at = ((size_t)b * a.nspan + span) * a.D + ch;
-    if (live) store_states(a.span_state, at * a.N, n0, a.N, E);
-    if (live && q == 0) a.span_dt[at] = total;
+    if (live) {
+        store_states(a.span_state, at * a.N, n0, a.N, E[0]);
+        if (q == 0) a.span_dt[at] = total.x;
+    }
+    if (live2) {
+        store_states(a.span_state, (at + 1) * a.N, n0, a.N, E[1]);
+        if (q == 0) a.span_dt[at + 1] = total.y;
+    }
 }
 
-// Backward.  The warps of a CTA hold neighbouring channels of one group and one span; they meet once a block to add up what
-// they have for gB and gC.
-template <int LPC>
+// Backward.  The warps of a CTA hold neighbouring channels of one group and one span.  They share the rows of B and C, and
+// once a block add up what they have for gB and gC; one barrier a block serves both (two buffers of each).
+//
+// A block is run forward once more from the state the forward pass left, which leaves the states before its quarters in
+// shared memory; then quarter by quarter from the last, forward again with decays and states in registers and back.
+//
+// gB and gC are sums over the channels: a thread adds up its two, then eight values a lane and token are exchanged.  Each
+// exchange halves the values: lanes 16 apart hold their two pairs of states in opposite order, so that the first one needs
+// no selects.
+template <typename F, int LPC>
 struct BwdGeo {
-    static constexpr int WARPS = LPC >= 8 ? 4 : 8;
+    static constexpr int WARPS = 4;
     static constexpr int CH = WARPS * Geo<LPC>::CPW;             // channels of a CTA
     static constexpr int VALUES = 8 * LPC;                       // gB and gC of a token: [8][LPC], state 4 q + (i & 3)
+    static constexpr int RUNS = TB * LPC;                        // runs of four of a block's rows of B (or C)
     struct Warp {
-        float4 d[TB][Geo<LPC>::CPW];                             // dt, dt u, dy, -
-        float b[TB * Geo<LPC>::NP], c[TB * Geo<LPC>::NP];
+        float4 d[TB][Geo<LPC>::ROW16];                              // dt, dt u of the first channel, of the second
+        float4 own[2][TB][Geo<LPC>::ROW16];                         // u, sigmoid(delta + bias), z, gy
+        float4 res[TB][Geo<LPC>::ROW16];                            // sums over the states: G . B of the two channels, G A a h of the two
+        float2 res_y[TB][Geo<LPC>::ROW8];                          // C . h
+        float4 state[2][4][32];                                  // before tokens 0, 4, 8, 12
+        float4 ckpt[2][32];                                      // the next block's: states before it; u, delta, z, gy
+        Raw<F, 2> in[4][TB][Geo<LPC>::CL];
+        float2 dy[TB][Geo<LPC>::ROW8];                             // of the two channels
         float sum[2][TB * VALUES];
     };
-    static constexpr int SMEM = WARPS * (int)sizeof(Warp);
+    struct Cta {
+        float4 b[2][2][RUNS], c[2][2][RUNS];                     // [buffer][as it is, pairs swapped]
+        Warp w[WARPS];
+    };
+    static constexpr int SMEM = (int)sizeof(Cta);
 };
 
-// the eight values of a lane summed over the warp's channels: what is left, `first` on, is given to put(i, value)
+// sizeof(R) bytes (4, 8 or 16) into shared memory without passing through registers; to be waited for by the same thread
+template <typename R>
+__device__ __forceinline__ void copy_async(R *to, const void *from) {
+    const uint32_t dst = (uint32_t)__cvta_generic_to_shared(to);
+    if constexpr (sizeof(R) == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(from) : "memory");
+    else asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(dst), "l"(from), "n"(sizeof(R)) : "memory");
+}
+__device__ __forceinline__ void copies_done() { asm volatile("cp.async.wait_all;" ::: "memory"); }
+
+// a lane's values for gB (vb) and gC (vc) summed over the warp's channels: put(kind, state & 3, sum) for each that is left
 template <int LPC, class Put>
-__device__ __forceinline__ void sum_channels(float (&v)[8], int lane, Put put) {
-    int first = 0;
-    int left = 8;
-#pragma unroll
-    for (int m = 16, k = 4; m >= LPC; m >>= 1, k >>= 1) {
-        if (k >= 1) {
-            const bool up = lane & m;
-#pragma unroll
-            for (int j = 0; j < 4; j++) {
-                if (j < k) {
-                    const float send = up ? v[j] : v[j + k], keep = up ? v[j + k] : v[j];
-                    v[j] = keep + __shfl_xor_sync(FULL_MASK, send, m);
-                }
-            }
-            first += up ? k : 0;
-            left = k;
-        } else {
-            v[0] += __shfl_xor_sync(FULL_MASK, v[0], m);
-        }
+__device__ __forceinline__ void sum_channels(f2 (&vb)[2], f2 (&vc)[2], int lane, Put put) {
+    const int hi = lane & 16 ? 2 : 0;
+    f2 b = add2(vb[0], make_float2(__shfl_xor_sync(FULL_MASK, vb[1].x, 16), __shfl_xor_sync(FULL_MASK, vb[1].y, 16)));
+    f2 c = add2(vc[0], make_float2(__shfl_xor_sync(FULL_MASK, vc[1].x, 16), __shfl_xor_sync(FULL_MASK, vc[1].y, 16)));
+    if (LPC == 16) {
+        put(0, hi, b.x); put(0, hi + 1, b.y);
+        put(1, hi, c.x); put(1, hi + 1, c.y);
+        return;
     }
+    const bool up8 = lane & 8;
+    const int n = hi + (up8 ? 1 : 0);
+    const float sb = (up8 ? b.y : b.x) + __shfl_xor_sync(FULL_MASK, up8 ? b.x : b.y, 8);
+    const float sc = (up8 ? c.y : c.x) + __shfl_xor_sync(FULL_MASK, up8 ? c.x : c.y, 8);
+    if (LPC == 8) {
+        put(0, n, sb);
+        put(1, n, sc);
+        return;
+    }
+    const bool up4 = lane & 4;
+    float s = (up4 ? sc : sb) + __shfl_xor_sync(FULL_MASK, up4 ? sb : sc, 4);
 #pragma unroll
-    for (int j = 0; j < 8; j++)
-        if (j < left) put(first + j, v[j]);
+    for (int m = 2; m >= LPC; m >>= 1) s += __shfl_xor_sync(FULL_MASK, s, m);
+    put(up4 ? 1 : 0, n, s);
 }
 
-template <typename F, int LPC>
-__global__ void __launch_bounds__(32 * BwdGeo<LPC>::WARPS) k_scan_bwd(ScanArgs a) {
+template <typename F, int LPC, bool FAST>
+__global__ void __launch_bounds__(32 * BwdGeo<F, LPC>::WARPS, 2) k_scan_bwd(ScanArgs a) {
     pdl_wait();
     pdl_trigger();
     using P = Geo<LPC>;
-    using Q = BwdGeo<LPC>;
-    constexpr int HALF = TB / 2, NB = LPC < 8 ? LPC : 8;
+    using Q = BwdGeo<F, LPC>;
+    constexpr int QT = 4, NB = LPC < QT ? LPC : QT, THREADS = 32 * Q::WARPS, RL = (2 * Q::RUNS + THREADS - 1) / THREADS;
     extern __shared__ __align__(16) char smem_raw[];
-    typename Q::Warp *all = reinterpret_cast<typename Q::Warp *>(smem_raw);
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, c = lane / LPC, q = lane % LPC;
-    typename Q::Warp &my = all[warp];
-    long long unit = blockIdx.x;
-    const int cb = (int)(unit % a.ncb);
-    unit /= a.ncb;
-    const int grp = (int)(unit % a.G);
-    unit /= a.G;
-    const int span = (int)(unit % a.nspan), b = (int)(unit / a.nspan);
-    const int cg = cb * Q::CH + warp * P::CPW + c, ch = grp * a.Dg + cg, n0 = 4 * q;
-    const bool live = cg < a.Dg;
+    typename Q::Cta &cta = *reinterpret_cast<typename Q::Cta *>(smem_raw);
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, c = lane / LPC, q = lane % LPC;
+    typename Q::Warp &my = cta.w[warp];
+    const Unit un(a, blockIdx.x, a.nspan);
+    const int b = un.b, grp = un.grp, span = un.span, cg = un.cb * Q::CH + warp * P::CPW + 2 * c, n0 = 4 * q;
+    const bool live = cg < a.Dg, live2 = cg + 1 < a.Dg, swap = lane & 16;
+    const int ch = grp * a.Dg + (live ? cg : 0), second = live2 ? 1 : 0;
     const size_t row = ((size_t)b * a.D + ch) * a.N;
-    float A2[4], E[4], gA[4];
-    load_states(live ? a.A : nullptr, (size_t)ch * a.N, n0, a.N, A2);
-    load_states(live ? a.gs_out : nullptr, row, n0, a.N, E);
-#pragma unroll
-    for (int i = 0; i < 4; i++) { A2[i] *= LOG2E; gA[i] = 0.f; }
+    f2 A2[2][2], E[2][2], gA[2][2];
+    load_decays(a.A, (size_t)ch * a.N, n0, a.N, A2[0], swap);
+    load_decays(a.A, (size_t)(ch + second) * a.N, n0, a.N, A2[1], swap);
+    load_states(live ? a.gs_out : nullptr, row, n0, a.N, E[0], swap);
+    load_states(live2 ? a.gs_out : nullptr, row + a.N, n0, a.N, E[1], swap);
+    gA[0][0] = gA[0][1] = gA[1][0] = gA[1][1] = both(0.f);
     for (int j = a.nspan - 1; j > span; j--) {
         const size_t at = ((size_t)b * a.nspan + j) * a.D + ch;
-        float V[4];
-        load_states(live ? a.span_state : nullptr, at * a.N, n0, a.N, V);
-        const float s = live ? a.span_dt[at] : 0.f;
 #pragma unroll
-        for (int i = 0; i < 4; i++) E[i] = ex2(A2[i] * s) * E[i] + V[i];
+        for (int k = 0; k < 2; k++) {
+            f2 V[2];
+            load_states((k ? live2 : live) ? a.span_state : nullptr, (at + k) * a.N, n0, a.N, V, swap);
+            const f2 s = both(a.span_dt[at + k * second]);
+#pragma unroll
+            for (int i = 0; i < 2; i++) E[k][i] = fma2(ex2(mul2(A2[k][i], s)), E[k][i], V[i]);
+        }
     }
-    const float bias = live && a.bias ? a.bias[ch] : 0.f, dskip = live && a.Dskip ? a.Dskip[ch] : 0.f;
-    float gD = 0.f, gbias = 0.f;
-    const int blk0 = span * a.span_blocks, blk1 = min(blk0 + a.span_blocks, a.nblk);
-    const F *pu = (const F *)a.u + (size_t)b * a.u_batch + ch, *pd = (const F *)a.delta + (size_t)b * a.delta_batch + ch;
-    const F *pz = a.z ? (const F *)a.z + (size_t)b * a.z_batch + ch : nullptr;
-    const F *pg = a.gy ? (const F *)a.gy + (size_t)b * a.T * a.D + ch : nullptr;
+    const f2 bias = a.bias ? make_float2(a.bias[ch], a.bias[ch + second]) : both(0.f);
+    const f2 dskip = a.Dskip ? make_float2(a.Dskip[ch], a.Dskip[ch + second]) : both(0.f);
+    f2 gD = both(0.f), gbias = both(0.f);
+    const int blk0 = span * a.span_blocks, blk1 = min(blk0 + a.span_blocks, a.nblk), t0 = (blk1 - 1) * TB;
+    const int su = (int)a.u_token, sd = (int)a.delta_token, sz = (int)a.z_token;
+    const F *pu = (const F *)a.u + (size_t)b * a.u_batch + (size_t)t0 * a.u_token + ch;
+    const F *pd = (const F *)a.delta + (size_t)b * a.delta_batch + (size_t)t0 * a.delta_token + ch;
+    const F *pz = (const F *)a.z + (size_t)b * a.z_batch + (size_t)t0 * a.z_token + ch;
+    const F *pg = (const F *)a.gy + ((size_t)b * a.T + t0) * a.D + ch;
+    const float *ck = a.ckpt + (((size_t)b * a.nblk + (blk1 - 1)) * a.D + ch) * a.N;
+    size_t out = ((size_t)b * a.T + t0 + q) * a.D + ch;           // of gu, gdelta, gz
 
-    F ru[P::PT], rd[P::PT], rz[P::PT], rg[P::PT];
-    float rh[4];
-    BlockBC<F, LPC> bc;
-    auto fetch = [&](int blk) {
-        if (blk < blk0) return;
+    // the CTA's threads bring in a block's rows of B (the first RUNS items) and of C
+    Raw<F, 4> rbc[RL];
+    auto fetch_rows = [&](int blk, int last) {
 #pragma unroll
-        for (int i = 0; i < P::PT; i++) {
-            const int t = blk * TB + q + LPC * i;
-            if (live && t < a.T) {
-                ru[i] = pu[(size_t)t * a.u_token];
-                rd[i] = pd[(size_t)t * a.delta_token];
-                if (pz) rz[i] = pz[(size_t)t * a.z_token];
-                if (pg) rg[i] = pg[(size_t)t * a.D];
-            }
+        for (int k = 0; k < RL; k++) {
+            const int i = tid + k * THREADS, run = i % Q::RUNS, m0 = 4 * (run % LPC), n = min(4, a.N - m0);
+            const bool isC = i >= Q::RUNS;
+            const long long token = isC ? a.C_token : a.B_token;
+            const F *p = isC ? (const F *)a.Cm + (size_t)b * a.C_batch : (const F *)a.Bm + (size_t)b * a.B_batch;
+            rbc[k].zero();
+            if (i < 2 * Q::RUNS && n > 0 && run / LPC <= last)
+                rbc[k].load(p + (long long)(blk * TB + run / LPC) * token + (size_t)grp * a.N + m0, FAST || (isC ? a.vec_c : a.vec_b), n);
         }
-        load_states(live ? a.ckpt : nullptr, (((size_t)b * a.nblk + blk) * a.D + ch) * a.N, n0, a.N, rh);
-        bc.load(a, b, grp, blk * TB, a.T, lane);
     };
-    fetch(blk1 - 1);
-    for (int blk = blk1 - 1; blk >= blk0; blk--) {
-        const int buf = blk & 1;
-        float u[P::PT], sg[P::PT], z[P::PT], g[P::PT], h0[4], mid[4];
+    auto put_rows = [&](int buf) {
 #pragma unroll
-        for (int i = 0; i < 4; i++) { h0[i] = rh[i]; mid[i] = rh[i]; }
-        __syncwarp();
+        for (int k = 0; k < RL; k++) {
+            const int i = tid + k * THREADS, run = i % Q::RUNS;
+            float f[4];
+            rbc[k].get(f);
+            if (i < 2 * Q::RUNS) {
+                float4(&to)[2][Q::RUNS] = i >= Q::RUNS ? cta.c[buf] : cta.b[buf];
+                to[0][run] = make_float4(f[0], f[1], f[2], f[3]);
+                to[1][run] = make_float4(f[2], f[3], f[0], f[1]);
+            }
+        }
+    };
+    int last = a.T - 1 - t0;
+    // a lane's own tokens of the next block, and the states before it
+    auto own_tokens = [&](Raw<F, 2>(&to)[TB][P::CL], const F *block, int token_stride) {
 #pragma unroll
         for (int i = 0; i < P::PT; i++) {
-            const int t = q + LPC * i;
-            float dt = 0.f, dy = 0.f;
-            u[i] = 0.f; sg[i] = 0.f; z[i] = 0.f; g[i] = 0.f;
-            if (live && blk * TB + t < a.T) {
-                u[i] = Elem<F>::ld(&ru[i]);
-                dt = Elem<F>::ld(&rd[i]) + bias;
-                sg[i] = 1.f;
-                if (a.softplus) dt = softplus(dt, sg[i]);
-                if (pg) g[i] = Elem<F>::ld(&rg[i]);
-                dy = g[i];
-                if (pz) {
-                    z[i] = Elem<F>::ld(&rz[i]);
-                    dy *= z[i] * sigmoidf(z[i]);
-                }
+            const F *p = block + (long long)min(q + LPC * i, last) * token_stride;
+            if (FAST) {
+                copy_async(&to[q + LPC * i][c], p);
+            } else {
+                F *t = reinterpret_cast<F *>(&to[q + LPC * i][c]);
+                t[0] = p[0];
+                t[1] = p[second];
             }
-            my.d[t][c] = make_float4(dt, dt * u[i], dy, 0.f);
         }
-        bc.put(my.b, my.c, lane);
-        __syncwarp();
-        fetch(blk - 1);
-        // the state before token HALF
+    };
+    auto fetch = [&]() {
+        own_tokens(my.in[0], pu, su);
+        own_tokens(my.in[1], pd, sd);
+        if (a.z) own_tokens(my.in[2], pz, sz);
+        if (a.gy) own_tokens(my.in[3], pg, a.D);
 #pragma unroll
-        for (int t = 0; t < HALF; t++) {
-            const float4 d = my.d[t][c], Bv = *reinterpret_cast<const float4 *>(&my.b[t * P::NP + n0]);
-            mid[0] = ex2(d.x * A2[0]) * mid[0] + d.y * Bv.x;
-            mid[1] = ex2(d.x * A2[1]) * mid[1] + d.y * Bv.y;
-            mid[2] = ex2(d.x * A2[2]) * mid[2] + d.y * Bv.z;
-            mid[3] = ex2(d.x * A2[3]) * mid[3] + d.y * Bv.w;
+        for (int k = 0; k < 2; k++) {
+            if (FAST) {
+                if (n0 < a.N) copy_async(&my.ckpt[k][lane], ck + k * second * a.N + n0);
+            } else {
+                f2 v[2];
+                load_states(ck, (size_t)(k * second) * a.N, n0, a.N, v);
+                my.ckpt[k][lane] = make_float4(v[0].x, v[0].y, v[1].x, v[1].y);
+            }
+        }
+        pu -= (long long)su * TB; pd -= (long long)sd * TB; pz -= (long long)sz * TB; pg -= (long long)a.D * TB;
+        ck -= (size_t)a.D * a.N;
+    };
+#pragma unroll
+    for (int k = 0; k < 2; k++)
+        if (n0 >= a.N) my.ckpt[k][lane] = make_float4(0.f, 0.f, 0.f, 0.f);       // (lanes of padded states: nothing is copied there)
+    fetch();
+    fetch_rows(blk1 - 1, last);
+    put_rows((blk1 - 1) & 1);
+    __syncthreads();
+    for (int blk = blk1 - 1; blk >= blk0; blk--) {
+        const int buf = blk & 1, end = last;
+        const float4 *sB = cta.b[buf][swap ? 1 : 0] + q, *sC = cta.c[buf][swap ? 1 : 0] + q;
+        if (FAST) copies_done();
+        f2 x[2][2];
+#pragma unroll
+        for (int k = 0; k < 2; k++) {
+            const float4 v = my.ckpt[k][lane];
+            const f2 v0 = make_float2(v.x, v.y), v1 = make_float2(v.z, v.w);
+            x[k][0] = (k ? live2 : live) ? (swap ? v1 : v0) : both(0.f);
+            x[k][1] = (k ? live2 : live) ? (swap ? v0 : v1) : both(0.f);
+            my.state[k][0][lane] = make_float4(x[k][0].x, x[k][0].y, x[k][1].x, x[k][1].y);
+        }
+        __syncwarp();
+        {
+            f2 dt[P::PT], sig[P::PT], dy[P::PT], z[P::PT];
+#pragma unroll
+            for (int i = 0; i < P::PT; i++) {
+                const int t = q + LPC * i;
+                dt[i] = add2(pair_of(my.in[1][t][c]), bias);
+                sig[i] = both(1.f);
+                dy[i] = a.gy ? pair_of(my.in[3][t][c]) : both(0.f);
+                z[i] = a.z ? pair_of(my.in[2][t][c]) : both(0.f);
+            }
+            if (a.softplus) softplus_all<true>(dt, sig);
+#pragma unroll
+            for (int i = 0; i < P::PT; i++) {
+                const int t = q + LPC * i;
+                f2 u = pair_of(my.in[0][t][c]);
+                const f2 g = dy[i];
+                if (a.z) dy[i] = mul2(g, make_float2(z[i].x * sigm(z[i].x), z[i].y * sigm(z[i].y)));
+                if (!live || t > end) dt[i].x = dy[i].x = u.x = 0.f;
+                if (!live2 || t > end) dt[i].y = dy[i].y = u.y = 0.f;
+                my.d[t][c] = make_float4(dt[i].x, dt[i].x * u.x, dt[i].y, dt[i].y * u.y);
+                my.dy[t][c] = dy[i];
+                my.own[0][t][c] = make_float4(u.x, sig[i].x, z[i].x, g.x);
+                my.own[1][t][c] = make_float4(u.y, sig[i].y, z[i].y, g.y);
+            }
+        }
+        __syncwarp();
+        last += TB;
+        if (blk > blk0) {
+            fetch();
+            fetch_rows(blk - 1, TB - 1);
+        }
+        // the states before the quarters
+#pragma unroll
+        for (int g = 0; g < TB / QT - 1; g++) {
+            f2 dec[QT][2][2], in[QT][2][2];
+#pragma unroll
+            for (int t = 0; t < QT; t++) {
+                const float4 d = my.d[g * QT + t][c];
+                f2 B[2];
+                pairs_at(&sB[(g * QT + t) * LPC].x, B[0], B[1]);
+#pragma unroll
+                for (int k = 0; k < 2; k++)
+#pragma unroll
+                    for (int m = 0; m < 2; m++) {
+                        dec[t][k][m] = mul2(both(k ? d.z : d.x), A2[k][m]);
+                        in[t][k][m] = mul2(both(k ? d.w : d.y), B[m]);
+                    }
+            }
+#pragma unroll
+            for (int t = 0; t < QT; t++)
+#pragma unroll
+                for (int k = 0; k < 2; k++)
+#pragma unroll
+                    for (int m = 0; m < 2; m++) dec[t][k][m] = ex2(dec[t][k][m]);
+#pragma unroll
+            for (int t = 0; t < QT; t++)
+#pragma unroll
+                for (int k = 0; k < 2; k++)
+#pragma unroll
+                    for (int m = 0; m < 2; m++) x[k][m] = fma2(dec[t][k][m], x[k][m], in[t][k][m]);
+            my.state[0][g + 1][lane] = make_float4(x[0][0].x, x[0][0].y, x[0][1].x, x[0][1].y);
+            my.state[1][g + 1][lane] = make_float4(x[1][0].x, x[1][0].y, x[1][1].x, x[1][1].y);
         }
 #pragma unroll 1
-        for (int half = 1; half >= 0; half--) {
-            const int tb = half * HALF;
-            float dec[HALF][4], h[HALF + 1][4];          // a_t; the state before token t
+        for (int quarter = TB / QT - 1; quarter >= 0; quarter--) {
+            const int tb = quarter * QT;
+            f2 G[QT][2][2], ah[QT][2][2], h[QT][2][2];             // [token][channel][pair]: a_t, later G_t; a_t h_{t-1}; h_t
+            {
+                f2 x0[2][2];
 #pragma unroll
-            for (int i = 0; i < 4; i++) h[0][i] = half ? mid[i] : h0[i];
+                for (int k = 0; k < 2; k++) pairs_at(&my.state[k][quarter][lane].x, x0[k][0], x0[k][1]);
+                f2 in[QT][2][2];
 #pragma unroll
-            for (int t = 0; t < HALF; t++) {
-                const float4 d = my.d[tb + t][c], Bv = *reinterpret_cast<const float4 *>(&my.b[(tb + t) * P::NP + n0]);
-                const float Bf[4] = {Bv.x, Bv.y, Bv.z, Bv.w};
+                for (int t = 0; t < QT; t++) {
+                    const float4 d = my.d[tb + t][c];
+                    f2 B[2];
+                    pairs_at(&sB[(tb + t) * LPC].x, B[0], B[1]);
 #pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    dec[t][i] = ex2(d.x * A2[i]);
-                    h[t + 1][i] = dec[t][i] * h[t][i] + d.y * Bf[i];
+                    for (int k = 0; k < 2; k++)
+#pragma unroll
+                        for (int m = 0; m < 2; m++) {
+                            G[t][k][m] = mul2(both(k ? d.z : d.x), A2[k][m]);
+                            in[t][k][m] = mul2(both(k ? d.w : d.y), B[m]);
+                        }
                 }
+#pragma unroll
+                for (int t = 0; t < QT; t++)
+#pragma unroll
+                    for (int k = 0; k < 2; k++)
+#pragma unroll
+                        for (int m = 0; m < 2; m++) G[t][k][m] = ex2(G[t][k][m]);
+#pragma unroll
+                for (int t = 0; t < QT; t++)
+#pragma unroll
+                    for (int k = 0; k < 2; k++)
+#pragma unroll
+                        for (int m = 0; m < 2; m++) {
+                            ah[t][k][m] = mul2(G[t][k][m], t ? h[t - 1][k][m] : x0[k][m]);
+                            h[t][k][m] = add2(ah[t][k][m], in[t][k][m]);
+                        }
             }
 #pragma unroll
-            for (int nb = HALF / NB - 1; nb >= 0; nb--) {
-                float gin[NB], gdec[NB], yv[NB];
+            for (int t = QT - 1; t >= 0; t--) {
+                const float2 dy = my.dy[tb + t][c];
+                f2 C[2];
+                pairs_at(&sC[(tb + t) * LPC].x, C[0], C[1]);
+#pragma unroll
+                for (int k = 0; k < 2; k++)
+#pragma unroll
+                    for (int m = 0; m < 2; m++) {
+                        const f2 g = fma2(C[m], both(k ? dy.y : dy.x), E[k][m]);
+                        E[k][m] = mul2(G[t][k][m], g);
+                        G[t][k][m] = g;
+                    }
+            }
+#pragma unroll
+            for (int nb = QT / NB - 1; nb >= 0; nb--) {
+                float gin[2][NB], gdec[2][NB], yv[2][NB];
 #pragma unroll
                 for (int j = NB - 1; j >= 0; j--) {
                     const int t = nb * NB + j;
-                    const float4 d = my.d[tb + t][c], Bv = *reinterpret_cast<const float4 *>(&my.b[(tb + t) * P::NP + n0]),
-                                 Cv = *reinterpret_cast<const float4 *>(&my.c[(tb + t) * P::NP + n0]);
-                    const float Bf[4] = {Bv.x, Bv.y, Bv.z, Bv.w}, Cf[4] = {Cv.x, Cv.y, Cv.z, Cv.w};
-                    float v[8], s0 = 0.f, s1 = 0.f, s2 = 0.f;
+                    const float4 d = my.d[tb + t][c];
+                    const float2 dy = my.dy[tb + t][c];
+                    f2 B[2], C[2], vb[2], vc[2];
+                    pairs_at(&sB[(tb + t) * LPC].x, B[0], B[1]);
+                    pairs_at(&sC[(tb + t) * LPC].x, C[0], C[1]);
 #pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        const float G = Cf[i] * d.z + E[i], ga = G * (dec[t][i] * h[t][i]);
-                        v[i] = G * d.y;
-                        v[4 + i] = h[t + 1][i] * d.z;
-                        s0 += G * Bf[i];
-                        s1 += ga * A2[i];
-                        s2 += Cf[i] * h[t + 1][i];
-                        gA[i] += ga * d.x;
-                        E[i] = dec[t][i] * G;
+                    for (int k = 0; k < 2; k++) {
+                        const f2 dt = both(k ? d.z : d.x), du = both(k ? d.w : d.y), g = both(k ? dy.y : dy.x);
+                        f2 s0, s1, s2;
+#pragma unroll
+                        for (int m = 0; m < 2; m++) {
+                            const f2 ga = mul2(G[t][k][m], ah[t][k][m]);
+                            vb[m] = k ? fma2(G[t][k][m], du, vb[m]) : mul2(G[t][k][m], du);
+                            vc[m] = k ? fma2(h[t][k][m], g, vc[m]) : mul2(h[t][k][m], g);
+                            s0 = m ? fma2(G[t][k][m], B[m], s0) : mul2(G[t][k][m], B[m]);
+                            s1 = m ? fma2(ga, A2[k][m], s1) : mul2(ga, A2[k][m]);
+                            s2 = m ? fma2(C[m], h[t][k][m], s2) : mul2(C[m], h[t][k][m]);
+                            gA[k][m] = fma2(ga, dt, gA[k][m]);
+                        }
+                        gin[k][j] = s0.x + s0.y; gdec[k][j] = s1.x + s1.y; yv[k][j] = s2.x + s2.y;
                     }
-                    gin[j] = s0; gdec[j] = s1; yv[j] = s2;
-                    float *out = &my.sum[buf][(tb + t) * Q::VALUES + q];
-                    sum_channels<LPC>(v, lane, [&](int i, float x) { out[i * LPC] = x; });
+                    float *to = &my.sum[buf][(tb + t) * Q::VALUES + q];
+                    sum_channels<LPC>(vb, vc, lane, [&](int kind, int n, float v) { to[(4 * kind + n) * LPC] = v; });
                 }
-                const float gi = sum_tokens<LPC, NB>(gin, q), gd = sum_tokens<LPC, NB>(gdec, q) * LN2, y0 = sum_tokens<LPC, NB>(yv, q);
-                // the lane's own token: NB < LPC when a channel has more lanes than a half has tokens
+                const f2 gi = make_float2(sum_tokens<LPC, NB>(gin[0], q), sum_tokens<LPC, NB>(gin[1], q));
+                const f2 gd = make_float2(sum_tokens<LPC, NB>(gdec[0], q), sum_tokens<LPC, NB>(gdec[1], q));
+                const f2 y0 = make_float2(sum_tokens<LPC, NB>(yv[0], q), sum_tokens<LPC, NB>(yv[1], q));
+                // (of channels with more lanes than a batch has tokens several hold the same)
                 const int t = tb + nb * NB + q % NB;
-                if (t % LPC == q && live && blk * TB + t < a.T) {
-                    constexpr int P2 = P::PT > 1 ? P::PT / 2 : 0;
-                    const int lo = P::PT > 1 ? nb : 0;
-                    const float uu = half ? u[P2 + lo] : u[lo], sv = half ? sg[P2 + lo] : sg[lo], zz = half ? z[P2 + lo] : z[lo],
-                                gg = half ? g[P2 + lo] : g[lo];
-                    const float4 d = my.d[t][c];
-                    const float graw = (uu * gi + gd) * sv;
-                    gD += d.z * uu;
-                    gbias += graw;
-                    const size_t at = ((size_t)b * a.T + blk * TB + t) * a.D + ch;
-                    if (a.gu) Elem<F>::st((F *)a.gu + at, d.x * gi + dskip * d.z);
-                    if (a.gdelta) Elem<F>::st((F *)a.gdelta + at, graw);
-                    if (a.gz) {
-                        const float s = sigmoidf(zz);
-                        Elem<F>::st((F *)a.gz + at, gg * (y0 + dskip * uu) * (s * (1.f + zz * (1.f - s))));
-                    }
+                my.res[t][c] = make_float4(gi.x, gi.y, gd.x, gd.y);
+                my.res_y[t][c] = y0;
+            }
+        }
+        __syncwarp();
+        // the lane's own tokens
+#pragma unroll
+        for (int i = 0; i < P::PT; i++) {
+            const int t = q + LPC * i;
+            const float4 o0 = my.own[0][t][c], o1 = my.own[1][t][c], d = my.d[t][c], r = my.res[t][c];
+            const f2 dy = my.dy[t][c], u = make_float2(o0.x, o1.x), gi = make_float2(r.x, r.y), gd = make_float2(r.z, r.w);
+            const f2 graw = mul2(fma2(u, gi, mul2(gd, both(LN2))), make_float2(o0.y, o1.y));
+            if (live && t <= end) {
+                gD = fma2(dy, u, gD);
+                gbias = add2(gbias, graw);
+                const size_t at = out + (size_t)(LPC * i) * a.D;
+                if (a.gu) store_pair<FAST>((F *)a.gu + at, live2, fma2(make_float2(d.x, d.z), gi, mul2(dskip, dy)));
+                if (a.gdelta) store_pair<FAST>((F *)a.gdelta + at, live2, graw);
+                if (a.gz) {
+                    const float sx = sigm(o0.z), sy = sigm(o1.z);
+                    const f2 dz = make_float2(sx * (1.f + o0.z * (1.f - sx)), sy * (1.f + o1.z * (1.f - sy)));
+                    store_pair<FAST>((F *)a.gz + at, live2, mul2(mul2(make_float2(o0.w, o1.w), fma2(dskip, u, my.res_y[t][c])), dz));
                 }
             }
         }
+        out -= (size_t)TB * a.D;
+        if (blk > blk0) put_rows(buf ^ 1);
+        __syncthreads();
         if (a.part_bc) {
-            // (two buffers: a warp that is a block ahead writes the other one)
-            __syncthreads();
-            for (int e = threadIdx.x; e < TB * Q::VALUES; e += 32 * Q::WARPS) {
-                const int t = blk * TB + e / Q::VALUES;
-                float s = all[0].sum[buf][e];
+            for (int e = tid; e < TB * Q::VALUES; e += THREADS) {
+                float s = cta.w[0].sum[buf][e];
 #pragma unroll
-                for (int w = 1; w < Q::WARPS; w++) s += all[w].sum[buf][e];
-                if (t < a.T)
-                    a.part_bc[((((size_t)cb * a.B + b) * a.T + t) * a.G + grp) * Q::VALUES + e % Q::VALUES] = s;
+                for (int w = 1; w < Q::WARPS; w++) s += cta.w[w].sum[buf][e];
+                if (e / Q::VALUES <= end)
+                    a.part_bc[((((size_t)un.cb * a.B + b) * a.T + blk * TB + e / Q::VALUES) * a.G + grp) * Q::VALUES + e % Q::VALUES] = s;
             }
         }
     }
 #pragma unroll
     for (int m = 1; m < LPC; m <<= 1) {
-        gD += __shfl_xor_sync(FULL_MASK, gD, m);
-        gbias += __shfl_xor_sync(FULL_MASK, gbias, m);
+        gD = add2(gD, make_float2(__shfl_xor_sync(FULL_MASK, gD.x, m), __shfl_xor_sync(FULL_MASK, gD.y, m)));
+        gbias = add2(gbias, make_float2(__shfl_xor_sync(FULL_MASK, gbias.x, m), __shfl_xor_sync(FULL_MASK, gbias.y, m)));
     }
-    if (live) {
-        if (span == 0 && a.gs_in) store_states(a.gs_in, row, n0, a.N, E);
-        if (a.part) {
-            float *p = a.part + ((size_t)b * a.nspan + span) * ((size_t)a.D * (a.N + 2));
-            store_states(p, (size_t)ch * a.N, n0, a.N, gA);
-            if (q == 0) {
-                p[(size_t)a.D * a.N + ch] = gD;
-                p[(size_t)a.D * (a.N + 1) + ch] = gbias;
+    float *p = a.part + ((size_t)b * a.nspan + span) * ((size_t)a.D * (a.N + 2));
+#pragma unroll
+    for (int k = 0; k < 2; k++) {
+        if (k ? live2 : live) {
+            if (span == 0 && a.gs_in) store_states(a.gs_in, row + k * a.N, n0, a.N, E[k], swap);
+            if (a.part) {
+                store_states(p, (size_t)(ch + k) * a.N, n0, a.N, gA[k], swap);
+                if (q == 0) {
+                    p[(size_t)a.D * a.N + ch + k] = k ? gD.y : gD.x;
+                    p[(size_t)a.D * (a.N + 1) + ch + k] = k ? gbias.y : gbias.x;
+                }
             }
         }
     }
@@ -630,7 +1001,9 @@ __global__ void __launch_bounds__(256) k_scan_fold_bc(const float *__restrict__ 
 }
 
 // ------------------------------------------------------------------------------------------------ host side
-int lanes_for(int N) { return N <= 4 ? 1 : N <= 8 ? 2 : N <= 16 ? 4 : N <= 32 ? 8 : 16; }
+constexpr long long MAX_STRIDE = 1 << 26;
+// (fewer than 5 states are padded to 8: one lane for four states and twice 64 channels a warp would need 255 registers and spill)
+int lanes_for(int N) { return N <= 8 ? 2 : N <= 16 ? 4 : N <= 32 ? 8 : 16; }
 
 int check_scan(const wkv_selective_scan_args_t *a) {
     if (!a) return WKV_ERR_NULL;
@@ -638,33 +1011,66 @@ int check_scan(const wkv_selective_scan_args_t *a) {
     if (!known_dtype(a->dtype)) return WKV_ERR_DTYPE;
     for (long long s : {a->u_batch, a->u_token, a->delta_batch, a->delta_token, a->B_batch, a->B_token, a->C_batch, a->C_token, a->z_batch, a->z_token})
         if (s < 0) return WKV_ERR_SHAPE;
+    // (the offsets inside a block of 16 tokens are 32-bit)
+    for (long long s : {(long long)a->D, a->u_token, a->delta_token, a->B_token, a->C_token, a->z_token})
+        if (s > MAX_STRIDE) return WKV_ERR_SHAPE;
     if (a->B == 0 || a->D == 0) return WKV_OK;
     if (!a->A || (a->T > 0 && (!a->u || !a->delta || !a->Bm || !a->Cm))) return WKV_ERR_NULL;
     return WKV_OK;
 }
 
-// spans of a row: enough for the GPU, of four blocks at least
-int plan_spans(const wkv_selective_scan_args_t *a) {
-    const int lpc = lanes_for(a->N), cpw = 32 / lpc, nblk = (a->T + TB - 1) / TB;
-    const long long warps = (long long)a->B * a->G * ((a->D / a->G + cpw - 1) / cpw);
-    long long n = a->time_groups;
-    if (n == 0) {
-        const long long want = (long long)device_sm_count() * 12;
-        n = warps * 2 > want ? 1 : want / warps;
-        if (n > 32) n = 32;
-        if (n > nblk / 4) n = nblk / 4;
-    }
+// n spans of whole blocks, none of them empty
+int whole_spans(long long n, int nblk) {
     if (n > nblk) n = nblk;
     if (n < 1) n = 1;
     const long long len = (nblk + n - 1) / n;
-    return len > 0 ? (int)((nblk + len - 1) / len) : 1;         // (no span is empty)
+    return len > 0 ? (int)((nblk + len - 1) / len) : 1;
+}
+int bwd_channel_blocks(const wkv_selective_scan_args_t *a) {
+    const int lpc = lanes_for(a->N), per = 4 * (64 / lpc);
+    return (a->D / a->G + per - 1) / per;
+}
+// Spans of a row, forward: none where one warp a scheduler or nearly that many are there without (512 warps: 59 us uncut, 67
+// in two spans; 320 warps: 754 us uncut, 500 in twelve); else so many that a few CTAs queue for every place, of eight blocks at
+// least, or of two while there are fewer warps than schedulers (2 rows of 509 tokens and 256 channels: 69 us uncut, 23 in 16).
+int plan_forward(const wkv_selective_scan_args_t *a) {
+    const int cpw = 64 / lanes_for(a->N), nblk = (a->T + TB - 1) / TB;
+    const long long warps = (long long)a->B * a->G * ((a->D / a->G + cpw - 1) / cpw), sms = device_sm_count();
+    long long n = a->time_groups;
+    if (n == 0) {
+        if (warps * 14 >= sms * 40) return 1;
+        long long most = nblk / 2 < sms * 4 / warps ? nblk / 2 : sms * 4 / warps;
+        if (nblk / 8 > most) most = nblk / 8;
+        n = sms * 24 / warps < most ? sms * 24 / warps : most;
+    }
+    return whole_spans(n, nblk);
 }
 
-ScanArgs scan_args(const wkv_selective_scan_args_t *a) {
+// Backward: the number of spans that a simple account of the time finds best.  A full pass of a block takes 1 with two CTAs on
+// an SM and 0.77 with one (932 and 715 us for 2048 tokens); a span starts up in 1.5 blocks; the summary pass takes 0.27 of a
+// full pass for the work that fills the GPU.  Against measurements of 1 to 32 spans (us: chosen, uncut, best of those tried): 4 rows of
+// 4096 tokens and channels 1684, 1684, 1684; 1 of 8191 x 5120 1230, 2399, 1219; 8 of 512 x 1024 145, 166, 145.
+int plan_backward(const wkv_selective_scan_args_t *a) {
+    const int nblk = (a->T + TB - 1) / TB;
+    if (a->time_groups) return whole_spans(a->time_groups, nblk);
+    const long long ctas = (long long)a->B * a->G * bwd_channel_blocks(a), sms = device_sm_count();
+    int best = 1;
+    double least = 0;
+    for (int n = 1; n <= 32 && (n == 1 || 2 * n <= nblk); n++) {
+        const long long x = ctas * n, rest = x % (2 * sms);
+        const int len = (nblk + n - 1) / n;
+        const double waves = (double)(x / (2 * sms)) + (rest == 0 ? 0.0 : rest <= sms ? 0.77 : 1.0);
+        const double t = waves * (len + 1.5) + 0.27 * (double)ctas / (double)(2 * sms) * (n - 1) * (len + 1);
+        if (n == 1 || t < least) { least = t; best = n; }
+    }
+    return whole_spans(best, nblk);
+}
+
+ScanArgs scan_args(const wkv_selective_scan_args_t *a, int nspan, bool &fast) {
     ScanArgs k = {};
     k.B = a->B; k.T = a->T; k.D = a->D; k.N = a->N; k.G = a->G; k.Dg = a->D / a->G; k.softplus = a->softplus != 0;
     k.nblk = (a->T + TB - 1) / TB;
-    k.nspan = plan_spans(a);
+    k.nspan = nspan;
     k.span_blocks = (k.nblk + k.nspan - 1) / k.nspan;
     k.u = a->u; k.delta = a->delta; k.Bm = a->Bm; k.Cm = a->Cm; k.z = a->z;
     k.u_batch = a->u_batch; k.u_token = a->u_token; k.delta_batch = a->delta_batch; k.delta_token = a->delta_token;
@@ -677,20 +1083,27 @@ ScanArgs scan_args(const wkv_selective_scan_args_t *a) {
     };
     k.vec_b = fits(a->Bm, a->B_batch, a->B_token);
     k.vec_c = fits(a->Cm, a->C_batch, a->C_token);
+    // two neighbouring channels in one access: in every tensor
+    const uintptr_t two = 2 * (uintptr_t)elem_size(a->dtype) - 1;
+    auto even = [&](const void *p, long long batch, long long token) {
+        return p == nullptr || (batch % 2 == 0 && token % 2 == 0 && (reinterpret_cast<uintptr_t>(p) & two) == 0);
+    };
+    const bool pairs = k.Dg % 2 == 0 && even(a->u, a->u_batch, a->u_token) && even(a->delta, a->delta_batch, a->delta_token) &&
+              even(a->z, a->z_batch, a->z_token) && even(a->y, 0, 0) && even(a->gy, 0, 0) && even(a->gu, 0, 0) && even(a->gdelta, 0, 0) &&
+              even(a->gz, 0, 0);
+    fast = pairs && k.vec_b && k.vec_c;
     return k;
 }
 
 template <class Fn>
 int by_lanes(int lpc, Fn f) {
     switch (lpc) {
-        case 1: return f(std::integral_constant<int, 1>{});
         case 2: return f(std::integral_constant<int, 2>{});
         case 4: return f(std::integral_constant<int, 4>{});
         case 8: return f(std::integral_constant<int, 8>{});
         default: return f(std::integral_constant<int, 16>{});
     }
 }
-int warps_of_cta(int lpc) { return lpc >= 8 ? 4 : 8; }
 
 size_t span_bytes(const wkv_selective_scan_args_t *a, int nspan) {
     if (nspan < 2) return 0;
@@ -701,15 +1114,11 @@ void place_spans(const wkv_selective_scan_args_t *a, ScanArgs &k, char *ws) {
     k.span_state = (float *)ws;
     k.span_dt = (float *)(ws + align256((size_t)a->B * k.nspan * a->D * a->N * 4));
 }
-int bwd_channel_blocks(const wkv_selective_scan_args_t *a) {
-    const int lpc = lanes_for(a->N), per = warps_of_cta(lpc) * (32 / lpc);
-    return (a->D / a->G + per - 1) / per;
-}
 struct BwdLayout {
     size_t spans, bc, params, total;
 };
 BwdLayout bwd_layout(const wkv_selective_scan_args_t *a) {
-    const int nspan = plan_spans(a);
+    const int nspan = plan_backward(a);
     BwdLayout l;
     l.spans = span_bytes(a, nspan);
     l.bc = align256((size_t)bwd_channel_blocks(a) * a->B * a->T * a->G * 8 * lanes_for(a->N) * 4);
@@ -731,7 +1140,7 @@ extern "C" size_t wkv_selective_scan_ckpt_bytes(const wkv_selective_scan_args_t 
 
 extern "C" size_t wkv_selective_scan_forward_workspace(const wkv_selective_scan_args_t *a) {
     if (check_scan(a) != WKV_OK || nothing(a)) return 0;
-    return span_bytes(a, plan_spans(a));
+    return span_bytes(a, plan_forward(a));
 }
 
 extern "C" int wkv_selective_scan_forward(const wkv_selective_scan_args_t *a, void *stream) {
@@ -748,14 +1157,22 @@ extern "C" int wkv_selective_scan_forward(const wkv_selective_scan_args_t *a, vo
     }
     if (!a->y) return WKV_ERR_NULL;
     if (a->T > 1 && a->state_in && a->state_in == a->state_out) return WKV_ERR_UNSUPPORTED;
-    ScanArgs k = scan_args(a);
+    bool fast;
+    ScanArgs k = scan_args(a, plan_forward(a), fast);
     k.y = a->y; k.state_out = a->state_out;
-    const int lpc = lanes_for(a->N), cpw = 32 / lpc;
+    const int lpc = lanes_for(a->N), cpw = 64 / lpc;
     if (a->T == 1 && !a->ckpt) {
-        const long long threads = (long long)a->B * a->D * lpc;
+        const long long threads = (long long)a->D * lpc;
+        const int rows = a->B >= 8 ? 4 : 1;             // (the launch takes 65535 blocks of rows)
+        if ((a->B + rows - 1) / rows > 65535) return WKV_ERR_SHAPE;
+        k.vec_a = a->N % 4 == 0 && aligned16(a->A);
+        k.vec_s = a->N % 4 == 0 && all_aligned({a->state_in, a->state_out});
+        const dim3 grid((unsigned)((threads + 255) / 256), (unsigned)((a->B + rows - 1) / rows));
         return by_dtype(a->dtype, [&](auto f) {
             return by_lanes(lpc, [&](auto l) {
-                return launch_chained(k_scan_step<decltype(f), decltype(l)::value>, dim3((unsigned)((threads + 255) / 256)), dim3(256), 0, s, k);
+                using F = decltype(f);
+                constexpr int LANES = decltype(l)::value;
+                return launch_chained(rows == 4 ? k_scan_step<F, LANES, 4> : k_scan_step<F, LANES, 1>, grid, dim3(256), 0, s, k);
             });
         });
     }
@@ -777,10 +1194,12 @@ extern "C" int wkv_selective_scan_forward(const wkv_selective_scan_args_t *a, vo
             using F = decltype(f);
             constexpr int LPC = decltype(l)::value;
             if (k.nspan > 1) {
-                const int r = launch_chained(k_scan_fwd<F, LPC, true>, dim3((unsigned)((per_span * (k.nspan - 1) + 3) / 4)), dim3(128), 0, s, k);
+                const int r = launch_chained(fast ? k_scan_fwd<F, LPC, true, true> : k_scan_fwd<F, LPC, true, false>,
+                                             dim3((unsigned)((per_span * (k.nspan - 1) + 3) / 4)), dim3(128), 0, s, k);
                 if (r != WKV_OK) return r;
             }
-            return launch_chained(k_scan_fwd<F, LPC, false>, dim3((unsigned)((per_span * k.nspan + 3) / 4)), dim3(128), 0, s, k);
+            return launch_chained(fast ? k_scan_fwd<F, LPC, false, true> : k_scan_fwd<F, LPC, false, false>,
+                                  dim3((unsigned)((per_span * k.nspan + 3) / 4)), dim3(128), 0, s, k);
         });
     });
 }
@@ -815,14 +1234,15 @@ extern "C" int wkv_selective_scan_backward(const wkv_selective_scan_args_t *a, v
     if (!a->ckpt || a->ckpt_bytes < wkv_selective_scan_ckpt_bytes(a)) return WKV_ERR_WORKSPACE;
     if (!a->workspace || a->workspace_bytes < l.total) return WKV_ERR_WORKSPACE;
     if (!aligned16(a->workspace) || !aligned16(a->ckpt)) return WKV_ERR_ALIGN;
-    ScanArgs k = scan_args(a);
+    bool fast;
+    ScanArgs k = scan_args(a, plan_backward(a), fast);
     char *ws = (char *)a->workspace;
     if (l.spans) place_spans(a, k, ws);
     k.ckpt = (float *)a->ckpt;
     k.gy = a->gy; k.gs_out = a->gstate_out; k.gu = a->gu; k.gdelta = a->gdelta; k.gz = a->z ? a->gz : nullptr; k.gs_in = a->gstate_in;
     k.part_bc = a->gB || a->gC ? (float *)(ws + l.spans) : nullptr;
     k.part = params ? (float *)(ws + l.spans + l.bc) : nullptr;
-    const int lpc = lanes_for(a->N), cpw = 32 / lpc;
+    const int lpc = lanes_for(a->N), cpw = 64 / lpc;
     const int ncb = bwd_channel_blocks(a);
     e = by_dtype(a->dtype, [&](auto f) {
         return by_lanes(lpc, [&](auto l_) {
@@ -832,14 +1252,15 @@ extern "C" int wkv_selective_scan_backward(const wkv_selective_scan_args_t *a, v
                 ScanArgs m = k;
                 m.ncb = (k.Dg + cpw - 1) / cpw;
                 const long long units = (long long)m.ncb * a->G * (k.nspan - 1) * a->B;
-                const int r = launch_chained(k_scan_bwd_summary<F, LPC>, dim3((unsigned)((units + 3) / 4)), dim3(128), 0, s, m);
+                const int r = launch_chained(fast ? k_scan_bwd_summary<F, LPC, true> : k_scan_bwd_summary<F, LPC, false>, dim3((unsigned)((units + 3) / 4)), dim3(128), 0, s, m);
                 if (r != WKV_OK) return r;
             }
             k.ncb = ncb;
-            static unsigned char done[64];
-            if (!set_max_smem_once(k_scan_bwd<F, LPC>, BwdGeo<LPC>::SMEM, done)) return (int)WKV_ERR_LAUNCH;
-            const int r = launch_chained(k_scan_bwd<F, LPC>, dim3((unsigned)((long long)ncb * a->G * k.nspan * a->B)),
-                                         dim3(32 * BwdGeo<LPC>::WARPS), BwdGeo<LPC>::SMEM, s, k);
+            static unsigned char done[2][64];
+            const auto kern = fast ? k_scan_bwd<F, LPC, true> : k_scan_bwd<F, LPC, false>;
+            if (!set_max_smem_once(kern, BwdGeo<F, LPC>::SMEM, done[fast])) return (int)WKV_ERR_LAUNCH;
+            const int r = launch_chained(kern, dim3((unsigned)((long long)ncb * a->G * k.nspan * a->B)),
+                                         dim3(32 * BwdGeo<F, LPC>::WARPS), BwdGeo<F, LPC>::SMEM, s, k);
             if (r != WKV_OK || !k.part_bc) return r;
             const long long rows = (long long)a->B * a->T * a->G;
             return launch_chained(k_scan_fold_bc<F>, dim3((unsigned)((rows * 8 * LPC + 255) / 256)), dim3(256), 0, s, k.part_bc, ncb, rows,

@@ -11,8 +11,8 @@
     rounded up.  ``scale = max|y| / 448``.  No gradient.
 
 x [..., C] in bf16, fp16 or fp32, 1 <= C <= 16384; the residual (and ``h``) in x's type or in fp32, ``y`` in x's type;
-weight [C] in any float type.  Sums are fp32; ``y`` is formed from ``h`` before it is rounded to the residual's type,
-the backward pass starts from the rounded ``h``.
+weight [C] in any float type.  Sums are fp32; ``y`` and the gradients are formed from ``h`` before it is rounded to the
+residual's type.
 """
 from __future__ import annotations
 

@@ -147,19 +147,16 @@ def conv_K(name, B, T, W):
 
 
 # ---------------------------------------------------------------------------------------- norm
-def norm_ref(x, w, res, eps, gy=None, gh=None, h=None):
-    """h: what the backward pass starts from (the rounded sum), else the exact one"""
+def norm_ref(x, w, res, eps, gy=None, gh=None):
     d = lambda t: None if t is None else t.detach().double()
-    x, w, res, gy, gh, h = (d(t) for t in (x, w, res, gy, gh, h))
+    x, w, res, gy, gh = (d(t) for t in (x, w, res, gy, gh))
     out = {}
-    full = x if res is None else x + res
-    r = torch.rsqrt((full * full).mean(-1, keepdim=True) + eps)
-    out["y"], out["h"] = full * r * w, full
+    h = x if res is None else x + res
+    r = torch.rsqrt((h * h).mean(-1, keepdim=True) + eps)
+    out["y"], out["h"] = h * r * w, h
     out["y_mag"], out["h_mag"] = out["y"].abs(), x.abs() + (0 if res is None else res.abs())
     if gy is None and gh is None:
         return out
-    h = full if h is None else h
-    r = torch.rsqrt((h * h).mean(-1, keepdim=True) + eps)
     gy = torch.zeros_like(x) if gy is None else gy
     gh = torch.zeros_like(x) if gh is None else gh
     xh, gn = h * r, gy * w

@@ -43,7 +43,7 @@ def train(c):
 def check(c, got):
     C = c["x"].shape[-1]
     rows = c["x"].numel() // C
-    ref = S.norm_ref(c["x"], c["weight"], c["residual"], EPS, c["gy"], c["gh"], got.get("h"))
+    ref = S.norm_ref(c["x"], c["weight"], c["residual"], EPS, c["gy"], c["gh"])
     for n, t in got.items():
         r = "gx" if n == "gres" else n
         S.close(n, t, ref[r], ref[r + "_mag"], K(r, rows, C))
@@ -135,12 +135,19 @@ def test_missing_gradients_and_one_alone():
 
 def test_residual_stream_changed_in_place_is_noticed():
     import rwkv_infctx_trainer_b200 as W
-    c = case(7, (4, 64), BF, BF)
+    c = case(7, (4, 64), BF, F32)
     x = c["x"].requires_grad_(True)
     y, h = W.rms_norm(x, c["weight"], c["residual"])
     h.add_(1)
     with pytest.raises(RuntimeError, match="inplace"):
         (y.float().sum() + h.float().sum()).backward()
+    # (a 16-bit h is not what the backward pass starts from)
+    c = case(7, (4, 64), BF, BF)
+    want = train(c)
+    x = c["x"].requires_grad_(True)
+    y, h = W.rms_norm(x, c["weight"], c["residual"], EPS)
+    h = h.add_(1)
+    assert torch.equal(torch.autograd.grad((y, h), x, (c["gy"], c["gh"]))[0], want["gx"])
 
 
 def test_the_residual_stream_is_not_kept_alive_by_its_own_history():
