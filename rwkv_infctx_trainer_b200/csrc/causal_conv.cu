@@ -6,8 +6,8 @@
 //   backward: ds = gy silu'(s),  gx_t = sum_j weight[d,j] ds_{t+W-1-j},  gweight[d,j] = sum_t ds_t x_{t-W+1+j},  gbias = sum ds;
 //   what reaches inputs of negative time is the state's gradient.
 //
-// Bound by HBM.  A thread owns a few neighbouring channels and walks a strip of tokens with the last W-1 inputs in
-// registers; neighbouring strips read W-1 tokens twice (from L2).  Nothing is kept for the backward pass: s is formed again.
+// Bound by HBM.  A thread owns four neighbouring channels and walks a strip of tokens with the last W-1 inputs in
+// registers, on packed arithmetic; neighbouring strips read W-1 tokens twice (from L2).  Nothing is kept for the backward pass: s is formed again.
 #include "elem_io.cuh"
 #include "wkv_internal.h"
 
@@ -15,6 +15,10 @@ namespace wkv {
 namespace {
 
 constexpr int MAX_W = 4;
+constexpr int V = 4;                     // channels of a thread
+// Tokens of a group and groups on their way (us forward, 4 rows of 4096 tokens and channels: 8 x 2 79, 4 x 4 80, 2 x 8 66, 1 x 16 115;
+// backward: 4 x 4 157, 3 x 4 149, 2 x 6 165): small groups leave registers for more threads.
+constexpr int FWD_GT = 2, FWD_AHEAD = 8, BWD_GT = 3, BWD_AHEAD = 4;
 
 struct ConvArgs {
     int B, T, D, w_dtype, silu;
@@ -24,185 +28,266 @@ struct ConvArgs {
     const void *gy, *gs_out;
     void *gx, *gs_in;
     float *part;                         // [B * strips of a row, D * (W + 1)]
-    int strip, nstrip, vec;
+    int strip, nstrip, vec, vec_w;
 };
 
-__device__ __forceinline__ float silu_grad(float s) {
-    const float sg = sigmoidf(s);
-    return sg * (1.f + s * (1.f - sg));
-}
-
 // inputs of the row at time t: from the state below zero (zeros without one)
-template <typename F, int V, int W>
+template <typename F, int W>
 __device__ __forceinline__ void input_at(const ConvArgs &a, int b, int c, int n, int t, Raw<F, V> &r) {
     if (t >= 0) r.load((const F *)a.x + (size_t)b * a.x_batch + (size_t)t * a.x_token + c, a.vec, n);
     else if (a.state_in) r.load((const F *)a.state_in + ((size_t)b * (W - 1) + (W - 1 + t)) * a.D + c, a.vec, n);
     else r.zero();
 }
 
-// V channels per thread: 16 bytes of them.  blockIdx.x: (row, strip), blockIdx.y: 256 runs of channels
+// the parameters of a thread's channels: two pairs of channels per tap
+template <int W>
+__device__ __forceinline__ void load_params(const ConvArgs &a, int c, int n, f2 (&w)[W][2], f2 (&bias)[2]) {
+    float t[V][W], bb[V];
+#pragma unroll
+    for (int q = 0; q < V; q++) {
+        bb[q] = a.bias && q < n ? param_at(a.bias, a.w_dtype, c + q) : 0.f;
+        if (W == 4 && a.vec_w) {
+            const float4 v = q < n ? __ldg(reinterpret_cast<const float4 *>((const float *)a.w + (size_t)(c + q) * W)) : make_float4(0.f, 0.f, 0.f, 0.f);
+            t[q][0] = v.x; t[q][1] = v.y; t[q][2 % W] = v.z; t[q][3 % W] = v.w;
+        } else {
+#pragma unroll
+            for (int j = 0; j < W; j++) t[q][j] = q < n ? param_at(a.w, a.w_dtype, (size_t)(c + q) * W + j) : 0.f;
+        }
+    }
+#pragma unroll
+    for (int p = 0; p < 2; p++) {
+        bias[p] = make_float2(bb[2 * p], bb[2 * p + 1]);
+#pragma unroll
+        for (int j = 0; j < W; j++) w[j][p] = make_float2(t[2 * p][j], t[2 * p + 1][j]);
+    }
+}
+template <typename F>
+__device__ __forceinline__ void get_pairs(const Raw<F, V> &r, f2 (&v)[2]) {
+    float f[V];
+    r.get(f);
+    v[0] = make_float2(f[0], f[1]);
+    v[1] = make_float2(f[2], f[3]);
+}
+template <typename F>
+__device__ __forceinline__ Raw<F, V> put_pairs(const f2 (&v)[2]) {
+    const float f[V] = {v[0].x, v[0].y, v[1].x, v[1].y};
+    Raw<F, V> r;
+    r.put(f);
+    return r;
+}
+__device__ __forceinline__ float rcp(float x) {
+    float y;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ f2 sigmoid2(f2 x) {
+    const f2 t = mul2(x, both(-1.4426950408889634f));
+    return make_float2(rcp(1.f + exp2f(t.x)), rcp(1.f + exp2f(t.y)));
+}
+
+// A thread's inputs on their way: a ring of AHEAD groups of GT tokens of N tensors in shared memory, a place of its own for
+// each thread (nobody else reads it: no barriers).  Held in registers instead, two groups were as many as fit: 78 us instead of 66
+// forward, 218 instead of 149 backward for 4 rows of 4096 tokens and channels.
+template <typename F, int GT, int N, int AHEAD>
+struct Ring {
+    Raw<F, V> *mine;
+    bool vec;
+    int n;
+    static constexpr int BYTES = AHEAD * GT * N * (int)sizeof(Raw<F, V>);        // a thread
+    __device__ __forceinline__ Raw<F, V> &at(int group, int i, int k) { return mine[(((group % AHEAD) * GT + i) * N + k) * blockDim.x]; }
+    __device__ __forceinline__ void load(int group, int i, int k, const F *p) {
+        Raw<F, V> &to = at(group, i, k);
+        if (vec) {
+            const uint32_t dst = (uint32_t)__cvta_generic_to_shared(&to);
+            if constexpr (sizeof(to) == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(p) : "memory");
+            else asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(dst), "l"(p) : "memory");
+        } else {
+            Raw<F, V> r;
+            r.load(p, false, n);
+            to = r;
+        }
+    }
+    __device__ __forceinline__ void commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+    // all but the last AHEAD - 1 groups have arrived
+    __device__ __forceinline__ void wait() { asm volatile("cp.async.wait_group %0;" ::"n"(AHEAD - 1) : "memory"); }
+};
+template <typename F>
+using FwdRing = Ring<F, FWD_GT, 1, FWD_AHEAD>;
+template <typename F>
+using BwdRing = Ring<F, BWD_GT, 2, BWD_AHEAD>;
+
+// blockIdx.x: (row, strip), blockIdx.y: runs of channels
 template <typename F, int W>
 __global__ void __launch_bounds__(256) k_conv_fwd(ConvArgs a) {
     pdl_wait();
     pdl_trigger();
-    constexpr int V = 16 / (int)sizeof(F), AHEAD = 4;
+    constexpr int GT = FWD_GT;
+    extern __shared__ __align__(16) char smem_raw[];
     const int c = (blockIdx.y * blockDim.x + threadIdx.x) * V;
     if (c >= a.D) return;
     const int n = min(V, a.D - c), b = blockIdx.x / a.nstrip, t0 = (blockIdx.x - b * a.nstrip) * a.strip;
     const int t1 = min(t0 + a.strip, a.T);
-    Raw<F, V> in[W - 1 + AHEAD];
+    FwdRing<F> ring = {reinterpret_cast<Raw<F, V> *>(smem_raw) + threadIdx.x, (bool)a.vec, n};
+    const F *px = (const F *)a.x + (size_t)b * a.x_batch + c;
+    auto fetch = [&](int group) {
 #pragma unroll
-    for (int j = 0; j < W - 1; j++) input_at<F, V, W>(a, b, c, n, t0 - (W - 1) + j, in[j]);
-    float w[V][W], bias[V];
+        for (int i = 0; i < GT; i++) {
+            const int t = t0 + group * GT + i;
+            if (t < t1) ring.load(group, i, 0, px + (size_t)t * a.x_token);
+        }
+        ring.commit();
+    };
 #pragma unroll
-    for (int q = 0; q < V; q++) {
-        bias[q] = a.bias && q < n ? param_at(a.bias, a.w_dtype, c + q) : 0.f;
+    for (int g = 0; g < FWD_AHEAD; g++) fetch(g);
+    f2 w[W][2], bias[2], x[W - 1 + GT][2];
+    load_params<W>(a, c, n, w, bias);
 #pragma unroll
-        for (int j = 0; j < W; j++) w[q][j] = q < n ? param_at(a.w, a.w_dtype, (size_t)(c + q) * W + j) : 0.f;
+    for (int j = 0; j < W - 1; j++) {
+        Raw<F, V> r;
+        input_at<F, W>(a, b, c, n, t0 - (W - 1) + j, r);
+        get_pairs(r, x[j]);
     }
     F *y = (F *)a.y + ((size_t)b * a.T) * a.D + c;
-    for (int t = t0; t < t1; t += AHEAD) {
+    for (int t = t0, group = 0; t < t1; t += GT, group++) {
+        ring.wait();
 #pragma unroll
-        for (int i = 0; i < AHEAD; i++) {
-            if (t + i < t1) input_at<F, V, W>(a, b, c, n, t + i, in[W - 1 + i]);
-        }
+        for (int i = 0; i < GT; i++) get_pairs(ring.at(group, i, 0), x[W - 1 + i]);
+        fetch(group + FWD_AHEAD);
 #pragma unroll
-        for (int i = 0; i < AHEAD; i++) {
-            if (t + i < t1) {
-                float s[V];
+        for (int i = 0; i < GT; i++) {
+            f2 s[2] = {bias[0], bias[1]};
 #pragma unroll
-                for (int q = 0; q < V; q++) s[q] = bias[q];
+            for (int j = 0; j < W; j++)
 #pragma unroll
-                for (int j = 0; j < W; j++) {
-                    float f[V];
-                    in[i + j].get(f);
+                for (int p = 0; p < 2; p++) s[p] = fma2(w[j][p], x[i + j][p], s[p]);
+            if (a.silu) {
 #pragma unroll
-                    for (int q = 0; q < V; q++) s[q] += w[q][j] * f[q];
-                }
-                if (a.silu) {
-#pragma unroll
-                    for (int q = 0; q < V; q++) s[q] *= sigmoidf(s[q]);
-                }
-                Raw<F, V> o;
-                o.put(s);
-                o.store(y + (size_t)(t + i) * a.D, a.vec, n);
+                for (int p = 0; p < 2; p++) s[p] = mul2(s[p], sigmoid2(s[p]));
             }
+            if (t + i < t1) put_pairs<F>(s).store(y + (size_t)(t + i) * a.D, a.vec, n);
         }
         // the last W-1 inputs that exist move to the front
-        const int k = min(AHEAD, t1 - t);
-        Raw<F, V> last[W - 1];
+        const int k = min(GT, t1 - t);
 #pragma unroll
-        for (int j = 0; j < W - 1; j++)
+        for (int j = 0; j < W - 1; j++) {
+            f2 l[2] = {x[GT + j][0], x[GT + j][1]};
+            if (k < GT) {
 #pragma unroll
-            for (int i = 1; i <= AHEAD; i++)
-                if (i == k) last[j] = in[i + j];
-#pragma unroll
-        for (int j = 0; j < W - 1; j++) in[j] = last[j];
+                for (int i = 1; i < GT; i++)
+                    if (i == k) { l[0] = x[i + j][0]; l[1] = x[i + j][1]; }
+            }
+            x[j][0] = l[0];
+            x[j][1] = l[1];
+        }
     }
     if (t1 == a.T && a.state_out) {
 #pragma unroll
-        for (int j = 0; j < W - 1; j++) in[j].store((F *)a.state_out + ((size_t)b * (W - 1) + j) * a.D + c, a.vec, n);
+        for (int j = 0; j < W - 1; j++) put_pairs<F>(x[j]).store((F *)a.state_out + ((size_t)b * (W - 1) + j) * a.D + c, a.vec, n);
     }
 }
 
-// A thread walks its strip forward, W-1 tokens past its end: at token t it forms s_t and ds_t, adds to the sums of the
-// parameters' gradients where t is its own, and hands out gx of token t-W+1, which is complete then.
+// A thread walks its strip forward, W-1 tokens past its end, in groups: it forms s and ds of a group's tokens, adds to the sums
+// of the parameters' gradients where they are its own, and hands out gx of the tokens W-1 earlier, which is complete then.
 template <typename F, int W>
 __global__ void __launch_bounds__(256) k_conv_bwd(ConvArgs a) {
     pdl_wait();
     pdl_trigger();
-    constexpr int V = 4;
+    constexpr int GT = BWD_GT;
+    extern __shared__ __align__(16) char smem_raw[];
     const int c = (blockIdx.y * blockDim.x + threadIdx.x) * V;
     if (c >= a.D) return;
     const int n = min(V, a.D - c), b = blockIdx.x / a.nstrip, t0 = (blockIdx.x - b * a.nstrip) * a.strip;
-    const int t1 = min(t0 + a.strip, a.T);
-    float w[V][W], bias[V], gw[V][W], gb[V];
+    const int t1 = min(t0 + a.strip, a.T), stop = t1 + W - 1, some = min(stop, a.T);
+    BwdRing<F> ring = {reinterpret_cast<Raw<F, V> *>(smem_raw) + threadIdx.x, (bool)a.vec, n};
+    const F *px = (const F *)a.x + (size_t)b * a.x_batch + c, *gy = (const F *)a.gy + ((size_t)b * a.T) * a.D + c;
+    auto fetch = [&](int group) {
 #pragma unroll
-    for (int q = 0; q < V; q++) {
-        bias[q] = a.bias && q < n ? param_at(a.bias, a.w_dtype, c + q) : 0.f;
-        gb[q] = 0.f;
-#pragma unroll
-        for (int j = 0; j < W; j++) {
-            w[q][j] = q < n ? param_at(a.w, a.w_dtype, (size_t)(c + q) * W + j) : 0.f;
-            gw[q][j] = 0.f;
+        for (int i = 0; i < GT; i++) {
+            const int t = t0 + group * GT + i;
+            if (t < some) {
+                ring.load(group, i, 0, px + (size_t)t * a.x_token);
+                if (a.gy) ring.load(group, i, 1, gy + (size_t)t * a.D);
+            }
         }
-    }
-    float x[V][W], g[V][W];              // x_{t-W+1} .. x_t;  sums for gx_{t-W+1} .. gx_t
+        ring.commit();
+    };
+#pragma unroll
+    for (int g = 0; g < BWD_AHEAD; g++) fetch(g);
+    f2 w[W][2], bias[2], gw[W][2], gb[2] = {both(0.f), both(0.f)};
+    f2 x[W - 1 + GT][2], ds[W - 1 + GT][2];              // of tokens t-W+1 .. t+GT-1
+    load_params<W>(a, c, n, w, bias);
+#pragma unroll
+    for (int j = 0; j < W; j++) gw[j][0] = gw[j][1] = both(0.f);
 #pragma unroll
     for (int j = 0; j < W - 1; j++) {
         Raw<F, V> r;
-        float f[V];
-        input_at<F, V, W>(a, b, c, n, t0 - (W - 1) + j, r);
-        r.get(f);
-#pragma unroll
-        for (int q = 0; q < V; q++) x[q][j] = f[q];
+        input_at<F, W>(a, b, c, n, t0 - (W - 1) + j, r);
+        get_pairs(r, x[j]);
+        ds[j][0] = ds[j][1] = both(0.f);
     }
-#pragma unroll
-    for (int q = 0; q < V; q++)
-#pragma unroll
-        for (int j = 0; j < W; j++) g[q][j] = 0.f;
-    const F *gy = a.gy ? (const F *)a.gy + ((size_t)b * a.T) * a.D + c : nullptr;
     // (of the tokens before the strip only the first strip's, the state, are its own)
     const int first = t0 == 0 ? -(W - 1) : t0;
-    for (int t = t0; t < t1 + W - 1; t++) {
-        float ds[V];
+    for (int t = t0, group = 0; t < stop; t += GT, group++) {
+        ring.wait();
 #pragma unroll
-        for (int q = 0; q < V; q++) ds[q] = 0.f;
-        if (t < a.T) {
-            Raw<F, V> rx, rg;
-            float f[V];
-            input_at<F, V, W>(a, b, c, n, t, rx);
-            rg.zero();
-            if (gy) rg.load(gy + (size_t)t * a.D, a.vec, n);
-            rx.get(f);
-            rg.get(ds);
+        for (int i = 0; i < GT; i++) {
+            get_pairs(ring.at(group, i, 0), x[W - 1 + i]);
+            if (a.gy) get_pairs(ring.at(group, i, 1), ds[W - 1 + i]);
+            else ds[W - 1 + i][0] = ds[W - 1 + i][1] = both(0.f);
+        }
+        fetch(group + BWD_AHEAD);
 #pragma unroll
-            for (int q = 0; q < V; q++) {
-                x[q][W - 1] = f[q];
-                if (a.silu) {
-                    float s = bias[q];
+        for (int i = 0; i < GT; i++) {
+            f2(&d)[2] = ds[W - 1 + i];
+            if (a.silu) {
 #pragma unroll
-                    for (int j = 0; j < W; j++) s += w[q][j] * x[q][j];
-                    ds[q] *= silu_grad(s);
-                }
-                if (t < t1) {
-                    gb[q] += ds[q];
+                for (int p = 0; p < 2; p++) {
+                    f2 s = bias[p];
 #pragma unroll
-                    for (int j = 0; j < W; j++) gw[q][j] += ds[q] * x[q][j];
+                    for (int j = 0; j < W; j++) s = fma2(w[j][p], x[i + j][p], s);
+                    const f2 sg = sigmoid2(s);
+                    d[p] = mul2(d[p], mul2(sg, fma2(s, sub2(both(1.f), sg), both(1.f))));
                 }
             }
-        }
-        const int to = t - (W - 1);       // the token whose gradient is complete
-        float o[V];
+            // behind the row there is no gradient (zero times what is formed from no inputs may be a NaN)
+            if (t + i >= a.T) d[0] = d[1] = both(0.f);
+            if (t + i < t1) {
 #pragma unroll
-        for (int q = 0; q < V; q++) {
+                for (int p = 0; p < 2; p++) {
+                    gb[p] = add2(gb[p], d[p]);
 #pragma unroll
-            for (int j = 0; j < W; j++) g[q][j] += w[q][j] * ds[q];
-            o[q] = g[q][0];
-        }
-        if (to >= first && to < t1) {
-            if (a.gs_out && to >= a.T - (W - 1)) {        // a token that is part of the state handed on
-                Raw<F, V> r;
-                float f[V];
-                r.load((const F *)a.gs_out + ((size_t)b * (W - 1) + (to - (a.T - (W - 1)))) * a.D + c, a.vec, n);
-                r.get(f);
-#pragma unroll
-                for (int q = 0; q < V; q++) o[q] += f[q];
+                    for (int j = 0; j < W; j++) gw[j][p] = fma2(d[p], x[i + j][p], gw[j][p]);
+                }
             }
-            Raw<F, V> r;
-            r.put(o);
-            if (to >= 0) {
-                if (a.gx) r.store((F *)a.gx + ((size_t)b * a.T + to) * a.D + c, a.vec, n);
-            } else if (a.gs_in) {
-                r.store((F *)a.gs_in + ((size_t)b * (W - 1) + (W - 1 + to)) * a.D + c, a.vec, n);
+            const int to = t + i - (W - 1);       // the token whose gradient is complete
+            if (to >= first && to < t1) {
+                f2 o[2] = {both(0.f), both(0.f)};
+#pragma unroll
+                for (int j = 0; j < W; j++)
+#pragma unroll
+                    for (int p = 0; p < 2; p++) o[p] = fma2(w[j][p], ds[W - 1 + i - j][p], o[p]);
+                if (a.gs_out && to >= a.T - (W - 1)) {        // a token that is part of the state handed on
+                    Raw<F, V> r;
+                    f2 f[2];
+                    r.load((const F *)a.gs_out + ((size_t)b * (W - 1) + (to - (a.T - (W - 1)))) * a.D + c, a.vec, n);
+                    get_pairs(r, f);
+                    o[0] = add2(o[0], f[0]);
+                    o[1] = add2(o[1], f[1]);
+                }
+                if (to >= 0) {
+                    if (a.gx) put_pairs<F>(o).store((F *)a.gx + ((size_t)b * a.T + to) * a.D + c, a.vec, n);
+                } else if (a.gs_in) {
+                    put_pairs<F>(o).store((F *)a.gs_in + ((size_t)b * (W - 1) + (W - 1 + to)) * a.D + c, a.vec, n);
+                }
             }
         }
 #pragma unroll
-        for (int q = 0; q < V; q++) {
+        for (int j = 0; j < W - 1; j++)
 #pragma unroll
-            for (int j = 0; j < W - 1; j++) { x[q][j] = x[q][j + 1]; g[q][j] = g[q][j + 1]; }
-            g[q][W - 1] = 0.f;
-        }
+            for (int p = 0; p < 2; p++) {
+                x[j][p] = x[GT + j][p];
+                ds[j][p] = ds[GT + j][p];
+            }
     }
     if (a.part) {
         float *p = a.part + (size_t)blockIdx.x * ((size_t)a.D * (W + 1));
@@ -210,8 +295,8 @@ __global__ void __launch_bounds__(256) k_conv_bwd(ConvArgs a) {
         for (int q = 0; q < V; q++) {
             if (q < n) {
 #pragma unroll
-                for (int j = 0; j < W; j++) p[(size_t)(c + q) * W + j] = gw[q][j];
-                p[(size_t)a.D * W + c + q] = gb[q];
+                for (int j = 0; j < W; j++) p[(size_t)(c + q) * W + j] = q & 1 ? gw[j][q / 2].y : gw[j][q / 2].x;
+                p[(size_t)a.D * W + c + q] = q & 1 ? gb[q / 2].y : gb[q / 2].x;
             }
         }
     }
@@ -227,18 +312,20 @@ int check_conv(const wkv_causal_conv_args_t *a) {
     return WKV_OK;
 }
 
-// tokens of a strip: so long that the W-1 tokens read twice do not count, and so short that the GPU is full
-int strip_for(int B, int T, int D, int per_thread, int longest) {
-    const long long across = (long long)B * ((D + per_thread - 1) / per_thread), want = (long long)device_sm_count() * 1536;
-    long long strip = across * T / want;
-    strip = strip < 16 ? 16 : strip > longest ? longest : strip;
-    return (int)strip;
+// Tokens of a strip: so many strips that the GPU has `threads` an SM, `longest` tokens at most: short ones leave little to hide a
+// load behind, long ones few threads (forward 64 tokens 66 us, 128 80, 32 76; backward 110 tokens 149, 220 171, 64 167).
+constexpr int FWD_THREADS = 1536, FWD_LONGEST = 64, BWD_THREADS = 1024, BWD_LONGEST = 256, SHORTEST = 16;
+int strip_for(int B, int T, int D, int threads, int longest) {
+    const long long across = (long long)B * ((D + V - 1) / V), want = (long long)device_sm_count() * threads;
+    const long long strip = across * T / want;
+    return (int)(strip < SHORTEST ? SHORTEST : strip > longest ? longest : strip);
 }
 
 ConvArgs conv_args(const wkv_causal_conv_args_t *a) {
     ConvArgs k = {};
     k.B = a->B; k.T = a->T; k.D = a->D; k.w_dtype = a->w_dtype; k.silu = a->silu != 0;
     k.x_batch = a->x_batch; k.x_token = a->x_token;
+    k.vec_w = a->w_dtype == WKV_F32 && aligned16(a->weight);
     k.x = a->x; k.w = a->weight; k.bias = a->bias; k.state_in = a->state_in;
     return k;
 }
@@ -257,7 +344,12 @@ int by_width(int W, Fn f) {
     }
 }
 
-constexpr int BWD_V = 4;
+// threads of a CTA: few of them where that gives every SM one
+int threads_for(int runs, long long strips) {
+    int nt = 256;
+    while (nt > 32 && (runs + nt - 1) / nt * strips < device_sm_count()) nt /= 2;
+    return nt;
+}
 
 }  // namespace
 }  // namespace wkv
@@ -270,26 +362,27 @@ extern "C" int wkv_causal_conv_forward(const wkv_causal_conv_args_t *a, void *st
     if (a->B == 0 || a->D == 0) return WKV_OK;
     if (a->T > 0 && !a->y) return WKV_ERR_NULL;
     // (a thread of the first strip reads the state after one of the last strip has written it)
-    if (a->T > 16 && a->state_in && a->state_in == a->state_out) return WKV_ERR_UNSUPPORTED;
+    if (a->T > SHORTEST && a->state_in && a->state_in == a->state_out) return WKV_ERR_UNSUPPORTED;
     ConvArgs k = conv_args(a);
     k.y = a->y; k.state_out = a->state_out;
     k.vec = conv_vec(a, {a->x, a->state_in, a->y, a->state_out});
-    const int per = 16 / elem_size(a->dtype);
-    k.strip = strip_for(a->B, a->T, a->D, per, 64);
+    k.strip = strip_for(a->B, a->T, a->D, FWD_THREADS, FWD_LONGEST);
     k.nstrip = a->T > 0 ? (a->T + k.strip - 1) / k.strip : 1;
-    const int runs = (a->D + per - 1) / per, nt = runs >= 256 ? 256 : (runs + 31) / 32 * 32;
+    const int runs = (a->D + V - 1) / V, nt = threads_for(runs, (long long)a->B * k.nstrip);
     return by_dtype(a->dtype, [&](auto f) {
         using F = decltype(f);
         return by_width(a->W, [&](auto w) {
-            return launch_chained(k_conv_fwd<F, decltype(w)::value>, dim3(a->B * k.nstrip, (runs + nt - 1) / nt), dim3(nt), 0,
-                                  (cudaStream_t)stream, k);
+            constexpr auto kern = k_conv_fwd<F, decltype(w)::value>;
+            static unsigned char done[64];
+            if (!set_max_smem_once(kern, 256 * FwdRing<F>::BYTES, done)) return (int)WKV_ERR_LAUNCH;
+            return launch_chained(kern, dim3(a->B * k.nstrip, (runs + nt - 1) / nt), dim3(nt), nt * FwdRing<F>::BYTES, (cudaStream_t)stream, k);
         });
     });
 }
 
 extern "C" size_t wkv_causal_conv_backward_workspace(const wkv_causal_conv_args_t *a) {
     if (check_conv(a) != WKV_OK || a->B == 0 || a->D == 0 || a->T == 0) return 0;
-    const int strip = strip_for(a->B, a->T, a->D, BWD_V, 256);
+    const int strip = strip_for(a->B, a->T, a->D, BWD_THREADS, BWD_LONGEST);
     return align256((size_t)a->B * ((a->T + strip - 1) / strip) * a->D * (a->W + 1) * 4);
 }
 
@@ -304,7 +397,7 @@ extern "C" int wkv_causal_conv_backward(const wkv_causal_conv_args_t *a, void *s
         ConvArgs k = conv_args(a);
         k.gy = a->gy; k.gs_out = a->gstate_out; k.gx = a->gx; k.gs_in = a->gstate_in;
         k.vec = conv_vec(a, {a->x, a->state_in, a->gy, a->gstate_out, a->gx, a->gstate_in});
-        k.strip = strip_for(a->B, a->T, a->D, BWD_V, 256);
+        k.strip = strip_for(a->B, a->T, a->D, BWD_THREADS, BWD_LONGEST);
         k.nstrip = a->T > 0 ? (a->T + k.strip - 1) / k.strip : 1;
         if (params && a->T > 0) {
             if (!a->workspace || a->workspace_bytes < wkv_causal_conv_backward_workspace(a)) return WKV_ERR_WORKSPACE;
@@ -312,11 +405,14 @@ extern "C" int wkv_causal_conv_backward(const wkv_causal_conv_args_t *a, void *s
             k.part = (float *)a->workspace;
             rows = a->B * k.nstrip;
         }
-        const int runs = (a->D + BWD_V - 1) / BWD_V, nt = runs >= 256 ? 256 : (runs + 31) / 32 * 32;
+        const int runs = (a->D + V - 1) / V, nt = threads_for(runs, (long long)a->B * k.nstrip);
         e = by_dtype(a->dtype, [&](auto f) {
             using F = decltype(f);
             return by_width(a->W, [&](auto w) {
-                return launch_chained(k_conv_bwd<F, decltype(w)::value>, dim3(a->B * k.nstrip, (runs + nt - 1) / nt), dim3(nt), 0, s, k);
+                constexpr auto kern = k_conv_bwd<F, decltype(w)::value>;
+                static unsigned char done[64];
+                if (!set_max_smem_once(kern, 256 * BwdRing<F>::BYTES, done)) return (int)WKV_ERR_LAUNCH;
+                return launch_chained(kern, dim3(a->B * k.nstrip, (runs + nt - 1) / nt), dim3(nt), nt * BwdRing<F>::BYTES, s, k);
             });
         });
         if (e != WKV_OK) return e;
