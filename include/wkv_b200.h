@@ -311,7 +311,7 @@ int wkv_rms_norm_backward(const wkv_rms_norm_args_t *a, void *stream);
  *   x [B,T,D] with strides x_batch, x_token (elements, channels adjacent); weight [D,W], bias
  *   [D] (or NULL) in w_dtype; state_in [B,W-1,D] (or NULL: zeros) the inputs before the first
  *   token, state_out the last W-1 inputs.  state_out may be state_in's memory for calls of at
- *   most 16 tokens.  Gradients: gx [B,T,D], gweight, gbias in w_dtype, gstate_in. */
+ *   most 16 tokens.  Gradients: gx [B,T,D], gweight, gbias in w_dtype, gstate_in.  D is at most 2^22. */
 typedef struct wkv_causal_conv_args {
     int B, T, D, W;
     int dtype, w_dtype, silu;
@@ -338,7 +338,7 @@ int wkv_causal_conv_backward(const wkv_causal_conv_args_t *a, void *stream);
  *   in parallel; the workspace sizes depend on it.  ckpt (wkv_selective_scan_ckpt_bytes()):
  *   the state at every 16th token, left by the forward call for the backward call, which
  *   needs it.  Gradients: gu, gdelta, gz [B,T,D], gB, gC [B,T,G,N] in dtype; gA, gD, gbias,
- *   gstate_in fp32. */
+ *   gstate_in fp32.  Token strides and D are at most 2^26, B D (T/16 + 1) and B T G less than 2^31. */
 typedef struct wkv_selective_scan_args {
     int B, T, D, N, G;
     int dtype, softplus, time_groups;

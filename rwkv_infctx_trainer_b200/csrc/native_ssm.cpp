@@ -89,7 +89,9 @@ struct RmsNormBackward : OpNode {
     variable_list apply(variable_list &&grads) override {
         at::AutoDispatchBelowADInplaceOrView below;
         const variable_list st = unpack();
-        const Tensor &weight = st[0], &x = st[1], &residual = st[2], &kept = st[3];
+        // (a saved-tensor hook may hand back another layout)
+        auto again = [](const Tensor &t) { return t.defined() ? contig(t) : t; };
+        const Tensor weight = again(st[0]), x = again(st[1]), residual = again(st[2]), kept = again(st[3]);
         const Tensor &h = kept.defined() ? kept : residual.defined() ? residual : x;      // (of h's size and type)
         c10::cuda::OptionalCUDAGuard guard(h.device());
         const Tensor gy = grads[0].defined() ? as_contig(grads[0], x_type) : Tensor();
@@ -349,7 +351,8 @@ struct SelectiveScanBackward : OpNode {
     variable_list apply(variable_list &&grads) override {
         at::AutoDispatchBelowADInplaceOrView below;
         const variable_list st = unpack();
-        const Tensor &u = st[0], &A = st[2], &Bm = st[3], &ckpt = st[8];
+        const Tensor &u = st[0], &A = st[2], &Bm = st[3];
+        const Tensor ckpt = st[8].defined() ? contig(st[8]) : st[8];
         c10::cuda::OptionalCUDAGuard guard(u.device());
         ScanCall c = scan_call(u, st[1], A, Bm, st[4], st[5], st[6], st[7], Tensor(), softplus);
         const auto dt = u.scalar_type();

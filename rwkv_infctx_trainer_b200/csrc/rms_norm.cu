@@ -13,7 +13,7 @@
 // All are bound by HBM: a row crosses once per pass, a thread owns runs of 8 channels and keeps them in registers from
 // the sum to the output.  A CTA takes every gridDim-th row, so that the weights (and the sums of their gradient) stay in
 // registers.  Sums are fp32 and in a fixed order.  16384 rows of 4096 bf16 channels with a bf16 residual: forward 90 us (6.0 TB/s),
-// backward 138 (4.9 TB/s of its 10 bytes a channel).
+// backward 128 (5.2 TB/s of its 10 bytes a channel).
 #include <cuda_fp8.h>
 
 #include "elem_io.cuh"
@@ -183,6 +183,27 @@ __global__ void __launch_bounds__(MAXT, 1024 / MAXT) k_rms_norm_fwd(NormArgs a) 
     }
 }
 
+// A run of channels of a row on its way to a thread's own place in shared memory (nobody else reads it), where `vec`; else it
+// passes through registers.
+template <typename T>
+__device__ __forceinline__ void run_async(Raw<T, RUN> *to, const T *p, bool vec, int n) {
+    if (vec) {
+        const uint32_t dst = (uint32_t)__cvta_generic_to_shared(to);
+#pragma unroll
+        for (int i = 0; i < (int)sizeof(*to); i += 16)
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst + i), "l"((const char *)p + i) : "memory");
+    } else {
+        Raw<T, RUN> r;
+        r.load(p, false, n);
+        *to = r;
+    }
+}
+template <int LEFT>
+__device__ __forceinline__ void rows_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(LEFT) : "memory"); }
+__device__ __forceinline__ void rows_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+// rows on their way, for 1024 threads an SM with `bytes` of a row each: what fits in 200 KB, three at most
+constexpr int rows_ahead(int bytes) { return 200 / bytes > 3 ? 3 : 200 / bytes < 1 ? 1 : 200 / bytes; }
+
 struct NormBwdArgs {
     const void *h, *x, *res, *w, *gy, *gh;         // h, or x and the residual
     void *gx, *gres;
@@ -193,6 +214,13 @@ struct NormBwdArgs {
 };
 
 // SUM: h = x + residual (or x alone), else h is read
+template <typename X, typename R, int NV, bool SUM>
+struct BwdPlace {
+    // (gy, x; h or the residual, gh -- the last passes through registers where threads have two runs: fp32 rows of 16384 channels
+    // are 192 KB without it)
+    static constexpr int TX = SUM ? 2 : 1, TR = NV == 1 ? 2 : 1;
+    static constexpr int ROW = NV * RUN * (int)(TX * sizeof(X) + TR * sizeof(R)), AHEAD = rows_ahead(ROW);
+};
 template <typename X, typename R, int NV, int MAXT, bool SUM>
 __global__ void __launch_bounds__(MAXT, 1024 / MAXT) k_rms_norm_bwd(NormBwdArgs a) {
     pdl_wait();
@@ -211,42 +239,60 @@ __global__ void __launch_bounds__(MAXT, 1024 / MAXT) k_rms_norm_bwd(NormBwdArgs 
 #pragma unroll
         for (int q = 0; q < RUN; q++) { w[i][q] = q < left[i] ? param_at(a.w, a.w_dtype, c + q) : 0.f; gw[i][q] = 0.f; }
     }
-    Raw<R, RUN> rh[NV], rg[NV];
-    Raw<X, RUN> ry[NV], rx[SUM ? NV : 1];
-    auto fetch = [&](long long row) {
+    using Place = BwdPlace<X, R, NV, SUM>;
+    constexpr int AHEAD = Place::AHEAD, TX = Place::TX, TR = Place::TR;
+    extern __shared__ __align__(16) char smem_raw[];
+    Raw<X, RUN> *sx = reinterpret_cast<Raw<X, RUN> *>(smem_raw) + tid;                   // [AHEAD][NV][gy, x][threads]
+    Raw<R, RUN> *sr = reinterpret_cast<Raw<R, RUN> *>(smem_raw + (size_t)AHEAD * NV * TX * nt * sizeof(Raw<X, RUN>)) + tid;     // [..][h, gh]
+    auto fetch = [&](long long row, int slot) {
+        if (row < a.rows) {
 #pragma unroll
-        for (int i = 0; i < NV; i++) {
-            const size_t at = (size_t)row * C + (size_t)(tid + i * nt) * RUN;
-            rh[i].zero(); rg[i].zero(); ry[i].zero();
-            if (SUM) rx[i].zero();
-            if (left[i] > 0) {
-                if (h) rh[i].load(h + at, vec, left[i]);
-                if (SUM) rx[i].load(x + at, vec, left[i]);
-                if (gy) ry[i].load(gy + at, vec, left[i]);
-                if (gh) rg[i].load(gh + at, vec, left[i]);
+            for (int i = 0; i < NV; i++) {
+                const size_t at = (size_t)row * C + (size_t)(tid + i * nt) * RUN;
+                const int k = slot * NV + i;
+                if (left[i] > 0) {
+                    if (h) run_async(sr + (TR * k) * nt, h + at, vec, left[i]);
+                    if (TR == 2 && gh) run_async(sr + (TR * k + 1) * nt, gh + at, vec, left[i]);
+                    if (gy) run_async(sx + (TX * k) * nt, gy + at, vec, left[i]);
+                    if (SUM) run_async(sx + (TX * k + 1) * nt, x + at, vec, left[i]);
+                }
             }
         }
+        rows_commit();
     };
-    int par = 0;
+#pragma unroll
+    for (int k = 0; k < AHEAD; k++) fetch(blockIdx.x + (long long)k * gridDim.x, k);
+    int par = 0, slot = 0;
     for (long long row = blockIdx.x; row < a.rows; row += gridDim.x, par ^= 1) {
-        fetch(row);
+        rows_wait<AHEAD - 1>();
         float hv[NV][RUN], g[NV][RUN];
         float2 s = make_float2(0.f, 0.f);       // sum h^2, sum gy w h
         Raw<R, RUN> keep[NV];
 #pragma unroll
         for (int i = 0; i < NV; i++) {
-            rh[i].get(hv[i]);
-            ry[i].get(g[i]);
-            if (SUM) {
-                float t[RUN];
-                rx[i].get(t);
+            const int k = slot * NV + i;
 #pragma unroll
-                for (int q = 0; q < RUN; q++) hv[i][q] += t[q];
+            for (int q = 0; q < RUN; q++) { hv[i][q] = 0.f; g[i][q] = 0.f; }
+            keep[i].zero();
+            if (left[i] > 0) {
+                if (h) sr[(TR * k) * nt].get(hv[i]);
+                if (gh) {
+                    if (TR == 2) keep[i] = sr[(TR * k + 1) * nt];
+                    else keep[i].load(gh + (size_t)row * C + (size_t)(tid + i * nt) * RUN, vec, left[i]);
+                }
+                if (gy) sx[(TX * k) * nt].get(g[i]);
+                if (SUM) {
+                    float t[RUN];
+                    sx[(TX * k + 1) * nt].get(t);
+#pragma unroll
+                    for (int q = 0; q < RUN; q++) hv[i][q] += t[q];
+                }
             }
-            keep[i] = rg[i];
 #pragma unroll
             for (int q = 0; q < RUN; q++) { s.x += hv[i][q] * hv[i][q]; s.y += g[i][q] * w[i][q] * hv[i][q]; }
         }
+        fetch(row + (long long)AHEAD * gridDim.x, slot);
+        slot = slot + 1 == AHEAD ? 0 : slot + 1;
         s = cta_sum2(s, red[par], nwarp);
         const float r = rsqrtf(s.x / (float)C + a.eps), m = s.y * r / (float)C;      // m = mean(gy w xh)
 #pragma unroll
@@ -277,9 +323,9 @@ __global__ void __launch_bounds__(MAXT, 1024 / MAXT) k_rms_norm_bwd(NormBwdArgs 
 
 constexpr int MAX_C = 16384;
 // How a row is divided: runs a thread, threads, CTAs for all SMs.  All kernels keep to 64 registers, 1024 threads an SM: with
-// several CTAs there one loads while another sums or stores.  (Twice the registers and the next row fetched ahead, us: forward 98 instead of
-// 90, 8-bit output of 1999 x 5120 33 instead of 29; backward 134 instead of 138, of 20000 x 1024 70 instead of 56.  One run a
-// thread forward: 111.)
+// several CTAs there one loads while another sums or stores.  (Us: forward with twice the registers and the next row fetched ahead 98
+// instead of 90, 8-bit output of 1999 x 5120 33 instead of 29; one run a thread 111.  Backward without rows on their way in shared
+// memory 136 instead of 128, of 8192 x 8192 148 instead of 132; forward with them 97.)
 struct Split {
     int nv, threads, ctas;
 };
@@ -294,6 +340,13 @@ Split split_of(long long rows, int C, int nv) {
 }
 Split forward_split(long long rows, int C) { return split_of(rows, C, 2); }
 Split backward_split(long long rows, int C) { return split_of(rows, C, C <= 8192 ? 1 : 2); }
+
+template <auto KERN, class Args>
+int run(const Args &k, const Split &sp, int smem, cudaStream_t s) {
+    static unsigned char done[64];
+    if (!set_max_smem_once(KERN, 227 * 1024 - 1024, done)) return WKV_ERR_LAUNCH;
+    return launch_chained(KERN, dim3(sp.ctas), dim3(sp.threads), smem, s, k);
+}
 
 int check_norm(const wkv_rms_norm_args_t *a) {
     if (!a) return WKV_ERR_NULL;
@@ -339,9 +392,9 @@ extern "C" int wkv_rms_norm_forward(const wkv_rms_norm_args_t *a, void *stream) 
     return by_types(a->dtype, a->res_dtype, [&](auto x, auto r) {
         using X = decltype(x);
         using R = decltype(r);
-        const auto run = [&](auto kern) { return launch_chained(kern, dim3(sp.ctas), dim3(sp.threads), 0, s, k); };
-        if (sp.threads <= 512) return k.scale ? run(k_rms_norm_fwd<X, R, 2, 512, true>) : run(k_rms_norm_fwd<X, R, 2, 512, false>);
-        return k.scale ? run(k_rms_norm_fwd<X, R, 2, 1024, true>) : run(k_rms_norm_fwd<X, R, 2, 1024, false>);
+        const auto go = [&](auto kern) { return launch_chained(kern, dim3(sp.ctas), dim3(sp.threads), 0, s, k); };
+        if (sp.threads <= 512) return k.scale ? go(k_rms_norm_fwd<X, R, 2, 512, true>) : go(k_rms_norm_fwd<X, R, 2, 512, false>);
+        return k.scale ? go(k_rms_norm_fwd<X, R, 2, 1024, true>) : go(k_rms_norm_fwd<X, R, 2, 1024, false>);
     });
 }
 
@@ -370,10 +423,17 @@ extern "C" int wkv_rms_norm_backward(const wkv_rms_norm_args_t *a, void *stream)
         e = by_types(a->dtype, a->res_dtype, [&](auto x, auto r) {
             using X = decltype(x);
             using R = decltype(r);
-            const auto run = [&](auto kern) { return launch_chained(kern, dim3(sp.ctas), dim3(sp.threads), 0, s, k); };
-            if (sp.nv == 2) return k.h ? run(k_rms_norm_bwd<X, R, 2, 1024, false>) : run(k_rms_norm_bwd<X, R, 2, 1024, true>);
-            if (sp.threads <= 512) return k.h ? run(k_rms_norm_bwd<X, R, 1, 512, false>) : run(k_rms_norm_bwd<X, R, 1, 512, true>);
-            return k.h ? run(k_rms_norm_bwd<X, R, 1, 1024, false>) : run(k_rms_norm_bwd<X, R, 1, 1024, true>);
+            const auto go = [&](auto sum) {
+                constexpr bool SUM = decltype(sum)::value;
+                using P1 = BwdPlace<X, R, 1, SUM>;
+                if (sp.nv == 2) {
+                    using P2 = BwdPlace<X, R, 2, SUM>;
+                    return run<k_rms_norm_bwd<X, R, 2, 1024, SUM>>(k, sp, sp.threads * P2::ROW * P2::AHEAD, s);
+                }
+                const int smem = sp.threads * P1::ROW * P1::AHEAD;
+                return sp.threads <= 512 ? run<k_rms_norm_bwd<X, R, 1, 512, SUM>>(k, sp, smem, s) : run<k_rms_norm_bwd<X, R, 1, 1024, SUM>>(k, sp, smem, s);
+            };
+            return k.h ? go(std::false_type{}) : go(std::true_type{});
         });
         if (e != WKV_OK) return e;
     }

@@ -173,6 +173,10 @@ def test_error_codes_without_gpu():
     assert lib.wkv_causal_conv_backward(ref(a), None) == 5
     a.x_token = -1
     assert lib.wkv_causal_conv_forward(ref(a), None) == 2
+    a.x_token, a.D = 8, (1 << 22) + 1
+    assert lib.wkv_causal_conv_forward(ref(a), None) == 2
+    a.D, a.B, a.T = 8, 1 << 20, 1 << 20
+    assert lib.wkv_causal_conv_forward(ref(a), None) == 2
     a = L.CausalConvArgs(W=4)
     assert lib.wkv_causal_conv_forward(ref(a), None) == 0
 
@@ -193,6 +197,10 @@ def test_error_codes_without_gpu():
     a.ckpt, a.ckpt_bytes = at, 16
     assert lib.wkv_selective_scan_forward(ref(a), None) == 5
     a.time_groups = -1
+    assert lib.wkv_selective_scan_forward(ref(a), None) == 2
+    a.time_groups, a.u_token = 0, 1 << 27                       # offsets inside a block of tokens are 32-bit
+    assert lib.wkv_selective_scan_forward(ref(a), None) == 2
+    a.u_token, a.T, a.B = 8, 1 << 30, 64
     assert lib.wkv_selective_scan_forward(ref(a), None) == 2
     a = L.SelectiveScanArgs(N=16, G=1)
     assert lib.wkv_selective_scan_forward(ref(a), None) == 0
