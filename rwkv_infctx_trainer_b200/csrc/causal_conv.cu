@@ -16,9 +16,9 @@ namespace {
 
 constexpr int MAX_W = 4, MAX_D = 1 << 22, SHORTEST = 16;            // (SHORTEST: tokens of a strip at least)
 constexpr int V = 4;                     // channels of a thread
-// Tokens of a group and groups on their way (us forward, 4 rows of 4096 tokens and channels: 8 x 2 79, 4 x 4 80, 2 x 8 66, 1 x 16 115;
-// backward: 4 x 4 157, 3 x 4 149, 2 x 6 165): small groups leave registers for more threads.
-constexpr int FWD_GT = 2, FWD_AHEAD = 8, BWD_GT = 3, BWD_AHEAD = 4;
+// Tokens of a group and groups on their way (us forward, 4 rows of 4096 tokens and channels: 6 x 3 63, 4 x 4 59, 4 x 3 57, 2 x 8 59;
+// backward: 6 x 2 140, 3 x 6 124, 3 x 4 122, 3 x 3 120): small groups leave registers for more threads.
+constexpr int FWD_GT = 4, FWD_AHEAD = 3, BWD_GT = 3, BWD_AHEAD = 3;
 
 struct ConvArgs {
     int B, T, D, w_dtype, silu;
@@ -28,14 +28,14 @@ struct ConvArgs {
     const void *gy, *gs_out;
     void *gx, *gs_in;
     float *part;                         // [B * strips of a row, D * (W + 1)]
-    int strip, nstrip, vec, vec_w;
+    int strip, nstrip, vec_w;
 };
 
 // inputs of the row at time t: from the state below zero (zeros without one)
-template <typename F, int W>
+template <typename F, int W, bool VEC>
 __device__ __forceinline__ void input_at(const ConvArgs &a, int b, int c, int n, int t, Raw<F, V> &r) {
-    if (t >= 0) r.load((const F *)a.x + (size_t)b * a.x_batch + (size_t)t * a.x_token + c, a.vec, n);
-    else if (a.state_in) r.load((const F *)a.state_in + ((size_t)b * (W - 1) + (W - 1 + t)) * a.D + c, a.vec, n);
+    if (t >= 0) r.load((const F *)a.x + (size_t)b * a.x_batch + (size_t)t * a.x_token + c, VEC, n);
+    else if (a.state_in) r.load((const F *)a.state_in + ((size_t)b * (W - 1) + (W - 1 + t)) * a.D + c, VEC, n);
     else r.zero();
 }
 
@@ -80,24 +80,28 @@ __device__ __forceinline__ float rcp(float x) {
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
 __device__ __forceinline__ f2 sigmoid2(f2 x) {
-    const f2 t = mul2(x, both(-1.4426950408889634f));
-    return make_float2(rcp(1.f + exp2f(t.x)), rcp(1.f + exp2f(t.y)));
+    const f2 t = mul2(x, both(-1.4426950408889634f)), d = add2(make_float2(ex2(t.x), ex2(t.y)), both(1.f));
+    return make_float2(rcp(d.x), rcp(d.y));
 }
 
 // A thread's inputs on their way: a ring of AHEAD groups of GT tokens of N tensors in shared memory, a place of its own for
-// each thread (nobody else reads it: no barriers).  Held in registers instead, two groups were as many as fit: 78 us instead of 66
-// forward, 218 instead of 149 backward for 4 rows of 4096 tokens and channels.
-template <typename F, int GT, int N, int AHEAD>
+// each thread (nobody else reads it: no barriers).  Held in registers instead, two groups were as many as fit: 4 rows of 4096 tokens
+// and channels took 78 us forward and 218 backward, with the ring 66 and 149.  Most groups are whole and inside the strip: those
+// run without a look at each token, and aligned rows (VEC) are compiled apart: 57 and 120 us.
+template <typename F, int GT, int N, int AHEAD, bool VEC>
 struct Ring {
-    Raw<F, V> *mine;
-    bool vec;
-    int n;
-    static constexpr int BYTES = AHEAD * GT * N * (int)sizeof(Raw<F, V>);        // a thread
-    __device__ __forceinline__ Raw<F, V> &at(int group, int i, int k) { return mine[(((group % AHEAD) * GT + i) * N + k) * blockDim.x]; }
-    __device__ __forceinline__ void load(int group, int i, int k, const F *p) {
-        Raw<F, V> &to = at(group, i, k);
-        if (vec) {
+    Raw<F, V> *mine;                     // [AHEAD][GT][N][threads]
+    int threads, n, in = 0, out = 0;     // the groups to be filled and to be read
+    __device__ __forceinline__ Raw<F, V> &at(int group, int i, int k) const { return mine[((group * GT + i) * N + k) * threads]; }
+    __device__ __forceinline__ void load(int i, int k, const F *p) {
+        Raw<F, V> &to = at(in, i, k);
+        if (VEC) {
             const uint32_t dst = (uint32_t)__cvta_generic_to_shared(&to);
             if constexpr (sizeof(to) == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(p) : "memory");
             else asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(dst), "l"(p) : "memory");
@@ -107,17 +111,21 @@ struct Ring {
             to = r;
         }
     }
-    __device__ __forceinline__ void commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-    // all but the last AHEAD - 1 groups have arrived
+    __device__ __forceinline__ void commit() {
+        asm volatile("cp.async.commit_group;" ::: "memory");
+        in = in + 1 == AHEAD ? 0 : in + 1;
+    }
+    // the next group to be read has arrived
     __device__ __forceinline__ void wait() { asm volatile("cp.async.wait_group %0;" ::"n"(AHEAD - 1) : "memory"); }
+    __device__ __forceinline__ void next() { out = out + 1 == AHEAD ? 0 : out + 1; }
 };
-template <typename F>
-using FwdRing = Ring<F, FWD_GT, 1, FWD_AHEAD>;
-template <typename F>
-using BwdRing = Ring<F, BWD_GT, 2, BWD_AHEAD>;
+template <typename F, bool VEC>
+using FwdRing = Ring<F, FWD_GT, 1, FWD_AHEAD, VEC>;
+template <typename F, bool VEC>
+using BwdRing = Ring<F, BWD_GT, 2, BWD_AHEAD, VEC>;
 
 // blockIdx.x: (row, strip), blockIdx.y: runs of channels
-template <typename F, int W>
+template <typename F, int W, bool VEC>
 __global__ void __launch_bounds__(256) k_conv_fwd(ConvArgs a) {
     pdl_wait();
     pdl_trigger();
@@ -127,32 +135,39 @@ __global__ void __launch_bounds__(256) k_conv_fwd(ConvArgs a) {
     if (c >= a.D) return;
     const int n = min(V, a.D - c), b = blockIdx.x / a.nstrip, t0 = (blockIdx.x - b * a.nstrip) * a.strip;
     const int t1 = min(t0 + a.strip, a.T);
-    FwdRing<F> ring = {reinterpret_cast<Raw<F, V> *>(smem_raw) + threadIdx.x, (bool)a.vec, n};
-    const F *px = (const F *)a.x + (size_t)b * a.x_batch + c;
-    auto fetch = [&](int group) {
+    FwdRing<F, VEC> ring = {reinterpret_cast<Raw<F, V> *>(smem_raw) + threadIdx.x, (int)blockDim.x, n};
+    const F *px = (const F *)a.x + (size_t)b * a.x_batch + (size_t)t0 * a.x_token + c;
+    int left = t1 - t0;                  // tokens that are still to be fetched
+    auto fetch = [&]() {
+        if (left >= GT) {
 #pragma unroll
-        for (int i = 0; i < GT; i++) {
-            const int t = t0 + group * GT + i;
-            if (t < t1) ring.load(group, i, 0, px + (size_t)t * a.x_token);
+            for (int i = 0; i < GT; i++) ring.load(i, 0, px + i * a.x_token);
+        } else {
+#pragma unroll
+            for (int i = 0; i < GT; i++)
+                if (i < left) ring.load(i, 0, px + i * a.x_token);
         }
         ring.commit();
+        px += GT * a.x_token;
+        left -= GT;
     };
 #pragma unroll
-    for (int g = 0; g < FWD_AHEAD; g++) fetch(g);
+    for (int g = 0; g < FWD_AHEAD; g++) fetch();
     f2 w[W][2], bias[2], x[W - 1 + GT][2];
     load_params<W>(a, c, n, w, bias);
 #pragma unroll
     for (int j = 0; j < W - 1; j++) {
         Raw<F, V> r;
-        input_at<F, W>(a, b, c, n, t0 - (W - 1) + j, r);
+        input_at<F, W, VEC>(a, b, c, n, t0 - (W - 1) + j, r);
         get_pairs(r, x[j]);
     }
-    F *y = (F *)a.y + ((size_t)b * a.T) * a.D + c;
-    for (int t = t0, group = 0; t < t1; t += GT, group++) {
+    F *y = (F *)a.y + ((size_t)b * a.T + t0) * a.D + c;
+    auto group = [&](auto whole, int count) {
         ring.wait();
 #pragma unroll
-        for (int i = 0; i < GT; i++) get_pairs(ring.at(group, i, 0), x[W - 1 + i]);
-        fetch(group + FWD_AHEAD);
+        for (int i = 0; i < GT; i++) get_pairs(ring.at(ring.out, i, 0), x[W - 1 + i]);
+        ring.next();
+        fetch();
 #pragma unroll
         for (int i = 0; i < GT; i++) {
             f2 s[2] = {bias[0], bias[1]};
@@ -164,31 +179,34 @@ __global__ void __launch_bounds__(256) k_conv_fwd(ConvArgs a) {
 #pragma unroll
                 for (int p = 0; p < 2; p++) s[p] = mul2(s[p], sigmoid2(s[p]));
             }
-            if (t + i < t1) put_pairs<F>(s).store(y + (size_t)(t + i) * a.D, a.vec, n);
+            if (decltype(whole)::value || i < count) put_pairs<F>(s).store(y + (size_t)i * a.D, VEC, n);
         }
+        y += (size_t)GT * a.D;
         // the last W-1 inputs that exist move to the front
-        const int k = min(GT, t1 - t);
 #pragma unroll
         for (int j = 0; j < W - 1; j++) {
             f2 l[2] = {x[GT + j][0], x[GT + j][1]};
-            if (k < GT) {
+            if (!decltype(whole)::value) {
 #pragma unroll
                 for (int i = 1; i < GT; i++)
-                    if (i == k) { l[0] = x[i + j][0]; l[1] = x[i + j][1]; }
+                    if (i == count) { l[0] = x[i + j][0]; l[1] = x[i + j][1]; }
             }
             x[j][0] = l[0];
             x[j][1] = l[1];
         }
-    }
+    };
+    int t = t0;
+    for (; t + GT <= t1; t += GT) group(std::true_type{}, GT);
+    if (t < t1) group(std::false_type{}, t1 - t);
     if (t1 == a.T && a.state_out) {
 #pragma unroll
-        for (int j = 0; j < W - 1; j++) put_pairs<F>(x[j]).store((F *)a.state_out + ((size_t)b * (W - 1) + j) * a.D + c, a.vec, n);
+        for (int j = 0; j < W - 1; j++) put_pairs<F>(x[j]).store((F *)a.state_out + ((size_t)b * (W - 1) + j) * a.D + c, VEC, n);
     }
 }
 
 // A thread walks its strip forward, W-1 tokens past its end, in groups: it forms s and ds of a group's tokens, adds to the sums
 // of the parameters' gradients where they are its own, and hands out gx of the tokens W-1 earlier, which is complete then.
-template <typename F, int W>
+template <typename F, int W, bool VEC>
 __global__ void __launch_bounds__(256) k_conv_bwd(ConvArgs a) {
     pdl_wait();
     pdl_trigger();
@@ -197,22 +215,34 @@ __global__ void __launch_bounds__(256) k_conv_bwd(ConvArgs a) {
     const int c = (blockIdx.y * blockDim.x + threadIdx.x) * V;
     if (c >= a.D) return;
     const int n = min(V, a.D - c), b = blockIdx.x / a.nstrip, t0 = (blockIdx.x - b * a.nstrip) * a.strip;
-    const int t1 = min(t0 + a.strip, a.T), stop = t1 + W - 1, some = min(stop, a.T);
-    BwdRing<F> ring = {reinterpret_cast<Raw<F, V> *>(smem_raw) + threadIdx.x, (bool)a.vec, n};
-    const F *px = (const F *)a.x + (size_t)b * a.x_batch + c, *gy = (const F *)a.gy + ((size_t)b * a.T) * a.D + c;
-    auto fetch = [&](int group) {
+    const int t1 = min(t0 + a.strip, a.T), stop = t1 + W - 1;
+    BwdRing<F, VEC> ring = {reinterpret_cast<Raw<F, V> *>(smem_raw) + threadIdx.x, (int)blockDim.x, n};
+    const F *px = (const F *)a.x + (size_t)b * a.x_batch + (size_t)t0 * a.x_token + c, *gy = (const F *)a.gy + ((size_t)b * a.T + t0) * a.D + c;
+    int left = min(stop, a.T) - t0;
+    auto fetch = [&]() {
+        if (left >= GT) {
 #pragma unroll
-        for (int i = 0; i < GT; i++) {
-            const int t = t0 + group * GT + i;
-            if (t < some) {
-                ring.load(group, i, 0, px + (size_t)t * a.x_token);
-                if (a.gy) ring.load(group, i, 1, gy + (size_t)t * a.D);
+            for (int i = 0; i < GT; i++) ring.load(i, 0, px + i * a.x_token);
+            if (a.gy) {
+#pragma unroll
+                for (int i = 0; i < GT; i++) ring.load(i, 1, gy + (size_t)i * a.D);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < GT; i++) {
+                if (i < left) {
+                    ring.load(i, 0, px + i * a.x_token);
+                    if (a.gy) ring.load(i, 1, gy + (size_t)i * a.D);
+                }
             }
         }
         ring.commit();
+        px += GT * a.x_token;
+        gy += (size_t)GT * a.D;
+        left -= GT;
     };
 #pragma unroll
-    for (int g = 0; g < BWD_AHEAD; g++) fetch(g);
+    for (int g = 0; g < BWD_AHEAD; g++) fetch();
     f2 w[W][2], bias[2], gw[W][2], gb[2] = {both(0.f), both(0.f)};
     f2 x[W - 1 + GT][2], ds[W - 1 + GT][2];              // of tokens t-W+1 .. t+GT-1
     load_params<W>(a, c, n, w, bias);
@@ -221,37 +251,44 @@ __global__ void __launch_bounds__(256) k_conv_bwd(ConvArgs a) {
 #pragma unroll
     for (int j = 0; j < W - 1; j++) {
         Raw<F, V> r;
-        input_at<F, W>(a, b, c, n, t0 - (W - 1) + j, r);
+        input_at<F, W, VEC>(a, b, c, n, t0 - (W - 1) + j, r);
         get_pairs(r, x[j]);
         ds[j][0] = ds[j][1] = both(0.f);
     }
     // (of the tokens before the strip only the first strip's, the state, are its own)
     const int first = t0 == 0 ? -(W - 1) : t0;
-    for (int t = t0, group = 0; t < stop; t += GT, group++) {
+    F *gx = (F *)a.gx + ((size_t)b * a.T + t0) * a.D + c - (long long)(W - 1) * a.D;      // of token t-W+1
+    // inside: the group's tokens are the strip's own, and so are those W-1 earlier
+    auto group = [&](auto inside, int t) {
+        constexpr bool IN = decltype(inside)::value;
         ring.wait();
 #pragma unroll
         for (int i = 0; i < GT; i++) {
-            get_pairs(ring.at(group, i, 0), x[W - 1 + i]);
-            if (a.gy) get_pairs(ring.at(group, i, 1), ds[W - 1 + i]);
+            get_pairs(ring.at(ring.out, i, 0), x[W - 1 + i]);
+            if (a.gy) get_pairs(ring.at(ring.out, i, 1), ds[W - 1 + i]);
             else ds[W - 1 + i][0] = ds[W - 1 + i][1] = both(0.f);
         }
-        fetch(group + BWD_AHEAD);
+        ring.next();
+        fetch();
+        if (a.silu) {
 #pragma unroll
-        for (int i = 0; i < GT; i++) {
-            f2(&d)[2] = ds[W - 1 + i];
-            if (a.silu) {
+            for (int i = 0; i < GT; i++)
 #pragma unroll
                 for (int p = 0; p < 2; p++) {
                     f2 s = bias[p];
 #pragma unroll
                     for (int j = 0; j < W; j++) s = fma2(w[j][p], x[i + j][p], s);
                     const f2 sg = sigmoid2(s);
-                    d[p] = mul2(d[p], mul2(sg, fma2(s, sub2(both(1.f), sg), both(1.f))));
+                    // silu'(s) = sg (1 + s (1 - sg)) = sg + s sg - s sg^2
+                    ds[W - 1 + i][p] = mul2(ds[W - 1 + i][p], mul2(sg, fma2(s, sub2(both(1.f), sg), both(1.f))));
                 }
-            }
+        }
+#pragma unroll
+        for (int i = 0; i < GT; i++) {
+            f2(&d)[2] = ds[W - 1 + i];
             // behind the row there is no gradient (zero times what is formed from no inputs may be a NaN)
-            if (t + i >= a.T) d[0] = d[1] = both(0.f);
-            if (t + i < t1) {
+            if (!IN && t + i >= a.T) d[0] = d[1] = both(0.f);
+            if (IN || t + i < t1) {
 #pragma unroll
                 for (int p = 0; p < 2; p++) {
                     gb[p] = add2(gb[p], d[p]);
@@ -260,27 +297,30 @@ __global__ void __launch_bounds__(256) k_conv_bwd(ConvArgs a) {
                 }
             }
             const int to = t + i - (W - 1);       // the token whose gradient is complete
-            if (to >= first && to < t1) {
-                f2 o[2] = {both(0.f), both(0.f)};
+            if (IN || (to >= first && to < t1)) {
+                f2 o[2];
 #pragma unroll
-                for (int j = 0; j < W; j++)
+                for (int p = 0; p < 2; p++) {
+                    o[p] = mul2(w[0][p], ds[W - 1 + i][p]);
 #pragma unroll
-                    for (int p = 0; p < 2; p++) o[p] = fma2(w[j][p], ds[W - 1 + i - j][p], o[p]);
-                if (a.gs_out && to >= a.T - (W - 1)) {        // a token that is part of the state handed on
+                    for (int j = 1; j < W; j++) o[p] = fma2(w[j][p], ds[W - 1 + i - j][p], o[p]);
+                }
+                if (!IN && a.gs_out && to >= a.T - (W - 1)) {        // a token that is part of the state handed on
                     Raw<F, V> r;
                     f2 f[2];
-                    r.load((const F *)a.gs_out + ((size_t)b * (W - 1) + (to - (a.T - (W - 1)))) * a.D + c, a.vec, n);
+                    r.load((const F *)a.gs_out + ((size_t)b * (W - 1) + (to - (a.T - (W - 1)))) * a.D + c, VEC, n);
                     get_pairs(r, f);
                     o[0] = add2(o[0], f[0]);
                     o[1] = add2(o[1], f[1]);
                 }
-                if (to >= 0) {
-                    if (a.gx) put_pairs<F>(o).store((F *)a.gx + ((size_t)b * a.T + to) * a.D + c, a.vec, n);
+                if (IN || to >= 0) {
+                    if (a.gx) put_pairs<F>(o).store(gx + (size_t)i * a.D, VEC, n);
                 } else if (a.gs_in) {
-                    put_pairs<F>(o).store((F *)a.gs_in + ((size_t)b * (W - 1) + (W - 1 + to)) * a.D + c, a.vec, n);
+                    put_pairs<F>(o).store((F *)a.gs_in + ((size_t)b * (W - 1) + (W - 1 + to)) * a.D + c, VEC, n);
                 }
             }
         }
+        gx += (size_t)GT * a.D;
 #pragma unroll
         for (int j = 0; j < W - 1; j++)
 #pragma unroll
@@ -288,7 +328,11 @@ __global__ void __launch_bounds__(256) k_conv_bwd(ConvArgs a) {
                 x[j][p] = x[GT + j][p];
                 ds[j][p] = ds[GT + j][p];
             }
-    }
+    };
+    int t = t0;
+    for (; t < stop && t - (W - 1) < t0; t += GT) group(std::false_type{}, t);
+    for (; t + GT <= t1; t += GT) group(std::true_type{}, t);
+    for (; t < stop; t += GT) group(std::false_type{}, t);
     if (a.part) {
         float *p = a.part + (size_t)blockIdx.x * ((size_t)a.D * (W + 1));
 #pragma unroll
@@ -314,7 +358,7 @@ int check_conv(const wkv_causal_conv_args_t *a) {
 }
 
 // Tokens of a strip: so many strips that the GPU has `threads` an SM, `longest` tokens at most: short ones leave little to hide a
-// load behind, long ones few threads (forward 64 tokens 66 us, 128 80, 32 76; backward 110 tokens 149, 220 171, 64 167).
+// load behind, long ones few threads (us with the ring alone: forward 64 tokens 66, 128 80, 32 76; backward 110 tokens 149, 220 171, 64 167).
 constexpr int FWD_THREADS = 1536, FWD_LONGEST = 64, BWD_THREADS = 1024, BWD_LONGEST = 256;
 int strip_for(int B, int T, int D, int threads, int longest) {
     const long long across = (long long)B * ((D + V - 1) / V), want = (long long)device_sm_count() * threads;
@@ -366,17 +410,18 @@ extern "C" int wkv_causal_conv_forward(const wkv_causal_conv_args_t *a, void *st
     if (a->T > SHORTEST && a->state_in && a->state_in == a->state_out) return WKV_ERR_UNSUPPORTED;
     ConvArgs k = conv_args(a);
     k.y = a->y; k.state_out = a->state_out;
-    k.vec = conv_vec(a, {a->x, a->state_in, a->y, a->state_out});
+    const bool vec = conv_vec(a, {a->x, a->state_in, a->y, a->state_out});
     k.strip = strip_for(a->B, a->T, a->D, FWD_THREADS, FWD_LONGEST);
     k.nstrip = a->T > 0 ? (a->T + k.strip - 1) / k.strip : 1;
     const int runs = (a->D + V - 1) / V, nt = threads_for(runs, (long long)a->B * k.nstrip);
     return by_dtype(a->dtype, [&](auto f) {
         using F = decltype(f);
         return by_width(a->W, [&](auto w) {
-            constexpr auto kern = k_conv_fwd<F, decltype(w)::value>;
-            static unsigned char done[64];
-            if (!set_max_smem_once(kern, 256 * FwdRing<F>::BYTES, done)) return (int)WKV_ERR_LAUNCH;
-            return launch_chained(kern, dim3(a->B * k.nstrip, (runs + nt - 1) / nt), dim3(nt), nt * FwdRing<F>::BYTES, (cudaStream_t)stream, k);
+            const auto kern = vec ? k_conv_fwd<F, decltype(w)::value, true> : k_conv_fwd<F, decltype(w)::value, false>;
+            constexpr int BYTES = FWD_AHEAD * FWD_GT * (int)sizeof(Raw<F, V>);       // a thread's ring
+            static unsigned char done[2][64];
+            if (!set_max_smem_once(kern, 256 * BYTES, done[vec])) return (int)WKV_ERR_LAUNCH;
+            return launch_chained(kern, dim3(a->B * k.nstrip, (runs + nt - 1) / nt), dim3(nt), nt * BYTES, (cudaStream_t)stream, k);
         });
     });
 }
@@ -397,7 +442,7 @@ extern "C" int wkv_causal_conv_backward(const wkv_causal_conv_args_t *a, void *s
     if (!empty) {
         ConvArgs k = conv_args(a);
         k.gy = a->gy; k.gs_out = a->gstate_out; k.gx = a->gx; k.gs_in = a->gstate_in;
-        k.vec = conv_vec(a, {a->x, a->state_in, a->gy, a->gstate_out, a->gx, a->gstate_in});
+        const bool vec = conv_vec(a, {a->x, a->state_in, a->gy, a->gstate_out, a->gx, a->gstate_in});
         k.strip = strip_for(a->B, a->T, a->D, BWD_THREADS, BWD_LONGEST);
         k.nstrip = a->T > 0 ? (a->T + k.strip - 1) / k.strip : 1;
         if (params && a->T > 0) {
@@ -410,10 +455,11 @@ extern "C" int wkv_causal_conv_backward(const wkv_causal_conv_args_t *a, void *s
         e = by_dtype(a->dtype, [&](auto f) {
             using F = decltype(f);
             return by_width(a->W, [&](auto w) {
-                constexpr auto kern = k_conv_bwd<F, decltype(w)::value>;
-                static unsigned char done[64];
-                if (!set_max_smem_once(kern, 256 * BwdRing<F>::BYTES, done)) return (int)WKV_ERR_LAUNCH;
-                return launch_chained(kern, dim3(a->B * k.nstrip, (runs + nt - 1) / nt), dim3(nt), nt * BwdRing<F>::BYTES, s, k);
+                const auto kern = vec ? k_conv_bwd<F, decltype(w)::value, true> : k_conv_bwd<F, decltype(w)::value, false>;
+                constexpr int BYTES = BWD_AHEAD * BWD_GT * 2 * (int)sizeof(Raw<F, V>);       // a thread's ring
+                static unsigned char done[2][64];
+                if (!set_max_smem_once(kern, 256 * BYTES, done[vec])) return (int)WKV_ERR_LAUNCH;
+                return launch_chained(kern, dim3(a->B * k.nstrip, (runs + nt - 1) / nt), dim3(nt), nt * BYTES, s, k);
             });
         });
         if (e != WKV_OK) return e;

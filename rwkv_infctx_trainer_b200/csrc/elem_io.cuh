@@ -10,7 +10,7 @@ namespace wkv {
 
 // N consecutive elements as they lie in memory, in whole 32-bit words (N * sizeof(F) is a multiple of 4)
 template <typename F, int N>
-struct Raw {
+struct alignas(N * sizeof(F) < 16 ? N * sizeof(F) : 16) Raw {
     static constexpr int WORDS = N * (int)sizeof(F) / 4;
     uint32_t w[WORDS];
 
