@@ -270,3 +270,37 @@ def test_every_cut_of_a_row_into_spans():
             L.check(getattr(lib, f"wkv_selective_scan_{fn}")(ctypes.byref(a), st), fn)
         torch.cuda.synchronize()
         check(c, out)
+
+
+@pytest.mark.parametrize("softplus", [True, False])
+def test_infinite_steps_gates_and_decays(softplus):
+    """a step of -inf (softplus: 0) leaves the state, an infinite A forgets it, z of +inf lets an infinity through, one of -87 and
+    below closes; a NaN in each reaches its own channel"""
+    c = S.scan_case(11, 1, 20, 16, 16, 1, F32)
+    if not softplus:
+        c["delta"] = c["delta"].abs() * 0.2
+        c["delta_bias"] = c["delta_bias"].abs() * 0.01
+    want = reference(c, softplus, False, False)
+    c["A"][3] = -float("inf")
+    c["z"][0, 5, 4] = float("inf")
+    c["z"][0, 6, 4] = -200.0
+    if softplus:
+        c["delta"][0, 7:, 5] = -float("inf")
+    for n, at in (("delta", (0, 9, 6)), ("z", (0, 9, 7)), ("u", (0, 9, 8))):
+        c[n][at] = float("nan")
+    y, s = call(c, softplus)
+    for t in (1, 10, 19):       # nothing of the tokens before: C . (dt u B) + D u
+        raw = (c["delta"][0, t, 3] + c["delta_bias"][3]).double()
+        dt = torch.nn.functional.softplus(raw) if softplus else raw
+        u, z = c["u"][0, t, 3].double(), c["z"][0, t, 3].double()
+        one = ((c["C"][0, t, 0].double() * c["B"][0, t, 0].double()).sum() * dt * u + c["D"][3].double() * u) * S.silu(z)
+        assert abs(float(y[0, t, 3]) - float(one)) <= 1e-4 * (1 + abs(float(one)))
+    assert torch.isinf(y[0, 5, 4]) and abs(float(y[0, 6, 4])) < 1e-30
+    assert torch.isfinite(s[0, 3]).all() and torch.isfinite(s[0, 4]).all()
+    if softplus:
+        six = S.scan_ref(*(c[n][:, :7] if n in ("u", "delta", "B", "C", "z") else c[n] for n in S.SCAN_LEAVES[:-1]), True, c["state"])["state"]
+        assert float((s[0, 5].double() - six[0, 5]).abs().max()) <= 1e-5 * float(six[0, 5].abs().max())
+    for ch, keeps in ((6, False), (8, False), (7, True)):
+        assert torch.isnan(y[0, 9, ch]) and bool(torch.isfinite(s[0, ch]).all()) == keeps
+    clean = [i for i in range(16) if i not in (3, 4, 5, 6, 7, 8)]
+    assert torch.isfinite(y[..., clean]).all() and float((s[0, clean].double() - want["state"][0, clean]).abs().max()) < 1e-4
