@@ -31,27 +31,72 @@ struct ConvArgs {
     int strip, nstrip, vec_w;
 };
 
+// How rows lie, and a thread's four channels.  RUNS: rows start at multiples of four elements, the channels are neighbours.
+// WORDS: at multiples of 4 bytes, the channels are 4-byte words (two of 16 bits, or one of 32) that are 32 words apart.  ONES: 16-bit
+// rows that start anywhere, single channels 32 apart.  In each a warp's access is one piece of a row.
+enum { RUNS, WORDS, ONES };
+template <typename F, int MODE>
+struct Lie {
+    static constexpr int UNIT = MODE == RUNS ? V : MODE == WORDS ? 4 / (int)sizeof(F) : 1, APART = MODE == RUNS ? V : 32 * UNIT;
+    static __device__ __forceinline__ int first() {
+        const int i = blockIdx.y * blockDim.x + threadIdx.x;
+        return MODE == RUNS ? i * V : (i >> 5) * (32 * V) + (i & 31) * UNIT;
+    }
+    // how many of the channels from c on exist
+    static __device__ __forceinline__ int left(int D, int c) { return MODE == RUNS ? V : min(V, (D - c + APART - 1) / APART * UNIT); }
+    static __device__ __forceinline__ int channel(int c, int q) { return c + q / UNIT * APART + q % UNIT; }
+    static __device__ __forceinline__ void load(Raw<F, V> &r, const F *p, int n) {
+        if constexpr (MODE == RUNS) r.load(p, true, V);
+        else if constexpr (MODE == ONES) r.template gather<32>(p, n);
+        else {
+#pragma unroll
+            for (int i = 0; i < Raw<F, V>::WORDS; i++) r.w[i] = i * UNIT < n ? *reinterpret_cast<const uint32_t *>(p + i * APART) : 0u;
+        }
+    }
+    static __device__ __forceinline__ void store(const Raw<F, V> &r, F *p, int n) {
+        if constexpr (MODE == RUNS) r.store(p, true, V);
+        else if constexpr (MODE == ONES) r.template scatter<32>(p, n);
+        else {
+#pragma unroll
+            for (int i = 0; i < Raw<F, V>::WORDS; i++)
+                if (i * UNIT < n) *reinterpret_cast<uint32_t *>(p + i * APART) = r.w[i];
+        }
+    }
+    // into shared memory without passing through registers (RUNS, WORDS)
+    static __device__ __forceinline__ void load_async(Raw<F, V> &to, const F *p, int n) {
+        const uint32_t dst = (uint32_t)__cvta_generic_to_shared(&to);
+        if constexpr (MODE == RUNS) {
+            if constexpr (sizeof(to) == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(p) : "memory");
+            else asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(dst), "l"(p) : "memory");
+        } else {
+#pragma unroll
+            for (int i = 0; i < Raw<F, V>::WORDS; i++)
+                if (i * UNIT < n) asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst + 4 * i), "l"(p + i * APART) : "memory");
+        }
+    }
+};
+
 // inputs of the row at time t: from the state below zero (zeros without one)
-template <typename F, int W, bool VEC>
+template <typename F, int W, int MODE>
 __device__ __forceinline__ void input_at(const ConvArgs &a, int b, int c, int n, int t, Raw<F, V> &r) {
-    if (t >= 0) r.load((const F *)a.x + (size_t)b * a.x_batch + (size_t)t * a.x_token + c, VEC, n);
-    else if (a.state_in) r.load((const F *)a.state_in + ((size_t)b * (W - 1) + (W - 1 + t)) * a.D + c, VEC, n);
+    if (t >= 0) Lie<F, MODE>::load(r, (const F *)a.x + (size_t)b * a.x_batch + (size_t)t * a.x_token + c, n);
+    else if (a.state_in) Lie<F, MODE>::load(r, (const F *)a.state_in + ((size_t)b * (W - 1) + (W - 1 + t)) * a.D + c, n);
     else r.zero();
 }
 
 // the parameters of a thread's channels: two pairs of channels per tap
-template <int W>
+template <typename F, int W, int MODE>
 __device__ __forceinline__ void load_params(const ConvArgs &a, int c, int n, f2 (&w)[W][2], f2 (&bias)[2]) {
     float t[V][W], bb[V];
 #pragma unroll
     for (int q = 0; q < V; q++) {
-        bb[q] = a.bias && q < n ? param_at(a.bias, a.w_dtype, c + q) : 0.f;
+        bb[q] = a.bias && q < n ? param_at(a.bias, a.w_dtype, Lie<F, MODE>::channel(c, q)) : 0.f;
         if (W == 4 && a.vec_w) {
-            const float4 v = q < n ? __ldg(reinterpret_cast<const float4 *>((const float *)a.w + (size_t)(c + q) * W)) : make_float4(0.f, 0.f, 0.f, 0.f);
+            const float4 v = q < n ? __ldg(reinterpret_cast<const float4 *>((const float *)a.w + (size_t)Lie<F, MODE>::channel(c, q) * W)) : make_float4(0.f, 0.f, 0.f, 0.f);
             t[q][0] = v.x; t[q][1] = v.y; t[q][2 % W] = v.z; t[q][3 % W] = v.w;
         } else {
 #pragma unroll
-            for (int j = 0; j < W; j++) t[q][j] = q < n ? param_at(a.w, a.w_dtype, (size_t)(c + q) * W + j) : 0.f;
+            for (int j = 0; j < W; j++) t[q][j] = q < n ? param_at(a.w, a.w_dtype, (size_t)Lie<F, MODE>::channel(c, q) * W + j) : 0.f;
         }
     }
 #pragma unroll
@@ -93,49 +138,47 @@ __device__ __forceinline__ f2 sigmoid2(f2 x) {
 // A thread's inputs on their way: a ring of AHEAD groups of GT tokens of N tensors in shared memory, a place of its own for
 // each thread (nobody else reads it: no barriers).  Held in registers instead, two groups were as many as fit: 4 rows of 4096 tokens
 // and channels took 78 us forward and 218 backward, with the ring 66 and 149.  Most groups are whole and inside the strip: those
-// run without a look at each token, and aligned rows (VEC) are compiled apart: 57 and 120 us.
-template <typename F, int GT, int N, int AHEAD, bool VEC>
+// run without a look at each token, and the ways that rows lie are compiled apart: 57 and 120 us.  (There are no copies of 2 bytes:
+// ONES has one group on its way, in registers.)
+template <typename F, int GT, int N, int AHEAD, int MODE>
 struct Ring {
     Raw<F, V> *mine;                     // [AHEAD][GT][N][threads]
     int threads, n, in = 0, out = 0;     // the groups to be filled and to be read
+    Raw<F, V> held[MODE != ONES ? 1 : GT * N];   // ONES: one group, in registers
     __device__ __forceinline__ Raw<F, V> &at(int group, int i, int k) const { return mine[((group * GT + i) * N + k) * threads]; }
     __device__ __forceinline__ void load(int i, int k, const F *p) {
-        Raw<F, V> &to = at(in, i, k);
-        if (VEC) {
-            const uint32_t dst = (uint32_t)__cvta_generic_to_shared(&to);
-            if constexpr (sizeof(to) == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(p) : "memory");
-            else asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(dst), "l"(p) : "memory");
-        } else {
-            Raw<F, V> r;
-            r.load(p, false, n);
-            to = r;
-        }
+        if constexpr (MODE != ONES) Lie<F, MODE>::load_async(at(in, i, k), p, n);
+        else Lie<F, MODE>::load(held[i * N + k], p, n);
     }
+    __device__ __forceinline__ const Raw<F, V> &read(int i, int k) const { return MODE != ONES ? at(out, i, k) : held[MODE != ONES ? 0 : i * N + k]; }
     __device__ __forceinline__ void commit() {
+        if (MODE == ONES) return;
         asm volatile("cp.async.commit_group;" ::: "memory");
         in = in + 1 == AHEAD ? 0 : in + 1;
     }
     // the next group to be read has arrived
-    __device__ __forceinline__ void wait() { asm volatile("cp.async.wait_group %0;" ::"n"(AHEAD - 1) : "memory"); }
+    __device__ __forceinline__ void wait() {
+        if (MODE != ONES) asm volatile("cp.async.wait_group %0;" ::"n"(AHEAD - 1) : "memory");
+    }
     __device__ __forceinline__ void next() { out = out + 1 == AHEAD ? 0 : out + 1; }
 };
-template <typename F, bool VEC>
-using FwdRing = Ring<F, FWD_GT, 1, FWD_AHEAD, VEC>;
-template <typename F, bool VEC>
-using BwdRing = Ring<F, BWD_GT, 2, BWD_AHEAD, VEC>;
+template <typename F, int MODE>
+using FwdRing = Ring<F, FWD_GT, 1, FWD_AHEAD, MODE>;
+template <typename F, int MODE>
+using BwdRing = Ring<F, BWD_GT, 2, BWD_AHEAD, MODE>;
 
 // blockIdx.x: (row, strip), blockIdx.y: runs of channels
-template <typename F, int W, bool VEC>
+template <typename F, int W, int MODE>
 __global__ void __launch_bounds__(256) k_conv_fwd(ConvArgs a) {
     pdl_wait();
     pdl_trigger();
     constexpr int GT = FWD_GT;
     extern __shared__ __align__(16) char smem_raw[];
-    const int c = (blockIdx.y * blockDim.x + threadIdx.x) * V;
+    const int c = Lie<F, MODE>::first();
     if (c >= a.D) return;
-    const int n = min(V, a.D - c), b = blockIdx.x / a.nstrip, t0 = (blockIdx.x - b * a.nstrip) * a.strip;
+    const int n = Lie<F, MODE>::left(a.D, c), b = blockIdx.x / a.nstrip, t0 = (blockIdx.x - b * a.nstrip) * a.strip;
     const int t1 = min(t0 + a.strip, a.T);
-    FwdRing<F, VEC> ring = {reinterpret_cast<Raw<F, V> *>(smem_raw) + threadIdx.x, (int)blockDim.x, n};
+    FwdRing<F, MODE> ring = {reinterpret_cast<Raw<F, V> *>(smem_raw) + threadIdx.x, (int)blockDim.x, n};
     const F *px = (const F *)a.x + (size_t)b * a.x_batch + (size_t)t0 * a.x_token + c;
     int left = t1 - t0;                  // tokens that are still to be fetched
     auto fetch = [&]() {
@@ -152,20 +195,20 @@ __global__ void __launch_bounds__(256) k_conv_fwd(ConvArgs a) {
         left -= GT;
     };
 #pragma unroll
-    for (int g = 0; g < FWD_AHEAD; g++) fetch();
+    for (int g = 0; g < (MODE != ONES ? FWD_AHEAD : 1); g++) fetch();
     f2 w[W][2], bias[2], x[W - 1 + GT][2];
-    load_params<W>(a, c, n, w, bias);
+    load_params<F, W, MODE>(a, c, n, w, bias);
 #pragma unroll
     for (int j = 0; j < W - 1; j++) {
         Raw<F, V> r;
-        input_at<F, W, VEC>(a, b, c, n, t0 - (W - 1) + j, r);
+        input_at<F, W, MODE>(a, b, c, n, t0 - (W - 1) + j, r);
         get_pairs(r, x[j]);
     }
     F *y = (F *)a.y + ((size_t)b * a.T + t0) * a.D + c;
     auto group = [&](auto whole, int count) {
         ring.wait();
 #pragma unroll
-        for (int i = 0; i < GT; i++) get_pairs(ring.at(ring.out, i, 0), x[W - 1 + i]);
+        for (int i = 0; i < GT; i++) get_pairs(ring.read(i, 0), x[W - 1 + i]);
         ring.next();
         fetch();
 #pragma unroll
@@ -179,7 +222,7 @@ __global__ void __launch_bounds__(256) k_conv_fwd(ConvArgs a) {
 #pragma unroll
                 for (int p = 0; p < 2; p++) s[p] = mul2(s[p], sigmoid2(s[p]));
             }
-            if (decltype(whole)::value || i < count) put_pairs<F>(s).store(y + (size_t)i * a.D, VEC, n);
+            if (decltype(whole)::value || i < count) Lie<F, MODE>::store(put_pairs<F>(s), y + (size_t)i * a.D, n);
         }
         y += (size_t)GT * a.D;
         // the last W-1 inputs that exist move to the front
@@ -200,23 +243,23 @@ __global__ void __launch_bounds__(256) k_conv_fwd(ConvArgs a) {
     if (t < t1) group(std::false_type{}, t1 - t);
     if (t1 == a.T && a.state_out) {
 #pragma unroll
-        for (int j = 0; j < W - 1; j++) put_pairs<F>(x[j]).store((F *)a.state_out + ((size_t)b * (W - 1) + j) * a.D + c, VEC, n);
+        for (int j = 0; j < W - 1; j++) Lie<F, MODE>::store(put_pairs<F>(x[j]), (F *)a.state_out + ((size_t)b * (W - 1) + j) * a.D + c, n);
     }
 }
 
 // A thread walks its strip forward, W-1 tokens past its end, in groups: it forms s and ds of a group's tokens, adds to the sums
 // of the parameters' gradients where they are its own, and hands out gx of the tokens W-1 earlier, which is complete then.
-template <typename F, int W, bool VEC>
+template <typename F, int W, int MODE>
 __global__ void __launch_bounds__(256) k_conv_bwd(ConvArgs a) {
     pdl_wait();
     pdl_trigger();
     constexpr int GT = BWD_GT;
     extern __shared__ __align__(16) char smem_raw[];
-    const int c = (blockIdx.y * blockDim.x + threadIdx.x) * V;
+    const int c = Lie<F, MODE>::first();
     if (c >= a.D) return;
-    const int n = min(V, a.D - c), b = blockIdx.x / a.nstrip, t0 = (blockIdx.x - b * a.nstrip) * a.strip;
+    const int n = Lie<F, MODE>::left(a.D, c), b = blockIdx.x / a.nstrip, t0 = (blockIdx.x - b * a.nstrip) * a.strip;
     const int t1 = min(t0 + a.strip, a.T), stop = t1 + W - 1;
-    BwdRing<F, VEC> ring = {reinterpret_cast<Raw<F, V> *>(smem_raw) + threadIdx.x, (int)blockDim.x, n};
+    BwdRing<F, MODE> ring = {reinterpret_cast<Raw<F, V> *>(smem_raw) + threadIdx.x, (int)blockDim.x, n};
     const F *px = (const F *)a.x + (size_t)b * a.x_batch + (size_t)t0 * a.x_token + c, *gy = (const F *)a.gy + ((size_t)b * a.T + t0) * a.D + c;
     int left = min(stop, a.T) - t0;
     auto fetch = [&]() {
@@ -242,16 +285,16 @@ __global__ void __launch_bounds__(256) k_conv_bwd(ConvArgs a) {
         left -= GT;
     };
 #pragma unroll
-    for (int g = 0; g < BWD_AHEAD; g++) fetch();
+    for (int g = 0; g < (MODE != ONES ? BWD_AHEAD : 1); g++) fetch();
     f2 w[W][2], bias[2], gw[W][2], gb[2] = {both(0.f), both(0.f)};
     f2 x[W - 1 + GT][2], ds[W - 1 + GT][2];              // of tokens t-W+1 .. t+GT-1
-    load_params<W>(a, c, n, w, bias);
+    load_params<F, W, MODE>(a, c, n, w, bias);
 #pragma unroll
     for (int j = 0; j < W; j++) gw[j][0] = gw[j][1] = both(0.f);
 #pragma unroll
     for (int j = 0; j < W - 1; j++) {
         Raw<F, V> r;
-        input_at<F, W, VEC>(a, b, c, n, t0 - (W - 1) + j, r);
+        input_at<F, W, MODE>(a, b, c, n, t0 - (W - 1) + j, r);
         get_pairs(r, x[j]);
         ds[j][0] = ds[j][1] = both(0.f);
     }
@@ -264,8 +307,8 @@ __global__ void __launch_bounds__(256) k_conv_bwd(ConvArgs a) {
         ring.wait();
 #pragma unroll
         for (int i = 0; i < GT; i++) {
-            get_pairs(ring.at(ring.out, i, 0), x[W - 1 + i]);
-            if (a.gy) get_pairs(ring.at(ring.out, i, 1), ds[W - 1 + i]);
+            get_pairs(ring.read(i, 0), x[W - 1 + i]);
+            if (a.gy) get_pairs(ring.read(i, 1), ds[W - 1 + i]);
             else ds[W - 1 + i][0] = ds[W - 1 + i][1] = both(0.f);
         }
         ring.next();
@@ -308,15 +351,15 @@ __global__ void __launch_bounds__(256) k_conv_bwd(ConvArgs a) {
                 if (!IN && a.gs_out && to >= a.T - (W - 1)) {        // a token that is part of the state handed on
                     Raw<F, V> r;
                     f2 f[2];
-                    r.load((const F *)a.gs_out + ((size_t)b * (W - 1) + (to - (a.T - (W - 1)))) * a.D + c, VEC, n);
+                    Lie<F, MODE>::load(r, (const F *)a.gs_out + ((size_t)b * (W - 1) + (to - (a.T - (W - 1)))) * a.D + c, n);
                     get_pairs(r, f);
                     o[0] = add2(o[0], f[0]);
                     o[1] = add2(o[1], f[1]);
                 }
                 if (IN || to >= 0) {
-                    if (a.gx) put_pairs<F>(o).store(gx + (size_t)i * a.D, VEC, n);
+                    if (a.gx) Lie<F, MODE>::store(put_pairs<F>(o), gx + (size_t)i * a.D, n);
                 } else if (a.gs_in) {
-                    put_pairs<F>(o).store((F *)a.gs_in + ((size_t)b * (W - 1) + (W - 1 + to)) * a.D + c, VEC, n);
+                    Lie<F, MODE>::store(put_pairs<F>(o), (F *)a.gs_in + ((size_t)b * (W - 1) + (W - 1 + to)) * a.D + c, n);
                 }
             }
         }
@@ -339,8 +382,8 @@ __global__ void __launch_bounds__(256) k_conv_bwd(ConvArgs a) {
         for (int q = 0; q < V; q++) {
             if (q < n) {
 #pragma unroll
-                for (int j = 0; j < W; j++) p[(size_t)(c + q) * W + j] = q & 1 ? gw[j][q / 2].y : gw[j][q / 2].x;
-                p[(size_t)a.D * W + c + q] = q & 1 ? gb[q / 2].y : gb[q / 2].x;
+                for (int j = 0; j < W; j++) p[(size_t)Lie<F, MODE>::channel(c, q) * W + j] = q & 1 ? gw[j][q / 2].y : gw[j][q / 2].x;
+                p[(size_t)a.D * W + Lie<F, MODE>::channel(c, q)] = q & 1 ? gb[q / 2].y : gb[q / 2].x;
             }
         }
     }
@@ -374,10 +417,23 @@ ConvArgs conv_args(const wkv_causal_conv_args_t *a) {
     k.x = a->x; k.w = a->weight; k.bias = a->bias; k.state_in = a->state_in;
     return k;
 }
-// whether every row of every tensor starts at a multiple of 16 bytes
-bool conv_vec(const wkv_causal_conv_args_t *a, std::initializer_list<const void *> ptrs) {
-    const int v = 16 / elem_size(a->dtype);
-    return a->D % v == 0 && a->x_token % v == 0 && a->x_batch % v == 0 && all_aligned(ptrs);
+// how the rows of all the tensors lie
+int lie_of(const wkv_causal_conv_args_t *a, std::initializer_list<const void *> ptrs) {
+    const int size = elem_size(a->dtype);
+    auto multiples = [&](int elements) {
+        for (const void *p : ptrs)
+            if (reinterpret_cast<uintptr_t>(p) & (uintptr_t)(elements * size - 1)) return false;
+        return a->D % elements == 0 && a->x_token % elements == 0 && a->x_batch % elements == 0;
+    };
+    return multiples(V) ? RUNS : multiples(4 / size) ? WORDS : ONES;
+}
+
+// f is called with the way the rows lie (fp32 rows always start at multiples of 4 bytes)
+template <typename F, class Fn>
+int by_lie(int lie, Fn f) {
+    if (lie == RUNS) return f(std::integral_constant<int, RUNS>{});
+    if (lie == WORDS || sizeof(F) == 4) return f(std::integral_constant<int, WORDS>{});
+    return f(std::integral_constant<int, sizeof(F) == 4 ? WORDS : ONES>{});
 }
 
 template <class Fn>
@@ -410,18 +466,20 @@ extern "C" int wkv_causal_conv_forward(const wkv_causal_conv_args_t *a, void *st
     if (a->T > SHORTEST && a->state_in && a->state_in == a->state_out) return WKV_ERR_UNSUPPORTED;
     ConvArgs k = conv_args(a);
     k.y = a->y; k.state_out = a->state_out;
-    const bool vec = conv_vec(a, {a->x, a->state_in, a->y, a->state_out});
+    const int lie = lie_of(a, {a->x, a->state_in, a->y, a->state_out});
     k.strip = strip_for(a->B, a->T, a->D, FWD_THREADS, FWD_LONGEST);
     k.nstrip = a->T > 0 ? (a->T + k.strip - 1) / k.strip : 1;
-    const int runs = (a->D + V - 1) / V, nt = threads_for(runs, (long long)a->B * k.nstrip);
+    const int runs = lie == RUNS ? a->D / V : (a->D + 32 * V - 1) / (32 * V) * 32, nt = threads_for(runs, (long long)a->B * k.nstrip);
     return by_dtype(a->dtype, [&](auto f) {
         using F = decltype(f);
         return by_width(a->W, [&](auto w) {
-            const auto kern = vec ? k_conv_fwd<F, decltype(w)::value, true> : k_conv_fwd<F, decltype(w)::value, false>;
-            constexpr int BYTES = FWD_AHEAD * FWD_GT * (int)sizeof(Raw<F, V>);       // a thread's ring
-            static unsigned char done[2][64];
-            if (!set_max_smem_once(kern, 256 * BYTES, done[vec])) return (int)WKV_ERR_LAUNCH;
-            return launch_chained(kern, dim3(a->B * k.nstrip, (runs + nt - 1) / nt), dim3(nt), nt * BYTES, (cudaStream_t)stream, k);
+            return by_lie<F>(lie, [&](auto m) {
+                constexpr auto kern = k_conv_fwd<F, decltype(w)::value, decltype(m)::value>;
+                constexpr int BYTES = FWD_AHEAD * FWD_GT * (int)sizeof(Raw<F, V>);       // a thread's ring
+                static unsigned char done[64];
+                if (!set_max_smem_once(kern, 256 * BYTES, done)) return (int)WKV_ERR_LAUNCH;
+                return launch_chained(kern, dim3(a->B * k.nstrip, (runs + nt - 1) / nt), dim3(nt), nt * BYTES, (cudaStream_t)stream, k);
+            });
         });
     });
 }
@@ -442,7 +500,7 @@ extern "C" int wkv_causal_conv_backward(const wkv_causal_conv_args_t *a, void *s
     if (!empty) {
         ConvArgs k = conv_args(a);
         k.gy = a->gy; k.gs_out = a->gstate_out; k.gx = a->gx; k.gs_in = a->gstate_in;
-        const bool vec = conv_vec(a, {a->x, a->state_in, a->gy, a->gstate_out, a->gx, a->gstate_in});
+        const int lie = lie_of(a, {a->x, a->state_in, a->gy, a->gstate_out, a->gx, a->gstate_in});
         k.strip = strip_for(a->B, a->T, a->D, BWD_THREADS, BWD_LONGEST);
         k.nstrip = a->T > 0 ? (a->T + k.strip - 1) / k.strip : 1;
         if (params && a->T > 0) {
@@ -451,15 +509,17 @@ extern "C" int wkv_causal_conv_backward(const wkv_causal_conv_args_t *a, void *s
             k.part = (float *)a->workspace;
             rows = a->B * k.nstrip;
         }
-        const int runs = (a->D + V - 1) / V, nt = threads_for(runs, (long long)a->B * k.nstrip);
+        const int runs = lie == RUNS ? a->D / V : (a->D + 32 * V - 1) / (32 * V) * 32, nt = threads_for(runs, (long long)a->B * k.nstrip);
         e = by_dtype(a->dtype, [&](auto f) {
             using F = decltype(f);
             return by_width(a->W, [&](auto w) {
-                const auto kern = vec ? k_conv_bwd<F, decltype(w)::value, true> : k_conv_bwd<F, decltype(w)::value, false>;
-                constexpr int BYTES = BWD_AHEAD * BWD_GT * 2 * (int)sizeof(Raw<F, V>);       // a thread's ring
-                static unsigned char done[2][64];
-                if (!set_max_smem_once(kern, 256 * BYTES, done[vec])) return (int)WKV_ERR_LAUNCH;
-                return launch_chained(kern, dim3(a->B * k.nstrip, (runs + nt - 1) / nt), dim3(nt), nt * BYTES, s, k);
+                return by_lie<F>(lie, [&](auto m) {
+                    constexpr auto kern = k_conv_bwd<F, decltype(w)::value, decltype(m)::value>;
+                    constexpr int BYTES = BWD_AHEAD * BWD_GT * 2 * (int)sizeof(Raw<F, V>);       // a thread's ring
+                    static unsigned char done[64];
+                    if (!set_max_smem_once(kern, 256 * BYTES, done)) return (int)WKV_ERR_LAUNCH;
+                    return launch_chained(kern, dim3(a->B * k.nstrip, (runs + nt - 1) / nt), dim3(nt), nt * BYTES, s, k);
+                });
             });
         });
         if (e != WKV_OK) return e;

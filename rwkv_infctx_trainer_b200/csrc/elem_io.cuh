@@ -68,6 +68,29 @@ struct alignas(N * sizeof(F) < 16 ? N * sizeof(F) : 16) Raw {
             }
         }
     }
+    // the same one by one from elements S apart, the first `n` of them (the rest zeros): neighbouring lanes' S-apart elements are
+    // one access for the warp where rows are not aligned
+    template <int S>
+    __device__ __forceinline__ void gather(const F *p, int n) {
+        zero();
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            if (i < n) {
+                if constexpr (sizeof(F) == 4) w[i] = reinterpret_cast<const uint32_t *>(p)[i * S];
+                else w[i / 2] |= (uint32_t) reinterpret_cast<const uint16_t *>(p)[i * S] << (16 * (i & 1));
+            }
+        }
+    }
+    template <int S>
+    __device__ __forceinline__ void scatter(F *p, int n) const {
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            if (i < n) {
+                if constexpr (sizeof(F) == 4) reinterpret_cast<uint32_t *>(p)[i * S] = w[i];
+                else reinterpret_cast<uint16_t *>(p)[i * S] = (uint16_t)(w[i / 2] >> (16 * (i & 1)));
+            }
+        }
+    }
     __device__ __forceinline__ void get(float *f) const {
         if constexpr (sizeof(F) == 4) {
 #pragma unroll
