@@ -48,12 +48,75 @@ __device__ __forceinline__ uint32_t warp_max_bits(uint32_t v, int lanes) {
     return v;
 }
 
+// How rows lie, and a thread's eight channels of a run.  RUNS: rows of a multiple of 8 channels, the channels are neighbours.
+// PAIRS: of an even number, four pairs that are 64 channels apart.  ONES: of any number, single channels 32 apart.  In each a warp has
+// 256 neighbouring channels and its accesses are whole pieces of a row.  (With neighbours in rows that are not aligned, 3635 rows
+// of 6965 channels took 168 us forward and 288 backward instead of 70 and 169.)
+enum { RUNS, PAIRS, ONES };
+template <int MODE>
+struct Lie {
+    static constexpr int UNIT = MODE == RUNS ? RUN : MODE == PAIRS ? 2 : 1, UNITS = RUN / UNIT, APART = MODE == RUNS ? RUN : 32 * UNIT;
+    static __device__ __forceinline__ int first(int i) {
+        const int tid = threadIdx.x, nt = blockDim.x;
+        return MODE == RUNS ? (tid + i * nt) * RUN : ((tid >> 5) + i * (nt >> 5)) * (32 * RUN) + (tid & 31) * UNIT;
+    }
+    // how many of the channels from c on exist
+    static __device__ __forceinline__ int left(int C, int c) { return c >= C ? 0 : MODE == RUNS ? RUN : min(RUN, (C - c + APART - 1) / APART * UNIT); }
+    static __device__ __forceinline__ int channel(int c, int q) { return c + q / UNIT * APART + q % UNIT; }
+    template <typename T>
+    static __device__ __forceinline__ void load(Raw<T, RUN> &r, const T *p, int n) {
+        if constexpr (MODE == RUNS) r.load(p, true, RUN);
+        else if constexpr (MODE == ONES) r.template gather<32>(p, n);
+        else {
+#pragma unroll
+            for (int i = 0; i < UNITS; i++) {
+                Raw<T, 2> u;
+                u.zero();
+                if (2 * i < n) u.load(p + i * APART, true, 2);
+#pragma unroll
+                for (int k = 0; k < u.WORDS; k++) r.w[i * u.WORDS + k] = u.w[k];
+            }
+        }
+    }
+    template <typename T>
+    static __device__ __forceinline__ void store(const Raw<T, RUN> &r, T *p, int n) {
+        if constexpr (MODE == RUNS) r.store(p, true, RUN);
+        else if constexpr (MODE == ONES) r.template scatter<32>(p, n);
+        else {
+#pragma unroll
+            for (int i = 0; i < UNITS; i++) {
+                Raw<T, 2> u;
+#pragma unroll
+                for (int k = 0; k < u.WORDS; k++) u.w[k] = r.w[i * u.WORDS + k];
+                if (2 * i < n) u.store(p + i * APART, true, 2);
+            }
+        }
+    }
+    // into shared memory without passing through registers (not ONES)
+    template <typename T>
+    static __device__ __forceinline__ void load_async(Raw<T, RUN> *to, const T *p, int n) {
+        const uint32_t dst = (uint32_t)__cvta_generic_to_shared(to);
+        constexpr int BYTES = UNIT * (int)sizeof(T), PIECE = BYTES < 16 ? BYTES : 16;
+#pragma unroll
+        for (int i = 0; i < UNITS; i++) {
+            if (i * UNIT < n) {
+#pragma unroll
+                for (int k = 0; k < BYTES; k += PIECE) {
+                    const char *from = (const char *)(p + i * APART) + k;
+                    if constexpr (PIECE == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst + i * BYTES + k), "l"(from) : "memory");
+                    else asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(dst + i * BYTES + k), "l"(from), "n"(PIECE) : "memory");
+                }
+            }
+        }
+    }
+};
+
 struct NormArgs {
     const void *x, *res, *w;
     void *y, *h;
     float *scale;
     long long rows;
-    int C, w_dtype, group, ngroup, vec;
+    int C, w_dtype, group, ngroup;
     float eps;
 };
 
@@ -65,7 +128,7 @@ __device__ __forceinline__ float q8_scale(uint32_t top) {
 }
 
 // NV runs a thread, MAXT threads at most
-template <typename X, typename R, int NV, int MAXT, bool Q8>
+template <typename X, typename R, int NV, int MAXT, bool Q8, int MODE>
 __global__ void __launch_bounds__(MAXT, 1024 / MAXT) k_rms_norm_fwd(NormArgs a) {
     pdl_wait();
     pdl_trigger();
@@ -74,26 +137,26 @@ __global__ void __launch_bounds__(MAXT, 1024 / MAXT) k_rms_norm_fwd(NormArgs a) 
     const int tid = threadIdx.x, nt = blockDim.x, nwarp = nt >> 5, C = a.C;
     const X *x = (const X *)a.x;
     const R *res = (const R *)a.res;
-    const bool vec = a.vec;
+    using L = Lie<MODE>;
     float w[NV][RUN];
     int left[NV];                       // channels of the run that exist
 #pragma unroll
     for (int i = 0; i < NV; i++) {
-        const int c = (tid + i * nt) * RUN;
-        left[i] = min(RUN, C - c);
+        const int c = L::first(i);
+        left[i] = L::left(C, c);
 #pragma unroll
-        for (int q = 0; q < RUN; q++) w[i][q] = q < left[i] ? param_at(a.w, a.w_dtype, c + q) : 0.f;
+        for (int q = 0; q < RUN; q++) w[i][q] = q < left[i] ? param_at(a.w, a.w_dtype, L::channel(c, q)) : 0.f;
     }
     Raw<X, RUN> rx[NV];
     Raw<R, RUN> rr[NV];
     auto fetch = [&](long long row) {
 #pragma unroll
         for (int i = 0; i < NV; i++) {
-            const size_t at = (size_t)row * C + (size_t)(tid + i * nt) * RUN;
+            const size_t at = (size_t)row * C + L::first(i);
             rx[i].zero(); rr[i].zero();
             if (left[i] > 0) {
-                rx[i].load(x + at, vec, left[i]);
-                if (res) rr[i].load(res + at, vec, left[i]);
+                L::load(rx[i], x + at, left[i]);
+                if (res) L::load(rr[i], res + at, left[i]);
             }
         }
     };
@@ -114,7 +177,7 @@ __global__ void __launch_bounds__(MAXT, 1024 / MAXT) k_rms_norm_fwd(NormArgs a) 
             for (int i = 0; i < NV; i++) {
                 Raw<R, RUN> o;
                 o.put(h[i]);
-                if (left[i] > 0) o.store((R *)a.h + (size_t)row * C + (size_t)(tid + i * nt) * RUN, vec, left[i]);
+                if (left[i] > 0) L::store(o, (R *)a.h + (size_t)row * C + L::first(i), left[i]);
             }
         }
         const float r = rsqrtf(cta_sum(ss, red[par], nwarp) / (float)C + a.eps);
@@ -127,55 +190,83 @@ __global__ void __launch_bounds__(MAXT, 1024 / MAXT) k_rms_norm_fwd(NormArgs a) 
             for (int i = 0; i < NV; i++) {
                 Raw<X, RUN> o;
                 o.put(h[i]);
-                if (left[i] > 0) o.store((X *)a.y + (size_t)row * C + (size_t)(tid + i * nt) * RUN, vec, left[i]);
+                if (left[i] > 0) L::store(o, (X *)a.y + (size_t)row * C + L::first(i), left[i]);
             }
         } else {
-            uint32_t top[NV];
+            // the largest of each unit of a thread's channels
+            uint32_t top[NV][L::UNITS];
 #pragma unroll
-            for (int i = 0; i < NV; i++) {
-                top[i] = 0u;
+            for (int i = 0; i < NV; i++)
 #pragma unroll
-                for (int q = 0; q < RUN; q++)
-                    if (q < left[i]) top[i] = max(top[i], __float_as_uint(h[i][q]) & 0x7FFFFFFFu);
-            }
+                for (int u = 0; u < L::UNITS; u++) {
+                    top[i][u] = 0u;
+#pragma unroll
+                    for (int q = u * L::UNIT; q < (u + 1) * L::UNIT; q++)
+                        if (q < left[i]) top[i][u] = max(top[i][u], __float_as_uint(h[i][q]) & 0x7FFFFFFFu);
+                }
             if (a.group) {
-                // a group is group / 8 neighbouring lanes of one warp
-                const int lanes = a.group / RUN;
+                // A group is some neighbouring lanes of one warp (RUNS: group / 8; PAIRS: half a unit's or all), and if these are all, one or
+                // more of the units
+                const int lanes = min(32, a.group / L::UNIT), units = MODE == RUNS ? 1 : max(1, a.group / L::APART);
 #pragma unroll
                 for (int i = 0; i < NV; i++) {
-                    top[i] = warp_max_bits(top[i], lanes);
-                    if (left[i] > 0 && (tid & (lanes - 1)) == 0) a.scale[(size_t)row * a.ngroup + (tid + i * nt) / lanes] = q8_scale(top[i]);
+#pragma unroll
+                    for (int u = 0; u < L::UNITS; u++) top[i][u] = warp_max_bits(top[i][u], lanes);
+#pragma unroll
+                    for (int m = 1; m < L::UNITS; m <<= 1)
+                        if (m < units) {
+                            uint32_t both[L::UNITS];
+#pragma unroll
+                            for (int u = 0; u < L::UNITS; u++) both[u] = max(top[i][u], top[i][u ^ m]);
+#pragma unroll
+                            for (int u = 0; u < L::UNITS; u++) top[i][u] = both[u];
+                        }
+#pragma unroll
+                    for (int u = 0; u < L::UNITS; u++)
+                        if (u * L::UNIT < left[i] && (tid & (lanes - 1)) == 0 && (u & (units - 1)) == 0)
+                            a.scale[(size_t)row * a.ngroup + (L::first(i) + u * L::APART) / a.group] = q8_scale(top[i][u]);
                 }
             } else {
+                uint32_t m = 0u;
 #pragma unroll
-                for (int i = 1; i < NV; i++) top[0] = max(top[0], top[i]);
-                uint32_t m = warp_max_bits(top[0], 32);
+                for (int i = 0; i < NV; i++)
+#pragma unroll
+                    for (int u = 0; u < L::UNITS; u++) m = max(m, top[i][u]);
+                m = warp_max_bits(m, 32);
                 if (nwarp > 1) {
                     if ((tid & 31) == 0) redm[par][tid >> 5] = m;
                     __syncthreads();
                     m = warp_max_bits((tid & 31) < nwarp ? redm[par][tid & 31] : 0u, 32);
                 }
 #pragma unroll
-                for (int i = 0; i < NV; i++) top[i] = m;
+                for (int i = 0; i < NV; i++)
+#pragma unroll
+                    for (int u = 0; u < L::UNITS; u++) top[i][u] = m;
                 if (tid == 0) a.scale[row] = q8_scale(m);
             }
 #pragma unroll
             for (int i = 0; i < NV; i++) {
-                const float inv = 1.f / q8_scale(top[i]);
                 uint32_t o[2] = {0u, 0u};
 #pragma unroll
                 for (int q = 0; q < RUN; q += 2) {
                     // to nearest, at most 448; a NaN stays one
-                    const uint32_t two = __nv_cvt_float2_to_fp8x2(make_float2(h[i][q] * inv, h[i][q + 1] * inv), __NV_SATFINITE, __NV_E4M3);
+                    const float i0 = 1.f / q8_scale(top[i][q / L::UNIT]), i1 = L::UNIT > 1 ? i0 : 1.f / q8_scale(top[i][(q + 1) / L::UNIT]);
+                    const uint32_t two = __nv_cvt_float2_to_fp8x2(make_float2(h[i][q] * i0, h[i][q + 1] * i1), __NV_SATFINITE, __NV_E4M3);
                     o[q / 4] |= two << (8 * (q & 3));
                 }
                 if (left[i] > 0) {
-                    unsigned char *p = (unsigned char *)a.y + (size_t)row * C + (size_t)(tid + i * nt) * RUN;
-                    if (vec) *reinterpret_cast<uint2 *>(p) = make_uint2(o[0], o[1]);
-                    else {
+                    unsigned char *p = (unsigned char *)a.y + (size_t)row * C + L::first(i);
+                    if (MODE == RUNS) {
+                        *reinterpret_cast<uint2 *>(p) = make_uint2(o[0], o[1]);
+                    } else {
 #pragma unroll
-                        for (int q = 0; q < RUN; q++)
-                            if (q < left[i]) p[q] = (unsigned char)(o[q / 4] >> (8 * (q & 3)));
+                        for (int u = 0; u < L::UNITS; u++) {
+                            const uint32_t v = o[u * L::UNIT / 4] >> (8 * (u * L::UNIT & 3));
+                            if (u * L::UNIT < left[i]) {
+                                if (MODE == PAIRS) *reinterpret_cast<uint16_t *>(p + u * L::APART) = (uint16_t)v;
+                                else p[u * L::APART] = (unsigned char)v;
+                            }
+                        }
                     }
                 }
             }
@@ -183,21 +274,6 @@ __global__ void __launch_bounds__(MAXT, 1024 / MAXT) k_rms_norm_fwd(NormArgs a) 
     }
 }
 
-// A run of channels of a row on its way to a thread's own place in shared memory (nobody else reads it), where `vec`; else it
-// passes through registers.
-template <typename T>
-__device__ __forceinline__ void run_async(Raw<T, RUN> *to, const T *p, bool vec, int n) {
-    if (vec) {
-        const uint32_t dst = (uint32_t)__cvta_generic_to_shared(to);
-#pragma unroll
-        for (int i = 0; i < (int)sizeof(*to); i += 16)
-            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst + i), "l"((const char *)p + i) : "memory");
-    } else {
-        Raw<T, RUN> r;
-        r.load(p, false, n);
-        *to = r;
-    }
-}
 template <int LEFT>
 __device__ __forceinline__ void rows_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(LEFT) : "memory"); }
 __device__ __forceinline__ void rows_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
@@ -209,7 +285,7 @@ struct NormBwdArgs {
     void *gx, *gres;
     float *part;                        // [gridDim.x, C], NULL when the weight needs no gradient
     long long rows;
-    int C, w_dtype, vec;
+    int C, w_dtype;
     float eps;
 };
 
@@ -221,7 +297,7 @@ struct BwdPlace {
     static constexpr int TX = SUM ? 2 : 1, TR = NV == 1 ? 2 : 1;
     static constexpr int ROW = NV * RUN * (int)(TX * sizeof(X) + TR * sizeof(R)), AHEAD = rows_ahead(ROW);
 };
-template <typename X, typename R, int NV, int MAXT, bool SUM>
+template <typename X, typename R, int NV, int MAXT, bool SUM, int MODE>
 __global__ void __launch_bounds__(MAXT, 1024 / MAXT) k_rms_norm_bwd(NormBwdArgs a) {
     pdl_wait();
     pdl_trigger();
@@ -229,15 +305,15 @@ __global__ void __launch_bounds__(MAXT, 1024 / MAXT) k_rms_norm_bwd(NormBwdArgs 
     const int tid = threadIdx.x, nt = blockDim.x, nwarp = nt >> 5, C = a.C;
     const R *h = SUM ? (const R *)a.res : (const R *)a.h, *gh = (const R *)a.gh;
     const X *x = (const X *)a.x, *gy = (const X *)a.gy;
-    const bool vec = a.vec;
+    using L = Lie<MODE>;
     float w[NV][RUN], gw[NV][RUN];
     int left[NV];
 #pragma unroll
     for (int i = 0; i < NV; i++) {
-        const int c = (tid + i * nt) * RUN;
-        left[i] = min(RUN, C - c);
+        const int c = L::first(i);
+        left[i] = L::left(C, c);
 #pragma unroll
-        for (int q = 0; q < RUN; q++) { w[i][q] = q < left[i] ? param_at(a.w, a.w_dtype, c + q) : 0.f; gw[i][q] = 0.f; }
+        for (int q = 0; q < RUN; q++) { w[i][q] = q < left[i] ? param_at(a.w, a.w_dtype, L::channel(c, q)) : 0.f; gw[i][q] = 0.f; }
     }
     using Place = BwdPlace<X, R, NV, SUM>;
     constexpr int AHEAD = Place::AHEAD, TX = Place::TX, TR = Place::TR;
@@ -248,13 +324,27 @@ __global__ void __launch_bounds__(MAXT, 1024 / MAXT) k_rms_norm_bwd(NormBwdArgs 
         if (row < a.rows) {
 #pragma unroll
             for (int i = 0; i < NV; i++) {
-                const size_t at = (size_t)row * C + (size_t)(tid + i * nt) * RUN;
+                const size_t at = (size_t)row * C + L::first(i);
                 const int k = slot * NV + i;
                 if (left[i] > 0) {
-                    if (h) run_async(sr + (TR * k) * nt, h + at, vec, left[i]);
-                    if (TR == 2 && gh) run_async(sr + (TR * k + 1) * nt, gh + at, vec, left[i]);
-                    if (gy) run_async(sx + (TX * k) * nt, gy + at, vec, left[i]);
-                    if (SUM) run_async(sx + (TX * k + 1) * nt, x + at, vec, left[i]);
+                    if constexpr (MODE != ONES) {
+                        if (h) L::load_async(sr + (TR * k) * nt, h + at, left[i]);
+                        if (TR == 2 && gh) L::load_async(sr + (TR * k + 1) * nt, gh + at, left[i]);
+                        if (gy) L::load_async(sx + (TX * k) * nt, gy + at, left[i]);
+                        if (SUM) L::load_async(sx + (TX * k + 1) * nt, x + at, left[i]);
+                    } else {
+                        // (there are no copies of 2 bytes: all loads, then all stores)
+                        Raw<R, RUN> r0, r1;
+                        Raw<X, RUN> x0, x1;
+                        if (h) L::load(r0, h + at, left[i]);
+                        if (TR == 2 && gh) L::load(r1, gh + at, left[i]);
+                        if (gy) L::load(x0, gy + at, left[i]);
+                        if (SUM) L::load(x1, x + at, left[i]);
+                        if (h) sr[(TR * k) * nt] = r0;
+                        if (TR == 2 && gh) sr[(TR * k + 1) * nt] = r1;
+                        if (gy) sx[(TX * k) * nt] = x0;
+                        if (SUM) sx[(TX * k + 1) * nt] = x1;
+                    }
                 }
             }
         }
@@ -278,7 +368,7 @@ __global__ void __launch_bounds__(MAXT, 1024 / MAXT) k_rms_norm_bwd(NormBwdArgs 
                 if (h) sr[(TR * k) * nt].get(hv[i]);
                 if (gh) {
                     if (TR == 2) keep[i] = sr[(TR * k + 1) * nt];
-                    else keep[i].load(gh + (size_t)row * C + (size_t)(tid + i * nt) * RUN, vec, left[i]);
+                    else L::load(keep[i], gh + (size_t)row * C + L::first(i), left[i]);
                 }
                 if (gy) sx[(TX * k) * nt].get(g[i]);
                 if (SUM) {
@@ -286,6 +376,11 @@ __global__ void __launch_bounds__(MAXT, 1024 / MAXT) k_rms_norm_bwd(NormBwdArgs 
                     sx[(TX * k + 1) * nt].get(t);
 #pragma unroll
                     for (int q = 0; q < RUN; q++) hv[i][q] += t[q];
+                }
+                if (MODE == PAIRS) {           // (nothing was copied for channels that do not exist)
+#pragma unroll
+                    for (int q = 0; q < RUN; q++)
+                        if (q >= left[i]) hv[i][q] = g[i][q] = 0.f;
                 }
             }
 #pragma unroll
@@ -306,9 +401,9 @@ __global__ void __launch_bounds__(MAXT, 1024 / MAXT) k_rms_norm_bwd(NormBwdArgs 
                 o[q] += r * (g[i][q] * w[i][q] - xh * m);
             }
             if (left[i] > 0) {
-                const size_t at = (size_t)row * C + (size_t)(tid + i * nt) * RUN;
-                if (a.gx) { Raw<X, RUN> t; t.put(o); t.store((X *)a.gx + at, vec, left[i]); }
-                if (a.gres) { Raw<R, RUN> t; t.put(o); t.store((R *)a.gres + at, vec, left[i]); }
+                const size_t at = (size_t)row * C + L::first(i);
+                if (a.gx) { Raw<X, RUN> t; t.put(o); L::store(t, (X *)a.gx + at, left[i]); }
+                if (a.gres) { Raw<R, RUN> t; t.put(o); L::store(t, (R *)a.gres + at, left[i]); }
             }
         }
     }
@@ -317,7 +412,7 @@ __global__ void __launch_bounds__(MAXT, 1024 / MAXT) k_rms_norm_bwd(NormBwdArgs 
         for (int i = 0; i < NV; i++)
 #pragma unroll
             for (int q = 0; q < RUN; q++)
-                if (q < left[i]) a.part[(size_t)blockIdx.x * C + (tid + i * nt) * RUN + q] = gw[i][q];
+                if (q < left[i]) a.part[(size_t)blockIdx.x * C + L::channel(L::first(i), q)] = gw[i][q];
     }
 }
 
@@ -341,6 +436,25 @@ Split split_of(long long rows, int C, int nv) {
 Split forward_split(long long rows, int C) { return split_of(rows, C, 2); }
 Split backward_split(long long rows, int C) { return split_of(rows, C, C <= 8192 ? 1 : 2); }
 
+// how the rows of all the tensors lie
+int lie_of(int C, std::initializer_list<std::pair<const void *, int>> tensors) {
+    auto multiples = [&](int elements) {
+        for (const auto &t : tensors) {
+            const int bytes = elements * t.second;
+            if (reinterpret_cast<uintptr_t>(t.first) & (uintptr_t)((bytes < 16 ? bytes : 16) - 1)) return false;
+        }
+        return C % elements == 0;
+    };
+    return multiples(RUN) ? RUNS : multiples(2) ? PAIRS : ONES;
+}
+template <class Fn>
+int by_lie(int lie, Fn f) {
+    switch (lie) {
+        case RUNS: return f(std::integral_constant<int, RUNS>{});
+        case PAIRS: return f(std::integral_constant<int, PAIRS>{});
+        default: return f(std::integral_constant<int, ONES>{});
+    }
+}
 template <auto KERN, class Args>
 int run(const Args &k, const Split &sp, int smem, cudaStream_t s) {
     static unsigned char done[64];
@@ -386,15 +500,19 @@ extern "C" int wkv_rms_norm_forward(const wkv_rms_norm_args_t *a, void *stream) 
     k.rows = a->rows; k.C = a->C; k.w_dtype = a->w_dtype; k.eps = a->eps;
     k.group = a->scale ? a->group : 0;
     k.ngroup = k.group ? (a->C + k.group - 1) / k.group : 1;
-    k.vec = a->C % RUN == 0 && all_aligned({a->x, a->residual, a->y, k.h});
+    const int xs = elem_size(a->dtype), rs = elem_size(a->res_dtype);
+    const int lie = lie_of(a->C, {{a->x, xs}, {a->residual, rs}, {a->y, a->scale ? 1 : xs}, {k.h, rs}});
     const Split sp = forward_split(a->rows, a->C);
     cudaStream_t s = (cudaStream_t)stream;
     return by_types(a->dtype, a->res_dtype, [&](auto x, auto r) {
         using X = decltype(x);
         using R = decltype(r);
         const auto go = [&](auto kern) { return launch_chained(kern, dim3(sp.ctas), dim3(sp.threads), 0, s, k); };
-        if (sp.threads <= 512) return k.scale ? go(k_rms_norm_fwd<X, R, 2, 512, true>) : go(k_rms_norm_fwd<X, R, 2, 512, false>);
-        return k.scale ? go(k_rms_norm_fwd<X, R, 2, 1024, true>) : go(k_rms_norm_fwd<X, R, 2, 1024, false>);
+        return by_lie(lie, [&](auto m) {
+            constexpr int M = decltype(m)::value;
+            if (sp.threads <= 512) return k.scale ? go(k_rms_norm_fwd<X, R, 2, 512, true, M>) : go(k_rms_norm_fwd<X, R, 2, 512, false, M>);
+            return k.scale ? go(k_rms_norm_fwd<X, R, 2, 1024, true, M>) : go(k_rms_norm_fwd<X, R, 2, 1024, false, M>);
+        });
     });
 }
 
@@ -418,7 +536,8 @@ extern "C" int wkv_rms_norm_backward(const wkv_rms_norm_args_t *a, void *stream)
     k.h = a->h; k.x = a->x; k.res = a->residual; k.w = a->weight; k.gy = a->gy; k.gh = a->gh; k.gx = a->gx; k.gres = a->gresidual;
     k.part = a->gweight ? (float *)a->workspace : nullptr;
     k.rows = a->rows; k.C = a->C; k.w_dtype = a->w_dtype; k.eps = a->eps;
-    k.vec = a->C % RUN == 0 && all_aligned({a->h, a->x, a->residual, a->gy, a->gh, a->gx, a->gresidual});
+    const int xs = elem_size(a->dtype), rs = elem_size(a->res_dtype);
+    const int lie = lie_of(a->C, {{a->h, rs}, {a->x, xs}, {a->residual, rs}, {a->gy, xs}, {a->gh, rs}, {a->gx, xs}, {a->gresidual, rs}});
     if (a->rows > 0) {
         e = by_types(a->dtype, a->res_dtype, [&](auto x, auto r) {
             using X = decltype(x);
@@ -426,12 +545,15 @@ extern "C" int wkv_rms_norm_backward(const wkv_rms_norm_args_t *a, void *stream)
             const auto go = [&](auto sum) {
                 constexpr bool SUM = decltype(sum)::value;
                 using P1 = BwdPlace<X, R, 1, SUM>;
-                if (sp.nv == 2) {
-                    using P2 = BwdPlace<X, R, 2, SUM>;
-                    return run<k_rms_norm_bwd<X, R, 2, 1024, SUM>>(k, sp, sp.threads * P2::ROW * P2::AHEAD, s);
-                }
-                const int smem = sp.threads * P1::ROW * P1::AHEAD;
-                return sp.threads <= 512 ? run<k_rms_norm_bwd<X, R, 1, 512, SUM>>(k, sp, smem, s) : run<k_rms_norm_bwd<X, R, 1, 1024, SUM>>(k, sp, smem, s);
+                return by_lie(lie, [&](auto m) {
+                    constexpr int M = decltype(m)::value;
+                    if (sp.nv == 2) {
+                        using P2 = BwdPlace<X, R, 2, SUM>;
+                        return run<k_rms_norm_bwd<X, R, 2, 1024, SUM, M>>(k, sp, sp.threads * P2::ROW * P2::AHEAD, s);
+                    }
+                    const int smem = sp.threads * P1::ROW * P1::AHEAD;
+                    return sp.threads <= 512 ? run<k_rms_norm_bwd<X, R, 1, 512, SUM, M>>(k, sp, smem, s) : run<k_rms_norm_bwd<X, R, 1, 1024, SUM, M>>(k, sp, smem, s);
+                });
             };
             return k.h ? go(std::false_type{}) : go(std::true_type{});
         });

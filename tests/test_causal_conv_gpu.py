@@ -47,7 +47,7 @@ def test_lengths_and_widths(W, T, dtype):
     check(c, train(c))
 
 
-@pytest.mark.parametrize("D", [1, 3, 4, 7, 8, 100, 2051])
+@pytest.mark.parametrize("D", [1, 2, 3, 4, 6, 7, 8, 33, 66, 100, 130, 2050, 2051])
 @pytest.mark.parametrize("dtype", [BF, F32])
 def test_channels(D, dtype):
     c = case(D, 3, 37, D, 4, dtype)

@@ -49,7 +49,7 @@ def check(c, got):
         S.close(n, t, ref[r], ref[r + "_mag"], K(r, rows, C))
 
 
-@pytest.mark.parametrize("C", [1, 7, 8, 31, 64, 255, 256, 520, 1000, 2049, 4096, 5120, 8200, 16384])
+@pytest.mark.parametrize("C", [1, 2, 7, 8, 31, 64, 66, 255, 256, 258, 520, 1000, 2049, 2050, 4096, 5120, 8199, 8200, 8202, 16381, 16382, 16384])
 @pytest.mark.parametrize("types", TYPES)
 def test_widths(C, types):
     c = case(C, (5, C), *types)
@@ -74,12 +74,16 @@ def test_types_of_the_weight(wtype):
 
 def test_rows_that_are_not_adjacent_and_start_anywhere():
     import rwkv_infctx_trainer_b200 as W
-    c = case(3, (6, 200), BF, F32)
-    want = train(c)
-    buf = torch.empty(6 * 200 + 1, dtype=BF, device="cuda")[1:].view(6, 200)
-    for x in (torch.cat((c["x"], c["x"]), 1)[:, :200], c["x"].t().contiguous().t(), buf.copy_(c["x"])):
-        for n, t in train(dict(c, x=x)).items():
-            assert torch.equal(t, want[n]), n
+    for rtype in (BF, F32):
+        c = case(3, (6, 200), BF, rtype)
+        want = train(c)
+        for x in (torch.cat((c["x"], c["x"]), 1)[:, :200], c["x"].t().contiguous().t()):
+            for n, t in train(dict(c, x=x)).items():
+                assert torch.equal(t, want[n]), n
+        # (another order of a row's sum)
+        for start in (1, 2, 3):
+            buf = torch.empty(6 * 200 + 8, dtype=BF, device="cuda")[start:start + 1200].view(6, 200)
+            check(dict(c, x=buf.copy_(c["x"])), train(dict(c, x=buf)))
 
 
 def test_empty_and_zero_rows():
@@ -171,7 +175,8 @@ def grouped(t, group):
 
 
 @pytest.mark.parametrize("C,group", [(64, None), (1000, None), (1001, None), (5120, None), (16384, None), (96, 32), (512, 128), (1000, 64),
-                                     (1001, 128), (8200, 256), (40, 256), (9000, 128)])
+                                     (1001, 128), (8200, 256), (40, 256), (9000, 128),
+                                     *((C, g) for C in (1002, 333, 9001) for g in (None, 32, 64, 128, 256)), (2, 32), (1, 256)])
 @pytest.mark.parametrize("types", TYPES)
 def test_8_bit_output(C, group, types):
     """scale: max|y| / 448 with the norm's fp32 error and two roundings more.  q: half a step of e4m3 (2^-4 of a normal
