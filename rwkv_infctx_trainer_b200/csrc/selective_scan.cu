@@ -734,33 +734,28 @@ __global__ void __launch_bounds__(32 * BwdGeo<F, LPC>::WARPS, 2) k_scan_bwd(Scan
         }
     };
     int last = a.T - 1 - t0;
-    // a lane's own tokens of the next block, and the states before it
-    auto own_tokens = [&](Raw<F, 2>(&to)[TB][P::CL], const F *block, int token_stride) {
+    // a lane's own tokens of the next block, and the states before it: copied into shared memory (FAST), else held in registers
+    Own<F, LPC, FAST> held[FAST ? 1 : 4];
+    f2 held_state[FAST ? 1 : 2][2];
+    auto own_tokens = [&](int k, const F *block, int token_stride) {
+        if constexpr (FAST) {
 #pragma unroll
-        for (int i = 0; i < P::PT; i++) {
-            const F *p = block + (long long)min(q + LPC * i, last) * token_stride;
-            if (FAST) {
-                copy_async(&to[q + LPC * i][c], p);
-            } else {
-                F *t = reinterpret_cast<F *>(&to[q + LPC * i][c]);
-                t[0] = p[0];
-                t[1] = p[second];
-            }
+            for (int i = 0; i < P::PT; i++) copy_async(&my.in[k][q + LPC * i][c], block + (long long)min(q + LPC * i, last) * token_stride);
+        } else {
+            held[k].load(block, token_stride, q, last, second);
         }
     };
     auto fetch = [&]() {
-        own_tokens(my.in[0], pu, su);
-        own_tokens(my.in[1], pd, sd);
-        if (a.z) own_tokens(my.in[2], pz, sz);
-        if (a.gy) own_tokens(my.in[3], pg, a.D);
+        own_tokens(0, pu, su);
+        own_tokens(1, pd, sd);
+        if (a.z) own_tokens(2, pz, sz);
+        if (a.gy) own_tokens(3, pg, a.D);
 #pragma unroll
         for (int k = 0; k < 2; k++) {
-            if (FAST) {
+            if constexpr (FAST) {
                 if (n0 < a.N) copy_async(&my.ckpt[k][lane], ck + k * second * a.N + n0);
             } else {
-                f2 v[2];
-                load_states(ck, (size_t)(k * second) * a.N, n0, a.N, v);
-                my.ckpt[k][lane] = make_float4(v[0].x, v[0].y, v[1].x, v[1].y);
+                load_states(ck, (size_t)(k * second) * a.N, n0, a.N, held_state[k]);
             }
         }
         pu -= (long long)su * TB; pd -= (long long)sd * TB; pz -= (long long)sz * TB; pg -= (long long)a.D * TB;
@@ -776,7 +771,17 @@ __global__ void __launch_bounds__(32 * BwdGeo<F, LPC>::WARPS, 2) k_scan_bwd(Scan
     for (int blk = blk1 - 1; blk >= blk0; blk--) {
         const int buf = blk & 1, end = last;
         const float4 *sB = cta.b[buf][swap ? 1 : 0] + q, *sC = cta.c[buf][swap ? 1 : 0] + q;
-        if (FAST) copies_done();
+        if constexpr (FAST) {
+            copies_done();
+        } else {
+#pragma unroll
+            for (int k = 0; k < 4; k++)
+#pragma unroll
+                for (int i = 0; i < P::PT; i++) my.in[k][q + LPC * i][c] = held[k].v[i];
+#pragma unroll
+            for (int k = 0; k < 2; k++)
+                my.ckpt[k][lane] = make_float4(held_state[k][0].x, held_state[k][0].y, held_state[k][1].x, held_state[k][1].y);
+        }
         f2 x[2][2];
 #pragma unroll
         for (int k = 0; k < 2; k++) {
