@@ -441,64 +441,63 @@ __global__ void __launch_bounds__(128, SUMMARY ? 4 : 3) k_scan_fwd(ScanArgs a) {
     }
 }
 
-// One token: a thread for four states of a channel, 16 bytes of each tensor, in R rows; state_out may be state_in (each
-// thread reads its own before it writes).  LANES a channel, N <= 4 LANES.  Bound by HBM where rows are many: with four rows a
-// thread A and the parameters are read once for four, and four states are on their way at once.
-template <typename F, int LANES, int R>
+// One token: a thread for eight states of a channel, in two runs of four that are LANES runs apart (the lanes of a channel read
+// whole sectors); state_out may be state_in (each thread reads its own before it writes).  N <= 8 LANES.
+// Bound by HBM where rows are many, then by a thread's other loads, most of 2 and 4 bytes (64 rows of 8192 channels with 16 states,
+// from HBM: one run a thread 27 us, two 20, four 28; two rows a thread 29, four 37; 256 rows 59: 4.5 TB/s).
+template <typename F, int LANES>
 __global__ void __launch_bounds__(256) k_scan_step(ScanArgs a) {
     pdl_wait();
     pdl_trigger();
-    const int i = (blockIdx.x * 256 + threadIdx.x) / LANES, n0 = 4 * (threadIdx.x % LANES), n = a.N - n0;
+    const int i = (blockIdx.x * 256 + threadIdx.x) / LANES, q = threadIdx.x % LANES, b = blockIdx.y;
     const bool live = i < a.D;
-    const int ch = live ? i : 0, grp = ch / a.Dg, b0 = blockIdx.y * R;
-    Raw<float, 4> rA, rh[R];
-    Raw<F, 4> rB[R], rC[R];
-    float u[R], dt[R], z[R];
+    const int ch = live ? i : 0, grp = ch / a.Dg;
+    const size_t row = ((size_t)b * a.D + ch) * a.N;
+    const F *pB = (const F *)a.Bm + (size_t)b * a.B_batch + (size_t)grp * a.N, *pC = (const F *)a.Cm + (size_t)b * a.C_batch + (size_t)grp * a.N;
+    Raw<float, 4> rA[2], rh[2];
+    Raw<F, 4> rB[2], rC[2];
 #pragma unroll
-    for (int r = 0; r < R; r++) {
-        const int b = min(b0 + r, a.B - 1);              // (rows behind the last: read as the last, not written)
-        rh[r].zero();
-        rB[r].zero();
-        rC[r].zero();
+    for (int j = 0; j < 2; j++) {
+        const int n0 = 4 * (q + j * LANES), n = a.N - n0;
+        rh[j].zero();
+        rA[j].zero();
+        rB[j].zero();
+        rC[j].zero();
         if (n > 0) {
-            if (a.state_in) rh[r].load(a.state_in + ((size_t)b * a.D + ch) * a.N + n0, a.vec_s, n);
-            rB[r].load((const F *)a.Bm + (size_t)b * a.B_batch + (size_t)grp * a.N + n0, a.vec_b, n);
-            rC[r].load((const F *)a.Cm + (size_t)b * a.C_batch + (size_t)grp * a.N + n0, a.vec_c, n);
+            if (a.state_in) rh[j].load(a.state_in + row + n0, a.vec_s, n);
+            rA[j].load(a.A + (size_t)ch * a.N + n0, a.vec_a, n);
+            rB[j].load(pB + n0, a.vec_b, n);
+            rC[j].load(pC + n0, a.vec_c, n);
         }
-        u[r] = Elem<F>::ld((const F *)a.u + (size_t)b * a.u_batch + ch);
-        dt[r] = Elem<F>::ld((const F *)a.delta + (size_t)b * a.delta_batch + ch);
-        z[r] = a.z ? Elem<F>::ld((const F *)a.z + (size_t)b * a.z_batch + ch) : 0.f;
     }
-    rA.zero();
-    if (n > 0) rA.load(a.A + (size_t)ch * a.N + n0, a.vec_a, n);
-    const float bias = a.bias ? a.bias[ch] : 0.f, dskip = a.Dskip ? a.Dskip[ch] : 0.f;
-    float A[4];
-    rA.get(A);
+    const float u = Elem<F>::ld((const F *)a.u + (size_t)b * a.u_batch + ch);
+    float dt = Elem<F>::ld((const F *)a.delta + (size_t)b * a.delta_batch + ch) + (a.bias ? a.bias[ch] : 0.f), sig, y = 0.f;
+    const float z = a.z ? Elem<F>::ld((const F *)a.z + (size_t)b * a.z_batch + ch) : 0.f, dskip = a.Dskip ? a.Dskip[ch] : 0.f;
+    if (a.softplus) dt = softplus<false>(dt, sig);
 #pragma unroll
-    for (int r = 0; r < R; r++) {
-        float h[4], B[4], C[4], y = 0.f, sig, d = dt[r] + bias;
-        if (a.softplus) d = softplus<false>(d, sig);
-        rh[r].get(h);
-        rB[r].get(B);
-        rC[r].get(C);
+    for (int j = 0; j < 2; j++) {
+        const int n0 = 4 * (q + j * LANES), n = a.N - n0;
+        float h[4], A[4], B[4], C[4];
+        rh[j].get(h);
+        rA[j].get(A);
+        rB[j].get(B);
+        rC[j].get(C);
 #pragma unroll
         for (int k = 0; k < 4; k++) {
-            h[k] = ex2(fmaf(d, A[k] * LOG2E, EX2_MEAN)) * h[k] + d * u[r] * B[k];
+            h[k] = ex2(fmaf(dt, A[k] * LOG2E, EX2_MEAN)) * h[k] + dt * u * B[k];
             y += C[k] * h[k];
         }
-#pragma unroll
-        for (int m = 1; m < LANES; m <<= 1) y += __shfl_xor_sync(FULL_MASK, y, m);
-        if (live && b0 + r < a.B) {
-            if (a.state_out && n > 0) {
-                rh[r].put(h);
-                rh[r].store(a.state_out + ((size_t)(b0 + r) * a.D + ch) * a.N + n0, a.vec_s, n);
-            }
-            if (n0 == 0) {
-                y += dskip * u[r];
-                if (a.z) y *= z[r] * sigm(z[r]);
-                Elem<F>::st((F *)a.y + (size_t)(b0 + r) * a.D + ch, y);
-            }
+        if (live && a.state_out && n > 0) {
+            rh[j].put(h);
+            rh[j].store(a.state_out + row + n0, a.vec_s, n);
         }
+    }
+#pragma unroll
+    for (int m = 1; m < LANES; m <<= 1) y += __shfl_xor_sync(FULL_MASK, y, m);
+    if (live && q == 0) {
+        y += dskip * u;
+        if (a.z) y *= z * sigm(z);
+        Elem<F>::st((F *)a.y + (size_t)b * a.D + ch, y);
     }
 }
 
@@ -1182,17 +1181,14 @@ extern "C" int wkv_selective_scan_forward(const wkv_selective_scan_args_t *a, vo
     k.y = a->y; k.state_out = a->state_out;
     const int lpc = lanes_for(a->N), cpw = 64 / lpc;
     if (a->T == 1 && !a->ckpt) {
-        const long long threads = (long long)a->D * lpc;
-        const int rows = a->B >= 8 ? 4 : 1;             // (the launch takes 65535 blocks of rows)
-        if ((a->B + rows - 1) / rows > 65535) return WKV_ERR_SHAPE;
+        if (a->B > 65535) return WKV_ERR_SHAPE;         // (blocks of a grid across)
         k.vec_a = a->N % 4 == 0 && aligned16(a->A);
         k.vec_s = a->N % 4 == 0 && all_aligned({a->state_in, a->state_out});
-        const dim3 grid((unsigned)((threads + 255) / 256), (unsigned)((a->B + rows - 1) / rows));
         return by_dtype(a->dtype, [&](auto f) {
             return by_lanes(lpc, [&](auto l) {
-                using F = decltype(f);
-                constexpr int LANES = decltype(l)::value;
-                return launch_chained(rows == 4 ? k_scan_step<F, LANES, 4> : k_scan_step<F, LANES, 1>, grid, dim3(256), 0, s, k);
+                constexpr int LANES = decltype(l)::value / 2;
+                const long long threads = (long long)a->D * LANES;
+                return launch_chained(k_scan_step<decltype(f), LANES>, dim3((unsigned)((threads + 255) / 256), a->B), dim3(256), 0, s, k);
             });
         });
     }
