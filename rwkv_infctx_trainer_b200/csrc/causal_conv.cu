@@ -160,7 +160,11 @@ struct Ring {
     __device__ __forceinline__ void wait() {
         if (MODE != ONES) asm volatile("cp.async.wait_group %0;" ::"n"(AHEAD - 1) : "memory");
     }
-    __device__ __forceinline__ void next() { out = out + 1 == AHEAD ? 0 : out + 1; }
+    // the group has been read (before anything is copied to its place)
+    __device__ __forceinline__ void next() {
+        __syncwarp(__activemask());
+        out = out + 1 == AHEAD ? 0 : out + 1;
+    }
 };
 template <typename F, int MODE>
 using FwdRing = Ring<F, FWD_GT, 1, FWD_AHEAD, MODE>;

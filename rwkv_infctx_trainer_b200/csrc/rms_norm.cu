@@ -386,9 +386,10 @@ __global__ void __launch_bounds__(MAXT, 1024 / MAXT) k_rms_norm_bwd(NormBwdArgs 
 #pragma unroll
             for (int q = 0; q < RUN; q++) { s.x += hv[i][q] * hv[i][q]; s.y += g[i][q] * w[i][q] * hv[i][q]; }
         }
+        s = cta_sum2(s, red[par], nwarp);
+        __syncwarp();                           // (the row has been read before anything is copied to its place)
         fetch(row + (long long)AHEAD * gridDim.x, slot);
         slot = slot + 1 == AHEAD ? 0 : slot + 1;
-        s = cta_sum2(s, red[par], nwarp);
         const float r = rsqrtf(s.x / (float)C + a.eps), m = s.y * r / (float)C;      // m = mean(gy w xh)
 #pragma unroll
         for (int i = 0; i < NV; i++) {

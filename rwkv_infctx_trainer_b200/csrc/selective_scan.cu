@@ -23,6 +23,13 @@
 //
 // The backward pass needs h_t at every token: the forward pass leaves the state before every 16th token (4 N / 16 bytes a
 // token and channel), a block is run again from there.
+//
+// Not bound by HBM: 4 rows of 4096 tokens and channels, 16 states, take 570 us forward and 1690 backward, of which their bytes would
+// take 83 and 147.  Per token and eight channels an SM takes 16 and 50 cycles; of these 10 and 17 are exponentials on the special
+// function unit (a state's decay is formed once forward, 1.75 times backward), 10 and 29 the shared memory's path (B, C, steps, and
+// the exchanges of the sums), 9 and 25 the issue of 37 and 101 instructions, with 7 warps an SM.  More warps did not help (their
+// states and decays do not fit: 12 warps of 165 registers 1785 us a pass where 8 of 254 took 1680), nor did a quarter of the
+// exponentials on the multiply-add pipe (prompts 2 % faster, nothing else).
 #include "elem_io.cuh"
 #include "wkv_internal.h"
 
@@ -1180,8 +1187,8 @@ extern "C" int wkv_selective_scan_forward(const wkv_selective_scan_args_t *a, vo
     ScanArgs k = scan_args(a, plan_forward(a), fast);
     k.y = a->y; k.state_out = a->state_out;
     const int lpc = lanes_for(a->N), cpw = 64 / lpc;
-    if (a->T == 1 && !a->ckpt) {
-        if (a->B > 65535) return WKV_ERR_SHAPE;         // (blocks of a grid across)
+    // (more rows than a grid has blocks across go through the kernel for prompts, where a thread too reads its states before it writes)
+    if (a->T == 1 && !a->ckpt && a->B <= 65535) {
         k.vec_a = a->N % 4 == 0 && aligned16(a->A);
         k.vec_s = a->N % 4 == 0 && all_aligned({a->state_in, a->state_out});
         return by_dtype(a->dtype, [&](auto f) {

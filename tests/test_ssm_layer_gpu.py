@@ -292,3 +292,32 @@ def test_offsets_that_pass_32_bits():
         y, _ = W.causal_conv(x.unsqueeze(0), w.unsqueeze(1).expand(c, 4).contiguous())
         tail, _ = W.causal_conv(x[-200:].unsqueeze(0), w.unsqueeze(1).expand(c, 4).contiguous())
         assert torch.equal(y[0, -150:], tail[0, -150:])
+
+
+def test_inference_mode_and_many_rows():
+    import rwkv_infctx_trainer_b200 as W
+    p = params(BF)
+    with torch.inference_mode():
+        x, res, cs, st = inputs(2, 3, BF)
+        y, _ = step(p, x[:, 0], res[:, 0], cs, st)
+    plain = st.clone(), cs.clone()                     # (of inference tensors, outside)
+    with torch.inference_mode():
+        step(p, x[:, 1], res[:, 1], plain[1], plain[0])
+        step(p, x[:, 1], res[:, 1], cs, st)
+    assert torch.equal(plain[0], st) and torch.equal(plain[1], cs)
+    # more rows than a grid has blocks across
+    B, d, n = 70000, 4, 4
+    c = S.scan_case(1, B, 1, d, n, 1, BF)
+    state = c["state"].clone()
+    one = lambda k, rows=slice(None): c[k][rows, 0]
+    y = W.selective_scan_step(one("u"), one("delta"), c["A"], one("B"), one("C"), state, c["D"], one("z"), c["delta_bias"])
+    few, r = c["state"][-500:].clone(), slice(-500, None)
+    y2 = W.selective_scan_step(one("u", r), one("delta", r), c["A"], one("B", r), one("C", r), few, c["D"], one("z", r), c["delta_bias"])
+    # (two kernels, the same formulas: another order of two sums)
+    assert float((state[-500:] - few).abs().max()) <= 4 * S.U * float(few.abs().max())
+    assert float((y[-500:].float() - y2.float()).abs().max()) <= 2.0 ** -7 * float(y2.float().abs().max())
+    xs, w = torch.randn((B, 8), device="cuda").to(BF), torch.randn((8, 4), device="cuda")
+    s0 = torch.randn((B, 3, 8), device="cuda").to(BF)
+    s1 = s0[-7:].clone()
+    y = W.causal_conv_step(xs, s0, w)
+    assert torch.equal(y[-7:], W.causal_conv_step(xs[-7:], s1, w)) and torch.equal(s0[-7:], s1)
