@@ -321,3 +321,77 @@ def test_inference_mode_and_many_rows():
     s1 = s0[-7:].clone()
     y = W.causal_conv_step(xs, s0, w)
     assert torch.equal(y[-7:], W.causal_conv_step(xs[-7:], s1, w)) and torch.equal(s0[-7:], s1)
+
+
+def _all_ops(c, x, res, w, cw, cb):
+    """the three operators in training, and every gradient (twice from one graph)"""
+    import rwkv_infctx_trainer_b200 as W
+    scan = {n: t for n, t in c.items() if n in ("u", "delta", "A", "B", "C", "D", "z", "delta_bias", "state")}
+    ins = [*scan.values(), x, res, w, cw, cb]
+    s = list(W.selective_scan(scan["u"], scan["delta"], scan["A"], scan["B"], scan["C"], scan["D"], scan["z"], scan["delta_bias"], True, scan["state"]))
+    outs = [*s, *W.causal_conv(x, cw, cb), *W.rms_norm(x, w, res)]
+    grads = [torch.autograd.grad(outs, ins, [torch.ones_like(o) for o in outs], retain_graph=True) for _ in range(2)]
+    for a, b in zip(*grads):
+        assert torch.equal(a, b)
+    return [o.detach() for o in outs] + list(grads[0])
+
+
+def _layer_inputs(seed, B=3, T=37, D=24, N=16):
+    g = torch.Generator("cuda").manual_seed(seed)
+    def r(*s, dtype=torch.bfloat16): return torch.randn(s, device="cuda", generator=g).to(dtype)
+    f = torch.float32
+    scan = dict(u=r(B, T, D), delta=r(B, T, D), A=-r(D, N, dtype=f).abs(), B=r(B, T, N), C=r(B, T, N), D=r(D, dtype=f), z=r(B, T, D),
+                delta_bias=r(D, dtype=f), state=r(B, D, N, dtype=f))
+    return scan, r(B, T, D), r(B, T, D), r(D, dtype=f), r(D, 4, dtype=f), r(D, dtype=f)
+
+
+# what of each tensor is one value for all: rows (0) or tokens (1)
+@pytest.mark.parametrize("dim", [0, 1])
+def test_broadcast_inputs_and_their_gradients(dim):
+    """the same bits as from copies, and as gradient their sum over what was broadcast"""
+    scan, x, res, w, cw, cb = _layer_inputs(dim)
+    names = ("u", "delta", "B", "C", "z") if dim else ("u", "delta", "B", "C", "z", "state")
+    small = {n: scan[n].narrow(dim, 0, 1).clone().requires_grad_(True) for n in names}
+    small["x"], small["res"] = (t.narrow(dim, 0, 1).clone().requires_grad_(True) for t in (x, res))
+    rest = [t.clone().requires_grad_(True) for t in (w, cw, cb)]
+    others = {n: t.clone().requires_grad_(True) for n, t in scan.items() if n not in names}
+
+    def run(copies):
+        wide = {}
+        for n, t in small.items():
+            v = t.detach().expand((scan[n] if n in scan else x).shape)
+            wide[n] = (v.contiguous() if copies else v).requires_grad_(True)
+        return _all_ops({**{n: wide.get(n, others.get(n)) for n in scan}}, wide["x"], wide["res"], *rest)
+    for a, b in zip(run(False), run(True)):
+        assert torch.equal(a, b)
+
+    # through the expansion itself
+    import rwkv_infctx_trainer_b200 as W
+    full = {n: t.expand((scan[n] if n in scan else x).shape) for n, t in small.items()}
+    y, h = W.rms_norm(full["x"], rest[0], full["res"])
+    got = torch.autograd.grad((y, h), (small["x"], small["res"]), (x, res))
+    leaf = [full[n].detach().contiguous().requires_grad_(True) for n in ("x", "res")]
+    y, h = W.rms_norm(leaf[0], rest[0], leaf[1])
+    for g, each in zip(got, torch.autograd.grad((y, h), leaf, (x, res))):
+        assert torch.equal(g, each.sum(dim, keepdim=True))
+
+
+def test_calls_at_once_on_two_streams():
+    """each with its own workspaces: the bits of the calls made alone"""
+    # (lengths that are cut into spans, so that workspaces are used forward as well)
+    sets = [_layer_inputs(seed, 2, 700, 130, 16) for seed in (5, 6)]
+    for scan, *others in sets:
+        for t in (*scan.values(), *others):
+            t.requires_grad_(True)
+    alone = [_all_ops(*s) for s in sets]
+    torch.cuda.synchronize()
+    streams, out = [torch.cuda.Stream() for _ in sets], [[], []]
+    for _ in range(3):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                out[i].append(_all_ops(*sets[i]))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for got in out[i]:
+            for a, b in zip(got, alone[i]):
+                assert torch.equal(a, b)
