@@ -244,14 +244,18 @@ __device__ __forceinline__ void store_states(float *p, size_t at, int n0, int N,
             if (n0 + i < N) p[at + n0 + i] = f[i];
     }
 }
-// A log2(e) of four states.  An infinite A (the exponential of a large parameter) becomes the largest number: its decay is
-// zero all the same, and a step of zero keeps the state.
-__device__ __forceinline__ void load_decays(const float *A, size_t at, int n0, int N, f2 (&A2)[2], bool swap = false) {
+// A log2(e).  An infinite A (the exponential of a large parameter), or one whose product is, becomes the largest number: its decay
+// is zero all the same, and a step of zero keeps the state.
+__device__ __forceinline__ float decay_rate(float A) {
     constexpr float MOST = 3.4e38f;
-    auto clamp = [](float x) { return x < -MOST ? -MOST : x > MOST ? MOST : x; };      // (a NaN stays)
+    const float x = A * LOG2E;
+    return x < -MOST ? -MOST : x > MOST ? MOST : x;      // (a NaN stays)
+}
+// the same of four states
+__device__ __forceinline__ void load_decays(const float *A, size_t at, int n0, int N, f2 (&A2)[2], bool swap = false) {
     load_states(A, at, n0, N, A2, swap);
 #pragma unroll
-    for (int i = 0; i < 2; i++) A2[i] = make_float2(clamp(A2[i].x * LOG2E), clamp(A2[i].y * LOG2E));
+    for (int i = 0; i < 2; i++) A2[i] = make_float2(decay_rate(A2[i].x), decay_rate(A2[i].y));
 }
 __device__ __forceinline__ f2 ex2(f2 x) { return make_float2(ex2(x.x), ex2(x.y)); }
 // The exponent of a token's decay, dt A log2(e), and a little: ex2 gives too little on average, by 2e-8 of it for exponents from
@@ -491,7 +495,7 @@ __global__ void __launch_bounds__(256) k_scan_step(ScanArgs a) {
         rC[j].get(C);
 #pragma unroll
         for (int k = 0; k < 4; k++) {
-            h[k] = ex2(fmaf(dt, A[k] * LOG2E, EX2_MEAN)) * h[k] + dt * u * B[k];
+            h[k] = ex2(fmaf(dt, decay_rate(A[k]), EX2_MEAN)) * h[k] + dt * u * B[k];
             y += C[k] * h[k];
         }
         if (live && a.state_out && n > 0) {

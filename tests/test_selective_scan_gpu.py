@@ -304,3 +304,37 @@ def test_infinite_steps_gates_and_decays(softplus):
         assert torch.isnan(y[0, 9, ch]) and bool(torch.isfinite(s[0, ch]).all()) == keeps
     clean = [i for i in range(16) if i not in (3, 4, 5, 6, 7, 8)]
     assert torch.isfinite(y[..., clean]).all() and float((s[0, clean].double() - want["state"][0, clean]).abs().max()) < 1e-4
+
+
+@pytest.mark.parametrize("N", [3, 8, 16, 33, 64])
+@pytest.mark.parametrize("softplus", [True, False])
+def test_single_token_with_decays_of_any_size(N, softplus):
+    """an A of -inf, or so large that A log2(e) is: a step of zero keeps the state (its bits), any other forgets it; what the call for
+    prompts gives, also for more rows than a grid has blocks across"""
+    import rwkv_infctx_trainer_b200 as W
+    c = S.scan_case(N, 6, 1, 40, N, 1, F32)
+    c["A"][3], c["A"][4], c["A"][5, 0] = -float("inf"), -3e38, -float("inf")
+    if softplus:
+        c["delta"][:3] = -300.0               # (softplus of it is 0)
+        c["delta_bias"] = c["delta_bias"].clamp(max=0.0)
+    else:
+        c["delta"] = c["delta"].abs() * 0.2 + 0.01
+        c["delta_bias"].zero_()
+        c["delta"][:3] = 0.0
+    want_y, want = call(c, softplus, u=c["u"].clone().requires_grad_(True))         # (with a gradient: the kernel for prompts)
+    want_y, want = want_y.detach(), want.detach()
+    s = c["state"].clone()
+    one = lambda n: c[n][:, 0]
+    y = W.selective_scan_step(one("u"), one("delta"), c["A"], one("B"), one("C"), s, c["D"], one("z"), c["delta_bias"], softplus)
+    assert torch.equal(s[:3], c["state"][:3]) and torch.equal(want[:3], c["state"][:3])
+    for a, b in zip(call(c, softplus), (y.unsqueeze(1), s)):
+        assert torch.equal(a, b)
+    # (two kernels, the same sums in another order: each term of a state passes 4 roundings, of y N + 8 more)
+    assert torch.isfinite(s).all() and torch.isfinite(y).all()
+    mag = c["state"].abs() + want.abs()
+    assert ((s - want).abs() <= 8 * S.U * mag).all()
+    ymag = ((mag * one("C").abs()).sum(-1) + (c["D"] * one("u")).abs()) * S.silu(one("z")).abs()
+    assert ((y - want_y[:, 0]).abs() <= (N + 64) * S.U * ymag).all()
+    ref = reference(c, softplus, False, False)["state"]
+    gone = s[3:, 3:5].double()
+    assert ((gone - (ref[3:, 3:5])).abs() <= 32 * S.U * ref[3:, 3:5].abs() + 1e-37).all()
