@@ -263,6 +263,16 @@ __device__ __forceinline__ f2 ex2(f2 x) { return make_float2(ex2(x.x), ex2(x.y))
 // alone is 1 (tokens behind a row's end, with a step of zero, keep the state).  Errors of the gradients of A, the bias and the
 // state against 64 bits halve (2 x 500 tokens, 512 channels: 1.06, 1.02, 0.75 -> 0.52, 0.51, 0.40 e-6).
 __device__ __forceinline__ f2 exponent(float dt, f2 A2) { return fma2(both(dt), A2, both(EX2_MEAN)); }
+// What a span with decay rates A2, sum of steps `s` and contribution U from zero does to the state before it: 2^(A2 s) h + U.  The
+// power is taken as two factors, of at most 2^127 and 2^127.9: a growing state's may be above the largest number, and then a state of
+// zero stays zero and a small one is what it grows to, as without spans.  (Of any other power the second factor is 1: the bits of
+// one exponential.)
+__device__ __forceinline__ f2 over_span(f2 A2, float s, f2 h, f2 U) {
+    const f2 e = mul2(A2, both(s));
+    auto first = [](float x) { return ex2(x > 127.f ? 127.f : x); };       // (a NaN stays)
+    auto rest = [](float x) { return ex2(fminf(fmaxf(x - 127.f, 0.f), 127.9f)); };
+    return fma2(make_float2(first(e.x), first(e.y)), mul2(make_float2(rest(e.x), rest(e.y)), h), U);
+}
 // two pairs of floats in shared memory
 __device__ __forceinline__ void pairs_at(const float *p, f2 &a, f2 &b) {
     const float4 v = *reinterpret_cast<const float4 *>(p);
@@ -313,9 +323,9 @@ __global__ void __launch_bounds__(128, SUMMARY ? 4 : 3) k_scan_fwd(ScanArgs a) {
             for (int k = 0; k < 2; k++) {
                 f2 U[2];
                 load_states(a.span_state, at * a.N + k * up, n0, a.N, U);
-                const f2 s = both(a.span_dt[at + k * second]);
+                const float s = a.span_dt[at + k * second];
 #pragma unroll
-                for (int i = 0; i < 2; i++) h[k][i] = fma2(ex2(mul2(A2[k][i], s)), h[k][i], U[i]);
+                for (int i = 0; i < 2; i++) h[k][i] = over_span(A2[k][i], s, h[k][i], U[i]);
             }
         }
     }
@@ -699,9 +709,9 @@ __global__ void __launch_bounds__(32 * BwdGeo<F, LPC>::WARPS, 2) k_scan_bwd(Scan
         for (int k = 0; k < 2; k++) {
             f2 V[2];
             load_states((k ? live2 : live) ? a.span_state : nullptr, (at + k) * a.N, n0, a.N, V, swap);
-            const f2 s = both(a.span_dt[at + k * second]);
+            const float s = a.span_dt[at + k * second];
 #pragma unroll
-            for (int i = 0; i < 2; i++) E[k][i] = fma2(ex2(mul2(A2[k][i], s)), E[k][i], V[i]);
+            for (int i = 0; i < 2; i++) E[k][i] = over_span(A2[k][i], s, E[k][i], V[i]);
         }
     }
     const f2 bias = a.bias ? make_float2(a.bias[ch], a.bias[ch + second]) : both(0.f);

@@ -338,3 +338,85 @@ def test_single_token_with_decays_of_any_size(N, softplus):
     ref = reference(c, softplus, False, False)["state"]
     gone = s[3:, 3:5].double()
     assert ((gone - (ref[3:, 3:5])).abs() <= 32 * S.U * ref[3:, 3:5].abs() + 1e-37).all()
+
+
+# ------------------------------------------------------------------ decays of any size, and rows cut into spans
+def train_by_abi(c, groups, softplus=True):
+    """forward and backward of one call of the C ABI with `groups` spans a row"""
+    import ctypes
+    from rwkv_infctx_trainer_b200 import _lib as L
+    lib = L.load()
+    (B, T, D), (_, N), G = c["u"].shape, c["A"].shape, c["B"].shape[2]
+    code = {BF: L.WKV_BF16, HF: L.WKV_F16, F32: L.WKV_F32}[c["u"].dtype]
+    a = L.SelectiveScanArgs(B=B, T=T, D=D, N=N, G=G, dtype=code, softplus=int(softplus), time_groups=groups)
+    for n, f in (("u", "u"), ("delta", "delta"), ("B", "Bm"), ("C", "Cm"), ("z", "z")):
+        setattr(a, f, c[n].data_ptr())
+        setattr(a, n + "_batch", c[n].stride(0))
+        setattr(a, n + "_token", c[n].stride(1))
+    like = {"y": "u", "state": "state", "gu": "u", "gdelta": "u", "gz": "u", "gB": "B", "gC": "B", "gA": "A", "gD": "D", "gbias": "D",
+            "gstate": "state"}
+    out = {n: torch.empty_like(c[t]) for n, t in like.items()}
+    for f, t in (("A", c["A"]), ("Dskip", c["D"]), ("delta_bias", c["delta_bias"]), ("state_in", c["state"]), ("gy", c["gy"]),
+                 ("gstate_out", c["gs"]), ("state_out", out["state"]), ("gstate_in", out["gstate"]),
+                 *((n, out[n]) for n in ("y", "gu", "gdelta", "gz", "gB", "gC", "gA", "gD", "gbias"))):
+        setattr(a, f, t.data_ptr())
+    n = lib.wkv_selective_scan_ckpt_bytes(ctypes.byref(a))
+    ck = torch.empty(n, dtype=torch.uint8, device="cuda")
+    a.ckpt, a.ckpt_bytes = ck.data_ptr(), n
+    st = torch.cuda.current_stream().cuda_stream
+    for fn in ("forward", "backward"):
+        n = getattr(lib, f"wkv_selective_scan_{fn}_workspace")(ctypes.byref(a))
+        ws = torch.empty(n, dtype=torch.uint8, device="cuda")
+        a.workspace, a.workspace_bytes = ws.data_ptr() if n else None, n
+        L.check(getattr(lib, f"wkv_selective_scan_{fn}")(ctypes.byref(a), st), fn)
+    torch.cuda.synchronize()
+    return out
+
+
+@pytest.mark.parametrize("groups", [1, 2, 4, 13])
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("N", [8, 16, 20])
+def test_growing_states_across_spans(groups, dtype, N):
+    """states that grow (A > 0), over a span by more than fp32 holds: what is zero before it stays zero, and what is small enough
+    to stay finite does, in every cut of the row as in the uncut one.  One token grows by e^4 at most, the last ten have inputs and the
+    first ten outgoing gradients, so that all that the uncut recurrence forms is finite (e^40 of a first-size number).
+    A term's exponent is 40 at most, an error of 2^-24 of it (in base 2: 58) in each of two roundings moves it by 2 58 2^-24."""
+    T = 208
+    c = S.scan_case(20 + N, 2, T, 24, N, 1, dtype)
+    c["A"] = c["A"].abs() * 0.5                # up to 4
+    c["A"][0] = 4.0
+    c["delta"] = torch.ones_like(c["delta"])
+    for n in ("delta_bias", "state", "gs"):
+        c[n].zero_()
+    c["u"][:, :T - 10] = 0
+    c["gy"][:, 10:] = 0
+    got = train_by_abi(c, groups, softplus=False)
+    want, mag = reference(c, False, True, False), reference(c, False, True, True)
+    for n, t in got.items():
+        S.close(n, t, want[n], mag[n], S.scan_K(n, 2, T, 24, N) + 4 * 58)
+    # by the call itself, which chooses the cut
+    for n, t in train(c, softplus=False).items():
+        S.close(n, t, want[n], mag[n], S.scan_K(n, 2, T, 24, N) + 4 * 58)
+
+
+@pytest.mark.parametrize("groups", [1, 2, 4])
+def test_small_states_that_grow_by_more_than_the_largest_number(groups):
+    """1e-37 times e^150 over the first half of a row, steps of zero behind it.  The exponent is 217 in base 2: two roundings of it and of
+    its parts move a term by 4 217 2^-24; in the uncut row each of 104 tokens by 8 2^-24 (scan_K)."""
+    T, N = 208, 16
+    c = S.scan_case(31, 1, T, 24, N, 1, F32)
+    c["A"] = torch.full_like(c["A"], 150.0 / 104)
+    c["delta"].fill_(1.0)
+    c["delta"][:, T // 2:] = 0
+    for n in ("delta_bias", "u", "gy"):
+        c[n].zero_()
+    c["state"] = c["state"].sign() * 1e-37
+    c["gs"] = c["gs"].sign() * 1e-37
+    got = train_by_abi(c, groups, softplus=False)
+    want, mag = reference(c, False, True, False), reference(c, False, True, True)
+    for n in ("y", "state", "gstate", "gu", "gA"):
+        K = S.scan_K(n, 1, T, 24, N) + 4 * 217
+        zeros = 0
+        if n in ("y", "gu"):
+            zeros = (N + 1) * torch.finfo(F32).tiny * (1 + (S.silu(c["z"].double()).abs() if n == "y" else 0))
+        S.close(n, got[n], want[n], mag[n] + zeros / (K * S.U), K)
