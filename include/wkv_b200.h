@@ -338,7 +338,7 @@ int wkv_causal_conv_backward(const wkv_causal_conv_args_t *a, void *stream);
  *   in parallel; the workspace sizes depend on it.  ckpt (wkv_selective_scan_ckpt_bytes()):
  *   the state at every 16th token, left by the forward call for the backward call, which
  *   needs it.  Gradients: gu, gdelta, gz [B,T,D], gB, gC [B,T,G,N] in dtype; gA, gD, gbias,
- *   gstate_in fp32.  Token strides and D are at most 2^26, B D (T/16 + 1) and B T G less than 2^31. */
+ *   gstate_in fp32.  Token strides and D are at most 2^26, B D (T/16 + 1) and B T G less than 2^31, T at most 2^31 - 17. */
 typedef struct wkv_selective_scan_args {
     int B, T, D, N, G;
     int dtype, softplus, time_groups;

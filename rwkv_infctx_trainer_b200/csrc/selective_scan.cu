@@ -1039,7 +1039,7 @@ __global__ void __launch_bounds__(256) k_scan_fold_bc(const float *__restrict__ 
 }
 
 // ------------------------------------------------------------------------------------------------ host side
-constexpr long long MAX_STRIDE = 1 << 26, MAX_BLOCKS = 0x7FFFFFFF;
+constexpr long long MAX_STRIDE = 1 << 26, MAX_BLOCKS = 0x7FFFFFFF, MAX_T = 0x7FFFFFFF - TB;
 // (fewer than 5 states are padded to 8: one lane for four states and twice 64 channels a warp would need 255 registers and spill)
 int lanes_for(int N) { return N <= 8 ? 2 : N <= 16 ? 4 : N <= 32 ? 8 : 16; }
 
@@ -1054,6 +1054,8 @@ int check_scan(const wkv_selective_scan_args_t *a) {
         if (s > MAX_STRIDE) return WKV_ERR_SHAPE;
     // (blocks of a grid: at most a warp's worth for each block of tokens, and the fold of gB and gC)
     if ((long long)a->B * a->D * (a->T / TB + 1) > MAX_BLOCKS || (long long)a->B * a->T * a->G > MAX_BLOCKS) return WKV_ERR_SHAPE;
+    // (token numbers up to the end of the last block are 32-bit)
+    if (a->T > MAX_T) return WKV_ERR_SHAPE;
     if (a->B == 0 || a->D == 0) return WKV_OK;
     if (!a->A || (a->T > 0 && (!a->u || !a->delta || !a->Bm || !a->Cm))) return WKV_ERR_NULL;
     return WKV_OK;

@@ -204,3 +204,22 @@ def test_error_codes_without_gpu():
     assert lib.wkv_selective_scan_forward(ref(a), None) == 2
     a = L.SelectiveScanArgs(N=16, G=1)
     assert lib.wkv_selective_scan_forward(ref(a), None) == 0
+
+
+def test_scans_of_more_tokens_than_can_be_numbered_are_refused():
+    """(nothing here reaches a launch: the sizes of the checkpoints, and calls that are refused)"""
+    import rwkv_infctx_trainer_b200._lib as L
+    lib = L.load()
+    buf = (ctypes.c_char * 4096)()
+    at = ctypes.addressof(buf) + (-ctypes.addressof(buf)) % 16
+    a = L.SelectiveScanArgs(B=1, D=1, N=4, G=1, dtype=1, softplus=1)
+    for f in ("u", "delta", "Bm", "Cm", "A", "y", "state_out"):
+        setattr(a, f, at)
+    a.T = 2 ** 31 - 17
+    blocks = (a.T + 15) // 16               # (of 16 bytes each)
+    assert lib.wkv_selective_scan_ckpt_bytes(ctypes.byref(a)) == (blocks * 16 + 255) // 256 * 256
+    for T in (2 ** 31 - 16, 2 ** 31 - 1):
+        a.T = T
+        assert lib.wkv_selective_scan_ckpt_bytes(ctypes.byref(a)) == 0
+        assert lib.wkv_selective_scan_forward(ctypes.byref(a), None) == 2
+        assert lib.wkv_selective_scan_backward(ctypes.byref(a), None) == 2
