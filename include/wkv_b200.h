@@ -311,7 +311,8 @@ int wkv_rms_norm_backward(const wkv_rms_norm_args_t *a, void *stream);
  *   x [B,T,D] with strides x_batch, x_token (elements, channels adjacent); weight [D,W], bias
  *   [D] (or NULL) in w_dtype; state_in [B,W-1,D] (or NULL: zeros) the inputs before the first
  *   token, state_out the last W-1 inputs.  state_out may be state_in's memory for calls of at
- *   most 16 tokens.  Gradients: gx [B,T,D], gweight, gbias in w_dtype, gstate_in.  D is at most 2^22. */
+ *   most 16 tokens.  Gradients: gx [B,T,D], gweight, gbias in w_dtype, gstate_in.  D is at most 2^22, T
+ *   at most 2^31 - 273. */
 typedef struct wkv_causal_conv_args {
     int B, T, D, W;
     int dtype, w_dtype, silu;

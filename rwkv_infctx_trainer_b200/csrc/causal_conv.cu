@@ -14,7 +14,9 @@
 namespace wkv {
 namespace {
 
-constexpr int MAX_W = 4, MAX_D = 1 << 22, SHORTEST = 16;            // (SHORTEST: tokens of a strip at least)
+constexpr int MAX_W = 4, MAX_D = 1 << 22, SHORTEST = 16, LONGEST = 256;            // (tokens of a strip, at least and at most)
+// (token numbers up to the end of the last strip, and a few behind it, are 32-bit)
+constexpr int MAX_T = 0x7FFFFFFF - LONGEST - 16;
 constexpr int V = 4;                     // channels of a thread
 // Tokens of a group and groups on their way (us forward, 4 rows of 4096 tokens and channels: 6 x 3 63, 4 x 4 59, 4 x 3 57, 2 x 8 59;
 // backward: 6 x 2 140, 3 x 6 124, 3 x 4 122, 3 x 3 120): small groups leave registers for more threads.
@@ -395,7 +397,7 @@ __global__ void __launch_bounds__(256) k_conv_bwd(ConvArgs a) {
 
 int check_conv(const wkv_causal_conv_args_t *a) {
     if (!a) return WKV_ERR_NULL;
-    if (a->B < 0 || a->T < 0 || a->D < 0 || a->W < 2 || a->W > MAX_W || a->D > MAX_D) return WKV_ERR_SHAPE;
+    if (a->B < 0 || a->T < 0 || a->D < 0 || a->W < 2 || a->W > MAX_W || a->D > MAX_D || a->T > MAX_T) return WKV_ERR_SHAPE;
     if ((long long)a->B * (a->T / SHORTEST + 1) > 0x7FFFFFFF) return WKV_ERR_SHAPE;       // (more strips than a grid has blocks)
     if (!known_dtype(a->dtype) || !known_dtype(a->w_dtype)) return WKV_ERR_DTYPE;
     if (a->x_batch < 0 || a->x_token < 0) return WKV_ERR_SHAPE;
@@ -406,7 +408,7 @@ int check_conv(const wkv_causal_conv_args_t *a) {
 
 // Tokens of a strip: so many strips that the GPU has `threads` an SM, `longest` tokens at most: short ones leave little to hide a
 // load behind, long ones few threads (us with the ring alone: forward 64 tokens 66, 128 80, 32 76; backward 110 tokens 149, 220 171, 64 167).
-constexpr int FWD_THREADS = 1536, FWD_LONGEST = 64, BWD_THREADS = 1024, BWD_LONGEST = 256;
+constexpr int FWD_THREADS = 1536, FWD_LONGEST = 64, BWD_THREADS = 1024, BWD_LONGEST = LONGEST;
 int strip_for(int B, int T, int D, int threads, int longest) {
     const long long across = (long long)B * ((D + V - 1) / V), want = (long long)device_sm_count() * threads;
     const long long strip = across * T / want;

@@ -223,3 +223,19 @@ def test_scans_of_more_tokens_than_can_be_numbered_are_refused():
         assert lib.wkv_selective_scan_ckpt_bytes(ctypes.byref(a)) == 0
         assert lib.wkv_selective_scan_forward(ctypes.byref(a), None) == 2
         assert lib.wkv_selective_scan_backward(ctypes.byref(a), None) == 2
+
+
+def test_convolutions_of_more_tokens_than_can_be_numbered_are_refused():
+    """(nothing here reaches a launch)"""
+    import rwkv_infctx_trainer_b200._lib as L
+    lib = L.load()
+    buf = (ctypes.c_char * 4096)()
+    at = ctypes.addressof(buf) + (-ctypes.addressof(buf)) % 16
+    a = L.CausalConvArgs(B=1, D=1, W=4, dtype=1, x=at, weight=at, y=at, state_out=at, x_batch=1, x_token=1)
+    for T in (2 ** 31 - 1, 2 ** 31 - 272):
+        a.T = T
+        assert lib.wkv_causal_conv_backward_workspace(ctypes.byref(a)) == 0
+        assert lib.wkv_causal_conv_forward(ctypes.byref(a), None) == 2
+        assert lib.wkv_causal_conv_backward(ctypes.byref(a), None) == 2
+    a.T = 2 ** 31 - 273
+    assert lib.wkv_causal_conv_backward_workspace(ctypes.byref(a)) > 0
