@@ -420,3 +420,16 @@ def test_small_states_that_grow_by_more_than_the_largest_number(groups):
         if n in ("y", "gu"):
             zeros = (N + 1) * torch.finfo(F32).tiny * (1 + (S.silu(c["z"].double()).abs() if n == "y" else 0))
         S.close(n, got[n], want[n], mag[n] + zeros / (K * S.U), K)
+
+
+# (channels of an odd number in two groups: single accesses; state sizes of each number of lanes, and of no multiple of four)
+@pytest.mark.parametrize("N", [3, 8, 11, 20, 32, 33, 64])
+@pytest.mark.parametrize("D,G", [(48, 2), (50, 2), (37, 1)])
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_every_state_size_in_spans(N, D, G, dtype):
+    c = S.scan_case(N + D, 2, 167, D, N, G, dtype)
+    want, mag = reference(c, True, True, False), reference(c, True, True, True)
+    for groups in (1, 2, 5, 1000):
+        got = train_by_abi(c, groups)
+        for n, t in got.items():
+            S.close(f"{n} in {groups}", t, want[n], mag[n], S.scan_K(n, 2, 167, D, N))
