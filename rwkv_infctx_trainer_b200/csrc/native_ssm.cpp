@@ -27,6 +27,8 @@ void refuse_grad(std::initializer_list<const Tensor *> ts, const char *call, con
 void check_in_place(const Tensor &state, const char *call) {
     TORCH_CHECK_VALUE(state.is_contiguous(), call, ": the state is updated in place and must be contiguous");
 }
+// Before the launch: torch refuses this for a tensor made in inference mode, outside of it, and then nothing may have changed.
+void changes_in_place(const Tensor &state) { torch::autograd::impl::bump_version(state); }
 
 // Rows of adjacent channels with any stride between rows and between tokens, as the kernels take them: a view of a wider
 // tensor stays one, anything else is copied.
@@ -287,8 +289,8 @@ Tensor causal_conv_step(const Tensor &x, const Tensor &state, const Tensor &weig
     ConvCall c = conv_call(rows_of(x, x.size(1), true), x.sizes(), weight, bias, state, silu);
     Tensor y = fresh(x.sizes(), x.scalar_type(), x);
     c.a.y = ptr(y); c.a.state_out = ptr(state);
+    changes_in_place(state);
     check(wkv_causal_conv_forward(&c.a, stream_of(x)), "wkv_causal_conv_forward");
-    torch::autograd::impl::bump_version(state);
     return y;
 }
 
@@ -430,8 +432,8 @@ Tensor selective_scan_step(const Tensor &u, const Tensor &delta, const Tensor &A
     ScanCall c = scan_call(u, delta, A, Bm, Cm, D, z, bias, state, softplus);
     Tensor y = fresh(u.sizes(), u.scalar_type(), u);
     c.a.y = ptr(y); c.a.state_out = (float *)ptr(state);
+    changes_in_place(state);
     check(wkv_selective_scan_forward(&c.a, stream_of(u)), "wkv_selective_scan_forward");
-    torch::autograd::impl::bump_version(state);
     return y;
 }
 

@@ -395,3 +395,21 @@ def test_calls_at_once_on_two_streams():
         for got in out[i]:
             for a, b in zip(got, alone[i]):
                 assert torch.equal(a, b)
+
+
+def test_states_made_in_inference_mode_are_not_touched_outside():
+    """torch refuses in-place changes of such tensors outside inference mode; the refusal comes before the token is taken in"""
+    import rwkv_infctx_trainer_b200 as W
+    p = params(BF)
+    with torch.inference_mode():
+        x, res, cs, st = inputs(2, 3, BF)
+    c = S.scan_case(1, 2, 1, D, N, 1, BF)
+    with torch.inference_mode():
+        keep = cs.clone(), st.clone()
+    for grad in (True, False):
+        with torch.set_grad_enabled(grad):
+            with pytest.raises(RuntimeError, match="[Ii]nference"):
+                W.causal_conv_step(c["u"][:, 0], cs, p["conv"].detach(), p["conv_bias"].detach())
+            with pytest.raises(RuntimeError, match="[Ii]nference"):
+                W.selective_scan_step(c["u"][:, 0], c["delta"][:, 0], p["A"], c["B"][:, 0], c["C"][:, 0], st)
+            assert torch.equal(cs, keep[0]) and torch.equal(st, keep[1])
