@@ -477,7 +477,7 @@ struct BlockBackward : OpNode {
     int64_t version;
     Meta meta;
     std::string name() const override { return "TimeMixBlockBackward"; }
-    variable_list apply(variable_list &&grads) override {
+    variable_list gradients(variable_list &&grads) override {
         at::AutoDispatchBelowADInplaceOrView below;
         const variable_list st = unpack();
         const Kind &k = kind_of(version);

@@ -4,6 +4,7 @@
 #include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/csrc/autograd/function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/saved_variable.h>
 #include <torch/extension.h>
@@ -64,9 +65,32 @@ inline bool wants_grad(std::initializer_list<const Tensor *> ts) {
     return false;
 }
 
+// The gradients of an operator that has no second derivative.  With create_graph=True they are given a history, that of the operator's
+// inputs (`inputs`) and of the incoming gradients, which ends in an error for whoever differentiates them: without one a term that
+// holds a gradient would add nothing, in silence.
+inline variable_list differentiated_once(variable_list outs, torch::autograd::edge_list inputs, const torch::autograd::edge_list &grads,
+                                         const std::string &name) {
+    inputs.insert(inputs.end(), grads.begin(), grads.end());
+    const auto error = std::make_shared<torch::autograd::Error>(
+        name + ": this operator has no second derivative (its gradients, taken with create_graph=True, cannot be differentiated)", std::move(inputs));
+    for (Tensor &g : outs) {
+        if (!g.defined()) continue;
+        g = g.variable_data();
+        torch::autograd::set_history(g, error);
+    }
+    return outs;
+}
+
 // An autograd node with a list of saved tensors, written out (torch::autograd::Function builds maps and
 // dictionaries around every call; at a few microseconds per kernel that shows).
 struct OpNode : torch::autograd::Node {
+    // the gradients of the inputs from those of the outputs
+    virtual variable_list gradients(variable_list &&grads) = 0;
+    variable_list apply(variable_list &&grads) final {
+        if (!at::GradMode::is_enabled()) return gradients(std::move(grads));
+        const auto edges = torch::autograd::collect_next_edges(grads);
+        return differentiated_once(gradients(std::move(grads)), next_edges(), edges, name());
+    }
     std::vector<torch::autograd::SavedVariable> saved;
     void keep(std::initializer_list<Tensor> ts) {
         saved.reserve(saved.size() + ts.size());

@@ -187,7 +187,7 @@ struct Wkv56Backward : OpNode {
     at::ScalarType k_type, v_type, w_type, u_type, s_type;      // of the caller's tensors
     std::vector<int64_t> w_shape, u_shape, s_shape;
     std::string name() const override { return "Wkv56Backward"; }
-    variable_list apply(variable_list &&grads) override {
+    variable_list gradients(variable_list &&grads) override {
         at::AutoDispatchBelowADInplaceOrView below;
         const variable_list st = unpack();
         const Tensor &r = st[0];
@@ -256,7 +256,7 @@ struct DropinBackward : OpNode {
     at::ScalarType w_type, s_type;
     std::vector<int64_t> w_shape, u_shape, s_shape;
     std::string name() const override { return "WkvDropinBackward"; }
-    variable_list apply(variable_list &&grads) override {
+    variable_list gradients(variable_list &&grads) override {
         if (!grads[0].defined()) return variable_list(6);
         at::AutoDispatchBelowADInplaceOrView below;
         const variable_list st = unpack();
@@ -358,7 +358,7 @@ namespace {
 struct Wkv4Backward : OpNode {
     at::ScalarType w_type, u_type, v_type, s_type;
     std::string name() const override { return "Wkv4Backward"; }
-    variable_list apply(variable_list &&grads) override {
+    variable_list gradients(variable_list &&grads) override {
         at::AutoDispatchBelowADInplaceOrView below;
         const variable_list st = unpack();
         const Tensor &k = st[2];

@@ -88,7 +88,7 @@ struct RmsNormBackward : OpNode {
     double eps;
     at::ScalarType x_type, w_type;
     std::string name() const override { return "RmsNormBackward"; }
-    variable_list apply(variable_list &&grads) override {
+    variable_list gradients(variable_list &&grads) override {
         at::AutoDispatchBelowADInplaceOrView below;
         const variable_list st = unpack();
         // (a saved-tensor hook may hand back another layout)
@@ -217,7 +217,7 @@ struct CausalConvBackward : OpNode {
     at::ScalarType w_type, b_type, s_type;
     std::vector<int64_t> w_shape;
     std::string name() const override { return "CausalConvBackward"; }
-    variable_list apply(variable_list &&grads) override {
+    variable_list gradients(variable_list &&grads) override {
         at::AutoDispatchBelowADInplaceOrView below;
         const variable_list st = unpack();
         const Tensor &x = st[0];
@@ -350,7 +350,7 @@ struct SelectiveScanBackward : OpNode {
     bool softplus;
     at::ScalarType A_type, D_type, bias_type, s_type;
     std::string name() const override { return "SelectiveScanBackward"; }
-    variable_list apply(variable_list &&grads) override {
+    variable_list gradients(variable_list &&grads) override {
         at::AutoDispatchBelowADInplaceOrView below;
         const variable_list st = unpack();
         const Tensor &u = st[0], &A = st[2], &Bm = st[3];

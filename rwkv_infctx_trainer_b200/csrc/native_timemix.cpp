@@ -16,6 +16,12 @@ std::array<void *, 5> rows_of(const Tensor &t) {
     return p;
 }
 
+// (the nodes that torch::autograd::Function makes)
+variable_list once(const char *name, variable_list outs, const variable_list &grads) {
+    if (!at::GradMode::is_enabled()) return outs;
+    return differentiated_once(std::move(outs), torch::autograd::get_current_node()->next_edges(), torch::autograd::collect_next_edges(grads), name);
+}
+
 struct LnxGate : torch::autograd::Function<LnxGate> {
     static Tensor forward(AutogradContext *ctx, const Tensor &y_, const Tensor &g_, const Tensor &weight, const Tensor &bias,
                           double eps, int64_t H) {
@@ -48,8 +54,8 @@ struct LnxGate : torch::autograd::Function<LnxGate> {
                                      stream_of(y)),
               "wkv_lnx_gate_backward");
         const auto types = ctx->saved_data["types"].toIntVector();
-        return {gy, gg, gga.view(ctx->saved_data["w_shape"].toIntVector()).to((at::ScalarType)types[0]),
-                gbe.view(ctx->saved_data["b_shape"].toIntVector()).to((at::ScalarType)types[1]), Tensor(), Tensor()};
+        return once("lnx_gate", {gy, gg, gga.view(ctx->saved_data["w_shape"].toIntVector()).to((at::ScalarType)types[0]),
+                                 gbe.view(ctx->saved_data["b_shape"].toIntVector()).to((at::ScalarType)types[1]), Tensor(), Tensor()}, grads);
     }
 };
 
@@ -80,7 +86,7 @@ struct DDLerp : torch::autograd::Function<DDLerp> {
         check(wkvx_ddlerp_backward(B, T, C, n, ptr(x), ptr(sh), p.data(), dtype_code(ma.scalar_type()), 0, ptr(m), ptr(gout), nullptr, nullptr,
                                    nullptr, ptr(gx), ptr(gm), ptr(gsh), gp.data(), ptr(ws), nb, stream_of(x)),
               "wkv_ddlerp_backward");
-        return {gx, gsh, gma.to((at::ScalarType)ctx->saved_data["type"].toInt()), gm};
+        return once("ddlerp", {gx, gsh, gma.to((at::ScalarType)ctx->saved_data["type"].toInt()), gm}, grads);
     }
 };
 
