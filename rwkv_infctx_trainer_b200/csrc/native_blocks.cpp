@@ -514,7 +514,10 @@ std::tuple<Tensor, Tensor, Tensor> block(int64_t version, const Tensor &x_, cons
     }
     k.check(params, C, H);
     require_cuda({&x_, &shift_, &state_});
-    for (const Tensor &p : params) require_cuda({&x_, &p});
+    for (const Tensor &p : params) {
+        require_cuda({&x_, &p});
+        refuse_tangents({&p});
+    }
     const Tensor x = x_.to(BF16).contiguous(), shift = shift_.to(BF16).contiguous();
     Tensor state = state_.to(at::kFloat).contiguous();
     if (version != 4 && state.sizes() != at::IntArrayRef({B, H, HEAD, HEAD})) state = state.view({B, H, HEAD, HEAD});

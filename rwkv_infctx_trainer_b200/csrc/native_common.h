@@ -57,8 +57,14 @@ inline Tensor fresh(at::IntArrayRef sizes, at::ScalarType dt, const Tensor &like
 }
 inline Tensor fresh_like(const Tensor &t) { return fresh(t.sizes(), t.scalar_type(), t); }
 inline Tensor bytes_like(const Tensor &t, size_t n) { return n ? fresh({(int64_t)n}, at::kByte, t) : Tensor(); }
+// The operators have no forward-mode derivatives: a tangent would be dropped in silence.
+inline void refuse_tangents(std::initializer_list<const Tensor *> ts) {
+    for (const Tensor *t : ts)
+        TORCH_CHECK(!t->defined() || !t->_fw_grad(0).defined(), "this operator has no forward-mode derivative: one of its inputs has a tangent");
+}
 // whether autograd will want a backward of a call on these tensors
 inline bool wants_grad(std::initializer_list<const Tensor *> ts) {
+    refuse_tangents(ts);
     if (!at::GradMode::is_enabled()) return false;
     for (const Tensor *t : ts)
         if (t->defined() && t->requires_grad()) return true;

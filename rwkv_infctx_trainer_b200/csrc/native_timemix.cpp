@@ -94,6 +94,7 @@ struct DDLerp : torch::autograd::Function<DDLerp> {
 
 Tensor lnx_gate(const Tensor &y, const Tensor &g, const Tensor &weight, const Tensor &bias, double eps, int64_t H) {
     require_cuda({&y, &g, &weight, &bias});
+    refuse_tangents({&y, &g, &weight, &bias});
     const int64_t C = y.size(-1);
     TORCH_CHECK_VALUE(C == H * HEAD && g.sizes() == y.sizes() && weight.numel() == C && bias.numel() == C,
                       "y, g must be [..., n_head*64]; weight, bias [n_head*64]");
@@ -103,6 +104,7 @@ Tensor lnx_gate(const Tensor &y, const Tensor &g, const Tensor &weight, const Te
 Tensor ddlerp(const Tensor &x, const Tensor &shift, const Tensor &maa, const OptTensor &m_) {
     const Tensor m = m_.has_value() ? *m_ : Tensor();
     require_cuda({&x, &shift, &maa, &m});
+    refuse_tangents({&x, &shift, &maa, &m});
     TORCH_CHECK_VALUE(x.dim() == 3 && maa.dim() == 2 && shift.dim() == 2, "x [B,T,C], shift [B,C], maa [n,C], m [n,B,T,C]");
     const int64_t B = x.size(0), T = x.size(1), C = x.size(2), n = maa.size(0);
     TORCH_CHECK_VALUE(maa.size(1) == C && shift.size(0) == B && shift.size(1) == C &&

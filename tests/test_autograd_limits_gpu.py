@@ -1,6 +1,8 @@
-"""What the operators' autograd nodes do not have, second derivatives, is refused: nothing is dropped in silence."""
+"""What the operators' autograd nodes do not have, second derivatives and forward-mode derivatives, is refused: nothing is
+dropped in silence."""
 import pytest
 import torch
+import torch.autograd.forward_ad as fwAD
 
 pytestmark = pytest.mark.gpu
 BF, F32 = torch.bfloat16, torch.float32
@@ -35,7 +37,7 @@ def ops():
                            [*rows(2), n(C, N, dtype=F32), n(B, T, N), n(B, T, N), n(C, dtype=F32), n(B, T, C), n(B, C, N, dtype=F32)]),
         "WKV6": (lambda r, k, v, w, u, s: W.wkv6(r, k, v, w, u, s), [*rows(4), n(1, 64), s64]),
         "WKV5": (lambda r, k, v, w, u, s: W.wkv5(r, k, v, w, u, s), [*rows(3), torch.rand(C).cuda() * 0.9 + 0.05, n(1, 64), s64]),
-        "WKV6STATE_CUDA": (lambda r, k, v, w, u, s: (W.WKV6STATE_CUDA.apply(B, T, C, 1, r, k, v, w, u, s64.clone()),), [*rows(4), n(1, 64), s64]),
+        "WKV6STATE_CUDA": (lambda r, k, v, w, u, s: (W.WKV6STATE_CUDA.apply(B, T, C, 1, r, k, v, w, u, s.clone()),), [*rows(4), n(1, 64), s64]),
         "wkv (v4)": (lambda w, u, k, v, s: W.wkv(w, u, k, v, s), [n(C, dtype=F32), n(C), *rows(2), n(B, C, 3, dtype=F32)]),
         "lnx_gate": (lambda y, g, w, b: (W.lnx_gate(y, g, w, b, 1e-5, 1),), [*rows(2), n(C), n(C)]),
         "ddlerp": (lambda x, s, m, d: (W.ddlerp(x, s, m, d),), [n(B, T, C), n(B, C), n(3, C), n(3, B, T, C)]),
@@ -74,3 +76,41 @@ def test_second_derivatives_are_refused(name):
     g = torch.autograd.grad(out, leaves, gy, create_graph=True)[0]
     with pytest.raises(RuntimeError, match="second derivative"):
         torch.autograd.grad(g.float().sum() + gy[0].float().sum(), gy[0])
+
+
+@pytest.mark.parametrize("name", NAMES)
+def test_forward_mode_is_refused(name):
+    call, ins = ops()[name]
+    for grad in (True, False):
+        for i, t in enumerate(ins):
+            with torch.set_grad_enabled(grad), fwAD.dual_level():
+                duals = [x.detach().clone() for x in ins]
+                duals[i] = fwAD.make_dual(duals[i], torch.ones_like(t))
+                with pytest.raises(RuntimeError, match="forward-mode"):
+                    call(*duals)
+    call(*ins)
+
+
+def test_forward_mode_is_refused_by_calls_without_gradients():
+    import rwkv_infctx_trainer_b200 as W
+    with torch.no_grad(), fwAD.dual_level():
+        x, s, w = n(B, C), n(B, 3, C), n(C, 4, dtype=F32)
+        dual = lambda t: fwAD.make_dual(t, torch.ones_like(t))
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            W.causal_conv_step(dual(x), s, w)
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            W.rms_norm_q8(dual(x), n(C, dtype=F32))
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            W.selective_scan_step(x, dual(n(B, C)), n(C, N, dtype=F32), n(B, N), n(B, N), n(B, C, N, dtype=F32))
+
+
+def test_parameters_of_a_block_in_forward_mode():
+    import rwkv_infctx_trainer_b200 as W
+    m = W.RWKV_TimeMix6_0(0, 2, C, 1, 64, C).cuda().to(BF)
+    with fwAD.dual_level():
+        p = fwAD.make_dual(m.time_maa_k.detach().clone(), torch.ones_like(m.time_maa_k))
+        del m.time_maa_k
+        m.time_maa_k = p
+        for grad in (True, False):
+            with torch.set_grad_enabled(grad), pytest.raises(RuntimeError, match="forward-mode"):
+                m(n(B, T, C), (n(B, C), n(B, 1, 64, 64, dtype=F32)))
