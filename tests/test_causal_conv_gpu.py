@@ -174,3 +174,11 @@ def test_nan_reaches_its_own_window_only():
         keep = torch.ones_like(y, dtype=torch.bool)
         keep[1, 7:11, 3] = False
         assert torch.equal(y[keep], want[keep])
+
+
+# rows and widths for which a thread's strip has more than its 16 tokens at least (about 30, and an odd number of groups in it)
+@pytest.mark.parametrize("W,D,dtype", [(4, 2048, BF), (4, 2050, BF), (4, 2051, BF), (4, 2051, F32), (3, 2048, HF), (3, 2051, HF), (2, 2048, BF),
+                                       (2, 2050, F32), (2, 2051, BF)])
+def test_strips_of_many_tokens(W, D, dtype):
+    c = case(D + W, 3, 3001, D, W, dtype)
+    check(c, train(c))

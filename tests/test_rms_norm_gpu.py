@@ -224,3 +224,58 @@ def test_8_bit_rows_with_nan_and_infinity():
     z[1, 7] = float("inf")
     q, s = W.rms_norm_q8(z, w, group=64)
     assert torch.isnan(s[1, 0]) and torch.equal(s[1, 1:], torch.ones_like(s[1, 1:])) and float(q[1, 64:].float().abs().max()) == 0.0
+
+
+# rows beyond what a CTA has on its way: CTAs of all SMs (1024 threads an SM) take nine rows and more each; ways that rows lie, one run and
+# two runs a thread
+@pytest.mark.parametrize("C", [2048, 2049, 2050, 8192, 12288, 12289, 12290])
+@pytest.mark.parametrize("types", [(BF, BF), (BF, F32), (HF, None), (F32, F32)])
+def test_rows_that_go_round_a_cta(C, types):
+    runs = (C + 7) // 8
+    threads = (runs if C <= 8192 else (runs + 1) // 2) + 31 & ~31
+    rows = torch.cuda.get_device_properties(0).multi_processor_count * max(1, 1024 // threads) * 9 + 5
+    c = case(C, (rows, C), *types)
+    got = train(c)
+    ref = S.norm_ref(c["x"], c["weight"], c["residual"], EPS, c["gy"], c["gh"])
+    for n, t in got.items():
+        r = "gx" if n == "gres" else n
+        S.close(n, t, ref[r], ref[r + "_mag"], K(r, rows, C))
+    # a row's values do not depend on the rows around it: the last ones, alone
+    some = {n: (t[-20:] if t is not None and t.dim() > 1 else t) for n, t in c.items()}
+    for n, t in train(some).items():
+        if n != "gw":
+            assert torch.equal(t, got[n][-20:]), n
+    # nor does the weight's gradient lose or repeat a row: with gy that is nonzero in one row of each 97 alone, the other rows' share is 0
+    thin = dict(c, gy=torch.zeros_like(c["gy"]))
+    thin["gy"][::97] = c["gy"][::97]
+    few = {n: (t[::97] if t is not None and t.dim() > 1 else t) for n, t in c.items()}
+    a, b = train(thin)["gw"].double(), S.norm_ref(few["x"], few["weight"], few["residual"], EPS, few["gy"], few["gh"])
+    n = few["x"].shape[0]
+    assert ((a - b["gw"]).abs() <= K("gw", n, C) * S.U * b["gw_mag"]).all()
+
+
+def test_histories_of_the_residual_stream_are_freed():
+    """an fp32 residual, of which the node keeps its own output h: without the garbage collector nothing is left of a call whose
+    results are dropped, with and without a backward pass"""
+    import gc
+
+    import rwkv_infctx_trainer_b200 as W
+    for types in ((BF, F32), (F32, F32), (BF, BF)):
+        c = case(8, (64, 4096), *types)
+        x = c["x"].requires_grad_(True)
+
+        def once(backward):
+            y, h = W.rms_norm(x, c["weight"], c["residual"])
+            if backward:
+                torch.autograd.grad((y, h), x, (c["gy"], c["gh"]))
+
+        gc.collect()
+        gc.disable()
+        try:
+            before = torch.cuda.memory_allocated()
+            for backward in (False, True, False, True):
+                for _ in range(5):
+                    once(backward)
+                assert torch.cuda.memory_allocated() == before
+        finally:
+            gc.enable()
