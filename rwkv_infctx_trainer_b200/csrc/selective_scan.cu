@@ -247,9 +247,10 @@ __device__ __forceinline__ void store_states(float *p, size_t at, int n0, int N,
 // A log2(e).  An infinite A (the exponential of a large parameter), or one whose product is, becomes the largest number: its decay
 // is zero all the same, and a step of zero keeps the state.
 __device__ __forceinline__ float decay_rate(float A) {
-    constexpr float MOST = 3.4e38f;
-    const float x = A * LOG2E;
-    return x < -MOST ? -MOST : x > MOST ? MOST : x;      // (a NaN stays)
+    float x = A * LOG2E;
+    asm("max.NaN.f32 %0, %0, %1;" : "+f"(x) : "f"(-3.4e38f));        // (a NaN stays)
+    asm("min.NaN.f32 %0, %0, %1;" : "+f"(x) : "f"(3.4e38f));
+    return x;
 }
 // the same of four states
 __device__ __forceinline__ void load_decays(const float *A, size_t at, int n0, int N, f2 (&A2)[2], bool swap = false) {
@@ -263,15 +264,32 @@ __device__ __forceinline__ f2 ex2(f2 x) { return make_float2(ex2(x.x), ex2(x.y))
 // alone is 1 (tokens behind a row's end, with a step of zero, keep the state).  Errors of the gradients of A, the bias and the
 // state against 64 bits halve (2 x 500 tokens, 512 channels: 1.06, 1.02, 0.75 -> 0.52, 0.51, 0.40 e-6).
 __device__ __forceinline__ f2 exponent(float dt, f2 A2) { return fma2(both(dt), A2, both(EX2_MEAN)); }
-// What a span with decay rates A2, sum of steps `s` and contribution U from zero does to the state before it: 2^(A2 s) h + U.  The
-// power is taken as two factors, of at most 2^127 and 2^127.9: a growing state's may be above the largest number, and then a state of
-// zero stays zero and a small one is what it grows to, as without spans.  (Of any other power the second factor is 1: the bits of
-// one exponential.)
-__device__ __forceinline__ f2 over_span(f2 A2, float s, f2 h, f2 U) {
-    const f2 e = mul2(A2, both(s));
-    auto first = [](float x) { return ex2(x > 127.f ? 127.f : x); };       // (a NaN stays)
-    auto rest = [](float x) { return ex2(fminf(fmaxf(x - 127.f, 0.f), 127.9f)); };
-    return fma2(make_float2(first(e.x), first(e.y)), mul2(make_float2(rest(e.x), rest(e.y)), h), U);
+// What a span with decay rates A2, sum of steps `s` and contribution U from zero does to the state before it: h = 2^(A2 s) h + U.
+// A growing state's power may be above the largest number, and then a state of zero has to stay zero and a small one to become what it
+// grows to, as without spans.  ANY power is taken as two factors, of at most 2^127 and 2^127.9 (the second is 1 for powers up to
+// 2^127: the same bits); decaying states need one.
+template <bool ANY>
+__device__ __forceinline__ void over_span(const f2 (&A2)[2], float s, f2 (&h)[2], const f2 (&U)[2], float &least) {
+    if (!ANY) least = fminf(least, s);
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+        const f2 e = mul2(A2[i], both(s));
+        if (ANY) {
+            auto first = [](float x) { return ex2(x > 127.f ? 127.f : x); };       // (a NaN stays)
+            auto rest = [](float x) { return ex2(fminf(fmaxf(x - 127.f, 0.f), 127.9f)); };
+            h[i] = fma2(make_float2(first(e.x), first(e.y)), mul2(make_float2(rest(e.x), rest(e.y)), h[i]), U[i]);
+        } else {
+            h[i] = fma2(ex2(e), h[i], U[i]);
+        }
+    }
+}
+// Whether a state of the warp may have grown over a span: a rate above zero, or a sum of steps below.  Only then is the fold taken
+// again with two factors (with them at once, the 512 spans of 1 x 65536 tokens of 64 channels: 249 us a pass instead of 215).
+__device__ __forceinline__ bool may_grow(const f2 (&A2)[2][2], float least) {
+    float most = 0.f;
+#pragma unroll
+    for (int i = 0; i < 4; i++) most = fmaxf(most, fmaxf(A2[i / 2][i & 1].x, A2[i / 2][i & 1].y));
+    return __any_sync(FULL_MASK, most > 0.f || least < 0.f);
 }
 // two pairs of floats in shared memory
 __device__ __forceinline__ void pairs_at(const float *p, f2 &a, f2 &b) {
@@ -315,19 +333,22 @@ __global__ void __launch_bounds__(128, SUMMARY ? 4 : 3) k_scan_fwd(ScanArgs a) {
     if (SUMMARY) {
         h[0][0] = h[0][1] = h[1][0] = h[1][1] = both(0.f);
     } else {
-        load_states(a.state_in, row, n0, a.N, h[0]);
-        load_states(a.state_in, row + up, n0, a.N, h[1]);
-        for (int j = 0; j < un.span; j++) {
-            const size_t at = ((size_t)b * a.nspan + j) * a.D + ch;
+        float least = 0.f;
+        auto from_spans = [&](auto any) {
+            load_states(a.state_in, row, n0, a.N, h[0]);
+            load_states(a.state_in, row + up, n0, a.N, h[1]);
+            for (int j = 0; j < un.span; j++) {
+                const size_t at = ((size_t)b * a.nspan + j) * a.D + ch;
 #pragma unroll
-            for (int k = 0; k < 2; k++) {
-                f2 U[2];
-                load_states(a.span_state, at * a.N + k * up, n0, a.N, U);
-                const float s = a.span_dt[at + k * second];
-#pragma unroll
-                for (int i = 0; i < 2; i++) h[k][i] = over_span(A2[k][i], s, h[k][i], U[i]);
+                for (int k = 0; k < 2; k++) {
+                    f2 U[2];
+                    load_states(a.span_state, at * a.N + k * up, n0, a.N, U);
+                    over_span<decltype(any)::value>(A2[k], a.span_dt[at + k * second], h[k], U, least);
+                }
             }
-        }
+        };
+        from_spans(std::false_type{});
+        if (un.span > 0 && may_grow(A2, least)) from_spans(std::true_type{});
     }
     const f2 bias = a.bias ? make_float2(a.bias[ch], a.bias[ch + second]) : both(0.f);
     const f2 dskip = a.Dskip ? make_float2(a.Dskip[ch], a.Dskip[ch + second]) : both(0.f);
@@ -700,20 +721,23 @@ __global__ void __launch_bounds__(32 * BwdGeo<F, LPC>::WARPS, 2) k_scan_bwd(Scan
     f2 A2[2][2], E[2][2], gA[2][2];
     load_decays(a.A, (size_t)ch * a.N, n0, a.N, A2[0], swap);
     load_decays(a.A, (size_t)(ch + second) * a.N, n0, a.N, A2[1], swap);
-    load_states(live ? a.gs_out : nullptr, row, n0, a.N, E[0], swap);
-    load_states(live2 ? a.gs_out : nullptr, row + a.N, n0, a.N, E[1], swap);
     gA[0][0] = gA[0][1] = gA[1][0] = gA[1][1] = both(0.f);
-    for (int j = a.nspan - 1; j > span; j--) {
-        const size_t at = ((size_t)b * a.nspan + j) * a.D + ch;
+    float least = 0.f;
+    auto from_spans = [&](auto any) {
+        load_states(live ? a.gs_out : nullptr, row, n0, a.N, E[0], swap);
+        load_states(live2 ? a.gs_out : nullptr, row + a.N, n0, a.N, E[1], swap);
+        for (int j = a.nspan - 1; j > span; j--) {
+            const size_t at = ((size_t)b * a.nspan + j) * a.D + ch;
 #pragma unroll
-        for (int k = 0; k < 2; k++) {
-            f2 V[2];
-            load_states((k ? live2 : live) ? a.span_state : nullptr, (at + k) * a.N, n0, a.N, V, swap);
-            const float s = a.span_dt[at + k * second];
-#pragma unroll
-            for (int i = 0; i < 2; i++) E[k][i] = over_span(A2[k][i], s, E[k][i], V[i]);
+            for (int k = 0; k < 2; k++) {
+                f2 V[2];
+                load_states((k ? live2 : live) ? a.span_state : nullptr, (at + k) * a.N, n0, a.N, V, swap);
+                over_span<decltype(any)::value>(A2[k], a.span_dt[at + k * second], E[k], V, least);
+            }
         }
-    }
+    };
+    from_spans(std::false_type{});
+    if (span + 1 < a.nspan && may_grow(A2, least)) from_spans(std::true_type{});
     const f2 bias = a.bias ? make_float2(a.bias[ch], a.bias[ch + second]) : both(0.f);
     const f2 dskip = a.Dskip ? make_float2(a.Dskip[ch], a.Dskip[ch + second]) : both(0.f);
     f2 gD = both(0.f), gbias = both(0.f);
