@@ -5,7 +5,8 @@ namespace wkv {
 namespace {
 
 // 32 columns by 8 row groups per CTA, the groups meet in shared memory in a fixed order: the same bits every time.
-// Bound by the latency of its loads (a few MB from L2): eight in flight per thread.
+// Bound by the latency of its loads (a few MB from L2): eight in flight per thread.  With few columns it has few CTAs: the 4096 rows of 320
+// columns of a convolution of 8 x 8192 tokens of 64 channels are read by 10 (backward 91 us in all).
 __global__ void __launch_bounds__(256) k_fold_params(const float *__restrict__ part, int rows, long long cols, FoldOut out) {
     pdl_wait();
     pdl_trigger();

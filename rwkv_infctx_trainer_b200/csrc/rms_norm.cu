@@ -10,10 +10,11 @@
 // Both passes start from the sum before it is rounded: a backward pass from an h in bf16 was 2^-9 off in gweight, which is
 // a sum in fp32.
 //
-// All are bound by HBM: a row crosses once per pass, a thread owns runs of 8 channels and keeps them in registers from
+// A row crosses HBM once per pass, a thread owns runs of 8 channels and keeps them in registers from
 // the sum to the output.  A CTA takes every gridDim-th row, so that the weights (and the sums of their gradient) stay in
-// registers.  Sums are fp32 and in a fixed order.  16384 rows of 4096 bf16 channels with a bf16 residual: forward 86 us (6.2 TB/s),
-// backward 128 (5.2 TB/s of its 10 bytes a channel).
+// registers.  Sums are fp32 and in a fixed order.  Bound by HBM forward, and backward for rows of a multiple of 8 channels, 8192 at most:
+// 16384 rows of 4096 bf16 channels with a bf16 residual take 88 us (6.1 TB/s) and 117 (5.7 TB/s of its 10 bytes a channel).  Wider rows,
+// and rows that start anywhere, spill registers backward (split_of): 4096 rows of 16384 channels 91 and 194 us.
 #include <cuda_fp8.h>
 
 #include "elem_io.cuh"
@@ -51,7 +52,7 @@ __device__ __forceinline__ uint32_t warp_max_bits(uint32_t v, int lanes) {
 // How rows lie, and a thread's eight channels of a run.  RUNS: rows of a multiple of 8 channels, the channels are neighbours.
 // PAIRS: of an even number, four pairs that are 64 channels apart.  ONES: of any number, single channels 32 apart.  In each a warp has
 // 256 neighbouring channels and its accesses are whole pieces of a row.  (With neighbours in rows that are not aligned, 3635 rows
-// of 6965 channels took 168 us forward and 288 backward instead of 70 and 169.)
+// of 6965 channels took 168 us forward and 288 backward; so 64 and 178.)
 enum { RUNS, PAIRS, ONES };
 template <int MODE>
 struct Lie {
@@ -419,7 +420,11 @@ __global__ void __launch_bounds__(MAXT, 1024 / MAXT) k_rms_norm_bwd(NormBwdArgs 
 
 constexpr int MAX_C = 16384;
 // How a row is divided: runs a thread, threads, CTAs for all SMs.  All kernels keep to 64 registers, 1024 threads an SM: with
-// several CTAs there one loads while another sums or stores.  (Us: forward with twice the registers and the next row fetched ahead 98
+// several CTAs there one loads while another sums or stores.  Forward nothing spills for that.  Backward a thread's weights, their gradient,
+// h and gy do not always fit: with two runs (more than 8192 channels) every form spills 364 to 776 bytes a thread, with one run those for
+// single channels (ONES) 152 to 336 and some of the others, with a 32-bit type, up to 36.  Us with a bf16 residual, forward and backward, and
+// of their bytes: 4096 x 12288 76, 156 (62, 78); 4096 x 16384 91, 194 (83, 104); 3635 x 6965 64, 178 (31, 39); 3635 x 6966 38, 79 (31, 39).
+// Another split of such rows has not been tried.  (Us: forward with twice the registers and the next row fetched ahead 98
 // instead of 90, 8-bit output of 1999 x 5120 33 instead of 29; one run a thread 111.  Backward without rows on their way in shared
 // memory 136 instead of 128, of 8192 x 8192 148 instead of 132; forward with them 97.)
 struct Split {

@@ -24,10 +24,12 @@
 // The backward pass needs h_t at every token: the forward pass leaves the state before every 16th token (4 N / 16 bytes a
 // token and channel), a block is run again from there.
 //
-// Not bound by HBM: 4 rows of 4096 tokens and channels, 16 states, take 570 us forward and 1690 backward, of which their bytes would
-// take 83 and 147.  Per token and eight channels an SM takes 16 and 50 cycles; of these 10 and 17 are exponentials on the special
-// function unit (a state's decay is formed once forward, 1.75 times backward), 10 and 29 the shared memory's path (B, C, steps, and
-// the exchanges of the sums), 9 and 25 the issue of 37 and 101 instructions, with 7 warps an SM.  More warps did not help (their
+// Not bound by HBM: 4 rows of 4096 tokens and channels, 16 states, take 605 us forward and 1700 backward, of which
+// their bytes would take 83 and 147.  (Forward calls that follow one another take 780: the next one's CTAs are placed while this one's
+// run, 256 of them for 444 places, and end up uneven on the SMs.  With ordinary launches 570.)  Per token and eight channels an SM that is full takes 18 and 54 cycles; of
+// these 10 and 17 are exponentials on the special function unit (a state's decay is formed once forward, 1.75 times backward), 9 and 29
+// the shared memory's path (B, C, steps, and the exchanges of the sums), 9 and 25 the issue of 37 and 101 instructions, with 7 warps an
+// SM.  None of these is a limit: what is left is latency, with few warps to hide it.  More warps did not help (their
 // states and decays do not fit: 12 warps of 165 registers 1785 us a pass where 8 of 254 took 1680), nor did a quarter of the
 // exponentials on the multiply-add pipe (prompts 2 % faster, nothing else).
 #include "elem_io.cuh"
@@ -69,8 +71,8 @@ __device__ __forceinline__ float rcp(float x) {
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
-// e^x for |x| up to some hundred: the rounding of the exponent x log2(e), up to 2^-24 of it, is made good, and so is the mean error
-// of ex2, -5e-8
+// e^x for x from -126 to 0: the rounding of the exponent x log2(e), up to 2^-24 of it, is made good, and so is the mean error of ex2,
+// -5e-8 over exponents below -1 (above them it is -2e-8 and less: 3e-8 too much is added there, half a rounding)
 __device__ __forceinline__ float exp_near(float x) {
     const float e = LOG2E * x, lo = fmaf(LOG2E, x, -e) + LOG2E_LOW * x, t = ex2(e);
     return fmaf(t, fmaf(lo, LN2, 5e-8f), t);
@@ -78,8 +80,8 @@ __device__ __forceinline__ float exp_near(float x) {
 __device__ __forceinline__ float sigm(float x) { return rcp(1.f + ex2(-LOG2E * x)); }
 
 // softplus(x) = max(x, 0) + log(1 + t), t = e^-|x|, and with SIG its derivative sigmoid(x), for any x: no term overflows.
-// log(1 + t) = 2 artanh(s), s = t / (2 + t) <= 1/3: its power series up to s^13 is off by less than 2 s^15 / 15, a
-// relative 1.4e-8, and keeps the digits of small steps (log of a rounded 1 + t does not).
+// log(1 + t) = 2 artanh(s), s = t / (2 + t) <= 1/3: its power series up to s^13 is short of it by less than 2 s^15 / (15 (1 - s^2)), at
+// most 1.05e-8 or a relative 1.5e-8, and keeps the digits of small steps (log of a rounded 1 + t does not).
 template <bool SIG>
 __device__ __forceinline__ float softplus(float x, float &sig) {
     float ax = -fabsf(x), s;
@@ -259,9 +261,10 @@ __device__ __forceinline__ void load_decays(const float *A, size_t at, int n0, i
     for (int i = 0; i < 2; i++) A2[i] = make_float2(decay_rate(A2[i].x), decay_rate(A2[i].y));
 }
 __device__ __forceinline__ f2 ex2(f2 x) { return make_float2(ex2(x.x), ex2(x.y)); }
-// The exponent of a token's decay, dt A log2(e), and a little: ex2 gives too little on average, by 2e-8 of it for exponents from
-// -0.5 to -0.01 and 0.5e-8 near zero, which over the memory of a state adds up.  1.8e-8 more leaves -0.8e-8 and 0.7e-8, and ex2 of it
-// alone is 1 (tokens behind a row's end, with a step of zero, keep the state).  Errors of the gradients of A, the bias and the
+// The exponent of a token's decay, dt A log2(e), and a little: ex2 gives too little on average, by 1.9e-8 of it for exponents from
+// -0.5 to -0.01 and by 0.6e-8 from -0.001 to 0 (by 5e-8 below -1, where a state is soon forgotten), which over the memory of a state
+// adds up.  1.8e-8 more in the exponent, 1.25e-8 of the power, leaves -0.7e-8 and 0.7e-8, and ex2 of it alone is 1 (tokens behind a row's
+// end, with a step of zero, keep the state).  Errors of the gradients of A, the bias and the
 // state against 64 bits halve (2 x 500 tokens, 512 channels: 1.06, 1.02, 0.75 -> 0.52, 0.51, 0.40 e-6).
 __device__ __forceinline__ f2 exponent(float dt, f2 A2) { return fma2(both(dt), A2, both(EX2_MEAN)); }
 // What a span with decay rates A2, sum of steps `s` and contribution U from zero does to the state before it: h = 2^(A2 s) h + U.
@@ -486,7 +489,8 @@ __global__ void __launch_bounds__(128, SUMMARY ? 4 : 3) k_scan_fwd(ScanArgs a) {
 // One token: a thread for eight states of a channel, in two runs of four that are LANES runs apart (the lanes of a channel read
 // whole sectors); state_out may be state_in (each thread reads its own before it writes).  N <= 8 LANES.
 // Bound by HBM where rows are many, then by a thread's other loads, most of 2 and 4 bytes (64 rows of 8192 channels with 16 states,
-// from HBM: one run a thread 27 us, two 20, four 28; two rows a thread 29, four 37; 256 rows 59: 4.5 TB/s).
+// from HBM: one run a thread 27 us, two 20, four 28; two rows a thread 29, four 37; 256 rows 59: 4.5 TB/s).  The limit of the decay
+// rates costs 0.3 us of 16 there.
 template <typename F, int LANES>
 __global__ void __launch_bounds__(256) k_scan_step(ScanArgs a) {
     pdl_wait();
@@ -639,9 +643,13 @@ __global__ void __launch_bounds__(128) k_scan_bwd_summary(ScanArgs a) {
 // A block is run forward once more from the state the forward pass left, which leaves the states before its quarters in
 // shared memory; then quarter by quarter from the last, forward again with decays and states in registers and back.
 //
-// gB and gC are sums over the channels: a thread adds up its two, then eight values a lane and token are exchanged.  Each
+// gB and gC are sums over the channels, of a CTA here and of all CTAs in k_scan_fold_bc (which costs a workspace of LPC^2 / 8 bytes a
+// token and channel: 0.5, 2, 8 and 32 for up to 8, 16, 32 and 64 states).  A thread adds up its two, then eight values a lane and token are exchanged.  Each
 // exchange halves the values: lanes 16 apart hold their two pairs of states in opposite order, so that the first one needs
 // no selects.
+//
+// Shared memory of a CTA, KB for 16-bit inputs and fp32: 152 and 168 for up to 8 states, 104 and 112 up to 16, 98 and 102 up to 32, 133 and
+// 135 up to 64.
 template <typename F, int LPC>
 struct BwdGeo {
     static constexpr int WARPS = 4;
@@ -1116,6 +1124,9 @@ int plan_forward(const wkv_selective_scan_args_t *a) {
 // an SM and 0.77 with one (932 and 715 us for 2048 tokens); a span starts up in 1.5 blocks; the summary pass takes 0.27 of a
 // full pass for the work that fills the GPU.  Against measurements of 1 to 32 spans (us: chosen, uncut, best of those tried): 4 rows of
 // 4096 tokens and channels 1684, 1684, 1684; 1 of 8191 x 5120 1230, 2399, 1219; 8 of 512 x 1024 145, 166, 145.
+// All of that is of 9 to 16 states.  Two CTAs fit on an SM for 9 to 32; with fewer states a CTA's shared memory is 152 KB (fp32 168), with
+// more 133 (135), and an SM has one: there the account is off by up to a wave, and the choice has not been measured.  Nor are more
+// than 32 spans tried: 1 x 65536 tokens of 64 channels run on 32 CTAs (790 us backward).
 int plan_backward(const wkv_selective_scan_args_t *a) {
     const int nblk = (a->T + TB - 1) / TB;
     if (a->time_groups) return whole_spans(a->time_groups, nblk);

@@ -9,13 +9,16 @@ state, with the contract of the WKV ops (state in, state out, the gradient of bo
 ``selective_scan(u, delta, A, B, C, D=None, z=None, delta_bias=None, delta_softplus=True, state=None) -> (y, state)``
     ``dt = softplus(delta + delta_bias)``, ``h_t = exp(dt A) h_{t-1} + dt u_t B_t``, ``y_t = (C_t . h_t + D u_t) silu(z_t)``
     per channel and state.  u, delta, z [B,T,D]; B, C [B,T,N] or [B,T,G,N] (channel d uses group d // (D / G));
-    A [D,N], 1 <= N <= 64; D, delta_bias [D]; state fp32 [B,D,N] (None: zeros).  Without z there is no gate.
+    A [D,N], 1 <= N <= 64; D, delta_bias [D]; state fp32 [B,D,N] (None: zeros).  Without z there is no gate.  An A of -inf forgets
+    the state at any step above zero; a step of zero keeps it.
 
-Both are differentiable w.r.t. every tensor, the state included.  Any T >= 0.
+Both are differentiable w.r.t. every tensor, the state included (once, and not in forward mode: anything else is refused).  Any T >= 0
+up to 2^31 - 273.
 
 ``causal_conv_step(x, state, weight, bias=None, silu=True) -> y``
 ``selective_scan_step(u, delta, A, B, C, state, D=None, z=None, delta_bias=None, delta_softplus=True) -> y``
-    one token (x, u, delta, z [B,D]; B, C [B,N] or [B,G,N]) with the state updated in place; no gradient.
+    one token (x, u, delta, z [B,D]; B, C [B,N] or [B,G,N]) with the state updated in place; no gradient.  (A state made in
+    ``torch.inference_mode()`` is updated there only.)
 
 Activations in bf16, fp16 or fp32 (of one type within a call); parameters in any float type; the scan's state in fp32.
 A view of a wider tensor along the channels (the halves of a projection) is read where it lies.
