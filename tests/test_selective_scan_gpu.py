@@ -355,7 +355,7 @@ def train_by_abi(c, groups, softplus=True):
         setattr(a, n + "_token", c[n].stride(1))
     like = {"y": "u", "state": "state", "gu": "u", "gdelta": "u", "gz": "u", "gB": "B", "gC": "B", "gA": "A", "gD": "D", "gbias": "D",
             "gstate": "state"}
-    out = {n: torch.empty_like(c[t]) for n, t in like.items()}
+    out = {n: torch.empty_like(c[t], memory_format=torch.contiguous_format) for n, t in like.items()}
     for f, t in (("A", c["A"]), ("Dskip", c["D"]), ("delta_bias", c["delta_bias"]), ("state_in", c["state"]), ("gy", c["gy"]),
                  ("gstate_out", c["gs"]), ("state_out", out["state"]), ("gstate_in", out["gstate"]),
                  *((n, out[n]) for n in ("y", "gu", "gdelta", "gz", "gB", "gC", "gA", "gD", "gbias"))):
