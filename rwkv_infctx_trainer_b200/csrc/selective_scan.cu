@@ -247,7 +247,7 @@ __device__ __forceinline__ void store_states(float *p, size_t at, int n0, int N,
     }
 }
 // A log2(e).  An infinite A (the exponential of a large parameter), or one whose product is, becomes the largest number: its decay
-// is zero all the same, and a step of zero keeps the state.
+// is zero all the same (for steps above 1e-36), and a step of zero keeps the state.
 __device__ __forceinline__ float decay_rate(float A) {
     float x = A * LOG2E;
     asm("max.NaN.f32 %0, %0, %1;" : "+f"(x) : "f"(-3.4e38f));        // (a NaN stays)

@@ -10,7 +10,7 @@ state, with the contract of the WKV ops (state in, state out, the gradient of bo
     ``dt = softplus(delta + delta_bias)``, ``h_t = exp(dt A) h_{t-1} + dt u_t B_t``, ``y_t = (C_t . h_t + D u_t) silu(z_t)``
     per channel and state.  u, delta, z [B,T,D]; B, C [B,T,N] or [B,T,G,N] (channel d uses group d // (D / G));
     A [D,N], 1 <= N <= 64; D, delta_bias [D]; state fp32 [B,D,N] (None: zeros).  Without z there is no gate.  An A of -inf forgets
-    the state at any step above zero; a step of zero keeps it.
+    the state at any step above 1e-36; a step of zero keeps it.
 
 Both are differentiable w.r.t. every tensor, the state included (once, and not in forward mode: anything else is refused).  Any T >= 0
 up to 2^31 - 273.
