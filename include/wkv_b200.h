@@ -363,6 +363,36 @@ int wkv_selective_scan_forward(const wkv_selective_scan_args_t *a, void *stream)
 size_t wkv_selective_scan_backward_workspace(const wkv_selective_scan_args_t *a);
 int wkv_selective_scan_backward(const wkv_selective_scan_args_t *a, void *stream);
 
+/* wkv_gated_recurrence_*: per channel, with gates r = sigmoid(decay_gate), i = sigmoid(input_gate),
+ *     a_t = exp(-c softplus(decay) r_t),  h_t = a_t h_{t-1} + sqrt(1 - a_t^2) i_t x_t,  y_t = h_t silu(z_t)
+ *   x, input_gate, decay_gate, z (or NULL: y = h) [B,T,D] in `dtype`, each with its own batch and
+ *   token stride (elements); decay [D], the states [B,D]: fp32; c > 0.  state_out may be
+ *   state_in's memory.  A decay gate of minus infinity keeps the state and takes no input.
+ *   ckpt (wkv_gated_recurrence_ckpt_bytes()): states that the forward call leaves for the backward
+ *   call, which needs them.  gy [B,T,D] contiguous.  Gradients: gx, ginput_gate, gdecay_gate, gz
+ *   [B,T,D] in dtype; gdecay, gstate_in fp32.  D is at most 2^22, T at most 2^31 - 4097. */
+typedef struct wkv_gated_recurrence_args {
+    int B, T, D, dtype;
+    float c;
+    const void *x, *input_gate, *decay_gate, *z;
+    long long x_batch, x_token, i_batch, i_token, r_batch, r_token, z_batch, z_token;
+    const float *decay, *state_in;
+    void *y;
+    float *state_out;
+    const void *gy;
+    const float *gstate_out;
+    void *gx, *ginput_gate, *gdecay_gate, *gz;
+    float *gdecay, *gstate_in;
+    void *ckpt;
+    size_t ckpt_bytes;
+    void *workspace;
+    size_t workspace_bytes;
+} wkv_gated_recurrence_args_t;
+size_t wkv_gated_recurrence_ckpt_bytes(const wkv_gated_recurrence_args_t *a);
+int wkv_gated_recurrence_forward(const wkv_gated_recurrence_args_t *a, void *stream);
+size_t wkv_gated_recurrence_backward_workspace(const wkv_gated_recurrence_args_t *a);
+int wkv_gated_recurrence_backward(const wkv_gated_recurrence_args_t *a, void *stream);
+
 /* Library build identification: "wkv_b200 <n> sm_100a". */
 const char *wkv_version(void);
 

@@ -5,6 +5,7 @@ from . import _lib
 from ._lib import (WKV_PATH_AUTO, WKV_PATH_CHUNKED, WKV_PATH_SCALAR, WKV_STATE_KV, WKV_STATE_VK,
                    WKV_W_NEGEXP, WKV_W_RAW)
 from .norm import rms_norm, rms_norm_q8
+from .recurrence import gated_recurrence, gated_recurrence_step
 from .ssm import causal_conv, causal_conv_step, selective_scan, selective_scan_step
 from .timemix import ddlerp, lnx_gate
 from .timemix_block import RWKV_TimeMix, RWKV_TimeMix6_0, RWKV_TimeMix_v4, TimeMixState
@@ -22,5 +23,5 @@ __all__ = [
     "WKV6", "wkv6", "WKV6STATE_CUDA", "RUN_WKV6STATE_CUDA", "wkv6state_cuda_kernel",
     "wkv6_cuda_kernel", "lnx_gate", "ddlerp", "RWKV_TimeMix", "RWKV_TimeMix6_0",
     "RWKV_TimeMix_v4", "TimeMixState", "rms_norm", "rms_norm_q8", "causal_conv", "causal_conv_step",
-    "selective_scan", "selective_scan_step",
+    "selective_scan", "selective_scan_step", "gated_recurrence", "gated_recurrence_step",
 ]

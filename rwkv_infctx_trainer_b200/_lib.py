@@ -75,6 +75,17 @@ class SelectiveScanArgs(ctypes.Structure):
     ]
 
 
+class GatedRecurrenceArgs(ctypes.Structure):
+    _fields_ = [
+        ("B", ctypes.c_int), ("T", ctypes.c_int), ("D", ctypes.c_int), ("dtype", ctypes.c_int), ("c", ctypes.c_float),
+        ("x", _vp), ("input_gate", _vp), ("decay_gate", _vp), ("z", _vp),
+        *((f"{n}_{s}", ctypes.c_longlong) for n in ("x", "i", "r", "z") for s in ("batch", "token")),
+        ("decay", _vp), ("state_in", _vp), ("y", _vp), ("state_out", _vp), ("gy", _vp), ("gstate_out", _vp),
+        ("gx", _vp), ("ginput_gate", _vp), ("gdecay_gate", _vp), ("gz", _vp), ("gdecay", _vp), ("gstate_in", _vp),
+        ("ckpt", _vp), ("ckpt_bytes", ctypes.c_size_t), ("workspace", _vp), ("workspace_bytes", ctypes.c_size_t),
+    ]
+
+
 EXPORTS = [
     "wkv_error_string", "wkv_version", "wkv56_uses_chunked", "wkv56_state_ckpt_bytes",
     "wkv4_forward_workspace", "wkv4_forward", "wkv4_backward_workspace", "wkv4_backward",
@@ -89,6 +100,8 @@ EXPORTS = [
     "wkv_causal_conv_forward", "wkv_causal_conv_backward_workspace", "wkv_causal_conv_backward",
     "wkv_selective_scan_ckpt_bytes", "wkv_selective_scan_forward_workspace", "wkv_selective_scan_forward",
     "wkv_selective_scan_backward_workspace", "wkv_selective_scan_backward",
+    "wkv_gated_recurrence_ckpt_bytes", "wkv_gated_recurrence_forward",
+    "wkv_gated_recurrence_backward_workspace", "wkv_gated_recurrence_backward",
 ]
 
 _lib = None
@@ -181,7 +194,8 @@ def load() -> ctypes.CDLL:
     lib.wkv_ddlerp_backward_workspace.argtypes = [i, i, i, i]
     lib.wkv_ddlerp_backward.restype = i
     lib.wkv_ddlerp_backward.argtypes = [i, i, i, i] + [f] * 10 + [_vp, sz, _vp]
-    for name, args in (("rms_norm", RmsNormArgs), ("causal_conv", CausalConvArgs), ("selective_scan", SelectiveScanArgs)):
+    for name, args in (("rms_norm", RmsNormArgs), ("causal_conv", CausalConvArgs), ("selective_scan", SelectiveScanArgs),
+                       ("gated_recurrence", GatedRecurrenceArgs)):
         for d in ("forward", "backward"):
             fn = getattr(lib, f"wkv_{name}_{d}")
             fn.restype = i
@@ -190,8 +204,10 @@ def load() -> ctypes.CDLL:
                 ws = getattr(lib, f"wkv_{name}_{d}_workspace")
                 ws.restype = sz
                 ws.argtypes = [ctypes.POINTER(args)]
-    lib.wkv_selective_scan_ckpt_bytes.restype = sz
-    lib.wkv_selective_scan_ckpt_bytes.argtypes = [ctypes.POINTER(SelectiveScanArgs)]
+    for name, args in (("selective_scan", SelectiveScanArgs), ("gated_recurrence", GatedRecurrenceArgs)):
+        fn = getattr(lib, f"wkv_{name}_ckpt_bytes")
+        fn.restype = sz
+        fn.argtypes = [ctypes.POINTER(args)]
     for v in ("wkv5", "wkv6"):
         for d in ("forward", "backward"):
             fn = getattr(lib, f"{v}_{d}")

@@ -1,58 +1,9 @@
-// PyTorch binding of the norm, the short causal convolution and the selective scan (see rms_norm.cu, causal_conv.cu,
-// selective_scan.cu): argument checks, allocation, autograd nodes.
-#include "native_ops.h"
+// PyTorch binding of the norm, the short causal convolution, the selective scan and the gated recurrence (see rms_norm.cu,
+// causal_conv.cu, selective_scan.cu, gated_recurrence.cu): argument checks, allocation, autograd nodes.
+#include "native_args.h"
 
 namespace wkv_native {
 namespace {
-
-Tensor opt(const OptTensor &t) { return t.has_value() ? *t : Tensor(); }
-
-int small(int64_t n, const char *what) {
-    TORCH_CHECK_VALUE(n <= std::numeric_limits<int>::max(), what, " is too large: ", n);
-    return (int)n;
-}
-void check_type(const Tensor &t, at::ScalarType dt, const char *name) {
-    TORCH_CHECK_TYPE(!t.defined() || t.scalar_type() == dt, name, " must be ", dt, ", got ", t.scalar_type());
-}
-void check_param(const Tensor &t, const char *name) {
-    TORCH_CHECK_TYPE(!t.defined() || at::isFloatingType(t.scalar_type()), name, " must be a floating point tensor");
-}
-void check_sizes(const Tensor &t, at::IntArrayRef want, const char *name) {
-    TORCH_CHECK_VALUE(!t.defined() || t.sizes() == want, name, " must have shape ", want, ", got ", t.sizes());
-}
-// the calls that update a state in place have no backward pass
-void refuse_grad(std::initializer_list<const Tensor *> ts, const char *call, const char *other) {
-    TORCH_CHECK(!wants_grad(ts), call, " updates the state in place and has no gradient: call it under torch.no_grad(), or ", other);
-}
-void check_in_place(const Tensor &state, const char *call) {
-    TORCH_CHECK_VALUE(state.is_contiguous(), call, ": the state is updated in place and must be contiguous");
-}
-// Before the launch: torch refuses this for a tensor made in inference mode, outside of it, and then nothing may have changed.
-void changes_in_place(const Tensor &state) { torch::autograd::impl::bump_version(state); }
-
-// Rows of adjacent channels with any stride between rows and between tokens, as the kernels take them: a view of a wider
-// tensor stays one, anything else is copied.
-struct Rows {
-    Tensor t;
-    int64_t batch = 0, token = 0;
-};
-// t: [B, T, ...], or [B, ...] for one token, with everything behind one run of `n` elements
-Rows rows_of(const Tensor &t, int64_t n, bool one_token) {
-    if (!t.defined()) return {};
-    const int64_t lead = one_token ? 1 : 2;
-    const auto sizes = t.sizes(), strides = t.strides();
-    int64_t run = 1;
-    bool packed = true;
-    for (int64_t i = t.dim() - 1; i >= lead; i--) {
-        if (sizes[i] != 1 && strides[i] != run) packed = false;
-        run *= sizes[i];
-    }
-    // (offsets inside a block of tokens are 32-bit, and a dimension of one element may have any stride)
-    if (!one_token && sizes[1] > 1 && strides[1] > (1 << 26)) packed = false;
-    const Tensor c = packed ? t : t.contiguous();
-    const int64_t token = one_token || c.size(1) <= 1 ? n : c.stride(1);
-    return {c, c.size(0) > 1 ? c.stride(0) : token, token};
-}
 
 // ------------------------------------------------------------------------------ norm
 struct NormCall {
@@ -437,6 +388,130 @@ Tensor selective_scan_step(const Tensor &u, const Tensor &delta, const Tensor &A
     return y;
 }
 
+// ------------------------------------------------------------------------------ gated recurrence
+struct RecCall {
+    Rows x, ig, rg, z;
+    Tensor decay, state;
+    wkv_gated_recurrence_args_t a = {};
+};
+// x, gates, z [B,T,D]; decay [D]; state [B,D]; for one token without T
+void check_rec(const Tensor &x, const Tensor &ig, const Tensor &rg, const Tensor &decay, const Tensor &z, const Tensor &state, double c) {
+    const auto dt = x.scalar_type();
+    dtype_code(dt);
+    for (auto [t, name] : {std::pair<const Tensor *, const char *>{&ig, "input_gate"}, {&rg, "decay_gate"}, {&z, "z"}}) {
+        check_type(*t, dt, name);
+        check_sizes(*t, x.sizes(), name);
+    }
+    check_param(decay, "decay");
+    check_param(state, "state");
+    check_sizes(decay, {x.size(-1)}, "decay");
+    check_sizes(state, {x.size(0), x.size(-1)}, "state");
+    TORCH_CHECK_VALUE(c > 0 && c <= 1e6, "c must be above 0 and at most 1e6, got ", c);
+    require_cuda({&x, &ig, &rg, &decay, &z, &state});
+}
+RecCall rec_call(const Tensor &x, const Tensor &ig, const Tensor &rg, const Tensor &decay, const Tensor &z, const Tensor &state, double c) {
+    RecCall r;
+    const bool one = x.dim() == 2;
+    const int64_t d = x.size(-1);
+    r.x = rows_of(x, d, one); r.ig = rows_of(ig, d, one); r.rg = rows_of(rg, d, one); r.z = rows_of(z, d, one);
+    r.decay = as_contig(decay, at::kFloat);
+    if (state.defined()) r.state = as_contig(state, at::kFloat);
+    wkv_gated_recurrence_args_t &a = r.a;
+    a.B = small(x.size(0), "B"); a.T = one ? 1 : small(x.size(1), "T"); a.D = small(d, "D");
+    a.dtype = dtype_code(x.scalar_type()); a.c = (float)c;
+    a.x = ptr(r.x.t); a.input_gate = ptr(r.ig.t); a.decay_gate = ptr(r.rg.t); a.z = ptr(r.z.t);
+    a.x_batch = r.x.batch; a.x_token = r.x.token; a.i_batch = r.ig.batch; a.i_token = r.ig.token;
+    a.r_batch = r.rg.batch; a.r_token = r.rg.token; a.z_batch = r.z.batch; a.z_token = r.z.token;
+    a.decay = (const float *)ptr(r.decay); a.state_in = (const float *)ptr(r.state);
+    return r;
+}
+
+struct GatedRecurrenceBackward : OpNode {
+    double c;
+    at::ScalarType decay_type, s_type;
+    std::string name() const override { return "GatedRecurrenceBackward"; }
+    variable_list gradients(variable_list &&grads) override {
+        at::AutoDispatchBelowADInplaceOrView below;
+        const variable_list st = unpack();
+        const Tensor &x = st[0];
+        const Tensor ckpt = st[5].defined() ? contig(st[5]) : st[5];
+        c10::cuda::OptionalCUDAGuard guard(x.device());
+        RecCall r = rec_call(x, st[1], st[2], st[3], st[4], Tensor(), c);
+        const auto dt = x.scalar_type();
+        const int64_t B = x.size(0), D = x.size(2);
+        const Tensor gy = grads[0].defined() ? as_contig(grads[0], dt) : Tensor(), gs = grads[1].defined() ? as_contig(grads[1], at::kFloat) : Tensor();
+        auto want = [&](size_t i, at::IntArrayRef sizes, at::ScalarType t) { return task_should_compute_output(i) ? fresh(sizes, t, x) : Tensor(); };
+        Tensor gx = want(0, x.sizes(), dt), gi = want(1, x.sizes(), dt), gr = want(2, x.sizes(), dt), gd = want(3, {D}, at::kFloat),
+               gz = want(4, x.sizes(), dt), gstate = want(5, {B, D}, at::kFloat);
+        wkv_gated_recurrence_args_t &a = r.a;
+        a.gy = ptr(gy); a.gstate_out = (const float *)ptr(gs);
+        a.gx = ptr(gx); a.ginput_gate = ptr(gi); a.gdecay_gate = ptr(gr); a.gz = ptr(gz);
+        a.gdecay = (float *)ptr(gd); a.gstate_in = (float *)ptr(gstate);
+        a.ckpt = ptr(ckpt);
+        a.ckpt_bytes = ckpt.defined() ? (size_t)ckpt.numel() : 0;
+        a.workspace_bytes = wkv_gated_recurrence_backward_workspace(&a);
+        Tensor ws = bytes_like(x, a.workspace_bytes);
+        a.workspace = ptr(ws);
+        check(wkv_gated_recurrence_backward(&a, stream_of(x)), "wkv_gated_recurrence_backward");
+        auto as = [](const Tensor &g, at::ScalarType t) { return g.defined() ? g.to(t) : g; };
+        return {gx, gi, gr, as(gd, decay_type), gz, as(gstate, s_type)};
+    }
+};
+
+std::tuple<Tensor, Tensor> gated_recurrence(const Tensor &x, const Tensor &ig, const Tensor &rg, const Tensor &decay, const OptTensor &z_,
+                                            const OptTensor &state_, double c) {
+    const Tensor z = opt(z_), state = opt(state_);
+    TORCH_CHECK_VALUE(x.dim() == 3, "x must be [B,T,D], got ", x.sizes());
+    check_rec(x, ig, rg, decay, z, state, c);
+    c10::cuda::OptionalCUDAGuard guard(x.device());
+    const bool save = wants_grad({&x, &ig, &rg, &decay, &z, &state});
+    std::shared_ptr<GatedRecurrenceBackward> node;
+    if (save) {
+        node = make_node<GatedRecurrenceBackward>({x, ig, rg, decay, z, state});
+        node->c = c;
+        node->decay_type = decay.scalar_type();
+        node->s_type = state.defined() ? state.scalar_type() : at::kFloat;
+    }
+    Tensor y, s;
+    {
+        at::AutoDispatchBelowADInplaceOrView below;
+        RecCall r = rec_call(x, ig, rg, decay, z, state, c);
+        y = fresh(x.sizes(), x.scalar_type(), x);
+        s = fresh({x.size(0), x.size(2)}, at::kFloat, x);
+        r.a.y = ptr(y); r.a.state_out = (float *)ptr(s);
+        Tensor ckpt;
+        if (save) {
+            r.a.ckpt_bytes = wkv_gated_recurrence_ckpt_bytes(&r.a);
+            ckpt = bytes_like(x, r.a.ckpt_bytes);
+            r.a.ckpt = ptr(ckpt);
+        }
+        check(wkv_gated_recurrence_forward(&r.a, stream_of(x)), "wkv_gated_recurrence_forward");
+        if (save) node->keep({r.x.t, r.ig.t, r.rg.t, r.decay, r.z.t, ckpt});
+    }
+    if (save) {
+        torch::autograd::set_history(y, node);
+        torch::autograd::set_history(s, node);
+    }
+    return {y, s};
+}
+
+Tensor gated_recurrence_step(const Tensor &x, const Tensor &ig, const Tensor &rg, const Tensor &decay, const Tensor &state, const OptTensor &z_,
+                             double c) {
+    const Tensor z = opt(z_);
+    TORCH_CHECK_VALUE(x.dim() == 2, "x must be [B,D], got ", x.sizes());
+    refuse_grad({&x, &ig, &rg, &decay, &z, &state}, "gated_recurrence_step", "gated_recurrence");
+    check_type(state, at::kFloat, "state");
+    check_in_place(state, "gated_recurrence_step");
+    check_rec(x, ig, rg, decay, z, state, c);
+    c10::cuda::OptionalCUDAGuard guard(x.device());
+    RecCall r = rec_call(x, ig, rg, decay, z, state, c);
+    Tensor y = fresh(x.sizes(), x.scalar_type(), x);
+    r.a.y = ptr(y); r.a.state_out = (float *)ptr(state);
+    changes_in_place(state);
+    check(wkv_gated_recurrence_forward(&r.a, stream_of(x)), "wkv_gated_recurrence_forward");
+    return y;
+}
+
 }  // namespace
 }  // namespace wkv_native
 
@@ -448,4 +523,6 @@ void bind_ssm(py::module_ &m) {
     m.def("causal_conv_step", &causal_conv_step);
     m.def("selective_scan", &selective_scan);
     m.def("selective_scan_step", &selective_scan_step);
+    m.def("gated_recurrence", &gated_recurrence);
+    m.def("gated_recurrence_step", &gated_recurrence_step);
 }
