@@ -393,6 +393,43 @@ int wkv_gated_recurrence_forward(const wkv_gated_recurrence_args_t *a, void *str
 size_t wkv_gated_recurrence_backward_workspace(const wkv_gated_recurrence_args_t *a);
 int wkv_gated_recurrence_backward(const wkv_gated_recurrence_args_t *a, void *stream);
 
+/* wkv_linear_*: matrix products with their epilogue, and their gradients (bf16 or fp16, fp32 sums; wkv_linear_args_t.pair = 0)
+ *     y = act(x w0^T + bias) mul + residual
+ *   or a gated pair (pair = 1; without bias, mul and residual)
+ *     y = act(x w0^T) (x w1^T)
+ *   x [rows,K], w0, w1 [N,K] with row strides (elements; columns adjacent); bias [N] in bias_dtype;
+ *   mul, residual, y [rows,N] contiguous; all but the bias in `dtype`.  act: WKV_ACT_*.  Any size and alignment is
+ *   taken; rows of 16-byte aligned pieces are read where they lie, others are copied into the
+ *   workspace first.
+ *   saved (wkv_linear_saved_bytes() bytes, or NULL): pre-activations that the forward call leaves
+ *   for the backward call, which needs them where that is not 0 bytes.
+ *   Gradients (NULL: not wanted): gx [rows,K], gw0, gw1 [N,K], gmul [rows,N] contiguous in dtype, gbias
+ *   [N] in bias_dtype; that of the residual is gy.  The gradient of the pre-activation is rounded
+ *   to dtype once, for the products; gbias is summed before that rounding.
+ *   status: device-visible word or NULL; WKV_LINEAR_TIMEOUT is set in it when a bounded wait ran out
+ *   and the results are invalid.  rows, K and N below 2^31 - 256. */
+enum { WKV_ACT_NONE = 0, WKV_ACT_SILU = 1, WKV_ACT_GELU = 2, WKV_ACT_RELU2 = 3, WKV_ACT_SIGMOID = 4 };
+enum { WKV_LINEAR_TIMEOUT = 64 };
+typedef struct wkv_linear_args {
+    long long rows, K, N;
+    int dtype, bias_dtype, act, pair;
+    const void *x, *w0, *w1, *bias, *mul, *residual;
+    long long x_row, w0_row, w1_row;
+    void *y;
+    const void *gy;
+    void *gx, *gw0, *gw1, *gbias, *gmul;
+    void *saved;
+    size_t saved_bytes;
+    void *workspace;
+    size_t workspace_bytes;
+    int *status;
+} wkv_linear_args_t;
+size_t wkv_linear_saved_bytes(const wkv_linear_args_t *a);
+size_t wkv_linear_forward_workspace(const wkv_linear_args_t *a);
+int wkv_linear_forward(const wkv_linear_args_t *a, void *stream);
+size_t wkv_linear_backward_workspace(const wkv_linear_args_t *a);
+int wkv_linear_backward(const wkv_linear_args_t *a, void *stream);
+
 /* Library build identification: "wkv_b200 <n> sm_100a". */
 const char *wkv_version(void);
 

@@ -4,6 +4,7 @@ libwkv_b200.so; there is no fallback if that fails."""
 from . import _lib
 from ._lib import (WKV_PATH_AUTO, WKV_PATH_CHUNKED, WKV_PATH_SCALAR, WKV_STATE_KV, WKV_STATE_VK,
                    WKV_W_NEGEXP, WKV_W_RAW)
+from .linear import gated_linear, linear_act
 from .norm import rms_norm, rms_norm_q8
 from .recurrence import gated_recurrence, gated_recurrence_step
 from .ssm import causal_conv, causal_conv_step, selective_scan, selective_scan_step
@@ -24,4 +25,5 @@ __all__ = [
     "wkv6_cuda_kernel", "lnx_gate", "ddlerp", "RWKV_TimeMix", "RWKV_TimeMix6_0",
     "RWKV_TimeMix_v4", "TimeMixState", "rms_norm", "rms_norm_q8", "causal_conv", "causal_conv_step",
     "selective_scan", "selective_scan_step", "gated_recurrence", "gated_recurrence_step",
+    "linear_act", "gated_linear",
 ]

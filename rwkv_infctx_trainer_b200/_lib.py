@@ -86,6 +86,18 @@ class GatedRecurrenceArgs(ctypes.Structure):
     ]
 
 
+class LinearArgs(ctypes.Structure):
+    _fields_ = [
+        ("rows", ctypes.c_longlong), ("K", ctypes.c_longlong), ("N", ctypes.c_longlong),
+        ("dtype", ctypes.c_int), ("bias_dtype", ctypes.c_int), ("act", ctypes.c_int), ("pair", ctypes.c_int),
+        ("x", _vp), ("w0", _vp), ("w1", _vp), ("bias", _vp), ("mul", _vp), ("residual", _vp),
+        ("x_row", ctypes.c_longlong), ("w0_row", ctypes.c_longlong), ("w1_row", ctypes.c_longlong),
+        ("y", _vp), ("gy", _vp), ("gx", _vp), ("gw0", _vp), ("gw1", _vp), ("gbias", _vp), ("gmul", _vp),
+        ("saved", _vp), ("saved_bytes", ctypes.c_size_t), ("workspace", _vp), ("workspace_bytes", ctypes.c_size_t),
+        ("status", _vp),
+    ]
+
+
 EXPORTS = [
     "wkv_error_string", "wkv_version", "wkv56_uses_chunked", "wkv56_state_ckpt_bytes",
     "wkv4_forward_workspace", "wkv4_forward", "wkv4_backward_workspace", "wkv4_backward",
@@ -102,6 +114,8 @@ EXPORTS = [
     "wkv_selective_scan_backward_workspace", "wkv_selective_scan_backward",
     "wkv_gated_recurrence_ckpt_bytes", "wkv_gated_recurrence_forward",
     "wkv_gated_recurrence_backward_workspace", "wkv_gated_recurrence_backward",
+    "wkv_linear_saved_bytes", "wkv_linear_forward_workspace", "wkv_linear_forward", "wkv_linear_backward_workspace",
+    "wkv_linear_backward",
 ]
 
 _lib = None
@@ -195,17 +209,17 @@ def load() -> ctypes.CDLL:
     lib.wkv_ddlerp_backward.restype = i
     lib.wkv_ddlerp_backward.argtypes = [i, i, i, i] + [f] * 10 + [_vp, sz, _vp]
     for name, args in (("rms_norm", RmsNormArgs), ("causal_conv", CausalConvArgs), ("selective_scan", SelectiveScanArgs),
-                       ("gated_recurrence", GatedRecurrenceArgs)):
+                       ("gated_recurrence", GatedRecurrenceArgs), ("linear", LinearArgs)):
         for d in ("forward", "backward"):
             fn = getattr(lib, f"wkv_{name}_{d}")
             fn.restype = i
             fn.argtypes = [ctypes.POINTER(args), _vp]
-            if d == "backward" or name == "selective_scan":
+            if d == "backward" or name in ("selective_scan", "linear"):
                 ws = getattr(lib, f"wkv_{name}_{d}_workspace")
                 ws.restype = sz
                 ws.argtypes = [ctypes.POINTER(args)]
-    for name, args in (("selective_scan", SelectiveScanArgs), ("gated_recurrence", GatedRecurrenceArgs)):
-        fn = getattr(lib, f"wkv_{name}_ckpt_bytes")
+    for name, args in (("selective_scan_ckpt", SelectiveScanArgs), ("gated_recurrence_ckpt", GatedRecurrenceArgs), ("linear_saved", LinearArgs)):
+        fn = getattr(lib, f"wkv_{name}_bytes")
         fn.restype = sz
         fn.argtypes = [ctypes.POINTER(args)]
     for v in ("wkv5", "wkv6"):

@@ -1,0 +1,601 @@
+// Matrix products with their epilogue, forward and backward:
+//
+//   linear_act    y = act(z) mul + residual,  z = x W^T + bias
+//       backward  gz = gy mul act'(z),  gx = gz W,  gW = gz^T x,  gbias = sum gz,  gmul = gy act(z),  gresidual = gy
+//   gated_linear  y = act(g) u,  g = x Wg^T,  u = x Wu^T
+//       backward  gu = gy act(g),  gg = gy u act'(g),  gx = gg Wg + gu Wu,  gWg = gg^T x,  gWu = gu^T x
+//
+// The products run on the tile kernel of linear_gemm.cuh.  The pair's forward pass is one product whose tile of 256 columns is half
+// of each matrix (a CTA of the pair brings the rows of one), so that g and u of an element end up in one thread; its gradient of x
+// is one product over both contractions, and that of the matrices one over the rows of both.  Few rows (a decoded token) are bound
+// by reading the matrix: k_few_rows streams it through registers once.
+//
+// What the forward pass keeps: the pre-activations, in the activations' type (the gradient differs from one taken at the unrounded z
+// by act'' times half a step of z, as much as rounding the gradient itself).
+#include <algorithm>
+
+#include "linear_gemm.cuh"
+#include "tma_host.cuh"
+#include "wkv_internal.h"
+
+namespace wkv {
+namespace linear {
+namespace {
+
+constexpr unsigned WAIT_LIMIT = 4000000u;
+
+inline long long up8(long long n) { return (n + 7) & ~7ll; }
+
+// ------------------------------------------------------------------------------------------ few rows
+// A CTA has 16 rows of the matrix (of a pair: 8 of each), its 8 warps every eighth run of 64 contraction steps; the warps' sums meet
+// in shared memory in a fixed order.  mma.sync with the matrix as the 16-row operand and the rows of x as the 8 columns: the
+// contraction steps may be numbered in any order that both operands share, so that a lane's 16-byte piece (8 steps of one row) is
+// its part of two instructions as it is, without a turn through shared memory.  (The tensor core's rate does not matter here.)
+template <typename F>
+__device__ __forceinline__ void mma16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    if constexpr (std::is_same<F, __nv_bfloat16>::value)
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                     : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+    else
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                     : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+constexpr int FEW_ROWS = 16, FEW_WARPS = 8;
+
+struct FewArgs {
+    int M, K, N;                       // M: rows of x
+    const void *x, *w[2];
+    long long x_row, w_row[2];
+    Epi e;
+};
+
+// VEC: every row of x and of the matrices is made of whole 16-byte pieces
+template <typename F, int TOKENS, bool PAIR, bool VEC>
+__global__ void __launch_bounds__(32 * FEW_WARPS) k_few_rows(const FewArgs g) {
+    pdl_wait();
+    pdl_trigger();
+    constexpr int NT = TOKENS / 8, OUT = PAIR ? 8 : 16, UNROLL = VEC ? 2 : 1;
+    __shared__ float part[FEW_WARPS][16][TOKENS + 1];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, q = lane >> 2, c = lane & 3;
+    const int row0 = blockIdx.x * OUT;
+    // this lane's two rows of the matrix: q and q + 8 of the tile (of a pair: row q of each)
+    const int r0 = row0 + q, r1 = PAIR ? row0 + q : row0 + q + 8;
+    const F *w0 = (const F *)g.w[0] + (size_t)min(r0, g.N - 1) * g.w_row[0];
+    const F *w1 = PAIR ? (const F *)g.w[1] + (size_t)min(r1, g.N - 1) * g.w_row[1] : (const F *)g.w[0] + (size_t)min(r1, g.N - 1) * g.w_row[0];
+    const F *x[NT];
+    bool live[NT];
+#pragma unroll
+    for (int j = 0; j < NT; j++) {
+        live[j] = 8 * j + q < g.M;
+        x[j] = (const F *)g.x + (size_t)(live[j] ? 8 * j + q : 0) * g.x_row;
+    }
+    float d[NT][4];
+#pragma unroll
+    for (int j = 0; j < NT; j++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) d[j][i] = 0.f;
+    auto run = [&](int k0, auto all) {
+        constexpr bool whole = decltype(all)::value;
+        Raw<F, 8> a[UNROLL][2][2], b[UNROLL][NT][2];
+#pragma unroll
+        for (int s = 0; s < UNROLL; s++) {
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                const int k = k0 + s * 64 * FEW_WARPS + h * 32 + c * 8, n = whole ? 8 : min(8, g.K - k);
+                if (whole || n > 0) {
+                    a[s][0][h].load(w0 + k, VEC, n);
+                    a[s][1][h].load(w1 + k, VEC, n);
+                } else {
+                    a[s][0][h].zero();
+                    a[s][1][h].zero();
+                }
+#pragma unroll
+                for (int j = 0; j < NT; j++) {
+                    if (live[j] && (whole || n > 0)) b[s][j][h].load(x[j] + k, VEC, n);
+                    else b[s][j][h].zero();
+                }
+            }
+        }
+#pragma unroll
+        for (int s = 0; s < UNROLL; s++)
+#pragma unroll
+            for (int h = 0; h < 2; h++)
+#pragma unroll
+                for (int j = 0; j < NT; j++) {
+                    mma16<F>(d[j], a[s][0][h].w[0], a[s][1][h].w[0], a[s][0][h].w[1], a[s][1][h].w[1], b[s][j][h].w[0], b[s][j][h].w[1]);
+                    mma16<F>(d[j], a[s][0][h].w[2], a[s][1][h].w[2], a[s][0][h].w[3], a[s][1][h].w[3], b[s][j][h].w[2], b[s][j][h].w[3]);
+                }
+    };
+    int k0 = warp * 64;
+    for (; k0 + (UNROLL - 1) * 64 * FEW_WARPS + 64 <= g.K; k0 += UNROLL * 64 * FEW_WARPS) run(k0, std::true_type{});
+    if (k0 < g.K) run(k0, std::false_type{});
+#pragma unroll
+    for (int j = 0; j < NT; j++) {
+        part[warp][q][8 * j + 2 * c] = d[j][0];
+        part[warp][q][8 * j + 2 * c + 1] = d[j][1];
+        part[warp][q + 8][8 * j + 2 * c] = d[j][2];
+        part[warp][q + 8][8 * j + 2 * c + 1] = d[j][3];
+    }
+    __syncthreads();
+    // neighbouring threads take neighbouring columns of y
+    if (threadIdx.x < OUT * TOKENS) {
+        const int o = threadIdx.x % OUT, t = threadIdx.x / OUT, col = row0 + o;
+        if (t < g.M && col < g.N) {
+            float f = 0.f, u = 0.f;
+#pragma unroll
+            for (int w = 0; w < FEW_WARPS; w++) {
+                f += part[w][o][t];
+                if (PAIR) u += part[w][o + 8][t];
+            }
+            finish1<F, PAIR ? EPI_GATED : EPI_LINEAR>(g.e, 0, t, col, f, u, !PAIR && g.e.bias != nullptr ? param_at(g.e.bias, g.e.bias_dtype, col) : 0.f);
+        }
+    }
+}
+
+// ------------------------------------------------------------------------------------------ split contraction
+// the parts' sums in order, then the epilogue: a thread has 8 columns of a row
+template <typename F>
+__global__ void __launch_bounds__(256) k_fold_split(const Epi e, long long M, int N, int splits) {
+    pdl_wait();
+    pdl_trigger();
+    const int pieces = (N + 7) / 8;
+    const long long i = (long long)blockIdx.x * 256 + threadIdx.x, row = i / pieces;
+    if (row >= M) return;
+    const int col = (int)(i - row * pieces) * 8, n = N - col;
+    float f[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, bias[8];
+    for (int s = 0; s < splits; s++) {
+        const float4 *p = reinterpret_cast<const float4 *>(e.part + ((size_t)s * M + row) * e.part_row + col);
+        const float4 a = p[0], b = p[1];
+        f[0] += a.x; f[1] += a.y; f[2] += a.z; f[3] += a.w; f[4] += b.x; f[5] += b.y; f[6] += b.z; f[7] += b.w;
+    }
+#pragma unroll
+    for (int k = 0; k < 8; k++) bias[k] = e.bias != nullptr && k < n ? param_at(e.bias, e.bias_dtype, col + k) : 0.f;
+    finish8<F, EPI_LINEAR>(e, 0, row, col, n, f, f, bias);
+}
+
+// ------------------------------------------------------------------------------------------ gradient of the pre-activation
+struct GradArgs {
+    long long rows;
+    int N, act, vec, rows_per;
+    const void *gy, *mul, *z[2];
+    long long z_row;
+    void *gz[2], *gmul;
+    long long gz_row;
+    float *part;                        // [gridDim.y, N] sums of gz over a CTA's rows
+};
+
+// act(z) and its derivative
+__device__ __forceinline__ void act_both(int act, float z, float &v, float &d) {
+    if (act == ACT_NONE) {
+        v = z; d = 1.f;
+    } else if (act == ACT_RELU2) {
+        const float p = z > 0.f ? z : (z == z ? 0.f : z);
+        v = p * p; d = 2.f * p;
+    } else if (act == ACT_GELU) {
+        const float phi = phi_of(z);
+        v = z * phi;
+        d = fmaf(z, 0.3989422804014327f * __expf(-0.5f * z * z), phi);
+    } else {
+        const float s = sigmoid_of(z), n = sigmoid_of(-z);
+        v = act == ACT_SILU ? z * s : s;
+        d = act == ACT_SILU ? s * fmaf(z, n, 1.f) : s * n;
+    }
+}
+
+// a warp walks down rows of 256 columns, 8 a lane; bound by HBM
+template <typename F, bool PAIR>
+__global__ void __launch_bounds__(256) k_grad_act(const GradArgs g) {
+    pdl_wait();
+    pdl_trigger();
+    __shared__ float red[8][256];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, col = blockIdx.x * 256 + lane * 8, n = g.N - col;
+    const bool whole = n >= 8, vec = g.vec && whole;
+    float sum[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    const long long r0 = (long long)blockIdx.y * g.rows_per, r1 = min(g.rows, r0 + g.rows_per);
+    if (n > 0) {
+#pragma unroll 2
+        for (long long row = r0 + warp; row < r1; row += 8) {
+            Raw<F, 8> r;
+            float gy[8], z[8], u[8], m[8], o[8];
+            r.load((const F *)g.gy + row * g.N + col, vec, n);
+            r.get(gy);
+            if (g.z[0] != nullptr) {
+                r.load((const F *)g.z[0] + row * g.z_row + col, whole, n);
+                r.get(z);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; i++) z[i] = 0.f;
+            }
+            if (PAIR) {
+                r.load((const F *)g.z[1] + row * g.z_row + col, whole, n);
+                r.get(u);
+            } else if (g.mul != nullptr) {
+                r.load((const F *)g.mul + row * g.N + col, vec, n);
+                r.get(m);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; i++) m[i] = 1.f;
+            }
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                float v, d;
+                act_both(g.act, z[i], v, d);
+                o[i] = gy[i] * v;
+                m[i] = gy[i] * (PAIR ? u[i] : m[i]) * d;
+                sum[i] += m[i];
+            }
+            if (g.gz[0] != nullptr) {
+                r.put(m);
+                r.store((F *)g.gz[0] + row * g.gz_row + col, whole, n);
+            }
+            if (PAIR) {
+                r.put(o);
+                r.store((F *)g.gz[1] + row * g.gz_row + col, whole, n);
+            } else if (g.gmul != nullptr) {
+                r.put(o);
+                r.store((F *)g.gmul + row * g.N + col, vec, n);
+            }
+        }
+    }
+    if (g.part == nullptr) return;
+#pragma unroll
+    for (int i = 0; i < 8; i++) red[warp][lane * 8 + i] = sum[i];
+    __syncthreads();
+    const int mine = blockIdx.x * 256 + threadIdx.x;
+    if (mine < g.N) {
+        float s = 0.f;
+#pragma unroll
+        for (int w = 0; w < 8; w++) s += red[w][threadIdx.x];
+        g.part[(size_t)blockIdx.y * g.N + mine] = s;
+    }
+}
+
+// rows that do not lie in whole 16-byte pieces -> rows that do
+template <typename F>
+__global__ void __launch_bounds__(256) k_repack(const F *from, long long from_row, F *to, long long to_row, long long rows, int cols) {
+    pdl_wait();
+    pdl_trigger();
+    const int pieces = (cols + 7) / 8;
+    const long long total = rows * pieces;
+    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < total; i += (long long)gridDim.x * 256) {
+        const long long row = i / pieces;
+        const int col = (int)(i - row * pieces) * 8;
+        Raw<F, 8> r;
+        r.load(from + row * from_row + col, false, cols - col);
+        r.store(to + row * to_row + col, true, 8);
+    }
+}
+
+// ------------------------------------------------------------------------------------------ host side
+struct Matrix {
+    const void *p;
+    long long rows, cols, pitch;
+};
+inline bool tma_ready(const void *p, long long pitch) { return aligned16(p) && pitch % 8 == 0 && pitch < (1ll << 38); }
+
+template <typename F>
+int repack(const Matrix &from, void *to, cudaStream_t s) {
+    const long long pitch = up8(from.cols), pieces = from.rows * (pitch / 8);
+    const unsigned grid = (unsigned)std::min<long long>((pieces + 255) / 256, 148 * 16);
+    return launch_chained(k_repack<F>, dim3(grid), dim3(256), 0, s, (const F *)from.p, from.pitch, (F *)to, pitch, from.rows, (int)from.cols);
+}
+
+// Scratch, handed out in order; with a NULL base only counted.
+struct Scratch {
+    char *base;
+    size_t used = 0;
+    void *take(size_t bytes) {
+        const size_t at = used;
+        used += align256(bytes);
+        return base ? base + at : nullptr;
+    }
+};
+
+// The shape of a product and how it is cut.  (us: from the kernel's rates on one B200, the same for every call.)
+struct Cut {
+    int cg, bn, splits, kb_split;
+};
+Cut cut_for(long long m, long long n, int sources, int kb, bool pair) {
+    const long long out256 = pair ? 128 : 256;
+    auto tiles = [&](long long bm, long long bn) { return sources * ((m + bm - 1) / bm) * ((n + bn - 1) / bn); };
+    const int sms = device_sm_count(), pairs = sms / 2;
+    auto waves = [](long long t, int places) { return (double)((t + places - 1) / places); };
+    // a stage of 64 steps takes a tile of 256 x 256 of two SMs 0.29 us, one of 128 x 128 of one SM 0.17; start and end 4 us
+    Cut best = {2, 256, 1, kb};
+    double t_best = waves(tiles(256, out256), pairs) * (0.29 * kb + 1.0);
+    const double t1 = waves(tiles(128, out256 / 2), sms) * (0.17 * kb + 1.0);
+    if (t1 < t_best) { best = {1, 128, 1, kb}; t_best = t1; }
+    if (!pair && sources == 1) {
+        const long long t = tiles(128, 128);
+        for (int s = 2; s <= 16 && kb / s >= 4; s++) {
+            const int len = (kb + s - 1) / s, used = (kb + len - 1) / len;
+            const double ts = waves(t * used, sms) * (0.17 * len + 1.0) + 3.0 + (double)used * m * n * 8e-6 / 4.0;
+            if (ts < t_best) { best = {1, 128, used, len}; t_best = ts; }
+        }
+    }
+    return best;
+}
+size_t split_bytes(const Cut &c, long long m, long long n) { return c.splits > 1 ? (size_t)c.splits * m * up8(n) * 4 : 0; }
+
+template <typename F, int CG, int BN, bool A_MN, bool B_MN, int EPI>
+int launch_gemm(GemmArgs &g, cudaStream_t s) {
+    using T = Tile<CG, BN>;
+    static unsigned char done[64];
+    const auto kern = k_gemm<F, CG, BN, A_MN, B_MN, EPI>;
+    if (!set_max_smem_once(kern, T::SMEM, done)) return WKV_ERR_LAUNCH;
+    const long long items = (long long)g.m_tiles * g.n_tiles * g.splits;
+    const int places = device_sm_count() / CG, grid = (int)std::min<long long>(items, places) * CG;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)grid);
+    cfg.blockDim = dim3(THREADS);
+    cfg.dynamicSmemBytes = T::SMEM;
+    cfg.stream = s;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = CG; attr[1].val.clusterDim.y = 1; attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = CG > 1 ? 2 : 1;
+    launch_count.fetch_add(1, std::memory_order_relaxed);
+    return cudaLaunchKernelEx(&cfg, kern, g) == cudaSuccess ? WKV_OK : WKV_ERR_LAUNCH;
+}
+
+// D = A B^T.  a, b: one or two sources.  How two are taken: `stack` = the rows of D are those of both (A's second source below the
+// first), else the contraction runs over both; a pair's forward pass has one A and two B.
+template <typename F, bool A_MN, bool B_MN, int EPI>
+int product(const Matrix (&a)[2], const Matrix (&b)[2], int a_sources, int b_sources, long long m, long long n, long long k, const Cut &cut, const Epi &e,
+            int *status, cudaStream_t s) {
+    constexpr bool PAIR = EPI == EPI_GATED;
+    GemmArgs g = {};
+    const int bm = 128 * cut.cg, out = PAIR ? cut.bn / 2 : cut.bn;
+    const bool stack = a_sources == 2 && b_sources == 1;
+    g.M = (int)m; g.N = (int)n;
+    g.m_tiles0 = (int)((m + bm - 1) / bm);
+    g.m_tiles = g.m_tiles0 * (stack ? 2 : 1);
+    g.n_tiles = (int)((n + out - 1) / out);
+    g.kb0 = (int)((k + KB - 1) / KB);
+    g.kb = g.kb0 * (a_sources == 2 && !stack ? 2 : 1);
+    g.splits = cut.splits; g.kb_split = cut.splits > 1 ? cut.kb_split : g.kb;
+    g.group = 8;
+    g.status = status; g.limit = WAIT_LIMIT;
+    g.e = e;
+    if ((long long)g.m_tiles * g.n_tiles * g.splits > 1 << 30) return WKV_ERR_SHAPE;
+    const int b_box = PAIR ? cut.bn / 2 : cut.bn / cut.cg;
+    for (int i = 0; i < 2; i++) {
+        const Matrix &ma = a[a_sources == 2 ? i : 0], &mb = b[b_sources == 2 ? i : 0];
+        if (!make_matrix_map(&g.a[i], ma.p, ma.rows, ma.cols, ma.pitch, A_MN ? 64 : 128) ||
+            !make_matrix_map(&g.b[i], mb.p, mb.rows, mb.cols, mb.pitch, B_MN ? 64 : b_box))
+            return WKV_ERR_LAUNCH;
+    }
+    if constexpr (EPI == EPI_PARTIAL) return launch_gemm<F, 1, 128, A_MN, B_MN, EPI>(g, s);
+    else if (cut.cg == 2) return launch_gemm<F, 2, 256, A_MN, B_MN, EPI>(g, s);
+    else return launch_gemm<F, 1, 128, A_MN, B_MN, EPI>(g, s);
+}
+// a product with the linear epilogue, its contraction split where that is faster
+template <typename F, bool A_MN, bool B_MN>
+int product_linear(const Matrix (&a)[2], const Matrix (&b)[2], int a_sources, int b_sources, long long m, long long n, long long k, const Cut &cut, Epi e,
+                   Scratch &ws, int *status, cudaStream_t s) {
+    if (cut.splits == 1) return product<F, A_MN, B_MN, EPI_LINEAR>(a, b, a_sources, b_sources, m, n, k, cut, e, status, s);
+    e.part = (float *)ws.take(split_bytes(cut, m, n));
+    e.part_row = up8(n);
+    const int rc = product<F, A_MN, B_MN, EPI_PARTIAL>(a, b, a_sources, b_sources, m, n, k, cut, e, status, s);
+    if (rc != WKV_OK) return rc;
+    const long long pieces = m * ((n + 7) / 8);
+    return launch_chained(k_fold_split<F>, dim3((unsigned)((pieces + 255) / 256)), dim3(256), 0, s, e, m, (int)n, cut.splits);
+}
+
+int check_args(const wkv_linear_args_t *a) {
+    if (a == nullptr) return WKV_ERR_NULL;
+    if (a->dtype != WKV_BF16 && a->dtype != WKV_F16) return known_dtype(a->dtype) ? WKV_ERR_UNSUPPORTED : WKV_ERR_DTYPE;
+    if (a->bias != nullptr && !known_dtype(a->bias_dtype)) return WKV_ERR_DTYPE;
+    const long long most = (1ll << 31) - 256;
+    if (a->rows < 0 || a->K < 1 || a->N < 1 || a->rows > most || a->K > most || a->N > most) return WKV_ERR_SHAPE;
+    if (a->act < 0 || a->act >= ACT_COUNT || a->pair < 0 || a->pair > 1) return WKV_ERR_SHAPE;
+    if (a->pair && (a->bias != nullptr || a->mul != nullptr || a->residual != nullptr || a->gbias != nullptr || a->gmul != nullptr)) return WKV_ERR_UNSUPPORTED;
+    return WKV_OK;
+}
+bool keeps(const wkv_linear_args_t *a) { return a->pair || a->act != ACT_NONE || a->mul != nullptr; }
+size_t saved_one(const wkv_linear_args_t *a) { return align256((size_t)a->rows * up8(a->N) * 2); }
+bool few(const wkv_linear_args_t *a) { return a->rows <= FEW_ROWS; }
+Matrix x_of(const wkv_linear_args_t *a) { return {a->x, a->rows, a->K, a->x_row}; }
+Matrix w_of(const wkv_linear_args_t *a, int i) { return {i ? a->w1 : a->w0, a->N, a->K, i ? a->w1_row : a->w0_row}; }
+
+// `m` where TMA can read it, else a copy in the scratch
+template <typename F>
+int ready(Matrix &m, Scratch &ws, cudaStream_t s) {
+    if (tma_ready(m.p, m.pitch)) return WKV_OK;
+    void *to = ws.take((size_t)m.rows * up8(m.cols) * 2);
+    if (ws.base == nullptr) return WKV_OK;
+    const int rc = repack<F>(m, to, s);
+    m.p = to;
+    m.pitch = up8(m.cols);
+    return rc;
+}
+
+Epi epilogue_of(const wkv_linear_args_t *a) {
+    Epi e = {};
+    e.act = a->act;
+    e.vec = a->N % 8 == 0 && all_aligned({a->y, a->mul, a->residual});
+    e.save_vec = 1;
+    e.bias = a->bias; e.bias_dtype = a->bias_dtype; e.mul = a->mul; e.residual = a->residual;
+    e.y[0] = a->y; e.y_row = a->N;
+    if (a->saved != nullptr && keeps(a)) {
+        e.z[0] = a->saved;
+        e.z[1] = a->pair ? (char *)a->saved + saved_one(a) : nullptr;
+        e.z_row = up8(a->N);
+    }
+    return e;
+}
+
+template <typename F>
+int forward(const wkv_linear_args_t *a, Scratch ws, size_t *need, cudaStream_t s) {
+    Matrix x = x_of(a), w[2] = {w_of(a, 0), w_of(a, a->pair)};
+    Epi e = epilogue_of(a);
+    const bool count = need != nullptr;
+    if (few(a)) {
+        if (count) { *need = 0; return WKV_OK; }
+        FewArgs g = {};
+        g.M = (int)a->rows; g.K = (int)a->K; g.N = (int)a->N;
+        g.x = x.p; g.x_row = x.pitch;
+        for (int i = 0; i < 2; i++) { g.w[i] = w[i].p; g.w_row[i] = w[i].pitch; }
+        g.e = e;
+        const bool vec = a->K % 8 == 0 && tma_ready(x.p, x.pitch) && tma_ready(w[0].p, w[0].pitch) && tma_ready(w[1].p, w[1].pitch);
+        const auto go = [&](auto kern) {
+            return launch_chained(kern, dim3((unsigned)((a->N + (a->pair ? 7 : 15)) / (a->pair ? 8 : 16))), dim3(32 * FEW_WARPS), 0, s, g);
+        };
+        if (a->rows <= 8) {
+            if (a->pair) return vec ? go(k_few_rows<F, 8, true, true>) : go(k_few_rows<F, 8, true, false>);
+            return vec ? go(k_few_rows<F, 8, false, true>) : go(k_few_rows<F, 8, false, false>);
+        }
+        if (a->pair) return vec ? go(k_few_rows<F, 16, true, true>) : go(k_few_rows<F, 16, true, false>);
+        return vec ? go(k_few_rows<F, 16, false, true>) : go(k_few_rows<F, 16, false, false>);
+    }
+    int rc = ready<F>(x, ws, s);
+    for (int i = 0; i <= a->pair && rc == WKV_OK; i++) rc = ready<F>(w[i], ws, s);
+    if (rc != WKV_OK) return rc;
+    const Cut cut = cut_for(a->rows, a->N, 1, (int)((a->K + KB - 1) / KB), a->pair);
+    if (count) {
+        *need = ws.used + align256(split_bytes(cut, a->rows, a->N));
+        return WKV_OK;
+    }
+    const Matrix xs[2] = {x, x};
+    if (a->pair) return product<F, false, false, EPI_GATED>(xs, w, 1, 2, a->rows, a->N, a->K, cut, e, a->status, s);
+    return product_linear<F, false, false>(xs, w, 1, 1, a->rows, a->N, a->K, cut, e, ws, a->status, s);
+}
+
+template <typename F>
+int backward(const wkv_linear_args_t *a, Scratch ws, size_t *need, cudaStream_t s) {
+    const bool count = need != nullptr;
+    const int sources = 1 + a->pair, kb_n = (int)((a->N + KB - 1) / KB) * sources, kb_r = (int)((a->rows + KB - 1) / KB);
+    const bool products = a->gx != nullptr || a->gw0 != nullptr || a->gw1 != nullptr;
+    // gz: gy itself where nothing stands between them
+    const bool act = keeps(a), own_gz = products && (act || !tma_ready(a->gy, a->N));
+    const int rows_per = (int)std::max<long long>(64, ((a->rows * ((a->N + 255) / 256) + 148 * 8 - 1) / (148 * 8) + 7) / 8 * 8);
+    const int row_blocks = (int)((a->rows + rows_per - 1) / rows_per);
+    GradArgs ga = {};
+    ga.rows = a->rows; ga.N = (int)a->N; ga.act = a->act; ga.rows_per = rows_per;
+    ga.vec = a->N % 8 == 0 && all_aligned({a->gy, a->mul, a->gmul});
+    ga.gy = a->gy; ga.mul = a->mul;
+    if (act) {
+        ga.z[0] = a->saved;
+        ga.z[1] = a->pair && a->saved != nullptr ? (char *)a->saved + saved_one(a) : nullptr;
+        ga.z_row = up8(a->N);
+    }
+    ga.gz_row = up8(a->N);
+    if (own_gz) {
+        for (int i = 0; i < sources; i++) ga.gz[i] = ws.take((size_t)a->rows * up8(a->N) * 2);
+    }
+    ga.gmul = a->gmul;
+    if (a->gbias != nullptr) ga.part = (float *)ws.take((size_t)row_blocks * a->N * 4);
+    int rc = WKV_OK;
+    if (!count && (own_gz || a->gmul != nullptr || a->gbias != nullptr)) {
+        const dim3 grid((unsigned)((a->N + 255) / 256), (unsigned)row_blocks);
+        rc = a->pair ? launch_chained(k_grad_act<F, true>, grid, dim3(256), 0, s, ga) : launch_chained(k_grad_act<F, false>, grid, dim3(256), 0, s, ga);
+        if (rc == WKV_OK && a->gbias != nullptr) {
+            FoldOut out = {};
+            out.p[0] = a->gbias; out.dtype[0] = a->bias_dtype;
+            for (int i = 1; i < 5; i++) out.start[i] = a->N;
+            rc = fold_params(ga.part, row_blocks, a->N, out, s);
+        }
+        if (rc != WKV_OK) return rc;
+    }
+    Matrix gz[2];
+    for (int i = 0; i < 2; i++) {
+        const int j = a->pair ? i : 0;
+        gz[i] = own_gz ? Matrix{ga.gz[j], a->rows, a->N, up8(a->N)} : Matrix{a->gy, a->rows, a->N, a->N};
+    }
+    size_t most = 0;
+    if (a->gx != nullptr) {
+        Matrix w[2] = {w_of(a, 0), w_of(a, a->pair)};
+        for (int i = 0; i <= a->pair && rc == WKV_OK; i++) rc = ready<F>(w[i], ws, s);
+        const Cut cut = cut_for(a->rows, a->K, 1, kb_n, false);
+        most = std::max(most, align256(split_bytes(cut, a->rows, a->K)));
+        if (!count && rc == WKV_OK) {
+            Epi e = {};
+            e.vec = a->K % 8 == 0 && aligned16(a->gx);
+            e.y[0] = a->gx; e.y_row = a->K;
+            Scratch parts = ws;
+            rc = product_linear<F, false, true>(gz, w, sources, sources, a->rows, a->K, a->N, cut, e, parts, a->status, s);
+        }
+    }
+    if (rc == WKV_OK && (a->gw0 != nullptr || a->gw1 != nullptr)) {
+        Matrix x = x_of(a);
+        rc = ready<F>(x, ws, s);
+        const Matrix xs[2] = {x, x};
+        const bool both = a->gw0 != nullptr && a->gw1 != nullptr;
+        const Cut cut = cut_for(a->N, a->K, 1 + both, kb_r, false);
+        most = std::max(most, align256(split_bytes(cut, a->N, a->K)));
+        if (!count && rc == WKV_OK) {
+            Epi e = {};
+            e.vec = a->K % 8 == 0 && all_aligned({a->gw0, a->gw1});
+            e.y[0] = a->gw0 != nullptr ? a->gw0 : a->gw1;
+            e.y[1] = a->gw1;
+            e.y_row = a->K;
+            if (a->gw0 == nullptr) gz[0] = gz[1];
+            Scratch parts = ws;
+            rc = product_linear<F, true, true>(gz, xs, 1 + both, 1, a->N, a->K, a->rows, cut, e, parts, a->status, s);
+        }
+    }
+    if (count) *need = ws.used + most;
+    return rc;
+}
+
+template <class Fn>
+int by_16bit(int d, Fn f) { return d == WKV_BF16 ? f(__nv_bfloat16{}) : f(__half{}); }
+
+}  // namespace
+}  // namespace linear
+}  // namespace wkv
+
+using namespace wkv;
+using namespace wkv::linear;
+
+extern "C" size_t wkv_linear_saved_bytes(const wkv_linear_args_t *a) {
+    return check_args(a) == WKV_OK && keeps(a) ? saved_one(a) * (1 + a->pair) : 0;
+}
+
+extern "C" size_t wkv_linear_forward_workspace(const wkv_linear_args_t *a) {
+    size_t n = 0;
+    if (check_args(a) == WKV_OK && a->rows > 0) by_16bit(a->dtype, [&](auto f) { return forward<decltype(f)>(a, Scratch{nullptr}, &n, nullptr); });
+    return n;
+}
+
+extern "C" int wkv_linear_forward(const wkv_linear_args_t *a, void *stream) {
+    const int e = check_args(a);
+    if (e != WKV_OK || a->rows == 0) return e;
+    if (a->x == nullptr || a->w0 == nullptr || (a->pair && a->w1 == nullptr) || a->y == nullptr) return WKV_ERR_NULL;
+    if (a->saved != nullptr && a->saved_bytes < wkv_linear_saved_bytes(a)) return WKV_ERR_WORKSPACE;
+    const size_t need = wkv_linear_forward_workspace(a);
+    if (need > 0 && (a->workspace == nullptr || a->workspace_bytes < need)) return WKV_ERR_WORKSPACE;
+    if (!all_aligned({a->workspace, a->saved})) return WKV_ERR_ALIGN;
+    return by_16bit(a->dtype, [&](auto f) { return forward<decltype(f)>(a, Scratch{(char *)a->workspace}, nullptr, (cudaStream_t)stream); });
+}
+
+extern "C" size_t wkv_linear_backward_workspace(const wkv_linear_args_t *a) {
+    size_t n = 0;
+    if (check_args(a) == WKV_OK && a->rows > 0) by_16bit(a->dtype, [&](auto f) { return backward<decltype(f)>(a, Scratch{nullptr}, &n, nullptr); });
+    return n;
+}
+
+extern "C" int wkv_linear_backward(const wkv_linear_args_t *a, void *stream) {
+    const int e = check_args(a);
+    if (e != WKV_OK) return e;
+    const cudaStream_t s = (cudaStream_t)stream;
+    if (a->rows == 0) {
+        for (void *p : {a->gw0, a->gw1})
+            if (p != nullptr && cudaMemsetAsync(p, 0, (size_t)a->N * a->K * 2, s) != cudaSuccess) return WKV_ERR_LAUNCH;
+        if (a->gbias != nullptr && cudaMemsetAsync(a->gbias, 0, (size_t)a->N * elem_size(a->bias_dtype), s) != cudaSuccess) return WKV_ERR_LAUNCH;
+        return WKV_OK;
+    }
+    if (a->gy == nullptr || (a->gx != nullptr && (a->w0 == nullptr || (a->pair && a->w1 == nullptr))) ||
+        ((a->gw0 != nullptr || a->gw1 != nullptr) && a->x == nullptr) || (!a->pair && a->gw1 != nullptr))
+        return WKV_ERR_NULL;
+    if (a->gbias != nullptr && !known_dtype(a->bias_dtype)) return WKV_ERR_DTYPE;
+    if (keeps(a) && (a->saved == nullptr || a->saved_bytes < wkv_linear_saved_bytes(a))) return WKV_ERR_WORKSPACE;
+    const size_t need = wkv_linear_backward_workspace(a);
+    if (need > 0 && (a->workspace == nullptr || a->workspace_bytes < need)) return WKV_ERR_WORKSPACE;
+    if (!all_aligned({a->workspace, a->saved})) return WKV_ERR_ALIGN;
+    return by_16bit(a->dtype, [&](auto f) { return backward<decltype(f)>(a, Scratch{(char *)a->workspace}, nullptr, s); });
+}

@@ -17,7 +17,7 @@ void raise_if_set(int device, int *word) {
     // reported once; taken and cleared in one step, so that a bit a kernel sets meanwhile is reported by this look or the next
     const int code = __atomic_exchange_n(word, 0, __ATOMIC_ACQ_REL);
     if (code == 0) return;      // (another thread reports it)
-    TORCH_CHECK(false, "a v5/v6 call on cuda:", device, ": a device-side wait ran out (status ", code,
+    TORCH_CHECK(false, "a v5/v6 call or a matrix product (status bit 64) on cuda:", device, ": a device-side wait ran out (status ", code,
                 "); the outputs of that call are invalid");
 }
 }  // namespace
@@ -416,6 +416,7 @@ py::object none_or(const Tensor &t) { return t.defined() ? py::cast(t) : py::non
 void bind_timemix(py::module_ &m);
 void bind_blocks(py::module_ &m);
 void bind_ssm(py::module_ &m);
+void bind_linear(py::module_ &m);
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("wkv56_apply", &wkv56_apply);
@@ -444,4 +445,5 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     bind_timemix(m);
     bind_blocks(m);
     bind_ssm(m);
+    bind_linear(m);
 }

@@ -65,4 +65,40 @@ inline bool make_btc_map(CUtensorMap *map, const void *base, int B, int T, int C
     return true;
 }
 
+// Map over a matrix [rows, cols] of 16-bit elements, rows `pitch` elements apart; box = box_rows x 64 columns, 128-byte swizzle,
+// what lies outside reads as zero.  base: 16-byte aligned, pitch a multiple of 8.  Remembered as above.
+inline bool make_matrix_map(CUtensorMap *map, const void *base, long long rows, long long cols, long long pitch, int box_rows) {
+    struct Entry {
+        CUtensorMap map;
+        const void *base;
+        long long rows, cols, pitch;
+        int box_rows;
+    };
+    constexpr int LOG_SLOTS = 9;
+    static thread_local Entry cache[1 << LOG_SLOTS];
+    const uint64_t key = (uint64_t)(uintptr_t)base ^ (uint64_t)rows << 40 ^ (uint64_t)cols << 50 ^ (uint64_t)box_rows << 32;
+    Entry &e = cache[(key >> 8) * 0x9E3779B97F4A7C15ull >> (64 - LOG_SLOTS)];
+    if (e.base == base && e.rows == rows && e.cols == cols && e.pitch == pitch && e.box_rows == box_rows && base != nullptr) {
+        *map = e.map;
+        return true;
+    }
+    encode_tiled_fn enc = tensor_map_encoder();
+    if (!enc) return false;
+    cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
+    cuuint64_t strides[1] = {(cuuint64_t)pitch * 2};
+    cuuint32_t box[2] = {64, (cuuint32_t)box_rows};
+    cuuint32_t estr[2] = {1, 1};
+    const auto encode = [&] {
+        // (the elements' type matters for arithmetic in the copy only: there is none)
+        return enc(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void *>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                   CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    };
+    if (encode() != CUDA_SUCCESS) {
+        int dev = 0;
+        if (cudaGetDevice(&dev) != cudaSuccess || cudaSetDevice(dev) != cudaSuccess || encode() != CUDA_SUCCESS) return false;
+    }
+    e.base = base; e.rows = rows; e.cols = cols; e.pitch = pitch; e.box_rows = box_rows; e.map = *map;
+    return true;
+}
+
 }  // namespace wkv
