@@ -370,7 +370,10 @@ int wkv_selective_scan_backward(const wkv_selective_scan_args_t *a, void *stream
  *   state_in's memory.  A decay gate of minus infinity keeps the state and takes no input.
  *   ckpt (wkv_gated_recurrence_ckpt_bytes()): states that the forward call leaves for the backward
  *   call, which needs them.  gy [B,T,D] contiguous.  Gradients: gx, ginput_gate, gdecay_gate, gz
- *   [B,T,D] in dtype; gdecay, gstate_in fp32.  D is at most 2^22, T at most 2^31 - 4097. */
+ *   [B,T,D] in dtype; gdecay, gstate_in fp32.  D is at most 2^22, a token stride 2^26, T 2^31 - 4097.
+ *   status: device-visible word or NULL; WKV_RECURRENCE_TIMEOUT is set in it when a bounded wait ran
+ *   out and the results are invalid. */
+enum { WKV_RECURRENCE_TIMEOUT = 128 };
 typedef struct wkv_gated_recurrence_args {
     int B, T, D, dtype;
     float c;
@@ -387,6 +390,7 @@ typedef struct wkv_gated_recurrence_args {
     size_t ckpt_bytes;
     void *workspace;
     size_t workspace_bytes;
+    int *status;
 } wkv_gated_recurrence_args_t;
 size_t wkv_gated_recurrence_ckpt_bytes(const wkv_gated_recurrence_args_t *a);
 int wkv_gated_recurrence_forward(const wkv_gated_recurrence_args_t *a, void *stream);

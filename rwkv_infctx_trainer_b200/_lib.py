@@ -82,7 +82,7 @@ class GatedRecurrenceArgs(ctypes.Structure):
         *((f"{n}_{s}", ctypes.c_longlong) for n in ("x", "i", "r", "z") for s in ("batch", "token")),
         ("decay", _vp), ("state_in", _vp), ("y", _vp), ("state_out", _vp), ("gy", _vp), ("gstate_out", _vp),
         ("gx", _vp), ("ginput_gate", _vp), ("gdecay_gate", _vp), ("gz", _vp), ("gdecay", _vp), ("gstate_in", _vp),
-        ("ckpt", _vp), ("ckpt_bytes", ctypes.c_size_t), ("workspace", _vp), ("workspace_bytes", ctypes.c_size_t),
+        ("ckpt", _vp), ("ckpt_bytes", ctypes.c_size_t), ("workspace", _vp), ("workspace_bytes", ctypes.c_size_t), ("status", _vp),
     ]
 
 

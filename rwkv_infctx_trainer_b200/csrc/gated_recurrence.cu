@@ -25,6 +25,8 @@
 #include <cooperative_groups.h>
 
 #include "elem_io.cuh"
+#include "sm100_primitives.cuh"
+#include "tma_host.cuh"
 #include "wkv_internal.h"
 
 namespace cg = cooperative_groups;
@@ -55,27 +57,32 @@ __device__ __forceinline__ float rsqrta(float x) {
 __device__ __forceinline__ float sig(float x) { return rcpa(1.f + ex2a(-LOG2E_ * x)); }
 
 struct RecArgs {
+    CUtensorMap in[5], out[4];            // TILES: decay gate, input gate, x, (gy,) z; y, or gx, ginput_gate, gdecay_gate, gz
     int T, D, slabs, cl, nsteps;          // slabs of CH channels; cl: CTAs of a cluster, nsteps: blocks of a row / cl, rounded up
     float c;
     const void *x, *ig, *rg, *z;
     long long x_batch, x_token, ig_batch, ig_token, rg_batch, rg_token, z_batch, z_token;
     const float *decay, *state_in;
     void *y;
-    float *state_out, *ckpt;              // ckpt [B, nsteps * cl, D]
+    float *state_out, *ckpt;              // ckpt [B, nkept, D]: the state before every CKPT tokens
+    int *status;
+    unsigned limit;
+    int nkept, pair;                      // pair: two neighbouring channels are one access in every output
     const void *gy;
     const float *gs_out;
     void *gx, *gig, *grg, *gz;
     float *gs_in, *part;                  // part [B * cl, D]
 };
 
-// Tokens of a warp in a block, and shared memory, for two CTAs an SM.
-template <typename F>
+// Tokens of a warp in a block (S), for two CTAs an SM: what a thread keeps of its tokens has to fit in 128 registers, because what
+// does not would wait for L2 (shared memory leaves no L1).
+template <typename F, bool BACK>
 struct Geo {
-    static constexpr int S = sizeof(F) == 2 ? 8 : 4, BT = NW * S, SLOT = BT * CH;        // SLOT: elements of one tensor's block
-    static constexpr int FWD_STAGES = 3, BWD_STAGES = 2;
-    static constexpr int fwd_ring(bool z) { return FWD_STAGES * (3 + z) * SLOT * (int)sizeof(F); }
-    static constexpr int bwd_ring(bool z) { return BWD_STAGES * (4 + z) * SLOT * (int)sizeof(F); }
+    static constexpr int S = sizeof(F) == 2 && !BACK ? 8 : 4, BT = NW * S, SLOT = BT * CH;        // SLOT: elements of one tensor's block
+    static constexpr int STAGES = sizeof(F) == 4 && BACK ? 2 : 3;
+    static constexpr int ring(bool z) { return STAGES * (3 + BACK + z) * SLOT * (int)sizeof(F); }
 };
+constexpr int CKPT = 32;                  // tokens between two states that are kept: a block of the backward pass
 
 // softplus(p) and its derivative over it, once per CTA and channel
 struct Rate {
@@ -93,59 +100,100 @@ __device__ __forceinline__ Rate rate_of(float p, float c) {
     return r;
 }
 
-// the gates of a token: decay a, 1 - a^2
-__device__ __forceinline__ float one_minus_square(float a, float x2) {
-    float p = fmaf(x2, -1.f / 720.f, 1.f / 120.f);
-    p = fmaf(x2, p, -1.f / 24.f);
-    p = fmaf(x2, p, 1.f / 6.f);
-    p = fmaf(x2, p, -0.5f);
-    p = fmaf(x2, p, 1.f) * x2;
-    return x2 < 0.25f ? p : fmaf(-a, a, 1.f);
+// 1 - a^2 of two channels; x2 = -2 L
+__device__ __forceinline__ f2 one_minus_square(f2 a, f2 x2) {
+    f2 p = fma2(x2, both(-1.f / 720.f), both(1.f / 120.f));
+    p = fma2(x2, p, both(-1.f / 24.f));
+    p = fma2(x2, p, both(1.f / 6.f));
+    p = fma2(x2, p, both(-0.5f));
+    p = mul2(fma2(x2, p, both(1.f)), x2);
+    const f2 d = fma2(neg2(a), a, both(1.f));
+    return make_float2(x2.x < 0.25f ? p.x : d.x, x2.y < 0.25f ? p.y : d.y);
 }
 
-template <int BYTES>
-__device__ __forceinline__ void cp_async(void *smem, const void *g, int valid) {
-    const uint32_t s = (uint32_t)__cvta_generic_to_shared(smem);
-    if constexpr (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(s), "l"(g), "r"(valid) : "memory");
-    else asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(s), "l"(g), "r"(valid) : "memory");
+// Sigmoids of two channels' gates (Z: and of the output gate): one reciprocal for a channel's two or three, of the product of their
+// 1 + e^-x, because special functions are what bounds the forward pass.  `range` adds up the products: while it is below 2^125 none
+// of them has left the range; else (gates below -28 or so, infinities, NaNs, which would spread from one gate to the others) the
+// caller takes the segment again with FAST = false: a reciprocal for each there, and the same bits for all others.
+constexpr float RANGE = 4.2535296e37f;
+template <bool Z, bool FAST>
+__device__ __forceinline__ void sigmoids(f2 rg, f2 ig, f2 z, f2 &r, f2 &i, f2 &s, f2 &range) {
+    // (a zero that the compiler does not know: it would keep what both ways have in common in registers, for all tokens)
+    f2 zero = both(0.f);
+    if (!FAST) asm volatile("mov.b32 %0, 0;" : "=f"(zero.x));
+    auto one_plus = [&](f2 x) {
+        const f2 e = FAST ? mul2(x, both(-LOG2E_)) : mul2(add2(x, both(zero.x)), both(-LOG2E_));
+        return add2(make_float2(ex2a(e.x), ex2a(e.y)), both(1.f));
+    };
+    const f2 pr = one_plus(rg), pi = one_plus(ig), ri = mul2(pr, pi);
+    f2 d = ri;
+    if (Z) {
+        const f2 pz = one_plus(z);
+        d = mul2(ri, pz);
+        const f2 inv = make_float2(rcpa(d.x), rcpa(d.y)), iz = mul2(inv, pz);
+        r = mul2(iz, pi);
+        i = mul2(iz, pr);
+        s = mul2(inv, ri);
+    } else {
+        const f2 inv = make_float2(rcpa(d.x), rcpa(d.y));
+        r = mul2(inv, pi);
+        i = mul2(inv, pr);
+    }
+    range = add2(range, d);
+    if (!FAST) {
+        if (!(d.x < RANGE)) {
+            r.x = sig(rg.x);
+            i.x = sig(ig.x);
+            if (Z) s.x = sig(z.x);
+        }
+        if (!(d.y < RANGE)) {
+            r.y = sig(rg.y);
+            i.y = sig(ig.y);
+            if (Z) s.y = sig(z.y);
+        }
+    }
+}
+__device__ __forceinline__ bool in_range(f2 range) { return __all_sync(0xffffffffu, range.x + range.y < RANGE); }
+__device__ __forceinline__ f2 decays(f2 r, f2 rate) {
+    const f2 e = fma2(r, rate, both(EX2_MEAN_));
+    return make_float2(ex2a(e.x), ex2a(e.y));
+}
+
+__device__ __forceinline__ void cp_async4(void *smem, const void *g, int valid) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(sm100::smem_u32(smem)), "l"(g), "r"(valid) : "memory");
 }
 __device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N> __device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
-// How rows lie: pieces of 16 bytes, words, or (two-byte elements) anywhere.
-enum { PIECES = 0, WORDS = 1, ANYWHERE = 2 };
+// How rows lie: pieces of 16 bytes (TMA brings a block's tile of each tensor, and takes the outputs' away), words, or (two-byte
+// elements) anywhere: a warp fetches its own tokens.
+enum { TILES = 0, WORDS = 1, ANYWHERE = 2 };
 
-// A warp's S tokens of one tensor -> its slot [S][CH] of the ring.  Tokens from `n` on and channels from D on become zeros.
-template <typename F, int MODE>
-__device__ __forceinline__ void fill(F *slot, const F *row, long long token, int n, int ch0, int D, int lane) {
-    constexpr int S = Geo<F>::S;
-    if constexpr (MODE == PIECES) {
-        constexpr int PER = 16 / sizeof(F), ROWP = CH / PER;
-#pragma unroll
-        for (int k = 0; k < S * ROWP / 32; k++) {
-            const int i = lane + 32 * k, s = i / ROWP, e = (i % ROWP) * PER;
-            const bool ok = s < n && ch0 + e < D;
-            cp_async<16>(slot + s * CH + e, ok ? row + s * token + e : row, ok ? 16 : 0);
-        }
-    } else if constexpr (MODE == WORDS) {
+// A warp's S tokens of one tensor -> its slot [S][CH] of the ring.  block: the CTA's first token; token: stride.  Tokens from `n` on
+// and channels from D on become zeros.  Offsets inside a block are 32-bit (the host checks the strides).
+template <typename F, int MODE, int S>
+__device__ __forceinline__ void fill(F *slot, const F *block, int token, int warp, int n, int left, int lane) {
+    if constexpr (MODE == WORDS) {
+        const uint32_t at = (uint32_t)(warp * S) * (uint32_t)token + 2 * lane;
+        left -= 2 * lane;
 #pragma unroll
         for (int s = 0; s < S; s++) {
-            const int e = 2 * lane, left = D - ch0 - e;
             const bool ok = s < n && left > 0;
-            const F *p = ok ? row + s * token + e : row;
+            const F *p = block + (ok ? at + (uint32_t)s * (uint32_t)token : 0u);
             if constexpr (sizeof(F) == 2) {
-                cp_async<4>(slot + s * CH + e, p, ok ? min(left, 2) * 2 : 0);
+                cp_async4(slot + s * CH + 2 * lane, p, ok ? min(left, 2) * 2 : 0);
             } else {
-                cp_async<4>(slot + s * CH + e, p, ok ? 4 : 0);
-                cp_async<4>(slot + s * CH + e + 1, ok && left > 1 ? p + 1 : row, ok && left > 1 ? 4 : 0);
+                cp_async4(slot + s * CH + 2 * lane, p, ok ? 4 : 0);
+                cp_async4(slot + s * CH + 2 * lane + 1, ok && left > 1 ? p + 1 : block, ok && left > 1 ? 4 : 0);
             }
         }
     } else {
+        const uint32_t at = (uint32_t)(warp * S) * (uint32_t)token + 2 * lane;
+        left -= 2 * lane;
         uint32_t w[S];
 #pragma unroll
         for (int s = 0; s < S; s++) {
-            const int e = 2 * lane, left = D - ch0 - e;
-            const uint16_t *p = reinterpret_cast<const uint16_t *>(row + s * token + e);
+            const uint16_t *p = reinterpret_cast<const uint16_t *>(block + (at + (uint32_t)s * (uint32_t)token));
             w[s] = 0;
             if (s < n && left > 0) w[s] = p[0];
             if (s < n && left > 1) w[s] |= (uint32_t)p[1] << 16;
@@ -162,108 +210,157 @@ __device__ __forceinline__ f2 pair_at(const F *slot, int s, int lane) {
     r.get(f);
     return make_float2(f[0], f[1]);
 }
-// The state before a token, in the places of its two gates (which are in registers by then): a lane's own.
-template <typename F>
-__device__ __forceinline__ void keep_state(F *slot, int next, int s, int lane, f2 h) {
-    if constexpr (sizeof(F) == 4) {
-        *reinterpret_cast<f2 *>(slot + s * CH + 2 * lane) = h;
-    } else {
-        *reinterpret_cast<float *>(slot + s * CH + 2 * lane) = h.x;
-        *reinterpret_cast<float *>(slot + next + s * CH + 2 * lane) = h.y;
-    }
-}
-template <typename F>
-__device__ __forceinline__ f2 kept_state(const F *slot, int next, int s, int lane) {
-    if constexpr (sizeof(F) == 4) return *reinterpret_cast<const f2 *>(slot + s * CH + 2 * lane);
-    else return make_float2(*reinterpret_cast<const float *>(slot + s * CH + 2 * lane), *reinterpret_cast<const float *>(slot + next + s * CH + 2 * lane));
-}
 // decay gates of minus infinity for the tokens behind the row's last: they keep the state (x is zero there)
-template <typename F>
+template <typename F, int S>
 __device__ __forceinline__ void close_gates(F *slot, int n, int lane) {
-    for (int s = max(n, 0); s < Geo<F>::S; s++) {
+    for (int s = n; s < S; s++) {
         const float f[2] = {-INFINITY, -INFINITY};
         Raw<F, 2> r;
         r.put(f);
         r.store(slot + s * CH + 2 * lane, true, 2);
     }
 }
+// two channels of a block's output, `at` elements from its first; left: channels there are
 template <typename F>
-__device__ __forceinline__ void store_out(F *p, f2 v, bool pair, int left) {
+__device__ __forceinline__ void store_out(F *block, uint32_t at, f2 v, bool pair, int left) {
     const float f[2] = {v.x, v.y};
     Raw<F, 2> r;
     r.put(f);
-    r.store(p, pair, left);
+    r.store(block + at, pair, left);
+}
+// the same into a slot of the ring, from where TMA takes it (a lane's own place)
+template <typename F>
+__device__ __forceinline__ void put_pair(F *slot, int s, int lane, f2 v) {
+    store_out<F>(slot, s * CH + 2 * lane, v, true, 2);
 }
 
 // what a segment does to the state (and to E): [side][segment][channel pair]
 struct Exchange {
     float4 seg[2][NW][32];                // P, hl of two channels
     float4 cta[2][MAX_CL][32];            // the same of the cluster's CTAs
+    uint64_t full[4];
+    int abort;
 };
 struct ExchangeBack {
     float4 seg[2][NW][32];                // P, hl
     f2 segE[2][NW][32];                   // E from zero
     float4 cta[2][MAX_CL][32];            // P, E of the cluster's CTAs
     f2 sum[NW][32];
+    uint64_t full[4];
+    int abort;
 };
 
+// The ring's blocks: TILES: one thread has TMA bring the block's tile of each tensor, all wait on the stage's barrier (bounded: a wait
+// that runs out is reported, the others of the CTA end at once, and the call's results are invalid).
+template <int ST, class X>
+__device__ __forceinline__ void init_tiles(X &ex) {
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < ST; i++) sm100::mbar_init(ex.full + i, 1);
+        ex.abort = 0;
+        sm100::fence_mbar_init();
+    }
+    __syncthreads();
+}
+template <int ST, class X>
+__device__ __forceinline__ void await_tiles(X &ex, const RecArgs &g, int k) {
+    if (!sm100::mbar_wait_or_abort(ex.full + k % ST, (k / ST) & 1, &ex.abort, g.limit)) {
+        *(volatile int *)&ex.abort = 1;
+        if (g.status != nullptr) atomicOr(g.status, WKV_RECURRENCE_TIMEOUT);
+    }
+}
+// (after a wait that ran out: tiles may still be on their way into this CTA's shared memory)
+template <int ST, class X>
+__device__ __forceinline__ void drain_tiles(X &ex, const RecArgs &g) {
+    if (threadIdx.x != 0 || *(volatile int *)&ex.abort == 0) return;
+    for (int k = max(0, g.nsteps - ST); k < g.nsteps; k++) sm100::mbar_wait(ex.full + k % ST, (k / ST) & 1, g.limit);
+}
+
 template <typename F, bool Z, int MODE>
-__global__ void __launch_bounds__(256, 2) k_rec_fwd(const RecArgs g) {
+__global__ void __launch_bounds__(256, 2) k_rec_fwd(const __grid_constant__ RecArgs g) {
     pdl_wait();
     pdl_trigger();
-    constexpr int S = Geo<F>::S, BT = Geo<F>::BT, SLOT = Geo<F>::SLOT, NT = 3 + Z, ST = Geo<F>::FWD_STAGES, RING = ST * NT * SLOT * (int)sizeof(F);
-    extern __shared__ __align__(16) unsigned char smem[];
+    using G = Geo<F, false>;
+    constexpr int S = G::S, BT = G::BT, SLOT = G::SLOT, NT = 3 + Z, ST = G::STAGES, RING = ST * NT * SLOT * (int)sizeof(F);
+    extern __shared__ __align__(128) unsigned char smem[];
     Exchange &ex = *reinterpret_cast<Exchange *>(smem + RING);
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int rank = blockIdx.x % g.cl, chain = blockIdx.x / g.cl, b = chain / g.slabs, ch0 = (chain - b * g.slabs) * CH, ch = ch0 + 2 * lane;
-    F *ring = reinterpret_cast<F *>(smem) + warp * S * CH;          // [stage][tensor][warp][S][CH]
+    F *ring = reinterpret_cast<F *>(smem);                          // [stage][tensor][warp][S][CH]
 
     const Rate k0 = rate_of(ch < g.D ? g.decay[ch] : 0.f, g.c), k1 = rate_of(ch + 1 < g.D ? g.decay[ch + 1] : 0.f, g.c);
+    const f2 rate = make_float2(k0.rate2, k1.rate2), x2 = make_float2(k0.x2, k1.x2);
     f2 h = make_float2(0.f, 0.f);
     if (g.state_in != nullptr) {
         if (ch < g.D) h.x = g.state_in[(size_t)b * g.D + ch];
         if (ch + 1 < g.D) h.y = g.state_in[(size_t)b * g.D + ch + 1];
     }
     auto start = [&](int step) {
-        const long long t0 = ((long long)step * g.cl + rank) * BT + warp * S;
-        const int n = (int)max(0ll, min((long long)S, g.T - t0));
-        const long long at = n > 0 ? t0 : 0;
+        const long long t0 = ((long long)step * g.cl + rank) * BT, at = t0 < g.T ? t0 : 0;
         F *slot = ring + (step % ST) * NT * SLOT;
-        fill<F, MODE>(slot, (const F *)g.rg + b * g.rg_batch + at * g.rg_token + ch0, g.rg_token, n, ch0, g.D, lane);
-        fill<F, MODE>(slot + SLOT, (const F *)g.ig + b * g.ig_batch + at * g.ig_token + ch0, g.ig_token, n, ch0, g.D, lane);
-        fill<F, MODE>(slot + 2 * SLOT, (const F *)g.x + b * g.x_batch + at * g.x_token + ch0, g.x_token, n, ch0, g.D, lane);
-        if (Z) fill<F, MODE>(slot + 3 * SLOT, (const F *)g.z + b * g.z_batch + at * g.z_token + ch0, g.z_token, n, ch0, g.D, lane);
-    };
+        if constexpr (MODE == TILES) {
+            sm100::mbar_expect_tx(ex.full + step % ST, NT * SLOT * sizeof(F));
 #pragma unroll
-    for (int p = 0; p < ST - 1; p++) {
-        if (p < g.nsteps) start(p);
-        cp_commit();
-    }
-    const bool pair = (g.D & 1) == 0;
-    for (int step = 0; step < g.nsteps; step++) {
-        __syncwarp();                                               // (all lanes are done with the slot that is filled now)
-        if (step + ST - 1 < g.nsteps) start(step + ST - 1);
-        cp_commit();
-        cp_wait<ST - 1>();
-        __syncwarp();
-        F *slot = ring + (step % ST) * NT * SLOT;
-        const long long blk = (long long)step * g.cl + rank, t0 = blk * BT + warp * S;
-        const int n = (int)max(0ll, min((long long)S, g.T - t0));
-        if (n < S) close_gates(slot, n, lane);
-        f2 a[S], v[S], P = both(1.f), hl = both(0.f);
-#pragma unroll
-        for (int s = 0; s < S; s++) {
-            const f2 rg = pair_at(slot, s, lane), ig = pair_at(slot + SLOT, s, lane), x = pair_at(slot + 2 * SLOT, s, lane);
-            const float r0 = sig(rg.x), r1 = sig(rg.y);
-            a[s] = make_float2(ex2a(fmaf(r0, k0.rate2, EX2_MEAN_)), ex2a(fmaf(r1, k1.rate2, EX2_MEAN_)));
-            const f2 m = make_float2(sqrtf(one_minus_square(a[s].x, r0 * k0.x2)), sqrtf(one_minus_square(a[s].y, r1 * k1.x2)));
-            v[s] = mul2(mul2(m, make_float2(sig(ig.x), sig(ig.y))), x);
-            hl = fma2(a[s], hl, v[s]);
-            P = mul2(P, a[s]);
+            for (int i = 0; i < NT; i++) sm100::tma_load_3d(slot + i * SLOT, g.in + i, ex.full + step % ST, ch0, (int)t0, b);
+        } else {
+            const int n = (int)max(0ll, min((long long)S, g.T - (t0 + warp * S))), left = g.D - ch0;
+            slot += warp * S * CH;
+            fill<F, MODE, S>(slot, (const F *)g.rg + (b * g.rg_batch + at * g.rg_token + ch0), (int)g.rg_token, warp, n, left, lane);
+            fill<F, MODE, S>(slot + SLOT, (const F *)g.ig + (b * g.ig_batch + at * g.ig_token + ch0), (int)g.ig_token, warp, n, left, lane);
+            fill<F, MODE, S>(slot + 2 * SLOT, (const F *)g.x + (b * g.x_batch + at * g.x_token + ch0), (int)g.x_token, warp, n, left, lane);
+            if (Z) fill<F, MODE, S>(slot + 3 * SLOT, (const F *)g.z + (b * g.z_batch + at * g.z_token + ch0), (int)g.z_token, warp, n, left, lane);
         }
+    };
+    if constexpr (MODE == TILES) {
+        init_tiles<ST>(ex);
+        if (threadIdx.x == 0) {
+            for (int p = 0; p < min(ST, g.nsteps); p++) start(p);
+        }
+    } else {
+#pragma unroll
+        for (int p = 0; p < ST - 1; p++) {
+            if (p < g.nsteps) start(p);
+            cp_commit();
+        }
+    }
+    for (int step = 0; step < g.nsteps; step++) {
+        if constexpr (MODE == TILES) {
+            await_tiles<ST>(ex, g, step);
+        } else {
+            __syncwarp();                                           // (all lanes are done with the slot that is filled now)
+            if (step + ST - 1 < g.nsteps) start(step + ST - 1);
+            cp_commit();
+            cp_wait<ST - 1>();
+            __syncwarp();
+        }
+        F *slot = ring + (step % ST) * NT * SLOT + warp * S * CH;
+        const long long t0 = ((long long)step * g.cl + rank) * BT;
+        const int n = (int)max(0ll, min((long long)S, g.T - (t0 + warp * S)));          // this warp's tokens of the block
+        if (n < S) close_gates<F, S>(slot, n, lane);
+        f2 a[S], v[S], gate[Z ? S : 1], P, hl;
+        auto segment = [&](auto fast) {
+            f2 range = both(0.f);
+            P = both(1.f);
+            hl = both(0.f);
+#pragma unroll
+            for (int s = 0; s < S; s++) {
+                const f2 x = pair_at(slot + 2 * SLOT, s, lane), z = Z ? pair_at(slot + 3 * SLOT, s, lane) : both(0.f);
+                f2 r, in, sz;
+                sigmoids<Z, decltype(fast)::value>(pair_at(slot, s, lane), pair_at(slot + SLOT, s, lane), z, r, in, sz, range);
+                a[s] = decays(r, rate);
+                const f2 q = one_minus_square(a[s], mul2(r, x2));
+                v[s] = mul2(mul2(make_float2(sqrtf(q.x), sqrtf(q.y)), in), x);
+                if (Z) gate[s] = mul2(z, sz);
+                hl = fma2(a[s], hl, v[s]);
+                P = mul2(P, a[s]);
+            }
+            return in_range(range);
+        };
+        if (!segment(std::true_type{})) segment(std::false_type{});
         const int side = step & 1;
         ex.seg[side][warp][lane] = make_float4(P.x, P.y, hl.x, hl.y);
+        if (MODE == TILES && lane == 0) sm100::tma_store_wait_read();                   // (of the block before: its stage is filled next)
         __syncthreads();
+        if (MODE == TILES && threadIdx.x == 0 && step > 0 && step + ST - 1 < g.nsteps) start(step + ST - 1);
         f2 hs = h;                                                  // before this warp's segment
         if (g.cl == 1) {
 #pragma unroll
@@ -271,11 +368,6 @@ __global__ void __launch_bounds__(256, 2) k_rec_fwd(const RecArgs g) {
                 const float4 q = ex.seg[side][w][lane];
                 if (w == warp) hs = h;
                 h = fma2(make_float2(q.x, q.y), h, make_float2(q.z, q.w));
-            }
-            if (g.ckpt != nullptr && warp == 0) {
-                float *c = g.ckpt + ((size_t)b * g.nsteps + blk) * g.D + ch;
-                if (ch < g.D) c[0] = hs.x;
-                if (ch + 1 < g.D) c[1] = hs.y;
             }
         } else {
             f2 Pc = both(1.f), hc = both(0.f), Pw = both(1.f), hw = both(0.f);
@@ -299,26 +391,36 @@ __global__ void __launch_bounds__(256, 2) k_rec_fwd(const RecArgs g) {
                 h = fma2(make_float2(e.x, e.y), h, make_float2(e.z, e.w));
             }
             hs = fma2(Pw, hr, hw);
-            if (g.ckpt != nullptr && warp == 0) {
-                float *c = g.ckpt + ((size_t)b * g.nsteps * g.cl + blk) * g.D + ch;
-                if (ch < g.D) c[0] = hr.x;
-                if (ch + 1 < g.D) c[1] = hr.y;
-            }
         }
-        if (ch < g.D) {
-            F *y = (F *)g.y + ((size_t)b * g.T + t0) * g.D + ch;
+        if (g.ckpt != nullptr && warp * S % CKPT == 0 && n > 0) {
+            float *c = g.ckpt + ((size_t)b * g.nkept + (t0 + warp * S) / CKPT) * g.D + ch;
+            if (ch < g.D) c[0] = hs.x;
+            if (ch + 1 < g.D) c[1] = hs.y;
+        }
+        if constexpr (MODE == TILES) {
 #pragma unroll
             for (int s = 0; s < S; s++) {
                 hs = fma2(a[s], hs, v[s]);
-                f2 o = hs;
-                if (Z) {
-                    const f2 z = pair_at(slot + 3 * SLOT, s, lane);
-                    o = mul2(o, mul2(z, make_float2(sig(z.x), sig(z.y))));
-                }
-                if (s < n) store_out(y + (size_t)s * g.D, o, pair, g.D - ch);
+                put_pair(slot + 2 * SLOT, s, lane, Z ? mul2(hs, gate[s]) : hs);
+            }
+            sm100::fence_async_smem();
+            __syncwarp();
+            if (lane == 0 && n > 0) {
+                sm100::tma_store_3d(g.out, slot + 2 * SLOT, ch0, (int)t0 + warp * S, b);
+                sm100::tma_store_commit();
+            }
+        } else {
+            const int m = ch < g.D ? n : 0;
+            F *y = (F *)g.y + (((size_t)b * g.T + t0) * g.D + ch0);
+#pragma unroll
+            for (int s = 0; s < S; s++) {
+                hs = fma2(a[s], hs, v[s]);
+                if (s < m) store_out(y, (uint32_t)(warp * S + s) * (uint32_t)g.D + 2 * lane, Z ? mul2(hs, gate[s]) : hs, g.pair, g.D - ch);
             }
         }
     }
+    if (MODE == TILES && lane == 0) sm100::tma_store_wait_all();
+    if (MODE == TILES) drain_tiles<ST>(ex, g);
     if (g.cl > 1) cg::this_cluster().sync();                        // (no CTA leaves while another may write to it)
     if (g.state_out != nullptr && warp == 0 && rank == 0) {
         if (ch < g.D) g.state_out[(size_t)b * g.D + ch] = h.x;
@@ -327,18 +429,20 @@ __global__ void __launch_bounds__(256, 2) k_rec_fwd(const RecArgs g) {
 }
 
 template <typename F, bool Z, int MODE>
-__global__ void __launch_bounds__(256, 2) k_rec_bwd(const RecArgs g) {
+__global__ void __launch_bounds__(256, 2) k_rec_bwd(const __grid_constant__ RecArgs g) {
     pdl_wait();
     pdl_trigger();
-    constexpr int S = Geo<F>::S, BT = Geo<F>::BT, SLOT = Geo<F>::SLOT, NT = 4 + Z, ST = Geo<F>::BWD_STAGES, RING = ST * NT * SLOT * (int)sizeof(F);
-    extern __shared__ __align__(16) unsigned char smem[];
+    using G = Geo<F, true>;
+    constexpr int S = G::S, BT = G::BT, SLOT = G::SLOT, NT = 4 + Z, ST = G::STAGES, RING = ST * NT * SLOT * (int)sizeof(F);
+    static_assert(BT == CKPT, "a block starts from a state that is kept");
+    extern __shared__ __align__(128) unsigned char smem[];
     ExchangeBack &ex = *reinterpret_cast<ExchangeBack *>(smem + RING);
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int rank = blockIdx.x % g.cl, chain = blockIdx.x / g.cl, b = chain / g.slabs, ch0 = (chain - b * g.slabs) * CH, ch = ch0 + 2 * lane;
-    F *ring = reinterpret_cast<F *>(smem) + warp * S * CH;
+    F *ring = reinterpret_cast<F *>(smem);
 
     const Rate k0 = rate_of(ch < g.D ? g.decay[ch] : 0.f, g.c), k1 = rate_of(ch + 1 < g.D ? g.decay[ch + 1] : 0.f, g.c);
-    const f2 rate = make_float2(k0.rate2, k1.rate2);
+    const f2 rate = make_float2(k0.rate2, k1.rate2), x2 = make_float2(k0.x2, k1.x2);
     f2 E = make_float2(0.f, 0.f), total = make_float2(0.f, 0.f);
     if (g.gs_out != nullptr) {
         if (ch < g.D) E.x = g.gs_out[(size_t)b * g.D + ch];
@@ -346,83 +450,111 @@ __global__ void __launch_bounds__(256, 2) k_rec_bwd(const RecArgs g) {
     }
     // (k counts the steps in the order of the walk)
     auto start = [&](int k) {
-        const int step = g.nsteps - 1 - k;
-        const long long t0 = ((long long)step * g.cl + rank) * BT + warp * S;
-        const int n = (int)max(0ll, min((long long)S, g.T - t0));
-        const long long at = n > 0 ? t0 : 0;
+        const long long t0 = ((long long)(g.nsteps - 1 - k) * g.cl + rank) * BT, at = t0 < g.T ? t0 : 0;
         F *slot = ring + (k % ST) * NT * SLOT;
-        fill<F, MODE>(slot, (const F *)g.rg + b * g.rg_batch + at * g.rg_token + ch0, g.rg_token, n, ch0, g.D, lane);
-        fill<F, MODE>(slot + SLOT, (const F *)g.ig + b * g.ig_batch + at * g.ig_token + ch0, g.ig_token, n, ch0, g.D, lane);
-        fill<F, MODE>(slot + 2 * SLOT, (const F *)g.x + b * g.x_batch + at * g.x_token + ch0, g.x_token, n, ch0, g.D, lane);
-        // (no incoming gradient: zeros)
-        fill<F, MODE>(slot + 3 * SLOT, g.gy != nullptr ? (const F *)g.gy + ((size_t)b * g.T + at) * g.D + ch0 : (const F *)g.x, g.D,
-                      g.gy != nullptr ? n : 0, ch0, g.D, lane);
-        if (Z) fill<F, MODE>(slot + 4 * SLOT, (const F *)g.z + b * g.z_batch + at * g.z_token + ch0, g.z_token, n, ch0, g.D, lane);
-    };
+        if constexpr (MODE == TILES) {
+            sm100::mbar_expect_tx(ex.full + k % ST, NT * SLOT * sizeof(F));
 #pragma unroll
-    for (int p = 0; p < ST - 1; p++) {
-        if (p < g.nsteps) start(p);
-        cp_commit();
+            for (int i = 0; i < NT; i++) sm100::tma_load_3d(slot + i * SLOT, g.in + i, ex.full + k % ST, ch0, (int)t0, b);
+        } else {
+            const int n = (int)max(0ll, min((long long)S, g.T - (t0 + warp * S))), left = g.D - ch0;
+            slot += warp * S * CH;
+            fill<F, MODE, S>(slot, (const F *)g.rg + (b * g.rg_batch + at * g.rg_token + ch0), (int)g.rg_token, warp, n, left, lane);
+            fill<F, MODE, S>(slot + SLOT, (const F *)g.ig + (b * g.ig_batch + at * g.ig_token + ch0), (int)g.ig_token, warp, n, left, lane);
+            fill<F, MODE, S>(slot + 2 * SLOT, (const F *)g.x + (b * g.x_batch + at * g.x_token + ch0), (int)g.x_token, warp, n, left, lane);
+            if (g.gy != nullptr) fill<F, MODE, S>(slot + 3 * SLOT, (const F *)g.gy + (((size_t)b * g.T + at) * g.D + ch0), g.D, warp, n, left, lane);
+            else fill<F, MODE, S>(slot + 3 * SLOT, (const F *)g.x, 0, warp, 0, left, lane);         // (no incoming gradient: zeros)
+            if (Z) fill<F, MODE, S>(slot + 4 * SLOT, (const F *)g.z + (b * g.z_batch + at * g.z_token + ch0), (int)g.z_token, warp, n, left, lane);
+        }
+    };
+    if constexpr (MODE == TILES) {
+        init_tiles<ST>(ex);
+        if (threadIdx.x == 0) {
+            for (int p = 0; p < min(ST, g.nsteps); p++) start(p);
+        }
+    } else {
+#pragma unroll
+        for (int p = 0; p < ST - 1; p++) {
+            if (p < g.nsteps) start(p);
+            cp_commit();
+        }
     }
-    const bool pair = (g.D & 1) == 0;
     for (int k = 0; k < g.nsteps; k++) {
-        __syncwarp();
-        if (k + ST - 1 < g.nsteps) start(k + ST - 1);
-        cp_commit();
-        const int step = g.nsteps - 1 - k;
-        const long long blk = (long long)step * g.cl + rank, t0 = blk * BT + warp * S;
+        const long long t0 = ((long long)(g.nsteps - 1 - k) * g.cl + rank) * BT;
         f2 h = make_float2(0.f, 0.f);                               // before the block
-        {
-            const float *c = g.ckpt + ((size_t)b * g.nsteps * g.cl + blk) * g.D + ch;
+        if (t0 < g.T) {
+            const float *c = g.ckpt + ((size_t)b * g.nkept + t0 / CKPT) * g.D + ch;
             if (ch < g.D) h.x = c[0];
             if (ch + 1 < g.D) h.y = c[1];
         }
-        cp_wait<ST - 1>();
-        __syncwarp();
-        F *slot = ring + (k % ST) * NT * SLOT;
-        const int n = (int)max(0ll, min((long long)S, g.T - t0));
-        if (n < S) close_gates(slot, n, lane);
-        f2 a[S], r[S], in[S], rs[S], P = both(1.f), hl = both(0.f), El = both(0.f);
-#pragma unroll
-        for (int s = 0; s < S; s++) {
-            const f2 rg = pair_at(slot, s, lane), ig = pair_at(slot + SLOT, s, lane), x = pair_at(slot + 2 * SLOT, s, lane);
-            r[s] = make_float2(sig(rg.x), sig(rg.y));
-            in[s] = make_float2(sig(ig.x), sig(ig.y));
-            a[s] = make_float2(ex2a(fmaf(r[s].x, k0.rate2, EX2_MEAN_)), ex2a(fmaf(r[s].y, k1.rate2, EX2_MEAN_)));
-            const f2 q = make_float2(one_minus_square(a[s].x, r[s].x * k0.x2), one_minus_square(a[s].y, r[s].y * k1.x2));
-            // 1 / m; where m is zero, so are L and m / that
-            rs[s] = make_float2(rsqrta(q.x > 1e-37f ? q.x : (q.x == q.x ? 1e-37f : q.x)), rsqrta(q.y > 1e-37f ? q.y : (q.y == q.y ? 1e-37f : q.y)));
-            hl = fma2(a[s], hl, mul2(mul2(mul2(q, rs[s]), in[s]), x));
-            P = mul2(P, a[s]);
+        if constexpr (MODE == TILES) {
+            await_tiles<ST>(ex, g, k);
+        } else {
+            __syncwarp();
+            if (k + ST - 1 < g.nsteps) start(k + ST - 1);
+            cp_commit();
+            cp_wait<ST - 1>();
+            __syncwarp();
         }
-        f2 sz[Z ? S : 1];
+        F *slot = ring + (k % ST) * NT * SLOT + warp * S * CH;
+        const int n = (int)max(0ll, min((long long)S, g.T - (t0 + warp * S)));
+        if (n < S) close_gates<F, S>(slot, n, lane);
+        // d = gy silu(z); e: what is left of gz without h; v = m i x.  i is m i / m, and 1 / (1 - a^2) the square of 1 / m.
+        f2 a[S], r[S], mi[S], rs[S], v[S], d[S], e[Z ? S : 1], P, hl, El = both(0.f);
+        auto segment = [&](auto fast) {
+            f2 range = both(0.f);
+            P = both(1.f);
+            hl = both(0.f);
 #pragma unroll
-        for (int s = S - 1; s >= 0; s--) {
-            f2 d = pair_at(slot + 3 * SLOT, s, lane);
-            if (Z) {
-                const f2 z = pair_at(slot + 4 * SLOT, s, lane);
-                sz[s] = make_float2(sig(z.x), sig(z.y));
-                d = mul2(d, mul2(z, sz[s]));
+            for (int s = 0; s < S; s++) {
+                const f2 z = Z ? pair_at(slot + 4 * SLOT, s, lane) : both(0.f);
+                f2 in, sz;
+                sigmoids<Z, decltype(fast)::value>(pair_at(slot, s, lane), pair_at(slot + SLOT, s, lane), z, r[s], in, sz, range);
+                a[s] = decays(r[s], rate);
+                const f2 q = one_minus_square(a[s], mul2(r[s], x2));
+                // (where 1 - a^2 is zero, so are L and m: any factor does; a NaN stays)
+                f2 low = q;
+                asm("max.NaN.f32 %0, %0, %1;" : "+f"(low.x) : "f"(1e-37f));
+                asm("max.NaN.f32 %0, %0, %1;" : "+f"(low.y) : "f"(1e-37f));
+                rs[s] = make_float2(rsqrta(low.x), rsqrta(low.y));
+                mi[s] = mul2(mul2(q, rs[s]), in);
+                v[s] = mul2(mi[s], pair_at(slot + 2 * SLOT, s, lane));
+                hl = fma2(a[s], hl, v[s]);
+                P = mul2(P, a[s]);
+                d[s] = pair_at(slot + 3 * SLOT, s, lane);
+                if (Z) {
+                    // silu' = s (1 + z (1 - s))
+                    const f2 gs = mul2(d[s], sz);
+                    d[s] = mul2(gs, z);
+                    e[s] = mul2(gs, fma2(z, sub2(both(1.f), sz), both(1.f)));
+                }
             }
-            El = mul2(a[s], add2(d, El));
-        }
+            return in_range(range);
+        };
+        if (!segment(std::true_type{})) segment(std::false_type{});
+#pragma unroll
+        for (int s = S - 1; s >= 0; s--) El = mul2(a[s], add2(d[s], El));
         const int side = k & 1;
         ex.seg[side][warp][lane] = make_float4(P.x, P.y, hl.x, hl.y);
         ex.segE[side][warp][lane] = El;
+        if (MODE == TILES && lane == 0) sm100::tma_store_wait_read();
         __syncthreads();
+        if (MODE == TILES && threadIdx.x == 0 && k > 0 && k + ST - 1 < g.nsteps) start(k + ST - 1);
         f2 Es = E;                                                  // behind this warp's segment
-#pragma unroll
-        for (int w = 0; w < NW; w++) {
-            const float4 q = ex.seg[side][w][lane];
-            if (w < warp) h = fma2(make_float2(q.x, q.y), h, make_float2(q.z, q.w));
-        }
         if (g.cl == 1) {
 #pragma unroll
-            for (int w = NW - 1; w >= 0; w--) {
-                const float4 q = ex.seg[side][w][lane];
-                if (w == warp) Es = E;
-                E = fma2(make_float2(q.x, q.y), E, ex.segE[side][w][lane]);
-            }
+            for (int w = NW - 1; w > 0; w--)
+                if (w > warp) {
+                    const float4 q = ex.seg[side][w][lane];
+                    Es = fma2(make_float2(q.x, q.y), Es, ex.segE[side][w][lane]);
+                }
+            E = fma2(P, Es, El);
+#pragma unroll
+            for (int w = NW - 2; w >= 0; w--)
+                if (w < warp) {
+                    const float4 q = ex.seg[side][w][lane];
+                    E = fma2(make_float2(q.x, q.y), E, ex.segE[side][w][lane]);
+                }
         } else {
             f2 Pc = both(1.f), Ec = both(0.f), Pw = both(1.f), Ew = both(0.f);
 #pragma unroll
@@ -440,48 +572,62 @@ __global__ void __launch_bounds__(256, 2) k_rec_bwd(const RecArgs g) {
             cl.sync();
             f2 Er = E;
             for (int q = g.cl - 1; q >= 0; q--) {
-                const float4 e = ex.cta[side][q][lane];
+                const float4 c = ex.cta[side][q][lane];
                 if (q == rank) Er = E;
-                E = fma2(make_float2(e.x, e.y), E, make_float2(e.z, e.w));
+                E = fma2(make_float2(c.x, c.y), E, make_float2(c.z, c.w));
             }
             Es = fma2(Pw, Er, Ew);
         }
 #pragma unroll
-        for (int s = 0; s < S; s++) {
-            keep_state(slot, SLOT, s, lane, h);
-            const f2 x = pair_at(slot + 2 * SLOT, s, lane);
-            const f2 q = make_float2(one_minus_square(a[s].x, r[s].x * k0.x2), one_minus_square(a[s].y, r[s].y * k1.x2));
-            h = fma2(a[s], h, mul2(mul2(mul2(q, rs[s]), in[s]), x));
-        }
+        for (int w = 0; w < NW - 1; w++)
+            if (w < warp) {
+                const float4 q = ex.seg[side][w][lane];
+                h = fma2(make_float2(q.x, q.y), h, make_float2(q.z, q.w));
+            }
+        f2 hb[S + 1];                                               // the states before the tokens
+        hb[0] = h;
+#pragma unroll
+        for (int s = 0; s < S; s++) hb[s + 1] = fma2(a[s], hb[s], v[s]);
+        const int m = ch < g.D ? n : 0;
+        const size_t block = ((size_t)b * g.T + t0) * g.D + ch0;
 #pragma unroll
         for (int s = S - 1; s >= 0; s--) {
-            const f2 x = pair_at(slot + 2 * SLOT, s, lane), gy = pair_at(slot + 3 * SLOT, s, lane), hb = kept_state(slot, SLOT, s, lane);
-            const f2 q = make_float2(one_minus_square(a[s].x, r[s].x * k0.x2), one_minus_square(a[s].y, r[s].y * k1.x2));
-            const f2 m = mul2(q, rs[s]), ix = mul2(in[s], x), mi = mul2(m, in[s]), L = mul2(r[s], rate);
-            f2 d = gy, gz = both(0.f);
-            if (Z) {
-                const f2 z = pair_at(slot + 4 * SLOT, s, lane);
-                const f2 hn = fma2(a[s], hb, mul2(m, ix));
-                d = mul2(d, mul2(z, sz[s]));
-                // silu' = s (1 + z (1 - s))
-                gz = mul2(mul2(gy, hn), mul2(sz[s], fma2(z, sub2(both(1.f), sz[s]), both(1.f))));
-            }
-            const f2 G = add2(d, Es), aL = mul2(a[s], L);
-            Es = mul2(a[s], G);
-            const f2 gx = mul2(G, mi), gi = mul2(mul2(mul2(G, m), ix), sub2(both(1.f), in[s]));
-            // G (h a L - i x a^2 L / m)
-            const f2 gLL = mul2(G, sub2(mul2(hb, aL), mul2(ix, mul2(mul2(a[s], aL), rs[s]))));
+            const f2 aL = mul2(a[s], mul2(r[s], rate)), Gs = add2(d[s], Es);
+            Es = mul2(a[s], Gs);
+            const f2 gx = mul2(Gs, mi[s]), gi = mul2(mul2(Gs, v[s]), sub2(both(1.f), mul2(mi[s], rs[s])));
+            // G (h a L - i x a^2 L / m), i / m = m i / m^2
+            const f2 gLL = mul2(Gs, sub2(mul2(hb[s], aL), mul2(mul2(mul2(v[s], rs[s]), rs[s]), mul2(a[s], aL))));
             total = add2(total, gLL);
-            const f2 gr = mul2(mul2(gLL, both(LN2_)), sub2(both(1.f), r[s]));
-            if (s < n && ch < g.D) {
-                const size_t at = ((size_t)b * g.T + t0 + s) * g.D + ch;
-                if (g.gx != nullptr) store_out((F *)g.gx + at, gx, pair, g.D - ch);
-                if (g.gig != nullptr) store_out((F *)g.gig + at, gi, pair, g.D - ch);
-                if (g.grg != nullptr) store_out((F *)g.grg + at, gr, pair, g.D - ch);
-                if (Z && g.gz != nullptr) store_out((F *)g.gz + at, gz, pair, g.D - ch);
+            const f2 gr = mul2(gLL, fma2(r[s], both(-LN2_), both(LN2_)));
+            const f2 gz = Z ? mul2(e[Z ? s : 0], hb[s + 1]) : both(0.f);
+            if constexpr (MODE == TILES) {
+                put_pair(slot, s, lane, gr);
+                put_pair(slot + SLOT, s, lane, gi);
+                put_pair(slot + 2 * SLOT, s, lane, gx);
+                if (Z) put_pair(slot + 3 * SLOT, s, lane, gz);
+            } else if (s < m) {
+                const uint32_t at = (uint32_t)(warp * S + s) * (uint32_t)g.D + 2 * lane;
+                if (g.gx != nullptr) store_out((F *)g.gx + block, at, gx, g.pair, g.D - ch);
+                if (g.gig != nullptr) store_out((F *)g.gig + block, at, gi, g.pair, g.D - ch);
+                if (g.grg != nullptr) store_out((F *)g.grg + block, at, gr, g.pair, g.D - ch);
+                if (Z && g.gz != nullptr) store_out((F *)g.gz + block, at, gz, g.pair, g.D - ch);
+            }
+        }
+        if constexpr (MODE == TILES) {
+            sm100::fence_async_smem();
+            __syncwarp();
+            if (lane == 0 && n > 0) {
+                const int t = (int)t0 + warp * S;
+                if (g.grg != nullptr) sm100::tma_store_3d(g.out + 2, slot, ch0, t, b);
+                if (g.gig != nullptr) sm100::tma_store_3d(g.out + 1, slot + SLOT, ch0, t, b);
+                if (g.gx != nullptr) sm100::tma_store_3d(g.out, slot + 2 * SLOT, ch0, t, b);
+                if (Z && g.gz != nullptr) sm100::tma_store_3d(g.out + 3, slot + 3 * SLOT, ch0, t, b);
+                sm100::tma_store_commit();
             }
         }
     }
+    if (MODE == TILES && lane == 0) sm100::tma_store_wait_all();
+    if (MODE == TILES) drain_tiles<ST>(ex, g);
     if (g.cl > 1) cg::this_cluster().sync();
     if (g.gs_in != nullptr && warp == 0 && rank == 0) {
         if (ch < g.D) g.gs_in[(size_t)b * g.D + ch] = E.x;
@@ -523,14 +669,14 @@ __global__ void __launch_bounds__(128) k_rec_step(const RecArgs g, long long pai
     if (g.state_in != nullptr) h = make_float2(g.state_in[at], n > 1 ? g.state_in[at + 1] : 0.f);
     auto one = [&](float h, float x, float ig, float rg, float p) {
         const Rate k = rate_of(p, g.c);
-        const float r = sig(rg), a = ex2a(fmaf(r, k.rate2, EX2_MEAN_)), m = sqrtf(one_minus_square(a, r * k.x2));
+        const float r = sig(rg), a = ex2a(fmaf(r, k.rate2, EX2_MEAN_)), m = sqrtf(one_minus_square(both(a), both(r * k.x2)).x);
         return fmaf(a, h, m * sig(ig) * x);
     };
     h = make_float2(one(h.x, x.x, ig.x, rg.x, g.decay[ch]), n > 1 ? one(h.y, x.y, ig.y, rg.y, g.decay[ch + 1]) : 0.f);
     g.state_out[at] = h.x;
     if (n > 1) g.state_out[at + 1] = h.y;
     if (g.z != nullptr) h = mul2(h, mul2(z, make_float2(sig(z.x), sig(z.y))));
-    store_out((F *)g.y + at, h, (g.D & 1) == 0 && ((uintptr_t)g.y & (2 * sizeof(F) - 1)) == 0, n);
+    store_out((F *)g.y + at, 0u, h, vec, n);
 }
 
 template <typename F> bool lies_in(const wkv_gated_recurrence_args_t *a, size_t bytes, bool back) {
@@ -543,27 +689,42 @@ template <typename F> bool lies_in(const wkv_gated_recurrence_args_t *a, size_t 
     look(a->input_gate, a->i_batch, a->i_token);
     look(a->decay_gate, a->r_batch, a->r_token);
     look(a->z, a->z_batch, a->z_token);
-    if (back) look(a->gy, (long long)a->T * a->D, a->D);
-    return ok && (bytes == 4 || a->D % e == 0);
+    if (back) {
+        for (const void *p : {a->gy, (const void *)a->gx, (const void *)a->ginput_gate, (const void *)a->gdecay_gate, (const void *)a->gz})
+            look(p, (long long)a->T * a->D, a->D);
+    } else {
+        look(a->y, (long long)a->T * a->D, a->D);
+    }
+    return ok && (bytes < 16 || a->D % e == 0);
 }
 
 // CTAs of a cluster: as many as there are places for (two CTAs an SM) and blocks of tokens to take
-int cluster_size(const wkv_gated_recurrence_args_t *a) {
-    const int bt = a->dtype == WKV_F32 ? Geo<float>::BT : Geo<__half>::BT;
+int cluster_size(const wkv_gated_recurrence_args_t *a, int bt) {
     const long long chains = (long long)a->B * ((a->D + CH - 1) / CH), places = 2ll * device_sm_count(), blocks = ((long long)a->T + bt - 1) / bt;
     int cl = 1;
     while (cl < MAX_CL && chains * cl * 2 <= places && cl * 2 <= blocks) cl *= 2;
     return cl;
 }
+int block_tokens(const wkv_gated_recurrence_args_t *a, bool back) {
+    if (back) return CKPT;
+    return a->dtype == WKV_F32 ? Geo<float, false>::BT : Geo<__half, false>::BT;
+}
 
+bool strides_ok(const wkv_gated_recurrence_args_t *a) {
+    for (long long t : {a->x_token, a->i_token, a->r_token, a->z != nullptr ? a->z_token : 0})
+        if (a->T > 1 && (t < 0 || t > 1 << 26)) return false;
+    return true;
+}
 bool sizes_ok(const wkv_gated_recurrence_args_t *a) {
     return a->B >= 0 && a->T >= 0 && a->D >= 0 && a->D <= (1 << 22) && a->T <= 2147483647 - 4096 && known_dtype(a->dtype) &&
-           (long long)a->B * ((a->D + CH - 1) / CH) <= 2147483647 / MAX_CL && (long long)a->B * a->D <= 1ll << 34 && a->c > 0.f;
+           (long long)a->B * ((a->D + CH - 1) / CH) <= 2147483647 / MAX_CL && (long long)a->B * a->D <= 1ll << 34 && a->c > 0.f &&
+           strides_ok(a);
 }
-RecArgs args_of(const wkv_gated_recurrence_args_t *a) {
+RecArgs args_of(const wkv_gated_recurrence_args_t *a, bool back) {
     RecArgs g = {};
-    const int bt = a->dtype == WKV_F32 ? Geo<float>::BT : Geo<__half>::BT;
-    g.T = a->T; g.D = a->D; g.slabs = (a->D + CH - 1) / CH; g.cl = cluster_size(a);
+    const int bt = block_tokens(a, back);
+    g.T = a->T; g.D = a->D; g.slabs = (a->D + CH - 1) / CH; g.cl = cluster_size(a, bt);
+    g.nkept = (int)(((long long)a->T + CKPT - 1) / CKPT);
     g.nsteps = (int)(((long long)a->T + (long long)bt * g.cl - 1) / ((long long)bt * g.cl));
     g.c = a->c;
     g.x = a->x; g.ig = a->input_gate; g.rg = a->decay_gate; g.z = a->z;
@@ -572,12 +733,10 @@ RecArgs args_of(const wkv_gated_recurrence_args_t *a) {
     g.decay = a->decay; g.state_in = a->state_in; g.y = a->y; g.state_out = a->state_out; g.ckpt = (float *)a->ckpt;
     g.gy = a->gy; g.gs_out = a->gstate_out; g.gx = a->gx; g.gig = a->ginput_gate; g.grg = a->gdecay_gate; g.gz = a->gz;
     g.gs_in = a->gstate_in; g.part = (float *)a->workspace;
+    g.status = a->status; g.limit = 4000000u;
     return g;
 }
-size_t ckpt_need(const wkv_gated_recurrence_args_t *a) {
-    const RecArgs g = args_of(a);
-    return (size_t)a->B * g.nsteps * g.cl * a->D * 4;
-}
+size_t ckpt_need(const wkv_gated_recurrence_args_t *a) { return (size_t)a->B * (((size_t)a->T + CKPT - 1) / CKPT) * a->D * 4; }
 
 template <class K>
 int launch_rec(K kern, const RecArgs &g, int B, int smem, unsigned char (&done)[64], cudaStream_t s) {
@@ -600,17 +759,38 @@ int launch_rec(K kern, const RecArgs &g, int B, int smem, unsigned char (&done)[
 template <typename F, bool Z, int MODE, bool BACK>
 int launch_as(const RecArgs &g, int B, cudaStream_t s) {
     static unsigned char done[64];
-    if constexpr (BACK) return launch_rec(k_rec_bwd<F, Z, MODE>, g, B, Geo<F>::bwd_ring(Z) + (int)sizeof(ExchangeBack), done, s);
-    else return launch_rec(k_rec_fwd<F, Z, MODE>, g, B, Geo<F>::fwd_ring(Z) + (int)sizeof(Exchange), done, s);
+    if constexpr (BACK) return launch_rec(k_rec_bwd<F, Z, MODE>, g, B, Geo<F, true>::ring(Z) + (int)sizeof(ExchangeBack), done, s);
+    else return launch_rec(k_rec_fwd<F, Z, MODE>, g, B, Geo<F, false>::ring(Z) + (int)sizeof(Exchange), done, s);
 }
+// the tiles' maps; false: TMA cannot read or write these rows
+template <typename F, bool BACK>
+bool make_maps(const wkv_gated_recurrence_args_t *a, RecArgs &g) {
+    using G = Geo<F, BACK>;
+    const long long yt = a->D, yb = (long long)a->T * a->D;
+    const int z = a->z != nullptr;
+    struct { const void *p; long long batch, token; } in[5] = {{a->decay_gate, a->r_batch, a->r_token}, {a->input_gate, a->i_batch, a->i_token}, {a->x, a->x_batch, a->x_token}};
+    in[3 + BACK] = {a->z, a->z_batch, a->z_token};
+    if (BACK) in[3] = {a->gy, yb, yt};
+    for (int i = 0; i < 3 + BACK + z; i++) {
+        // (a dimension of one element may have any stride)
+        const long long token = a->T > 1 ? in[i].token : yt, batch = a->B > 1 ? in[i].batch : token * a->T;
+        if (in[i].p == nullptr || !make_tile_map(&g.in[i], in[i].p, sizeof(F), a->B, a->T, a->D, batch, token, CH, G::BT)) return false;
+    }
+    void *out[4] = {BACK ? a->gx : a->y, a->ginput_gate, a->gdecay_gate, a->gz};
+    for (int i = 0; i < (BACK ? 3 + z : 1); i++)
+        if (out[i] != nullptr && !make_tile_map(&g.out[i], out[i], sizeof(F), a->B, a->T, a->D, yb, yt, CH, G::S)) return false;
+    return true;
+}
+
 template <bool BACK>
-int launch_by(const wkv_gated_recurrence_args_t *a, const RecArgs &g, cudaStream_t s) {
+int launch_by(const wkv_gated_recurrence_args_t *a, RecArgs &g, cudaStream_t s) {
     return by_dtype(a->dtype, [&](auto f) {
         using F = decltype(f);
-        const int mode = lies_in<F>(a, 16, BACK) ? PIECES : sizeof(F) == 4 || lies_in<F>(a, 4, BACK) ? WORDS : ANYWHERE;
+        g.pair = a->D % 2 == 0 && lies_in<F>(a, 2 * sizeof(F), BACK);
+        const int mode = a->T > 0 && lies_in<F>(a, 16, BACK) && make_maps<F, BACK>(a, g) ? TILES : sizeof(F) == 4 || lies_in<F>(a, 4, BACK) ? WORDS : ANYWHERE;
         auto go = [&](auto zc) {
             constexpr bool Z = decltype(zc)::value;
-            if (mode == PIECES) return launch_as<F, Z, PIECES, BACK>(g, a->B, s);
+            if (mode == TILES) return launch_as<F, Z, TILES, BACK>(g, a->B, s);
             if constexpr (sizeof(F) == 2) {
                 if (mode == ANYWHERE) return launch_as<F, Z, ANYWHERE, BACK>(g, a->B, s);
             }
@@ -634,7 +814,7 @@ extern "C" int wkv_gated_recurrence_forward(const wkv_gated_recurrence_args_t *a
     if ((long long)a->B * a->D == 0) return WKV_OK;
     if (a->decay == nullptr || a->state_out == nullptr) return WKV_ERR_NULL;
     if (a->T > 0 && (a->x == nullptr || a->input_gate == nullptr || a->decay_gate == nullptr || a->y == nullptr)) return WKV_ERR_NULL;
-    RecArgs g = args_of(a);
+    RecArgs g = args_of(a, false);
     const cudaStream_t s = (cudaStream_t)stream;
     if (a->T == 1 && a->ckpt == nullptr) {
         const int row = (a->D + 1) / 2;
@@ -650,7 +830,7 @@ extern "C" int wkv_gated_recurrence_forward(const wkv_gated_recurrence_args_t *a
 }
 
 extern "C" size_t wkv_gated_recurrence_backward_workspace(const wkv_gated_recurrence_args_t *a) {
-    return a != nullptr && sizes_ok(a) && a->gdecay != nullptr ? (size_t)a->B * cluster_size(a) * a->D * 4 : 0;
+    return a != nullptr && sizes_ok(a) && a->gdecay != nullptr ? (size_t)a->B * cluster_size(a, CKPT) * a->D * 4 : 0;
 }
 
 extern "C" int wkv_gated_recurrence_backward(const wkv_gated_recurrence_args_t *a, void *stream) {
@@ -665,7 +845,7 @@ extern "C" int wkv_gated_recurrence_backward(const wkv_gated_recurrence_args_t *
     if (a->decay == nullptr || (a->T > 0 && (a->x == nullptr || a->input_gate == nullptr || a->decay_gate == nullptr))) return WKV_ERR_NULL;
     if (a->T > 0 && (a->ckpt == nullptr || a->ckpt_bytes < ckpt_need(a))) return WKV_ERR_WORKSPACE;
     if (a->gdecay != nullptr && (a->workspace == nullptr || a->workspace_bytes < wkv_gated_recurrence_backward_workspace(a))) return WKV_ERR_WORKSPACE;
-    RecArgs g = args_of(a);
+    RecArgs g = args_of(a, true);
     if (a->gdecay == nullptr) g.part = nullptr;
     const int rc = launch_by<true>(a, g, s);
     if (rc != WKV_OK || a->gdecay == nullptr) return rc;

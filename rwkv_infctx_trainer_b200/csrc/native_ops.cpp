@@ -17,7 +17,7 @@ void raise_if_set(int device, int *word) {
     // reported once; taken and cleared in one step, so that a bit a kernel sets meanwhile is reported by this look or the next
     const int code = __atomic_exchange_n(word, 0, __ATOMIC_ACQ_REL);
     if (code == 0) return;      // (another thread reports it)
-    TORCH_CHECK(false, "a v5/v6 call or a matrix product (status bit 64) on cuda:", device, ": a device-side wait ran out (status ", code,
+    TORCH_CHECK(false, "a v5/v6 call, a matrix product (status bit 64) or a gated recurrence (128) on cuda:", device, ": a device-side wait ran out (status ", code,
                 "); the outputs of that call are invalid");
 }
 }  // namespace

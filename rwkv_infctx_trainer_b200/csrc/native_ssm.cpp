@@ -423,6 +423,8 @@ RecCall rec_call(const Tensor &x, const Tensor &ig, const Tensor &rg, const Tens
     a.x_batch = r.x.batch; a.x_token = r.x.token; a.i_batch = r.ig.batch; a.i_token = r.ig.token;
     a.r_batch = r.rg.batch; a.r_token = r.rg.token; a.z_batch = r.z.batch; a.z_token = r.z.token;
     a.decay = (const float *)ptr(r.decay); a.state_in = (const float *)ptr(r.state);
+    a.status = status_word(x.device().index());
+    poll_status(x.device().index(), false);
     return r;
 }
 

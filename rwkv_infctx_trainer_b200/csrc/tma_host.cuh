@@ -101,4 +101,42 @@ inline bool make_matrix_map(CUtensorMap *map, const void *base, long long rows, 
     return true;
 }
 
+// Map over activations [B, T, D] of 2- or 4-byte elements, channels adjacent, rows `batch` and `token` elements apart; box = channels x
+// tokens x 1, unswizzled, what lies outside reads as zero and is not written.  False where TMA cannot take them (addresses and strides that
+// are no multiples of 16 bytes, strides it has no room for).  Remembered as above.
+inline bool make_tile_map(CUtensorMap *map, const void *base, int elem, int B, int T, int D, long long batch, long long token, int channels, int tokens) {
+    struct Entry {
+        CUtensorMap map;
+        const void *base;
+        int elem, B, T, D, channels, tokens;
+        long long batch, token;
+    };
+    constexpr int LOG_SLOTS = 9;
+    static thread_local Entry cache[1 << LOG_SLOTS];
+    if (base == nullptr || (uintptr_t)base % 16 || batch * elem % 16 || token * elem % 16 || batch < 0 || token < 0 || batch >= 1ll << 37 || token >= 1ll << 37)
+        return false;
+    const uint64_t key = (uint64_t)(uintptr_t)base ^ (uint64_t)T << 40 ^ (uint64_t)D << 52 ^ (uint64_t)B << 48 ^ (uint64_t)tokens << 34;
+    Entry &e = cache[(key >> 8) * 0x9E3779B97F4A7C15ull >> (64 - LOG_SLOTS)];
+    if (e.base == base && e.elem == elem && e.B == B && e.T == T && e.D == D && e.channels == channels && e.tokens == tokens && e.batch == batch && e.token == token) {
+        *map = e.map;
+        return true;
+    }
+    encode_tiled_fn enc = tensor_map_encoder();
+    if (!enc) return false;
+    cuuint64_t dims[3] = {(cuuint64_t)D, (cuuint64_t)T, (cuuint64_t)B};
+    cuuint64_t strides[2] = {(cuuint64_t)(token * elem), (cuuint64_t)(batch * elem)};
+    cuuint32_t box[3] = {(cuuint32_t)channels, (cuuint32_t)tokens, 1};
+    cuuint32_t estr[3] = {1, 1, 1};
+    const auto encode = [&] {
+        return enc(map, elem == 2 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 3, const_cast<void *>(base), dims, strides, box, estr,
+                   CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    };
+    if (encode() != CUDA_SUCCESS) {
+        int dev = 0;
+        if (cudaGetDevice(&dev) != cudaSuccess || cudaSetDevice(dev) != cudaSuccess || encode() != CUDA_SUCCESS) return false;
+    }
+    e.base = base; e.elem = elem; e.B = B; e.T = T; e.D = D; e.channels = channels; e.tokens = tokens; e.batch = batch; e.token = token; e.map = *map;
+    return true;
+}
+
 }  // namespace wkv
