@@ -393,6 +393,7 @@ typedef struct wkv_gated_recurrence_args {
     int *status;
 } wkv_gated_recurrence_args_t;
 size_t wkv_gated_recurrence_ckpt_bytes(const wkv_gated_recurrence_args_t *a);
+size_t wkv_gated_recurrence_forward_workspace(const wkv_gated_recurrence_args_t *a);
 int wkv_gated_recurrence_forward(const wkv_gated_recurrence_args_t *a, void *stream);
 size_t wkv_gated_recurrence_backward_workspace(const wkv_gated_recurrence_args_t *a);
 int wkv_gated_recurrence_backward(const wkv_gated_recurrence_args_t *a, void *stream);

@@ -112,7 +112,7 @@ EXPORTS = [
     "wkv_causal_conv_forward", "wkv_causal_conv_backward_workspace", "wkv_causal_conv_backward",
     "wkv_selective_scan_ckpt_bytes", "wkv_selective_scan_forward_workspace", "wkv_selective_scan_forward",
     "wkv_selective_scan_backward_workspace", "wkv_selective_scan_backward",
-    "wkv_gated_recurrence_ckpt_bytes", "wkv_gated_recurrence_forward",
+    "wkv_gated_recurrence_ckpt_bytes", "wkv_gated_recurrence_forward_workspace", "wkv_gated_recurrence_forward",
     "wkv_gated_recurrence_backward_workspace", "wkv_gated_recurrence_backward",
     "wkv_linear_saved_bytes", "wkv_linear_forward_workspace", "wkv_linear_forward", "wkv_linear_backward_workspace",
     "wkv_linear_backward",
@@ -214,7 +214,7 @@ def load() -> ctypes.CDLL:
             fn = getattr(lib, f"wkv_{name}_{d}")
             fn.restype = i
             fn.argtypes = [ctypes.POINTER(args), _vp]
-            if d == "backward" or name in ("selective_scan", "linear"):
+            if d == "backward" or name not in ("rms_norm", "causal_conv"):
                 ws = getattr(lib, f"wkv_{name}_{d}_workspace")
                 ws.restype = sz
                 ws.argtypes = [ctypes.POINTER(args)]

@@ -15,26 +15,24 @@
 // in registers.  So the serial chain is 8 + S steps a block, and the gates, which are most of the work, are formed once.
 // A warp's inputs come through a ring of its own in shared memory (cp.async), the blocks behind on their way meanwhile.
 //
-// Few chains: the CTAs of a cluster take neighbouring blocks of one row and exchange their folds through distributed shared
-// memory (one cluster barrier a step); nothing is read twice and nothing is waited for in global memory.
+// Few chains: a row is cut into spans that run in parallel.  A first pass leaves what a span does to the state (its decay and its state
+// from zero; backward: to E), without a barrier: its warps take an eighth of a span each.  The full pass starts from the fold of the
+// spans before it.  (A cluster's CTAs on neighbouring blocks of a row, their folds exchanged through distributed shared memory at
+// every step, read nothing twice, and took 2 us a step more: 4 x 4096 x 4096 forward 258 us with two CTAs a cluster, 165 without.)
 //
 // Backward: blocks in reverse.  The forward pass leaves the state before each block (4 bytes a channel per 8 S tokens); hl and
 // P are formed again, and with them the segment's E from zero, so that one exchange serves both directions.
 //
 // 1 - a^2 is -expm1(2L): its series below 1/4 (2^-24 of it are left out there), 1 - a a above.
-#include <cooperative_groups.h>
-
 #include "elem_io.cuh"
 #include "sm100_primitives.cuh"
 #include "tma_host.cuh"
 #include "wkv_internal.h"
 
-namespace cg = cooperative_groups;
-
 namespace wkv {
 namespace {
 
-constexpr int CH = 64, NW = 8, MAX_CL = 8;
+constexpr int CH = 64, NW = 8, MAX_SPANS = 256;
 constexpr float LOG2E_ = 1.4426950408889634f, LN2_ = 0.6931471805599453f;
 // the mean error of ex2 over exponents from -0.5 to -0.01, made good in its argument (selective_scan.cu)
 constexpr float EX2_MEAN_ = 1.8e-8f;
@@ -57,8 +55,9 @@ __device__ __forceinline__ float rsqrta(float x) {
 __device__ __forceinline__ float sig(float x) { return rcpa(1.f + ex2a(-LOG2E_ * x)); }
 
 struct RecArgs {
+    CUtensorMap in_spans[5];              // as `in`, the tiles of a warp
     CUtensorMap in[5], out[4];            // TILES: decay gate, input gate, x, (gy,) z; y, or gx, ginput_gate, gdecay_gate, gz
-    int T, D, slabs, cl, nsteps;          // slabs of CH channels; cl: CTAs of a cluster, nsteps: blocks of a row / cl, rounded up
+    int T, D, slabs, nspan, span;         // slabs of CH channels; spans of a row, tokens of a span (a multiple of a block)
     float c;
     const void *x, *ig, *rg, *z;
     long long x_batch, x_token, ig_batch, ig_token, rg_batch, rg_token, z_batch, z_token;
@@ -71,7 +70,8 @@ struct RecArgs {
     const void *gy;
     const float *gs_out;
     void *gx, *gig, *grg, *gz;
-    float *gs_in, *part;                  // part [B * cl, D]
+    float *gs_in, *part;                  // part [B * nspan, D]
+    float2 *spans;                        // [B, nspan, D]: a span's decay, and its state (backward: E) from zero
 };
 
 // Tokens of a warp in a block (S), for two CTAs an SM: what a thread keeps of its tokens has to fit in 128 registers, because what
@@ -237,14 +237,12 @@ __device__ __forceinline__ void put_pair(F *slot, int s, int lane, f2 v) {
 // what a segment does to the state (and to E): [side][segment][channel pair]
 struct Exchange {
     float4 seg[2][NW][32];                // P, hl of two channels
-    float4 cta[2][MAX_CL][32];            // the same of the cluster's CTAs
     uint64_t full[4];
     int abort;
 };
 struct ExchangeBack {
     float4 seg[2][NW][32];                // P, hl
     f2 segE[2][NW][32];                   // E from zero
-    float4 cta[2][MAX_CL][32];            // P, E of the cluster's CTAs
     f2 sum[NW][32];
     uint64_t full[4];
     int abort;
@@ -268,11 +266,28 @@ __device__ __forceinline__ void await_tiles(X &ex, const RecArgs &g, int k) {
         if (g.status != nullptr) atomicOr(g.status, WKV_RECURRENCE_TIMEOUT);
     }
 }
+// two channels' state (or E) behind the spans from `first` up to `last`
+__device__ __forceinline__ f2 fold_spans(const RecArgs &g, int b, int first, int last, int dir, int ch, f2 h) {
+    const float2 *p = g.spans + (size_t)b * g.nspan * g.D + ch;
+#pragma unroll 4
+    for (int i = first; i != last; i += dir) {
+        if (ch < g.D) {
+            const float2 q = p[(size_t)i * g.D];
+            h.x = fmaf(q.x, h.x, q.y);
+        }
+        if (ch + 1 < g.D) {
+            const float2 q = p[(size_t)i * g.D + 1];
+            h.y = fmaf(q.x, h.y, q.y);
+        }
+    }
+    return h;
+}
+
 // (after a wait that ran out: tiles may still be on their way into this CTA's shared memory)
 template <int ST, class X>
-__device__ __forceinline__ void drain_tiles(X &ex, const RecArgs &g) {
+__device__ __forceinline__ void drain_tiles(X &ex, const RecArgs &g, int nsteps) {
     if (threadIdx.x != 0 || *(volatile int *)&ex.abort == 0) return;
-    for (int k = max(0, g.nsteps - ST); k < g.nsteps; k++) sm100::mbar_wait(ex.full + k % ST, (k / ST) & 1, g.limit);
+    for (int k = max(0, nsteps - ST); k < nsteps; k++) sm100::mbar_wait(ex.full + k % ST, (k / ST) & 1, g.limit);
 }
 
 template <typename F, bool Z, int MODE>
@@ -284,7 +299,9 @@ __global__ void __launch_bounds__(256, 2) k_rec_fwd(const __grid_constant__ RecA
     extern __shared__ __align__(128) unsigned char smem[];
     Exchange &ex = *reinterpret_cast<Exchange *>(smem + RING);
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int rank = blockIdx.x % g.cl, chain = blockIdx.x / g.cl, b = chain / g.slabs, ch0 = (chain - b * g.slabs) * CH, ch = ch0 + 2 * lane;
+    const int span = blockIdx.x % g.nspan, chain = blockIdx.x / g.nspan, b = chain / g.slabs, ch0 = (chain - b * g.slabs) * CH, ch = ch0 + 2 * lane;
+    const long long begin = (long long)span * g.span;
+    const int nsteps = (int)((min((long long)g.T, begin + g.span) - begin + BT - 1) / BT);
     F *ring = reinterpret_cast<F *>(smem);                          // [stage][tensor][warp][S][CH]
 
     const Rate k0 = rate_of(ch < g.D ? g.decay[ch] : 0.f, g.c), k1 = rate_of(ch + 1 < g.D ? g.decay[ch + 1] : 0.f, g.c);
@@ -294,8 +311,9 @@ __global__ void __launch_bounds__(256, 2) k_rec_fwd(const __grid_constant__ RecA
         if (ch < g.D) h.x = g.state_in[(size_t)b * g.D + ch];
         if (ch + 1 < g.D) h.y = g.state_in[(size_t)b * g.D + ch + 1];
     }
+    if (span > 0) h = fold_spans(g, b, 0, span, 1, ch, h);
     auto start = [&](int step) {
-        const long long t0 = ((long long)step * g.cl + rank) * BT, at = t0 < g.T ? t0 : 0;
+        const long long t0 = begin + (long long)step * BT;
         F *slot = ring + (step % ST) * NT * SLOT;
         if constexpr (MODE == TILES) {
             sm100::mbar_expect_tx(ex.full + step % ST, NT * SLOT * sizeof(F));
@@ -304,36 +322,36 @@ __global__ void __launch_bounds__(256, 2) k_rec_fwd(const __grid_constant__ RecA
         } else {
             const int n = (int)max(0ll, min((long long)S, g.T - (t0 + warp * S))), left = g.D - ch0;
             slot += warp * S * CH;
-            fill<F, MODE, S>(slot, (const F *)g.rg + (b * g.rg_batch + at * g.rg_token + ch0), (int)g.rg_token, warp, n, left, lane);
-            fill<F, MODE, S>(slot + SLOT, (const F *)g.ig + (b * g.ig_batch + at * g.ig_token + ch0), (int)g.ig_token, warp, n, left, lane);
-            fill<F, MODE, S>(slot + 2 * SLOT, (const F *)g.x + (b * g.x_batch + at * g.x_token + ch0), (int)g.x_token, warp, n, left, lane);
-            if (Z) fill<F, MODE, S>(slot + 3 * SLOT, (const F *)g.z + (b * g.z_batch + at * g.z_token + ch0), (int)g.z_token, warp, n, left, lane);
+            fill<F, MODE, S>(slot, (const F *)g.rg + (b * g.rg_batch + t0 * g.rg_token + ch0), (int)g.rg_token, warp, n, left, lane);
+            fill<F, MODE, S>(slot + SLOT, (const F *)g.ig + (b * g.ig_batch + t0 * g.ig_token + ch0), (int)g.ig_token, warp, n, left, lane);
+            fill<F, MODE, S>(slot + 2 * SLOT, (const F *)g.x + (b * g.x_batch + t0 * g.x_token + ch0), (int)g.x_token, warp, n, left, lane);
+            if (Z) fill<F, MODE, S>(slot + 3 * SLOT, (const F *)g.z + (b * g.z_batch + t0 * g.z_token + ch0), (int)g.z_token, warp, n, left, lane);
         }
     };
     if constexpr (MODE == TILES) {
         init_tiles<ST>(ex);
         if (threadIdx.x == 0) {
-            for (int p = 0; p < min(ST, g.nsteps); p++) start(p);
+            for (int p = 0; p < min(ST, nsteps); p++) start(p);
         }
     } else {
 #pragma unroll
         for (int p = 0; p < ST - 1; p++) {
-            if (p < g.nsteps) start(p);
+            if (p < nsteps) start(p);
             cp_commit();
         }
     }
-    for (int step = 0; step < g.nsteps; step++) {
+    for (int step = 0; step < nsteps; step++) {
         if constexpr (MODE == TILES) {
             await_tiles<ST>(ex, g, step);
         } else {
             __syncwarp();                                           // (all lanes are done with the slot that is filled now)
-            if (step + ST - 1 < g.nsteps) start(step + ST - 1);
+            if (step + ST - 1 < nsteps) start(step + ST - 1);
             cp_commit();
             cp_wait<ST - 1>();
             __syncwarp();
         }
         F *slot = ring + (step % ST) * NT * SLOT + warp * S * CH;
-        const long long t0 = ((long long)step * g.cl + rank) * BT;
+        const long long t0 = begin + (long long)step * BT;
         const int n = (int)max(0ll, min((long long)S, g.T - (t0 + warp * S)));          // this warp's tokens of the block
         if (n < S) close_gates<F, S>(slot, n, lane);
         f2 a[S], v[S], gate[Z ? S : 1], P, hl;
@@ -360,37 +378,13 @@ __global__ void __launch_bounds__(256, 2) k_rec_fwd(const __grid_constant__ RecA
         ex.seg[side][warp][lane] = make_float4(P.x, P.y, hl.x, hl.y);
         if (MODE == TILES && lane == 0) sm100::tma_store_wait_read();                   // (of the block before: its stage is filled next)
         __syncthreads();
-        if (MODE == TILES && threadIdx.x == 0 && step > 0 && step + ST - 1 < g.nsteps) start(step + ST - 1);
+        if (MODE == TILES && threadIdx.x == 0 && step > 0 && step + ST - 1 < nsteps) start(step + ST - 1);
         f2 hs = h;                                                  // before this warp's segment
-        if (g.cl == 1) {
 #pragma unroll
-            for (int w = 0; w < NW; w++) {
-                const float4 q = ex.seg[side][w][lane];
-                if (w == warp) hs = h;
-                h = fma2(make_float2(q.x, q.y), h, make_float2(q.z, q.w));
-            }
-        } else {
-            f2 Pc = both(1.f), hc = both(0.f), Pw = both(1.f), hw = both(0.f);
-#pragma unroll
-            for (int w = 0; w < NW; w++) {
-                const float4 q = ex.seg[side][w][lane];
-                if (w == warp) { Pw = Pc; hw = hc; }
-                hc = fma2(make_float2(q.x, q.y), hc, make_float2(q.z, q.w));
-                Pc = mul2(Pc, make_float2(q.x, q.y));
-            }
-            cg::cluster_group cl = cg::this_cluster();
-            if (warp < g.cl) {
-                Exchange *to = cl.map_shared_rank(&ex, warp);
-                to->cta[side][rank][lane] = make_float4(Pc.x, Pc.y, hc.x, hc.y);
-            }
-            cl.sync();
-            f2 hr = h;
-            for (int q = 0; q < g.cl; q++) {
-                const float4 e = ex.cta[side][q][lane];
-                if (q == rank) hr = h;
-                h = fma2(make_float2(e.x, e.y), h, make_float2(e.z, e.w));
-            }
-            hs = fma2(Pw, hr, hw);
+        for (int w = 0; w < NW; w++) {
+            const float4 q = ex.seg[side][w][lane];
+            if (w == warp) hs = h;
+            h = fma2(make_float2(q.x, q.y), h, make_float2(q.z, q.w));
         }
         if (g.ckpt != nullptr && warp * S % CKPT == 0 && n > 0) {
             float *c = g.ckpt + ((size_t)b * g.nkept + (t0 + warp * S) / CKPT) * g.D + ch;
@@ -420,9 +414,8 @@ __global__ void __launch_bounds__(256, 2) k_rec_fwd(const __grid_constant__ RecA
         }
     }
     if (MODE == TILES && lane == 0) sm100::tma_store_wait_all();
-    if (MODE == TILES) drain_tiles<ST>(ex, g);
-    if (g.cl > 1) cg::this_cluster().sync();                        // (no CTA leaves while another may write to it)
-    if (g.state_out != nullptr && warp == 0 && rank == 0) {
+    if (MODE == TILES) drain_tiles<ST>(ex, g, nsteps);
+    if (g.state_out != nullptr && warp == 0 && span == g.nspan - 1) {
         if (ch < g.D) g.state_out[(size_t)b * g.D + ch] = h.x;
         if (ch + 1 < g.D) g.state_out[(size_t)b * g.D + ch + 1] = h.y;
     }
@@ -438,7 +431,9 @@ __global__ void __launch_bounds__(256, 2) k_rec_bwd(const __grid_constant__ RecA
     extern __shared__ __align__(128) unsigned char smem[];
     ExchangeBack &ex = *reinterpret_cast<ExchangeBack *>(smem + RING);
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int rank = blockIdx.x % g.cl, chain = blockIdx.x / g.cl, b = chain / g.slabs, ch0 = (chain - b * g.slabs) * CH, ch = ch0 + 2 * lane;
+    const int span = blockIdx.x % g.nspan, chain = blockIdx.x / g.nspan, b = chain / g.slabs, ch0 = (chain - b * g.slabs) * CH, ch = ch0 + 2 * lane;
+    const long long begin = (long long)span * g.span;
+    const int nsteps = (int)((min((long long)g.T, begin + g.span) - begin + BT - 1) / BT);
     F *ring = reinterpret_cast<F *>(smem);
 
     const Rate k0 = rate_of(ch < g.D ? g.decay[ch] : 0.f, g.c), k1 = rate_of(ch + 1 < g.D ? g.decay[ch + 1] : 0.f, g.c);
@@ -449,8 +444,9 @@ __global__ void __launch_bounds__(256, 2) k_rec_bwd(const __grid_constant__ RecA
         if (ch + 1 < g.D) E.y = g.gs_out[(size_t)b * g.D + ch + 1];
     }
     // (k counts the steps in the order of the walk)
+    if (span < g.nspan - 1) E = fold_spans(g, b, g.nspan - 1, span, -1, ch, E);
     auto start = [&](int k) {
-        const long long t0 = ((long long)(g.nsteps - 1 - k) * g.cl + rank) * BT, at = t0 < g.T ? t0 : 0;
+        const long long t0 = begin + (long long)(nsteps - 1 - k) * BT;
         F *slot = ring + (k % ST) * NT * SLOT;
         if constexpr (MODE == TILES) {
             sm100::mbar_expect_tx(ex.full + k % ST, NT * SLOT * sizeof(F));
@@ -459,30 +455,30 @@ __global__ void __launch_bounds__(256, 2) k_rec_bwd(const __grid_constant__ RecA
         } else {
             const int n = (int)max(0ll, min((long long)S, g.T - (t0 + warp * S))), left = g.D - ch0;
             slot += warp * S * CH;
-            fill<F, MODE, S>(slot, (const F *)g.rg + (b * g.rg_batch + at * g.rg_token + ch0), (int)g.rg_token, warp, n, left, lane);
-            fill<F, MODE, S>(slot + SLOT, (const F *)g.ig + (b * g.ig_batch + at * g.ig_token + ch0), (int)g.ig_token, warp, n, left, lane);
-            fill<F, MODE, S>(slot + 2 * SLOT, (const F *)g.x + (b * g.x_batch + at * g.x_token + ch0), (int)g.x_token, warp, n, left, lane);
-            if (g.gy != nullptr) fill<F, MODE, S>(slot + 3 * SLOT, (const F *)g.gy + (((size_t)b * g.T + at) * g.D + ch0), g.D, warp, n, left, lane);
+            fill<F, MODE, S>(slot, (const F *)g.rg + (b * g.rg_batch + t0 * g.rg_token + ch0), (int)g.rg_token, warp, n, left, lane);
+            fill<F, MODE, S>(slot + SLOT, (const F *)g.ig + (b * g.ig_batch + t0 * g.ig_token + ch0), (int)g.ig_token, warp, n, left, lane);
+            fill<F, MODE, S>(slot + 2 * SLOT, (const F *)g.x + (b * g.x_batch + t0 * g.x_token + ch0), (int)g.x_token, warp, n, left, lane);
+            if (g.gy != nullptr) fill<F, MODE, S>(slot + 3 * SLOT, (const F *)g.gy + (((size_t)b * g.T + t0) * g.D + ch0), g.D, warp, n, left, lane);
             else fill<F, MODE, S>(slot + 3 * SLOT, (const F *)g.x, 0, warp, 0, left, lane);         // (no incoming gradient: zeros)
-            if (Z) fill<F, MODE, S>(slot + 4 * SLOT, (const F *)g.z + (b * g.z_batch + at * g.z_token + ch0), (int)g.z_token, warp, n, left, lane);
+            if (Z) fill<F, MODE, S>(slot + 4 * SLOT, (const F *)g.z + (b * g.z_batch + t0 * g.z_token + ch0), (int)g.z_token, warp, n, left, lane);
         }
     };
     if constexpr (MODE == TILES) {
         init_tiles<ST>(ex);
         if (threadIdx.x == 0) {
-            for (int p = 0; p < min(ST, g.nsteps); p++) start(p);
+            for (int p = 0; p < min(ST, nsteps); p++) start(p);
         }
     } else {
 #pragma unroll
         for (int p = 0; p < ST - 1; p++) {
-            if (p < g.nsteps) start(p);
+            if (p < nsteps) start(p);
             cp_commit();
         }
     }
-    for (int k = 0; k < g.nsteps; k++) {
-        const long long t0 = ((long long)(g.nsteps - 1 - k) * g.cl + rank) * BT;
+    for (int k = 0; k < nsteps; k++) {
+        const long long t0 = begin + (long long)(nsteps - 1 - k) * BT;
         f2 h = make_float2(0.f, 0.f);                               // before the block
-        if (t0 < g.T) {
+        {
             const float *c = g.ckpt + ((size_t)b * g.nkept + t0 / CKPT) * g.D + ch;
             if (ch < g.D) h.x = c[0];
             if (ch + 1 < g.D) h.y = c[1];
@@ -491,7 +487,7 @@ __global__ void __launch_bounds__(256, 2) k_rec_bwd(const __grid_constant__ RecA
             await_tiles<ST>(ex, g, k);
         } else {
             __syncwarp();
-            if (k + ST - 1 < g.nsteps) start(k + ST - 1);
+            if (k + ST - 1 < nsteps) start(k + ST - 1);
             cp_commit();
             cp_wait<ST - 1>();
             __syncwarp();
@@ -539,45 +535,21 @@ __global__ void __launch_bounds__(256, 2) k_rec_bwd(const __grid_constant__ RecA
         ex.segE[side][warp][lane] = El;
         if (MODE == TILES && lane == 0) sm100::tma_store_wait_read();
         __syncthreads();
-        if (MODE == TILES && threadIdx.x == 0 && k > 0 && k + ST - 1 < g.nsteps) start(k + ST - 1);
+        if (MODE == TILES && threadIdx.x == 0 && k > 0 && k + ST - 1 < nsteps) start(k + ST - 1);
         f2 Es = E;                                                  // behind this warp's segment
-        if (g.cl == 1) {
 #pragma unroll
-            for (int w = NW - 1; w > 0; w--)
-                if (w > warp) {
-                    const float4 q = ex.seg[side][w][lane];
-                    Es = fma2(make_float2(q.x, q.y), Es, ex.segE[side][w][lane]);
-                }
-            E = fma2(P, Es, El);
-#pragma unroll
-            for (int w = NW - 2; w >= 0; w--)
-                if (w < warp) {
-                    const float4 q = ex.seg[side][w][lane];
-                    E = fma2(make_float2(q.x, q.y), E, ex.segE[side][w][lane]);
-                }
-        } else {
-            f2 Pc = both(1.f), Ec = both(0.f), Pw = both(1.f), Ew = both(0.f);
-#pragma unroll
-            for (int w = NW - 1; w >= 0; w--) {
+        for (int w = NW - 1; w > 0; w--)
+            if (w > warp) {
                 const float4 q = ex.seg[side][w][lane];
-                if (w == warp) { Pw = Pc; Ew = Ec; }
-                Ec = fma2(make_float2(q.x, q.y), Ec, ex.segE[side][w][lane]);
-                Pc = mul2(Pc, make_float2(q.x, q.y));
+                Es = fma2(make_float2(q.x, q.y), Es, ex.segE[side][w][lane]);
             }
-            cg::cluster_group cl = cg::this_cluster();
-            if (warp < g.cl) {
-                ExchangeBack *to = cl.map_shared_rank(&ex, warp);
-                to->cta[side][rank][lane] = make_float4(Pc.x, Pc.y, Ec.x, Ec.y);
+        E = fma2(P, Es, El);
+#pragma unroll
+        for (int w = NW - 2; w >= 0; w--)
+            if (w < warp) {
+                const float4 q = ex.seg[side][w][lane];
+                E = fma2(make_float2(q.x, q.y), E, ex.segE[side][w][lane]);
             }
-            cl.sync();
-            f2 Er = E;
-            for (int q = g.cl - 1; q >= 0; q--) {
-                const float4 c = ex.cta[side][q][lane];
-                if (q == rank) Er = E;
-                E = fma2(make_float2(c.x, c.y), E, make_float2(c.z, c.w));
-            }
-            Es = fma2(Pw, Er, Ew);
-        }
 #pragma unroll
         for (int w = 0; w < NW - 1; w++)
             if (w < warp) {
@@ -627,9 +599,8 @@ __global__ void __launch_bounds__(256, 2) k_rec_bwd(const __grid_constant__ RecA
         }
     }
     if (MODE == TILES && lane == 0) sm100::tma_store_wait_all();
-    if (MODE == TILES) drain_tiles<ST>(ex, g);
-    if (g.cl > 1) cg::this_cluster().sync();
-    if (g.gs_in != nullptr && warp == 0 && rank == 0) {
+    if (MODE == TILES) drain_tiles<ST>(ex, g, nsteps);
+    if (g.gs_in != nullptr && warp == 0 && span == 0) {
         if (ch < g.D) g.gs_in[(size_t)b * g.D + ch] = E.x;
         if (ch + 1 < g.D) g.gs_in[(size_t)b * g.D + ch + 1] = E.y;
     }
@@ -639,10 +610,135 @@ __global__ void __launch_bounds__(256, 2) k_rec_bwd(const __grid_constant__ RecA
         if (warp == 0) {
 #pragma unroll
             for (int w = 1; w < NW; w++) total = add2(total, ex.sum[w][lane]);
-            float *p = g.part + ((size_t)b * g.cl + rank) * g.D + ch;
+            float *p = g.part + ((size_t)b * g.nspan + span) * g.D + ch;
             if (ch < g.D) p[0] = total.x * (LN2_ * k0.ratio);
             if (ch + 1 < g.D) p[1] = total.y * (LN2_ * k1.ratio);
         }
+    }
+}
+
+// What a span does to the state, or (BACK) to E: its warps take an eighth of its tokens each, with a ring each, and meet at its end.
+template <typename F, bool Z, int MODE, bool BACK>
+__global__ void __launch_bounds__(256, 2) k_rec_spans(const __grid_constant__ RecArgs g) {
+    pdl_wait();
+    pdl_trigger();
+    constexpr int S = Geo<F, BACK>::S, NT = BACK ? 2 + Z : 3, ST = 4, SLOT = S * CH;
+    extern __shared__ __align__(128) unsigned char smem[];
+    __shared__ float4 seg[NW][32];
+    __shared__ uint64_t bars[NW][ST];
+    __shared__ int abort;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    // (the last span forward and the first one backward are not needed)
+    const int n1 = g.nspan - 1, span = blockIdx.x % n1 + BACK, chain = blockIdx.x / n1, b = chain / g.slabs, ch0 = (chain - b * g.slabs) * CH, ch = ch0 + 2 * lane;
+    F *ring = reinterpret_cast<F *>(smem) + warp * ST * NT * SLOT;
+    const Rate k0 = rate_of(ch < g.D ? g.decay[ch] : 0.f, g.c), k1 = rate_of(ch + 1 < g.D ? g.decay[ch + 1] : 0.f, g.c);
+    const f2 rate = make_float2(k0.rate2, k1.rate2), x2 = make_float2(k0.x2, k1.x2);
+    // this warp's tokens
+    const long long begin = (long long)span * g.span, end = min((long long)g.T, begin + g.span), part = g.span / NW;
+    const long long from = min(end, begin + warp * part), to = min(end, from + part);
+    const int nsteps = (int)((to - from + S - 1) / S);
+    auto at_step = [&](int k) { return from + (long long)(BACK ? nsteps - 1 - k : k) * S; };
+    auto start = [&](int k) {
+        const long long t0 = at_step(k);
+        F *slot = ring + (k % ST) * NT * SLOT;
+        if constexpr (MODE == TILES) {
+            if (lane == 0) {
+                uint64_t *bar = &bars[warp][k % ST];
+                sm100::mbar_expect_tx(bar, NT * SLOT * sizeof(F));
+                sm100::tma_load_3d(slot, g.in_spans, bar, ch0, (int)t0, b);
+                sm100::tma_load_3d(slot + SLOT, g.in_spans + (BACK ? 3 : 1), bar, ch0, (int)t0, b);
+                if (!BACK || Z) sm100::tma_load_3d(slot + 2 * SLOT, g.in_spans + (BACK ? 4 : 2), bar, ch0, (int)t0, b);
+            }
+        } else {
+            const int n = (int)min((long long)S, to - t0), left = g.D - ch0;
+            fill<F, MODE, S>(slot, (const F *)g.rg + (b * g.rg_batch + t0 * g.rg_token + ch0), (int)g.rg_token, 0, n, left, lane);
+            if (!BACK) {
+                fill<F, MODE, S>(slot + SLOT, (const F *)g.ig + (b * g.ig_batch + t0 * g.ig_token + ch0), (int)g.ig_token, 0, n, left, lane);
+                fill<F, MODE, S>(slot + 2 * SLOT, (const F *)g.x + (b * g.x_batch + t0 * g.x_token + ch0), (int)g.x_token, 0, n, left, lane);
+            } else {
+                if (g.gy != nullptr) fill<F, MODE, S>(slot + SLOT, (const F *)g.gy + (((size_t)b * g.T + t0) * g.D + ch0), g.D, 0, n, left, lane);
+                else fill<F, MODE, S>(slot + SLOT, (const F *)g.x, 0, 0, 0, left, lane);
+                if (Z) fill<F, MODE, S>(slot + 2 * SLOT, (const F *)g.z + (b * g.z_batch + t0 * g.z_token + ch0), (int)g.z_token, 0, n, left, lane);
+            }
+        }
+    };
+    if constexpr (MODE == TILES) {
+        if (lane == 0) {
+            for (int i = 0; i < ST; i++) sm100::mbar_init(&bars[warp][i], 1);
+            sm100::fence_mbar_init();
+        }
+        if (threadIdx.x == 0) abort = 0;
+        __syncthreads();
+    }
+#pragma unroll
+    for (int p = 0; p < ST - 1; p++) {
+        if (p < nsteps) start(p);
+        if (MODE != TILES) cp_commit();
+    }
+    f2 P = both(1.f), h = both(0.f);
+    for (int k = 0; k < nsteps; k++) {
+        __syncwarp();
+        if (k + ST - 1 < nsteps) start(k + ST - 1);
+        if constexpr (MODE == TILES) {
+            if (!sm100::mbar_wait_or_abort(&bars[warp][k % ST], (k / ST) & 1, &abort, g.limit)) {
+                *(volatile int *)&abort = 1;
+                if (g.status != nullptr) atomicOr(g.status, WKV_RECURRENCE_TIMEOUT);
+            }
+        } else {
+            cp_commit();
+            cp_wait<ST - 1>();
+            __syncwarp();
+        }
+        F *slot = ring + (k % ST) * NT * SLOT;
+        const int n = (int)min((long long)S, to - at_step(k));
+        if (n < S) close_gates<F, S>(slot, n, lane);
+        f2 a[S], v[S];
+        auto gates = [&](auto fast) {
+            f2 range = both(0.f);
+#pragma unroll
+            for (int s = 0; s < S; s++) {
+                f2 r, in, sz;
+                if (!BACK) {
+                    sigmoids<false, decltype(fast)::value>(pair_at(slot, s, lane), pair_at(slot + SLOT, s, lane), both(0.f), r, in, sz, range);
+                    a[s] = decays(r, rate);
+                    const f2 q = one_minus_square(a[s], mul2(r, x2));
+                    v[s] = mul2(mul2(make_float2(sqrtf(q.x), sqrtf(q.y)), in), pair_at(slot + 2 * SLOT, s, lane));
+                } else {
+                    const f2 z = Z ? pair_at(slot + 2 * SLOT, s, lane) : both(0.f);
+                    sigmoids<false, decltype(fast)::value>(pair_at(slot, s, lane), z, both(0.f), r, sz, in, range);
+                    a[s] = decays(r, rate);
+                    v[s] = pair_at(slot + SLOT, s, lane);
+                    if (Z) v[s] = mul2(v[s], mul2(z, sz));
+                }
+            }
+            return in_range(range);
+        };
+        if (!gates(std::true_type{})) gates(std::false_type{});
+#pragma unroll
+        for (int i = 0; i < S; i++) {
+            const int s = BACK ? S - 1 - i : i;
+            h = BACK ? mul2(a[s], add2(v[s], h)) : fma2(a[s], h, v[s]);
+            P = mul2(P, a[s]);
+        }
+    }
+    if constexpr (MODE == TILES) {
+        if (lane == 0 && *(volatile int *)&abort != 0)
+            for (int k = max(0, nsteps - ST); k < nsteps; k++) sm100::mbar_wait(&bars[warp][k % ST], (k / ST) & 1, g.limit);
+    }
+    seg[warp][lane] = make_float4(P.x, P.y, h.x, h.y);
+    __syncthreads();
+    if (warp == 0) {
+        P = both(1.f);
+        h = both(0.f);
+#pragma unroll
+        for (int i = 0; i < NW; i++) {
+            const float4 q = seg[BACK ? NW - 1 - i : i][lane];
+            h = fma2(make_float2(q.x, q.y), h, make_float2(q.z, q.w));
+            P = mul2(P, make_float2(q.x, q.y));
+        }
+        float2 *o = g.spans + ((size_t)b * g.nspan + span) * g.D + ch;
+        if (ch < g.D) o[0] = make_float2(P.x, h.x);
+        if (ch + 1 < g.D) o[1] = make_float2(P.y, h.y);
     }
 }
 
@@ -698,16 +794,36 @@ template <typename F> bool lies_in(const wkv_gated_recurrence_args_t *a, size_t 
     return ok && (bytes < 16 || a->D % e == 0);
 }
 
-// CTAs of a cluster: as many as there are places for (two CTAs an SM) and blocks of tokens to take
-int cluster_size(const wkv_gated_recurrence_args_t *a, int bt) {
-    const long long chains = (long long)a->B * ((a->D + CH - 1) / CH), places = 2ll * device_sm_count(), blocks = ((long long)a->T + bt - 1) / bt;
-    int cl = 1;
-    while (cl < MAX_CL && chains * cl * 2 <= places && cl * 2 <= blocks) cl *= 2;
-    return cl;
-}
 int block_tokens(const wkv_gated_recurrence_args_t *a, bool back) {
     if (back) return CKPT;
     return a->dtype == WKV_F32 ? Geo<float, false>::BT : Geo<__half, false>::BT;
+}
+
+// Spans of a row and their length.  A full pass takes a CTA 40 ns a token where two share an SM, 27 where it is alone (4 x 4096 x 4096
+// forward 165 us, 1 x 8192 x 5120 in one span 215), the first pass over spans about half of that.
+struct Spans {
+    int n, tokens;
+};
+Spans spans_for(const wkv_gated_recurrence_args_t *a, bool back) {
+    const long long unit = block_tokens(a, back), chains = (long long)a->B * ((a->D + CH - 1) / CH), sms = device_sm_count();
+    const long long blocks = (a->T + unit - 1) / unit;
+    auto time = [&](long long ctas, long long tokens) {                  // CTAs of so many tokens, two at most on an SM
+        const long long full = ctas / (2 * sms), rest = ctas - full * 2 * sms;
+        return (double)tokens * (full * 40.0 + (rest == 0 ? 0.0 : rest <= sms ? 27.0 : 40.0));
+    };
+    Spans best = {1, (int)std::max(unit, blocks * unit)};
+    double t_best = time(chains, a->T);
+    for (long long n = 2; n <= MAX_SPANS && n * 2 <= blocks && (n - 1) * chains <= 8 * sms; n++) {
+        const long long len = (blocks + n - 1) / n * unit, used = (a->T + len - 1) / len;
+        if (used != n) continue;
+        const double t = time(chains * n, len) + 0.5 * time(chains * (n - 1), len) + 4000.0 + 100.0 * n;
+        if (t < t_best) { best = {(int)n, (int)len}; t_best = t; }
+    }
+    return best;
+}
+size_t spans_bytes(const wkv_gated_recurrence_args_t *a, bool back) {
+    const int n = spans_for(a, back).n;
+    return n > 1 ? align256((size_t)a->B * n * a->D * sizeof(float2)) : 0;
 }
 
 bool strides_ok(const wkv_gated_recurrence_args_t *a) {
@@ -717,50 +833,44 @@ bool strides_ok(const wkv_gated_recurrence_args_t *a) {
 }
 bool sizes_ok(const wkv_gated_recurrence_args_t *a) {
     return a->B >= 0 && a->T >= 0 && a->D >= 0 && a->D <= (1 << 22) && a->T <= 2147483647 - 4096 && known_dtype(a->dtype) &&
-           (long long)a->B * ((a->D + CH - 1) / CH) <= 2147483647 / MAX_CL && (long long)a->B * a->D <= 1ll << 34 && a->c > 0.f &&
+           (long long)a->B * ((a->D + CH - 1) / CH) <= 2147483647 / MAX_SPANS && (long long)a->B * a->D <= 1ll << 34 && a->c > 0.f &&
            strides_ok(a);
 }
 RecArgs args_of(const wkv_gated_recurrence_args_t *a, bool back) {
     RecArgs g = {};
-    const int bt = block_tokens(a, back);
-    g.T = a->T; g.D = a->D; g.slabs = (a->D + CH - 1) / CH; g.cl = cluster_size(a, bt);
+    const Spans sp = spans_for(a, back);
+    g.T = a->T; g.D = a->D; g.slabs = (a->D + CH - 1) / CH; g.nspan = sp.n; g.span = sp.tokens;
     g.nkept = (int)(((long long)a->T + CKPT - 1) / CKPT);
-    g.nsteps = (int)(((long long)a->T + (long long)bt * g.cl - 1) / ((long long)bt * g.cl));
     g.c = a->c;
     g.x = a->x; g.ig = a->input_gate; g.rg = a->decay_gate; g.z = a->z;
     g.x_batch = a->x_batch; g.x_token = a->x_token; g.ig_batch = a->i_batch; g.ig_token = a->i_token;
     g.rg_batch = a->r_batch; g.rg_token = a->r_token; g.z_batch = a->z_batch; g.z_token = a->z_token;
     g.decay = a->decay; g.state_in = a->state_in; g.y = a->y; g.state_out = a->state_out; g.ckpt = (float *)a->ckpt;
     g.gy = a->gy; g.gs_out = a->gstate_out; g.gx = a->gx; g.gig = a->ginput_gate; g.grg = a->gdecay_gate; g.gz = a->gz;
-    g.gs_in = a->gstate_in; g.part = (float *)a->workspace;
+    g.gs_in = a->gstate_in;
+    g.spans = (float2 *)a->workspace;
+    g.part = (float *)((char *)a->workspace + (back ? spans_bytes(a, true) : 0));
     g.status = a->status; g.limit = 4000000u;
     return g;
 }
 size_t ckpt_need(const wkv_gated_recurrence_args_t *a) { return (size_t)a->B * (((size_t)a->T + CKPT - 1) / CKPT) * a->D * 4; }
 
 template <class K>
-int launch_rec(K kern, const RecArgs &g, int B, int smem, unsigned char (&done)[64], cudaStream_t s) {
+int launch_rec(K kern, const RecArgs &g, long long ctas, int smem, unsigned char (&done)[64], cudaStream_t s) {
     if (!set_max_smem_once(kern, smem, done)) return WKV_ERR_LAUNCH;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(B * g.slabs * g.cl));
-    cfg.blockDim = dim3(256);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = s;
-    cudaLaunchAttribute attr[2];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    attr[1].id = cudaLaunchAttributeClusterDimension;
-    attr[1].val.clusterDim.x = g.cl; attr[1].val.clusterDim.y = 1; attr[1].val.clusterDim.z = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = g.cl > 1 ? 2 : 1;
-    launch_count.fetch_add(1, std::memory_order_relaxed);
-    return cudaLaunchKernelEx(&cfg, kern, g) == cudaSuccess ? WKV_OK : WKV_ERR_LAUNCH;
+    return launch_chained(kern, dim3((unsigned)ctas), dim3(256), smem, s, g);
 }
 template <typename F, bool Z, int MODE, bool BACK>
 int launch_as(const RecArgs &g, int B, cudaStream_t s) {
-    static unsigned char done[64];
-    if constexpr (BACK) return launch_rec(k_rec_bwd<F, Z, MODE>, g, B, Geo<F, true>::ring(Z) + (int)sizeof(ExchangeBack), done, s);
-    else return launch_rec(k_rec_fwd<F, Z, MODE>, g, B, Geo<F, false>::ring(Z) + (int)sizeof(Exchange), done, s);
+    static unsigned char done[2][64];
+    const long long chains = (long long)B * g.slabs;
+    if (g.nspan > 1) {
+        const int smem = NW * 4 * (BACK ? 2 + Z : 3) * Geo<F, BACK>::S * CH * (int)sizeof(F);
+        const int rc = launch_rec(k_rec_spans<F, Z, MODE, BACK>, g, chains * (g.nspan - 1), smem, done[1], s);
+        if (rc != WKV_OK) return rc;
+    }
+    if constexpr (BACK) return launch_rec(k_rec_bwd<F, Z, MODE>, g, chains * g.nspan, Geo<F, true>::ring(Z) + (int)sizeof(ExchangeBack), done[0], s);
+    else return launch_rec(k_rec_fwd<F, Z, MODE>, g, chains * g.nspan, Geo<F, false>::ring(Z) + (int)sizeof(Exchange), done[0], s);
 }
 // the tiles' maps; false: TMA cannot read or write these rows
 template <typename F, bool BACK>
@@ -775,6 +885,8 @@ bool make_maps(const wkv_gated_recurrence_args_t *a, RecArgs &g) {
         // (a dimension of one element may have any stride)
         const long long token = a->T > 1 ? in[i].token : yt, batch = a->B > 1 ? in[i].batch : token * a->T;
         if (in[i].p == nullptr || !make_tile_map(&g.in[i], in[i].p, sizeof(F), a->B, a->T, a->D, batch, token, CH, G::BT)) return false;
+        const bool first = BACK ? i == 0 || i >= 3 : i < 3;               // what the pass over spans reads
+        if (g.nspan > 1 && first && !make_tile_map(&g.in_spans[i], in[i].p, sizeof(F), a->B, a->T, a->D, batch, token, CH, G::S)) return false;
     }
     void *out[4] = {BACK ? a->gx : a->y, a->ginput_gate, a->gdecay_gate, a->gz};
     for (int i = 0; i < (BACK ? 3 + z : 1); i++)
@@ -807,6 +919,10 @@ using namespace wkv;
 
 extern "C" size_t wkv_gated_recurrence_ckpt_bytes(const wkv_gated_recurrence_args_t *a) { return a != nullptr && sizes_ok(a) ? ckpt_need(a) : 0; }
 
+extern "C" size_t wkv_gated_recurrence_forward_workspace(const wkv_gated_recurrence_args_t *a) {
+    return a != nullptr && sizes_ok(a) && a->T > 1 ? spans_bytes(a, false) : 0;
+}
+
 extern "C" int wkv_gated_recurrence_forward(const wkv_gated_recurrence_args_t *a, void *stream) {
     if (a == nullptr) return WKV_ERR_NULL;
     if (!known_dtype(a->dtype)) return WKV_ERR_DTYPE;
@@ -826,11 +942,15 @@ extern "C" int wkv_gated_recurrence_forward(const wkv_gated_recurrence_args_t *a
         });
     }
     if (a->ckpt != nullptr && a->ckpt_bytes < ckpt_need(a)) return WKV_ERR_WORKSPACE;
+    const size_t need = wkv_gated_recurrence_forward_workspace(a);
+    if (need > 0 && (a->workspace == nullptr || a->workspace_bytes < need)) return WKV_ERR_WORKSPACE;
+    if (!aligned16(a->workspace)) return WKV_ERR_ALIGN;
     return launch_by<false>(a, g, s);
 }
 
 extern "C" size_t wkv_gated_recurrence_backward_workspace(const wkv_gated_recurrence_args_t *a) {
-    return a != nullptr && sizes_ok(a) && a->gdecay != nullptr ? (size_t)a->B * cluster_size(a, CKPT) * a->D * 4 : 0;
+    if (a == nullptr || !sizes_ok(a)) return 0;
+    return spans_bytes(a, true) + (a->gdecay != nullptr ? (size_t)a->B * spans_for(a, true).n * a->D * 4 : 0);
 }
 
 extern "C" int wkv_gated_recurrence_backward(const wkv_gated_recurrence_args_t *a, void *stream) {
@@ -844,10 +964,12 @@ extern "C" int wkv_gated_recurrence_backward(const wkv_gated_recurrence_args_t *
     if ((long long)a->B * a->D == 0) return a->gdecay != nullptr && a->D > 0 ? fold_params(nullptr, 0, a->D, out, s) : WKV_OK;
     if (a->decay == nullptr || (a->T > 0 && (a->x == nullptr || a->input_gate == nullptr || a->decay_gate == nullptr))) return WKV_ERR_NULL;
     if (a->T > 0 && (a->ckpt == nullptr || a->ckpt_bytes < ckpt_need(a))) return WKV_ERR_WORKSPACE;
-    if (a->gdecay != nullptr && (a->workspace == nullptr || a->workspace_bytes < wkv_gated_recurrence_backward_workspace(a))) return WKV_ERR_WORKSPACE;
+    const size_t need = wkv_gated_recurrence_backward_workspace(a);
+    if (need > 0 && (a->workspace == nullptr || a->workspace_bytes < need)) return WKV_ERR_WORKSPACE;
+    if (!aligned16(a->workspace)) return WKV_ERR_ALIGN;
     RecArgs g = args_of(a, true);
     if (a->gdecay == nullptr) g.part = nullptr;
     const int rc = launch_by<true>(a, g, s);
     if (rc != WKV_OK || a->gdecay == nullptr) return rc;
-    return fold_params(g.part, a->B * g.cl, a->D, out, s);
+    return fold_params(g.part, a->B * g.nspan, a->D, out, s);
 }

@@ -487,6 +487,9 @@ std::tuple<Tensor, Tensor> gated_recurrence(const Tensor &x, const Tensor &ig, c
             ckpt = bytes_like(x, r.a.ckpt_bytes);
             r.a.ckpt = ptr(ckpt);
         }
+        r.a.workspace_bytes = wkv_gated_recurrence_forward_workspace(&r.a);
+        Tensor ws = bytes_like(x, r.a.workspace_bytes);
+        r.a.workspace = ptr(ws);
         check(wkv_gated_recurrence_forward(&r.a, stream_of(x)), "wkv_gated_recurrence_forward");
         if (save) node->keep({r.x.t, r.ig.t, r.rg.t, r.decay, r.z.t, ckpt});
     }

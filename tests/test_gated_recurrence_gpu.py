@@ -139,7 +139,7 @@ def test_channels(D, dtype):
 
 @pytest.mark.parametrize("B,T,D", [(1, 1100, 64), (1, 513, 40), (2, 700, 1000), (1, 300, 5121), (9, 140, 2048), (40, 65, 520), (1, 4099, 9)])
 @pytest.mark.parametrize("dtype", [BF, F32])
-def test_rows_cut_among_the_ctas_of_a_cluster(B, T, D, dtype):
+def test_rows_cut_into_spans(B, T, D, dtype):
     check(c := case(B, B, T, D, dtype), train(c))
 
 
