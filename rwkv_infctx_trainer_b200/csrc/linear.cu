@@ -27,7 +27,7 @@ constexpr unsigned WAIT_LIMIT = 4000000u;
 inline long long up8(long long n) { return (n + 7) & ~7ll; }
 
 // ------------------------------------------------------------------------------------------ few rows
-// A CTA has 16 rows of the matrix (of a pair: 8 of each), its 8 warps every eighth run of 64 contraction steps; the warps' sums meet
+// A CTA has 16 rows of the matrix (of a pair: 8 of each), its 4 or 8 warps runs of 256 contraction steps in turn; the warps' sums meet
 // in shared memory in a fixed order.  mma.sync with the matrix as the 16-row operand and the rows of x as the 8 columns: the
 // contraction steps may be numbered in any order that both operands share, so that a lane's 16-byte piece (8 steps of one row) is
 // its part of two instructions as it is, without a turn through shared memory.  (The tensor core's rate does not matter here.)
@@ -41,7 +41,7 @@ __device__ __forceinline__ void mma16(float (&d)[4], uint32_t a0, uint32_t a1, u
                      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-constexpr int FEW_ROWS = 16, FEW_WARPS = 8;
+constexpr int FEW_ROWS = 16;
 
 struct FewArgs {
     int M, K, N;                       // M: rows of x
@@ -51,11 +51,11 @@ struct FewArgs {
 };
 
 // VEC: every row of x and of the matrices is made of whole 16-byte pieces
-template <typename F, int TOKENS, bool PAIR, bool VEC>
+template <typename F, int TOKENS, bool PAIR, bool VEC, int FEW_WARPS>
 __global__ void __launch_bounds__(32 * FEW_WARPS) k_few_rows(const FewArgs g) {
     pdl_wait();
     pdl_trigger();
-    constexpr int NT = TOKENS / 8, OUT = PAIR ? 8 : 16, UNROLL = VEC ? 2 : 1;
+    constexpr int NT = TOKENS / 8, OUT = PAIR ? 8 : 16, UNROLL = 4;
     __shared__ float part[FEW_WARPS][16][TOKENS + 1];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, q = lane >> 2, c = lane & 3;
     const int row0 = blockIdx.x * OUT;
@@ -82,7 +82,7 @@ __global__ void __launch_bounds__(32 * FEW_WARPS) k_few_rows(const FewArgs g) {
         for (int s = 0; s < UNROLL; s++) {
 #pragma unroll
             for (int h = 0; h < 2; h++) {
-                const int k = k0 + s * 64 * FEW_WARPS + h * 32 + c * 8, n = whole ? 8 : min(8, g.K - k);
+                const int k = k0 + s * 64 + h * 32 + c * 8, n = whole ? 8 : min(8, g.K - k);
                 if (whole || n > 0) {
                     a[s][0][h].load(w0 + k, VEC, n);
                     a[s][1][h].load(w1 + k, VEC, n);
@@ -107,8 +107,8 @@ __global__ void __launch_bounds__(32 * FEW_WARPS) k_few_rows(const FewArgs g) {
                     mma16<F>(d[j], a[s][0][h].w[2], a[s][1][h].w[2], a[s][0][h].w[3], a[s][1][h].w[3], b[s][j][h].w[2], b[s][j][h].w[3]);
                 }
     };
-    int k0 = warp * 64;
-    for (; k0 + (UNROLL - 1) * 64 * FEW_WARPS + 64 <= g.K; k0 += UNROLL * 64 * FEW_WARPS) run(k0, std::true_type{});
+    int k0 = warp * 64 * UNROLL;
+    for (; k0 + 64 * UNROLL <= g.K; k0 += UNROLL * 64 * FEW_WARPS) run(k0, std::true_type{});
     if (k0 < g.K) run(k0, std::false_type{});
 #pragma unroll
     for (int j = 0; j < NT; j++) {
@@ -119,8 +119,8 @@ __global__ void __launch_bounds__(32 * FEW_WARPS) k_few_rows(const FewArgs g) {
     }
     __syncthreads();
     // neighbouring threads take neighbouring columns of y
-    if (threadIdx.x < OUT * TOKENS) {
-        const int o = threadIdx.x % OUT, t = threadIdx.x / OUT, col = row0 + o;
+    for (int i = threadIdx.x; i < OUT * TOKENS; i += 32 * FEW_WARPS) {
+        const int o = i % OUT, t = i / OUT, col = row0 + o;
         if (t < g.M && col < g.N) {
             float f = 0.f, u = 0.f;
 #pragma unroll
@@ -128,7 +128,7 @@ __global__ void __launch_bounds__(32 * FEW_WARPS) k_few_rows(const FewArgs g) {
                 f += part[w][o][t];
                 if (PAIR) u += part[w][o + 8][t];
             }
-            finish1<F, PAIR ? EPI_GATED : EPI_LINEAR>(g.e, 0, t, col, f, u, !PAIR && g.e.bias != nullptr ? param_at(g.e.bias, g.e.bias_dtype, col) : 0.f);
+            finish1<F, PAIR ? EPI_GATED : EPI_LINEAR>(g.e, 0, t, col, f, u, PAIR ? 0.f : bias_at(g.e, col));
         }
     }
 }
@@ -150,7 +150,7 @@ __global__ void __launch_bounds__(256) k_fold_split(const Epi e, long long M, in
         f[0] += a.x; f[1] += a.y; f[2] += a.z; f[3] += a.w; f[4] += b.x; f[5] += b.y; f[6] += b.z; f[7] += b.w;
     }
 #pragma unroll
-    for (int k = 0; k < 8; k++) bias[k] = e.bias != nullptr && k < n ? param_at(e.bias, e.bias_dtype, col + k) : 0.f;
+    for (int k = 0; k < 8; k++) bias[k] = k < n ? bias_at(e, col + k) : 0.f;
     finish8<F, EPI_LINEAR>(e, 0, row, col, n, f, f, bias);
 }
 
@@ -442,15 +442,20 @@ int forward(const wkv_linear_args_t *a, Scratch ws, size_t *need, cudaStream_t s
         for (int i = 0; i < 2; i++) { g.w[i] = w[i].p; g.w_row[i] = w[i].pitch; }
         g.e = e;
         const bool vec = a->K % 8 == 0 && tma_ready(x.p, x.pitch) && tma_ready(w[0].p, w[0].pitch) && tma_ready(w[1].p, w[1].pitch);
-        const auto go = [&](auto kern) {
-            return launch_chained(kern, dim3((unsigned)((a->N + (a->pair ? 7 : 15)) / (a->pair ? 8 : 16))), dim3(32 * FEW_WARPS), 0, s, g);
+        const long long ctas = (a->N + (a->pair ? 7 : 15)) / (a->pair ? 8 : 16);
+        const auto go = [&](auto pair, auto tokens) {
+            constexpr bool PAIR = decltype(pair)::value;
+            constexpr int TOKENS = decltype(tokens)::value;
+            auto with = [&](auto kern, int warps) { return launch_chained(kern, dim3((unsigned)ctas), dim3(32 * warps), 0, s, g); };
+            // (8 warps have more of the matrix on its way where CTAs are few: 8 rows of 4096 -> 4096 8.0 us, with 4 warps 10.3; 4 start and end
+            // sooner where they are many: 1 row of 2560 -> a pair of 8960 17.1 us, with 8 warps 20.4.  The sums' order depends on it: not on alignment.)
+            if (ctas <= 4 * device_sm_count()) return vec ? with(k_few_rows<F, TOKENS, PAIR, true, 8>, 8) : with(k_few_rows<F, TOKENS, PAIR, false, 8>, 8);
+            return vec ? with(k_few_rows<F, TOKENS, PAIR, true, 4>, 4) : with(k_few_rows<F, TOKENS, PAIR, false, 4>, 4);
         };
-        if (a->rows <= 8) {
-            if (a->pair) return vec ? go(k_few_rows<F, 8, true, true>) : go(k_few_rows<F, 8, true, false>);
-            return vec ? go(k_few_rows<F, 8, false, true>) : go(k_few_rows<F, 8, false, false>);
-        }
-        if (a->pair) return vec ? go(k_few_rows<F, 16, true, true>) : go(k_few_rows<F, 16, true, false>);
-        return vec ? go(k_few_rows<F, 16, false, true>) : go(k_few_rows<F, 16, false, false>);
+        using N8 = std::integral_constant<int, 8>;
+        using N16 = std::integral_constant<int, 16>;
+        if (a->rows <= 8) return a->pair ? go(std::true_type{}, N8{}) : go(std::false_type{}, N8{});
+        return a->pair ? go(std::true_type{}, N16{}) : go(std::false_type{}, N16{});
     }
     int rc = ready<F>(x, ws, s);
     for (int i = 0; i <= a->pair && rc == WKV_OK; i++) rc = ready<F>(w[i], ws, s);

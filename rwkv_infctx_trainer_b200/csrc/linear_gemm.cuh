@@ -77,6 +77,15 @@ struct Epi {
     long long part_row;
 };
 
+// Element i of the bias, 0 without one.  Plain loads: those of the read-only path (__ldg) may be moved by the compiler, and were, out of
+// a loop and in front of the check.
+__device__ __forceinline__ float bias_at(const Epi &e, int i) {
+    if (e.bias == nullptr) return 0.f;
+    if (e.bias_dtype == WKV_F32) return Elem<float>::ld((const float *)e.bias + i);
+    if (e.bias_dtype == WKV_BF16) return Elem<__nv_bfloat16>::ld((const __nv_bfloat16 *)e.bias + i);
+    return Elem<__half>::ld((const __half *)e.bias + i);
+}
+
 struct GemmArgs {
     CUtensorMap a[2], b[2];
     int M, N;                         // of one source
@@ -470,7 +479,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_gemm(const __grid_constant__ Gem
                     float bias[8];
                     if (EPI == EPI_LINEAR && e.bias != nullptr) {
 #pragma unroll
-                        for (int k = 0; k < 8; k++) bias[k] = k < n ? param_at(e.bias, e.bias_dtype, col0 + cc + k) : 0.f;
+                        for (int k = 0; k < 8; k++) bias[k] = k < n ? bias_at(e, col0 + cc + k) : 0.f;
                     }
 #pragma unroll
                     for (int k = 0; k < 32 / ROWS; k++) {
@@ -482,7 +491,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_gemm(const __grid_constant__ Gem
                     }
                 } else {
                     const int cc = lane % PASS, col = col0 + cc;
-                    const float bias = EPI == EPI_LINEAR && e.bias != nullptr && col < g.N ? param_at(e.bias, e.bias_dtype, col) : 0.f;
+                    const float bias = EPI == EPI_LINEAR && col < g.N ? bias_at(e, col) : 0.f;
 #pragma unroll 4
                     for (int r = lane / PASS; r < 32; r += 32 / PASS) {
                         const float f = turn[r * 32 + (((cc >> 2) ^ (r & 7)) << 2) + (cc & 3)];
