@@ -128,30 +128,14 @@ __global__ void __launch_bounds__(32 * FEW_WARPS) k_few_rows(const FewArgs g) {
                 f += part[w][o][t];
                 if (PAIR) u += part[w][o + 8][t];
             }
-            finish1<F, PAIR ? EPI_GATED : EPI_LINEAR>(g.e, 0, t, col, f, u, PAIR ? 0.f : bias_at(g.e, col));
+            Finish<F, PAIR ? EPI_GATED : EPI_LINEAR, 1, 1, false> out;
+            const bool ok[1] = {true};
+            float v[1][1] = {{f}};
+            const float w[1][1] = {{u}}, bias[1] = {PAIR ? 0.f : bias_at(g.e, col)};
+            out.ask(g.e, t, 1, col, 1, ok);
+            out.finish(g.e, 0, t, 1, col, 1, ok, v, w, bias);
         }
     }
-}
-
-// ------------------------------------------------------------------------------------------ split contraction
-// the parts' sums in order, then the epilogue: a thread has 8 columns of a row
-template <typename F>
-__global__ void __launch_bounds__(256) k_fold_split(const Epi e, long long M, int N, int splits) {
-    pdl_wait();
-    pdl_trigger();
-    const int pieces = (N + 7) / 8;
-    const long long i = (long long)blockIdx.x * 256 + threadIdx.x, row = i / pieces;
-    if (row >= M) return;
-    const int col = (int)(i - row * pieces) * 8, n = N - col;
-    float f[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, bias[8];
-    for (int s = 0; s < splits; s++) {
-        const float4 *p = reinterpret_cast<const float4 *>(e.part + ((size_t)s * M + row) * e.part_row + col);
-        const float4 a = p[0], b = p[1];
-        f[0] += a.x; f[1] += a.y; f[2] += a.z; f[3] += a.w; f[4] += b.x; f[5] += b.y; f[6] += b.z; f[7] += b.w;
-    }
-#pragma unroll
-    for (int k = 0; k < 8; k++) bias[k] = k < n ? bias_at(e, col + k) : 0.f;
-    finish8<F, EPI_LINEAR>(e, 0, row, col, n, f, f, bias);
 }
 
 // ------------------------------------------------------------------------------------------ gradient of the pre-activation
@@ -292,39 +276,46 @@ struct Scratch {
     }
 };
 
-// The shape of a product and how it is cut.  (us: from the kernel's rates on one B200, the same for every call.)
+// How a product is cut: the tile, and the tiles behind the last full wave whose contraction is cut (Item in linear_gemm.cuh).
 struct Cut {
-    int cg, bn, splits, kb_split;
+    int cg, bn, m_tiles0, m_tiles, n_tiles, main, rest, splits, kb_split;
+    size_t part_bytes() const { return splits > 1 ? (size_t)rest * splits * (128 * cg) * bn * 4 : 0; }
 };
+// The cut that takes least by this estimate (us on one B200, 64 contraction steps a block).  A block's operands come into an SM at about 60
+// bytes a cycle, which is what a tile costs: 32 KB a CTA for 256 x 256 of two (0.27; its products take as long) and for 128 x 128 of one, 24 KB
+// for 256 x 128 of two (0.20) and 128 x 64 of one.  Cut contractions cost their sums' way through L2, and a launch.
 Cut cut_for(long long m, long long n, int sources, int kb, bool pair) {
-    const long long out256 = pair ? 128 : 256;
-    auto tiles = [&](long long bm, long long bn) { return sources * ((m + bm - 1) / bm) * ((n + bn - 1) / bn); };
-    const int sms = device_sm_count(), pairs = sms / 2;
-    auto waves = [](long long t, int places) { return (double)((t + places - 1) / places); };
-    // a stage of 64 steps takes a tile of 256 x 256 of two SMs 0.29 us, one of 128 x 128 of one SM 0.17; start and end 4 us
-    Cut best = {2, 256, 1, kb};
-    double t_best = waves(tiles(256, out256), pairs) * (0.29 * kb + 1.0);
-    const double t1 = waves(tiles(128, out256 / 2), sms) * (0.17 * kb + 1.0);
-    if (t1 < t_best) { best = {1, 128, 1, kb}; t_best = t1; }
-    if (!pair && sources == 1) {
-        const long long t = tiles(128, 128);
-        for (int s = 2; s <= 16 && kb / s >= 4; s++) {
+    struct { int cg, bn; double block; } tiles[4] = {{2, 256, 0.27}, {2, 128, 0.20}, {1, 128, 0.27}, {1, 64, 0.20}};
+    const int sms = device_sm_count();
+    Cut best = {};
+    double t_best = 1e30;
+    for (const auto &t : tiles) {
+        const long long bm = 128 * t.cg, out = pair ? t.bn / 2 : t.bn, m0 = (m + bm - 1) / bm, nt = (n + out - 1) / out, all = sources * m0 * nt;
+        if (all > 1 << 29) continue;
+        const int places = sms / t.cg;
+        const long long waves = all / places, rest = all - waves * places;
+        for (int s = 1; s <= 16 && s <= std::max(1, kb / 2); s++) {
+            if (s > 1 && (rest == 0 || rest * (s - 1) >= places)) break;
             const int len = (kb + s - 1) / s, used = (kb + len - 1) / len;
-            const double ts = waves(t * used, sms) * (0.17 * len + 1.0) + 3.0 + (double)used * m * n * 8e-6 / 4.0;
-            if (ts < t_best) { best = {1, 128, used, len}; t_best = ts; }
+            if (used != s) continue;
+            double us = 4.0 + t.block * 0.4 * t.bn * t.cg / 64 + waves * kb * t.block + (rest ? (double)((rest * s + places - 1) / places) * len * t.block : 0.0);
+            if (s > 1) us += 2.5 + (double)rest * s * bm * t.bn * 8 / 4e6;
+            if (us < t_best) {
+                t_best = us;
+                best = {t.cg, t.bn, (int)m0, (int)(sources * m0), (int)nt, (int)(all - rest), (int)rest, s, len};
+            }
         }
     }
     return best;
 }
-size_t split_bytes(const Cut &c, long long m, long long n) { return c.splits > 1 ? (size_t)c.splits * m * up8(n) * 4 : 0; }
 
 template <typename F, int CG, int BN, bool A_MN, bool B_MN, int EPI>
-int launch_gemm(GemmArgs &g, cudaStream_t s) {
+int launch_gemm(const GemmArgs &g, cudaStream_t s) {
     using T = Tile<CG, BN>;
     static unsigned char done[64];
     const auto kern = k_gemm<F, CG, BN, A_MN, B_MN, EPI>;
     if (!set_max_smem_once(kern, T::SMEM, done)) return WKV_ERR_LAUNCH;
-    const long long items = (long long)g.m_tiles * g.n_tiles * g.splits;
+    const long long items = g.main + (long long)g.rest * g.splits;
     const int places = device_sm_count() / CG, grid = (int)std::min<long long>(items, places) * CG;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)grid);
@@ -339,29 +330,29 @@ int launch_gemm(GemmArgs &g, cudaStream_t s) {
     cfg.attrs = attr;
     cfg.numAttrs = CG > 1 ? 2 : 1;
     launch_count.fetch_add(1, std::memory_order_relaxed);
-    return cudaLaunchKernelEx(&cfg, kern, g) == cudaSuccess ? WKV_OK : WKV_ERR_LAUNCH;
+    if (cudaLaunchKernelEx(&cfg, kern, g) != cudaSuccess) return WKV_ERR_LAUNCH;
+    if (g.splits == 1) return WKV_OK;
+    constexpr int CTAS = T::BM * (EPI == EPI_GATED ? BN / 2 : BN) / 8 / 256;
+    return launch_chained(k_fold_parts<F, EPI, T::BM, BN>, dim3((unsigned)(g.rest * CTAS)), dim3(256), 0, s, g);
 }
 
-// D = A B^T.  a, b: one or two sources.  How two are taken: `stack` = the rows of D are those of both (A's second source below the
+// D = A B^T.  a, b: one or two sources.  How two are taken: with one B the rows of D are those of both (A's second source below the
 // first), else the contraction runs over both; a pair's forward pass has one A and two B.
 template <typename F, bool A_MN, bool B_MN, int EPI>
 int product(const Matrix (&a)[2], const Matrix (&b)[2], int a_sources, int b_sources, long long m, long long n, long long k, const Cut &cut, const Epi &e,
-            int *status, cudaStream_t s) {
+            void *part, int *status, cudaStream_t s) {
     constexpr bool PAIR = EPI == EPI_GATED;
+    if (cut.cg == 0) return WKV_ERR_SHAPE;
     GemmArgs g = {};
-    const int bm = 128 * cut.cg, out = PAIR ? cut.bn / 2 : cut.bn;
-    const bool stack = a_sources == 2 && b_sources == 1;
     g.M = (int)m; g.N = (int)n;
-    g.m_tiles0 = (int)((m + bm - 1) / bm);
-    g.m_tiles = g.m_tiles0 * (stack ? 2 : 1);
-    g.n_tiles = (int)((n + out - 1) / out);
+    g.m_tiles0 = cut.m_tiles0; g.m_tiles = cut.m_tiles; g.n_tiles = cut.n_tiles;
     g.kb0 = (int)((k + KB - 1) / KB);
-    g.kb = g.kb0 * (a_sources == 2 && !stack ? 2 : 1);
-    g.splits = cut.splits; g.kb_split = cut.splits > 1 ? cut.kb_split : g.kb;
+    g.kb = g.kb0 * (a_sources == 2 && b_sources == 2 ? 2 : 1);
+    g.main = cut.main; g.rest = cut.rest; g.splits = cut.splits; g.kb_split = cut.kb_split;
     g.group = 8;
     g.status = status; g.limit = WAIT_LIMIT;
     g.e = e;
-    if ((long long)g.m_tiles * g.n_tiles * g.splits > 1 << 30) return WKV_ERR_SHAPE;
+    g.e.part = (float *)part;
     const int b_box = PAIR ? cut.bn / 2 : cut.bn / cut.cg;
     for (int i = 0; i < 2; i++) {
         const Matrix &ma = a[a_sources == 2 ? i : 0], &mb = b[b_sources == 2 ? i : 0];
@@ -369,21 +360,8 @@ int product(const Matrix (&a)[2], const Matrix (&b)[2], int a_sources, int b_sou
             !make_matrix_map(&g.b[i], mb.p, mb.rows, mb.cols, mb.pitch, B_MN ? 64 : b_box))
             return WKV_ERR_LAUNCH;
     }
-    if constexpr (EPI == EPI_PARTIAL) return launch_gemm<F, 1, 128, A_MN, B_MN, EPI>(g, s);
-    else if (cut.cg == 2) return launch_gemm<F, 2, 256, A_MN, B_MN, EPI>(g, s);
-    else return launch_gemm<F, 1, 128, A_MN, B_MN, EPI>(g, s);
-}
-// a product with the linear epilogue, its contraction split where that is faster
-template <typename F, bool A_MN, bool B_MN>
-int product_linear(const Matrix (&a)[2], const Matrix (&b)[2], int a_sources, int b_sources, long long m, long long n, long long k, const Cut &cut, Epi e,
-                   Scratch &ws, int *status, cudaStream_t s) {
-    if (cut.splits == 1) return product<F, A_MN, B_MN, EPI_LINEAR>(a, b, a_sources, b_sources, m, n, k, cut, e, status, s);
-    e.part = (float *)ws.take(split_bytes(cut, m, n));
-    e.part_row = up8(n);
-    const int rc = product<F, A_MN, B_MN, EPI_PARTIAL>(a, b, a_sources, b_sources, m, n, k, cut, e, status, s);
-    if (rc != WKV_OK) return rc;
-    const long long pieces = m * ((n + 7) / 8);
-    return launch_chained(k_fold_split<F>, dim3((unsigned)((pieces + 255) / 256)), dim3(256), 0, s, e, m, (int)n, cut.splits);
+    if (cut.cg == 2) return cut.bn == 256 ? launch_gemm<F, 2, 256, A_MN, B_MN, EPI>(g, s) : launch_gemm<F, 2, 128, A_MN, B_MN, EPI>(g, s);
+    return cut.bn == 128 ? launch_gemm<F, 1, 128, A_MN, B_MN, EPI>(g, s) : launch_gemm<F, 1, 64, A_MN, B_MN, EPI>(g, s);
 }
 
 int check_args(const wkv_linear_args_t *a) {
@@ -418,7 +396,6 @@ Epi epilogue_of(const wkv_linear_args_t *a) {
     Epi e = {};
     e.act = a->act;
     e.vec = a->N % 8 == 0 && all_aligned({a->y, a->mul, a->residual});
-    e.save_vec = 1;
     e.bias = a->bias; e.bias_dtype = a->bias_dtype; e.mul = a->mul; e.residual = a->residual;
     e.y[0] = a->y; e.y_row = a->N;
     if (a->saved != nullptr && keeps(a)) {
@@ -462,12 +439,13 @@ int forward(const wkv_linear_args_t *a, Scratch ws, size_t *need, cudaStream_t s
     if (rc != WKV_OK) return rc;
     const Cut cut = cut_for(a->rows, a->N, 1, (int)((a->K + KB - 1) / KB), a->pair);
     if (count) {
-        *need = ws.used + align256(split_bytes(cut, a->rows, a->N));
+        *need = ws.used + align256(cut.part_bytes());
         return WKV_OK;
     }
     const Matrix xs[2] = {x, x};
-    if (a->pair) return product<F, false, false, EPI_GATED>(xs, w, 1, 2, a->rows, a->N, a->K, cut, e, a->status, s);
-    return product_linear<F, false, false>(xs, w, 1, 1, a->rows, a->N, a->K, cut, e, ws, a->status, s);
+    void *part = ws.take(cut.part_bytes());
+    if (a->pair) return product<F, false, false, EPI_GATED>(xs, w, 1, 2, a->rows, a->N, a->K, cut, e, part, a->status, s);
+    return product<F, false, false, EPI_LINEAR>(xs, w, 1, 1, a->rows, a->N, a->K, cut, e, part, a->status, s);
 }
 
 template <typename F>
@@ -516,13 +494,13 @@ int backward(const wkv_linear_args_t *a, Scratch ws, size_t *need, cudaStream_t 
         Matrix w[2] = {w_of(a, 0), w_of(a, a->pair)};
         for (int i = 0; i <= a->pair && rc == WKV_OK; i++) rc = ready<F>(w[i], ws, s);
         const Cut cut = cut_for(a->rows, a->K, 1, kb_n, false);
-        most = std::max(most, align256(split_bytes(cut, a->rows, a->K)));
+        most = std::max(most, align256(cut.part_bytes()));
         if (!count && rc == WKV_OK) {
             Epi e = {};
             e.vec = a->K % 8 == 0 && aligned16(a->gx);
             e.y[0] = a->gx; e.y_row = a->K;
             Scratch parts = ws;
-            rc = product_linear<F, false, true>(gz, w, sources, sources, a->rows, a->K, a->N, cut, e, parts, a->status, s);
+            rc = product<F, false, true, EPI_LINEAR>(gz, w, sources, sources, a->rows, a->K, a->N, cut, e, parts.take(cut.part_bytes()), a->status, s);
         }
     }
     if (rc == WKV_OK && (a->gw0 != nullptr || a->gw1 != nullptr)) {
@@ -531,7 +509,7 @@ int backward(const wkv_linear_args_t *a, Scratch ws, size_t *need, cudaStream_t 
         const Matrix xs[2] = {x, x};
         const bool both = a->gw0 != nullptr && a->gw1 != nullptr;
         const Cut cut = cut_for(a->N, a->K, 1 + both, kb_r, false);
-        most = std::max(most, align256(split_bytes(cut, a->N, a->K)));
+        most = std::max(most, align256(cut.part_bytes()));
         if (!count && rc == WKV_OK) {
             Epi e = {};
             e.vec = a->K % 8 == 0 && all_aligned({a->gw0, a->gw1});
@@ -540,7 +518,7 @@ int backward(const wkv_linear_args_t *a, Scratch ws, size_t *need, cudaStream_t 
             e.y_row = a->K;
             if (a->gw0 == nullptr) gz[0] = gz[1];
             Scratch parts = ws;
-            rc = product_linear<F, true, true>(gz, xs, 1 + both, 1, a->N, a->K, a->rows, cut, e, parts, a->status, s);
+            rc = product<F, true, true, EPI_LINEAR>(gz, xs, 1 + both, 1, a->N, a->K, a->rows, cut, e, parts.take(cut.part_bytes()), a->status, s);
         }
     }
     if (count) *need = ws.used + most;

@@ -31,41 +31,37 @@ namespace linear {
 enum { ACT_NONE = 0, ACT_SILU = 1, ACT_GELU = 2, ACT_RELU2 = 3, ACT_SIGMOID = 4, ACT_COUNT = 5 };
 
 constexpr int EPI_WARPS = 8, THREADS = 32 * (EPI_WARPS + 2), KB = 64, ACC = 2;
-enum { EPI_LINEAR = 0, EPI_GATED = 1, EPI_PARTIAL = 2 };
+enum { EPI_LINEAR = 0, EPI_GATED = 1 };
 constexpr int STATUS_LINEAR = 64;          // the status word's bit of these kernels
 
 __device__ __forceinline__ float sigmoid_of(float x) { return __fdividef(1.f, 1.f + __expf(-x)); }
 // Phi(z) through erfc, which keeps its digits where Phi is small
 __device__ __forceinline__ float phi_of(float z) { return 0.5f * erfcf(-0.7071067811865476f * z); }
 
-template <int N>
-__device__ __forceinline__ void act_values(int act, float (&z)[N]) {
+template <int R, int N>
+__device__ __forceinline__ void act_values(int act, float (&z)[R][N]) {
+    auto each = [&](auto f) {
+#pragma unroll
+        for (int k = 0; k < R; k++)
+#pragma unroll
+            for (int i = 0; i < N; i++) z[k][i] = f(z[k][i]);
+    };
     switch (act) {
-        case ACT_SILU:
-#pragma unroll
-            for (int i = 0; i < N; i++) z[i] = z[i] * sigmoid_of(z[i]);
-            break;
-        case ACT_GELU:
-#pragma unroll
-            for (int i = 0; i < N; i++) z[i] = z[i] * phi_of(z[i]);
-            break;
+        case ACT_SILU: each([](float z) { return z * sigmoid_of(z); }); break;
+        case ACT_GELU: each([](float z) { return z * phi_of(z); }); break;
         case ACT_RELU2:
-#pragma unroll
-            for (int i = 0; i < N; i++) {
-                const float p = z[i] > 0.f ? z[i] : (z[i] == z[i] ? 0.f : z[i]);
-                z[i] = p * p;
-            }
+            each([](float z) {
+                const float p = z > 0.f ? z : (z == z ? 0.f : z);
+                return p * p;
+            });
             break;
-        case ACT_SIGMOID:
-#pragma unroll
-            for (int i = 0; i < N; i++) z[i] = sigmoid_of(z[i]);
-            break;
+        case ACT_SIGMOID: each([](float z) { return sigmoid_of(z); }); break;
         default: break;
     }
 }
 
 struct Epi {
-    int act, vec, save_vec;           // vec: whole 16-byte pieces in y, mul and residual
+    int act, vec;                     // vec: y, mul and residual are rows of whole 16-byte pieces
     const void *bias;                 // [N]
     int bias_dtype;
     const void *mul, *residual;       // [M,N]
@@ -73,8 +69,7 @@ struct Epi {
     long long y_row;                  // their row stride, and that of mul and residual
     void *z[2];                       // pre-activations (or NULL)
     long long z_row;
-    float *part;                      // EPI_PARTIAL: [splits][pair][M][part_row]
-    long long part_row;
+    float *part;                      // sums of parts of a contraction: [tile][part][row of the tile][column of the tile]
 };
 
 // Element i of the bias, 0 without one.  Plain loads: those of the read-only path (__ldg) may be moved by the compiler, and were, out of
@@ -92,7 +87,8 @@ struct GemmArgs {
     int m_tiles, n_tiles;             // m_tiles: of all sources
     int m_tiles0;                     // tiles of A's first source (rows of the second one after them); m_tiles where there is one
     int kb, kb0;                      // contraction blocks of 64, of all sources and of the first one
-    int splits, kb_split;             // contraction split: its parts and their length
+    int main, rest;                   // tiles that are computed whole, and those behind them whose contraction is cut
+    int splits, kb_split;             // into so many parts of so many blocks: a wave of CTAs that the rest alone would not fill
     int group;                        // tiles of M that are walked together
     int *status;
     unsigned limit;
@@ -204,78 +200,107 @@ struct Tile {
 };
 
 struct Item {
-    int m, n, split, kb, kb_end;
+    int m, n, part, kb, kb_end;       // part: index of the sums that are left, -1 where the tile is finished
 };
-__device__ __forceinline__ Item item_at(const GemmArgs &g, int i) {
-    Item t;
-    const int tiles = g.m_tiles * g.n_tiles;
-    t.split = i / tiles;
-    i -= t.split * tiles;
+__device__ __forceinline__ void tile_at(const GemmArgs &g, int i, int &m, int &n) {
     const int per = g.group * g.n_tiles, grp = i / per, first = grp * g.group, rows = min(g.group, g.m_tiles - first);
     i -= grp * per;
-    t.n = i / rows;
-    t.m = first + i - t.n * rows;
-    t.kb = t.split * g.kb_split;
-    t.kb_end = min(g.kb, t.kb + g.kb_split);
+    n = i / rows;
+    m = first + i - n * rows;
+}
+__device__ __forceinline__ Item item_at(const GemmArgs &g, int i) {
+    Item t;
+    t.part = -1;
+    t.kb = 0;
+    t.kb_end = g.kb;
+    if (i >= g.main) {
+        const int j = i - g.main, split = j / g.rest, r = j - split * g.rest;
+        i = g.main + r;
+        if (g.splits > 1) {
+            t.part = r * g.splits + split;
+            t.kb = split * g.kb_split;
+            t.kb_end = min(g.kb, t.kb + g.kb_split);
+        }
+    }
+    tile_at(g, i, t.m, t.n);
     return t;
 }
 
-// one piece of 8 columns of a row -> its outputs.  f: accumulators of the piece (EPI_GATED: u in f2)
-template <typename F, int EPI>
-__device__ __forceinline__ void finish8(const Epi &e, int src, long long row, int col, int n, float (&f)[8], const float (&u)[8], const float *bias) {
-    const bool whole = n >= 8;
-    if (EPI == EPI_LINEAR) {
-        if (e.bias != nullptr) {
+// R pieces of W columns each (accumulators f; EPI_GATED: u in `u`), `rows` apart from row `row` on -> their outputs.  What is read for them is
+// asked for first; the activation is chosen once for all of them.  ok: whether a piece's row exists; n: columns of a piece that exist (W at least
+// where VEC: one access of 16 bytes each).
+template <typename F, int EPI, int R, int W, bool VEC>
+struct Finish {
+    Raw<F, VEC ? 8 : 2> mul[R], res[R];
+
+    __device__ __forceinline__ void ask(const Epi &e, long long row, int rows, int col, int n, const bool (&ok)[R]) {
+        if (EPI != EPI_LINEAR) return;
+        auto get = [&](const void *p, Raw<F, VEC ? 8 : 2> (&to)[R]) {
 #pragma unroll
-            for (int i = 0; i < 8; i++) f[i] += bias[i];
+            for (int k = 0; k < R; k++) {
+                to[k].zero();
+                const F *q = (const F *)p + (row + k * rows) * e.y_row + col;
+                if (ok[k] && n > 0) to[k].load(q, VEC, n);
+            }
+        };
+        if (e.mul != nullptr) get(e.mul, mul);
+        if (e.residual != nullptr) get(e.residual, res);
+    }
+    __device__ __forceinline__ void put(void *p, long long at, const float (&f)[W], bool ok, int n) const {
+        if constexpr (W == 8) {
+            Raw<F, 8> r;
+            r.put(f);
+            if (ok && n > 0) r.store((F *)p + at, true, 8);
+        } else {
+            if (ok && n > 0) Elem<F>::st((F *)p + at, f[0]);
         }
     }
-    Raw<F, 8> r;
-    if (e.z[0] != nullptr) {
-        r.put(f);
-        r.store((F *)e.z[0] + row * e.z_row + col, e.save_vec && whole, n);
+    __device__ __forceinline__ void finish(const Epi &e, int src, long long row, int rows, int col, int n, const bool (&ok)[R], float (&f)[R][W],
+                                           const float (&u)[R][W], const float (&bias)[W]) {
+        if (EPI == EPI_LINEAR && e.bias != nullptr) {
+#pragma unroll
+            for (int k = 0; k < R; k++)
+#pragma unroll
+                for (int i = 0; i < W; i++) f[k][i] += bias[i];
+        }
+        if (e.z[0] != nullptr) {
+#pragma unroll
+            for (int k = 0; k < R; k++) {
+                const long long at = (row + k * rows) * e.z_row + col;
+                put(e.z[0], at, f[k], ok[k], n);
+                if (EPI == EPI_GATED) put(e.z[1], at, u[k], ok[k], n);
+            }
+        }
+        act_values(e.act, f);
         if (EPI == EPI_GATED) {
-            r.put(u);
-            r.store((F *)e.z[1] + row * e.z_row + col, e.save_vec && whole, n);
+#pragma unroll
+            for (int k = 0; k < R; k++)
+#pragma unroll
+                for (int i = 0; i < W; i++) f[k][i] *= u[k][i];
         }
-    }
-    act_values(e.act, f);
-    if (EPI == EPI_GATED) {
+        if (EPI == EPI_LINEAR && e.mul != nullptr) {
 #pragma unroll
-        for (int i = 0; i < 8; i++) f[i] *= u[i];
-    }
-    if (EPI == EPI_LINEAR && e.mul != nullptr) {
-        float m[8];
-        r.load((const F *)e.mul + row * e.y_row + col, e.vec && whole, n);
-        r.get(m);
+            for (int k = 0; k < R; k++) {
+                float m[VEC ? 8 : 2];
+                mul[k].get(m);
 #pragma unroll
-        for (int i = 0; i < 8; i++) f[i] *= m[i];
-    }
-    if (EPI == EPI_LINEAR && e.residual != nullptr) {
-        float m[8];
-        r.load((const F *)e.residual + row * e.y_row + col, e.vec && whole, n);
-        r.get(m);
+                for (int i = 0; i < W; i++) f[k][i] *= m[i];
+            }
+        }
+        if (EPI == EPI_LINEAR && e.residual != nullptr) {
 #pragma unroll
-        for (int i = 0; i < 8; i++) f[i] += m[i];
+            for (int k = 0; k < R; k++) {
+                float m[VEC ? 8 : 2];
+                res[k].get(m);
+#pragma unroll
+                for (int i = 0; i < W; i++) f[k][i] += m[i];
+            }
+        }
+        void *y = src ? e.y[1] : e.y[0];
+#pragma unroll
+        for (int k = 0; k < R; k++) put(y, (row + k * rows) * e.y_row + col, f[k], ok[k], n);
     }
-    r.put(f);
-    r.store((F *)(src ? e.y[1] : e.y[0]) + row * e.y_row + col, e.vec && whole, n);
-}
-// the same for one column (rows that do not lie in whole pieces: neighbouring lanes take neighbouring columns)
-template <typename F, int EPI>
-__device__ __forceinline__ void finish1(const Epi &e, int src, long long row, int col, float f, float u, float bias) {
-    if (EPI == EPI_LINEAR) f += bias;
-    if (e.z[0] != nullptr) {
-        Elem<F>::st((F *)e.z[0] + row * e.z_row + col, f);
-        if (EPI == EPI_GATED) Elem<F>::st((F *)e.z[1] + row * e.z_row + col, u);
-    }
-    float v[1] = {f};
-    act_values(e.act, v);
-    if (EPI == EPI_GATED) v[0] *= u;
-    if (EPI == EPI_LINEAR && e.mul != nullptr) v[0] *= Elem<F>::ld((const F *)e.mul + row * e.y_row + col);
-    if (EPI == EPI_LINEAR && e.residual != nullptr) v[0] += Elem<F>::ld((const F *)e.residual + row * e.y_row + col);
-    Elem<F>::st((F *)(src ? e.y[1] : e.y[0]) + row * e.y_row + col, v[0]);
-}
+};
 
 template <typename F, int CG, int BN, bool A_MN, bool B_MN, int EPI>
 __global__ void __launch_bounds__(THREADS, 1) k_gemm(const __grid_constant__ GemmArgs g) {
@@ -289,7 +314,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_gemm(const __grid_constant__ Gem
     volatile int *abort = reinterpret_cast<int *>(tmem + 1);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t rank = CG == 2 ? cluster_rank() : 0;
-    const int first = blockIdx.x / CG, step = gridDim.x / CG, items = g.m_tiles * g.n_tiles * g.splits;
+    const int first = blockIdx.x / CG, step = gridDim.x / CG, items = g.main + g.rest * g.splits;
 
     pdl_wait();
     pdl_trigger();
@@ -437,66 +462,85 @@ __global__ void __launch_bounds__(THREADS, 1) k_gemm(const __grid_constant__ Gem
 #pragma unroll 1
             for (int p = 0; p < PASSES; p++) {
                 const int c = half * (OUT / 2) + p * PASS, col0 = t.n * OUT + c;
-                float v[32];
-                if (EPI == EPI_GATED) {
-                    sm100::tmem_ld16(lanes + c, v);
-                    sm100::tmem_ld16(lanes + OUT + c, v + 16);
-                } else {
-                    tmem_ld32(lanes + c, v);
-                }
-                sm100::tmem_ld_wait();
-                if (p == PASSES - 1) {
-                    // (the accumulator is in registers: the next tile's products may have it)
-                    sm100::tc_fence_before();
-                    __syncwarp();
-                    if (lane == 0) {
-                        if (CG == 2) arrive_remote(map_rank(acc_empty + buf, 0));
-                        else sm100::mbar_arrive(acc_empty + buf);
+                auto turn_in = [&] {
+                    float v[32];
+                    if (EPI == EPI_GATED) {
+                        sm100::tmem_ld16(lanes + c, v);
+                        sm100::tmem_ld16(lanes + OUT + c, v + 16);
+                    } else {
+                        tmem_ld32(lanes + c, v);
                     }
-                }
+                    sm100::tmem_ld_wait();
+                    if (p == PASSES - 1) {
+                        // (the accumulator is in registers: the next tile's products may have it)
+                        sm100::tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) {
+                            if (CG == 2) arrive_remote(map_rank(acc_empty + buf, 0));
+                            else sm100::mbar_arrive(acc_empty + buf);
+                        }
+                    }
 #pragma unroll
-                for (int j = 0; j < 8; j++)
-                    asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(turn_w + ((j ^ (lane & 7)) << 4)), "f"(v[4 * j]),
-                                 "f"(v[4 * j + 1]), "f"(v[4 * j + 2]), "f"(v[4 * j + 3]) : "memory");
-                __syncwarp();
+                    for (int j = 0; j < 8; j++)
+                        asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(turn_w + ((j ^ (lane & 7)) << 4)), "f"(v[4 * j]),
+                                     "f"(v[4 * j + 1]), "f"(v[4 * j + 2]), "f"(v[4 * j + 3]) : "memory");
+                    __syncwarp();
+                };
                 auto at = [&](int r, int chunk) { return *reinterpret_cast<const float4 *>(turn + r * 32 + ((chunk ^ (r & 7)) << 2)); };
                 auto get8 = [&](int r, int chunk, float (&f)[8]) {
                     const float4 x = at(r, chunk), y = at(r, chunk + 1);
                     f[0] = x.x; f[1] = x.y; f[2] = x.z; f[3] = x.w; f[4] = y.x; f[5] = y.y; f[6] = y.z; f[7] = y.w;
                 };
-                if (EPI == EPI_PARTIAL) {
-                    // (rows of part are whole pieces; its columns behind N are never read)
-                    const int cc = (lane & 7) * 4;
-                    float *out = e.part + ((size_t)t.split * g.M + row0) * e.part_row + col0 + cc;
+                if (t.part >= 0) {
+                    turn_in();
+                    // (of a pair: 16 columns of each half)
+                    const int cc = (lane & 7) * 4, pc = EPI == EPI_GATED ? (cc < 16 ? c + cc : OUT + c + cc - 16) : c + cc;
+                    float *out = e.part + ((size_t)t.part * T::BM + rank * 128 + quarter * 32) * BN + pc;
 #pragma unroll
                     for (int k = 0; k < 8; k++) {
                         const int r = k * 4 + (lane >> 3);
-                        if (row0 + r < g.M && col0 + cc < e.part_row) *reinterpret_cast<float4 *>(out + (size_t)r * e.part_row) = at(r, lane & 7);
+                        *reinterpret_cast<float4 *>(out + (size_t)r * BN) = at(r, lane & 7);
                     }
                 } else if (e.vec) {
-                    constexpr int LANES = PASS / 8, ROWS = 32 / LANES;       // lanes of a row, rows of an access
-                    const int cc = (lane % LANES) * 8, n = g.N - (col0 + cc);
-                    float bias[8];
+                    constexpr int LANES = PASS / 8, ROWS = 32 / LANES, R = 32 / ROWS;        // lanes of a row, rows of an access, accesses
+                    const int cc = (lane % LANES) * 8, col = col0 + cc, n = g.N - col, r0 = lane / LANES;
+                    Finish<F, EPI, R, 8, true> out;
+                    bool ok[R];
+#pragma unroll
+                    for (int k = 0; k < R; k++) ok[k] = row0 + r0 + k * ROWS < g.M;
+                    out.ask(e, row0 + r0, ROWS, col, n, ok);
+                    float bias[8], f[R][8], u[R][8];
                     if (EPI == EPI_LINEAR && e.bias != nullptr) {
 #pragma unroll
-                        for (int k = 0; k < 8; k++) bias[k] = k < n ? bias_at(e, col0 + cc + k) : 0.f;
+                        for (int k = 0; k < 8; k++) bias[k] = k < n ? bias_at(e, col + k) : 0.f;
                     }
+                    turn_in();
 #pragma unroll
-                    for (int k = 0; k < 32 / ROWS; k++) {
-                        const int r = k * ROWS + lane / LANES;
-                        float f[8], u[8];
-                        get8(r, cc / 4, f);
-                        if (EPI == EPI_GATED) get8(r, 4 + cc / 4, u);
-                        if (row0 + r < g.M && n > 0) finish8<F, EPI>(e, src, row0 + r, col0 + cc, n, f, u, bias);
+                    for (int k = 0; k < R; k++) {
+                        get8(r0 + k * ROWS, cc / 4, f[k]);
+                        if (EPI == EPI_GATED) get8(r0 + k * ROWS, 4 + cc / 4, u[k]);
                     }
+                    out.finish(e, src, row0 + r0, ROWS, col, n, ok, f, u, bias);
                 } else {
-                    const int cc = lane % PASS, col = col0 + cc;
-                    const float bias = EPI == EPI_LINEAR && col < g.N ? bias_at(e, col) : 0.f;
-#pragma unroll 4
-                    for (int r = lane / PASS; r < 32; r += 32 / PASS) {
-                        const float f = turn[r * 32 + (((cc >> 2) ^ (r & 7)) << 2) + (cc & 3)];
-                        const float u = EPI == EPI_GATED ? turn[r * 32 + (((4 + (cc >> 2)) ^ (r & 7)) << 2) + (cc & 3)] : 0.f;
-                        if (row0 + r < g.M && col < g.N) finish1<F, EPI>(e, src, row0 + r, col, f, u, bias);
+                    constexpr int ROWS = 32 / PASS, R = 8;
+                    const int cc = lane % PASS, col = col0 + cc, n = g.N - col;
+                    float bias[1] = {EPI == EPI_LINEAR && n > 0 ? bias_at(e, col) : 0.f};
+                    turn_in();
+#pragma unroll 1
+                    for (int r0 = lane / PASS; r0 < 32; r0 += R * ROWS) {
+                        Finish<F, EPI, R, 1, false> out;
+                        bool ok[R];
+                        float f[R][1], u[R][1];
+#pragma unroll
+                        for (int k = 0; k < R; k++) ok[k] = row0 + r0 + k * ROWS < g.M;
+                        out.ask(e, row0 + r0, ROWS, col, min(n, 1), ok);
+#pragma unroll
+                        for (int k = 0; k < R; k++) {
+                            const int r = r0 + k * ROWS;
+                            f[k][0] = turn[r * 32 + (((cc >> 2) ^ (r & 7)) << 2) + (cc & 3)];
+                            if (EPI == EPI_GATED) u[k][0] = turn[r * 32 + (((4 + (cc >> 2)) ^ (r & 7)) << 2) + (cc & 3)];
+                        }
+                        out.finish(e, src, row0 + r0, ROWS, col, n, ok, f, u, bias);
                     }
                 }
                 __syncwarp();
@@ -509,6 +553,51 @@ __global__ void __launch_bounds__(THREADS, 1) k_gemm(const __grid_constant__ Gem
     if (CG == 2) cluster_sync();
     sm100::tc_fence_after();
     if (warp == EPI_WARPS + 1) tmem_free<CG>(acc0, T::COLS);
+}
+
+// The sums of the parts of the tiles behind `main`, in order, then the epilogue: a thread has 8 columns of a row.
+template <typename F, int EPI, int BM, int BN>
+__global__ void __launch_bounds__(256) k_fold_parts(const __grid_constant__ GemmArgs g) {
+    pdl_wait();
+    pdl_trigger();
+    constexpr int OUT = EPI == EPI_GATED ? BN / 2 : BN, PIECES = OUT / 8, CTAS = BM * PIECES / 256;      // CTAs of a tile
+    const int r = blockIdx.x / CTAS, i = (blockIdx.x - r * CTAS) * 256 + threadIdx.x, y = i / PIECES, c = (i - y * PIECES) * 8;
+    int tm, tn;
+    tile_at(g, g.main + r, tm, tn);
+    const int src = tm >= g.m_tiles0, col = tn * OUT + c, n = g.N - col;
+    const long long row = (long long)(tm - (src ? g.m_tiles0 : 0)) * BM + y;
+    if (row >= g.M || n <= 0) return;
+    float f[1][8], u[1][8], bias[8];
+#pragma unroll
+    for (int k = 0; k < 8; k++) f[0][k] = u[0][k] = 0.f;
+    const float *p = g.e.part + ((size_t)r * g.splits * BM + y) * BN + c;
+    auto add = [&](const float *q, float (&to)[8]) {
+        const float4 a = *reinterpret_cast<const float4 *>(q), b = *reinterpret_cast<const float4 *>(q + 4);
+        to[0] += a.x; to[1] += a.y; to[2] += a.z; to[3] += a.w; to[4] += b.x; to[5] += b.y; to[6] += b.z; to[7] += b.w;
+    };
+#pragma unroll 4
+    for (int s = 0; s < g.splits; s++) {
+        add(p + (size_t)s * BM * BN, f[0]);
+        if (EPI == EPI_GATED) add(p + (size_t)s * BM * BN + OUT, u[0]);
+    }
+    const bool ok[1] = {true};
+    if (g.e.vec) {
+        Finish<F, EPI, 1, 8, true> out;
+        out.ask(g.e, row, 1, col, n, ok);
+#pragma unroll
+        for (int k = 0; k < 8; k++) bias[k] = EPI == EPI_LINEAR ? bias_at(g.e, col + k) : 0.f;
+        out.finish(g.e, src, row, 1, col, n, ok, f, u, bias);
+    } else {
+#pragma unroll
+        for (int k = 0; k < 8; k++) {
+            if (k >= n) break;
+            Finish<F, EPI, 1, 1, false> out;
+            float v[1][1] = {{f[0][k]}};
+            const float w[1][1] = {{u[0][k]}}, b[1] = {EPI == EPI_LINEAR ? bias_at(g.e, col + k) : 0.f};
+            out.ask(g.e, row, 1, col + k, 1, ok);
+            out.finish(g.e, src, row, 1, col + k, 1, ok, v, w, b);
+        }
+    }
 }
 
 }  // namespace linear
