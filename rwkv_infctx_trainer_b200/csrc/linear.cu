@@ -157,9 +157,10 @@ __device__ __forceinline__ void act_both(int act, float z, float &v, float &d) {
         const float p = z > 0.f ? z : (z == z ? 0.f : z);
         v = p * p; d = 2.f * p;
     } else if (act == ACT_GELU) {
-        const float phi = phi_of(z);
+        float g;
+        const float phi = phi_of(z, g);
         v = z * phi;
-        d = fmaf(z, 0.3989422804014327f * __expf(-0.5f * z * z), phi);
+        d = fmaf(z, 0.3989422804014327f * g, phi);
     } else {
         const float s = sigmoid_of(z), n = sigmoid_of(-z);
         v = act == ACT_SILU ? z * s : s;
