@@ -141,7 +141,7 @@ __global__ void __launch_bounds__(32 * FEW_WARPS) k_few_rows(const FewArgs g) {
 // ------------------------------------------------------------------------------------------ gradient of the pre-activation
 struct GradArgs {
     long long rows;
-    int N, act, vec, rows_per;
+    int N, act, rows_per;
     const void *gy, *mul, *z[2];
     long long z_row;
     void *gz[2], *gmul;
@@ -149,77 +149,115 @@ struct GradArgs {
     float *part;                        // [gridDim.y, N] sums of gz over a CTA's rows
 };
 
-// act(z) and its derivative
-__device__ __forceinline__ void act_both(int act, float z, float &v, float &d) {
-    if (act == ACT_NONE) {
-        v = z; d = 1.f;
-    } else if (act == ACT_RELU2) {
-        const float p = z > 0.f ? z : (z == z ? 0.f : z);
-        v = p * p; d = 2.f * p;
-    } else if (act == ACT_GELU) {
-        float g;
-        const float phi = phi_of(z, g);
-        v = z * phi;
-        d = fmaf(z, 0.3989422804014327f * g, phi);
-    } else {
-        const float s = sigmoid_of(z), n = sigmoid_of(-z);
-        v = act == ACT_SILU ? z * s : s;
-        d = act == ACT_SILU ? s * fmaf(z, n, 1.f) : s * n;
+// act(z) and its derivative, of N elements: the activation is chosen once
+template <int N>
+__device__ __forceinline__ void act_both(int act, const float (&z)[N], float (&v)[N], float (&d)[N]) {
+    auto each = [&](auto f) {
+#pragma unroll
+        for (int i = 0; i < N; i++) f(z[i], v[i], d[i]);
+    };
+    // sigmoid(z) and sigmoid(-z) from one exponential: both keep their digits
+    auto sigmoids = [](float z, float &s, float &n) {
+        const float e = __expf(-fabsf(z)), r = __fdividef(1.f, 1.f + e), q = e * r;
+        s = z >= 0.f ? r : q;
+        n = z >= 0.f ? q : r;
+    };
+    switch (act) {
+        case ACT_SILU:
+            each([&](float z, float &v, float &d) {
+                float s, n;
+                sigmoids(z, s, n);
+                v = z * s;
+                d = s * fmaf(z, n, 1.f);
+            });
+            break;
+        case ACT_SIGMOID:
+            each([&](float z, float &v, float &d) {
+                float n;
+                sigmoids(z, v, n);
+                d = v * n;
+            });
+            break;
+        case ACT_GELU:
+            each([&](float z, float &v, float &d) {
+                float g;
+                const float phi = phi_of(z, g);
+                v = z * phi;
+                d = fmaf(z, 0.3989422804014327f * g, phi);
+            });
+            break;
+        case ACT_RELU2:
+            each([&](float z, float &v, float &d) {
+                const float p = z > 0.f ? z : (z == z ? 0.f : z);
+                v = p * p;
+                d = 2.f * p;
+            });
+            break;
+        default:
+            each([&](float z, float &v, float &d) {
+                v = z;
+                d = 1.f;
+            });
     }
 }
 
-// a warp walks down rows of 256 columns, 8 a lane; bound by HBM
-template <typename F, bool PAIR>
+// A warp walks down rows of 256 columns, 8 a lane, R rows on their way at once.  Bound by HBM.  VEC: gy, mul and gmul are rows of whole pieces (z and gz always
+// are).
+template <typename F, bool PAIR, bool VEC>
 __global__ void __launch_bounds__(256) k_grad_act(const GradArgs g) {
     pdl_wait();
     pdl_trigger();
+    constexpr int R = 2;
     __shared__ float red[8][256];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, col = blockIdx.x * 256 + lane * 8, n = g.N - col;
-    const bool whole = n >= 8, vec = g.vec && whole;
+    const bool whole = VEC || n >= 8;
     float sum[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
     const long long r0 = (long long)blockIdx.y * g.rows_per, r1 = min(g.rows, r0 + g.rows_per);
     if (n > 0) {
-#pragma unroll 2
-        for (long long row = r0 + warp; row < r1; row += 8) {
-            Raw<F, 8> r;
-            float gy[8], z[8], u[8], m[8], o[8];
-            r.load((const F *)g.gy + row * g.N + col, vec, n);
-            r.get(gy);
-            if (g.z[0] != nullptr) {
-                r.load((const F *)g.z[0] + row * g.z_row + col, whole, n);
-                r.get(z);
-            } else {
+#pragma unroll 1
+        for (long long row = r0 + warp; row < r1; row += 8 * R) {
+            Raw<F, 8> ry[R], rz[R], rm[R];
+            bool ok[R];
 #pragma unroll
-                for (int i = 0; i < 8; i++) z[i] = 0.f;
-            }
-            if (PAIR) {
-                r.load((const F *)g.z[1] + row * g.z_row + col, whole, n);
-                r.get(u);
-            } else if (g.mul != nullptr) {
-                r.load((const F *)g.mul + row * g.N + col, vec, n);
-                r.get(m);
-            } else {
-#pragma unroll
-                for (int i = 0; i < 8; i++) m[i] = 1.f;
+            for (int k = 0; k < R; k++) {
+                const long long at = row + 8 * k;
+                ok[k] = at < r1;
+                ry[k].zero();
+                rz[k].zero();
+                rm[k].zero();
+                if (!ok[k]) continue;
+                ry[k].load((const F *)g.gy + at * g.N + col, VEC, n);
+                if (g.z[0] != nullptr) rz[k].load((const F *)g.z[0] + at * g.z_row + col, whole, n);
+                if (PAIR) rm[k].load((const F *)g.z[1] + at * g.z_row + col, whole, n);
+                else if (g.mul != nullptr) rm[k].load((const F *)g.mul + at * g.N + col, VEC, n);
             }
 #pragma unroll
-            for (int i = 0; i < 8; i++) {
-                float v, d;
-                act_both(g.act, z[i], v, d);
-                o[i] = gy[i] * v;
-                m[i] = gy[i] * (PAIR ? u[i] : m[i]) * d;
-                sum[i] += m[i];
-            }
-            if (g.gz[0] != nullptr) {
-                r.put(m);
-                r.store((F *)g.gz[0] + row * g.gz_row + col, whole, n);
-            }
-            if (PAIR) {
-                r.put(o);
-                r.store((F *)g.gz[1] + row * g.gz_row + col, whole, n);
-            } else if (g.gmul != nullptr) {
-                r.put(o);
-                r.store((F *)g.gmul + row * g.N + col, vec, n);
+            for (int k = 0; k < R; k++) {
+                const long long at = row + 8 * k;
+                float gy[8], z[8], m[8], v[8], d[8];
+                ry[k].get(gy);
+                rz[k].get(z);
+                rm[k].get(m);
+                act_both(g.act, z, v, d);
+                const bool factor = PAIR || g.mul != nullptr;
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    v[i] *= gy[i];
+                    d[i] *= factor ? gy[i] * m[i] : gy[i];
+                    sum[i] += d[i];
+                }
+                if (!ok[k]) continue;
+                if (g.gz[0] != nullptr) {
+                    ry[k].put(d);
+                    ry[k].store((F *)g.gz[0] + at * g.gz_row + col, whole, n);
+                }
+                if (PAIR) {
+                    ry[k].put(v);
+                    ry[k].store((F *)g.gz[1] + at * g.gz_row + col, whole, n);
+                } else if (g.gmul != nullptr) {
+                    ry[k].put(v);
+                    ry[k].store((F *)g.gmul + at * g.N + col, VEC, n);
+                }
             }
         }
     }
@@ -460,7 +498,6 @@ int backward(const wkv_linear_args_t *a, Scratch ws, size_t *need, cudaStream_t 
     const int row_blocks = (int)((a->rows + rows_per - 1) / rows_per);
     GradArgs ga = {};
     ga.rows = a->rows; ga.N = (int)a->N; ga.act = a->act; ga.rows_per = rows_per;
-    ga.vec = a->N % 8 == 0 && all_aligned({a->gy, a->mul, a->gmul});
     ga.gy = a->gy; ga.mul = a->mul;
     if (act) {
         ga.z[0] = a->saved;
@@ -476,7 +513,9 @@ int backward(const wkv_linear_args_t *a, Scratch ws, size_t *need, cudaStream_t 
     int rc = WKV_OK;
     if (!count && (own_gz || a->gmul != nullptr || a->gbias != nullptr)) {
         const dim3 grid((unsigned)((a->N + 255) / 256), (unsigned)row_blocks);
-        rc = a->pair ? launch_chained(k_grad_act<F, true>, grid, dim3(256), 0, s, ga) : launch_chained(k_grad_act<F, false>, grid, dim3(256), 0, s, ga);
+        const bool vec = a->N % 8 == 0 && all_aligned({a->gy, a->mul, a->gmul});
+        rc = a->pair ? launch_chained(vec ? k_grad_act<F, true, true> : k_grad_act<F, true, false>, grid, dim3(256), 0, s, ga)
+                     : launch_chained(vec ? k_grad_act<F, false, true> : k_grad_act<F, false, false>, grid, dim3(256), 0, s, ga);
         if (rc == WKV_OK && a->gbias != nullptr) {
             FoldOut out = {};
             out.p[0] = a->gbias; out.dtype[0] = a->bias_dtype;

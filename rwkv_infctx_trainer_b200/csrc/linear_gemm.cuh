@@ -521,7 +521,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_gemm(const __grid_constant__ Gem
 #pragma unroll
                     for (int k = 0; k < 8; k++) {
                         const int r = k * 4 + (lane >> 3);
-                        *reinterpret_cast<float4 *>(out + (size_t)r * BN) = at(r, lane & 7);
+                        if (row0 + r < g.M) *reinterpret_cast<float4 *>(out + (size_t)r * BN) = at(r, lane & 7);
                     }
                 } else if (e.vec) {
                     constexpr int LANES = PASS / 8, ROWS = 32 / LANES, R = 32 / ROWS;        // lanes of a row, rows of an access, accesses
