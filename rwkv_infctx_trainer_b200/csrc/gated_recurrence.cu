@@ -74,13 +74,21 @@ struct RecArgs {
     float2 *spans;                        // [B, nspan, D]: a span's decay, and its state (backward: E) from zero
 };
 
+// How rows lie: pieces of 16 bytes (TMA brings a block's tile of each tensor, and takes the outputs' away), words, or (two-byte
+// elements) anywhere: a warp fetches its own tokens.
+enum { TILES = 0, WORDS = 1, ANYWHERE = 2 };
+// elements of a token's row in the ring: CH channels, and where rows start at any element one more word, because they are copied from the word that
+// their first element is in (which is of the same allocation: those start and end at words)
+__host__ __device__ constexpr int row_of(int mode) { return mode == ANYWHERE ? CH + 4 : CH; }
+
 // Tokens of a warp in a block (S), for two CTAs an SM: what a thread keeps of its tokens has to fit in 128 registers, because what
 // does not would wait for L2 (shared memory leaves no L1).
 template <typename F, bool BACK>
 struct Geo {
-    static constexpr int S = sizeof(F) == 2 && !BACK ? 8 : 4, BT = NW * S, SLOT = BT * CH;        // SLOT: elements of one tensor's block
+    static constexpr int S = sizeof(F) == 2 && !BACK ? 8 : 4, BT = NW * S;
+    static __host__ __device__ constexpr int slot(int mode) { return BT * row_of(mode); }                             // elements of one tensor's block
     static constexpr int STAGES = sizeof(F) == 4 && BACK ? 2 : 3;
-    static constexpr int ring(bool z) { return STAGES * (3 + BACK + z) * SLOT * (int)sizeof(F); }
+    static constexpr int ring(bool z, int mode) { return STAGES * (3 + BACK + z) * slot(mode) * (int)sizeof(F); }
 };
 constexpr int CKPT = 32;                  // tokens between two states that are kept: a block of the backward pass
 
@@ -165,60 +173,75 @@ __device__ __forceinline__ void cp_async4(void *smem, const void *g, int valid) 
 __device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N> __device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
-// How rows lie: pieces of 16 bytes (TMA brings a block's tile of each tensor, and takes the outputs' away), words, or (two-byte
-// elements) anywhere: a warp fetches its own tokens.
-enum { TILES = 0, WORDS = 1, ANYWHERE = 2 };
 
-// A warp's S tokens of one tensor -> its slot [S][CH] of the ring.  block: the CTA's first token; token: stride.  Tokens from `n` on
-// and channels from D on become zeros.  Offsets inside a block are 32-bit (the host checks the strides).
+// A warp's S tokens of one tensor -> its slot of the ring.  block: the CTA's first token; token: stride.  Tokens from `n` on and channels
+// from D on become zeros (ANYWHERE: a channel behind the last may become anything).  Offsets inside a block are 32-bit (the host checks the strides).
 template <typename F, int MODE, int S>
 __device__ __forceinline__ void fill(F *slot, const F *block, int token, int warp, int n, int left, int lane) {
+    constexpr int ROW = row_of(MODE);
+    const uint32_t at = (uint32_t)(warp * S) * (uint32_t)token;
     if constexpr (MODE == WORDS) {
-        const uint32_t at = (uint32_t)(warp * S) * (uint32_t)token + 2 * lane;
         left -= 2 * lane;
 #pragma unroll
         for (int s = 0; s < S; s++) {
             const bool ok = s < n && left > 0;
-            const F *p = block + (ok ? at + (uint32_t)s * (uint32_t)token : 0u);
+            const F *p = block + (ok ? at + 2 * lane + (uint32_t)s * (uint32_t)token : 0u);
             if constexpr (sizeof(F) == 2) {
-                cp_async4(slot + s * CH + 2 * lane, p, ok ? min(left, 2) * 2 : 0);
+                cp_async4(slot + s * ROW + 2 * lane, p, ok ? min(left, 2) * 2 : 0);
             } else {
-                cp_async4(slot + s * CH + 2 * lane, p, ok ? 4 : 0);
-                cp_async4(slot + s * CH + 2 * lane + 1, ok && left > 1 ? p + 1 : block, ok && left > 1 ? 4 : 0);
+                cp_async4(slot + s * ROW + 2 * lane, p, ok ? 4 : 0);
+                cp_async4(slot + s * ROW + 2 * lane + 1, ok && left > 1 ? p + 1 : block, ok && left > 1 ? 4 : 0);
             }
         }
     } else {
-        const uint32_t at = (uint32_t)(warp * S) * (uint32_t)token + 2 * lane;
-        left -= 2 * lane;
-        uint32_t w[S];
+        auto word = [&](int s, int w) {
+            const uintptr_t row = reinterpret_cast<uintptr_t>(block + (at + (uint32_t)s * (uint32_t)token));
+            const int odd = (int)(row >> 1) & 1;
+            const bool ok = s < n && 2 * w - odd < left;
+            cp_async4(slot + s * ROW + 2 * w, reinterpret_cast<const void *>(((ok ? row : reinterpret_cast<uintptr_t>(block)) & ~(uintptr_t)3) + (ok ? 4 * w : 0)),
+                      ok ? 4 : 0);
+        };
 #pragma unroll
-        for (int s = 0; s < S; s++) {
-            const uint16_t *p = reinterpret_cast<const uint16_t *>(block + (at + (uint32_t)s * (uint32_t)token));
-            w[s] = 0;
-            if (s < n && left > 0) w[s] = p[0];
-            if (s < n && left > 1) w[s] |= (uint32_t)p[1] << 16;
-        }
-#pragma unroll
-        for (int s = 0; s < S; s++) *reinterpret_cast<uint32_t *>(slot + s * CH + 2 * lane) = w[s];
+        for (int s = 0; s < S; s++) word(s, lane);
+        if (lane < S) word(lane, 32);
     }
 }
-template <typename F>
-__device__ __forceinline__ f2 pair_at(const F *slot, int s, int lane) {
+// bit s: whether the row of a warp's token s starts in the second half of a word (the same for every block: their tokens are even in number)
+template <typename F, int MODE, int S>
+__device__ __forceinline__ uint32_t odd_rows(const void *p, long long at, long long token, int warp) {
+    uint32_t m = 0;
+    if constexpr (MODE == ANYWHERE) {
+        const long long first = (long long)(reinterpret_cast<uintptr_t>(p) >> 1) + at + (long long)warp * S * token;
+#pragma unroll
+        for (int s = 0; s < S; s++) m |= (uint32_t)((first + s * token) & 1) << s;
+    }
+    return m;
+}
+template <typename F, int MODE>
+__device__ __forceinline__ f2 pair_at(const F *slot, int s, int lane, uint32_t odd) {
     Raw<F, 2> r;
-    r.load(slot + s * CH + 2 * lane, true, 2);
+    const F *p = slot + s * row_of(MODE) + 2 * lane;
+    r.load(p, true, 2);
+    if constexpr (MODE == ANYWHERE) {
+        const uint32_t next = *reinterpret_cast<const uint32_t *>(p + 2);
+        r.w[0] = odd >> s & 1 ? __funnelshift_r(r.w[0], next, 16) : r.w[0];
+    }
     float f[2];
     r.get(f);
     return make_float2(f[0], f[1]);
 }
 // decay gates of minus infinity for the tokens behind the row's last: they keep the state (x is zero there)
-template <typename F, int S>
+template <typename F, int MODE, int S>
 __device__ __forceinline__ void close_gates(F *slot, int n, int lane) {
+    __syncwarp();                         // (ANYWHERE: a neighbour's word is written)
     for (int s = n; s < S; s++) {
         const float f[2] = {-INFINITY, -INFINITY};
         Raw<F, 2> r;
         r.put(f);
-        r.store(slot + s * CH + 2 * lane, true, 2);
+        r.store(slot + s * row_of(MODE) + 2 * lane, true, 2);
+        if (MODE == ANYWHERE && lane == 0) r.store(slot + s * row_of(MODE) + CH, true, 2);
     }
+    __syncwarp();
 }
 // two channels of a block's output, `at` elements from its first; left: channels there are
 template <typename F>
@@ -295,7 +318,7 @@ __global__ void __launch_bounds__(256, 2) k_rec_fwd(const __grid_constant__ RecA
     pdl_wait();
     pdl_trigger();
     using G = Geo<F, false>;
-    constexpr int S = G::S, BT = G::BT, SLOT = G::SLOT, NT = 3 + Z, ST = G::STAGES, RING = ST * NT * SLOT * (int)sizeof(F);
+    constexpr int S = G::S, BT = G::BT, ROW = row_of(MODE), SLOT = G::slot(MODE), NT = 3 + Z, ST = G::STAGES, RING = ST * NT * SLOT * (int)sizeof(F);
     extern __shared__ __align__(128) unsigned char smem[];
     Exchange &ex = *reinterpret_cast<Exchange *>(smem + RING);
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -312,6 +335,10 @@ __global__ void __launch_bounds__(256, 2) k_rec_fwd(const __grid_constant__ RecA
         if (ch + 1 < g.D) h.y = g.state_in[(size_t)b * g.D + ch + 1];
     }
     if (span > 0) h = fold_spans(g, b, 0, span, 1, ch, h);
+    const uint32_t odd_r = odd_rows<F, MODE, S>(g.rg, b * g.rg_batch + begin * g.rg_token + ch0, g.rg_token, warp),
+                   odd_i = odd_rows<F, MODE, S>(g.ig, b * g.ig_batch + begin * g.ig_token + ch0, g.ig_token, warp),
+                   odd_x = odd_rows<F, MODE, S>(g.x, b * g.x_batch + begin * g.x_token + ch0, g.x_token, warp),
+                   odd_z = Z ? odd_rows<F, MODE, S>(g.z, b * g.z_batch + begin * g.z_token + ch0, g.z_token, warp) : 0u;
     auto start = [&](int step) {
         const long long t0 = begin + (long long)step * BT;
         F *slot = ring + (step % ST) * NT * SLOT;
@@ -321,7 +348,7 @@ __global__ void __launch_bounds__(256, 2) k_rec_fwd(const __grid_constant__ RecA
             for (int i = 0; i < NT; i++) sm100::tma_load_3d(slot + i * SLOT, g.in + i, ex.full + step % ST, ch0, (int)t0, b);
         } else {
             const int n = (int)max(0ll, min((long long)S, g.T - (t0 + warp * S))), left = g.D - ch0;
-            slot += warp * S * CH;
+            slot += warp * S * ROW;
             fill<F, MODE, S>(slot, (const F *)g.rg + (b * g.rg_batch + t0 * g.rg_token + ch0), (int)g.rg_token, warp, n, left, lane);
             fill<F, MODE, S>(slot + SLOT, (const F *)g.ig + (b * g.ig_batch + t0 * g.ig_token + ch0), (int)g.ig_token, warp, n, left, lane);
             fill<F, MODE, S>(slot + 2 * SLOT, (const F *)g.x + (b * g.x_batch + t0 * g.x_token + ch0), (int)g.x_token, warp, n, left, lane);
@@ -350,10 +377,10 @@ __global__ void __launch_bounds__(256, 2) k_rec_fwd(const __grid_constant__ RecA
             cp_wait<ST - 1>();
             __syncwarp();
         }
-        F *slot = ring + (step % ST) * NT * SLOT + warp * S * CH;
+        F *slot = ring + (step % ST) * NT * SLOT + warp * S * ROW;
         const long long t0 = begin + (long long)step * BT;
         const int n = (int)max(0ll, min((long long)S, g.T - (t0 + warp * S)));          // this warp's tokens of the block
-        if (n < S) close_gates<F, S>(slot, n, lane);
+        if (n < S) close_gates<F, MODE, S>(slot, n, lane);
         f2 a[S], v[S], gate[Z ? S : 1], P, hl;
         auto segment = [&](auto fast) {
             f2 range = both(0.f);
@@ -361,9 +388,9 @@ __global__ void __launch_bounds__(256, 2) k_rec_fwd(const __grid_constant__ RecA
             hl = both(0.f);
 #pragma unroll
             for (int s = 0; s < S; s++) {
-                const f2 x = pair_at(slot + 2 * SLOT, s, lane), z = Z ? pair_at(slot + 3 * SLOT, s, lane) : both(0.f);
+                const f2 x = pair_at<F, MODE>(slot + 2 * SLOT, s, lane, odd_x), z = Z ? pair_at<F, MODE>(slot + 3 * SLOT, s, lane, odd_z) : both(0.f);
                 f2 r, in, sz;
-                sigmoids<Z, decltype(fast)::value>(pair_at(slot, s, lane), pair_at(slot + SLOT, s, lane), z, r, in, sz, range);
+                sigmoids<Z, decltype(fast)::value>(pair_at<F, MODE>(slot, s, lane, odd_r), pair_at<F, MODE>(slot + SLOT, s, lane, odd_i), z, r, in, sz, range);
                 a[s] = decays(r, rate);
                 const f2 q = one_minus_square(a[s], mul2(r, x2));
                 v[s] = mul2(mul2(make_float2(sqrtf(q.x), sqrtf(q.y)), in), x);
@@ -426,7 +453,7 @@ __global__ void __launch_bounds__(256, 2) k_rec_bwd(const __grid_constant__ RecA
     pdl_wait();
     pdl_trigger();
     using G = Geo<F, true>;
-    constexpr int S = G::S, BT = G::BT, SLOT = G::SLOT, NT = 4 + Z, ST = G::STAGES, RING = ST * NT * SLOT * (int)sizeof(F);
+    constexpr int S = G::S, BT = G::BT, ROW = row_of(MODE), SLOT = G::slot(MODE), NT = 4 + Z, ST = G::STAGES, RING = ST * NT * SLOT * (int)sizeof(F);
     static_assert(BT == CKPT, "a block starts from a state that is kept");
     extern __shared__ __align__(128) unsigned char smem[];
     ExchangeBack &ex = *reinterpret_cast<ExchangeBack *>(smem + RING);
@@ -443,6 +470,11 @@ __global__ void __launch_bounds__(256, 2) k_rec_bwd(const __grid_constant__ RecA
         if (ch < g.D) E.x = g.gs_out[(size_t)b * g.D + ch];
         if (ch + 1 < g.D) E.y = g.gs_out[(size_t)b * g.D + ch + 1];
     }
+    const uint32_t odd_r = odd_rows<F, MODE, S>(g.rg, b * g.rg_batch + begin * g.rg_token + ch0, g.rg_token, warp),
+                   odd_i = odd_rows<F, MODE, S>(g.ig, b * g.ig_batch + begin * g.ig_token + ch0, g.ig_token, warp),
+                   odd_x = odd_rows<F, MODE, S>(g.x, b * g.x_batch + begin * g.x_token + ch0, g.x_token, warp),
+                   odd_z = Z ? odd_rows<F, MODE, S>(g.z, b * g.z_batch + begin * g.z_token + ch0, g.z_token, warp) : 0u,
+                   odd_g = odd_rows<F, MODE, S>(g.gy, ((long long)b * g.T + begin) * g.D + ch0, g.D, warp);
     // (k counts the steps in the order of the walk)
     if (span < g.nspan - 1) E = fold_spans(g, b, g.nspan - 1, span, -1, ch, E);
     auto start = [&](int k) {
@@ -454,7 +486,7 @@ __global__ void __launch_bounds__(256, 2) k_rec_bwd(const __grid_constant__ RecA
             for (int i = 0; i < NT; i++) sm100::tma_load_3d(slot + i * SLOT, g.in + i, ex.full + k % ST, ch0, (int)t0, b);
         } else {
             const int n = (int)max(0ll, min((long long)S, g.T - (t0 + warp * S))), left = g.D - ch0;
-            slot += warp * S * CH;
+            slot += warp * S * ROW;
             fill<F, MODE, S>(slot, (const F *)g.rg + (b * g.rg_batch + t0 * g.rg_token + ch0), (int)g.rg_token, warp, n, left, lane);
             fill<F, MODE, S>(slot + SLOT, (const F *)g.ig + (b * g.ig_batch + t0 * g.ig_token + ch0), (int)g.ig_token, warp, n, left, lane);
             fill<F, MODE, S>(slot + 2 * SLOT, (const F *)g.x + (b * g.x_batch + t0 * g.x_token + ch0), (int)g.x_token, warp, n, left, lane);
@@ -492,9 +524,9 @@ __global__ void __launch_bounds__(256, 2) k_rec_bwd(const __grid_constant__ RecA
             cp_wait<ST - 1>();
             __syncwarp();
         }
-        F *slot = ring + (k % ST) * NT * SLOT + warp * S * CH;
+        F *slot = ring + (k % ST) * NT * SLOT + warp * S * ROW;
         const int n = (int)max(0ll, min((long long)S, g.T - (t0 + warp * S)));
-        if (n < S) close_gates<F, S>(slot, n, lane);
+        if (n < S) close_gates<F, MODE, S>(slot, n, lane);
         // d = gy silu(z); e: what is left of gz without h; v = m i x.  i is m i / m, and 1 / (1 - a^2) the square of 1 / m.
         f2 a[S], r[S], mi[S], rs[S], v[S], d[S], e[Z ? S : 1], P, hl, El = both(0.f);
         auto segment = [&](auto fast) {
@@ -503,9 +535,9 @@ __global__ void __launch_bounds__(256, 2) k_rec_bwd(const __grid_constant__ RecA
             hl = both(0.f);
 #pragma unroll
             for (int s = 0; s < S; s++) {
-                const f2 z = Z ? pair_at(slot + 4 * SLOT, s, lane) : both(0.f);
+                const f2 z = Z ? pair_at<F, MODE>(slot + 4 * SLOT, s, lane, odd_z) : both(0.f);
                 f2 in, sz;
-                sigmoids<Z, decltype(fast)::value>(pair_at(slot, s, lane), pair_at(slot + SLOT, s, lane), z, r[s], in, sz, range);
+                sigmoids<Z, decltype(fast)::value>(pair_at<F, MODE>(slot, s, lane, odd_r), pair_at<F, MODE>(slot + SLOT, s, lane, odd_i), z, r[s], in, sz, range);
                 a[s] = decays(r[s], rate);
                 const f2 q = one_minus_square(a[s], mul2(r[s], x2));
                 // (where 1 - a^2 is zero, so are L and m: any factor does; a NaN stays)
@@ -514,10 +546,10 @@ __global__ void __launch_bounds__(256, 2) k_rec_bwd(const __grid_constant__ RecA
                 asm("max.NaN.f32 %0, %0, %1;" : "+f"(low.y) : "f"(1e-37f));
                 rs[s] = make_float2(rsqrta(low.x), rsqrta(low.y));
                 mi[s] = mul2(mul2(q, rs[s]), in);
-                v[s] = mul2(mi[s], pair_at(slot + 2 * SLOT, s, lane));
+                v[s] = mul2(mi[s], pair_at<F, MODE>(slot + 2 * SLOT, s, lane, odd_x));
                 hl = fma2(a[s], hl, v[s]);
                 P = mul2(P, a[s]);
-                d[s] = pair_at(slot + 3 * SLOT, s, lane);
+                d[s] = pair_at<F, MODE>(slot + 3 * SLOT, s, lane, odd_g);
                 if (Z) {
                     // silu' = s (1 + z (1 - s))
                     const f2 gs = mul2(d[s], sz);
@@ -622,7 +654,7 @@ template <typename F, bool Z, int MODE, bool BACK>
 __global__ void __launch_bounds__(256, 2) k_rec_spans(const __grid_constant__ RecArgs g) {
     pdl_wait();
     pdl_trigger();
-    constexpr int S = Geo<F, BACK>::S, NT = BACK ? 2 + Z : 3, ST = 4, SLOT = S * CH;
+    constexpr int S = Geo<F, BACK>::S, NT = BACK ? 2 + Z : 3, ST = 4, SLOT = S * row_of(MODE);
     extern __shared__ __align__(128) unsigned char smem[];
     __shared__ float4 seg[NW][32];
     __shared__ uint64_t bars[NW][ST];
@@ -637,6 +669,11 @@ __global__ void __launch_bounds__(256, 2) k_rec_spans(const __grid_constant__ Re
     const long long begin = (long long)span * g.span, end = min((long long)g.T, begin + g.span), part = g.span / NW;
     const long long from = min(end, begin + warp * part), to = min(end, from + part);
     const int nsteps = (int)((to - from + S - 1) / S);
+    const uint32_t odd_r = odd_rows<F, MODE, S>(g.rg, b * g.rg_batch + from * g.rg_token + ch0, g.rg_token, 0),
+                   odd_i = odd_rows<F, MODE, S>(g.ig, b * g.ig_batch + from * g.ig_token + ch0, g.ig_token, 0),
+                   odd_x = odd_rows<F, MODE, S>(g.x, b * g.x_batch + from * g.x_token + ch0, g.x_token, 0),
+                   odd_z = Z ? odd_rows<F, MODE, S>(g.z, b * g.z_batch + from * g.z_token + ch0, g.z_token, 0) : 0u,
+                   odd_g = odd_rows<F, MODE, S>(g.gy, ((long long)b * g.T + from) * g.D + ch0, g.D, 0);
     auto at_step = [&](int k) { return from + (long long)(BACK ? nsteps - 1 - k : k) * S; };
     auto start = [&](int k) {
         const long long t0 = at_step(k);
@@ -691,7 +728,7 @@ __global__ void __launch_bounds__(256, 2) k_rec_spans(const __grid_constant__ Re
         }
         F *slot = ring + (k % ST) * NT * SLOT;
         const int n = (int)min((long long)S, to - at_step(k));
-        if (n < S) close_gates<F, S>(slot, n, lane);
+        if (n < S) close_gates<F, MODE, S>(slot, n, lane);
         f2 a[S], v[S];
         auto gates = [&](auto fast) {
             f2 range = both(0.f);
@@ -699,15 +736,15 @@ __global__ void __launch_bounds__(256, 2) k_rec_spans(const __grid_constant__ Re
             for (int s = 0; s < S; s++) {
                 f2 r, in, sz;
                 if (!BACK) {
-                    sigmoids<false, decltype(fast)::value>(pair_at(slot, s, lane), pair_at(slot + SLOT, s, lane), both(0.f), r, in, sz, range);
+                    sigmoids<false, decltype(fast)::value>(pair_at<F, MODE>(slot, s, lane, odd_r), pair_at<F, MODE>(slot + SLOT, s, lane, odd_i), both(0.f), r, in, sz, range);
                     a[s] = decays(r, rate);
                     const f2 q = one_minus_square(a[s], mul2(r, x2));
-                    v[s] = mul2(mul2(make_float2(sqrtf(q.x), sqrtf(q.y)), in), pair_at(slot + 2 * SLOT, s, lane));
+                    v[s] = mul2(mul2(make_float2(sqrtf(q.x), sqrtf(q.y)), in), pair_at<F, MODE>(slot + 2 * SLOT, s, lane, odd_x));
                 } else {
-                    const f2 z = Z ? pair_at(slot + 2 * SLOT, s, lane) : both(0.f);
-                    sigmoids<false, decltype(fast)::value>(pair_at(slot, s, lane), z, both(0.f), r, sz, in, range);
+                    const f2 z = Z ? pair_at<F, MODE>(slot + 2 * SLOT, s, lane, odd_z) : both(0.f);
+                    sigmoids<false, decltype(fast)::value>(pair_at<F, MODE>(slot, s, lane, odd_r), z, both(0.f), r, sz, in, range);
                     a[s] = decays(r, rate);
-                    v[s] = pair_at(slot + SLOT, s, lane);
+                    v[s] = pair_at<F, MODE>(slot + SLOT, s, lane, odd_g);
                     if (Z) v[s] = mul2(v[s], mul2(z, sz));
                 }
             }
@@ -865,12 +902,12 @@ int launch_as(const RecArgs &g, int B, cudaStream_t s) {
     static unsigned char done[2][64];
     const long long chains = (long long)B * g.slabs;
     if (g.nspan > 1) {
-        const int smem = NW * 4 * (BACK ? 2 + Z : 3) * Geo<F, BACK>::S * CH * (int)sizeof(F);
+        const int smem = NW * 4 * (BACK ? 2 + Z : 3) * Geo<F, BACK>::S * row_of(MODE) * (int)sizeof(F);
         const int rc = launch_rec(k_rec_spans<F, Z, MODE, BACK>, g, chains * (g.nspan - 1), smem, done[1], s);
         if (rc != WKV_OK) return rc;
     }
-    if constexpr (BACK) return launch_rec(k_rec_bwd<F, Z, MODE>, g, chains * g.nspan, Geo<F, true>::ring(Z) + (int)sizeof(ExchangeBack), done[0], s);
-    else return launch_rec(k_rec_fwd<F, Z, MODE>, g, chains * g.nspan, Geo<F, false>::ring(Z) + (int)sizeof(Exchange), done[0], s);
+    if constexpr (BACK) return launch_rec(k_rec_bwd<F, Z, MODE>, g, chains * g.nspan, Geo<F, true>::ring(Z, MODE) + (int)sizeof(ExchangeBack), done[0], s);
+    else return launch_rec(k_rec_fwd<F, Z, MODE>, g, chains * g.nspan, Geo<F, false>::ring(Z, MODE) + (int)sizeof(Exchange), done[0], s);
 }
 // the tiles' maps; false: TMA cannot read or write these rows
 template <typename F, bool BACK>
