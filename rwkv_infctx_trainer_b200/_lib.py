@@ -115,7 +115,7 @@ EXPORTS = [
     "wkv_gated_recurrence_ckpt_bytes", "wkv_gated_recurrence_forward_workspace", "wkv_gated_recurrence_forward",
     "wkv_gated_recurrence_backward_workspace", "wkv_gated_recurrence_backward",
     "wkv_linear_saved_bytes", "wkv_linear_forward_workspace", "wkv_linear_forward", "wkv_linear_backward_workspace",
-    "wkv_linear_backward",
+    "wkv_linear_backward", "wkv_linear_selftest_abort", "wkv_gated_recurrence_selftest_abort",
 ]
 
 _lib = None
@@ -222,6 +222,10 @@ def load() -> ctypes.CDLL:
         fn = getattr(lib, f"wkv_{name}_bytes")
         fn.restype = sz
         fn.argtypes = [ctypes.POINTER(args)]
+    for name, args in (("linear", LinearArgs), ("gated_recurrence", GatedRecurrenceArgs)):
+        fn = getattr(lib, f"wkv_{name}_selftest_abort")
+        fn.restype = i
+        fn.argtypes = [ctypes.POINTER(args), i, i, ctypes.c_uint, _vp]
     for v in ("wkv5", "wkv6"):
         for d in ("forward", "backward"):
             fn = getattr(lib, f"{v}_{d}")

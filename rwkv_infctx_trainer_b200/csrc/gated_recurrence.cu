@@ -54,6 +54,11 @@ __device__ __forceinline__ float rsqrta(float x) {
 }
 __device__ __forceinline__ float sig(float x) { return rcpa(1.f + ex2a(-LOG2E_ * x)); }
 
+constexpr unsigned WAIT_LIMIT = 4000000u;
+// (what a self-test changes in the calls of its thread)
+thread_local int t_skip = -1;
+thread_local unsigned t_limit = WAIT_LIMIT;
+
 struct RecArgs {
     CUtensorMap in_spans[5];              // as `in`, the tiles of a warp
     CUtensorMap in[5], out[4];            // TILES: decay gate, input gate, x, (gy,) z; y, or gx, ginput_gate, gdecay_gate, gz
@@ -65,7 +70,8 @@ struct RecArgs {
     void *y;
     float *state_out, *ckpt;              // ckpt [B, nkept, D]: the state before every CKPT tokens
     int *status;
-    unsigned limit;
+    unsigned limit;                       // polls of a wait
+    int skip;                             // self-test: the block whose tiles are never loaded (-1)
     int nkept, pair;                      // pair: two neighbouring channels are one access in every output
     const void *gy;
     const float *gs_out;
@@ -306,11 +312,11 @@ __device__ __forceinline__ f2 fold_spans(const RecArgs &g, int b, int first, int
     return h;
 }
 
-// (after a wait that ran out: tiles may still be on their way into this CTA's shared memory)
-template <int ST, class X>
-__device__ __forceinline__ void drain_tiles(X &ex, const RecArgs &g, int nsteps) {
-    if (threadIdx.x != 0 || *(volatile int *)&ex.abort == 0) return;
-    for (int k = max(0, nsteps - ST); k < nsteps; k++) sm100::mbar_wait(ex.full + k % ST, (k / ST) & 1, g.limit);
+// After a wait that ran out tiles may still be on their way into this CTA's shared memory, and the stages' phases are no longer what their number
+// says: copies take microseconds, a millisecond is waited.
+__device__ __forceinline__ void let_copies_land(const int *abort) {
+    if (*(volatile const int *)abort == 0) return;
+    for (int i = 0; i < 100; i++) __nanosleep(10000);
 }
 
 template <typename F, bool Z, int MODE>
@@ -343,6 +349,7 @@ __global__ void __launch_bounds__(256, 2) k_rec_fwd(const __grid_constant__ RecA
         const long long t0 = begin + (long long)step * BT;
         F *slot = ring + (step % ST) * NT * SLOT;
         if constexpr (MODE == TILES) {
+            if (step == g.skip) return;
             sm100::mbar_expect_tx(ex.full + step % ST, NT * SLOT * sizeof(F));
 #pragma unroll
             for (int i = 0; i < NT; i++) sm100::tma_load_3d(slot + i * SLOT, g.in + i, ex.full + step % ST, ch0, (int)t0, b);
@@ -441,7 +448,7 @@ __global__ void __launch_bounds__(256, 2) k_rec_fwd(const __grid_constant__ RecA
         }
     }
     if (MODE == TILES && lane == 0) sm100::tma_store_wait_all();
-    if (MODE == TILES) drain_tiles<ST>(ex, g, nsteps);
+    if (MODE == TILES && threadIdx.x == 0) let_copies_land(&ex.abort);
     if (g.state_out != nullptr && warp == 0 && span == g.nspan - 1) {
         if (ch < g.D) g.state_out[(size_t)b * g.D + ch] = h.x;
         if (ch + 1 < g.D) g.state_out[(size_t)b * g.D + ch + 1] = h.y;
@@ -481,6 +488,7 @@ __global__ void __launch_bounds__(256, 2) k_rec_bwd(const __grid_constant__ RecA
         const long long t0 = begin + (long long)(nsteps - 1 - k) * BT;
         F *slot = ring + (k % ST) * NT * SLOT;
         if constexpr (MODE == TILES) {
+            if (k == g.skip) return;
             sm100::mbar_expect_tx(ex.full + k % ST, NT * SLOT * sizeof(F));
 #pragma unroll
             for (int i = 0; i < NT; i++) sm100::tma_load_3d(slot + i * SLOT, g.in + i, ex.full + k % ST, ch0, (int)t0, b);
@@ -631,7 +639,7 @@ __global__ void __launch_bounds__(256, 2) k_rec_bwd(const __grid_constant__ RecA
         }
     }
     if (MODE == TILES && lane == 0) sm100::tma_store_wait_all();
-    if (MODE == TILES) drain_tiles<ST>(ex, g, nsteps);
+    if (MODE == TILES && threadIdx.x == 0) let_copies_land(&ex.abort);
     if (g.gs_in != nullptr && warp == 0 && span == 0) {
         if (ch < g.D) g.gs_in[(size_t)b * g.D + ch] = E.x;
         if (ch + 1 < g.D) g.gs_in[(size_t)b * g.D + ch + 1] = E.y;
@@ -679,7 +687,7 @@ __global__ void __launch_bounds__(256, 2) k_rec_spans(const __grid_constant__ Re
         const long long t0 = at_step(k);
         F *slot = ring + (k % ST) * NT * SLOT;
         if constexpr (MODE == TILES) {
-            if (lane == 0) {
+            if (lane == 0 && k != g.skip) {
                 uint64_t *bar = &bars[warp][k % ST];
                 sm100::mbar_expect_tx(bar, NT * SLOT * sizeof(F));
                 sm100::tma_load_3d(slot, g.in_spans, bar, ch0, (int)t0, b);
@@ -759,8 +767,7 @@ __global__ void __launch_bounds__(256, 2) k_rec_spans(const __grid_constant__ Re
         }
     }
     if constexpr (MODE == TILES) {
-        if (lane == 0 && *(volatile int *)&abort != 0)
-            for (int k = max(0, nsteps - ST); k < nsteps; k++) sm100::mbar_wait(&bars[warp][k % ST], (k / ST) & 1, g.limit);
+        if (lane == 0) let_copies_land(&abort);
     }
     seg[warp][lane] = make_float4(P.x, P.y, h.x, h.y);
     __syncthreads();
@@ -887,7 +894,7 @@ RecArgs args_of(const wkv_gated_recurrence_args_t *a, bool back) {
     g.gs_in = a->gstate_in;
     g.spans = (float2 *)a->workspace;
     g.part = (float *)((char *)a->workspace + (back ? spans_bytes(a, true) : 0));
-    g.status = a->status; g.limit = 4000000u;
+    g.status = a->status; g.limit = t_limit; g.skip = t_skip;
     return g;
 }
 size_t ckpt_need(const wkv_gated_recurrence_args_t *a) { return (size_t)a->B * (((size_t)a->T + CKPT - 1) / CKPT) * a->D * 4; }
@@ -1009,4 +1016,14 @@ extern "C" int wkv_gated_recurrence_backward(const wkv_gated_recurrence_args_t *
     const int rc = launch_by<true>(a, g, s);
     if (rc != WKV_OK || a->gdecay == nullptr) return rc;
     return fold_params(g.part, a->B * g.nspan, a->D, out, s);
+}
+
+extern "C" int wkv_gated_recurrence_selftest_abort(const wkv_gated_recurrence_args_t *a, int backward_call, int skip_block, unsigned limit, void *stream) {
+    if (skip_block < 0 || limit < 1 || limit > 100000) return WKV_ERR_SHAPE;
+    t_skip = skip_block;
+    t_limit = limit;
+    const int rc = backward_call ? wkv_gated_recurrence_backward(a, stream) : wkv_gated_recurrence_forward(a, stream);
+    t_skip = -1;
+    t_limit = WAIT_LIMIT;
+    return rc;
 }

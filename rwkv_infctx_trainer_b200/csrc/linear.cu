@@ -23,6 +23,9 @@ namespace linear {
 namespace {
 
 constexpr unsigned WAIT_LIMIT = 4000000u;
+// (what a self-test changes in the calls of its thread)
+thread_local int t_skip = -1;
+thread_local unsigned t_limit = WAIT_LIMIT;
 
 inline long long up8(long long n) { return (n + 7) & ~7ll; }
 
@@ -389,7 +392,7 @@ int product(const Matrix (&a)[2], const Matrix (&b)[2], int a_sources, int b_sou
     g.kb = g.kb0 * (a_sources == 2 && b_sources == 2 ? 2 : 1);
     g.main = cut.main; g.rest = cut.rest; g.splits = cut.splits; g.kb_split = cut.kb_split;
     g.group = 8;
-    g.status = status; g.limit = WAIT_LIMIT;
+    g.status = status; g.limit = t_limit; g.skip = t_skip;
     g.e = e;
     g.e.part = (float *)part;
     const int b_box = PAIR ? cut.bn / 2 : cut.bn / cut.cg;
@@ -621,4 +624,14 @@ extern "C" int wkv_linear_backward(const wkv_linear_args_t *a, void *stream) {
     if (need > 0 && (a->workspace == nullptr || a->workspace_bytes < need)) return WKV_ERR_WORKSPACE;
     if (!all_aligned({a->workspace, a->saved})) return WKV_ERR_ALIGN;
     return by_16bit(a->dtype, [&](auto f) { return backward<decltype(f)>(a, Scratch{(char *)a->workspace}, nullptr, s); });
+}
+
+extern "C" int wkv_linear_selftest_abort(const wkv_linear_args_t *a, int backward_call, int skip_block, unsigned limit, void *stream) {
+    if (skip_block < 0 || limit < 1 || limit > 100000) return WKV_ERR_SHAPE;
+    t_skip = skip_block;
+    t_limit = limit;
+    const int rc = backward_call ? wkv_linear_backward(a, stream) : wkv_linear_forward(a, stream);
+    t_skip = -1;
+    t_limit = WAIT_LIMIT;
+    return rc;
 }

@@ -113,7 +113,8 @@ struct GemmArgs {
     int splits, kb_split;             // into so many parts of so many blocks: a wave of CTAs that the rest alone would not fill
     int group;                        // tiles of M that are walked together
     int *status;
-    unsigned limit;
+    unsigned limit;                   // polls of a wait
+    int skip;                         // self-test: the block of a CTA's first tile that is never loaded (-1)
     Epi e;
 };
 
@@ -390,6 +391,11 @@ __global__ void __launch_bounds__(THREADS, 1) k_gemm(const __grid_constant__ Gem
                 for (int kb = t.kb; kb < t.kb_end; kb++) {
                     ok = wait(empty + st, parity ^ 1);
                     if (!ok) break;
+                    issued++;
+                    if (kb == g.skip && i == first) {
+                        if (++st == ST) { st = 0; parity ^= 1; }
+                        continue;
+                    }
                     unsigned char *a = smem + st * T::STAGE, *b = a + T::A_BYTES;
                     const uint32_t bar = CG == 2 ? map_rank(full + st, 0) : sm100::smem_u32(full + st);
                     if (rank == 0) sm100::mbar_expect_tx(full + st, CG * T::STAGE);
@@ -410,7 +416,6 @@ __global__ void __launch_bounds__(THREADS, 1) k_gemm(const __grid_constant__ Gem
                     } else {
                         tma_2d<CG>(b, mb, bar, k0, n0);
                     }
-                    issued++;
                     if (++st == ST) { st = 0; parity ^= 1; }
                 }
             }
