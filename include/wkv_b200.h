@@ -406,7 +406,7 @@ int wkv_gated_recurrence_backward(const wkv_gated_recurrence_args_t *a, void *st
  *   mul, residual, y [rows,N] contiguous; all but the bias in `dtype`.  act: WKV_ACT_*.  Any size and alignment is
  *   taken; rows of 16-byte aligned pieces are read where they lie, others are copied into the
  *   workspace first.
- *   saved (wkv_linear_saved_bytes() bytes, or NULL): pre-activations that the forward call leaves
+ *   saved (wkv_linear_saved_bytes() bytes, or NULL): pre-activations, in fp32, that the forward call leaves
  *   for the backward call, which needs them where that is not 0 bytes.
  *   Gradients (NULL: not wanted): gx [rows,K], gw0, gw1 [N,K], gmul [rows,N] contiguous in dtype, gbias
  *   [N] in bias_dtype; that of the residual is gy.  The gradient of the pre-activation is rounded

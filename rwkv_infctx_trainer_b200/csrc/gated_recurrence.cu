@@ -25,6 +25,7 @@
 //
 // 1 - a^2 is -expm1(2L): its series below 1/4 (2^-24 of it are left out there), 1 - a a above.
 #include "elem_io.cuh"
+#include "elem_math.cuh"
 #include "sm100_primitives.cuh"
 #include "tma_host.cuh"
 #include "wkv_internal.h"
@@ -33,26 +34,11 @@ namespace wkv {
 namespace {
 
 constexpr int CH = 64, NW = 8, MAX_SPANS = 256;
-constexpr float LOG2E_ = 1.4426950408889634f, LN2_ = 0.6931471805599453f;
-// the mean error of ex2 over exponents from -0.5 to -0.01, made good in its argument (selective_scan.cu)
-constexpr float EX2_MEAN_ = 1.8e-8f;
-
-__device__ __forceinline__ float ex2a(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-__device__ __forceinline__ float rcpa(float x) {
-    float y;
-    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
 __device__ __forceinline__ float rsqrta(float x) {
     float y;
     asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
-__device__ __forceinline__ float sig(float x) { return rcpa(1.f + ex2a(-LOG2E_ * x)); }
 
 constexpr unsigned WAIT_LIMIT = 4000000u;
 // (what a self-test changes in the calls of its thread)
@@ -103,12 +89,13 @@ struct Rate {
     float rate2, x2, ratio;               // L log2(e) = rate2 r;  -2 L = x2 r;  sigmoid(p) / softplus(p)
 };
 __device__ __forceinline__ Rate rate_of(float p, float c) {
-    const float t = expf(-fabsf(p)), s = fmaxf(p, 0.f) + log1pf(t), sg = p >= 0.f ? 1.f / (1.f + t) : t / (1.f + t);
+    float sg;
+    const float s = softplus<true>(p, sg);
     Rate r;
     // (an infinite rate becomes the largest one: a decay gate of zero then keeps the state; a NaN stays)
     float k = c * s;
     asm("min.NaN.f32 %0, %0, %1;" : "+f"(k) : "f"(1.1e38f));
-    r.rate2 = -k * LOG2E_;
+    r.rate2 = -k * LOG2E;
     r.x2 = 2.f * k;
     r.ratio = s > 1e-30f ? sg / s : (s == s ? 1.f : s);
     return r;
@@ -136,41 +123,41 @@ __device__ __forceinline__ void sigmoids(f2 rg, f2 ig, f2 z, f2 &r, f2 &i, f2 &s
     f2 zero = both(0.f);
     if (!FAST) asm volatile("mov.b32 %0, 0;" : "=f"(zero.x));
     auto one_plus = [&](f2 x) {
-        const f2 e = FAST ? mul2(x, both(-LOG2E_)) : mul2(add2(x, both(zero.x)), both(-LOG2E_));
-        return add2(make_float2(ex2a(e.x), ex2a(e.y)), both(1.f));
+        const f2 e = FAST ? mul2(x, both(-LOG2E)) : mul2(add2(x, both(zero.x)), both(-LOG2E));
+        return add2(make_float2(ex2(e.x), ex2(e.y)), both(1.f));
     };
     const f2 pr = one_plus(rg), pi = one_plus(ig), ri = mul2(pr, pi);
     f2 d = ri;
     if (Z) {
         const f2 pz = one_plus(z);
         d = mul2(ri, pz);
-        const f2 inv = make_float2(rcpa(d.x), rcpa(d.y)), iz = mul2(inv, pz);
+        const f2 inv = make_float2(rcp(d.x), rcp(d.y)), iz = mul2(inv, pz);
         r = mul2(iz, pi);
         i = mul2(iz, pr);
         s = mul2(inv, ri);
     } else {
-        const f2 inv = make_float2(rcpa(d.x), rcpa(d.y));
+        const f2 inv = make_float2(rcp(d.x), rcp(d.y));
         r = mul2(inv, pi);
         i = mul2(inv, pr);
     }
     range = add2(range, d);
     if (!FAST) {
         if (!(d.x < RANGE)) {
-            r.x = sig(rg.x);
-            i.x = sig(ig.x);
-            if (Z) s.x = sig(z.x);
+            r.x = sigm(rg.x);
+            i.x = sigm(ig.x);
+            if (Z) s.x = sigm(z.x);
         }
         if (!(d.y < RANGE)) {
-            r.y = sig(rg.y);
-            i.y = sig(ig.y);
-            if (Z) s.y = sig(z.y);
+            r.y = sigm(rg.y);
+            i.y = sigm(ig.y);
+            if (Z) s.y = sigm(z.y);
         }
     }
 }
 __device__ __forceinline__ bool in_range(f2 range) { return __all_sync(0xffffffffu, range.x + range.y < RANGE); }
 __device__ __forceinline__ f2 decays(f2 r, f2 rate) {
-    const f2 e = fma2(r, rate, both(EX2_MEAN_));
-    return make_float2(ex2a(e.x), ex2a(e.y));
+    const f2 e = fma2(r, rate, both(EX2_MEAN));
+    return make_float2(ex2(e.x), ex2(e.y));
 }
 
 __device__ __forceinline__ void cp_async4(void *smem, const void *g, int valid) {
@@ -610,7 +597,7 @@ __global__ void __launch_bounds__(256, 2) k_rec_bwd(const __grid_constant__ RecA
             // G (h a L - i x a^2 L / m), i / m = m i / m^2
             const f2 gLL = mul2(Gs, sub2(mul2(hb[s], aL), mul2(mul2(mul2(v[s], rs[s]), rs[s]), mul2(a[s], aL))));
             total = add2(total, gLL);
-            const f2 gr = mul2(gLL, fma2(r[s], both(-LN2_), both(LN2_)));
+            const f2 gr = mul2(gLL, fma2(r[s], both(-LN2), both(LN2)));
             const f2 gz = Z ? mul2(e[Z ? s : 0], hb[s + 1]) : both(0.f);
             if constexpr (MODE == TILES) {
                 put_pair(slot, s, lane, gr);
@@ -651,8 +638,8 @@ __global__ void __launch_bounds__(256, 2) k_rec_bwd(const __grid_constant__ RecA
 #pragma unroll
             for (int w = 1; w < NW; w++) total = add2(total, ex.sum[w][lane]);
             float *p = g.part + ((size_t)b * g.nspan + span) * g.D + ch;
-            if (ch < g.D) p[0] = total.x * (LN2_ * k0.ratio);
-            if (ch + 1 < g.D) p[1] = total.y * (LN2_ * k1.ratio);
+            if (ch < g.D) p[0] = total.x * (LN2 * k0.ratio);
+            if (ch + 1 < g.D) p[1] = total.y * (LN2 * k1.ratio);
         }
     }
 }
@@ -809,13 +796,13 @@ __global__ void __launch_bounds__(128) k_rec_step(const RecArgs g, long long pai
     if (g.state_in != nullptr) h = make_float2(g.state_in[at], n > 1 ? g.state_in[at + 1] : 0.f);
     auto one = [&](float h, float x, float ig, float rg, float p) {
         const Rate k = rate_of(p, g.c);
-        const float r = sig(rg), a = ex2a(fmaf(r, k.rate2, EX2_MEAN_)), m = sqrtf(one_minus_square(both(a), both(r * k.x2)).x);
-        return fmaf(a, h, m * sig(ig) * x);
+        const float r = sigm(rg), a = ex2(fmaf(r, k.rate2, EX2_MEAN)), m = sqrtf(one_minus_square(both(a), both(r * k.x2)).x);
+        return fmaf(a, h, m * sigm(ig) * x);
     };
     h = make_float2(one(h.x, x.x, ig.x, rg.x, g.decay[ch]), n > 1 ? one(h.y, x.y, ig.y, rg.y, g.decay[ch + 1]) : 0.f);
     g.state_out[at] = h.x;
     if (n > 1) g.state_out[at + 1] = h.y;
-    if (g.z != nullptr) h = mul2(h, mul2(z, make_float2(sig(z.x), sig(z.y))));
+    if (g.z != nullptr) h = mul2(h, mul2(z, make_float2(sigm(z.x), sigm(z.y))));
     store_out((F *)g.y + at, 0u, h, vec, n);
 }
 

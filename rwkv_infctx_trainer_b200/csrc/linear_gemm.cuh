@@ -89,7 +89,7 @@ struct Epi {
     const void *mul, *residual;       // [M,N]
     void *y[2];                       // [M,N] of each source of rows (the second: the gradient of a second matrix)
     long long y_row;                  // their row stride, and that of mul and residual
-    void *z[2];                       // pre-activations (or NULL)
+    float *z[2];                      // pre-activations (or NULL)
     long long z_row;
     float *part;                      // sums of parts of a contraction: [tile][part][row of the tile][column of the tile]
 };
@@ -278,6 +278,15 @@ struct Finish {
             if (ok && n > 0) Elem<F>::st((F *)p + at, f[0]);
         }
     }
+    __device__ __forceinline__ void keep(float *p, const float (&f)[W], bool ok, int n) const {
+        if (!ok || n <= 0) return;
+        if constexpr (W == 8) {
+            *reinterpret_cast<float4 *>(p) = make_float4(f[0], f[1], f[2], f[3]);
+            *reinterpret_cast<float4 *>(p + 4) = make_float4(f[4], f[5], f[6], f[7]);
+        } else {
+            *p = f[0];
+        }
+    }
     __device__ __forceinline__ void finish(const Epi &e, int src, long long row, int rows, int col, int n, const bool (&ok)[R], float (&f)[R][W],
                                            const float (&u)[R][W], const float (&bias)[W]) {
         if (EPI == EPI_LINEAR && e.bias != nullptr) {
@@ -290,8 +299,8 @@ struct Finish {
 #pragma unroll
             for (int k = 0; k < R; k++) {
                 const long long at = (row + k * rows) * e.z_row + col;
-                put(e.z[0], at, f[k], ok[k], n);
-                if (EPI == EPI_GATED) put(e.z[1], at, u[k], ok[k], n);
+                keep(e.z[0] + at, f[k], ok[k], n);
+                if (EPI == EPI_GATED) keep(e.z[1] + at, u[k], ok[k], n);
             }
         }
         act_values(e.act, f);

@@ -33,21 +33,14 @@
 // states and decays do not fit: 12 warps of 165 registers 1785 us a pass where 8 of 254 took 1680), nor did a quarter of the
 // exponentials on the multiply-add pipe (prompts 2 % faster, nothing else).
 #include "elem_io.cuh"
+#include "elem_math.cuh"
 #include "wkv_internal.h"
 
 namespace wkv {
 namespace {
 
 constexpr int TB = 16;               // tokens of a block
-// (log2(e) as the sum of two floats)
-constexpr float LOG2E = 1.4426950408889634f, LOG2E_LOW = 1.9259629911266175e-8f, LN2 = 0.6931471805599453f, EX2_MEAN = 1.8e-8f;
 constexpr unsigned FULL_MASK = 0xffffffffu;
-
-__device__ __forceinline__ float ex2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
 
 struct ScanArgs {
     int B, T, D, N, G, Dg, softplus;
@@ -65,46 +58,6 @@ struct ScanArgs {
     float *gs_in;
     float *part_bc, *part;                       // [ncb, B, T, G, 8 LPC]; [B * nspan, D (N + 2)]
 };
-
-__device__ __forceinline__ float rcp(float x) {
-    float y;
-    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-// e^x for x from -126 to 0: the rounding of the exponent x log2(e), up to 2^-24 of it, is made good, and so is the mean error of ex2,
-// -5e-8 over exponents below -1 (above them it is -2e-8 and less: 3e-8 too much is added there, half a rounding)
-__device__ __forceinline__ float exp_near(float x) {
-    const float e = LOG2E * x, lo = fmaf(LOG2E, x, -e) + LOG2E_LOW * x, t = ex2(e);
-    return fmaf(t, fmaf(lo, LN2, 5e-8f), t);
-}
-__device__ __forceinline__ float sigm(float x) { return rcp(1.f + ex2(-LOG2E * x)); }
-
-// softplus(x) = max(x, 0) + log(1 + t), t = e^-|x|, and with SIG its derivative sigmoid(x), for any x: no term overflows.
-// log(1 + t) = 2 artanh(s), s = t / (2 + t) <= 1/3: its power series up to s^13 is short of it by less than 2 s^15 / (15 (1 - s^2)), at
-// most 1.05e-8 or a relative 1.5e-8, and keeps the digits of small steps (log of a rounded 1 + t does not).
-template <bool SIG>
-__device__ __forceinline__ float softplus(float x, float &sig) {
-    float ax = -fabsf(x), s;
-    asm("max.NaN.f32 %0, %0, %1;" : "+f"(ax) : "f"(-126.f));        // (infinities; a NaN stays)
-    const float t = exp_near(ax);
-    if (SIG) {
-        const float w = rcp((1.f + t) * (2.f + t)), r = (2.f + t) * w;       // r = 1 / (1 + t)
-        s = t * (1.f + t) * w;
-        sig = x >= 0.f ? r : t * r;
-    } else {
-        s = t * rcp(2.f + t);
-    }
-    const float s2 = s * s;
-    float p = 1.f / 13.f;
-    p = p * s2 + 1.f / 11.f;
-    p = p * s2 + 1.f / 9.f;
-    p = p * s2 + 1.f / 7.f;
-    p = p * s2 + 1.f / 5.f;
-    p = p * s2 + 1.f / 3.f;
-    p = p * s2 + 1.f;
-    // (fmaxf drops a NaN, s brings it back)
-    return fmaxf(x, 0.f) + 2.f * s * p;
-}
 
 template <bool SIG, int PT>
 __device__ __forceinline__ void softplus_all(f2 (&x)[PT], f2 (&sig)[PT]) {
@@ -260,7 +213,6 @@ __device__ __forceinline__ void load_decays(const float *A, size_t at, int n0, i
 #pragma unroll
     for (int i = 0; i < 2; i++) A2[i] = make_float2(decay_rate(A2[i].x), decay_rate(A2[i].y));
 }
-__device__ __forceinline__ f2 ex2(f2 x) { return make_float2(ex2(x.x), ex2(x.y)); }
 // The exponent of a token's decay, dt A log2(e), and a little: ex2 gives too little on average, by 1.9e-8 of it for exponents from
 // -0.5 to -0.01 and by 0.6e-8 from -0.001 to 0 (by 5e-8 below -1, where a state is soon forgotten), which over the memory of a state
 // adds up.  1.8e-8 more in the exponent, 1.25e-8 of the power, leaves -0.7e-8 and 0.7e-8, and ex2 of it alone is 1 (tokens behind a row's

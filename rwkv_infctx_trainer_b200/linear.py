@@ -14,7 +14,8 @@ activation: ``"none"``, ``"silu"`` (z sigmoid(z)), ``"gelu"`` (z Phi(z), with th
 
 x, the matrices, mul, residual and y in bf16 or fp16 (of one type within a call; fp32 is refused: the tensor cores would take it
 at 10 bits).  Sums, bias, activation, product and residual are in fp32 and rounded once.  For the backward pass the
-pre-activations are kept in x's type; their gradient is rounded to that type once, as an operand of the products.  Any size and
+pre-activations are kept in fp32 (where an activation or ``mul`` needs them); their gradient is rounded to x's type once, as an operand of the
+products (the bias' gradient is summed before that).  Any size and
 alignment is taken; rows whose length or stride is no multiple of 8 elements are copied first, except for up to 16 rows of x, which are
 read where they lie.
 """

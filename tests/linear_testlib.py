@@ -5,7 +5,7 @@ core cuts off where it does not round) of the terms' absolute values.  A sigmoid
 exponent's product 2|z|, the exponential, the sum, the quotient and the products behind it 16), Phi(z) through erfc by z^2 + 2|z| + 24
 (erfc 8 steps and its argument's rounding, which its slope carries z^2 times).  An error of z moves an activation by at most its largest
 slope (1.13 for gelu, 1.1 for silu, 1/4 for the sigmoid, 2|z| for the squared ReLU), its derivative by at most its largest curvature
-(0.8, 0.5, 0.1 and 2).  The pre-activation that is kept, the gradient of it that the products take and every output are rounded to
+(0.8, 0.5, 0.1 and 2).  The pre-activation is kept in fp32; the gradient of it that the products take and every output are rounded to
 the type: half a step of it, and half the smallest subnormal."""
 import math
 
@@ -75,7 +75,7 @@ def linear_ref(x, w, bias, name, mul, res, gy=None):
     if gy is None:
         return out
     kept = name != "none" or mul is not None
-    dz = ez + h * (z.abs() + ez) + least(dt) if kept else 0 * z                   # of the z that the backward pass sees
+    dz = ez if kept else 0 * z
     _, da = act(name, z)
     _, s2, rel = slopes(name, z, dz)
     gz = gy * m * da
@@ -99,7 +99,7 @@ def gated_ref(x, wg, wu, name, gy=None):
     out = {"y": (a * u, ea * (u.abs() + eu) + a.abs() * eu + 2 * U * (a * u).abs())}
     if gy is None:
         return out
-    dg, du = eg + h * (g.abs() + eg) + least(dt), eu + h * (u.abs() + eu) + least(dt)
+    dg, du = eg, eu
     a, ea = values(name, g, dg)
     _, da = act(name, g)
     _, s2, rel = slopes(name, g, dg)

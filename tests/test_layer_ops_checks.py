@@ -197,13 +197,13 @@ def test_error_codes_of_the_products(memory):
     a.bias = None
     assert fwd(ref(a), None) == 1                               # its second matrix
     a.w1 = at
-    assert lib.wkv_linear_saved_bytes(ref(a)) == 2 * 768        # [40, 8] of 2 bytes, twice, each rounded up to 256
-    a.saved, a.saved_bytes = at, 1500
+    assert lib.wkv_linear_saved_bytes(ref(a)) == 2 * 1280       # [40, 8] of 4 bytes, twice
+    a.saved, a.saved_bytes = at, 2500
     assert fwd(ref(a), None) == 5 and bwd(ref(a), None) == 5
     a.saved = None
     assert bwd(ref(a), None) == 5
     a.pair, a.act, a.w1 = 0, 1, None
-    assert lib.wkv_linear_saved_bytes(ref(a)) == 768 and bwd(ref(a), None) == 5
+    assert lib.wkv_linear_saved_bytes(ref(a)) == 1280 and bwd(ref(a), None) == 5
     a.act, a.gw1 = 0, at
     assert lib.wkv_linear_saved_bytes(ref(a)) == 0 and bwd(ref(a), None) == 1
     a.gw1, a.x, a.x_row = None, at + 2, 25                      # rows that are copied first need a workspace
