@@ -29,6 +29,29 @@ thread_local unsigned t_limit = WAIT_LIMIT;
 
 inline long long up8(long long n) { return (n + 7) & ~7ll; }
 
+// 8 elements from any address (the first n of them): in words, which lie in the allocation of the elements that are in them
+template <typename F>
+__device__ __forceinline__ void load_any(Raw<F, 8> &r, const F *p, int n) {
+    if (n < 8) {
+        r.load(p, false, n);
+        return;
+    }
+    const uintptr_t at = reinterpret_cast<uintptr_t>(p);
+    const uint32_t *q = reinterpret_cast<const uint32_t *>(at & ~(uintptr_t)3);
+    uint32_t w[5];
+#pragma unroll
+    for (int i = 0; i < 4; i++) w[i] = q[i];
+    const bool odd = at & 2;
+    w[4] = odd ? q[4] : 0u;
+#pragma unroll
+    for (int i = 0; i < 4; i++) r.w[i] = odd ? __funnelshift_r(w[i], w[i + 1], 16) : w[i];
+}
+template <bool VEC, typename F>
+__device__ __forceinline__ void load_piece(Raw<F, 8> &r, const F *p, int n) {
+    if (VEC) r.load(p, true, 8);
+    else load_any(r, p, n);
+}
+
 // ------------------------------------------------------------------------------------------ few rows
 // A CTA has 16 rows of the matrix (of a pair: 8 of each), its 4 or 8 warps runs of 256 contraction steps in turn; the warps' sums meet
 // in shared memory in a fixed order.  mma.sync with the matrix as the 16-row operand and the rows of x as the 8 columns: the
@@ -87,15 +110,15 @@ __global__ void __launch_bounds__(32 * FEW_WARPS) k_few_rows(const FewArgs g) {
             for (int h = 0; h < 2; h++) {
                 const int k = k0 + s * 64 + h * 32 + c * 8, n = whole ? 8 : min(8, g.K - k);
                 if (whole || n > 0) {
-                    a[s][0][h].load(w0 + k, VEC, n);
-                    a[s][1][h].load(w1 + k, VEC, n);
+                    load_piece<VEC>(a[s][0][h], w0 + k, n);
+                    load_piece<VEC>(a[s][1][h], w1 + k, n);
                 } else {
                     a[s][0][h].zero();
                     a[s][1][h].zero();
                 }
 #pragma unroll
                 for (int j = 0; j < NT; j++) {
-                    if (live[j] && (whole || n > 0)) b[s][j][h].load(x[j] + k, VEC, n);
+                    if (live[j] && (whole || n > 0)) load_piece<VEC>(b[s][j][h], x[j] + k, n);
                     else b[s][j][h].zero();
                 }
             }
@@ -232,10 +255,10 @@ __global__ void __launch_bounds__(256) k_grad_act(const GradArgs g) {
                 rm[k].zero();
                 if (PAIR) ru[PAIR ? k : 0].zero();
                 if (!ok[k]) continue;
-                ry[k].load((const F *)g.gy + at * g.N + col, VEC, n);
+                load_piece<VEC>(ry[k], (const F *)g.gy + at * g.N + col, n);
                 if (g.z[0] != nullptr) rz[k].load(g.z[0] + at * g.z_row + col, whole, n);
                 if (PAIR) ru[PAIR ? k : 0].load(g.z[1] + at * g.z_row + col, whole, n);
-                else if (g.mul != nullptr) rm[k].load((const F *)g.mul + at * g.N + col, VEC, n);
+                else if (g.mul != nullptr) load_piece<VEC>(rm[k], (const F *)g.mul + at * g.N + col, n);
             }
 #pragma unroll
             for (int k = 0; k < R; k++) {
@@ -281,19 +304,25 @@ __global__ void __launch_bounds__(256) k_grad_act(const GradArgs g) {
     }
 }
 
-// rows that do not lie in whole 16-byte pieces -> rows that do
+// rows that do not lie in whole 16-byte pieces -> rows that do; up to three matrices (blockIdx.y)
+struct RepackArgs {
+    struct One {
+        const void *from;
+        void *to;
+        long long rows, cols, from_row, to_row;
+    } m[3];
+};
 template <typename F>
-__global__ void __launch_bounds__(256) k_repack(const F *from, long long from_row, F *to, long long to_row, long long rows, int cols) {
+__global__ void __launch_bounds__(256) k_repack(const RepackArgs g) {
     pdl_wait();
     pdl_trigger();
-    const int pieces = (cols + 7) / 8;
-    const long long total = rows * pieces;
+    const RepackArgs::One &m = g.m[blockIdx.y];
+    const long long pieces = (m.cols + 7) / 8, total = m.rows * pieces;
     for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < total; i += (long long)gridDim.x * 256) {
-        const long long row = i / pieces;
-        const int col = (int)(i - row * pieces) * 8;
+        const long long row = i / pieces, col = (i - row * pieces) * 8;
         Raw<F, 8> r;
-        r.load(from + row * from_row + col, false, cols - col);
-        r.store(to + row * to_row + col, true, 8);
+        load_any(r, (const F *)m.from + row * m.from_row + col, (int)min(8ll, m.cols - col));
+        r.store((F *)m.to + row * m.to_row + col, true, 8);
     }
 }
 
@@ -303,13 +332,6 @@ struct Matrix {
     long long rows, cols, pitch;
 };
 inline bool tma_ready(const void *p, long long pitch) { return aligned16(p) && pitch % 8 == 0 && pitch < (1ll << 38); }
-
-template <typename F>
-int repack(const Matrix &from, void *to, cudaStream_t s) {
-    const long long pitch = up8(from.cols), pieces = from.rows * (pitch / 8);
-    const unsigned grid = (unsigned)std::min<long long>((pieces + 255) / 256, 148 * 16);
-    return launch_chained(k_repack<F>, dim3(grid), dim3(256), 0, s, (const F *)from.p, from.pitch, (F *)to, pitch, from.rows, (int)from.cols);
-}
 
 // Scratch, handed out in order; with a NULL base only counted.
 struct Scratch {
@@ -426,16 +448,24 @@ bool few(const wkv_linear_args_t *a) { return a->rows <= FEW_ROWS; }
 Matrix x_of(const wkv_linear_args_t *a) { return {a->x, a->rows, a->K, a->x_row}; }
 Matrix w_of(const wkv_linear_args_t *a, int i) { return {i ? a->w1 : a->w0, a->N, a->K, i ? a->w1_row : a->w0_row}; }
 
-// `m` where TMA can read it, else a copy in the scratch
+// The matrices where TMA can read them, else copies in the scratch.
 template <typename F>
-int ready(Matrix &m, Scratch &ws, cudaStream_t s) {
-    if (tma_ready(m.p, m.pitch)) return WKV_OK;
-    void *to = ws.take((size_t)m.rows * up8(m.cols) * 2);
-    if (ws.base == nullptr) return WKV_OK;
-    const int rc = repack<F>(m, to, s);
-    m.p = to;
-    m.pitch = up8(m.cols);
-    return rc;
+int ready(std::initializer_list<Matrix *> ms, Scratch &ws, cudaStream_t s) {
+    RepackArgs r = {};
+    int n = 0;
+    long long most = 0;
+    for (Matrix *m : ms) {
+        if (tma_ready(m->p, m->pitch)) continue;
+        const long long pitch = up8(m->cols);
+        void *to = ws.take((size_t)m->rows * pitch * 2);
+        r.m[n++] = {m->p, to, m->rows, m->cols, m->pitch, pitch};
+        most = std::max(most, m->rows * (pitch / 8));
+        if (ws.base == nullptr) continue;
+        m->p = to;
+        m->pitch = pitch;
+    }
+    if (n == 0 || ws.base == nullptr) return WKV_OK;
+    return launch_chained(k_repack<F>, dim3((unsigned)std::min<long long>((most + 255) / 256, 148 * 16), (unsigned)n), dim3(256), 0, s, r);
 }
 
 Epi epilogue_of(const wkv_linear_args_t *a) {
@@ -480,8 +510,7 @@ int forward(const wkv_linear_args_t *a, Scratch ws, size_t *need, cudaStream_t s
         if (a->rows <= 8) return a->pair ? go(std::true_type{}, N8{}) : go(std::false_type{}, N8{});
         return a->pair ? go(std::true_type{}, N16{}) : go(std::false_type{}, N16{});
     }
-    int rc = ready<F>(x, ws, s);
-    for (int i = 0; i <= a->pair && rc == WKV_OK; i++) rc = ready<F>(w[i], ws, s);
+    const int rc = a->pair ? ready<F>({&x, &w[0], &w[1]}, ws, s) : ready<F>({&x, &w[0]}, ws, s);
     if (rc != WKV_OK) return rc;
     const Cut cut = cut_for(a->rows, a->N, 1, (int)((a->K + KB - 1) / KB), a->pair);
     if (count) {
@@ -501,7 +530,7 @@ int backward(const wkv_linear_args_t *a, Scratch ws, size_t *need, cudaStream_t 
     const bool products = a->gx != nullptr || a->gw0 != nullptr || a->gw1 != nullptr;
     // gz: gy itself where nothing stands between them
     const bool act = keeps(a), own_gz = products && (act || !tma_ready(a->gy, a->N));
-    const int rows_per = (int)std::max<long long>(64, ((a->rows * ((a->N + 255) / 256) + 148 * 8 - 1) / (148 * 8) + 7) / 8 * 8);
+    const int rows_per = (int)std::max<long long>(16, ((a->rows * ((a->N + 255) / 256) + 148 * 8 - 1) / (148 * 8) + 7) / 8 * 8);
     const int row_blocks = (int)((a->rows + rows_per - 1) / rows_per);
     GradArgs ga = {};
     ga.rows = a->rows; ga.N = (int)a->N; ga.act = a->act; ga.rows_per = rows_per;
@@ -539,7 +568,7 @@ int backward(const wkv_linear_args_t *a, Scratch ws, size_t *need, cudaStream_t 
     size_t most = 0;
     if (a->gx != nullptr) {
         Matrix w[2] = {w_of(a, 0), w_of(a, a->pair)};
-        for (int i = 0; i <= a->pair && rc == WKV_OK; i++) rc = ready<F>(w[i], ws, s);
+        rc = a->pair ? ready<F>({&w[0], &w[1]}, ws, s) : ready<F>({&w[0]}, ws, s);
         const Cut cut = cut_for(a->rows, a->K, 1, kb_n, false);
         most = std::max(most, align256(cut.part_bytes()));
         if (!count && rc == WKV_OK) {
@@ -552,7 +581,7 @@ int backward(const wkv_linear_args_t *a, Scratch ws, size_t *need, cudaStream_t 
     }
     if (rc == WKV_OK && (a->gw0 != nullptr || a->gw1 != nullptr)) {
         Matrix x = x_of(a);
-        rc = ready<F>(x, ws, s);
+        rc = ready<F>({&x}, ws, s);
         const Matrix xs[2] = {x, x};
         const bool both = a->gw0 != nullptr && a->gw1 != nullptr;
         const Cut cut = cut_for(a->N, a->K, 1 + both, kb_r, false);
