@@ -8,19 +8,25 @@
 //   gL L = G (h_{t-1} a L - i x a^2 L / m),  gdecay_gate = gL L (1 - r),  gdecay = sum_t gL L  sigmoid(decay) / softplus(decay)
 //   (dm/dL = -a^2 / m has no bound where a is near 1; L dm/dL goes to zero there, and only that product is formed)
 //
-// Bound by HBM: five elements a token and channel forward (two fewer... none are read twice), nine and four backward.  A CTA
-// owns 64 channels of a row (two a lane) and walks over its tokens in blocks of 8 warps x S tokens.  A warp's S tokens are a
+// A CTA owns 64 channels of a row (two a lane) and walks over its tokens in blocks of 8 warps x S tokens.  A warp's S tokens are a
 // segment: from zero its state is hl and its decay P = prod a; the eight segments' (P, hl) meet in shared memory, every thread
 // folds them in order (one barrier a block) and runs its segment again from the state that it then knows, its a and m i x still
-// in registers.  So the serial chain is 8 + S steps a block, and the gates, which are most of the work, are formed once.
-// A warp's inputs come through a ring of its own in shared memory (cp.async), the blocks behind on their way meanwhile.
+// in registers.  So the serial chain is 8 + S steps a block, the gates, which are most of the work, are formed once, and every input
+// is read once.  TMA brings a block's tile of each tensor into a ring in shared memory, blocks ahead, and takes the outputs from there, from the places of
+// inputs that are in registers by then; rows that are not made of 16-byte pieces are copied by their warps (cp.async, in words).
+//
+// What bounds it (4 x 4096 x 4096 in bf16 with z, two CTAs of 256 threads an SM): forward 166 us (4.0 TB/s; the bytes take 103 at the copy
+// rate), backward 284 (4.2; 185).  No single resource: special functions are busy for 63 % of the time on an SM with two CTAs (6 a token and
+// channel: 4 exponentials, a root, and one reciprocal for the three sigmoids; one each took 217 us), issue 55 %, HBM 62 %; 256 CTAs are 1.73 an SM.
+// Segments of 4 tokens instead of 8: 185 and 306 (folds and barriers twice as often).  Registers are what limits the segment: what does not
+// fit waits for L2 (forward 475 us with 40 bytes a thread of that), so that backward d and e go to shared memory, into the places of the gates.
 //
 // Few chains: a row is cut into spans that run in parallel.  A first pass leaves what a span does to the state (its decay and its state
 // from zero; backward: to E), without a barrier: its warps take an eighth of a span each.  The full pass starts from the fold of the
 // spans before it.  (A cluster's CTAs on neighbouring blocks of a row, their folds exchanged through distributed shared memory at
 // every step, read nothing twice, and took 2 us a step more: 4 x 4096 x 4096 forward 258 us with two CTAs a cluster, 165 without.)
 //
-// Backward: blocks in reverse.  The forward pass leaves the state before each block (4 bytes a channel per 8 S tokens); hl and
+// Backward: blocks in reverse.  The forward pass leaves the state before each block (4 bytes a channel per 64 tokens, of fp32 32); hl and
 // P are formed again, and with them the segment's E from zero, so that one exchange serves both directions.
 //
 // 1 - a^2 is -expm1(2L): its series below 1/4 (2^-24 of it are left out there), 1 - a a above.
@@ -54,7 +60,7 @@ struct RecArgs {
     long long x_batch, x_token, ig_batch, ig_token, rg_batch, rg_token, z_batch, z_token;
     const float *decay, *state_in;
     void *y;
-    float *state_out, *ckpt;              // ckpt [B, nkept, D]: the state before every CKPT tokens
+    float *state_out, *ckpt;              // ckpt [B, nkept, D]: the state before every ckpt_tokens()
     int *status;
     unsigned limit;                       // polls of a wait
     int skip;                             // self-test: the block whose tiles are never loaded (-1)
@@ -77,12 +83,13 @@ __host__ __device__ constexpr int row_of(int mode) { return mode == ANYWHERE ? C
 // does not would wait for L2 (shared memory leaves no L1).
 template <typename F, bool BACK>
 struct Geo {
-    static constexpr int S = sizeof(F) == 2 && !BACK ? 8 : 4, BT = NW * S;
+    static constexpr int S = sizeof(F) == 2 ? 8 : 4, BT = NW * S;
     static __host__ __device__ constexpr int slot(int mode) { return BT * row_of(mode); }                             // elements of one tensor's block
-    static constexpr int STAGES = sizeof(F) == 4 && BACK ? 2 : 3;
+    static constexpr int STAGES = BACK ? 2 : 3;
     static constexpr int ring(bool z, int mode) { return STAGES * (3 + BACK + z) * slot(mode) * (int)sizeof(F); }
 };
-constexpr int CKPT = 32;                  // tokens between two states that are kept: a block of the backward pass
+// tokens between two states that are kept: a block of the backward pass
+__host__ __device__ constexpr int ckpt_tokens(int elem) { return elem == 2 ? 64 : 32; }
 
 // softplus(p) and its derivative over it, once per CTA and channel
 struct Rate {
@@ -222,6 +229,23 @@ __device__ __forceinline__ f2 pair_at(const F *slot, int s, int lane, uint32_t o
     float f[2];
     r.get(f);
     return make_float2(f[0], f[1]);
+}
+// Two fp32 values of a lane in the places of two tensors' pairs that it no longer needs.
+template <typename F, int MODE>
+__device__ __forceinline__ void keep_pair(F *slot, F *other, int s, int lane, f2 v) {
+    const int at = s * row_of(MODE) + 2 * lane;
+    if constexpr (sizeof(F) == 4) {
+        *reinterpret_cast<f2 *>(slot + at) = v;
+    } else {
+        *reinterpret_cast<float *>(slot + at) = v.x;
+        *reinterpret_cast<float *>(other + at) = v.y;
+    }
+}
+template <typename F, int MODE>
+__device__ __forceinline__ f2 kept_pair(const F *slot, const F *other, int s, int lane) {
+    const int at = s * row_of(MODE) + 2 * lane;
+    if constexpr (sizeof(F) == 4) return *reinterpret_cast<const f2 *>(slot + at);
+    else return make_float2(*reinterpret_cast<const float *>(slot + at), *reinterpret_cast<const float *>(other + at));
 }
 // decay gates of minus infinity for the tokens behind the row's last: they keep the state (x is zero there)
 template <typename F, int MODE, int S>
@@ -407,8 +431,10 @@ __global__ void __launch_bounds__(256, 2) k_rec_fwd(const __grid_constant__ RecA
             if (w == warp) hs = h;
             h = fma2(make_float2(q.x, q.y), h, make_float2(q.z, q.w));
         }
-        if (g.ckpt != nullptr && warp * S % CKPT == 0 && n > 0) {
-            float *c = g.ckpt + ((size_t)b * g.nkept + (t0 + warp * S) / CKPT) * g.D + ch;
+        constexpr int CKPT = ckpt_tokens(sizeof(F));
+        static_assert(BT == CKPT, "the state before a block is kept");
+        if (g.ckpt != nullptr && warp == 0) {
+            float *c = g.ckpt + ((size_t)b * g.nkept + t0 / CKPT) * g.D + ch;
             if (ch < g.D) c[0] = hs.x;
             if (ch + 1 < g.D) c[1] = hs.y;
         }
@@ -448,6 +474,7 @@ __global__ void __launch_bounds__(256, 2) k_rec_bwd(const __grid_constant__ RecA
     pdl_trigger();
     using G = Geo<F, true>;
     constexpr int S = G::S, BT = G::BT, ROW = row_of(MODE), SLOT = G::slot(MODE), NT = 4 + Z, ST = G::STAGES, RING = ST * NT * SLOT * (int)sizeof(F);
+    constexpr int CKPT = ckpt_tokens(sizeof(F));
     static_assert(BT == CKPT, "a block starts from a state that is kept");
     extern __shared__ __align__(128) unsigned char smem[];
     ExchangeBack &ex = *reinterpret_cast<ExchangeBack *>(smem + RING);
@@ -522,17 +549,19 @@ __global__ void __launch_bounds__(256, 2) k_rec_bwd(const __grid_constant__ RecA
         F *slot = ring + (k % ST) * NT * SLOT + warp * S * ROW;
         const int n = (int)max(0ll, min((long long)S, g.T - (t0 + warp * S)));
         if (n < S) close_gates<F, MODE, S>(slot, n, lane);
-        // d = gy silu(z); e: what is left of gz without h; v = m i x.  i is m i / m, and 1 / (1 - a^2) the square of 1 / m.
-        f2 a[S], r[S], mi[S], rs[S], v[S], d[S], e[Z ? S : 1], P, hl, El = both(0.f);
+        // i is m i / m, and 1 / (1 - a^2) the square of 1 / m.
+        f2 a[S], r[S], mi[S], rs[S], sz[Z ? S : 1], P, hl, El = both(0.f);
         auto segment = [&](auto fast) {
             f2 range = both(0.f);
             P = both(1.f);
             hl = both(0.f);
 #pragma unroll
             for (int s = 0; s < S; s++) {
+                // (loads of all tokens at once would need registers that there are not: 200 bytes a thread went to L2)
+                if (s % 2 == 0) __syncwarp();
                 const f2 z = Z ? pair_at<F, MODE>(slot + 4 * SLOT, s, lane, odd_z) : both(0.f);
-                f2 in, sz;
-                sigmoids<Z, decltype(fast)::value>(pair_at<F, MODE>(slot, s, lane, odd_r), pair_at<F, MODE>(slot + SLOT, s, lane, odd_i), z, r[s], in, sz, range);
+                f2 in;
+                sigmoids<Z, decltype(fast)::value>(pair_at<F, MODE>(slot, s, lane, odd_r), pair_at<F, MODE>(slot + SLOT, s, lane, odd_i), z, r[s], in, sz[Z ? s : 0], range);
                 a[s] = decays(r[s], rate);
                 const f2 q = one_minus_square(a[s], mul2(r[s], x2));
                 // (where 1 - a^2 is zero, so are L and m: any factor does; a NaN stays)
@@ -541,22 +570,28 @@ __global__ void __launch_bounds__(256, 2) k_rec_bwd(const __grid_constant__ RecA
                 asm("max.NaN.f32 %0, %0, %1;" : "+f"(low.y) : "f"(1e-37f));
                 rs[s] = make_float2(rsqrta(low.x), rsqrta(low.y));
                 mi[s] = mul2(mul2(q, rs[s]), in);
-                v[s] = mul2(mi[s], pair_at<F, MODE>(slot + 2 * SLOT, s, lane, odd_x));
-                hl = fma2(a[s], hl, v[s]);
+                hl = fma2(a[s], hl, mul2(mi[s], pair_at<F, MODE>(slot + 2 * SLOT, s, lane, odd_x)));
                 P = mul2(P, a[s]);
-                d[s] = pair_at<F, MODE>(slot + 3 * SLOT, s, lane, odd_g);
-                if (Z) {
-                    // silu' = s (1 + z (1 - s))
-                    const f2 gs = mul2(d[s], sz);
-                    d[s] = mul2(gs, z);
-                    e[s] = mul2(gs, fma2(z, sub2(both(1.f), sz), both(1.f)));
-                }
             }
             return in_range(range);
         };
         if (!segment(std::true_type{})) segment(std::false_type{});
+        __syncwarp();
+        // d = gy silu(z), and e, what is left of gz without h, go where the gates, gy and z were
 #pragma unroll
-        for (int s = S - 1; s >= 0; s--) El = mul2(a[s], add2(d[s], El));
+        for (int s = S - 1; s >= 0; s--) {
+            __syncwarp();             // (ANYWHERE: a neighbour reads this lane's words.  All: loads moved up would need registers that there are not)
+            f2 d = pair_at<F, MODE>(slot + 3 * SLOT, s, lane, odd_g);
+            if (Z) {
+                // silu' = s (1 + z (1 - s))
+                const f2 z = pair_at<F, MODE>(slot + 4 * SLOT, s, lane, odd_z), gs = mul2(d, sz[Z ? s : 0]);
+                d = mul2(gs, z);
+                if (MODE == ANYWHERE) __syncwarp();
+                keep_pair<F, MODE>(slot + 4 * SLOT, slot + 3 * SLOT, s, lane, mul2(gs, fma2(z, sub2(both(1.f), sz[Z ? s : 0]), both(1.f))));
+            }
+            keep_pair<F, MODE>(slot, slot + SLOT, s, lane, d);
+            El = mul2(a[s], add2(d, El));
+        }
         const int side = k & 1;
         ex.seg[side][warp][lane] = make_float4(P.x, P.y, hl.x, hl.y);
         ex.segE[side][warp][lane] = El;
@@ -586,19 +621,20 @@ __global__ void __launch_bounds__(256, 2) k_rec_bwd(const __grid_constant__ RecA
         f2 hb[S + 1];                                               // the states before the tokens
         hb[0] = h;
 #pragma unroll
-        for (int s = 0; s < S; s++) hb[s + 1] = fma2(a[s], hb[s], v[s]);
+        for (int s = 0; s < S; s++) hb[s + 1] = fma2(a[s], hb[s], mul2(mi[s], pair_at<F, MODE>(slot + 2 * SLOT, s, lane, odd_x)));
         const int m = ch < g.D ? n : 0;
         const size_t block = ((size_t)b * g.T + t0) * g.D + ch0;
 #pragma unroll
         for (int s = S - 1; s >= 0; s--) {
-            const f2 aL = mul2(a[s], mul2(r[s], rate)), Gs = add2(d[s], Es);
+            const f2 v = mul2(mi[s], pair_at<F, MODE>(slot + 2 * SLOT, s, lane, odd_x));
+            const f2 aL = mul2(a[s], mul2(r[s], rate)), Gs = add2(kept_pair<F, MODE>(slot, slot + SLOT, s, lane), Es);
             Es = mul2(a[s], Gs);
-            const f2 gx = mul2(Gs, mi[s]), gi = mul2(mul2(Gs, v[s]), sub2(both(1.f), mul2(mi[s], rs[s])));
+            const f2 gx = mul2(Gs, mi[s]), gi = mul2(mul2(Gs, v), sub2(both(1.f), mul2(mi[s], rs[s])));
             // G (h a L - i x a^2 L / m), i / m = m i / m^2
-            const f2 gLL = mul2(Gs, sub2(mul2(hb[s], aL), mul2(mul2(mul2(v[s], rs[s]), rs[s]), mul2(a[s], aL))));
+            const f2 gLL = mul2(Gs, sub2(mul2(hb[s], aL), mul2(mul2(mul2(v, rs[s]), rs[s]), mul2(a[s], aL))));
             total = add2(total, gLL);
             const f2 gr = mul2(gLL, fma2(r[s], both(-LN2), both(LN2)));
-            const f2 gz = Z ? mul2(e[Z ? s : 0], hb[s + 1]) : both(0.f);
+            const f2 gz = Z ? mul2(kept_pair<F, MODE>(slot + 4 * SLOT, slot + 3 * SLOT, s, lane), hb[s + 1]) : both(0.f);
             if constexpr (MODE == TILES) {
                 put_pair(slot, s, lane, gr);
                 put_pair(slot + SLOT, s, lane, gi);
@@ -826,7 +862,7 @@ template <typename F> bool lies_in(const wkv_gated_recurrence_args_t *a, size_t 
 }
 
 int block_tokens(const wkv_gated_recurrence_args_t *a, bool back) {
-    if (back) return CKPT;
+    if (back) return a->dtype == WKV_F32 ? Geo<float, true>::BT : Geo<__half, true>::BT;
     return a->dtype == WKV_F32 ? Geo<float, false>::BT : Geo<__half, false>::BT;
 }
 
@@ -867,11 +903,15 @@ bool sizes_ok(const wkv_gated_recurrence_args_t *a) {
            (long long)a->B * ((a->D + CH - 1) / CH) <= 2147483647 / MAX_SPANS && (long long)a->B * a->D <= 1ll << 34 && a->c > 0.f &&
            strides_ok(a);
 }
+long long kept_states(const wkv_gated_recurrence_args_t *a) {
+    const int t = ckpt_tokens(elem_size(a->dtype));
+    return ((long long)a->T + t - 1) / t;
+}
 RecArgs args_of(const wkv_gated_recurrence_args_t *a, bool back) {
     RecArgs g = {};
     const Spans sp = spans_for(a, back);
     g.T = a->T; g.D = a->D; g.slabs = (a->D + CH - 1) / CH; g.nspan = sp.n; g.span = sp.tokens;
-    g.nkept = (int)(((long long)a->T + CKPT - 1) / CKPT);
+    g.nkept = (int)kept_states(a);
     g.c = a->c;
     g.x = a->x; g.ig = a->input_gate; g.rg = a->decay_gate; g.z = a->z;
     g.x_batch = a->x_batch; g.x_token = a->x_token; g.ig_batch = a->i_batch; g.ig_token = a->i_token;
@@ -884,7 +924,7 @@ RecArgs args_of(const wkv_gated_recurrence_args_t *a, bool back) {
     g.status = a->status; g.limit = t_limit; g.skip = t_skip;
     return g;
 }
-size_t ckpt_need(const wkv_gated_recurrence_args_t *a) { return (size_t)a->B * (((size_t)a->T + CKPT - 1) / CKPT) * a->D * 4; }
+size_t ckpt_need(const wkv_gated_recurrence_args_t *a) { return (size_t)a->B * kept_states(a) * a->D * 4; }
 
 template <class K>
 int launch_rec(K kern, const RecArgs &g, long long ctas, int smem, unsigned char (&done)[64], cudaStream_t s) {

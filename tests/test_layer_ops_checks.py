@@ -150,7 +150,7 @@ def test_error_codes_of_the_recurrence(memory):
     for f in ("decay", "x", "input_gate", "decay_gate", "y", "state_out"):
         setattr(a, f, at)
     assert bwd(ref(a), None) == 5                               # the states that the forward pass leaves
-    assert lib.wkv_gated_recurrence_ckpt_bytes(ref(a)) == 10 * 8 * 4
+    assert lib.wkv_gated_recurrence_ckpt_bytes(ref(a)) == 5 * 8 * 4        # the state before every 64 tokens
     a.ckpt, a.ckpt_bytes = at, 16
     assert fwd(ref(a), None) == 5 and bwd(ref(a), None) == 5
     a.ckpt_bytes, a.gdecay = 4096, at
