@@ -338,11 +338,13 @@ struct Cut {
     int cg, bn, m_tiles0, m_tiles, n_tiles, main, rest, splits, kb_split;
     size_t part_bytes() const { return splits > 1 ? (size_t)rest * splits * (128 * cg) * bn * 4 : 0; }
 };
-// The cut that takes least by this estimate (us on one B200, 64 contraction steps a block).  A block's operands come into an SM at about 60
-// bytes a cycle, which is what a tile costs: 32 KB a CTA for 256 x 256 of two (0.27; its products take as long) and for 128 x 128 of one, 24 KB
-// for 256 x 128 of two (0.20) and 128 x 64 of one.  Cut contractions cost their sums' way through L2, and a launch.
+// The cut that takes least by this estimate, in us, fitted to one B200 (`first`: a launch with its first and its last tile's latency; `block`: 64
+// contraction steps of a tile on every SM).  256 x 256 of two CTAs runs at the tensor cores' rate (8.4 million multiply-adds in 0.365 us); the other tiles are bound by
+// their operands' way into an SM, about 60 bytes a cycle: 24 KB a block for 256 x 128 of two and 128 x 64 of one, 32 KB for 128 x 128 of one.  Cut
+// contractions cost a launch and their sums' way through L2.  (2048 x 2560 -> 2560, 80 tiles on 74 pairs: 28 us with the last 6 cut in four, 31 without;
+// 1500 x 8192 -> 1000, 24 tiles: 25 cut in three, 44 without.)
 Cut cut_for(long long m, long long n, int sources, int kb, bool pair) {
-    struct { int cg, bn; double block; } tiles[4] = {{2, 256, 0.27}, {2, 128, 0.20}, {1, 128, 0.27}, {1, 64, 0.20}};
+    struct { int cg, bn; double first, block; } tiles[4] = {{2, 256, 6.2, 0.365}, {2, 128, 5.7, 0.222}, {1, 128, 4.7, 0.272}, {1, 64, 4.5, 0.228}};
     const int sms = device_sm_count();
     Cut best = {};
     double t_best = 1e30;
@@ -355,8 +357,8 @@ Cut cut_for(long long m, long long n, int sources, int kb, bool pair) {
             if (s > 1 && (rest == 0 || rest * (s - 1) >= places)) break;
             const int len = (kb + s - 1) / s, used = (kb + len - 1) / len;
             if (used != s) continue;
-            double us = 4.0 + t.block * 0.4 * t.bn * t.cg / 64 + waves * kb * t.block + (rest ? (double)((rest * s + places - 1) / places) * len * t.block : 0.0);
-            if (s > 1) us += 2.5 + (double)rest * s * bm * t.bn * 8 / 4e6;
+            double us = t.first + waves * kb * t.block + (rest ? (double)((rest * s + places - 1) / places) * len * t.block : 0.0);
+            if (s > 1) us += 2.0 + 0.4 * s + (double)rest * s * bm * t.bn * 8 / 3e7;
             if (us < t_best) {
                 t_best = us;
                 best = {t.cg, t.bn, (int)m0, (int)(sources * m0), (int)nt, (int)(all - rest), (int)rest, s, len};
@@ -565,7 +567,7 @@ int backward(const wkv_linear_args_t *a, Scratch ws, size_t *need, cudaStream_t 
             e.vec = a->K % 8 == 0 && aligned16(a->gx);
             e.y[0] = a->gx; e.y_row = a->K;
             Scratch parts = ws;
-            rc = product<F, false, true, EPI_LINEAR>(gz, w, sources, sources, a->rows, a->K, a->N, cut, e, parts.take(cut.part_bytes()), a->status, s);
+            rc = product<F, false, true, EPI_PLAIN>(gz, w, sources, sources, a->rows, a->K, a->N, cut, e, parts.take(cut.part_bytes()), a->status, s);
         }
     }
     if (rc == WKV_OK && (a->gw0 != nullptr || a->gw1 != nullptr)) {
@@ -583,7 +585,7 @@ int backward(const wkv_linear_args_t *a, Scratch ws, size_t *need, cudaStream_t 
             e.y_row = a->K;
             if (a->gw0 == nullptr) gz[0] = gz[1];
             Scratch parts = ws;
-            rc = product<F, true, true, EPI_LINEAR>(gz, xs, 1 + both, 1, a->N, a->K, a->rows, cut, e, parts.take(cut.part_bytes()), a->status, s);
+            rc = product<F, true, true, EPI_PLAIN>(gz, xs, 1 + both, 1, a->N, a->K, a->rows, cut, e, parts.take(cut.part_bytes()), a->status, s);
         }
     }
     if (count) *need = ws.used + most;

@@ -31,7 +31,7 @@ namespace linear {
 enum { ACT_NONE = 0, ACT_SILU = 1, ACT_GELU = 2, ACT_RELU2 = 3, ACT_SIGMOID = 4, ACT_COUNT = 5 };
 
 constexpr int EPI_WARPS = 8, THREADS = 32 * (EPI_WARPS + 2), KB = 64, ACC = 2;
-enum { EPI_LINEAR = 0, EPI_GATED = 1 };
+enum { EPI_LINEAR = 0, EPI_GATED = 1, EPI_PLAIN = 2 };         // (PLAIN: the sums alone, of the gradients)
 constexpr int STATUS_LINEAR = 64;          // the status word's bit of these kernels
 
 __device__ __forceinline__ float sigmoid_of(float x) { return __fdividef(1.f, 1.f + __expf(-x)); }
@@ -130,8 +130,10 @@ __device__ __forceinline__ uint32_t map_rank(const void *p, uint32_t rank) {
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(sm100::smem_u32(p)), "r"(rank));
     return r;
 }
+// (what it orders are reads of tensor memory, which tcgen05's fence has ordered: with .release.cluster it waited for the outputs' stores, 0.15 of the
+// epilogue's time)
 __device__ __forceinline__ void arrive_remote(uint32_t bar) {
-    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+    asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 __device__ __forceinline__ void cluster_sync() {
     asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
@@ -295,7 +297,7 @@ struct Finish {
 #pragma unroll
                 for (int i = 0; i < W; i++) f[k][i] += bias[i];
         }
-        if (e.z[0] != nullptr) {
+        if (EPI != EPI_PLAIN && e.z[0] != nullptr) {
 #pragma unroll
             for (int k = 0; k < R; k++) {
                 const long long at = (row + k * rows) * e.z_row + col;
@@ -303,7 +305,7 @@ struct Finish {
                 if (EPI == EPI_GATED) keep(e.z[1] + at, u[k], ok[k], n);
             }
         }
-        act_values(e.act, f);
+        if (EPI != EPI_PLAIN) act_values(e.act, f);
         if (EPI == EPI_GATED) {
 #pragma unroll
             for (int k = 0; k < R; k++)
@@ -348,8 +350,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_gemm(const __grid_constant__ Gem
     const uint32_t rank = CG == 2 ? cluster_rank() : 0;
     const int first = blockIdx.x / CG, step = gridDim.x / CG, items = g.main + g.rest * g.splits;
 
-    pdl_wait();
-    pdl_trigger();
+    // (before pdl_wait: shared memory alone, and the tensor maps, which are arguments)
     if (threadIdx.x == 0) {
         for (int i = 0; i < ST; i++) {
             sm100::mbar_init(full + i, 1);
@@ -361,14 +362,12 @@ __global__ void __launch_bounds__(THREADS, 1) k_gemm(const __grid_constant__ Gem
         }
         *abort = 0;
         sm100::fence_mbar_init();
+        sm100::prefetch_tmap(g.a);
+        sm100::prefetch_tmap(g.b);
     }
-    if (warp == EPI_WARPS) {
-        if (lane == 0) {
-            sm100::prefetch_tmap(g.a);
-            sm100::prefetch_tmap(g.b);
-        }
-        __syncwarp();
-    }
+    __syncwarp();
+    pdl_wait();
+    pdl_trigger();
     if (warp == EPI_WARPS + 1) tmem_get<CG>(tmem, T::COLS);
     sm100::tc_fence_before();
     __syncthreads();

@@ -254,11 +254,11 @@ def test_two_streams_at_once():
 
 
 def test_more_than_two_to_the_31_elements():
-    """rows behind 2^31 elements of x and of y are the rows of a call of their own"""
+    """rows behind 2^31 elements of x and of y (a call of fewer rows may add up its sums in another order: against 64 bits)"""
     import rwkv_infctx_trainer_b200 as W
     rows, K, N = 265000, 8192, 8200
     w = torch.randn((N, K), device="cuda", dtype=BF) * K ** -0.5
     x = torch.randn((rows, K), device="cuda", dtype=BF)
     y = W.linear_act(x, w)
     for at in (0, 262143, rows - 300):
-        assert torch.equal(y[at:at + 256], W.linear_act(x[at:at + 256], w)), at
+        L.close(f"y {at}", y[at:at + 256], *L.linear_ref(x[at:at + 256], w, None, "none", None, None)["y"])
