@@ -108,17 +108,6 @@ __device__ __forceinline__ Rate rate_of(float p, float c) {
     return r;
 }
 
-// 1 - a^2 of two channels; x2 = -2 L
-__device__ __forceinline__ f2 one_minus_square(f2 a, f2 x2) {
-    f2 p = fma2(x2, both(-1.f / 720.f), both(1.f / 120.f));
-    p = fma2(x2, p, both(-1.f / 24.f));
-    p = fma2(x2, p, both(1.f / 6.f));
-    p = fma2(x2, p, both(-0.5f));
-    p = mul2(fma2(x2, p, both(1.f)), x2);
-    const f2 d = fma2(neg2(a), a, both(1.f));
-    return make_float2(x2.x < 0.25f ? p.x : d.x, x2.y < 0.25f ? p.y : d.y);
-}
-
 // Sigmoids of two channels' gates (Z: and of the output gate): one reciprocal for a channel's two or three, of the product of their
 // 1 + e^-x, because special functions are what bounds the forward pass.  `range` adds up the products: while it is below 2^125 none
 // of them has left the range; else (gates below -28 or so, infinities, NaNs, which would spread from one gate to the others) the
@@ -162,9 +151,29 @@ __device__ __forceinline__ void sigmoids(f2 rg, f2 ig, f2 z, f2 &r, f2 &i, f2 &s
     }
 }
 __device__ __forceinline__ bool in_range(f2 range) { return __all_sync(0xffffffffu, range.x + range.y < RANGE); }
-__device__ __forceinline__ f2 decays(f2 r, f2 rate) {
-    const f2 e = fma2(r, rate, both(EX2_MEAN));
-    return make_float2(ex2(e.x), ex2(e.y));
+// Decays a of two channels and q = 1 - a^2; x = -2 L.  EXACT (fp32 tensors): below x = 1/4 the decay is its power series, too (y^7 / 5040 is left
+// out, 1e-10): rounded once, where ex2 is off by up to three roundings, which over the memory of a state add up.
+template <bool EXACT>
+__device__ __forceinline__ void decays(f2 r, f2 rate, f2 x2, f2 &a, f2 &q) {
+    const f2 e = fma2(r, rate, both(EX2_MEAN)), x = mul2(r, x2);
+    a = make_float2(ex2(e.x), ex2(e.y));
+    if (EXACT) {
+        const f2 y = mul2(x, both(0.5f));
+        f2 t = fma2(y, both(1.f / 720.f), both(-1.f / 120.f));
+        t = fma2(y, t, both(1.f / 24.f));
+        t = fma2(y, t, both(-1.f / 6.f));
+        t = fma2(y, t, both(0.5f));
+        t = fma2(y, t, both(-1.f));
+        t = fma2(y, t, both(1.f));
+        a = make_float2(x.x < 0.25f ? t.x : a.x, x.y < 0.25f ? t.y : a.y);
+    }
+    f2 p = fma2(x, both(-1.f / 720.f), both(1.f / 120.f));
+    p = fma2(x, p, both(-1.f / 24.f));
+    p = fma2(x, p, both(1.f / 6.f));
+    p = fma2(x, p, both(-0.5f));
+    p = mul2(fma2(x, p, both(1.f)), x);
+    const f2 d = fma2(neg2(a), a, both(1.f));
+    q = make_float2(x.x < 0.25f ? p.x : d.x, x.y < 0.25f ? p.y : d.y);
 }
 
 __device__ __forceinline__ void cp_async4(void *smem, const void *g, int valid) {
@@ -409,8 +418,8 @@ __global__ void __launch_bounds__(256, 2) k_rec_fwd(const __grid_constant__ RecA
                 const f2 x = pair_at<F, MODE>(slot + 2 * SLOT, s, lane, odd_x), z = Z ? pair_at<F, MODE>(slot + 3 * SLOT, s, lane, odd_z) : both(0.f);
                 f2 r, in, sz;
                 sigmoids<Z, decltype(fast)::value>(pair_at<F, MODE>(slot, s, lane, odd_r), pair_at<F, MODE>(slot + SLOT, s, lane, odd_i), z, r, in, sz, range);
-                a[s] = decays(r, rate);
-                const f2 q = one_minus_square(a[s], mul2(r, x2));
+                f2 q;
+                decays<sizeof(F) == 4>(r, rate, x2, a[s], q);
                 v[s] = mul2(mul2(make_float2(sqrtf(q.x), sqrtf(q.y)), in), x);
                 if (Z) gate[s] = mul2(z, sz);
                 hl = fma2(a[s], hl, v[s]);
@@ -562,8 +571,8 @@ __global__ void __launch_bounds__(256, 2) k_rec_bwd(const __grid_constant__ RecA
                 const f2 z = Z ? pair_at<F, MODE>(slot + 4 * SLOT, s, lane, odd_z) : both(0.f);
                 f2 in;
                 sigmoids<Z, decltype(fast)::value>(pair_at<F, MODE>(slot, s, lane, odd_r), pair_at<F, MODE>(slot + SLOT, s, lane, odd_i), z, r[s], in, sz[Z ? s : 0], range);
-                a[s] = decays(r[s], rate);
-                const f2 q = one_minus_square(a[s], mul2(r[s], x2));
+                f2 q;
+                decays<sizeof(F) == 4>(r[s], rate, x2, a[s], q);
                 // (where 1 - a^2 is zero, so are L and m: any factor does; a NaN stays)
                 f2 low = q;
                 asm("max.NaN.f32 %0, %0, %1;" : "+f"(low.x) : "f"(1e-37f));
@@ -768,13 +777,14 @@ __global__ void __launch_bounds__(256, 2) k_rec_spans(const __grid_constant__ Re
                 f2 r, in, sz;
                 if (!BACK) {
                     sigmoids<false, decltype(fast)::value>(pair_at<F, MODE>(slot, s, lane, odd_r), pair_at<F, MODE>(slot + SLOT, s, lane, odd_i), both(0.f), r, in, sz, range);
-                    a[s] = decays(r, rate);
-                    const f2 q = one_minus_square(a[s], mul2(r, x2));
+                    f2 q;
+                    decays<sizeof(F) == 4>(r, rate, x2, a[s], q);
                     v[s] = mul2(mul2(make_float2(sqrtf(q.x), sqrtf(q.y)), in), pair_at<F, MODE>(slot + 2 * SLOT, s, lane, odd_x));
                 } else {
                     const f2 z = Z ? pair_at<F, MODE>(slot + 2 * SLOT, s, lane, odd_z) : both(0.f);
                     sigmoids<false, decltype(fast)::value>(pair_at<F, MODE>(slot, s, lane, odd_r), z, both(0.f), r, sz, in, range);
-                    a[s] = decays(r, rate);
+                    f2 q;
+                    decays<sizeof(F) == 4>(r, rate, x2, a[s], q);
                     v[s] = pair_at<F, MODE>(slot + SLOT, s, lane, odd_g);
                     if (Z) v[s] = mul2(v[s], mul2(z, sz));
                 }
@@ -832,8 +842,9 @@ __global__ void __launch_bounds__(128) k_rec_step(const RecArgs g, long long pai
     if (g.state_in != nullptr) h = make_float2(g.state_in[at], n > 1 ? g.state_in[at + 1] : 0.f);
     auto one = [&](float h, float x, float ig, float rg, float p) {
         const Rate k = rate_of(p, g.c);
-        const float r = sigm(rg), a = ex2(fmaf(r, k.rate2, EX2_MEAN)), m = sqrtf(one_minus_square(both(a), both(r * k.x2)).x);
-        return fmaf(a, h, m * sigm(ig) * x);
+        f2 a, q;
+        decays<sizeof(F) == 4>(both(sigm(rg)), both(k.rate2), both(k.x2), a, q);
+        return fmaf(a.x, h, sqrtf(q.x) * sigm(ig) * x);
     };
     h = make_float2(one(h.x, x.x, ig.x, rg.x, g.decay[ch]), n > 1 ? one(h.y, x.y, ig.y, rg.y, g.decay[ch + 1]) : 0.f);
     g.state_out[at] = h.x;
