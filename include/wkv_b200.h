@@ -367,7 +367,7 @@ int wkv_selective_scan_backward(const wkv_selective_scan_args_t *a, void *stream
  *     a_t = exp(-c softplus(decay) r_t),  h_t = a_t h_{t-1} + sqrt(1 - a_t^2) i_t x_t,  y_t = h_t silu(z_t)
  *   x, input_gate, decay_gate, z (or NULL: y = h) [B,T,D] in `dtype`, each with its own batch and
  *   token stride (elements); decay [D], the states [B,D]: fp32; c > 0.  state_out may be
- *   state_in's memory.  A decay gate of minus infinity keeps the state and takes no input.
+ *   state_in's memory when T is 0 or 1.  A decay gate of minus infinity keeps the state and takes no input.
  *   ckpt (wkv_gated_recurrence_ckpt_bytes()): states that the forward call leaves for the backward
  *   call, which needs them.  gy [B,T,D] contiguous.  Gradients: gx, ginput_gate, gdecay_gate, gz
  *   [B,T,D] in dtype; gdecay, gstate_in fp32.  D is at most 2^22, a token stride 2^26, T 2^31 - 4097.
@@ -412,7 +412,8 @@ int wkv_gated_recurrence_backward(const wkv_gated_recurrence_args_t *a, void *st
  *   [N] in bias_dtype; that of the residual is gy.  The gradient of the pre-activation is rounded
  *   to dtype once, for the products; gbias is summed before that rounding.
  *   status: device-visible word or NULL; WKV_LINEAR_TIMEOUT is set in it when a bounded wait ran out
- *   and the results are invalid.  rows, K and N below 2^31 - 256. */
+ *   and the results are invalid.  rows, K and N are at most 2^31 - 4096, rows do not
+ *   overlap. */
 enum { WKV_ACT_NONE = 0, WKV_ACT_SILU = 1, WKV_ACT_GELU = 2, WKV_ACT_RELU2 = 3, WKV_ACT_SIGMOID = 4 };
 enum { WKV_LINEAR_TIMEOUT = 64 };
 typedef struct wkv_linear_args {

@@ -1023,6 +1023,7 @@ extern "C" int wkv_gated_recurrence_forward(const wkv_gated_recurrence_args_t *a
                                   lies_in<F>(a, 2 * sizeof(F), false) && a->D % 2 == 0);
         });
     }
+    if (a->T > 1 && a->state_out == a->state_in) return WKV_ERR_UNSUPPORTED;        // (spans of a row start from it at any time)
     if (a->ckpt != nullptr && a->ckpt_bytes < ckpt_need(a)) return WKV_ERR_WORKSPACE;
     const size_t need = wkv_gated_recurrence_forward_workspace(a);
     if (need > 0 && (a->workspace == nullptr || a->workspace_bytes < need)) return WKV_ERR_WORKSPACE;

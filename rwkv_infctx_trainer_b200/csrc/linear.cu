@@ -413,12 +413,10 @@ int product(const Matrix (&a)[2], const Matrix (&b)[2], int a_sources, int b_sou
     g.e = e;
     g.e.part = (float *)part;
     const int b_box = PAIR ? cut.bn / 2 : cut.bn / cut.cg;
-    for (int i = 0; i < 2; i++) {
-        const Matrix &ma = a[a_sources == 2 ? i : 0], &mb = b[b_sources == 2 ? i : 0];
-        if (!make_matrix_map(&g.a[i], ma.p, ma.rows, ma.cols, ma.pitch, A_MN ? 64 : 128) ||
-            !make_matrix_map(&g.b[i], mb.p, mb.rows, mb.cols, mb.pitch, B_MN ? 64 : b_box))
-            return WKV_ERR_LAUNCH;
-    }
+    for (int i = 0; i < a_sources; i++)
+        if (!make_matrix_map(&g.a[i], a[i].p, a[i].rows, a[i].cols, a[i].pitch, A_MN ? 64 : 128)) return WKV_ERR_LAUNCH;
+    for (int i = 0; i < b_sources; i++)
+        if (!make_matrix_map(&g.b[i], b[i].p, b[i].rows, b[i].cols, b[i].pitch, B_MN ? 64 : b_box)) return WKV_ERR_LAUNCH;
     if (cut.cg == 2) return cut.bn == 256 ? launch_gemm<F, 2, 256, A_MN, B_MN, EPI>(g, s) : launch_gemm<F, 2, 128, A_MN, B_MN, EPI>(g, s);
     return cut.bn == 128 ? launch_gemm<F, 1, 128, A_MN, B_MN, EPI>(g, s) : launch_gemm<F, 1, 64, A_MN, B_MN, EPI>(g, s);
 }
@@ -427,8 +425,11 @@ int check_args(const wkv_linear_args_t *a) {
     if (a == nullptr) return WKV_ERR_NULL;
     if (a->dtype != WKV_BF16 && a->dtype != WKV_F16) return known_dtype(a->dtype) ? WKV_ERR_UNSUPPORTED : WKV_ERR_DTYPE;
     if (a->bias != nullptr && !known_dtype(a->bias_dtype)) return WKV_ERR_DTYPE;
-    const long long most = (1ll << 31) - 256;
+    const long long most = (1ll << 31) - 4096;         // (numbers of rows and columns, and what loops add to them, are 32-bit)
     if (a->rows < 0 || a->K < 1 || a->N < 1 || a->rows > most || a->K > most || a->N > most) return WKV_ERR_SHAPE;
+    if ((a->x != nullptr && a->rows > 1 && a->x_row < a->K) || (a->w0 != nullptr && a->N > 1 && a->w0_row < a->K) ||
+        (a->pair && a->w1 != nullptr && a->N > 1 && a->w1_row < a->K))
+        return WKV_ERR_SHAPE;
     if (a->act < 0 || a->act >= ACT_COUNT || a->pair < 0 || a->pair > 1) return WKV_ERR_SHAPE;
     if (a->pair && (a->bias != nullptr || a->mul != nullptr || a->residual != nullptr || a->gbias != nullptr || a->gmul != nullptr)) return WKV_ERR_UNSUPPORTED;
     return WKV_OK;

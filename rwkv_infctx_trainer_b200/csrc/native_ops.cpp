@@ -30,7 +30,12 @@ int *status_word(int device) {
         p = g_status[device].load(std::memory_order_acquire);
         if (p == nullptr) {
             // a cache line per device, kept for the life of the process
-            C10_CUDA_CHECK(cudaHostAlloc((void **)&p, 128, cudaHostAllocPortable | cudaHostAllocMapped));
+            // (a first call inside a capture: the allocation is not part of it)
+            cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+            C10_CUDA_CHECK(cudaThreadExchangeStreamCaptureMode(&mode));
+            const cudaError_t e = cudaHostAlloc((void **)&p, 128, cudaHostAllocPortable | cudaHostAllocMapped);
+            C10_CUDA_CHECK(cudaThreadExchangeStreamCaptureMode(&mode));
+            C10_CUDA_CHECK(e);
             *p = 0;
             g_status[device].store(p, std::memory_order_release);
         }

@@ -66,22 +66,8 @@ inline bool make_btc_map(CUtensorMap *map, const void *base, int B, int T, int C
 }
 
 // Map over a matrix [rows, cols] of 16-bit elements, rows `pitch` elements apart; box = box_rows x 64 columns, 128-byte swizzle,
-// what lies outside reads as zero.  base: 16-byte aligned, pitch a multiple of 8.  Remembered as above.
+// what lies outside reads as zero.  base: 16-byte aligned, pitch a multiple of 8.
 inline bool make_matrix_map(CUtensorMap *map, const void *base, long long rows, long long cols, long long pitch, int box_rows) {
-    struct Entry {
-        CUtensorMap map;
-        const void *base;
-        long long rows, cols, pitch;
-        int box_rows;
-    };
-    constexpr int LOG_SLOTS = 9;
-    static thread_local Entry cache[1 << LOG_SLOTS];
-    const uint64_t key = (uint64_t)(uintptr_t)base ^ (uint64_t)rows << 40 ^ (uint64_t)cols << 50 ^ (uint64_t)box_rows << 32;
-    Entry &e = cache[(key >> 8) * 0x9E3779B97F4A7C15ull >> (64 - LOG_SLOTS)];
-    if (e.base == base && e.rows == rows && e.cols == cols && e.pitch == pitch && e.box_rows == box_rows && base != nullptr) {
-        *map = e.map;
-        return true;
-    }
     encode_tiled_fn enc = tensor_map_encoder();
     if (!enc) return false;
     cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
@@ -91,36 +77,19 @@ inline bool make_matrix_map(CUtensorMap *map, const void *base, long long rows, 
     const auto encode = [&] {
         // (the elements' type matters for arithmetic in the copy only: there is none)
         return enc(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void *>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                   CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+                   CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
     };
-    if (encode() != CUDA_SUCCESS) {
-        int dev = 0;
-        if (cudaGetDevice(&dev) != cudaSuccess || cudaSetDevice(dev) != cudaSuccess || encode() != CUDA_SUCCESS) return false;
-    }
-    e.base = base; e.rows = rows; e.cols = cols; e.pitch = pitch; e.box_rows = box_rows; e.map = *map;
-    return true;
+    // (a thread that has not been in the runtime yet: see make_btc_map)
+    int dev = 0;
+    return encode() || (cudaGetDevice(&dev) == cudaSuccess && cudaSetDevice(dev) == cudaSuccess && encode());
 }
 
 // Map over activations [B, T, D] of 2- or 4-byte elements, channels adjacent, rows `batch` and `token` elements apart; box = channels x
 // tokens x 1, unswizzled, what lies outside reads as zero and is not written.  False where TMA cannot take them (addresses and strides that
-// are no multiples of 16 bytes, strides it has no room for).  Remembered as above.
+// are no multiples of 16 bytes, strides it has no room for).
 inline bool make_tile_map(CUtensorMap *map, const void *base, int elem, int B, int T, int D, long long batch, long long token, int channels, int tokens) {
-    struct Entry {
-        CUtensorMap map;
-        const void *base;
-        int elem, B, T, D, channels, tokens;
-        long long batch, token;
-    };
-    constexpr int LOG_SLOTS = 9;
-    static thread_local Entry cache[1 << LOG_SLOTS];
     if (base == nullptr || (uintptr_t)base % 16 || batch * elem % 16 || token * elem % 16 || batch < 0 || token < 0 || batch >= 1ll << 37 || token >= 1ll << 37)
         return false;
-    const uint64_t key = (uint64_t)(uintptr_t)base ^ (uint64_t)T << 40 ^ (uint64_t)D << 52 ^ (uint64_t)B << 48 ^ (uint64_t)tokens << 34;
-    Entry &e = cache[(key >> 8) * 0x9E3779B97F4A7C15ull >> (64 - LOG_SLOTS)];
-    if (e.base == base && e.elem == elem && e.B == B && e.T == T && e.D == D && e.channels == channels && e.tokens == tokens && e.batch == batch && e.token == token) {
-        *map = e.map;
-        return true;
-    }
     encode_tiled_fn enc = tensor_map_encoder();
     if (!enc) return false;
     cuuint64_t dims[3] = {(cuuint64_t)D, (cuuint64_t)T, (cuuint64_t)B};
@@ -129,14 +98,10 @@ inline bool make_tile_map(CUtensorMap *map, const void *base, int elem, int B, i
     cuuint32_t estr[3] = {1, 1, 1};
     const auto encode = [&] {
         return enc(map, elem == 2 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 3, const_cast<void *>(base), dims, strides, box, estr,
-                   CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+                   CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
     };
-    if (encode() != CUDA_SUCCESS) {
-        int dev = 0;
-        if (cudaGetDevice(&dev) != cudaSuccess || cudaSetDevice(dev) != cudaSuccess || encode() != CUDA_SUCCESS) return false;
-    }
-    e.base = base; e.elem = elem; e.B = B; e.T = T; e.D = D; e.channels = channels; e.tokens = tokens; e.batch = batch; e.token = token; e.map = *map;
-    return true;
+    int dev = 0;
+    return encode() || (cudaGetDevice(&dev) == cudaSuccess && cudaSetDevice(dev) == cudaSuccess && encode());
 }
 
 }  // namespace wkv

@@ -150,6 +150,9 @@ def test_error_codes_of_the_recurrence(memory):
     for f in ("decay", "x", "input_gate", "decay_gate", "y", "state_out"):
         setattr(a, f, at)
     assert bwd(ref(a), None) == 5                               # the states that the forward pass leaves
+    a.state_in = at
+    assert fwd(ref(a), None) == 7                               # state in place over more than one token
+    a.state_in = None
     assert lib.wkv_gated_recurrence_ckpt_bytes(ref(a)) == 5 * 8 * 4        # the state before every 64 tokens
     a.ckpt, a.ckpt_bytes = at, 16
     assert fwd(ref(a), None) == 5 and bwd(ref(a), None) == 5
@@ -183,7 +186,7 @@ def test_error_codes_of_the_products(memory):
     a.dtype = 1
     assert fwd(ref(a), None) == 1 and bwd(ref(a), None) == 1
     a.x, a.w0, a.y, a.gy = at, at, at, at
-    for field, value in (("rows", -1), ("K", 0), ("N", 0), ("rows", 2 ** 31), ("K", 2 ** 31 - 255), ("N", 2 ** 31), ("act", 5), ("act", -1), ("pair", 2)):
+    for field, value in (("rows", -1), ("K", 0), ("N", 0), ("rows", 2 ** 31), ("K", 2 ** 31 - 4095), ("N", 2 ** 31), ("x_row", 23), ("w0_row", -24), ("act", 5), ("act", -1), ("pair", 2)):
         old = getattr(a, field)
         setattr(a, field, value)
         assert fwd(ref(a), None) == 2 and bwd(ref(a), None) == 2, field

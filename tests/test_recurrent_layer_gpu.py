@@ -180,6 +180,31 @@ def test_a_decode_step_and_a_training_step_in_a_graph():
             assert torch.equal(a, b)
 
 
+def test_the_first_call_of_a_process_inside_a_capture():
+    import os
+    import subprocess
+    import sys
+    code = """
+import torch, rwkv_infctx_trainer_b200 as W
+n = lambda *s: torch.randn(s, device="cuda", dtype=torch.bfloat16)
+x, w, z = n(40, 64), n(72, 64), n(1, 40, 64)
+decay = torch.zeros(64, device="cuda")
+torch.cuda.synchronize()
+g = torch.cuda.CUDAGraph()
+with torch.no_grad(), torch.cuda.graph(g):
+    y = W.linear_act(x, w, activation="gelu")
+    r, s = W.gated_recurrence(z, z, z, decay)
+g.replay()
+torch.cuda.synchronize()
+with torch.no_grad():
+    assert torch.equal(y, W.linear_act(x, w, activation="gelu")) and torch.equal(r, W.gated_recurrence(z, z, z, decay)[0])
+print("same")
+"""
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    out = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True, timeout=300)
+    assert out.returncode == 0 and "same" in out.stdout, out.stderr[-2000:]
+
+
 def test_threads():
     p = params(BF)
     rows = [inputs(2, 33, BF, seed) for seed in range(4)]
