@@ -7,7 +7,7 @@
 //
 // The products run on the tile kernel of linear_gemm.cuh.  The pair's forward pass is one product whose tile of 256 columns is half
 // of each matrix (a CTA of the pair brings the rows of one), so that g and u of an element end up in one thread; its gradient of x
-// is one product over both contractions, and that of the matrices one over the rows of both.  Few rows (a decoded token) are bound
+// is one product over both contractions, and that of the matrices one over the rows of both.  Few rows (decoded tokens) are bound
 // by reading the matrix: k_few_rows streams it through registers once.
 //
 // What the forward pass keeps: the pre-activations, in fp32.  (In the activations' type the gradients of the matrices were 0.0031 off
@@ -67,7 +67,6 @@ __device__ __forceinline__ void mma16(float (&d)[4], uint32_t a0, uint32_t a1, u
                      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-constexpr int FEW_ROWS = 16;
 
 struct FewArgs {
     int M, K, N;                       // M: rows of x
@@ -81,7 +80,7 @@ template <typename F, int TOKENS, bool PAIR, bool VEC, int FEW_WARPS>
 __global__ void __launch_bounds__(32 * FEW_WARPS) k_few_rows(const FewArgs g) {
     pdl_wait();
     pdl_trigger();
-    constexpr int NT = TOKENS / 8, OUT = PAIR ? 8 : 16, UNROLL = 4;
+    constexpr int NT = TOKENS / 8, OUT = PAIR ? 8 : 16, UNROLL = TOKENS == 32 ? 2 : 4;
     __shared__ float part[FEW_WARPS][16][TOKENS + 1];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, q = lane >> 2, c = lane & 3;
     const int row0 = blockIdx.x * OUT;
@@ -450,7 +449,9 @@ int check_args(const wkv_linear_args_t *a) {
 }
 bool keeps(const wkv_linear_args_t *a) { return a->pair || a->act != ACT_NONE || a->mul != nullptr; }
 size_t saved_one(const wkv_linear_args_t *a) { return align256((size_t)a->rows * up8(a->N) * 4); }
-bool few(const wkv_linear_args_t *a) { return a->rows <= FEW_ROWS; }
+// Up to 16 rows, and up to 32 of matrices of up to 2^24 elements, where starting and ending the tile kernel counts (us, streamed and in tiles: 32 rows of
+// 2560 -> 2560 8.1 and 12, of 4096 -> 4096 12 and 13.5, of 4096 -> 14336 39 and 27: the rows of x come from L1 for every 16 of the matrix).
+bool few(const wkv_linear_args_t *a) { return a->rows <= 16 || (a->rows <= 32 && (1 + a->pair) * a->N <= (1 << 24) / a->K); }
 Matrix x_of(const wkv_linear_args_t *a) { return {a->x, a->rows, a->K, a->x_row}; }
 Matrix w_of(const wkv_linear_args_t *a, int i) { return {i ? a->w1 : a->w0, a->N, a->K, i ? a->w1_row : a->w0_row}; }
 
@@ -513,7 +514,9 @@ int forward(const wkv_linear_args_t *a, Scratch ws, size_t *need, cudaStream_t s
         };
         using N8 = std::integral_constant<int, 8>;
         using N16 = std::integral_constant<int, 16>;
+        using N32 = std::integral_constant<int, 32>;
         if (a->rows <= 8) return a->pair ? go(std::true_type{}, N8{}) : go(std::false_type{}, N8{});
+        if (a->rows > 16) return a->pair ? go(std::true_type{}, N32{}) : go(std::false_type{}, N32{});
         return a->pair ? go(std::true_type{}, N16{}) : go(std::false_type{}, N16{});
     }
     const int rc = a->pair ? ready<F>({&x, &w[0], &w[1]}, ws, s) : ready<F>({&x, &w[0]}, ws, s);

@@ -16,8 +16,8 @@ x, the matrices, mul, residual and y in bf16 or fp16 (of one type within a call;
 at 10 bits).  Sums, bias, activation, product and residual are in fp32 and rounded once.  For the backward pass the
 pre-activations are kept in fp32 (where an activation or ``mul`` needs them); their gradient is rounded to x's type once, as an operand of the
 products (the bias' gradient is summed before that).  Any size and
-alignment is taken; rows whose length or stride is no multiple of 8 elements are copied first, except for up to 16 rows of x, which are
-read where they lie.
+alignment is taken; rows whose length or stride is no multiple of 8 elements are copied first, except in calls of few rows
+(up to 16, or 32 of a small matrix).
 """
 from __future__ import annotations
 
