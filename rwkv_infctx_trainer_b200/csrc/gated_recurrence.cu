@@ -768,7 +768,12 @@ __global__ void __launch_bounds__(256, 2) k_rec_spans(const __grid_constant__ Re
         }
         F *slot = ring + (k % ST) * NT * SLOT;
         const int n = (int)min((long long)S, to - at_step(k));
-        if (n < S) close_gates<F, MODE, S>(slot, n, lane);
+        if (n < S) {
+            close_gates<F, MODE, S>(slot, n, lane);
+            // (backward it is the first step, and TMA fills the stage again: ordered behind these stores by the fence, and by the warp's barrier
+            // that every refill stands behind)
+            if (MODE == TILES) sm100::fence_async_smem();
+        }
         f2 a[S], v[S];
         auto gates = [&](auto fast) {
             f2 range = both(0.f);
