@@ -283,11 +283,19 @@ __device__ __forceinline__ void put_pair(F *slot, int s, int lane, f2 v) {
     store_out<F>(slot, s * CH + 2 * lane, v, true, 2);
 }
 
+// What the thread that fills a ring keeps of it, in shared memory: blocks 0 .. asked - 1 were asked for; lost: the first one whose wait it gave up.
+// A stage whose barrier still counts bytes must not be armed again: nothing is asked for once a wait has run out, so that block k's phase stays
+// (k / ST) & 1.
+struct Filled {
+    int asked, lost;
+};
+constexpr int NEVER = 0x7fffffff;
 // what a segment does to the state (and to E): [side][segment][channel pair]
 struct Exchange {
     float4 seg[2][NW][32];                // P, hl of two channels
     uint64_t full[4];
     int abort;
+    Filled filled;
 };
 struct ExchangeBack {
     float4 seg[2][NW][32];                // P, hl
@@ -295,25 +303,33 @@ struct ExchangeBack {
     f2 sum[NW][32];
     uint64_t full[4];
     int abort;
+    Filled filled;
 };
 
 // The ring's blocks: TILES: one thread has TMA bring the block's tile of each tensor, all wait on the stage's barrier (bounded: a wait
-// that runs out is reported, the others of the CTA end at once, and the call's results are invalid).
+// that runs out is reported, the others of the CTA end at once, and the call's results are invalid; no stage is filled after it).
 template <int ST, class X>
 __device__ __forceinline__ void init_tiles(X &ex) {
     if (threadIdx.x == 0) {
         for (int i = 0; i < ST; i++) sm100::mbar_init(ex.full + i, 1);
         ex.abort = 0;
+        ex.filled = {0, NEVER};
         sm100::fence_mbar_init();
     }
     __syncthreads();
 }
-template <int ST, class X>
-__device__ __forceinline__ void await_tiles(X &ex, const RecArgs &g, int k) {
-    if (!sm100::mbar_wait_or_abort(ex.full + k % ST, (k / ST) & 1, &ex.abort, g.limit)) {
-        *(volatile int *)&ex.abort = 1;
-        if (g.status != nullptr) atomicOr(g.status, WKV_RECURRENCE_TIMEOUT);
-    }
+// bar: of block k; fills: whether this thread fills the ring
+__device__ __forceinline__ void await_tile(uint64_t *bar, int parity, int k, int *abort, Filled *f, bool fills, const RecArgs &g) {
+    if (sm100::mbar_wait_or_abort(bar, parity, abort, g.limit)) return;
+    *(volatile int *)abort = 1;
+    if (g.status != nullptr) atomicOr(g.status, WKV_RECURRENCE_TIMEOUT);
+    if (fills) f->lost = min(f->lost, k);
+}
+__device__ __forceinline__ bool given_up(const int *abort) { return *(volatile const int *)abort != 0; }
+// Before the CTA's shared memory may go: what was asked for and not waited for has landed (bounded).
+template <int ST>
+__device__ __forceinline__ void let_tiles_land(uint64_t *bars, const Filled &f, unsigned limit) {
+    for (int k = f.lost; k < f.asked; k++) sm100::mbar_wait(bars + k % ST, (k / ST) & 1, limit);
 }
 // two channels' state (or E) behind the spans from `first` up to `last`
 __device__ __forceinline__ f2 fold_spans(const RecArgs &g, int b, int first, int last, int dir, int ch, f2 h) {
@@ -330,13 +346,6 @@ __device__ __forceinline__ f2 fold_spans(const RecArgs &g, int b, int first, int
         }
     }
     return h;
-}
-
-// After a wait that ran out tiles may still be on their way into this CTA's shared memory, and the stages' phases are no longer what their number
-// says: copies take microseconds, a millisecond is waited.
-__device__ __forceinline__ void let_copies_land(const int *abort) {
-    if (*(volatile const int *)abort == 0) return;
-    for (int i = 0; i < 100; i++) __nanosleep(10000);
 }
 
 template <typename F, bool Z, int MODE>
@@ -369,8 +378,9 @@ __global__ void __launch_bounds__(256, 2) k_rec_fwd(const __grid_constant__ RecA
         const long long t0 = begin + (long long)step * BT;
         F *slot = ring + (step % ST) * NT * SLOT;
         if constexpr (MODE == TILES) {
-            if (step == g.skip) return;
             sm100::mbar_expect_tx(ex.full + step % ST, NT * SLOT * sizeof(F));
+            ex.filled.asked = step + 1;
+            if (step == g.skip) return;
 #pragma unroll
             for (int i = 0; i < NT; i++) sm100::tma_load_3d(slot + i * SLOT, g.in + i, ex.full + step % ST, ch0, (int)t0, b);
         } else {
@@ -396,7 +406,7 @@ __global__ void __launch_bounds__(256, 2) k_rec_fwd(const __grid_constant__ RecA
     }
     for (int step = 0; step < nsteps; step++) {
         if constexpr (MODE == TILES) {
-            await_tiles<ST>(ex, g, step);
+            await_tile(ex.full + step % ST, (step / ST) & 1, step, &ex.abort, &ex.filled, threadIdx.x == 0, g);
         } else {
             __syncwarp();                                           // (all lanes are done with the slot that is filled now)
             if (step + ST - 1 < nsteps) start(step + ST - 1);
@@ -432,7 +442,7 @@ __global__ void __launch_bounds__(256, 2) k_rec_fwd(const __grid_constant__ RecA
         ex.seg[side][warp][lane] = make_float4(P.x, P.y, hl.x, hl.y);
         if (MODE == TILES && lane == 0) sm100::tma_store_wait_read();                   // (of the block before: its stage is filled next)
         __syncthreads();
-        if (MODE == TILES && threadIdx.x == 0 && step > 0 && step + ST - 1 < nsteps) start(step + ST - 1);
+        if (MODE == TILES && threadIdx.x == 0 && step > 0 && step + ST - 1 < nsteps && !given_up(&ex.abort)) start(step + ST - 1);
         f2 hs = h;                                                  // before this warp's segment
 #pragma unroll
         for (int w = 0; w < NW; w++) {
@@ -470,7 +480,7 @@ __global__ void __launch_bounds__(256, 2) k_rec_fwd(const __grid_constant__ RecA
         }
     }
     if (MODE == TILES && lane == 0) sm100::tma_store_wait_all();
-    if (MODE == TILES && threadIdx.x == 0) let_copies_land(&ex.abort);
+    if (MODE == TILES && threadIdx.x == 0) let_tiles_land<ST>(ex.full, ex.filled, g.limit);
     if (g.state_out != nullptr && warp == 0 && span == g.nspan - 1) {
         if (ch < g.D) g.state_out[(size_t)b * g.D + ch] = h.x;
         if (ch + 1 < g.D) g.state_out[(size_t)b * g.D + ch + 1] = h.y;
@@ -511,8 +521,9 @@ __global__ void __launch_bounds__(256, 2) k_rec_bwd(const __grid_constant__ RecA
         const long long t0 = begin + (long long)(nsteps - 1 - k) * BT;
         F *slot = ring + (k % ST) * NT * SLOT;
         if constexpr (MODE == TILES) {
-            if (k == g.skip) return;
             sm100::mbar_expect_tx(ex.full + k % ST, NT * SLOT * sizeof(F));
+            ex.filled.asked = k + 1;
+            if (k == g.skip) return;
 #pragma unroll
             for (int i = 0; i < NT; i++) sm100::tma_load_3d(slot + i * SLOT, g.in + i, ex.full + k % ST, ch0, (int)t0, b);
         } else {
@@ -547,7 +558,7 @@ __global__ void __launch_bounds__(256, 2) k_rec_bwd(const __grid_constant__ RecA
             if (ch + 1 < g.D) h.y = c[1];
         }
         if constexpr (MODE == TILES) {
-            await_tiles<ST>(ex, g, k);
+            await_tile(ex.full + k % ST, (k / ST) & 1, k, &ex.abort, &ex.filled, threadIdx.x == 0, g);
         } else {
             __syncwarp();
             if (k + ST - 1 < nsteps) start(k + ST - 1);
@@ -606,7 +617,7 @@ __global__ void __launch_bounds__(256, 2) k_rec_bwd(const __grid_constant__ RecA
         ex.segE[side][warp][lane] = El;
         if (MODE == TILES && lane == 0) sm100::tma_store_wait_read();
         __syncthreads();
-        if (MODE == TILES && threadIdx.x == 0 && k > 0 && k + ST - 1 < nsteps) start(k + ST - 1);
+        if (MODE == TILES && threadIdx.x == 0 && k > 0 && k + ST - 1 < nsteps && !given_up(&ex.abort)) start(k + ST - 1);
         f2 Es = E;                                                  // behind this warp's segment
 #pragma unroll
         for (int w = NW - 1; w > 0; w--)
@@ -671,7 +682,7 @@ __global__ void __launch_bounds__(256, 2) k_rec_bwd(const __grid_constant__ RecA
         }
     }
     if (MODE == TILES && lane == 0) sm100::tma_store_wait_all();
-    if (MODE == TILES && threadIdx.x == 0) let_copies_land(&ex.abort);
+    if (MODE == TILES && threadIdx.x == 0) let_tiles_land<ST>(ex.full, ex.filled, g.limit);
     if (g.gs_in != nullptr && warp == 0 && span == 0) {
         if (ch < g.D) g.gs_in[(size_t)b * g.D + ch] = E.x;
         if (ch + 1 < g.D) g.gs_in[(size_t)b * g.D + ch + 1] = E.y;
@@ -699,6 +710,7 @@ __global__ void __launch_bounds__(256, 2) k_rec_spans(const __grid_constant__ Re
     __shared__ float4 seg[NW][32];
     __shared__ uint64_t bars[NW][ST];
     __shared__ int abort;
+    __shared__ Filled filled[NW];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     // (the last span forward and the first one backward are not needed)
     const int n1 = g.nspan - 1, span = blockIdx.x % n1 + BACK, chain = blockIdx.x / n1, b = chain / g.slabs, ch0 = (chain - b * g.slabs) * CH, ch = ch0 + 2 * lane;
@@ -719,9 +731,11 @@ __global__ void __launch_bounds__(256, 2) k_rec_spans(const __grid_constant__ Re
         const long long t0 = at_step(k);
         F *slot = ring + (k % ST) * NT * SLOT;
         if constexpr (MODE == TILES) {
-            if (lane == 0 && k != g.skip) {
+            if (lane == 0) {
                 uint64_t *bar = &bars[warp][k % ST];
                 sm100::mbar_expect_tx(bar, NT * SLOT * sizeof(F));
+                filled[warp].asked = k + 1;
+                if (k == g.skip) return;
                 sm100::tma_load_3d(slot, g.in_spans, bar, ch0, (int)t0, b);
                 sm100::tma_load_3d(slot + SLOT, g.in_spans + (BACK ? 3 : 1), bar, ch0, (int)t0, b);
                 if (!BACK || Z) sm100::tma_load_3d(slot + 2 * SLOT, g.in_spans + (BACK ? 4 : 2), bar, ch0, (int)t0, b);
@@ -742,6 +756,7 @@ __global__ void __launch_bounds__(256, 2) k_rec_spans(const __grid_constant__ Re
     if constexpr (MODE == TILES) {
         if (lane == 0) {
             for (int i = 0; i < ST; i++) sm100::mbar_init(&bars[warp][i], 1);
+            filled[warp] = {0, NEVER};
             sm100::fence_mbar_init();
         }
         if (threadIdx.x == 0) abort = 0;
@@ -755,12 +770,9 @@ __global__ void __launch_bounds__(256, 2) k_rec_spans(const __grid_constant__ Re
     f2 P = both(1.f), h = both(0.f);
     for (int k = 0; k < nsteps; k++) {
         __syncwarp();
-        if (k + ST - 1 < nsteps) start(k + ST - 1);
+        if (k + ST - 1 < nsteps && (MODE != TILES || !given_up(&abort))) start(k + ST - 1);
         if constexpr (MODE == TILES) {
-            if (!sm100::mbar_wait_or_abort(&bars[warp][k % ST], (k / ST) & 1, &abort, g.limit)) {
-                *(volatile int *)&abort = 1;
-                if (g.status != nullptr) atomicOr(g.status, WKV_RECURRENCE_TIMEOUT);
-            }
+            await_tile(&bars[warp][k % ST], (k / ST) & 1, k, &abort, filled + warp, lane == 0, g);
         } else {
             cp_commit();
             cp_wait<ST - 1>();
@@ -805,7 +817,7 @@ __global__ void __launch_bounds__(256, 2) k_rec_spans(const __grid_constant__ Re
         }
     }
     if constexpr (MODE == TILES) {
-        if (lane == 0) let_copies_land(&abort);
+        if (lane == 0) let_tiles_land<ST>(bars[warp], filled[warp], g.limit);
     }
     seg[warp][lane] = make_float4(P.x, P.y, h.x, h.y);
     __syncthreads();
