@@ -16,10 +16,14 @@
 // inputs that are in registers by then; rows that are not made of 16-byte pieces are copied by their warps (cp.async, in words).
 //
 // What bounds it (4 x 4096 x 4096 in bf16 with z, two CTAs of 256 threads an SM): forward 166 us (4.0 TB/s; the bytes take 103 at the copy
-// rate), backward 284 (4.2; 185).  No single resource: special functions are busy for 63 % of the time on an SM with two CTAs (6 a token and
+// rate), backward 294 (4.1; 185).  No single resource: special functions are busy for 63 % of the time on an SM with two CTAs (6 a token and
 // channel: 4 exponentials, a root, and one reciprocal for the three sigmoids; one each took 217 us), issue 55 %, HBM 62 %; 256 CTAs are 1.73 an SM.
-// Segments of 4 tokens instead of 8: 185 and 306 (folds and barriers twice as often).  Registers are what limits the segment: what does not
-// fit waits for L2 (forward 475 us with 40 bytes a thread of that), so that backward d and e go to shared memory, into the places of the gates.
+// Segments of 4 tokens instead of 8: 185 and 306 (of 284) (folds and barriers twice as often).  Registers are what limits the segment: what does not
+// fit waits for L2 (forward 475 us with 40 bytes a thread of that), so that backward d and e go to shared memory, into the places of the gates, and
+// 1 - i beside the ring.
+//
+// What is left of an open gate, 1 - i and 1 - r, has digits of its own: e^-x times the sigmoid, not a difference (which was 12 % off at a gate of 12).
+// Backward 294 us for 284; kept as differences' parts in registers, with the quotient of L and 1 - a^2 formed again, 324.
 //
 // Few chains: a row is cut into spans that run in parallel.  A first pass leaves what a span does to the state (its decay and its state
 // from zero; backward: to E), without a barrier: its warps take an eighth of a span each.  The full pass starts from the fold of the
@@ -77,7 +81,7 @@ struct RecArgs {
 enum { TILES = 0, WORDS = 1, ANYWHERE = 2 };
 // elements of a token's row in the ring: CH channels, and where rows start at any element one more word, because they are copied from the word that
 // their first element is in (which is of the same allocation: those start and end at words)
-__host__ __device__ constexpr int row_of(int mode) { return mode == ANYWHERE ? CH + 4 : CH; }
+__host__ __device__ constexpr int row_of(int mode) { return mode == ANYWHERE ? CH + 2 : CH; }
 
 // Tokens of a warp in a block (S), for two CTAs an SM: what a thread keeps of its tokens has to fit in 128 registers, because what
 // does not would wait for L2 (shared memory leaves no L1).
@@ -85,7 +89,7 @@ template <typename F, bool BACK>
 struct Geo {
     static constexpr int S = sizeof(F) == 2 ? 8 : 4, BT = NW * S;
     static __host__ __device__ constexpr int slot(int mode) { return BT * row_of(mode); }                             // elements of one tensor's block
-    static constexpr int STAGES = BACK ? 2 : 3;
+    static constexpr int STAGES = BACK ? 2 : 3, KEPT = BT * 32 * 8;                      // KEPT (backward): 1 - i of a block, two channels a lane
     static constexpr int ring(bool z, int mode) { return STAGES * (3 + BACK + z) * slot(mode) * (int)sizeof(F); }
 };
 // tokens between two states that are kept: a block of the backward pass
@@ -113,19 +117,18 @@ __device__ __forceinline__ Rate rate_of(float p, float c) {
 // of them has left the range; else (gates below -28 or so, infinities, NaNs, which would spread from one gate to the others) the
 // caller takes the segment again with FAST = false: a reciprocal for each there, and the same bits for all others.
 constexpr float RANGE = 4.2535296e37f;
-template <bool Z, bool FAST>
-__device__ __forceinline__ void sigmoids(f2 rg, f2 ig, f2 z, f2 &r, f2 &i, f2 &s, f2 &range) {
+// REST: and e^-x of the decay gate (at most 3e38, whose sigmoid is zero), from which r and 1 - r follow, and 1 - i as e^-x times the sigmoid: the
+// difference would have no digits where a gate is open.
+template <bool Z, bool FAST, bool REST>
+__device__ __forceinline__ void sigmoids(f2 rg, f2 ig, f2 z, f2 &r, f2 &i, f2 &s, f2 &range, f2 &exp_r, f2 &rest_i) {
     // (a zero that the compiler does not know: it would keep what both ways have in common in registers, for all tokens)
     f2 zero = both(0.f);
     if (!FAST) asm volatile("mov.b32 %0, 0;" : "=f"(zero.x));
-    auto one_plus = [&](f2 x) {
-        const f2 e = FAST ? mul2(x, both(-LOG2E)) : mul2(add2(x, both(zero.x)), both(-LOG2E));
-        return add2(make_float2(ex2(e.x), ex2(e.y)), both(1.f));
-    };
-    const f2 pr = one_plus(rg), pi = one_plus(ig), ri = mul2(pr, pi);
+    auto exp_of = [&](f2 x) { return ex2(FAST ? mul2(x, both(-LOG2E)) : mul2(add2(x, both(zero.x)), both(-LOG2E))); };
+    const f2 er = exp_of(rg), ei = exp_of(ig), pr = add2(er, both(1.f)), pi = add2(ei, both(1.f)), ri = mul2(pr, pi);
     f2 d = ri;
     if (Z) {
-        const f2 pz = one_plus(z);
+        const f2 pz = add2(exp_of(z), both(1.f));
         d = mul2(ri, pz);
         const f2 inv = make_float2(rcp(d.x), rcp(d.y)), iz = mul2(inv, pz);
         r = mul2(iz, pi);
@@ -136,19 +139,34 @@ __device__ __forceinline__ void sigmoids(f2 rg, f2 ig, f2 z, f2 &r, f2 &i, f2 &s
         r = mul2(inv, pi);
         i = mul2(inv, pr);
     }
+    if (REST) {
+        exp_r = er;
+        rest_i = mul2(ei, i);
+    }
     range = add2(range, d);
     if (!FAST) {
+        if (REST) {
+            asm("min.NaN.f32 %0, %0, %1;" : "+f"(exp_r.x) : "f"(3e38f));
+            asm("min.NaN.f32 %0, %0, %1;" : "+f"(exp_r.y) : "f"(3e38f));
+        }
         if (!(d.x < RANGE)) {
             r.x = sigm(rg.x);
             i.x = sigm(ig.x);
             if (Z) s.x = sigm(z.x);
+            if (REST) rest_i.x = sigm(-ig.x);
         }
         if (!(d.y < RANGE)) {
             r.y = sigm(rg.y);
             i.y = sigm(ig.y);
             if (Z) s.y = sigm(z.y);
+            if (REST) rest_i.y = sigm(-ig.y);
         }
     }
+}
+template <bool Z, bool FAST>
+__device__ __forceinline__ void sigmoids(f2 rg, f2 ig, f2 z, f2 &r, f2 &i, f2 &s, f2 &range) {
+    f2 exp_r, rest_i;
+    sigmoids<Z, FAST, false>(rg, ig, z, r, i, s, range, exp_r, rest_i);
 }
 __device__ __forceinline__ bool in_range(f2 range) { return __all_sync(0xffffffffu, range.x + range.y < RANGE); }
 // Decays a of two channels and q = 1 - a^2; x = -2 L.  EXACT (fp32 tensors): below x = 1/4 the decay is its power series, too (y^7 / 5040 is left
@@ -297,7 +315,7 @@ struct Exchange {
     int abort;
     Filled filled;
 };
-struct ExchangeBack {
+struct alignas(16) ExchangeBack {
     float4 seg[2][NW][32];                // P, hl
     f2 segE[2][NW][32];                   // E from zero
     f2 sum[NW][32];
@@ -505,6 +523,8 @@ __global__ void __launch_bounds__(256, 2) k_rec_bwd(const __grid_constant__ RecA
 
     const Rate k0 = rate_of(ch < g.D ? g.decay[ch] : 0.f, g.c), k1 = rate_of(ch + 1 < g.D ? g.decay[ch + 1] : 0.f, g.c);
     const f2 rate = make_float2(k0.rate2, k1.rate2), x2 = make_float2(k0.x2, k1.x2);
+    const f2 rate_e = mul2(x2, both(-0.5f));                        // L = rate_e r
+    f2 *kept = reinterpret_cast<f2 *>(smem + RING + sizeof(ExchangeBack)) + warp * S * 32 + lane;       // [warp][S][lane]: 1 - i
     f2 E = make_float2(0.f, 0.f), total = make_float2(0.f, 0.f);
     if (g.gs_out != nullptr) {
         if (ch < g.D) E.x = g.gs_out[(size_t)b * g.D + ch];
@@ -569,8 +589,8 @@ __global__ void __launch_bounds__(256, 2) k_rec_bwd(const __grid_constant__ RecA
         F *slot = ring + (k % ST) * NT * SLOT + warp * S * ROW;
         const int n = (int)max(0ll, min((long long)S, g.T - (t0 + warp * S)));
         if (n < S) close_gates<F, MODE, S>(slot, n, lane);
-        // i is m i / m, and 1 / (1 - a^2) the square of 1 / m.
-        f2 a[S], r[S], mi[S], rs[S], sz[Z ? S : 1], P, hl, El = both(0.f);
+        // er: e^-x of the decay gate.  i is m i / m, and 1 / (1 - a^2) the square of 1 / m.
+        f2 a[S], er[S], mi[S], rs[S], sz[Z ? S : 1], P, hl, El = both(0.f);
         auto segment = [&](auto fast) {
             f2 range = both(0.f);
             P = both(1.f);
@@ -580,14 +600,14 @@ __global__ void __launch_bounds__(256, 2) k_rec_bwd(const __grid_constant__ RecA
                 // (loads of all tokens at once would need registers that there are not: 200 bytes a thread went to L2)
                 if (s % 2 == 0) __syncwarp();
                 const f2 z = Z ? pair_at<F, MODE>(slot + 4 * SLOT, s, lane, odd_z) : both(0.f);
-                f2 in;
-                sigmoids<Z, decltype(fast)::value>(pair_at<F, MODE>(slot, s, lane, odd_r), pair_at<F, MODE>(slot + SLOT, s, lane, odd_i), z, r[s], in, sz[Z ? s : 0], range);
-                f2 q;
-                decays<sizeof(F) == 4>(r[s], rate, x2, a[s], q);
-                // (where 1 - a^2 is zero, so are L and m: any factor does; a NaN stays)
+                f2 r, in, rest, q;
+                sigmoids<Z, decltype(fast)::value, true>(pair_at<F, MODE>(slot, s, lane, odd_r), pair_at<F, MODE>(slot + SLOT, s, lane, odd_i), z, r, in, sz[Z ? s : 0], range, er[s], rest);
+                kept[s * 32] = rest;
+                decays<sizeof(F) == 4>(r, rate, x2, a[s], q);
+                // (where 1 - a^2 is zero, so are L and m: any factor does; the smallest normal number keeps its root, a NaN stays)
                 f2 low = q;
-                asm("max.NaN.f32 %0, %0, %1;" : "+f"(low.x) : "f"(1e-37f));
-                asm("max.NaN.f32 %0, %0, %1;" : "+f"(low.y) : "f"(1e-37f));
+                asm("max.NaN.f32 %0, %0, %1;" : "+f"(low.x) : "f"(1.17549435e-38f));
+                asm("max.NaN.f32 %0, %0, %1;" : "+f"(low.y) : "f"(1.17549435e-38f));
                 rs[s] = make_float2(rsqrta(low.x), rsqrta(low.y));
                 mi[s] = mul2(mul2(q, rs[s]), in);
                 hl = fma2(a[s], hl, mul2(mi[s], pair_at<F, MODE>(slot + 2 * SLOT, s, lane, odd_x)));
@@ -647,13 +667,14 @@ __global__ void __launch_bounds__(256, 2) k_rec_bwd(const __grid_constant__ RecA
 #pragma unroll
         for (int s = S - 1; s >= 0; s--) {
             const f2 v = mul2(mi[s], pair_at<F, MODE>(slot + 2 * SLOT, s, lane, odd_x));
-            const f2 aL = mul2(a[s], mul2(r[s], rate)), Gs = add2(kept_pair<F, MODE>(slot, slot + SLOT, s, lane), Es);
+            const f2 p1 = add2(er[s], both(1.f)), r = make_float2(rcp(p1.x), rcp(p1.y)), rest = mul2(er[s], r);
+            const f2 ar = mul2(a[s], rate_e), Gs = add2(kept_pair<F, MODE>(slot, slot + SLOT, s, lane), Es);
             Es = mul2(a[s], Gs);
-            const f2 gx = mul2(Gs, mi[s]), gi = mul2(mul2(Gs, v), sub2(both(1.f), mul2(mi[s], rs[s])));
-            // G (h a L - i x a^2 L / m), i / m = m i / m^2
-            const f2 gLL = mul2(Gs, sub2(mul2(hb[s], aL), mul2(mul2(mul2(v, rs[s]), rs[s]), mul2(a[s], aL))));
+            const f2 gx = mul2(Gs, mi[s]), gi = mul2(mul2(Gs, v), kept[s * 32]);
+            // G (h a L - i x a^2 L / m), i / m = m i / m^2; r first, which alone may be as small as 1 / m^2 is large
+            const f2 gLL = mul2(Gs, sub2(mul2(hb[s], mul2(ar, r)), mul2(mul2(mul2(mul2(mul2(v, rs[s]), rs[s]), r), a[s]), ar)));
             total = add2(total, gLL);
-            const f2 gr = mul2(gLL, fma2(r[s], both(-LN2), both(LN2)));
+            const f2 gr = mul2(gLL, rest);
             const f2 gz = Z ? mul2(kept_pair<F, MODE>(slot + 4 * SLOT, slot + 3 * SLOT, s, lane), hb[s + 1]) : both(0.f);
             if constexpr (MODE == TILES) {
                 put_pair(slot, s, lane, gr);
@@ -694,8 +715,8 @@ __global__ void __launch_bounds__(256, 2) k_rec_bwd(const __grid_constant__ RecA
 #pragma unroll
             for (int w = 1; w < NW; w++) total = add2(total, ex.sum[w][lane]);
             float *p = g.part + ((size_t)b * g.nspan + span) * g.D + ch;
-            if (ch < g.D) p[0] = total.x * (LN2 * k0.ratio);
-            if (ch + 1 < g.D) p[1] = total.y * (LN2 * k1.ratio);
+            if (ch < g.D) p[0] = total.x * k0.ratio;
+            if (ch + 1 < g.D) p[1] = total.y * k1.ratio;
         }
     }
 }
@@ -981,7 +1002,7 @@ int launch_as(const RecArgs &g, int B, cudaStream_t s) {
         const int rc = launch_rec(k_rec_spans<F, Z, MODE, BACK>, g, chains * (g.nspan - 1), smem, done[1], s);
         if (rc != WKV_OK) return rc;
     }
-    if constexpr (BACK) return launch_rec(k_rec_bwd<F, Z, MODE>, g, chains * g.nspan, Geo<F, true>::ring(Z, MODE) + (int)sizeof(ExchangeBack), done[0], s);
+    if constexpr (BACK) return launch_rec(k_rec_bwd<F, Z, MODE>, g, chains * g.nspan, Geo<F, true>::ring(Z, MODE) + (int)sizeof(ExchangeBack) + Geo<F, true>::KEPT, done[0], s);
     else return launch_rec(k_rec_fwd<F, Z, MODE>, g, chains * g.nspan, Geo<F, false>::ring(Z, MODE) + (int)sizeof(Exchange), done[0], s);
 }
 // the tiles' maps; false: TMA cannot read or write these rows

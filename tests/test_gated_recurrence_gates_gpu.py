@@ -5,7 +5,9 @@ are relative.
 In units of 2^-24 (U): a sigmoid of x and its complement, sigmoid(-x), are off by 4|x| + 16 relative to themselves (an exponential by 2|x| + 4, the
 sum and the quotient by 4, their product by 1), a decay a = e^L by |L| times the error of L, and 5, the root m of 1 - a^2 by half of the error of
 1 - a^2: its series by 8 and by the error of L, above it 7 decays' and 5.  G adds one decay and 3 a token, and 40 for what regrouping tokens
-into segments changes.  What a normal fp32 number cannot hold is flushed to zero."""
+into segments changes.  What a normal fp32 number cannot hold is flushed to zero: a sigmoid r below 2^-126 makes 1 - a^2 too small by up to 2 c
+softplus(p) 2^-126, one of 1 - a^2 below it by up to 2^-126, and m by no more than the root of that (`lost`); i x a^2 L / m is then i x m / 2, and half as
+much is missing of it; a flushed L is missing in h a L."""
 import pytest
 import torch
 
@@ -40,6 +42,8 @@ def ref(x, ig, rg, p, h0, gy):
     dL = ds(rg) + (13 + 2.4 * p.abs()) * U
     da = L.abs() * dL + 5 * U
     dm = 0.5 * (dL + 8 * U) + 3.5 * da + 7 * U
+    sp = torch.nn.functional.softplus(p)
+    lost = torch.where((r < 2.0 ** -126) | (q < 2.0 ** -126), (2 * C * sp).clamp_min(1.0).sqrt() * 2.0 ** -63, 0.0)
     hs, h = [h0], h0
     for t in range(T):
         h = a[:, t] * h + m[:, t] * i[:, t] * x[:, t]
@@ -59,7 +63,9 @@ def ref(x, ig, rg, p, h0, gy):
     gLL = G * (t1 + t2)
     egLL = G * (t1.abs() * (dG + dh + da + dL + 4 * U) + t2.abs() * (dG + 2 * da + dL + dm + ds(ig) + 10 * U)) + G * (t1.abs() + t2.abs()) * U
     gr = torch.sigmoid(-rg)
-    return {"gx": (gx, gx * dgx), "ginput": (gi, gi * (dgx + ds(ig) + 2 * U)), "gdecay_gate": (gLL * gr, gr * (egLL + gLL.abs() * (ds(rg) + 2 * U)))}
+    egLL = egLL + G * i * x * lost / 2 + G * h[:, :-1] * (C * sp).clamp_min(1.0) * 2.0 ** -126 * (lost > 0)
+    return {"gx": (gx, gx * dgx + G * i * lost), "ginput": (gi, gi * (dgx + ds(ig) + 2 * U) + G * i * x * torch.sigmoid(-ig) * lost),
+            "gdecay_gate": (gLL * gr, gr * (egLL + gLL.abs() * (ds(rg) + 2 * U)))}
 
 
 def inputs(seed, T, D, dtype, low=-1.0, high=1.0):
@@ -86,6 +92,19 @@ def test_open_and_closed_gates(gate, T, D, dtype):
 def test_gates_far_out(gate, value):
     c = inputs(1, 9, 72, F32, -9.0, -3.0)
     c[gate] = torch.full_like(c[gate], value)
+    got, want = gradients(**c), ref(**c)
+    for n in want:
+        close(n, got[n], *want[n])
+
+
+@pytest.mark.parametrize("D", [72, 71])
+def test_decays_next_to_one(D):
+    """1 - a^2 from the smallest normal number on: its root is that of the forward pass"""
+    c = inputs(2, 1, D, F32)
+    c["p"] = torch.full_like(c["p"], -5.07)                       # 2 c softplus(p) = 0.1
+    c["rg"] = torch.linspace(-84.8, -80.0, D).expand(2, 1, D).contiguous().cuda()
+    q = -torch.expm1(-2 * C * torch.nn.functional.softplus(c["p"].double()) * torch.sigmoid(c["rg"].double()))
+    assert 2.0 ** -126 * (1 + 400 * U) < float(q.min()) < 2e-38
     got, want = gradients(**c), ref(**c)
     for n in want:
         close(n, got[n], *want[n])
