@@ -16,14 +16,14 @@
 // inputs that are in registers by then; rows that are not made of 16-byte pieces are copied by their warps (cp.async, in words).
 //
 // What bounds it (4 x 4096 x 4096 in bf16 with z, two CTAs of 256 threads an SM): forward 166 us (4.0 TB/s; the bytes take 103 at the copy
-// rate), backward 294 (4.1; 185).  No single resource: special functions are busy for 63 % of the time on an SM with two CTAs (6 a token and
+// rate), backward 297 (4.0; 185).  No single resource: special functions are busy for 63 % of the time on an SM with two CTAs (6 a token and
 // channel: 4 exponentials, a root, and one reciprocal for the three sigmoids; one each took 217 us), issue 55 %, HBM 62 %; 256 CTAs are 1.73 an SM.
 // Segments of 4 tokens instead of 8: 185 and 306 (of 284) (folds and barriers twice as often).  Registers are what limits the segment: what does not
 // fit waits for L2 (forward 475 us with 40 bytes a thread of that), so that backward d and e go to shared memory, into the places of the gates, and
 // 1 - i beside the ring.
 //
 // What is left of an open gate, 1 - i and 1 - r, has digits of its own: e^-x times the sigmoid, not a difference (which was 12 % off at a gate of 12).
-// Backward 294 us for 284; kept as differences' parts in registers, with the quotient of L and 1 - a^2 formed again, 324.
+// Backward 297 us for 284; kept as differences' parts in registers, with the quotient of L and 1 - a^2 formed again, 324.
 //
 // Few chains: a row is cut into spans that run in parallel.  A first pass leaves what a span does to the state (its decay and its state
 // from zero; backward: to E), without a barrier: its warps take an eighth of a span each.  The full pass starts from the fold of the
@@ -623,11 +623,12 @@ __global__ void __launch_bounds__(256, 2) k_rec_bwd(const __grid_constant__ RecA
             __syncwarp();             // (ANYWHERE: a neighbour reads this lane's words.  All: loads moved up would need registers that there are not)
             f2 d = pair_at<F, MODE>(slot + 3 * SLOT, s, lane, odd_g);
             if (Z) {
-                // silu' = s (1 + z (1 - s))
-                const f2 z = pair_at<F, MODE>(slot + 4 * SLOT, s, lane, odd_z), gs = mul2(d, sz[Z ? s : 0]);
+                // silu' = sz (1 + z (1 - sz)).  From 17 on z (1 - sz) is below 7e-7, and the difference is made of sz's roundings: with 17 in place of a
+                // larger z they stay below 3e-6.
+                const f2 z = pair_at<F, MODE>(slot + 4 * SLOT, s, lane, odd_z), gs = mul2(d, sz[Z ? s : 0]), zc = make_float2(fminf(z.x, 17.f), fminf(z.y, 17.f));
                 d = mul2(gs, z);
                 if (MODE == ANYWHERE) __syncwarp();
-                keep_pair<F, MODE>(slot + 4 * SLOT, slot + 3 * SLOT, s, lane, mul2(gs, fma2(z, sub2(both(1.f), sz[Z ? s : 0]), both(1.f))));
+                keep_pair<F, MODE>(slot + 4 * SLOT, slot + 3 * SLOT, s, lane, mul2(gs, fma2(zc, sub2(both(1.f), sz[Z ? s : 0]), both(1.f))));
             }
             keep_pair<F, MODE>(slot, slot + SLOT, s, lane, d);
             El = mul2(a[s], add2(d, El));

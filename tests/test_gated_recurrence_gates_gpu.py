@@ -108,3 +108,27 @@ def test_decays_next_to_one(D):
     got, want = gradients(**c), ref(**c)
     for n in want:
         close(n, got[n], *want[n])
+
+
+@pytest.mark.parametrize("D", [68, 69])
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_output_gates_far_out(D, dtype):
+    """the gradient of z, gy h s (1 + z (1 - s)): off by the errors of h, of s and of 1 - s, the latter where z carries them"""
+    c = inputs(3, 9, D, dtype)
+    z = [-3e38, -100.0, -30.0, -5.0, -1.5, 0.0, 0.5, 3.0, 8.0, 12.0, 20.0, 50.0, 90.0, 1e3, 1e4, 1e6, 1e20, 3e38]
+    z = torch.tensor((z * 4)[:D]).expand(2, 9, D).contiguous().to(dtype).cuda()
+    got = gradients(**c, z=z)["gz"]
+    x, ig, rg, p, h, gy, z = (t.double() for t in (c["x"], c["ig"], c["rg"], c["p"], c["h0"], c["gy"], z))
+    L = -C * torch.nn.functional.softplus(p) * torch.sigmoid(rg)
+    a, m = torch.exp(L), torch.sqrt(-torch.expm1(2 * L))
+    da = L.abs() * (ds(rg) + (13 + 2.4 * p.abs()) * U) + 5 * U
+    hs = []
+    for t in range(9):
+        h = a[:, t] * h + m[:, t] * torch.sigmoid(ig[:, t]) * x[:, t]
+        hs.append(h)
+    h = torch.stack(hs, 1)
+    dh = 9 * (da + 0.5 * ds(rg) + 3.5 * da + ds(ig) + (0.5 * (21 + 2.4 * p.abs()) + 13) * U).amax(1, keepdim=True) + 40 * U
+    s, rest = torch.sigmoid(z), torch.sigmoid(-z)
+    want = gy * h * s * (1 + z * rest)
+    err = gy * h * s * (1 + z.abs() * rest) * (dh + 2 * ds(z).clamp_max(1.0) + 4 * U)
+    close("gz", got, want, err)
