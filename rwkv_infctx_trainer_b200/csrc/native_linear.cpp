@@ -75,38 +75,50 @@ LinearCall linear_call(const Tensor &x, const Tensor &w0, const Tensor &w1, cons
     return c;
 }
 
+// What is kept depends on which gradients are wanted: x for those of the matrices, the matrices for that of x, mul and the pre-activations for any but the
+// residual's.  (A frozen matrix' x may go, or change, before the backward pass.)
 struct LinearBackward : OpNode {
     int act;
     bool pair;
-    at::ScalarType b_type;
+    int64_t rows, K, N;
+    std::vector<int64_t> x_sizes;
+    at::ScalarType b_type, b_kept;
     std::string name() const override { return pair ? "GatedLinearBackward" : "LinearActBackward"; }
     // inputs: x, w0, then of a pair w1, else bias, mul, residual
     variable_list gradients(variable_list &&grads) override {
         at::AutoDispatchBelowADInplaceOrView below;
         const variable_list st = unpack();
-        const Tensor &x = st[0], &w0 = st[1], &w1 = st[2], &bias = st[3], &mul = st[4];
-        const Tensor saved = st[5].defined() ? contig(st[5]) : st[5];
         if (!grads[0].defined()) return variable_list(pair ? 3 : 5);
-        c10::cuda::OptionalCUDAGuard guard(x.device());
-        poll_status(x.device().index(), false);
-        LinearCall c = linear_call(x, w0, w1, bias, mul, Tensor(), act);
-        wkv_linear_args_t &a = c.a;
-        const auto dt = x.scalar_type();
-        Tensor gy = contig(grads[0]);
+        const Tensor gy = contig(grads[0]);
         auto want = [&](size_t i) { return task_should_compute_output(i); };
+        auto matrix = [&](const Tensor &t) { return t.defined() ? matrix_of(t) : Mat(); };
+        const Mat x = matrix(st[0]), w0 = matrix(st[1]), w1 = matrix(st[2]);
+        const Tensor mul = st[3].defined() ? contig(st[3]) : st[3], saved = st[4].defined() ? contig(st[4]) : st[4];
+        const auto dt = gy.scalar_type();
+        c10::cuda::OptionalCUDAGuard guard(gy.device());
+        poll_status(gy.device().index(), false);
         Tensor gx, gw0, gw1, gb, gm;
-        if (want(0)) gx = fresh(x.sizes(), dt, x);
-        if (want(1)) gw0 = fresh(w0.sizes(), dt, x);
-        if (pair && want(2)) gw1 = fresh(w1.sizes(), dt, x);
-        if (!pair && want(2)) gb = fresh(bias.sizes(), c.bias.scalar_type(), x);
-        if (!pair && want(3)) gm = fresh(mul.sizes(), dt, x);
+        if (want(0)) gx = fresh(x_sizes, dt, gy);
+        if (want(1)) gw0 = fresh({N, K}, dt, gy);
+        if (pair && want(2)) gw1 = fresh({N, K}, dt, gy);
+        if (!pair && want(2)) gb = fresh({N}, b_kept, gy);
+        if (!pair && want(3)) gm = fresh(gy.sizes(), dt, gy);
+        wkv_linear_args_t a = {};
+        a.rows = rows; a.K = K; a.N = N;
+        a.dtype = dtype_code(dt); a.bias_dtype = dtype_code(b_kept);
+        a.act = act; a.pair = pair;
+        a.x = ptr(x.t); a.w0 = ptr(w0.t); a.w1 = ptr(w1.t); a.mul = ptr(mul);
+        a.x_row = x.row; a.w0_row = w0.row; a.w1_row = w1.row;
+        a.status = status_word(gy.device().index());
         a.gy = ptr(gy); a.gx = ptr(gx); a.gw0 = ptr(gw0); a.gw1 = ptr(gw1); a.gbias = ptr(gb); a.gmul = ptr(gm);
         a.saved = ptr(saved);
         a.saved_bytes = saved.defined() ? (size_t)saved.numel() : 0;
-        a.workspace_bytes = wkv_linear_backward_workspace(&a);
-        Tensor ws = bytes_like(x, a.workspace_bytes);
-        a.workspace = ptr(ws);
-        check(wkv_linear_backward(&a, stream_of(x)), "wkv_linear_backward");
+        if (gx.defined() || gw0.defined() || gw1.defined() || gb.defined() || gm.defined()) {
+            a.workspace_bytes = wkv_linear_backward_workspace(&a);
+            Tensor ws = bytes_like(gy, a.workspace_bytes);
+            a.workspace = ptr(ws);
+            check(wkv_linear_backward(&a, stream_of(gy)), "wkv_linear_backward");
+        }
         if (pair) return {gx, gw0, gw1};
         return {gx, gw0, gb.defined() ? gb.to(b_type) : gb, gm, want(4) ? grads[0] : Tensor()};
     }
@@ -123,7 +135,11 @@ Tensor linear_forward(const Tensor &x, const Tensor &w0, const Tensor &w1, const
         else node = make_node<LinearBackward>({x, w0, bias, mul, residual});
         node->act = act;
         node->pair = w1.defined();
-        node->b_type = bias.defined() ? bias.scalar_type() : at::kFloat;
+        node->b_type = node->b_kept = at::kFloat;
+        if (bias.defined()) {
+            node->b_type = bias.scalar_type();
+            node->b_kept = param_type(bias);
+        }
     }
     Tensor y;
     {
@@ -132,8 +148,10 @@ Tensor linear_forward(const Tensor &x, const Tensor &w0, const Tensor &w1, const
         wkv_linear_args_t &a = c.a;
         y = fresh(out_sizes(x, a.N), x.scalar_type(), x);
         a.y = ptr(y);
+        const auto grad = [&](const Tensor &t) { return save && t.defined() && t.requires_grad(); };
+        const bool of_x = grad(x), of_w = grad(w0) || grad(w1), any = of_x || of_w || grad(bias) || grad(mul);
         Tensor saved;
-        if (save) {
+        if (any) {
             a.saved_bytes = wkv_linear_saved_bytes(&a);
             saved = bytes_like(x, a.saved_bytes);
             a.saved = ptr(saved);
@@ -142,7 +160,12 @@ Tensor linear_forward(const Tensor &x, const Tensor &w0, const Tensor &w1, const
         Tensor ws = bytes_like(x, a.workspace_bytes);
         a.workspace = ptr(ws);
         check(wkv_linear_forward(&a, stream_of(x)), "wkv_linear_forward");
-        if (save) node->keep({c.x.t, c.w0.t, c.w1.t, c.bias, c.mul, saved});
+        if (save) {
+            node->rows = a.rows; node->K = a.K; node->N = a.N;
+            node->x_sizes = x.sizes().vec();
+            const Tensor none;
+            node->keep({of_w ? c.x.t : none, of_x ? c.w0.t : none, of_x ? c.w1.t : none, any ? c.mul : none, saved});
+        }
     }
     if (save) torch::autograd::set_history(y, node);
     return y;
