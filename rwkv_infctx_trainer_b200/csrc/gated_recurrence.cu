@@ -347,7 +347,7 @@ __device__ __forceinline__ bool given_up(const int *abort) { return *(volatile c
 // Before the CTA's shared memory may go: what was asked for and not waited for has landed (bounded).
 template <int ST>
 __device__ __forceinline__ void let_tiles_land(uint64_t *bars, const Filled &f, unsigned limit) {
-    for (int k = f.lost; k < f.asked; k++) sm100::mbar_wait(bars + k % ST, (k / ST) & 1, limit);
+    for (int k = f.lost; k < f.asked; k++) sm100::mbar_wait_landed(bars + k % ST, (k / ST) & 1, limit);
 }
 // two channels' state (or E) behind the spans from `first` up to `last`
 __device__ __forceinline__ f2 fold_spans(const RecArgs &g, int b, int first, int last, int dir, int ch, f2 h) {

@@ -113,6 +113,10 @@ __device__ __forceinline__ bool mbar_wait_or_abort(uint64_t *bar, uint32_t parit
     return ok != 0;
 }
 
+// The same for copies in flight that a kernel which gives up must still wait for, before its shared memory may go: not cut short by a small limit (a copy
+// takes microseconds, this many polls a fraction of a millisecond at least).
+__device__ __forceinline__ void mbar_wait_landed(uint64_t *bar, uint32_t parity, uint32_t limit) { mbar_wait(bar, parity, limit > 20000u ? limit : 20000u); }
+
 // ---------------------------------------------------------------------- TMA
 // 3-D tiled load (coordinates: c0 innermost).  c0 * element size must be a
 // multiple of 16 bytes.
