@@ -461,8 +461,8 @@ int wkv56_selftest_abort(const wkv_args_t *a, int per_token_w, int backward_call
                          int skip_chunk, unsigned limit, void *stream);
 
 /* The same for the matrix products and the gated recurrence: a normal call in which block
- * `skip_block` (64 contraction steps of every CTA's first tile; a block of tokens of every CTA, whose stage counts on bytes that
- * do not come) is never loaded, with every wait cut to `limit` polls (1..100000).  Returns WKV_OK; the call's status word then has
+ * `skip_block` (64 contraction steps of every CTA's first tile, of a pair of CTAs the first one's half of them; a block of tokens of
+ * every CTA, whose stage counts on bytes that do not come) is never loaded, with every wait cut to `limit` polls (1..100000).  Returns WKV_OK; the call's status word then has
  * WKV_LINEAR_TIMEOUT or WKV_RECURRENCE_TIMEOUT set and the outputs are invalid.  (Calls that do not load tiles -- few
  * rows, a recurrence's rows that are not made of 16-byte pieces -- have no waits and run as ever.) */
 int wkv_linear_selftest_abort(const wkv_linear_args_t *a, int backward_call, int skip_block, unsigned limit, void *stream);

@@ -130,6 +130,9 @@ __device__ __forceinline__ uint32_t map_rank(const void *p, uint32_t rank) {
 __device__ __forceinline__ void arrive_remote(uint32_t bar) {
     asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
+__device__ __forceinline__ void store_remote(uint32_t at, uint32_t v) {
+    asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(at), "r"(v) : "memory");
+}
 __device__ __forceinline__ void cluster_sync() {
     asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
@@ -215,7 +218,7 @@ struct Tile {
     static constexpr int STAGES = (STAGE * 6 <= 196608) ? (196608 / STAGE > 8 ? 8 : 196608 / STAGE) : 5;
     static constexpr int TURN = EPI_WARPS * 4096;                                            // epilogue: 32 x 32 floats a warp
     static constexpr int BARS = STAGES * STAGE + TURN;
-    static constexpr int SMEM = BARS + (2 * STAGES + 2 * ACC) * 8 + 16 + 1024;                // (1024: alignment of the stages)
+    static constexpr int SMEM = BARS + (2 * STAGES + 2 * ACC) * 8 + 16 + 1024;                // (16: four words; 1024: alignment of the stages)
     static constexpr uint32_t COLS = ACC * BN;
 };
 
@@ -340,7 +343,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_gemm(const __grid_constant__ Gem
     unsigned char *smem = raw + ((1024 - (sm100::smem_u32(raw) & 1023)) & 1023);
     uint64_t *full = reinterpret_cast<uint64_t *>(smem + T::BARS), *empty = full + ST, *acc_full = empty + ST, *acc_empty = acc_full + ACC;
     uint32_t *tmem = reinterpret_cast<uint32_t *>(acc_empty + ACC);
-    volatile int *abort = reinterpret_cast<int *>(tmem + 1);
+    volatile int *abort = reinterpret_cast<int *>(tmem + 1), *asked = abort + 1;             // asked: stages each CTA of the pair has asked for (of the first CTA)
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t rank = CG == 2 ? cluster_rank() : 0;
     const int first = blockIdx.x / CG, step = gridDim.x / CG, items = g.main + g.rest * g.splits;
@@ -356,6 +359,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_gemm(const __grid_constant__ Gem
             sm100::mbar_init(acc_empty + i, CG * EPI_WARPS);
         }
         *abort = 0;
+        asked[0] = asked[1] = 0;
         sm100::fence_mbar_init();
         sm100::prefetch_tmap(g.a);
         sm100::prefetch_tmap(g.b);
@@ -395,7 +399,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_gemm(const __grid_constant__ Gem
                     ok = wait(empty + st, parity ^ 1);
                     if (!ok) break;
                     issued++;
-                    if (kb == g.skip && i == first) {
+                    if (kb == g.skip && i == first && rank == 0) {
                         if (++st == ST) { st = 0; parity ^= 1; }
                         continue;
                     }
@@ -422,18 +426,16 @@ __global__ void __launch_bounds__(THREADS, 1) k_gemm(const __grid_constant__ Gem
                     if (++st == ST) { st = 0; parity ^= 1; }
                 }
             }
-            // Before this CTA's shared memory may go: all stages read, and after an abort at least written.
+            // Before this CTA's shared memory may go: all stages read, and after an abort (below) at least written.
             for (int k = 0; k < ST && issued > 0; k++) {
                 if (ok && (unsigned)k < issued) {
                     const unsigned last = issued - 1 - k;
                     ok = wait(empty + last % ST, (last / ST) & 1);
                 }
             }
-            if (!ok && rank == 0) {
-                for (int k = 0; k < ST && (unsigned)k < issued; k++) {
-                    const unsigned last = issued - 1 - k;
-                    sm100::mbar_wait(full + last % ST, (last / ST) & 1, g.limit);
-                }
+            if (!ok) {
+                if (rank == 0) asked[0] = (int)issued;
+                else store_remote(map_rank(const_cast<int *>(asked) + 1, 0), issued);
             }
         }
         __syncwarp();
@@ -468,7 +470,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_gemm(const __grid_constant__ Gem
             if (!ok) {
                 // (products in flight read this shared memory and write this tensor memory)
                 commit<CG>(acc_full + buf);
-                sm100::mbar_wait(acc_full + buf, acc_parity, g.limit);
+                sm100::mbar_wait_landed(acc_full + buf, acc_parity, g.limit);
             }
         }
         __syncwarp();
@@ -580,7 +582,22 @@ __global__ void __launch_bounds__(THREADS, 1) k_gemm(const __grid_constant__ Gem
     }
     sm100::tc_fence_before();
     __syncthreads();
-    if (CG == 2) cluster_sync();
+    if (CG == 2) {
+        if (threadIdx.x == 0 && *abort) store_remote(map_rank(const_cast<int *>(abort), rank ^ 1), 1);
+        __syncwarp();
+        cluster_sync();
+    }
+    if (*abort) {
+        // (the same for both CTAs of a pair.)  Copies on their way: of the last ST stages that were asked for.  The second CTA's bytes are counted here, and where it was
+        // ahead nothing waits for them yet.
+        if (threadIdx.x == 0 && rank == 0) {
+            const int n0 = asked[0], n1 = CG == 2 ? asked[1] : 0, n = max(n0, n1);
+            for (int k = n0; n0 > 0 && k < n1; k++) sm100::mbar_expect_tx(full + k % ST, T::STAGE);
+            for (int k = max(0, n - ST); k < n; k++) sm100::mbar_wait_landed(full + k % ST, (k / ST) & 1, g.limit);
+        }
+        __syncwarp();
+        if (CG == 2) cluster_sync();
+    }
     sm100::tc_fence_after();
     if (warp == EPI_WARPS + 1) tmem_free<CG>(acc0, T::COLS);
 }
