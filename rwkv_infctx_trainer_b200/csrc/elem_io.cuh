@@ -124,12 +124,13 @@ struct alignas(N * sizeof(F) < 16 ? N * sizeof(F) : 16) Raw {
     }
 };
 
-// element i of a parameter of element type `dtype`.  Plain loads, which stay behind the checks in front of them: the 16-bit forms of __ldg are
-// instructions without an effect to the compiler, which may take them out of a loop and past the check for a parameter that is not there.
+// element i of a parameter of element type `dtype`.  Volatile, as __ldg of a float is: the 16-bit forms of __ldg are instructions without an effect to
+// the compiler, which may take them out of a loop and past the check for a parameter that is not there.
 __device__ __forceinline__ float param_at(const void *p, int dtype, size_t i) {
-    if (dtype == WKV_F32) return Elem<float>::ld((const float *)p + i);
-    if (dtype == WKV_BF16) return Elem<__nv_bfloat16>::ld((const __nv_bfloat16 *)p + i);
-    return Elem<__half>::ld((const __half *)p + i);
+    if (dtype == WKV_F32) return __ldg((const float *)p + i);
+    unsigned short v;
+    asm volatile("ld.global.nc.u16 %0, [%1];" : "=h"(v) : "l"((const unsigned short *)p + i));
+    return dtype == WKV_BF16 ? __uint_as_float((uint32_t)v << 16) : __half2float(__ushort_as_half(v));
 }
 
 inline bool known_dtype(int d) { return d == WKV_F32 || d == WKV_BF16 || d == WKV_F16; }

@@ -95,8 +95,14 @@ struct Epi {
     float *part;                      // sums of parts of a contraction: [tile][part][row of the tile][column of the tile]
 };
 
-// element i of the bias, 0 without one
-__device__ __forceinline__ float bias_at(const Epi &e, int i) { return e.bias == nullptr ? 0.f : param_at(e.bias, e.bias_dtype, i); }
+// Element i of the bias, 0 without one.  Plain loads: the compiler may move the 16-bit forms of __ldg, and did, out of a loop and in front of the
+// check.
+__device__ __forceinline__ float bias_at(const Epi &e, int i) {
+    if (e.bias == nullptr) return 0.f;
+    if (e.bias_dtype == WKV_F32) return Elem<float>::ld((const float *)e.bias + i);
+    if (e.bias_dtype == WKV_BF16) return Elem<__nv_bfloat16>::ld((const __nv_bfloat16 *)e.bias + i);
+    return Elem<__half>::ld((const __half *)e.bias + i);
+}
 
 struct GemmArgs {
     CUtensorMap a[2], b[2];
