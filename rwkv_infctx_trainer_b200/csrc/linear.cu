@@ -53,7 +53,7 @@ __device__ __forceinline__ void load_piece(Raw<F, 8> &r, const F *p, int n) {
 }
 
 // ------------------------------------------------------------------------------------------ few rows
-// A CTA has 16 rows of the matrix (of a pair: 8 of each), its 4 or 8 warps runs of 256 contraction steps in turn; the warps' sums meet
+// A CTA has 16 rows of the matrix (of a pair: 8 of each), its 4 or 8 warps runs of 256 contraction steps (for 32 rows of x 128) in turn; the warps' sums meet
 // in shared memory in a fixed order.  mma.sync with the matrix as the 16-row operand and the rows of x as the 8 columns: the
 // contraction steps may be numbered in any order that both operands share, so that a lane's 16-byte piece (8 steps of one row) is
 // its part of two instructions as it is, without a turn through shared memory.  (The tensor core's rate does not matter here.)
@@ -338,7 +338,7 @@ struct Cut {
     size_t part_bytes() const { return splits > 1 ? (size_t)rest * splits * (128 * cg) * bn * 4 : 0; }
 };
 // The cut that takes least by this estimate, in us, fitted to one B200 (`first`: a launch with its first and its last tile's latency; `block`: 64
-// contraction steps of a tile on every SM).  256 x 256 of two CTAs runs at the tensor cores' rate (8.4 million multiply-adds in 0.365 us); the other tiles are bound by
+// contraction steps of a tile on every SM).  256 x 256 of two CTAs runs at the tensor cores' rate (4.2 million multiply-adds of a pair in 0.365 us); the other tiles are bound by
 // their operands' way into an SM, about 60 bytes a cycle: 24 KB a block for 256 x 128 of two and 128 x 64 of one, 32 KB for 128 x 128 of one.  Cut
 // contractions cost a launch and their sums' way through L2.  (2048 x 2560 -> 2560, 80 tiles on 74 pairs: 28 us with the last 6 cut in four, 31 without;
 // 1500 x 8192 -> 1000, 24 tiles: 25 cut in three, 44 without.)

@@ -15,7 +15,8 @@ activation: ``"none"``, ``"silu"`` (z sigmoid(z)), ``"gelu"`` (z Phi(z), with th
 x, the matrices, mul, residual and y in bf16 or fp16 (of one type within a call; fp32 is refused: the tensor cores would take it
 at 10 bits).  Sums, bias, activation, product and residual are in fp32 and rounded once.  For the backward pass the
 pre-activations are kept in fp32 (where an activation or ``mul`` needs them); their gradient is rounded to x's type once, as an operand of the
-products (the bias' gradient is summed before that).  Any size and
+products (the bias' gradient is summed before that; in fp16 what is above 65504 there is an infinity).  Kept is what the wanted
+gradients need: x for those of the matrices, the matrices for that of x, ``mul`` and the pre-activations for any but the residual's.  Any size and
 alignment is taken; rows whose length or stride is no multiple of 8 elements are copied first, except in calls of few rows
 (up to 16, or 32 of a small matrix).
 """
