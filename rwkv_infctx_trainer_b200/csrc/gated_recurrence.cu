@@ -397,7 +397,7 @@ __global__ void __launch_bounds__(256, 2) k_rec_fwd(const __grid_constant__ RecA
         F *slot = ring + (step % ST) * NT * SLOT;
         if constexpr (MODE == TILES) {
             sm100::mbar_expect_tx(ex.full + step % ST, NT * SLOT * sizeof(F));
-            ex.filled.asked = step + 1;
+            ex.filled.asked++;
             if (step == g.skip) return;
 #pragma unroll
             for (int i = 0; i < NT; i++) sm100::tma_load_3d(slot + i * SLOT, g.in + i, ex.full + step % ST, ch0, (int)t0, b);
@@ -542,7 +542,7 @@ __global__ void __launch_bounds__(256, 2) k_rec_bwd(const __grid_constant__ RecA
         F *slot = ring + (k % ST) * NT * SLOT;
         if constexpr (MODE == TILES) {
             sm100::mbar_expect_tx(ex.full + k % ST, NT * SLOT * sizeof(F));
-            ex.filled.asked = k + 1;
+            ex.filled.asked++;
             if (k == g.skip) return;
 #pragma unroll
             for (int i = 0; i < NT; i++) sm100::tma_load_3d(slot + i * SLOT, g.in + i, ex.full + k % ST, ch0, (int)t0, b);
@@ -756,7 +756,7 @@ __global__ void __launch_bounds__(256, 2) k_rec_spans(const __grid_constant__ Re
             if (lane == 0) {
                 uint64_t *bar = &bars[warp][k % ST];
                 sm100::mbar_expect_tx(bar, NT * SLOT * sizeof(F));
-                filled[warp].asked = k + 1;
+                filled[warp].asked++;
                 if (k == g.skip) return;
                 sm100::tma_load_3d(slot, g.in_spans, bar, ch0, (int)t0, b);
                 sm100::tma_load_3d(slot + SLOT, g.in_spans + (BACK ? 3 : 1), bar, ch0, (int)t0, b);
