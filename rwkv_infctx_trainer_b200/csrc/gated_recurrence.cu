@@ -18,12 +18,12 @@
 // What bounds it (4 x 4096 x 4096 in bf16 with z, two CTAs of 256 threads an SM): forward 166 us (4.0 TB/s; the bytes take 103 at the copy
 // rate), backward 297 (4.0; 185).  No single resource: special functions are busy for 63 % of the time on an SM with two CTAs (6 a token and
 // channel: 4 exponentials, a root, and one reciprocal for the three sigmoids; one each took 217 us), issue 55 %, HBM 62 %; 256 CTAs are 1.73 an SM.
-// Segments of 4 tokens instead of 8: 185 and 306 (of 284) (folds and barriers twice as often).  Registers are what limits the segment: what does not
+// Segments of 4 tokens instead of 8: 185 and, of 284 then, 306 (folds and barriers twice as often).  Registers are what limits the segment: what does not
 // fit waits for L2 (forward 475 us with 40 bytes a thread of that), so that backward d and e go to shared memory, into the places of the gates, and
 // 1 - i beside the ring.
 //
 // What is left of an open gate, 1 - i and 1 - r, has digits of its own: e^-x times the sigmoid, not a difference (which was 12 % off at a gate of 12).
-// Backward 297 us for 284; kept as differences' parts in registers, with the quotient of L and 1 - a^2 formed again, 324.
+// Backward 297 us, 284 with the differences; 324 with the smaller of r and 1 - r in a register, 1 - i in another, and L / (1 - a^2) formed again.
 //
 // Few chains: a row is cut into spans that run in parallel.  A first pass leaves what a span does to the state (its decay and its state
 // from zero; backward: to E), without a barrier: its warps take an eighth of a span each.  The full pass starts from the fold of the

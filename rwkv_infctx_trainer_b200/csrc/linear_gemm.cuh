@@ -39,7 +39,7 @@ __device__ __forceinline__ float sigmoid_of(float x) { return __fdividef(1.f, 1.
 // Phi(z), and g = e^(-z^2 / 2).  For t = |z| the tail is g R(t), R(t) = erfcx(t / sqrt 2) / 2, a smooth function that falls from 1/2 as 0.4 / t:
 // w P(w) in w = 1 / (1 + 0.35 t), P of degree 8 fitted for the least largest relative error (with its rounded coefficients 3.7e-8 below t = 1, 5.7e-8 at 13).
 // A small tail keeps digits, which 1 + erf does not: g's exponent is rounded, so that in all it is off by 4e-7 of itself below t = 1, 2e-6 at 6 and 8e-6
-// at 13, 1/500 of half a step of the outputs' 16 bits.  (Through erfcf the epilogue of 1999 x 2560 -> 8960 took 128 us of a
+// at 13, 1/500 of half a step of bf16.  (Through erfcf the epilogue of 1999 x 2560 -> 8960 took 128 us of a
 // product's 78.)
 __device__ __forceinline__ float phi_of(float z, float &g) {
     const float t = fabsf(z), w = __fdividef(1.f, fmaf(0.35f, t, 1.f));

@@ -91,3 +91,29 @@ def test_what_is_not_kept_may_change():
     h.zero_()
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         torch.autograd.grad(y, w, c["gy"])
+
+
+def test_saved_on_the_host_and_formed_again():
+    """what is kept goes through the hooks for saved tensors, and a call may be made again in the backward pass"""
+    import rwkv_infctx_trainer_b200 as W
+    from torch.utils.checkpoint import checkpoint
+    c, g = L.linear_case(5, 70, 72, 48, BF, bias=True, mul=True, residual=True), L.gated_case(5, 70, 72, 48, BF)
+    want, pair = L.train_linear(c, "gelu"), L.train_gated(g, "silu")
+    n = lambda *s: torch.randn(s, device="cuda", dtype=BF)
+    rec = [n(2, 70, 48), n(2, 70, 48), n(2, 70, 48), torch.randn(48, device="cuda"), n(2, 70, 48), torch.randn(2, 48, device="cuda")]
+    seeds = (n(2, 70, 48), torch.randn(2, 48, device="cuda"))
+
+    def recurrence(call):
+        leaves = [t.detach().requires_grad_(True) for t in rec]
+        return torch.autograd.grad(call(*leaves), leaves, seeds)
+    plain = recurrence(W.gated_recurrence)
+    again = lambda f: lambda *a: checkpoint(f, *a, use_reentrant=False)
+    with torch.autograd.graph.save_on_cpu():
+        got, got_pair, got_rec = L.train_linear(c, "gelu"), L.train_gated(g, "silu"), recurrence(W.gated_recurrence)
+    for a, b in ((got, want), (got_pair, pair), (dict(enumerate(got_rec)), dict(enumerate(plain))), (dict(enumerate(recurrence(again(W.gated_recurrence)))), dict(enumerate(plain)))):
+        for k in b:
+            assert torch.equal(a[k], b[k]), k
+    leaves = {k: c[k].detach().requires_grad_(True) for k in L.LINEAR}
+    y = checkpoint(lambda *a: call(c, dict(zip(L.LINEAR, a)), "gelu"), *leaves.values(), use_reentrant=False)
+    for k, t in zip(L.LINEAR, torch.autograd.grad(y, list(leaves.values()), c["gy"])):
+        assert torch.equal(t, want["g" + k]), k
